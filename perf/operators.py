@@ -252,15 +252,15 @@ def _k8_unpack(kf):
 
 
 # ----------------------------------------------------------------------------- quantisation
-# One scale 2^e per token and head: the smallest power of two with amax <= 448 * 2^e (448: e4m3's largest value).
-# Held as the biased exponent e + 127 in 8 bits.  Codes are x / 2^e rounded to e4m3, nearest even.
+# One scale 2^e per token and head: the smallest power of two with amax <= 448 * 2^e (448: e4m3's largest value), and
+# e >= -117, so that every value is a normal bf16 number.  Held as the biased exponent e + 127 in 8 bits.  Codes are x / 2^e rounded to e4m3, nearest even.
 
 def _quantise(x):
     """x [.., d] -> (codes as bytes [.., d], biased exponents [..])."""
     x = x.float()
     m, e = torch.frexp(x.abs().amax(-1))                       # amax = m * 2^e, 0.5 <= m < 1; 448 = 0.875 * 2^9
     e = torch.where(m > 0.875, e - 8, e - 9)
-    e = torch.where(m > 0, e, torch.zeros_like(e)).clamp(-126, 127)
+    e = torch.where(m > 0, e, torch.zeros_like(e)).clamp(-117, 127)
     codes = torch.ldexp(x, -e[..., None]).to(torch.float8_e4m3fn)
     return codes.view(torch.uint8), (e + 127).to(torch.uint8)
 
@@ -506,7 +506,7 @@ def _held(x):
     """What the 8-bit cache holds for vectors x [.., d]."""
     x = x.double()
     amax = x.abs().amax(-1, keepdim=True)
-    e = torch.ceil(torch.log2(torch.where(amax > 0, amax, 448.0) / 448.0)).clamp(min=-126.0)
+    e = torch.ceil(torch.log2(torch.where(amax > 0, amax, 448.0) / 448.0)).clamp(min=-117.0)
     return _e4m3(x / torch.exp2(e)) * torch.exp2(e)
 
 
