@@ -12,6 +12,7 @@
 
 #define LSK_DTYPE_F32 0
 #define LSK_DTYPE_BF16 1
+#define LSK_DTYPE_KV8 2  // an 8-bit KV cache (lsk_kv8_append); not a tensor dtype
 
 typedef __bf16 lsk_bf16x8 __attribute__((ext_vector_type(8)));
 typedef short lsk_s16x4 __attribute__((ext_vector_type(4)));

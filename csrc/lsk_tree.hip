@@ -1,0 +1,260 @@
+// Trees of drafted tokens: ancestor masks, greedy acceptance, and the move of the accepted path's K / V.
+//
+// A block's T nodes are its tokens 0 .. T - 1; node 0 is the root (the last committed token) and parents[i] < i is the
+// index of node i's parent within the block.  Node i's K / V sit in slot pos0 + i of its cache row, whatever its depth.
+#include "lsk_common.h"
+#include "../include/lsk.h"
+
+// Node i's ancestors and i itself as bits, and i's depth.  One thread walks from a node to the root; parents decrease
+// along the walk, so the words are finished from the last to the first.  A parent outside [0, i) ends the walk.
+__global__ __launch_bounds__(64) void tree_masks_kernel(const int32_t* __restrict__ parents,
+                                                        const int32_t* __restrict__ starts,
+                                                        const int32_t* __restrict__ lens, int N,
+                                                        uint32_t* __restrict__ mask, int W,
+                                                        int32_t* __restrict__ depth) {
+  const int start = starts[blockIdx.x], T = lens[blockIdx.x];
+  if (start < 0 || T < 0 || T > N - start) return;
+  for (int i = blockIdx.y * 64 + threadIdx.x; i < T; i += 64 * gridDim.y) {
+    uint32_t* out = mask + (long)(start + i) * W;
+    int n = i, d = 0, w = W - 1;
+    uint32_t bits = 0;
+    while (true) {
+      for (; w > (n >> 5); --w) {                    // (a node past the words: none of its bits fit)
+        out[w] = bits;
+        bits = 0;
+      }
+      if (w == (n >> 5)) bits |= 1u << (n & 31);
+      const int up = parents[start + n];
+      if (up < 0 || up >= n) break;
+      n = up;
+      ++d;
+    }
+    for (; w >= 0; --w) {
+      out[w] = bits;
+      bits = 0;
+    }
+    if (depth != nullptr) depth[start + i] = d;
+  }
+}
+
+extern "C" int lsk_tree_masks(const int32_t* parents, const int32_t* starts, const int32_t* lens, int nb, int n_tokens,
+                              int max_nodes, uint32_t* mask, int mask_words, int32_t* depth, void* stream) {
+  const char* what = "lsk_tree_masks";
+  LSK_REQUIRE(parents && starts && lens && mask, LSK_EARG, "%s: null pointer", what);
+  LSK_REQUIRE(nb >= 0 && n_tokens >= 0 && max_nodes >= 0 && mask_words > 0 && (long)mask_words * 32 >= max_nodes,
+              LSK_ESHAPE, "%s: %d mask words for trees of up to %d nodes", what, mask_words, max_nodes);
+  if (nb == 0 || n_tokens == 0 || max_nodes == 0) return 0;
+  const int gy = (max_nodes + 63) / 64;
+  tree_masks_kernel<<<dim3(nb, gy < 65535 ? gy : 65535), 64, 0, (hipStream_t)stream>>>(parents, starts, lens, n_tokens,
+                                                                                      mask, mask_words, depth);
+  return lsk_check_launch(what);
+}
+
+// Greedy acceptance of one verified tree per wave: from the root, the next node is the lowest child that carries the
+// verifier's greedy token of the current one.  path[b] = the accepted nodes (the root first), out[b] = the verifier's
+// tokens of those nodes (the tokens to commit), both -1 past the end; acc[b] = the number of accepted drafts.
+// A block outside the tokens or without nodes: acc = -1.  At most max_nodes nodes of a block take part.
+// Children come after their parent, so the walk only goes up and ends.  Up to 64 nodes a lane holds one node and a step
+// is a ballot and two lane reads; the loads of larger trees come from the caches.
+__global__ __launch_bounds__(64) void tree_accept_kernel(const int64_t* __restrict__ Yv,
+                                                         const int64_t* __restrict__ tokens,
+                                                         const int32_t* __restrict__ parents,
+                                                         const int32_t* __restrict__ starts,
+                                                         const int32_t* __restrict__ lens, int N, int max_nodes,
+                                                         int64_t* __restrict__ acc, int32_t* __restrict__ path,
+                                                         int64_t* __restrict__ out) {
+  const int b = blockIdx.x, lane = threadIdx.x;
+  const int start = starts[b];
+  int T = lens[b];
+  if (start < 0 || T <= 0 || T > N - start) T = 0;
+  T = min(T, max_nodes);
+  int32_t* prow = path + (long)b * max_nodes;
+  int64_t* orow = out + (long)b * max_nodes;
+  int n = 0;                                         // nodes on the path
+  if (T > 0 && T <= 64) {
+    const bool in = lane < T;
+    const int par = in ? parents[start + lane] : -1;
+    const int64_t tok = in ? tokens[start + lane] : 0, y = in ? Yv[start + lane] : 0;
+    int cur = 0, my_node = -1;
+    int64_t my_out = -1;
+    while (true) {
+      const int64_t yc = __shfl(y, cur, 64);
+      if (lane == n) {
+        my_node = cur;
+        my_out = yc;
+      }
+      ++n;
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(in && lane > cur && par == cur && tok == yc);
+      if (hit == 0ull) break;
+      cur = __builtin_ctzll(hit);
+    }
+    if (lane < T) {                                  // (T <= max_nodes)
+      prow[lane] = my_node;
+      orow[lane] = my_out;
+    }
+    for (int i = T + lane; i < max_nodes; i += 64) {
+      prow[i] = -1;
+      orow[i] = -1;
+    }
+  } else {
+    int cur = 0;
+    while (T > 0) {
+      const int64_t yc = Yv[start + cur];
+      if (lane == 0) {
+        prow[n] = cur;
+        orow[n] = yc;
+      }
+      ++n;
+      int next = -1;
+      for (int base = cur + 1; base < T && next < 0; base += 64) {
+        const int i = base + lane;
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(i < T && parents[start + i] == cur && tokens[start + i] == yc);
+        if (hit != 0ull) next = base + __builtin_ctzll(hit);
+      }
+      if (next < 0) break;
+      cur = next;
+    }
+    for (int i = n + lane; i < max_nodes; i += 64) {
+      prow[i] = -1;
+      orow[i] = -1;
+    }
+  }
+  if (lane == 0) acc[b] = n - 1;
+}
+
+extern "C" int lsk_tree_accept(const int64_t* Yv, const int64_t* tokens, const int32_t* parents, const int32_t* starts,
+                               const int32_t* lens, int nb, int n_tokens, int max_nodes, int64_t* acc_out,
+                               int32_t* path_out, int64_t* tokens_out, void* stream) {
+  const char* what = "lsk_tree_accept";
+  LSK_REQUIRE(Yv && tokens && parents && starts && lens && acc_out && path_out && tokens_out, LSK_EARG,
+              "%s: null pointer", what);
+  LSK_REQUIRE(nb >= 0 && n_tokens >= 0 && max_nodes > 0, LSK_ESHAPE, "%s: bad shape", what);
+  if (nb == 0) return 0;
+  tree_accept_kernel<<<nb, 64, 0, (hipStream_t)stream>>>(Yv, tokens, parents, starts, lens, n_tokens, max_nodes, acc_out,
+                                                         path_out, tokens_out);
+  return lsk_check_launch(what);
+}
+
+// Slot pos0 + j takes what slot pos0 + path[j] holds, for the accepted j = 1 .. acc, in every layer: the accepted path's
+// K / V become consecutive and the committed length is pos0 + acc + 1.  Sources lie at or after their destinations
+// (path is increasing, path[j] >= j) and later destinations never reach an earlier chunk's sources, so a workgroup reads
+// 16 slots of one (layer, block, KV head), waits, and writes them, chunk after chunk.  Slots that stay are skipped.
+// FMT: 0 fp32 (K [S, D], V in 32-position blocks), 1 bf16 (fragment-major K, V in 32-position blocks), 2 8-bit.
+#define COMPACT_CHUNK 16
+#define COMPACT_THREADS 256
+
+template <int FMT>
+__device__ __forceinline__ long compact_k(int p, int d, int D) {  // element offsets in a stripe
+  if constexpr (FMT == 0) return (long)p * D + d;
+  if constexpr (FMT == 1) return k_cache_offset<uint16_t>(p, d, D);
+  const int pp = p & 63, a = (pp >> 2) & 3, l16 = ((pp >> 4) << 2) | (pp & 3);
+  return (long)(p >> 6) * 64 * D + (long)((a * (D >> 6) + (d >> 6)) * 64 + ((d >> 4) & 3) * 16 + l16) * 16 + (d & 15);
+}
+template <int FMT>
+__device__ __forceinline__ long compact_v(int p, int d, int D) {
+  constexpr int B = FMT == 2 ? 64 : 32;
+  return (long)(p / B) * B * D + (long)d * B + p % B;
+}
+
+template <int FMT> struct CompactElem;
+template <> struct CompactElem<0> { using T = uint32_t; };
+template <> struct CompactElem<1> { using T = uint16_t; };
+template <> struct CompactElem<2> { using T = uint8_t; };
+
+template <int FMT, int D>
+__global__ __launch_bounds__(COMPACT_THREADS) void kv_compact_kernel(
+    void* kc_, void* vc_, uint8_t* ks, uint8_t* vs, const int32_t* __restrict__ rows, const int32_t* __restrict__ pos0,
+    const int64_t* __restrict__ acc, const int32_t* __restrict__ path, int max_nodes, int max_batch, int Hkv, int S) {
+  using T = typename CompactElem<FMT>::T;
+  constexpr int PER = COMPACT_CHUNK * D / COMPACT_THREADS;
+  const int b = blockIdx.x, h = blockIdx.y, layer = blockIdx.z;
+  const int row = rows[b], p0 = pos0[b];
+  if (row < 0 || row >= max_batch || p0 < 0 || p0 >= S) return;
+  const int n = (int)min(acc[b], (int64_t)(max_nodes - 1));
+  const long stripe = (((long)layer * max_batch + row) * Hkv + h) * (long)S;
+  T* kc = (T*)kc_ + stripe * D;
+  T* vc = (T*)vc_ + stripe * D;
+  const int tid = threadIdx.x;
+  for (int j0 = 1; j0 <= n; j0 += COMPACT_CHUNK) {
+    T kx[PER], vx[PER];
+    uint8_t ek = 0, ev = 0;
+    auto moves = [&](int j, int& src) {              // whether slot p0 + j takes another's contents
+      if (j > n) return false;
+      const int node = path[(long)b * max_nodes + j];
+      src = p0 + node;
+      return node > j && node < S - p0;
+    };
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = tid + i * COMPACT_THREADS, j = j0 + e / D, d = e % D;
+      int src;
+      if (moves(j, src)) {
+        kx[i] = kc[compact_k<FMT>(src, d, D)];
+        vx[i] = vc[compact_v<FMT>(src, d, D)];
+      }
+    }
+    if constexpr (FMT == 2) {
+      int src;
+      if (tid < COMPACT_CHUNK && moves(j0 + tid, src)) {
+        ek = ks[stripe + src];
+        ev = vs[stripe + src];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = tid + i * COMPACT_THREADS, j = j0 + e / D, d = e % D;
+      int src;
+      if (moves(j, src)) {
+        kc[compact_k<FMT>(p0 + j, d, D)] = kx[i];
+        vc[compact_v<FMT>(p0 + j, d, D)] = vx[i];
+      }
+    }
+    if constexpr (FMT == 2) {
+      int src;
+      if (tid < COMPACT_CHUNK && moves(j0 + tid, src)) {
+        ks[stripe + p0 + j0 + tid] = ek;
+        vs[stripe + p0 + j0 + tid] = ev;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+extern "C" int lsk_kv_compact(int dtype, void* kcache, void* vcache, void* k_exp, void* v_exp, int n_layers,
+                              const int32_t* rows, const int32_t* pos0, const int64_t* accepted, const int32_t* path,
+                              int nb, int max_nodes, int n_kv_heads, int head_dim, int max_batch, int max_seq,
+                              void* stream) {
+  const char* what = "lsk_kv_compact";
+  LSK_REQUIRE(kcache && vcache && rows && pos0 && accepted && path, LSK_EARG, "%s: null pointer", what);
+  LSK_REQUIRE(dtype == LSK_DTYPE_F32 || dtype == LSK_DTYPE_BF16 || dtype == LSK_DTYPE_KV8, LSK_EUNSUPPORTED,
+              "%s: dtype %d", what, dtype);
+  LSK_REQUIRE(dtype != LSK_DTYPE_KV8 || (k_exp && v_exp), LSK_EARG, "%s: null exponents", what);
+  LSK_REQUIRE(n_layers >= 0 && n_layers <= 65535 && nb >= 0 && max_nodes > 0 && n_kv_heads > 0 && n_kv_heads <= 65535 &&
+                  max_batch > 0 && max_seq > 0 && max_seq % (dtype == LSK_DTYPE_KV8 ? 64 : 32) == 0,
+              LSK_ESHAPE, "%s: bad shape", what);
+  if (nb == 0 || n_layers == 0) return 0;
+  const dim3 grid(nb, n_kv_heads, n_layers);
+  hipStream_t s = (hipStream_t)stream;
+#define LSK_COMPACT(FMT, DD)                                                                                       \
+  kv_compact_kernel<FMT, DD><<<grid, COMPACT_THREADS, 0, s>>>(kcache, vcache, (uint8_t*)k_exp, (uint8_t*)v_exp, rows, \
+                                                              pos0, accepted, path, max_nodes, max_batch, n_kv_heads, \
+                                                              max_seq)
+#define LSK_COMPACT_D(FMT)                              \
+  do {                                                  \
+    if (head_dim == 128) LSK_COMPACT(FMT, 128);         \
+    else LSK_COMPACT(FMT, 64);                          \
+  } while (0)
+  if (dtype == LSK_DTYPE_F32 && (head_dim == 16 || head_dim == 32)) {
+    if (head_dim == 16) LSK_COMPACT(0, 16);
+    else LSK_COMPACT(0, 32);
+  } else {
+    LSK_REQUIRE(head_dim == 64 || head_dim == 128, LSK_EUNSUPPORTED, "%s: head_dim %d", what, head_dim);
+    if (dtype == LSK_DTYPE_F32) LSK_COMPACT_D(0);
+    else if (dtype == LSK_DTYPE_BF16) LSK_COMPACT_D(1);
+    else LSK_COMPACT_D(2);
+  }
+#undef LSK_COMPACT_D
+#undef LSK_COMPACT
+  return lsk_check_launch(what);
+}

@@ -4,7 +4,8 @@
  * replaces the eager torch ops of one step of its hot path, cited as file:line of the reference.
  *
  * Conventions
- *   - dtype codes: LSK_DTYPE_F32 (0) and LSK_DTYPE_BF16 (1); bf16 is torch.bfloat16 storage.
+ *   - dtype codes: LSK_DTYPE_F32 (0) and LSK_DTYPE_BF16 (1); bf16 is torch.bfloat16 storage.  lsk_kv_compact also
+ *     takes LSK_DTYPE_KV8 (2), the 8-bit KV cache.
  *   - All pointers are device pointers unless stated; the library never allocates or frees
  *     device memory: tensors and workspaces belong to the caller (the PyTorch caching allocator).
  *   - `stream` is a hipStream_t; every call is asynchronous on it, nothing synchronises inside.
@@ -23,7 +24,7 @@
 extern "C" {
 #endif
 
-#define LSK_ABI_VERSION 13
+#define LSK_ABI_VERSION 14
 
 #define LSK_EPI_NONE 0     /* C = rnd(A W^T)                                   */
 #define LSK_EPI_RESIDUAL 1 /* C = rnd(R + rnd(A W^T))                          */
@@ -273,6 +274,78 @@ int lsk_kv_rollback(int64_t* kv_len, const int32_t* slots, const int64_t* accept
 int lsk_shift_segment_positions(int32_t* meta, int n_tokens, int nb, int n_works, int n_groups, int n_recs, int group,
                                 const int64_t* accepted, const int32_t* vslots, const int32_t* vdrafts, int nv,
                                 void* stream);
+
+/* ---- 8-bit KV cache (no counterpart in the reference, whose cache is the model's dtype) ----
+ * One token's K (V) of one KV head: head_dim e4m3 codes and a power-of-two scale 2^e held as the byte e + 127:
+ *   amax = largest finite |x|, e = smallest integer >= -117 with amax <= 448 * 2^e (0 for amax = 0),
+ *   code = x * 2^-e rounded to e4m3, nearest even (NaN and infinities: NaN), value = code * 2^e.
+ * Storage of a layer (head_dim 64 or 128, S = max_seq a multiple of 64, tensors at multiples of 16 bytes):
+ *   k8 [B, Hkv, S/64, 4, D/64, 64, 16] bytes: lane 16 lg + l16 of fragment (a, j) of a 64-position block holds position
+ *      16 (l16 / 4) + 4 a + l16 % 4 and d = 64 j + 16 lg .. + 15;
+ *   v8 [B, Hkv, S/64, D, 64] bytes: blocks transposed;   k_exp, v_exp [B, Hkv, S] bytes.
+ *
+ * lsk_kv8_append: k, v [n_tokens, n_kv_heads, head_dim] (bf16 or fp32; strides in elements, dims contiguous) go to
+ * (rows[t], pos[t]).  A token outside [0, max_batch) x [0, max_seq) is skipped.  The (row, position) pairs of a call
+ * have to differ: of equal ones, one token's codes may meet the other's scale.
+ * lsk_kv8_read: the values at (rows[t], pos[t]) as contiguous k, v [n_tokens, n_kv_heads, head_dim] (bf16 exactly, or
+ * fp32); zeros for a token outside the cache.
+ * Beside lsk_kv_append (solutions/packed.py:180-181). */
+int lsk_kv8_append(int dtype, const void* k, const void* v, long stride_t, long stride_h, void* k8, void* v8,
+                   void* k_exp, void* v_exp, const int32_t* rows, const int32_t* pos, int n_tokens, int n_kv_heads,
+                   int head_dim, int max_batch, int max_seq, void* stream);
+int lsk_kv8_read(int dtype, const void* k8, const void* v8, const void* k_exp, const void* v_exp, const int32_t* rows,
+                 const int32_t* pos, void* k, void* v, int n_tokens, int n_kv_heads, int head_dim, int max_batch,
+                 int max_seq, void* stream);
+
+/* Attention over a layer's 8-bit cache (lsk_kv8_attn) and over trees of drafted tokens (lsk_tree_attn: bf16 or fp32
+ * caches in lsk_ragged_attn's layouts; lsk_kv8_attn with a mask).  q [n_tokens, n_heads, head_dim] (bf16; fp32 for fp32
+ * trees), any strides in elements, dims contiguous; out [n_tokens, n_heads * head_dim] contiguous, q's dtype.
+ * Token t of block {q_start, pos0, T, row} sits in slot pos0 + t of its cache row and reads slots 0 .. pos0 + t; with a
+ * mask (uint32 [n_tokens][mask_words]), of the block's own slots only those whose bit is set: bit j % 32 of word j / 32
+ * for node j; bits of later nodes and bits past the words count as 0.  A row that reads nothing gives zeros.  Values in
+ * slots that a row does not read never reach it, whatever they are.
+ * The plan (blocks .. rows_cap) is lsk_attn_plan's and lsk_attn_schedule's, as for lsk_ragged_attn; fp32 plans are
+ * unsplit.  workspace >= lsk_attn_workspace_bytes(n_parts, n_kv_heads, head_dim), 16-byte aligned, and a call's own.
+ * head_dim 64 or 128 (fp32 also 16 and 32).  A row's result depends on its own block only; over a bf16 or fp32 cache a
+ * chain (every ancestor's bit set) gives lsk_ragged_attn's bits.
+ * Beside lsk_ragged_attn (solutions/packed.py:142-166). */
+int lsk_kv8_attn(const void* q, long q_stride_t, long q_stride_h, const void* k8, const void* v8, const void* k_exp,
+                 const void* v_exp, const uint32_t* mask, int mask_words, const int32_t* blocks, int n_works,
+                 const int32_t* groups, int n_groups, int n_parts, const int32_t* recs, int n_rounds, int n_slots,
+                 int rows_cap, void* out, int n_heads, int n_kv_heads, int head_dim, int max_seq, float scale,
+                 void* workspace, size_t ws_bytes, void* stream);
+int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_stride_h, const void* kcache, const void* vcache,
+                  const uint32_t* mask, int mask_words, const int32_t* blocks, const int32_t* works, int n_works,
+                  const int32_t* groups, int n_groups, int n_parts, const int32_t* recs, int n_rounds, int n_slots,
+                  int rows_cap, void* out, int n_heads, int n_kv_heads, int head_dim, int max_seq, float scale,
+                  void* workspace, size_t ws_bytes, void* stream);
+
+/* ---- trees of drafted tokens (the reference drafts chains) ----
+ * A block's nodes are its tokens 0 .. lens[b] - 1 from starts[b]; node 0 is the root (the last committed token),
+ * parents[starts[b] + i] < i the parent of node i (anything outside [0, i): none).  Node i's K / V sit in slot pos0 + i.
+ *
+ * lsk_tree_masks: mask [n_tokens][mask_words] (32 * mask_words >= max_nodes >= every len) = the bits of each node's
+ * ancestors and its own; depth [n_tokens] (optional) = its number of ancestors (its RoPE position is pos0 + depth).
+ * Blocks outside [0, n_tokens) are skipped.
+ *
+ * lsk_tree_accept: from the root, the next node is the lowest child whose token equals the verifier's greedy token
+ * Yv of the current one.  acc_out[b] = accepted drafts (-1: no nodes, or a block outside the tokens), path_out
+ * [nb][max_nodes] = the accepted nodes from the root on, tokens_out [nb][max_nodes] = Yv of those nodes (the tokens to
+ * commit), both -1 past the end.  Nodes from max_nodes on take no part.  A chain gives lsk_greedy_accept's counts
+ * (solutions/engine.py:461-476).
+ *
+ * lsk_kv_compact: slot pos0[b] + j of cache row rows[b] takes what slot pos0[b] + path[b][j] holds, j = 1 ..
+ * accepted[b], in every layer and KV head (caches [n_layers, max_batch, ...], contiguous; k_exp, v_exp for
+ * LSK_DTYPE_KV8, else NULL); then lsk_kv_rollback's pointer update holds as for a chain.  path as lsk_tree_accept
+ * writes it (increasing); the rows of a call have to differ.  Blocks outside the cache are skipped. */
+int lsk_tree_masks(const int32_t* parents, const int32_t* starts, const int32_t* lens, int nb, int n_tokens,
+                   int max_nodes, uint32_t* mask, int mask_words, int32_t* depth, void* stream);
+int lsk_tree_accept(const int64_t* Yv, const int64_t* tokens, const int32_t* parents, const int32_t* starts,
+                    const int32_t* lens, int nb, int n_tokens, int max_nodes, int64_t* acc_out, int32_t* path_out,
+                    int64_t* tokens_out, void* stream);
+int lsk_kv_compact(int dtype, void* kcache, void* vcache, void* k_exp, void* v_exp, int n_layers, const int32_t* rows,
+                   const int32_t* pos0, const int64_t* accepted, const int32_t* path, int nb, int max_nodes,
+                   int n_kv_heads, int head_dim, int max_batch, int max_seq, void* stream);
 
 /* ---- native layer-range runner (solutions/packed.py:169-196, packed_layer / packed_layers) ----
  * A model handle holds host copies of per-layer device pointers (weights [out, in]: packed for bf16 --

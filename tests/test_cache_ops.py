@@ -1,0 +1,869 @@
+"""The 8-bit KV cache (write, read, attention) and trees of drafted tokens (masks, attention, acceptance, compaction)
+against plain 64-bit implementations; refusals on the CPU.
+
+Tolerances.  The cache: exact.  Attention: with w the exact normalised weights and A = sum w |v| (per output element),
+the kernel rounds each weight to bf16 (relative 2^-8 at most, eps / 2) and the output to bf16 (2^-8 |out|); the fp32
+score of a position is off by at most (D + 4) 2^-24 sum |q k| scale, which moves its weight by that much relatively (and
+the sum of the weights likewise): below 2^-12 for every case here.  So |got - ref| <= 1.01 * 2^-8 (|ref| + A) + 2^-12 A.
+fp32: the sums of n positions and D products, one after the other: (n + D + 64) 2^-24 (1 + max sum |q k| scale) 2 A.
+"""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+BF16, F32 = torch.bfloat16, torch.float32
+E4M3 = torch.float8_e4m3fn
+
+
+def _lsk():
+    from thesis_amd import _lsk
+
+    _lsk.load()
+    return _lsk
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _i32(x, dev):
+    return torch.as_tensor(np.asarray(x), dtype=torch.int32).to(dev)
+
+
+def _cat(xs, dtype, dev):
+    return torch.as_tensor(np.concatenate([np.asarray(x, dtype=np.int64) for x in xs]), dtype=dtype).to(dev)
+
+
+# ----------------------------------------------------------------------------- plain forms
+
+def exponents(x):
+    """e of the cache's rule for vectors x [.., d] (64 bits): the smallest integer >= -117 with amax <= 448 * 2^e."""
+    a = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x)).amax(-1).double()
+    e = torch.ceil(torch.log2(torch.where(a > 0, a, 448.0) / 448.0)).clamp(min=-117)
+    assert (a <= 448.0 * torch.exp2(e)).all()
+    return e.to(torch.int64)
+
+
+def held(x):
+    """What the 8-bit cache stands for (64 bits), from e4m3's definition: units of 2^(max(floor log2, -6) - 3)."""
+    s = torch.exp2(exponents(x).double())[..., None]
+    y = x.double() / s
+    unit = torch.exp2(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -40))).clamp(min=-6.0) - 3.0)
+    r = torch.round(y / unit) * unit * s
+    return torch.where(torch.isfinite(x), r, torch.full_like(r, math.nan))
+
+
+def ancestors(parents):
+    """Index sets a node reads: its ancestors and itself (a parent outside [0, i) is none)."""
+    out = []
+    for i, p in enumerate(parents):
+        out.append((out[p] if 0 <= p < i else frozenset()) | {i})
+    return out
+
+
+def random_tree(rng, t):
+    return [-1] + [int(i - 1 if rng.random() < 0.5 else rng.integers(i)) for i in range(1, t)]
+
+
+def words_of(sets, w):
+    m = np.zeros((len(sets), w), dtype=np.uint32)
+    for i, s in enumerate(sets):
+        for j in s:
+            if j < 32 * w:
+                m[i, j // 32] |= np.uint32(1 << (j % 32))
+    return m.view(np.int32)
+
+
+def attention(q, k, v, blocks, scale, sets=None):
+    """q [N, Hq, D], k / v [B, Hkv, S, D] (64 bits) -> (out [N, Hq D], A [N, Hq D], largest sum |q k| scale)."""
+    N, Hq, D = q.shape
+    g = Hq // k.shape[1]
+    out = torch.zeros(N, Hq, D, dtype=torch.float64)
+    mag = torch.zeros_like(out)
+    big = 0.0
+    for (qs, p0, T, row) in blocks:
+        for t in range(T):
+            reads = list(range(p0 + t + 1)) if sets is None else \
+                list(range(p0)) + [p0 + j for j in sorted(sets[qs + t]) if j <= t]
+            if not reads:
+                continue
+            kr, vr = k[row][:, reads], v[row][:, reads]
+            qt = q[qs + t].view(-1, g, D)
+            s = (qt[:, :, None] * kr[:, None]).sum(-1) * scale
+            qk = (qt.abs()[:, :, None] * kr.abs()[:, None]).sum(-1) * scale
+            big = max(big, float(qk.nan_to_num(0, 0, 0).max()))
+            w = torch.softmax(s, dim=-1)
+            out[qs + t] = (w[..., None] * vr[:, None]).sum(2).view(Hq, D)
+            mag[qs + t] = (w[..., None] * vr.abs()[:, None]).sum(2).view(Hq, D)
+    return out.view(N, -1), mag.view(N, -1), big
+
+
+def assert_close_bf16(got, ref, mag):
+    got, ref, mag = got.double().cpu(), ref.cpu(), mag.cpu()
+    fine = torch.isfinite(ref)
+    assert torch.equal(torch.isfinite(got), fine)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    tol = 1.01 * 2.0 ** -8 * (ref.abs() + mag) + 2.0 ** -12 * mag + 1e-30
+    err = (got - ref).abs()
+    assert (err[fine] <= tol[fine]).all(), (err[fine] / tol[fine]).max()
+    assert torch.equal(got[~fine & ~torch.isnan(ref)], ref[~fine & ~torch.isnan(ref)])
+
+
+def assert_close_f32(got, ref, mag, n, d, big):
+    tol = (n + d + 64) * 2.0 ** -24 * (1 + big) * 2 * mag + 1e-30
+    assert ((got.double().cpu() - ref).abs() <= tol).all()
+
+
+def pack_blocks(blocks):
+    """[(row, pos0, T)] -> [(q_start, pos0, T, row)]"""
+    out, off = [], 0
+    for (row, p0, t) in blocks:
+        out.append((off, p0, t, row))
+        off += t
+    return out, off
+
+
+def kv8_from(lsk, cuda, k, v):
+    """An 8-bit cache written by kv8_append with dense k, v [B, Hkv, S, D] (bf16)."""
+    B, H, S, D = k.shape
+    cache = lsk.KV8.zeros(B, H, S, D, cuda)
+    rows = torch.arange(B).repeat_interleave(S)
+    pos = torch.arange(S).repeat(B)
+    flat = lambda x: x.permute(0, 2, 1, 3).reshape(B * S, H, D).contiguous().to(cuda)  # noqa: E731
+    lsk.kv8_append(flat(k), flat(v), cache, _i32(rows, cuda), _i32(pos, cuda))
+    return cache
+
+
+def k8_dense(codes):
+    """K codes [.., S/64, 4, D/64, 64, 16] -> [.., S, D], index by index from the documented layout."""
+    *lead, nb, _, J, _, _ = codes.shape
+    S, D = nb * 64, J * 64
+    p, d = np.meshgrid(np.arange(S), np.arange(D), indexing="ij")
+    pp = p % 64
+    a, l16 = pp // 4 % 4, pp // 16 * 4 + pp % 4
+    j, lg = d // 64, d // 16 % 4
+    off = p // 64 * 64 * D + ((a * J + j) * 64 + lg * 16 + l16) * 16 + d % 16
+    flat = codes.view(torch.uint8).reshape(*lead, S * D)
+    return flat[..., torch.as_tensor(off.reshape(-1))].reshape(*lead, S, D)
+
+
+# ----------------------------------------------------------------------------- the 8-bit cache
+
+def _awkward(g, n, h, d, dtype):
+    """Vectors of every size: all-zero, tiny, subnormal, huge, with the largest value at and next to 448 * 2^e, ties."""
+    x = torch.randn(n, h, d, generator=g) * torch.exp2(torch.randint(-30, 30, (n, h, 1), generator=g).float())
+    flat = x.view(-1, d)
+    m = flat.shape[0]
+    flat[0 % m] = 0.0
+    flat[1 % m] = torch.randn(d, generator=g) * 1e-39
+    flat[2 % m] = torch.randn(d, generator=g).clamp(-1, 1) * 3e38
+    flat[3 % m, 0], flat[3 % m, 1:] = 448.0, torch.arange(1, d).float() / 8          # ties between e4m3 values
+    flat[4 % m, 0], flat[4 % m, 1:] = 450.0, torch.arange(1, d).float()              # just past 448: the next scale
+    flat[5 % m] = 0.0
+    flat[5 % m, d - 1] = -2.0 ** -133
+    return x.to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,h", [(1, 1), (7, 3), (16, 8), (33, 2), (200, 8)])
+def test_kv8_append_and_read_are_exact(cuda, dtype, D, n, h):
+    """Codes, exponents and storage layout are the definition's; what is read back is code * 2^e; everything else of
+    the cache stays as it was, and tokens outside the cache leave it alone."""
+    lsk = _lsk()
+    g = _gen(n * 7 + D)
+    B, S = 3, 192
+    k, v = _awkward(g, n, h, D, dtype), _awkward(g, n, h, D, dtype).flip(0)
+    slot = torch.randperm(B * S, generator=g)[:n]
+    rows, pos = slot // S, slot % S
+    if n > 8:                                                         # padding and stray tokens
+        rows[3], pos[5], rows[6], pos[7] = -1, S, B, -2
+    ok = (rows >= 0) & (rows < B) & (pos >= 0) & (pos < S)
+    cache = lsk.KV8.zeros(B, h, S, D, cuda)
+    before = torch.randint(0, 120, cache.k.view(torch.uint8).shape, generator=g, dtype=torch.uint8)
+    cache.k.view(torch.uint8).copy_(before)
+    lsk.kv8_append(k.to(cuda), v.to(cuda), cache, _i32(rows, cuda), _i32(pos, cuda))
+    kd = k8_dense(cache.k.cpu())
+    vd = cache.v.cpu().view(torch.uint8).transpose(-1, -2).reshape(B, h, S, D)
+    want_k, want_v = k8_dense(before.view(E4M3)), torch.zeros(B, h, S, D, dtype=torch.uint8)
+    want_ks = torch.full((B, h, S), 127, dtype=torch.uint8)
+    want_vs = want_ks.clone()
+    for x, codes, exps in ((k, want_k, want_ks), (v, want_v, want_vs)):
+        e = exponents(x.double())
+        c = (held(x) / torch.exp2(e.double())[..., None]).to(torch.float32).to(E4M3).view(torch.uint8)  # exact values
+        codes[rows[ok], :, pos[ok]] = c[ok]
+        exps[rows[ok], :, pos[ok]] = (e + 127).to(torch.uint8)[ok]
+    neg0 = lambda t: torch.where(t == 128, torch.zeros_like(t), t)    # noqa: E731  (the sign of a zero is free)
+    assert torch.equal(cache.ks.cpu(), want_ks) and torch.equal(cache.vs.cpu(), want_vs)
+    assert torch.equal(neg0(kd), neg0(want_k)) and torch.equal(neg0(vd), neg0(want_v))
+    for out in (BF16, F32):
+        kr, vr = lsk.kv8_read(cache, _i32(rows, cuda), _i32(pos, cuda), out)
+        for got, x in ((kr, k), (vr, v)):
+            want = torch.where(ok[:, None, None], held(x), torch.zeros(1, dtype=torch.float64))
+            assert torch.equal(got.cpu().double(), want)
+
+
+@pytest.mark.gpu
+def test_kv8_rounds_every_bf16_value_to_the_nearest_code(cuda):
+    """All finite bf16 values with a fixed largest value in the vector: the code is the nearest e4m3 value, ties to
+    even (torch's own conversion of the scaled value)."""
+    lsk = _lsk()
+    bits = torch.arange(0, 0x43E0, dtype=torch.int32)                 # 0 .. 448 in bf16
+    vals = bits.to(torch.int16).view(BF16)
+    n = (len(vals) + 62) // 63
+    x = torch.zeros(n, 1, 64, dtype=BF16)
+    x[:, 0, 0] = 448.0
+    body = torch.zeros(n * 63, dtype=BF16)
+    body[:len(vals)] = vals * torch.where(torch.arange(len(vals)) % 2 == 0, 1.0, -1.0).to(BF16)
+    x[:, 0, 1:] = body.view(n, 63)
+    S = (n + 63) // 64 * 64
+    cache = lsk.KV8.zeros(1, 1, S, 64, cuda)
+    rows, pos = _i32(np.zeros(n), cuda), _i32(np.arange(n), cuda)
+    lsk.kv8_append(x.to(cuda), x.to(cuda), cache, rows, pos)
+    assert (cache.ks.cpu()[0, 0, :n] == 127).all()
+    want = x.float().to(E4M3).float()
+    for got in lsk.kv8_read(cache, rows, pos, F32):
+        assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.gpu
+def test_kv8_append_takes_strides_and_non_finite_values(cuda):
+    """k and v as views of a fused qkv row (at any bf16 address); NaN and infinities become NaN and leave the scale to
+    the finite values."""
+    lsk = _lsk()
+    g = _gen(5)
+    n, h, D, S = 9, 2, 64, 64
+    buf = torch.randn(n * 2 * (h * D) + n + 1, generator=g).to(BF16)
+    buf[1 + 5], buf[1 + 70], buf[1 + 130 + h * D] = math.nan, math.inf, -math.inf
+    dev = buf.to(cuda)
+    view = lambda t, o: torch.as_strided(t, (n, h, D), (2 * h * D + 1, D, 1), o)  # noqa: E731
+    cache = lsk.KV8.zeros(1, h, S, D, cuda)
+    rows, pos = _i32(np.zeros(n), cuda), _i32(np.arange(n), cuda)
+    lsk.kv8_append(view(dev, 1), view(dev, 1 + h * D), cache, rows, pos)
+    for got, x in zip(lsk.kv8_read(cache, rows, pos, F32), (view(buf, 1), view(buf, 1 + h * D))):
+        want = held(x)
+        assert torch.equal(torch.isnan(got.cpu()), torch.isnan(want))
+        assert torch.equal(got.cpu().double().nan_to_num(0), want.nan_to_num(0))
+    assert torch.isnan(held(view(buf, 1))).sum() == 3
+
+
+# ----------------------------------------------------------------------------- attention
+
+def _heads(case):
+    return {"gqa128": (8, 2, 128), "gqa64": (8, 2, 64), "mha64": (3, 3, 64), "mqa128": (5, 1, 128)}[case]
+
+
+# (row, pos0, T) blocks: single tokens at the first position and far along, blocks that start or end inside a step or
+# at its edge, contexts over several splits, repeated cache rows, blocks without tokens
+BLOCKS = {
+    "first": [(0, 0, 1)],
+    "decode": [(2, 0, 1), (0, 63, 1), (1, 64, 1), (3, 300, 1)],
+    "verify": [(1, 0, 5), (0, 60, 9), (3, 127, 2), (2, 1000, 7)],
+    "wide": [(0, 10, 40), (2, 500, 23), (1, 0, 64)],
+    "empty": [(0, 5, 0), (1, 700, 3), (2, 0, 0)],
+    "shared": [(1, 90, 3), (1, 40, 2), (0, 1023, 1)],
+}
+
+
+def _attn_inputs(seed, heads, blocks, dtype=BF16, S=1088, B=4):
+    Hq, Hkv, D = heads
+    g = _gen(seed)
+    tab, n = pack_blocks(blocks)
+    q = torch.randn(n, Hq, D, generator=g).to(dtype)
+    k = (torch.randn(B, Hkv, S, D, generator=g) * torch.exp(0.4 * torch.randn(1, Hkv, 1, D, generator=g))).to(dtype)
+    v = torch.randn(B, Hkv, S, D, generator=g).to(dtype)
+    return tab, q, k, v
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [None, 64, 256])
+@pytest.mark.parametrize("blocks", BLOCKS)
+@pytest.mark.parametrize("heads", ["gqa128", "gqa64", "mha64", "mqa128"])
+def test_kv8_attention_matches_64_bits(cuda, heads, blocks, split):
+    lsk = _lsk()
+    Hq, Hkv, D = _heads(heads)
+    tab, q, k, v = _attn_inputs(11, (Hq, Hkv, D), BLOCKS[blocks])
+    cache = kv8_from(lsk, cuda, k, v)
+    plan = lsk.AttnPlan(tab, Hq, cache, split=split)
+    got = lsk.kv8_attn(q.to(cuda), cache, plan)
+    ref, mag, _ = attention(q.double(), held(k), held(v), tab, 1 / math.sqrt(D))
+    assert_close_bf16(got, ref, mag)
+
+
+def _tree_blocks(blocks, seed):
+    rng = np.random.default_rng(seed)
+    parents = [random_tree(rng, t) if t else [] for (_, _, t) in blocks]
+    return parents, [s for p in parents for s in ancestors(p)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [None, 64])
+@pytest.mark.parametrize("blocks", BLOCKS)
+@pytest.mark.parametrize("kind,heads", [("bf16", "gqa128"), ("bf16", "gqa64"), ("bf16", "mqa128"), ("kv8", "gqa128"),
+                                        ("kv8", "mha64"), ("fp32", "gqa64"), ("fp32", "mqa128")])
+def test_tree_attention_matches_64_bits(cuda, kind, heads, blocks, split):
+    lsk = _lsk()
+    Hq, Hkv, D = _heads(heads)
+    dtype = F32 if kind == "fp32" else BF16
+    tab, q, k, v = _attn_inputs(13, (Hq, Hkv, D), BLOCKS[blocks], dtype)
+    parents, sets = _tree_blocks(BLOCKS[blocks], 3)
+    mask = torch.from_numpy(words_of(sets, (max(t for _, _, t in BLOCKS[blocks]) + 31) // 32)).to(cuda)
+    if kind == "kv8":
+        cache = kv8_from(lsk, cuda, k, v)
+        got = lsk.kv8_attn(q.to(cuda), cache, lsk.AttnPlan(tab, Hq, cache, split=split), mask)
+        k, v = held(k), held(v)
+    else:
+        ks = (lsk.k_to_frag(k) if kind == "bf16" else k).to(cuda)
+        got = lsk.tree_attn(q.to(cuda), ks, lsk.v_to_blocked(v).to(cuda), lsk.AttnPlan(tab, Hq, ks, split=split), mask)
+    ref, mag, big = attention(q.double(), k.double(), v.double(), tab, 1 / math.sqrt(D), sets)
+    if kind == "fp32":
+        assert_close_f32(got, ref, mag, 1088, D, big)
+    else:
+        assert_close_bf16(got, ref, mag)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "kv8", "fp32"])
+def test_masks_of_any_kind_and_rows_that_read_nothing(cuda, kind):
+    """Masks that are no tree: rows without a set bit at position 0 give zeros, bits of later nodes and words that a
+    long block does not have count as 0, trees of more than 32 and 64 nodes."""
+    lsk = _lsk()
+    Hq, Hkv, D = 4, 2, 64
+    blocks = [(0, 0, 70), (1, 3, 130), (2, 0, 1)]
+    dtype = F32 if kind == "fp32" else BF16
+    tab, q, k, v = _attn_inputs(17, (Hq, Hkv, D), blocks, dtype, S=192, B=3)
+    n = len(q)
+    rng = np.random.default_rng(2)
+    bits = rng.random((n, 96)) < 0.2                                  # 3 words: nodes from 96 on are never read
+    bits[:5] = False                                                  # block 0's first rows read nothing
+    bits[n - 1] = False
+    sets = [set(np.flatnonzero(r).tolist()) for r in bits]
+    mask = torch.from_numpy(words_of(sets, 3)).to(cuda)
+    if kind == "kv8":
+        cache = kv8_from(lsk, cuda, k, v)
+
+        def run(split):
+            return lsk.kv8_attn(q.to(cuda), cache, lsk.AttnPlan(tab, Hq, cache, split=split), mask)
+
+        k, v = held(k), held(v)
+    else:
+        ks = (lsk.k_to_frag(k) if kind == "bf16" else k).to(cuda)
+        vs = lsk.v_to_blocked(v).to(cuda)
+
+        def run(split):
+            return lsk.tree_attn(q.to(cuda), ks, vs, lsk.AttnPlan(tab, Hq, ks, split=split), mask)
+
+    ref, mag, big = attention(q.double(), k.double(), v.double(), tab, 1 / math.sqrt(D), sets)
+    for split in (None, 64):
+        got = run(split)
+        assert (got[:5] == 0).all() and (got[n - 1] == 0).all()
+        if kind == "fp32":
+            assert_close_f32(got, ref, mag, 192, D, big)
+        else:
+            assert_close_bf16(got, ref, mag)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("kind", ["bf16", "kv8", "kv8 causal", "fp32"])
+def test_values_that_a_row_does_not_read_never_reach_it(cuda, kind, bad):
+    """NaN and infinities in nodes that a row does not read, in the slots behind the block and in those of other rows
+    leave its bits as they are; a row that reads such a V gets what the formula gives."""
+    lsk = _lsk()
+    Hq, Hkv, D = 4, 2, 128
+    blocks = [(0, 70, 12), (2, 0, 30), (1, 131, 1)]
+    dtype = F32 if kind == "fp32" else BF16
+    tab, q, k, v = _attn_inputs(19, (Hq, Hkv, D), blocks, dtype, S=192, B=3)
+    v[0, :, 77, 100] = 5.0                                            # (the largest also without the dims below)
+    parents, sets = _tree_blocks(blocks, 5)
+    if kind == "kv8 causal":
+        sets = [set(range(i + 1)) for (_, _, t) in blocks for i in range(t)]
+    mask = torch.from_numpy(words_of(sets, 1)).to(cuda)
+
+    def run(k, v):
+        if kind.startswith("kv8"):
+            cache = kv8_from(lsk, cuda, k, v)
+            if bad != bad:                                            # slots never written: any byte as a scale
+                for b, (_, p0, t, row) in enumerate(tab):
+                    cache.ks[row, :, p0 + t:], cache.vs[row, :, p0 + t:] = 255, 255
+            return lsk.kv8_attn(q.to(cuda), cache, lsk.AttnPlan(tab, Hq, cache), mask if kind == "kv8" else None).cpu()
+        ks = (lsk.k_to_frag(k) if kind == "bf16" else k).to(cuda)
+        return lsk.tree_attn(q.to(cuda), ks, lsk.v_to_blocked(v).to(cuda), lsk.AttnPlan(tab, Hq, ks), mask).cpu()
+
+    clean = run(k, v)
+    k2, v2 = k.clone(), v.clone()
+    for (_, p0, t, row) in tab:
+        k2[row, :, p0 + t:], v2[row, :, p0 + t:] = bad, bad
+    assert torch.equal(run(k2, v2), clean)
+    node = 7                                                          # of block 0, and its V's dims 0 .. 9 and 40
+    k2[0, :, 70 + node], v2[0, :, 70 + node, :10], v2[0, :, 70 + node, 40] = bad, bad, bad
+    got = run(k2, v2)
+    reads = torch.tensor([b == 0 and node in sets[q0 + i] for b, (q0, _, t, _) in enumerate(tab) for i in range(t)])
+    assert torch.equal(got[~reads], clean[~reads]) and reads.any() and not reads.all()
+    assert torch.isnan(got[reads]).all()                              # (a score that is not finite)
+    v3 = v2.clone()
+    got = run(torch.where(torch.isfinite(k2), k2, k), v3).view(len(q), Hq, D)
+    assert torch.equal(got[~reads], clean.view(len(q), Hq, D)[~reads])
+    hit = torch.zeros(D, dtype=torch.bool)
+    hit[:10], hit[40] = True, True
+    assert torch.equal(got[reads][..., ~hit], clean.view(len(q), Hq, D)[reads][..., ~hit])
+    want = torch.full_like(got[reads][..., hit], math.nan if kind.startswith("kv8") else bad)
+    assert torch.equal(got[reads][..., hit].nan_to_num(7.0), want.nan_to_num(7.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_chain_gives_the_ragged_attentions_bits(cuda, dtype, D):
+    lsk = _lsk()
+    Hq, Hkv = 8, 2
+    blocks = [(0, 0, 5), (2, 63, 9), (1, 700, 40), (3, 1000, 1)]
+    tab, q, k, v = _attn_inputs(23, (Hq, Hkv, D), blocks, dtype)
+    ks = (lsk.k_to_frag(k) if dtype == BF16 else k).to(cuda)
+    vs = lsk.v_to_blocked(v).to(cuda)
+    sets = [set(range(i + 1)) for (_, _, t) in blocks for i in range(t)]
+    mask = torch.from_numpy(words_of(sets, 2)).to(cuda)
+    for split in (256, 2048):
+        p = lsk.AttnPlan(tab, Hq, ks, split=split)
+        want = torch.empty(len(q), Hq * D, dtype=dtype, device=cuda)
+        ws = torch.empty(max(p.ws_bytes, 1), dtype=torch.uint8, device=cuda)
+        lsk.ragged_attn(q.to(cuda), ks, vs, p.blocks, p.works, p.n_works, p.groups, p.n_groups, p.n_parts, want, Hq,
+                        1 / math.sqrt(D), ws, p.recs, p.n_rounds, p.n_slots, p.rows_cap)
+        assert torch.equal(lsk.tree_attn(q.to(cuda), ks, vs, p, mask), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["kv8", "kv8 tree", "tree"])
+def test_a_rows_result_depends_on_its_block_only(cuda, kind):
+    """The same rows alone, in another order, next to others and as single tokens (causal) give the same bits; so do
+    other rows-per-item caps."""
+    lsk = _lsk()
+    Hq, Hkv, D = 8, 2, 128
+    blocks = [(0, 37, 9), (3, 500, 30), (1, 0, 3), (2, 900, 60)]
+    tab, q, k, v = _attn_inputs(29, (Hq, Hkv, D), blocks)
+    _, sets = _tree_blocks(blocks, 7)
+    words = torch.from_numpy(words_of(sets, 2)).to(cuda)
+    qd = q.to(cuda)
+    cache = kv8_from(lsk, cuda, k, v)
+    kf, vf = lsk.k_to_frag(k).to(cuda), lsk.v_to_blocked(v).to(cuda)
+
+    def run(sel, cap=None):
+        """sel: [(row, pos0, T, first token)]"""
+        tab, _ = pack_blocks([s[:3] for s in sel])
+        idx = torch.cat([torch.arange(s[3], s[3] + s[2]) for s in sel]).to(cuda)
+        plan = lsk.AttnPlan(tab, Hq, kf if kind == "tree" else cache, split=256)
+        if cap:
+            b = np.array(tab, dtype=np.int32)
+            works, groups, plan.n_parts = lsk.attn_plan(b, Hq // Hkv, 256, cap)
+            recs, plan.n_rounds = lsk.attn_schedule(works, Hkv, plan.n_slots)
+            up = [torch.from_numpy(x.ravel().copy()).to(cuda) for x in (works, groups, recs)]
+            plan.works, plan.groups, plan.recs = up
+            plan.n_works, plan.n_groups, plan.rows_cap = len(works), len(groups), cap
+            plan.ws_bytes = lsk.attn_workspace_bytes(plan.n_parts, Hkv, D)
+        m = words[idx].contiguous()
+        if kind == "tree":
+            return lsk.tree_attn(qd[idx], kf, vf, plan, m), idx
+        return lsk.kv8_attn(qd[idx], cache, plan, m if kind == "kv8 tree" else None), idx
+
+    whole = [(r, p, t, a) for (a, p, t, r) in tab]
+    full, _ = run(whole)
+    for cap in (16, 32, 48):
+        assert torch.equal(run(whole, cap)[0], full)
+    for sel in ([whole[1]], [whole[3], whole[0]], whole[::-1]):
+        got, idx = run(sel)
+        assert torch.equal(got, full[idx])
+    if kind == "kv8":
+        r, p, t, a = whole[1]
+        got, idx = run([(r, p + i, 1, a + i) for i in range(t)])
+        assert torch.equal(got, full[idx])
+
+
+@pytest.mark.gpu
+def test_attention_takes_strided_queries_at_any_address(cuda):
+    lsk = _lsk()
+    Hq, Hkv, D = 8, 2, 64
+    blocks = [(0, 37, 9), (1, 0, 3), (2, 200, 20)]
+    tab, q, k, v = _attn_inputs(31, (Hq, Hkv, D), blocks, S=256)
+    n = len(q)
+    _, sets = _tree_blocks(blocks, 9)
+    mask = torch.from_numpy(words_of(sets, 1)).to(cuda)
+    cache = kv8_from(lsk, cuda, k, v)
+    kf, vf = lsk.k_to_frag(k).to(cuda), lsk.v_to_blocked(v).to(cuda)
+    buf = torch.zeros(n * 1001 + 1, dtype=BF16, device=cuda)
+    strided = torch.as_strided(buf, (n, Hq, D), (1001, D + 3, 1), 1)
+    strided.copy_(q)
+    heads_first = q.transpose(0, 1).contiguous().to(cuda).transpose(0, 1)
+    odd = torch.zeros(n * Hq * D + 1, dtype=BF16, device=cuda)
+    out = odd[1:].view(n, Hq * D)                                     # an output that is only 2-byte aligned
+    p8, pt = lsk.AttnPlan(tab, Hq, cache, split=64), lsk.AttnPlan(tab, Hq, kf, split=64)
+    for run in (lambda x, o: lsk.kv8_attn(x, cache, p8, out=o), lambda x, o: lsk.kv8_attn(x, cache, p8, mask, out=o),
+                lambda x, o: lsk.tree_attn(x, kf, vf, pt, mask, out=o)):
+        want = run(q.to(cuda), None)
+        for x in (strided, heads_first):
+            assert torch.equal(run(x, None), want)
+        assert run(q.to(cuda), out) is out and torch.equal(out, want) and odd[0] == 0
+    same = q[:, :1].expand(n, Hq, D)                                  # one query for every head (stride 0)
+    assert torch.equal(lsk.kv8_attn(same.to(cuda)[:, :1].expand(n, Hq, D), cache, p8),
+                       lsk.kv8_attn(same.contiguous().to(cuda), cache, p8))
+
+
+@pytest.mark.gpu
+def test_attention_scale_streams_and_graph_replays(cuda):
+    """A scale of the caller's; calls on a side stream; a captured call replayed with new queries and cache contents
+    between eager calls (each call's split partials are its own)."""
+    lsk = _lsk()
+    Hq, Hkv, D = 8, 2, 128
+    blocks = [(0, 700, 9), (1, 900, 3)]
+    tab, q, k, v = _attn_inputs(37, (Hq, Hkv, D), blocks)
+    _, sets = _tree_blocks(blocks, 9)
+    mask = torch.from_numpy(words_of(sets, 1)).to(cuda)
+    cache = kv8_from(lsk, cuda, k, v)
+    kf, vf = lsk.k_to_frag(k).to(cuda), lsk.v_to_blocked(v).to(cuda)
+    p8, pt = lsk.AttnPlan(tab, Hq, cache, split=256), lsk.AttnPlan(tab, Hq, kf, split=256)
+    assert p8.n_parts > 0 and pt.n_parts > 0
+    qd = q.to(cuda)
+    ref, mag, _ = attention(q.double(), held(k), held(v), tab, 0.03)
+    assert_close_bf16(lsk.kv8_attn(qd, cache, p8, scale=0.03), ref, mag)
+
+    def both():
+        return lsk.kv8_attn(qd, cache, p8), lsk.tree_attn(qd, kf, vf, pt, mask)
+
+    want = both()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = both()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = both()
+        graphs.append((g, outs))
+    for i in range(4):
+        qd.copy_((torch.randn(q.shape, generator=_gen(100 + i))).to(BF16))
+        want = both()
+        for g, outs in graphs:
+            g.replay()
+            _ = both()
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.gpu
+def test_attention_of_offsets_past_32_bits(cuda):
+    """Cache rows whose first byte lies past 4 GiB: appended, read and attended to."""
+    lsk = _lsk()
+    Hq, Hkv, D, S = 2, 1, 128, 65536
+    B = (5 << 30) // (S * D)                                          # K codes of 5 GiB
+    cache = lsk.KV8.zeros(B, Hkv, S, D, cuda)
+    g = _gen(41)
+    n, row = 300, B - 1
+    k, v = (torch.randn(n, Hkv, D, generator=g).to(BF16) for _ in range(2))
+    pos = torch.arange(n)
+    rows = _i32(np.full(n, row), cuda)
+    lsk.kv8_append(k.to(cuda), v.to(cuda), cache, rows, _i32(pos, cuda))
+    assert torch.equal(lsk.kv8_read(cache, rows, _i32(pos, cuda), F32)[0].cpu().double(), held(k))
+    tab, q = [(0, n - 4, 4, row)], torch.randn(4, Hq, D, generator=g).to(BF16)
+    got = lsk.kv8_attn(q.to(cuda), cache, lsk.AttnPlan(tab, Hq, cache))
+    dense = lambda x: held(x).permute(1, 0, 2)[None].expand(row + 1, -1, -1, -1)  # noqa: E731
+    ref, mag, _ = attention(q.double(), dense(k), dense(v), tab, 1 / math.sqrt(D))
+    assert_close_bf16(got, ref, mag)
+
+
+# ----------------------------------------------------------------------------- masks, acceptance, compaction
+
+def accept(parents, tokens, y):
+    path = [0] if parents else []
+    while path:
+        nxt = [c for c in range(path[-1] + 1, len(parents)) if parents[c] == path[-1] and tokens[c] == y[path[-1]]]
+        if not nxt:
+            break
+        path.append(nxt[0])
+    return path
+
+
+def _forest(seed, sizes, vocab=3):
+    """Trees with few different tokens (siblings share some, long paths match by chance)."""
+    rng = np.random.default_rng(seed)
+    parents = [random_tree(rng, t) if t else [] for t in sizes]
+    tokens = [rng.integers(0, vocab, t) for t in sizes]
+    y = [rng.integers(0, vocab, t) for t in sizes]
+    return parents, tokens, y
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", [[1], [64, 1, 0, 13], [65, 33, 2], [300, 64, 7], [1] * 70])
+def test_tree_masks_and_acceptance_are_exact(cuda, sizes):
+    lsk = _lsk()
+    parents, tokens, y = _forest(len(sizes), sizes)
+    if len(sizes) == 4:
+        parents[3][5], parents[3][6] = 9, -3                          # no parents: a later node, a negative index
+        tokens[0][:], y[0][:] = 1, 1                                  # every child matches: the lowest is taken
+    starts = np.concatenate([[0], np.cumsum(sizes)[:-1]])
+    n, most = sum(sizes), max(sizes)
+    flat = lambda xs, dt: _cat(xs, dt, cuda)                          # noqa: E731
+    par = flat(parents, torch.int32)
+    mask, depth = lsk.tree_masks(par, _i32(starts, cuda), _i32(sizes, cuda), most)
+    sets = [s for p in parents for s in ancestors(p)]
+    assert np.array_equal(mask.cpu().numpy(), words_of(sets, (most + 31) // 32))
+    assert depth.cpu().tolist() == [len(s) - 1 for s in sets]
+    for extra in (0, 5):
+        acc, path, out = lsk.tree_accept(flat(y, torch.int64), flat(tokens, torch.int64), par, _i32(starts, cuda),
+                                         _i32(sizes, cuda), most + extra)
+        for b in range(len(sizes)):
+            want = accept(parents[b], tokens[b], y[b])
+            pad = [-1] * (most + extra - len(want))
+            assert int(acc[b]) == len(want) - 1
+            assert path[b].tolist() == want + pad
+            assert out[b].tolist() == [int(y[b][i]) for i in want] + pad
+    # a chain: lsk_greedy_accept's counts
+    T = 9
+    draft = np.array([5, 1, 2, 3, 4, 5, 6, 7, 8])
+    yv = np.array([1, 2, 3, 9, 5, 6, 7, 8, 1])
+    acc, path, out = lsk.tree_accept(*(torch.as_tensor(x).to(cuda) for x in (yv, draft)), _i32(np.arange(T) - 1, cuda),
+                                     _i32([0], cuda), _i32([T], cuda), T)
+    seq = torch.as_tensor(draft[None]).to(cuda).contiguous()
+    a2, y2 = torch.empty(1, dtype=torch.long, device=cuda), torch.empty(T, dtype=torch.long, device=cuda)
+    lsk.greedy_accept(torch.as_tensor(yv).to(cuda), seq, T, _i32([0], cuda), _i32([0], cuda), _i32([T], cuda), None, 1,
+                      a2, y2)
+    assert int(acc) == int(a2) == 3 and out[0, :4].tolist() == yv[:4].tolist()
+
+
+@pytest.mark.gpu
+def test_tree_acceptance_of_blocks_outside_the_tokens(cuda):
+    """Blocks that reach past the tokens, and nodes past max_nodes, take no part; nothing is read out of bounds."""
+    lsk = _lsk()
+    n = 10
+    par, tok = _i32(np.arange(n) - 1, cuda), torch.zeros(n, dtype=torch.int64, device=cuda)
+    starts, lens = _i32([0, 8, -1, 11, 0], cuda), _i32([10, 3, 2, 1, -4], cuda)
+    acc, path, out = lsk.tree_accept(tok, tok, par, starts, lens, 4)
+    assert acc.tolist() == [3, -1, -1, -1, -1] and path[0].tolist() == [0, 1, 2, 3] and (path[1:] == -1).all()
+    mask, depth = lsk.tree_masks(par, starts[:4], _i32([0, 3, 2, 1], cuda), 4)
+    assert (mask == 0).all() and (depth == 0).all()
+
+
+def _caches(lsk, cuda, fmt, L, B, H, S, D, g):
+    dt = F32 if fmt == "fp32" else BF16
+    k, v = (torch.randn(L, B, H, S, D, generator=g).to(dt) for _ in range(2))
+    if fmt == "kv8":
+        layers = [kv8_from(lsk, cuda, k[i], v[i]) for i in range(L)]
+        cache = lsk.KV8(*(torch.stack([c[j].view(torch.uint8) for c in layers]) for j in range(4)))
+        return lsk.KV8(cache.k.view(E4M3), cache.v.view(E4M3), cache.ks, cache.vs), held(k), held(v)
+    return ((lsk.k_to_frag(k) if fmt == "bf16" else k).to(cuda), lsk.v_to_blocked(v).to(cuda)), k.clone(), v.clone()
+
+
+def _dense(lsk, cuda, fmt, cache, dims):
+    L, B, H, S, D = dims
+    if fmt != "kv8":
+        k, v = cache
+        return (lsk.k_from_frag(k.cpu()) if fmt == "bf16" else k.cpu()), lsk.v_from_blocked(v.cpu())
+    rows, pos = _i32(np.repeat(np.arange(B), S), cuda), _i32(np.tile(np.arange(S), B), cuda)
+    out = [lsk.kv8_read(cache.layer(i), rows, pos, F32) for i in range(L)]
+    return tuple(torch.stack([o[j] for o in out]).view(L, B, S, H, D).transpose(2, 3).cpu() for j in (0, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,D", [("bf16", 128), ("bf16", 64), ("fp32", 16), ("fp32", 32), ("fp32", 128), ("kv8", 128),
+                                   ("kv8", 64)])
+def test_compaction_moves_the_accepted_paths_and_nothing_else(cuda, fmt, D):
+    lsk = _lsk()
+    L, B, H, S = 2, 5, 2, 192
+    cache, k, v = _caches(lsk, cuda, fmt, L, B, H, S, D, _gen(D))
+    rows, pos0 = [3, 0, 4, 1, 7, 2], [5, 60, 0, 191, 3, 100]          # row 7 is outside, row 1 ends with the cache
+    paths = [[0, 2, 3, 7, 20], [0] + list(range(2, 72, 2)), [0], [0, 1], [0, 3], []]
+    acc = [len(p) - 1 for p in paths]
+    most = max(len(p) for p in paths) + 1
+    path = np.full((len(paths), most), -1)
+    for i, p in enumerate(paths):
+        path[i, :len(p)] = p
+    args = (_i32(rows, cuda), _i32(pos0, cuda), torch.tensor(acc, device=cuda), _i32(path, cuda))
+    (lsk.kv8_compact(cache, *args) if fmt == "kv8" else lsk.kv_compact(*cache, *args))
+    for r, p0, p in zip(rows, pos0, paths):
+        if r >= B or (r == 1):
+            continue
+        src = [p0 + i for i in p]
+        for x in (k, v):
+            x[:, r, :, p0:p0 + len(p)] = x[:, r][:, :, src].clone()
+    got = _dense(lsk, cuda, fmt, cache, (L, B, H, S, D))
+    assert torch.equal(got[0].double(), k.double()) and torch.equal(got[1].double(), v.double())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "kv8", "fp32"])
+def test_a_run_of_tree_steps(cuda, fmt):
+    """Steps as an engine makes them: write a tree's K / V behind the committed prefix, attend, accept, compact, move
+    the length, and attend the next token over the compacted cache; against the 64-bit forms on a dense cache."""
+    lsk = _lsk()
+    Hq, Hkv, D, S, B = 4, 2, 64, 256, 3
+    dt = F32 if fmt == "fp32" else BF16
+    g = _gen(3)
+    if fmt == "kv8":
+        cache = lsk.KV8.zeros(B, Hkv, S, D, cuda, layers=1)
+        plan_cache = cache.layer(0)
+    else:
+        shape = (1, B, Hkv, S // 32, D // 16, 64, 8) if fmt == "bf16" else (1, B, Hkv, S, D)
+        kc = torch.zeros(shape, dtype=dt, device=cuda)
+        vc = torch.zeros(1, B, Hkv, S // 32, D, 32, dtype=dt, device=cuda)
+        plan_cache = kc[0]
+    kd, vd = (torch.zeros(B, Hkv, S, D, dtype=torch.float64) for _ in range(2))
+    kv_len = torch.zeros(B, dtype=torch.int64, device=cuda)
+    length = [0] * B
+    rng = np.random.default_rng(8)
+    for step in range(5):
+        sizes = [40, 20, 33] if step == 0 else [int(rng.integers(1, 30)) for _ in range(B)]
+        parents, tokens, y = _forest(step, sizes, vocab=2)
+        order = rng.permutation(B)
+        tab, n = pack_blocks([(int(r), length[r], sizes[r]) for r in order])
+        cat = lambda xs, t: _cat([xs[r] for r in order], t, cuda)     # noqa: E731
+        k, v = (torch.randn(n, Hkv, D, generator=g).to(dt) for _ in range(2))
+        q = torch.randn(n, Hq, D, generator=g).to(dt)
+        rows = np.concatenate([[r] * sizes[r] for r in order])
+        pos = np.concatenate([length[r] + np.arange(sizes[r]) for r in order])
+        starts, lens = _i32([b[0] for b in tab], cuda), _i32([b[2] for b in tab], cuda)
+        par = cat(parents, torch.int32)
+        mask, _ = lsk.tree_masks(par, starts, lens, max(sizes))
+        plan = lsk.AttnPlan(tab, Hq, plan_cache, split=None if step % 2 else 64)
+        if fmt == "kv8":
+            lsk.kv8_append(k.to(cuda), v.to(cuda), cache.layer(0), _i32(rows, cuda), _i32(pos, cuda))
+            got = lsk.kv8_attn(q.to(cuda), cache.layer(0), plan, mask)
+            k, v = held(k), held(v)
+        else:
+            lsk.kv_append(k.to(cuda), v.to(cuda), kc[0], vc[0], _i32(rows, cuda), _i32(pos, cuda))
+            got = lsk.tree_attn(q.to(cuda), kc[0], vc[0], plan, mask)
+        kd[rows, :, pos], vd[rows, :, pos] = k.double(), v.double()
+        sets = [s for r in order for s in ancestors(parents[r])]
+        ref, mag, big = attention(q.double(), kd, vd, tab, 1 / math.sqrt(D), sets)
+        assert_close_f32(got, ref, mag, S, D, big) if fmt == "fp32" else assert_close_bf16(got, ref, mag)
+        acc, path, _ = lsk.tree_accept(cat(y, torch.int64), cat(tokens, torch.int64), par, starts, lens, max(sizes))
+        r_t, p_t = _i32(order, cuda), _i32([length[r] for r in order], cuda)
+        if fmt == "kv8":
+            lsk.kv8_compact(cache, r_t, p_t, acc, path)
+        else:
+            lsk.kv_compact(kc, vc, r_t, p_t, acc, path)
+        lsk.kv_rollback(kv_len, r_t, acc, B)
+        for i, r in enumerate(order):
+            p = accept(parents[r], tokens[r], y[r])
+            assert int(acc[i]) == len(p) - 1
+            src = [length[r] + j for j in p]
+            kd[r, :, length[r]:length[r] + len(p)] = kd[r][:, src].clone()
+            vd[r, :, length[r]:length[r] + len(p)] = vd[r][:, src].clone()
+            length[r] += len(p)
+        assert kv_len.cpu().tolist() == length
+
+
+# ----------------------------------------------------------------------------- refusals (no GPU needed)
+
+def test_entry_points_refuse_bad_arguments():
+    lib = _lsk().load()
+    P = 16
+    a = lib.lsk_kv8_append
+    ok = [1, P, P, 128, 64, P, P, P, P, P, P, 4, 2, 64, 3, 128, None]
+    bad = lambda i, x: a(*(ok[:i] + [x] + ok[i + 1:]))                # noqa: E731
+    for i in (1, 2, 5, 6, 7, 8, 9, 10):
+        assert bad(i, None) == -1
+    assert bad(0, 7) == -3 and bad(13, 96) == -3 and bad(15, 96) == -2 and bad(11, -1) == -2 and bad(3, -1) == -2
+    assert bad(5, 24) == -1 and bad(14, 0) == -2                      # a cache off 16 bytes; no rows
+    assert bad(11, 0) == 0                                            # no tokens: no launch
+    r = lib.lsk_kv8_read
+    assert r(1, P, P, P, P, P, P, P, None, 4, 2, 64, 3, 128, None) == -1
+    assert r(1, P, P, P, P, P, P, P, P, 4, 2, 32, 3, 128, None) == -3
+    assert r(1, P, P, P, P, P, P, P, P, 0, 2, 64, 3, 128, None) == 0
+    ok = [P, 512, 64, P, P, P, P, None, 0, P, 1, None, 0, 0, P, 1, 1, 16, P, 8, 2, 64, 128, 0.125, None, 0, None]
+    k8 = lambda **kw: lib.lsk_kv8_attn(*[kw.get(f"a{i}", x) for i, x in enumerate(ok)])  # noqa: E731
+    assert k8(a0=None) == -1 and k8(a5=None) == -1 and k8(a14=None) == -1 and k8(a17=24) == -1 and k8(a7=P) == -1
+    assert k8(a19=7) == -2 and k8(a22=96) == -2 and k8(a21=32) == -3 and k8(a3=24) == -1 and k8(a1=-1) == -2
+    assert k8(a13=3) == -4 and k8(a13=3, a11=P, a24=P, a25=100) == -4          # split partials without their workspace
+    assert k8(a22=1 << 25) == -2                                               # a stripe of 2 GiB and more
+    assert k8(a10=0) == 0
+    ok2 = [1, P, 512, 64, P, P, P, 1, P, P, 1, None, 0, 0, P, 1, 1, 16, P, 8, 2, 64, 128, 0.125, None, 0, None]
+    tr = lambda **kw: lib.lsk_tree_attn(*[kw.get(f"a{i}", x) for i, x in enumerate(ok2)])  # noqa: E731
+    assert tr(a6=None) == -1 and tr(a7=0) == -1 and tr(a0=2) == -3 and tr(a14=None) == -1 and tr(a21=96) == -3
+    assert tr(a0=0, a13=2) == -1 and tr(a0=0, a21=80) == -3 and tr(a0=0, a9=None) == -1 and tr(a10=0) == 0
+    m = lib.lsk_tree_masks
+    assert m(None, P, P, 1, 4, 4, P, 1, None, None) == -1 and m(P, P, P, 1, 4, 33, P, 1, None, None) == -2
+    assert m(P, P, P, 0, 4, 4, P, 1, None, None) == 0 and m(P, P, P, 1, 0, 4, P, 1, None, None) == 0
+    t = lib.lsk_tree_accept
+    assert t(P, P, P, P, None, 1, 4, 4, P, P, P, None) == -1 and t(P, P, P, P, P, 1, 4, 0, P, P, P, None) == -2
+    assert t(P, P, P, P, P, 0, 4, 4, P, P, P, None) == 0
+    c = lib.lsk_kv_compact
+    assert c(1, None, P, None, None, 1, P, P, P, P, 1, 4, 2, 64, 3, 128, None) == -1
+    assert c(2, P, P, None, P, 1, P, P, P, P, 1, 4, 2, 64, 3, 128, None) == -1
+    assert c(3, P, P, P, P, 1, P, P, P, P, 1, 4, 2, 64, 3, 128, None) == -3
+    assert c(1, P, P, None, None, 1, P, P, P, P, 1, 4, 2, 32, 3, 128, None) == -3
+    assert c(2, P, P, P, P, 1, P, P, P, P, 1, 4, 2, 64, 3, 96, None) == -2
+    assert c(1, P, P, None, None, 0, P, P, P, P, 1, 4, 2, 64, 3, 128, None) == 0
+
+
+def test_plans_refuse_blocks_outside_the_cache():
+    lsk = _lsk()
+    cache = lsk.KV8.zeros(2, 2, 128, 64, "cpu")
+    plan = lsk.AttnPlan([(0, 3, 2, 1), (2, 0, 0, 0), (2, 127, 1, 0)], 4, cache)
+    assert plan.n_tokens == 3 and plan.n_works > 0 and plan.split == 512
+    for b in ([(0, 3, 2, 2)], [(0, 3, 2, -1)], [(0, 127, 2, 0)], [(0, -1, 2, 0)], [(1, 0, 2, 0)], [(0, 0, -1, 0)]):
+        with pytest.raises(ValueError):
+            lsk.AttnPlan(b, 4, cache)
+    with pytest.raises(ValueError):
+        lsk.AttnPlan([(0, 0, 1, 0)], 3, cache)
+    with pytest.raises(ValueError):
+        lsk.AttnPlan([(0, 0, 1, 0)], 4, cache, split=100)
+    with pytest.raises(ValueError):
+        lsk.KV8.zeros(2, 2, 100, 64, "cpu")
+    with pytest.raises(ValueError):
+        lsk.KV8.zeros(2, 2, 128, 96, "cpu")
+    assert lsk.AttnPlan([], 4, cache).n_works == 0
+    assert lsk.cache_attn_split(1, 8, 131072) * 128 >= 131072 and lsk.cache_attn_split(256, 8, 8192) == 8192
+
+
+def test_wrappers_refuse_tensors_off_the_gpu():
+    lsk = _lsk()
+    cache = lsk.KV8.zeros(1, 1, 64, 64, "cpu")
+    x, i = torch.zeros(1, 1, 64, dtype=BF16), torch.zeros(1, dtype=torch.int32)
+    plan = lsk.AttnPlan([(0, 0, 1, 0)], 1, cache)
+    for f in (lambda: lsk.kv8_append(x, x, cache, i, i), lambda: lsk.kv8_read(cache, i, i),
+              lambda: lsk.kv8_attn(x, cache, plan), lambda: lsk.tree_masks(i, i, i, 1)):
+        with pytest.raises(lsk.LskError):
+            f()
+
+
+@pytest.mark.gpu
+def test_wrappers_refuse_what_does_not_fit(cuda):
+    lsk = _lsk()
+    cache = lsk.KV8.zeros(2, 2, 128, 64, cuda)
+    x, i = torch.zeros(3, 2, 64, dtype=BF16, device=cuda), torch.zeros(3, dtype=torch.int32, device=cuda)
+    plan = lsk.AttnPlan([(0, 0, 3, 0)], 4, cache)
+    q = torch.zeros(3, 4, 64, dtype=BF16, device=cuda)
+    m = torch.zeros(3, 1, dtype=torch.int32, device=cuda)
+    kf = torch.zeros(2, 2, 4, 4, 64, 8, dtype=BF16, device=cuda)
+    vf = torch.zeros(2, 2, 4, 64, 32, dtype=BF16, device=cuda)
+    pt = lsk.AttnPlan([(0, 0, 3, 0)], 4, kf)
+    big = lsk.KV8.zeros(2, 2, 192, 64, cuda)
+    a = torch.zeros(1, dtype=torch.int64, device=cuda)
+    calls = [lambda: lsk.kv8_append(x.half(), x.half(), cache, i, i), lambda: lsk.kv8_append(x, x[:2], cache, i, i),
+             lambda: lsk.kv8_append(x, x, cache, i.long(), i), lambda: lsk.kv8_append(x, x, cache, i[:2], i),
+             lambda: lsk.kv8_append(x.transpose(0, 2).contiguous().transpose(0, 2), x, cache, i, i),
+             lambda: lsk.kv8_append(x, x, cache._replace(ks=cache.ks[:1]), i, i),
+             lambda: lsk.kv8_append(x.cpu(), x, cache, i, i), lambda: lsk.kv8_read(cache, i, i, torch.float16),
+             lambda: lsk.kv8_attn(q, big, plan), lambda: lsk.kv8_attn(q[:2], cache, plan),
+             lambda: lsk.kv8_attn(q.float(), cache, plan), lambda: lsk.kv8_attn(q, cache, pt),
+             lambda: lsk.kv8_attn(q, cache, plan, m[:2]), lambda: lsk.kv8_attn(q, cache, plan, m.long()),
+             lambda: lsk.kv8_attn(q, cache, plan, out=torch.zeros(3, 128, dtype=BF16, device=cuda)),
+             lambda: lsk.tree_attn(q, kf, vf, plan, m), lambda: lsk.tree_attn(q, kf, vf[:, :1], pt, m),
+             lambda: lsk.tree_attn(q, kf, vf, pt, m.cpu()),
+             lambda: lsk.kv_compact(kf, vf, i[:1], i[:1], a, m[:1]),
+             lambda: lsk.kv_compact(kf[None], vf[None], i[:1], i[:1], a[:0], m[:1]),
+             lambda: lsk.kv8_compact(cache, i[:1], i[:1], a, m[:1]),
+             lambda: lsk.tree_accept(a, a, i, i[:1], i[:1], 1)]
+    for f in calls:
+        with pytest.raises(lsk.LskError):
+            f()
+    assert lsk.kv8_attn(q[:0], cache, lsk.AttnPlan([], 4, cache)).shape == (0, 256)
+    k, v = lsk.kv8_read(cache, i[:0], i[:0])
+    assert k.shape == v.shape == (0, 2, 64)

@@ -7,9 +7,12 @@ There is no fallback: a missing or stale library raises at the first call.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import math
 import os
 from pathlib import Path
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -18,11 +21,12 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liblsk.so"
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_KV8 = 2             # an 8-bit KV cache, where an entry point takes one
 EPI_NONE, EPI_RESIDUAL, EPI_SILU_MUL = 0, 1, 2
 EPI_PARTIAL, EPI_ARGMAX, EPI_QKV_ROPE = 3, 4, 5   # launch kinds known to lsk_gemm_wide_config
 ATTN_SPLIT = 8192         # LSK_ATTN_SPLIT
 ATTN_ROWS = 48            # query rows per attention work item (csrc/lsk_attention.hip ATTN_ROWS)
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 # name -> (restype, argtypes)
 _P, _I, _L, _F, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float, ctypes.c_size_t
@@ -73,6 +77,15 @@ _SIGS = {
     "lsk_gemm_residual_frag": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "lsk_forward_layers": (_I, [_L, _P, _P, _I, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P, _Z, _P,
                                 ctypes.c_double, ctypes.c_double, _P]),
+    "lsk_kv8_append": (_I, [_I, _P, _P, _L, _L] + [_P] * 6 + [_I] * 5 + [_P]),
+    "lsk_kv8_read": (_I, [_I] + [_P] * 8 + [_I] * 5 + [_P]),
+    "lsk_kv8_attn": (_I, [_P, _L, _L] + [_P] * 5 + [_I, _P, _I, _P, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _I, _F, _P,
+                          _Z, _P]),
+    "lsk_tree_attn": (_I, [_I, _P, _L, _L, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _I,
+                           _F, _P, _Z, _P]),
+    "lsk_tree_masks": (_I, [_P, _P, _P, _I, _I, _I, _P, _I, _P, _P]),
+    "lsk_tree_accept": (_I, [_P] * 5 + [_I, _I, _I] + [_P] * 4),
+    "lsk_kv_compact": (_I, [_I] + [_P] * 4 + [_I] + [_P] * 4 + [_I] * 6 + [_P]),
     "lsk_prof_enable": (_I, [_I]),
     "lsk_prof_start": (_I, [_I, ctypes.c_double, ctypes.c_double, _P]),
     "lsk_prof_stop": (_I, [_P]),
@@ -502,6 +515,312 @@ def shift_segment_positions(meta, n_tokens: int, nb: int, n_works: int, n_groups
     _check(load().lsk_shift_segment_positions(_ptr(meta), n_tokens, nb, n_works, n_groups, n_recs, group,
                                               _ptr(accepted), _ptr(vslots), _ptr(vdrafts), nv, _stream()),
            "lsk_shift_segment_positions")
+
+
+# ----------------------------------------------------------------------------- 8-bit cache and trees of drafted tokens
+
+def _one_device(*ts) -> torch.device:
+    """The device that all the tensors are on (None is skipped); LskError otherwise."""
+    _dev(*ts)
+    devs = {t.device for t in ts if t is not None}
+    if len(devs) != 1:
+        raise LskError(f"tensors on different devices: {sorted(map(str, devs))}")
+    return devs.pop()
+
+
+def _current(device: torch.device):
+    """A context in which `device` is the current one (its current stream takes the launch)."""
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _want(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise LskError(f"{what}: {name} must be a contiguous {list(shape)} {dtype} tensor, got {list(t.shape)} {t.dtype}"
+                       f"{'' if t.is_contiguous() else ', not contiguous'}")
+
+
+class KV8(NamedTuple):
+    """An 8-bit K / V cache (lsk_kv8_append): e4m3 codes and one power-of-two scale per position and KV head, the byte
+    e + 127.  A layer's tensors, or with a leading layer axis those of several:
+      k [B, Hkv, S/64, 4, D/64, 64, 16] and v [B, Hkv, S/64, D, 64] float8_e4m3fn, ks and vs [B, Hkv, S] uint8."""
+    k: torch.Tensor
+    v: torch.Tensor
+    ks: torch.Tensor
+    vs: torch.Tensor
+
+    @classmethod
+    def zeros(cls, max_batch: int, n_kv_heads: int, max_seq: int, head_dim: int, device, layers: int | None = None):
+        if head_dim not in (64, 128) or max_seq % 64 or max_seq <= 0:
+            raise ValueError(f"8-bit caches need head_dim 64 or 128 and max_seq a multiple of 64 (got {head_dim}, "
+                             f"{max_seq})")
+        lead = (max_batch, n_kv_heads) if layers is None else (layers, max_batch, n_kv_heads)
+        codes = dict(dtype=torch.uint8, device=device)
+        return cls(torch.zeros(*lead, max_seq // 64, 4, head_dim // 64, 64, 16, **codes).view(torch.float8_e4m3fn),
+                   torch.zeros(*lead, max_seq // 64, head_dim, 64, **codes).view(torch.float8_e4m3fn),
+                   torch.full((*lead, max_seq), 127, **codes), torch.full((*lead, max_seq), 127, **codes))
+
+    def layer(self, i: int) -> "KV8":
+        return KV8(self.k[i], self.v[i], self.ks[i], self.vs[i])
+
+    @property
+    def dims(self) -> tuple:
+        """(B, Hkv, S, D)"""
+        *_, B, Hkv, S = self.ks.shape
+        return B, Hkv, S, self.v.shape[-2]
+
+    def check(self, what: str, layers: bool = False) -> None:
+        n = 1 if layers else 0
+        if self.ks.dim() != 3 + n or self.v.dim() != 5 + n:
+            raise LskError(f"{what}: an 8-bit cache of {'several layers' if layers else 'one layer'} is needed")
+        lead = tuple(self.ks.shape[:2 + n])
+        _, _, S, D = self.dims
+        if D not in (64, 128) or S % 64 or S == 0:
+            raise LskError(f"{what}: 8-bit caches need head_dim 64 or 128 and max_seq a multiple of 64 (got {D}, {S})")
+        _want(what, "k codes", self.k, torch.float8_e4m3fn, (*lead, S // 64, 4, D // 64, 64, 16))
+        _want(what, "v codes", self.v, torch.float8_e4m3fn, (*lead, S // 64, D, 64))
+        _want(what, "k exponents", self.ks, torch.uint8, (*lead, S))
+        _want(what, "v exponents", self.vs, torch.uint8, (*lead, S))
+
+
+def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor) -> None:
+    """k, v [N, Hkv, D] (bf16 or fp32, of equal strides; dims contiguous) quantised into a layer's 8-bit cache at
+    (rows, pos).  Tokens outside the cache are skipped; the (row, position) pairs of a call have to differ."""
+    dev = _one_device(k, v, *cache, rows_i32, pos_i32)
+    cache.check("kv8_append")
+    B, Hkv, S, D = cache.dims
+    n = k.shape[0]
+    if k.shape != (n, Hkv, D) or v.shape != k.shape or v.dtype != k.dtype:
+        raise LskError(f"kv8_append: k and v must be [N, {Hkv}, {D}] of one dtype, got {list(k.shape)} {k.dtype} and "
+                       f"{list(v.shape)} {v.dtype}")
+    if n and (k.stride(2) != 1 or v.stride(2) != 1 or k.stride() != v.stride()):
+        raise LskError("kv8_append: k and v need contiguous dims and the same strides")
+    _want("kv8_append", "rows", rows_i32, torch.int32, (n,))
+    _want("kv8_append", "pos", pos_i32, torch.int32, (n,))
+    code = dtype_code(k.dtype)
+    if n == 0:
+        return
+    with _current(dev):
+        _check(load().lsk_kv8_append(code, _ptr(k), _ptr(v), k.stride(0), k.stride(1), *map(_ptr, cache), _ptr(rows_i32),
+                                     _ptr(pos_i32), n, Hkv, D, B, S, _stream()), "lsk_kv8_append")
+
+
+def kv8_read(cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
+             out: tuple | None = None) -> tuple:
+    """The K and V that a layer's 8-bit cache holds at (rows, pos): two [N, Hkv, D] tensors (bf16: exactly); zeros for
+    tokens outside the cache."""
+    dev = _one_device(*cache, rows_i32, pos_i32, *(out or ()))
+    cache.check("kv8_read")
+    B, Hkv, S, D = cache.dims
+    n = rows_i32.numel()
+    _want("kv8_read", "rows", rows_i32, torch.int32, (n,))
+    _want("kv8_read", "pos", pos_i32, torch.int32, (n,))
+    code = dtype_code(dtype if out is None else out[0].dtype)
+    if out is None:
+        out = tuple(torch.empty(n, Hkv, D, dtype=dtype, device=dev) for _ in range(2))
+    for t in out:
+        _want("kv8_read", "out", t, out[0].dtype, (n, Hkv, D))
+    if n:
+        with _current(dev):
+            _check(load().lsk_kv8_read(code, *map(_ptr, cache), _ptr(rows_i32), _ptr(pos_i32), _ptr(out[0]),
+                                       _ptr(out[1]), n, Hkv, D, B, S, _stream()), "lsk_kv8_read")
+    return out
+
+
+def cache_attn_split(max_batch: int, n_kv_heads: int, max_seq: int) -> int:
+    """KV positions per attention split of a cache: fixed by the cache, so that a row's result never depends on the
+    batch it is in.  Caches of many (row, KV head) stripes keep a context whole; with fewer, a context is shared by
+    several workgroups.  At most 128 splits per context."""
+    stripes = max_batch * n_kv_heads
+    split = ATTN_SPLIT if stripes >= 1024 else 2048 if stripes >= 256 else 512
+    return max(split, (max_seq + 128 * 64 - 1) // (128 * 64) * 64)
+
+
+class AttnPlan:
+    """The plan of an attention launch over packed blocks, shared by the layers of a segment (lsk_attn_plan and
+    lsk_attn_schedule, on the device).  blocks: int [nb, 4] = (q_start, pos0, T, row) with q_start the running sum of
+    T; cache: a layer's KV8, or the K storage of a bf16 or fp32 cache.  split: KV positions per split (fp32: unsplit)."""
+
+    def __init__(self, blocks, n_heads: int, cache, split: int | None = None):
+        kcache = cache.k if isinstance(cache, KV8) else cache
+        self.dims = B, Hkv, S, D = cache.dims if isinstance(cache, KV8) else k_dims(cache)
+        self.kv8, self.dtype = isinstance(cache, KV8), kcache.dtype
+        if n_heads <= 0 or n_heads % Hkv:
+            raise ValueError(f"{n_heads} query heads over {Hkv} KV heads")
+        b = np.asarray(blocks, dtype=np.int64).reshape(-1, 4)
+        if len(b) and (not np.array_equal(b[:, 0], np.cumsum(b[:, 2]) - b[:, 2]) or (b[:, 1:3] < 0).any()):
+            raise ValueError("blocks: q_start must be the running sum of T, pos0 and T not negative")
+        if len(b) and ((b[:, 3] < 0) | (b[:, 3] >= B) | (b[:, 1] + b[:, 2] > S)).any():
+            raise ValueError(f"a block lies outside the cache's {B} rows x {S} positions")
+        if (split is not None and (split < 64 or split % 64)) or len(b) and int(b[:, 2].sum()) >= 1 << 30:
+            raise ValueError(f"a split of {split} positions (a multiple of 64), or too many tokens")
+        if self.dtype == torch.float32:
+            split = 1 << 30
+        elif split is None:
+            split = cache_attn_split(B, Hkv, S)
+        self.n_heads, self.split, self.n_tokens = n_heads, split, int(b[:, 2].sum())
+        self.device, group = kcache.device, n_heads // Hkv
+        b = b.astype(np.int32)
+        self.n_slots = cu_count(self.device)
+        self.rows_cap = attn_rows_cap(b, group, split, Hkv, D, self.n_slots)
+        works, groups, self.n_parts = attn_plan(b, group, split, self.rows_cap)
+        recs, self.n_rounds = attn_schedule(works, Hkv, self.n_slots)
+        self.n_works, self.n_groups = len(works), len(groups)
+        parts = [b.ravel(), works.ravel(), groups.ravel(), recs]
+        meta = torch.from_numpy(np.concatenate(parts).astype(np.int32))
+        if self.device.type == "cuda":
+            meta = meta.pin_memory().to(self.device, non_blocking=True)
+        self.blocks, self.works, self.groups, self.recs = meta.split([len(p) for p in parts])
+        self.ws_bytes = attn_workspace_bytes(self.n_parts, Hkv, D) if self.n_parts else 0
+
+
+def _plan_call(what: str, q: torch.Tensor, plan: AttnPlan, dims: tuple, kv8: bool, dtype: torch.dtype, mask, scale, out,
+               workspace):
+    """Checks shared by kv8_attn and tree_attn; returns (scale, out, workspace, its bytes)."""
+    if plan.dims != dims or plan.kv8 != kv8 or plan.dtype != dtype:
+        raise LskError(f"{what}: the plan was made for another cache ({plan.dims} {plan.dtype})")
+    _, Hkv, _, D = dims
+    want = torch.bfloat16 if kv8 else dtype
+    if q.shape != (plan.n_tokens, plan.n_heads, D) or q.dtype != want or (q.numel() and q.stride(2) != 1):
+        raise LskError(f"{what}: q must be [{plan.n_tokens}, {plan.n_heads}, {D}] {want} with contiguous dims, got "
+                       f"{list(q.shape)} {q.dtype}")
+    if mask is not None and (mask.dim() != 2 or mask.shape[1] < 1):
+        raise LskError(f"{what}: mask must be [{plan.n_tokens}, words]")
+    if mask is not None:
+        _want(what, "mask", mask, torch.int32, (plan.n_tokens, mask.shape[1]))
+    if out is None:
+        out = torch.empty(plan.n_tokens, plan.n_heads * D, dtype=want, device=q.device)
+    _want(what, "out", out, want, (plan.n_tokens, plan.n_heads * D))
+    if workspace is None and plan.ws_bytes:
+        workspace = torch.empty(plan.ws_bytes, dtype=torch.uint8, device=q.device)
+    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    return 1.0 / math.sqrt(D) if scale is None else float(scale), out, workspace, ws_bytes
+
+
+def kv8_attn(q: torch.Tensor, cache: KV8, plan: AttnPlan, mask: torch.Tensor | None = None, scale: float | None = None,
+             out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Ragged verify / decode attention over a layer's 8-bit cache (lsk_kv8_attn): q [N, Hq, D] bf16 -> [N, Hq * D].
+    mask (int32 [N, words], tree_masks): blocks are trees of drafted tokens.  scale: 1 / sqrt(D) unless given.  Without
+    a workspace one is taken from torch's allocator for the call."""
+    dev = _one_device(q, *cache, plan.recs, mask, out, workspace)
+    cache.check("kv8_attn")
+    scale, out, workspace, ws = _plan_call("kv8_attn", q, plan, cache.dims, True, cache.k.dtype, mask, scale, out,
+                                           workspace)
+    if plan.n_works:
+        _, Hkv, S, D = cache.dims
+        with _current(dev):
+            _check(load().lsk_kv8_attn(_ptr(q), q.stride(0), q.stride(1), *map(_ptr, cache), _ptr(mask),
+                                       mask.shape[1] if mask is not None else 0, _ptr(plan.blocks), plan.n_works,
+                                       _ptr(plan.groups), plan.n_groups, plan.n_parts, _ptr(plan.recs), plan.n_rounds,
+                                       plan.n_slots, plan.rows_cap, _ptr(out), plan.n_heads, Hkv, D, S, scale,
+                                       _ptr(workspace), ws, _stream()), "lsk_kv8_attn")
+    return out
+
+
+def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, plan: AttnPlan, mask: torch.Tensor,
+              scale: float | None = None, out: torch.Tensor | None = None,
+              workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of trees of drafted tokens over a layer's bf16 or fp32 cache (lsk_tree_attn): q [N, Hq, D] ->
+    [N, Hq * D].  kcache: K cache storage (k_dims); vcache: the blocked-transposed V storage; mask: int32 [N, words]
+    (tree_masks).  scale: 1 / sqrt(D) unless given."""
+    dev = _one_device(q, kcache, vcache, plan.recs, mask, out, workspace)
+    _check_kcache(kcache.dtype, kcache)
+    code = dtype_code(kcache.dtype)
+    dims = B, Hkv, S, D = k_dims(kcache)
+    if not kcache.is_contiguous():
+        raise LskError("tree_attn: the K cache must be contiguous")
+    _want("tree_attn", "V cache", vcache, kcache.dtype, (B, Hkv, S // 32, D, 32))
+    scale, out, workspace, ws = _plan_call("tree_attn", q, plan, dims, False, kcache.dtype, mask, scale, out, workspace)
+    if plan.n_works:
+        with _current(dev):
+            _check(load().lsk_tree_attn(code, _ptr(q), q.stride(0), q.stride(1), _ptr(kcache), _ptr(vcache), _ptr(mask),
+                                        mask.shape[1], _ptr(plan.blocks), _ptr(plan.works), plan.n_works,
+                                        _ptr(plan.groups), plan.n_groups, plan.n_parts, _ptr(plan.recs), plan.n_rounds,
+                                        plan.n_slots, plan.rows_cap, _ptr(out), plan.n_heads, Hkv, D, S, scale,
+                                        _ptr(workspace), ws, _stream()), "lsk_tree_attn")
+    return out
+
+
+def tree_masks(parents: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, max_nodes: int) -> tuple:
+    """Trees of drafted tokens -> (mask int32 [N, words], depth int32 [N]) (lsk_tree_masks): the bits of each node's
+    ancestors and its own, and its depth.  parents [N], starts and lens [nb] int32 on the device; max_nodes >= every
+    len."""
+    dev = _one_device(parents, starts, lens)
+    n, nb = parents.numel(), starts.numel()
+    for name, t, k in (("parents", parents, n), ("starts", starts, nb), ("lens", lens, nb)):
+        _want("tree_masks", name, t, torch.int32, (k,))
+    words = max(1, (max_nodes + 31) // 32)
+    mask = torch.zeros(n, words, dtype=torch.int32, device=dev)
+    depth = torch.zeros(n, dtype=torch.int32, device=dev)
+    if n and nb:
+        with _current(dev):
+            _check(load().lsk_tree_masks(_ptr(parents), _ptr(starts), _ptr(lens), nb, n, max_nodes, _ptr(mask), words,
+                                         _ptr(depth), _stream()), "lsk_tree_masks")
+    return mask, depth
+
+
+def tree_accept(Yv: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, starts: torch.Tensor,
+                lens: torch.Tensor, max_nodes: int) -> tuple:
+    """Greedy acceptance of verified trees (lsk_tree_accept) -> (accepted int64 [nb], path int32 [nb, max_nodes],
+    tokens int64 [nb, max_nodes]): the accepted nodes and the tokens to commit, -1 past the end.  Yv (the verifier's
+    greedy token of every node) and tokens int64 [N], parents int32 [N], starts and lens int32 [nb]."""
+    dev = _one_device(Yv, tokens, parents, starts, lens)
+    n, nb = parents.numel(), starts.numel()
+    for name, t, dt, k in (("Yv", Yv, torch.int64, n), ("tokens", tokens, torch.int64, n),
+                           ("parents", parents, torch.int32, n), ("starts", starts, torch.int32, nb),
+                           ("lens", lens, torch.int32, nb)):
+        _want("tree_accept", name, t, dt, (k,))
+    if max_nodes < 1:
+        raise LskError(f"tree_accept: max_nodes {max_nodes}")
+    acc = torch.empty(nb, dtype=torch.int64, device=dev)
+    path = torch.empty(nb, max_nodes, dtype=torch.int32, device=dev)
+    out = torch.empty(nb, max_nodes, dtype=torch.int64, device=dev)
+    if nb and n == 0:
+        acc.fill_(-1), path.fill_(-1), out.fill_(-1)
+    elif nb:
+        with _current(dev):
+            _check(load().lsk_tree_accept(_ptr(Yv), _ptr(tokens), _ptr(parents), _ptr(starts), _ptr(lens), nb, n,
+                                          max_nodes, _ptr(acc), _ptr(path), _ptr(out), _stream()), "lsk_tree_accept")
+    return acc, path, out
+
+
+def _compact(what, code, k, v, ks, vs, layers, dims, rows_i32, pos0_i32, accepted, path) -> None:
+    dev = _one_device(k, v, ks, vs, rows_i32, pos0_i32, accepted, path)
+    nb = rows_i32.numel()
+    B, Hkv, S, D = dims
+    _want(what, "rows", rows_i32, torch.int32, (nb,))
+    _want(what, "pos0", pos0_i32, torch.int32, (nb,))
+    _want(what, "accepted", accepted, torch.int64, (nb,))
+    if path.dim() != 2 or path.shape[1] < 1:
+        raise LskError(f"{what}: path must be [{nb}, max_nodes]")
+    _want(what, "path", path, torch.int32, (nb, path.shape[1]))
+    if nb and layers:
+        with _current(dev):
+            _check(load().lsk_kv_compact(code, _ptr(k), _ptr(v), _ptr(ks), _ptr(vs), layers, _ptr(rows_i32),
+                                         _ptr(pos0_i32), _ptr(accepted), _ptr(path), nb, path.shape[1], Hkv, D, B, S,
+                                         _stream()), "lsk_kv_compact")
+
+
+def kv_compact(k: torch.Tensor, v: torch.Tensor, rows_i32, pos0_i32, accepted, path) -> None:
+    """The accepted paths' K / V move to consecutive slots in every layer (lsk_kv_compact): slot pos0 + j of a cache row
+    takes slot pos0 + path[j], j = 1 .. accepted.  k, v: the layers' storage (KVCache.kf_all or fp32 rows, and vb_all;
+    or a run of their layers); path and accepted: tree_accept's; rows, pos0 int32 [nb], the rows different."""
+    if k.dim() not in (5, 7) or not k.is_contiguous():
+        raise LskError("kv_compact: the K storage of several layers is needed, contiguous")
+    _check_kcache(k.dtype, k[0] if k.shape[0] else k.new_empty(k.shape[1:]))
+    code = dtype_code(k.dtype)
+    B, Hkv = k.shape[1:3]
+    S, D = (k.shape[3] * 32, k.shape[4] * 16) if k.dim() == 7 else (k.shape[3], k.shape[4])
+    _want("kv_compact", "V storage", v, k.dtype, (k.shape[0], B, Hkv, S // 32, D, 32))
+    _compact("kv_compact", code, k, v, None, None, k.shape[0], (B, Hkv, S, D), rows_i32, pos0_i32, accepted, path)
+
+
+def kv8_compact(cache: KV8, rows_i32, pos0_i32, accepted, path) -> None:
+    """kv_compact for the layers of an 8-bit cache (tensors with a leading layer axis)."""
+    cache.check("kv8_compact", layers=True)
+    _compact("kv8_compact", DTYPE_KV8, cache.k, cache.v, cache.ks, cache.vs, cache.k.shape[0], cache.dims, rows_i32,
+             pos0_i32, accepted, path)
 
 
 # ----------------------------------------------------------------------------- layer-range runner
