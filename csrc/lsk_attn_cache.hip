@@ -27,6 +27,8 @@
 // The 8 waves of a workgroup take the STEP-position steps of an item round robin and are merged in wave order through
 // LDS.  Which wave takes a step and every order of additions depend on absolute positions only: a row's result never
 // depends on what else is in the launch, and a chain over a bf16 cache gives the ragged attention's bits.
+#include <type_traits>
+
 #include "lsk_attn.h"
 #include "../include/lsk.h"
 
@@ -50,8 +52,8 @@ struct CacheAttnArgs {
   float scale_log2;
 };
 
-// The 16 (NE) mask bits of a token for its block's slots first .. first + NE - 1, relative to pos0: slots before the
-// block are read by every token; bits past the words are 0.
+// The mask bits of a token for its block's slots rel .. rel + 31, relative to pos0: slots before the block are read by
+// every token; bits past the words are 0.
 __device__ __forceinline__ uint32_t mask_window(const uint32_t* words, int W, int rel) {
   const int w = rel >> 5, sh = rel & 31;
   const uint32_t lo = (w >= 0 && w < W) ? words[w] : 0u;
@@ -75,12 +77,12 @@ __device__ __forceinline__ float exp_bits(uint32_t byte) { return __uint_as_floa
 
 }  // namespace
 
+#define ORDER() __builtin_amdgcn_sched_barrier(0)
+
 template <int D, int QT, bool KV8, bool TREE>
 __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const CacheAttnArgs A) {
   constexpr int STEP = KV8 ? 64 : 32;                // positions per step of a wave
-  constexpr int NA = STEP / 16;                      // 16-position S^T tiles per step
-  constexpr int NE = 4 * NA;                         // consecutive positions per lane
-  constexpr int HV = STEP / 32;                      // P^T operands per step
+  constexpr int HV = STEP / 32;                      // 32-position halves of a step; a lane group has 8 slots of each
   constexpr int KF = D / 32;                         // K operands per 16-position tile
   constexpr int CT = D / 16;                         // 16-byte loads per lane of a step, for K and for V
   constexpr int NW = ATTN_WAVES;
@@ -91,7 +93,6 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
   constexpr int QLD = D + 8;                         // 16 rows' 16-byte reads hit distinct banks
   constexpr int QCH = D / 8;
   constexpr int QPT = (ROWS * QCH + 64 * NW - 1) / (64 * NW);
-  constexpr uint32_t ALL = NE == 16 ? 0xffffu : 0xffu;
   __shared__ float s_ml[NW][2][ROWS];
   __shared__ __attribute__((aligned(16))) float s_o[NW][MR][D + 4];
   __shared__ __attribute__((aligned(16))) uint16_t s_q[QREG ? 1 : ROWS][QLD];
@@ -206,13 +207,10 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
     const int kv_hi = cur.kv_hi;
     const Stripe sr = stripe(cur);
     int qpos[QT];                                    // the row's own slot; -1: no such row
-    const uint32_t* words[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const int rl = 16 * qt + l16;
-      const int t = (cur.row0 + (rl < cur.nrows ? rl : 0)) / G;
-      qpos[qt] = rl < cur.nrows ? cur.pos0 + t : -1;
-      if constexpr (TREE) words[qt] = A.mask + (long)(cur.q_start + t) * A.W;
+      qpos[qt] = rl < cur.nrows ? cur.pos0 + (cur.row0 + rl) / G : -1;
     }
     // slots that every row of the item reads
     const int full_lim = min(kv_hi - 1, TREE ? cur.pos0 - 1 : cur.pos0 + cur.row0 / G);
@@ -225,35 +223,55 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
 #pragma unroll
       for (int c = 0; c < CT; ++c) oacc[qt][c] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    for (int sb = first_step(cur); sb < kv_hi; sb += STRIDE) {
-      const int sn = sb + STRIDE;
-      const bool full = sb + STEP - 1 <= full_lim;   // wave-uniform
-      uint32_t allow[QT];                            // bit e: the row reads slot sb + NE lg + e
+    // bit e: row l16 of tile qt reads slot s0 + e
+    auto allow = [&](int qt, int s0) {
+      const int n = min(kv_hi - 1, qpos[qt]) - s0 + 1;
+      uint32_t bits = n >= 8 ? 0xffu : n <= 0 ? 0u : (1u << n) - 1u;
+      if constexpr (TREE) {
+        const int t = max(qpos[qt] - cur.pos0, 0);
+        bits &= mask_window(A.mask + (long)(cur.q_start + t) * A.W, A.W, s0 - cur.pos0);
+      }
+      return bits;
+    };
+    // One step over NQ tiles: 32 slots (8 per lane group) at a time.  FULL: every row reads all of them.
+    auto step = [&](auto nq_, auto full_, int sb) {
+      constexpr int NQ = decltype(nq_)::value;
+      constexpr bool FULL = decltype(full_)::value;
+      // In a step that some row does not read whole, a slot whose V holds an infinity or NaN must not reach the rows
+      // that do not read it (0 x NaN): the values past the item and the non-finite ones are cleared here, and the rows
+      // that do read such a value get it after the products (below).
+      bool odd = false;
+      if constexpr (!FULL) {
+        constexpr int PER = 2 * HV;                  // slots of a dword
+        const int nk = kv_hi - (sb + 8 * HV * lg);   // slots of this lane that the item covers
+        uint32_t any = 0;
 #pragma unroll
-      for (int qt = 0; qt < QT; ++qt) allow[qt] = ALL;
-      if (!full) {
-        const int s0 = sb + NE * lg;
+        for (int w = 0; w < 4; ++w) {
+          const int m = nk - PER * w;
+          const uint32_t keep = m >= PER ? 0xffffffffu : m <= 0 ? 0u : (1u << (32 / PER * m)) - 1u;
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-          if (qt < nq) {
-            const int n = min(kv_hi - 1, qpos[qt]) - s0 + 1;
-            allow[qt] = n >= NE ? ALL : n <= 0 ? 0u : (1u << n) - 1u;
-            if constexpr (TREE) allow[qt] &= mask_window(words[qt], A.W, s0 - cur.pos0);
+          for (int c = 0; c < CT; ++c) {
+            const uint32_t x = (uint32_t)vr[c][w] & keep;
+            const uint32_t nf = KV8 ? ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u
+                                    : ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;  // the top bits of its slots
+            vr[c][w] = (int)(x & ~((nf - (nf >> (KV8 ? 7 : 15))) | nf));
+            any |= nf;
           }
         }
+        odd = __builtin_amdgcn_ballot_w64(any != 0u) != 0ull;
       }
-      // S^T = K Q^T, two 16-position tiles at a time
-      lsk_f32x4 sacc[QT][NA];
 #pragma unroll
-      for (int a0 = 0; a0 < NA; a0 += 2) {
+      for (int hv = 0; hv < HV; ++hv) {
+        const int s0 = sb + 8 * HV * lg + 8 * hv;    // this lane group's 8 slots
+        ORDER();
         lsk_bf16x8 kf[2][KF];
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
           if constexpr (KV8) {
-            const float sc = exp_bits(((uint32_t)ksr[a0 + a] >> (8 * (l16 & 3))) & 255u);
+            const float sc = exp_bits(((uint32_t)ksr[2 * hv + a] >> (8 * (l16 & 3))) & 255u);
 #pragma unroll
             for (int f = 0; f < KF; ++f) {
-              const lsk_i32x4 x = kr[(a0 + a) * (KF / 2) + (f >> 1)];
+              const lsk_i32x4 x = kr[(2 * hv + a) * (KF / 2) + (f >> 1)];
               kf[a][f] = codes_to_bf16(x[2 * (f & 1)], x[2 * (f & 1) + 1], sc);
             }
           } else {
@@ -261,35 +279,33 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
             for (int f = 0; f < KF; ++f) kf[a][f] = __builtin_bit_cast(lsk_bf16x8, kr[a * KF + f]);
           }
         }
+        lsk_bf16x8 pb[NQ];
+        float alpha[NQ];
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-          if (qt < nq) {
-            lsk_bf16x8 qf[KF];
+        for (int qt = 0; qt < NQ; ++qt) {
+          ORDER();
+          // S^T = K Q^T: sacc[a][e] <-> slot s0 + 4 a + e
+          lsk_f32x4 sacc[2];
+          lsk_bf16x8 qf[KF];
+#pragma unroll
+          for (int f = 0; f < KF; ++f)
+            qf[f] = QREG ? qreg[f] : *(const lsk_bf16x8*)(&s_q[16 * qt + l16][q_dim(f)]);
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            sacc[a] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int f = 0; f < KF; ++f)
-              qf[f] = QREG ? qreg[f] : *(const lsk_bf16x8*)(&s_q[16 * qt + l16][q_dim(f)]);
-#pragma unroll
-            for (int a = 0; a < 2; ++a) {
-              lsk_f32x4 acc = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int f = 0; f < KF; ++f) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a][f], qf[f], acc, 0, 0, 0);
-              sacc[qt][a0 + a] = acc;
-            }
+              sacc[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a][f], qf[f], sacc[a], 0, 0, 0);
           }
-        }
-      }
-      // the online softmax of each tile's 16 query columns; sacc[qt][a][e] <-> slot sb + NE lg + 4 a + e
-      lsk_bf16x8 pb[QT][HV];
-      float alpha[QT];
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt) {
-        if (qt < nq) {
-          float sv[NE];
+          uint32_t reads = 0xffu;
+          if constexpr (!FULL) reads = allow(qt, s0);
+          // the online softmax of the tile's 16 query columns
+          float sv[8];
           float mt = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < NE; ++i) {
-            float sc = sacc[qt][i >> 2][i & 3] * A.scale_log2;
-            if (!full) sc = (allow[qt] >> i) & 1u ? sc : -INFINITY;
+          for (int i = 0; i < 8; ++i) {
+            float sc = sacc[i >> 2][i & 3] * A.scale_log2;
+            if constexpr (!FULL) sc = (reads >> i) & 1u ? sc : -INFINITY;
             sv[i] = sc;
             mt = fmaxf(mt, sc);
           }
@@ -298,102 +314,95 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
           alpha[qt] = (m_new == m_run[qt]) ? 1.f : fast_exp2(m_run[qt] - m_new);
           float rs = 0.f;
 #pragma unroll
-          for (int i = 0; i < NE; ++i) {
+          for (int i = 0; i < 8; ++i) {
             const float pe = (sv[i] == -INFINITY) ? 0.f : fast_exp2(sv[i] - m_new);
             rs += pe;
             float pv = pe;
             if constexpr (KV8) {
-              pv = pe * exp_bits(((uint32_t)vsr[i >> 2] >> (8 * (i & 3))) & 255u);
-              if (!full) pv = (allow[qt] >> i) & 1u ? pv : 0.f;  // (a slot never written may hold any exponent)
+              pv = pe * exp_bits(((uint32_t)vsr[2 * hv + (i >> 2)] >> (8 * (i & 3))) & 255u);
+              if constexpr (!FULL) pv = (reads >> i) & 1u ? pv : 0.f;  // (a slot never written: any exponent)
             }
-            pb[qt][i >> 3][i & 7] = static_cast<__bf16>(pv);
+            pb[qt][i] = static_cast<__bf16>(pv);
           }
           rs = rows_sum(rs);
           l_run[qt] = l_run[qt] * alpha[qt] + rs;
           m_run[qt] = m_new;
         }
-      }
-      load_k(sr, sn);
-      // In a step that some row does not read whole, a slot whose V holds an infinity or NaN must not reach the rows
-      // that do not read it (0 x NaN): slots past the item are cleared, and where a non-finite value remains the
-      // operands are split into their finite part and a count of the non-finite values that each row reads.
-      bool odd = false;
-      if (!full) {
-        const int nk = kv_hi - (sb + NE * lg);       // slots of this lane that the item covers
-        uint32_t any = 0;
+        ORDER();
+        if (hv == HV - 1) load_k(sr, sb + STRIDE);   // the next step's K streams in during this step's P V
+        // O^T = alpha O^T + V^T P^T
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int m = nk - (NE / 4) * w;           // of the NE / 4 slots of dword w
-          const uint32_t keep = m >= NE / 4 ? 0xffffffffu : m <= 0 ? 0u : (1u << (128 / NE * m)) - 1u;
+        for (int c = 0; c < CT; ++c) {
+          if (c % 2 == 0) ORDER();
+          lsk_bf16x8 vf;
+          if constexpr (KV8) vf = codes_to_bf16(vr[c][2 * hv], vr[c][2 * hv + 1], 1.f);
+          else vf = __builtin_bit_cast(lsk_bf16x8, vr[c]);
 #pragma unroll
-          for (int c = 0; c < CT; ++c) {
-            const uint32_t x = (uint32_t)vr[c][w] & keep;
-            vr[c][w] = (int)x;
-            any |= KV8 ? ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u
-                       : ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-          }
-        }
-        odd = __builtin_amdgcn_ballot_w64(any != 0u) != 0ull;
-      }
-      auto v_op = [&](int c, int hv) {
-        if constexpr (KV8) return codes_to_bf16(vr[c][2 * hv], vr[c][2 * hv + 1], 1.f);
-        else return __builtin_bit_cast(lsk_bf16x8, vr[c]);
-      };
-      // O^T = alpha O^T + V^T P^T
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt)
-        if (qt < nq)
-#pragma unroll
-          for (int c = 0; c < CT; ++c)
+          for (int qt = 0; qt < NQ; ++qt) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) oacc[qt][c][i] *= alpha[qt];
-      if (!odd) {
-#pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-          for (int hv = 0; hv < HV; ++hv) {
-            const lsk_bf16x8 vf = v_op(c, hv);
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-              if (qt < nq) oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pb[qt][hv], oacc[qt][c], 0, 0, 0);
+            oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pb[qt], oacc[qt][c], 0, 0, 0);
           }
-      } else {
-#pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
+        }
+      }
+      if constexpr (!FULL) {
+        if (odd) {
+          // V again, as a count of its non-finite values (cnt) and their kind (sgn: +-1 for +-inf, 2^20 for NaN): of
+          // those that a row reads, one kind of infinity gives that infinity, anything else NaN.
           for (int hv = 0; hv < HV; ++hv) {
-            typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-            const lsk_bf16x8 vf = v_op(c, hv);
-            const u16x8 bits = __builtin_bit_cast(u16x8, vf);
-            lsk_bf16x8 fin, cnt, sgn;                // finite part; 1 where not finite; +-1: +-inf, 2^20: NaN
+            const int s0 = sb + 8 * HV * lg + 8 * hv;
+            lsk_bf16x8 rd[NQ];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const uint16_t u = bits[e];
-              const bool nf = (u & 0x7f80u) == 0x7f80u, nan = nf && (u & 0x7fu);
-              fin[e] = nf ? static_cast<__bf16>(0.f) : vf[e];
-              cnt[e] = static_cast<__bf16>(nf ? 1.f : 0.f);
-              sgn[e] = static_cast<__bf16>(!nf ? 0.f : nan ? 1048576.f : (u >> 15) ? -1.f : 1.f);
+            for (int qt = 0; qt < NQ; ++qt) {
+              const uint32_t reads = allow(qt, s0);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) rd[qt][e] = static_cast<__bf16>((float)((reads >> e) & 1u));
             }
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-              if (qt < nq) {
-                lsk_bf16x8 rd;
+            for (int c = 0; c < CT; ++c) {
+              const lsk_i32x4 x = ld(sr.v, v_vo, sb / STEP * 64 * D + c * 1024);
+              lsk_bf16x8 cnt, sgn;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) rd[e] = static_cast<__bf16>((float)((allow[qt] >> (8 * hv + e)) & 1u));
+              for (int e = 0; e < 8; ++e) {
+                bool nf, nan, neg;
+                if constexpr (KV8) {
+                  const uint32_t u = (uint32_t)(hv ? x[2 + e / 4] : x[e / 4]) >> (8 * (e & 3));
+                  nf = nan = (u & 0x7fu) == 0x7fu;
+                  neg = false;
+                } else {
+                  const uint32_t u = (uint32_t)x[e / 2] >> (16 * (e & 1));
+                  nf = (u & 0x7f80u) == 0x7f80u;
+                  nan = nf && (u & 0x7fu) != 0u;
+                  neg = (u & 0x8000u) != 0u;
+                }
+                cnt[e] = static_cast<__bf16>(nf ? 1.f : 0.f);
+                sgn[e] = static_cast<__bf16>(!nf ? 0.f : nan ? 1048576.f : neg ? -1.f : 1.f);
+              }
+#pragma unroll
+              for (int qt = 0; qt < NQ; ++qt) {
                 const lsk_f32x4 z = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
-                const lsk_f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cnt, rd, z, 0, 0, 0);
-                const lsk_f32x4 s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sgn, rd, z, 0, 0, 0);
-                oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fin, pb[qt][hv], oacc[qt][c], 0, 0, 0);
+                const lsk_f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cnt, rd[qt], z, 0, 0, 0);
+                const lsk_f32x4 s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sgn, rd[qt], z, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   const float add = s[i] == n[i] ? INFINITY : s[i] == -n[i] ? -INFINITY : __builtin_nanf("");
-                  if (n[i] > 0.f) oacc[qt][c][i] += add;
+                  oacc[qt][c][i] = n[i] > 0.f ? oacc[qt][c][i] + add : oacc[qt][c][i];
                 }
               }
+            }
           }
+        }
       }
-      load_v(sr, sn);
-    }
+      load_v(sr, sb + STRIDE);
+    };
+    auto steps = [&](auto nq_) {
+      int sb = first_step(cur);
+      for (; sb + STEP - 1 <= full_lim; sb += STRIDE) step(nq_, std::true_type{}, sb);
+      for (; sb < kv_hi; sb += STRIDE) step(nq_, std::false_type{}, sb);
+    };
+    if (QT == 1 || nq == 1) steps(std::integral_constant<int, 1>{});
+    else if (QT == 2 || nq == 2) steps(std::integral_constant<int, (QT < 2 ? QT : 2)>{});
+    else steps(std::integral_constant<int, QT>{});
     // the next item's Q and first K / V loads fly while this item is merged
     const Item done = cur;
     cur = nxt;
@@ -628,6 +637,8 @@ static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t
               "%s: max_seq %d (a multiple of %d, stripes below 2 GiB)", what, a.S, ATTN_TILE);
   LSK_REQUIRE(aligned16(a.kc) && aligned16(a.vc) && (!kv8 || (aligned16(a.ks) && aligned16(a.vs))), LSK_EARG,
               "%s: the cache tensors start at multiples of 16 bytes", what);
+  LSK_REQUIRE(head_dim == 64 || rows_cap <= 32, LSK_EUNSUPPORTED, "%s: rows_cap %d (head_dim 128: 16 or 32)", what,
+              rows_cap);
   if (n_parts > 0) {
     const size_t need = lsk_attn_workspace_bytes(n_parts, a.Hkv, head_dim);
     LSK_REQUIRE(workspace != nullptr && aligned16(workspace) && ws_bytes >= need && groups != nullptr && blocks != nullptr,
@@ -639,15 +650,17 @@ static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t
   a.scale_log2 = scale * 1.4426950408889634f;
 #define LSK_CACHE_ATTN(DD, QT, K8, TR) \
   cache_attn_kernel<DD, QT, K8, TR><<<n_slots, 64 * ATTN_WAVES, 0, s>>>(a)
-#define LSK_CACHE_ATTN_QT(DD, K8, TR) \
-  do { if (rows_cap == 16) LSK_CACHE_ATTN(DD, 1, K8, TR); else LSK_CACHE_ATTN(DD, ATTN_QT, K8, TR); } while (0)
-#define LSK_CACHE_ATTN_D(K8, TR) \
-  do { if (head_dim == 128) LSK_CACHE_ATTN_QT(128, K8, TR); else LSK_CACHE_ATTN_QT(64, K8, TR); } while (0)
+#define LSK_CACHE_ATTN_D(K8, TR)                                                            \
+  do {                                                                                      \
+    if (head_dim == 128 && rows_cap == 16) LSK_CACHE_ATTN(128, 1, K8, TR);                  \
+    else if (head_dim == 128) LSK_CACHE_ATTN(128, 2, K8, TR);                               \
+    else if (rows_cap == 16) LSK_CACHE_ATTN(64, 1, K8, TR);                                 \
+    else LSK_CACHE_ATTN(64, ATTN_QT, K8, TR);                                               \
+  } while (0)
   if (!kv8) LSK_CACHE_ATTN_D(false, true);
   else if (a.mask != nullptr) LSK_CACHE_ATTN_D(true, true);
   else LSK_CACHE_ATTN_D(true, false);
 #undef LSK_CACHE_ATTN_D
-#undef LSK_CACHE_ATTN_QT
 #undef LSK_CACHE_ATTN
   int rc = lsk_check_launch(what);
   if (rc || n_groups == 0) return rc;

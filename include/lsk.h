@@ -304,8 +304,8 @@ int lsk_kv8_read(int dtype, const void* k8, const void* v8, const void* k_exp, c
  * mask (uint32 [n_tokens][mask_words]), of the block's own slots only those whose bit is set: bit j % 32 of word j / 32
  * for node j; bits of later nodes and bits past the words count as 0.  A row that reads nothing gives zeros.  Values in
  * slots that a row does not read never reach it, whatever they are.
- * The plan (blocks .. rows_cap) is lsk_attn_plan's and lsk_attn_schedule's, as for lsk_ragged_attn; fp32 plans are
- * unsplit.  workspace >= lsk_attn_workspace_bytes(n_parts, n_kv_heads, head_dim), 16-byte aligned, and a call's own.
+ * The plan (blocks .. rows_cap) is lsk_attn_plan's and lsk_attn_schedule's, as for lsk_ragged_attn, with rows_cap 16 or
+ * 32 where head_dim is 128 (not fp32); fp32 plans are unsplit.  workspace >= lsk_attn_workspace_bytes(n_parts, n_kv_heads, head_dim), 16-byte aligned, and a call's own.
  * head_dim 64 or 128 (fp32 also 16 and 32).  A row's result depends on its own block only; over a bf16 or fp32 cache a
  * chain (every ancestor's bit set) gives lsk_ragged_attn's bits.
  * Beside lsk_ragged_attn (solutions/packed.py:142-166). */

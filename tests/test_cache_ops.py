@@ -431,7 +431,7 @@ def test_a_chain_gives_the_ragged_attentions_bits(cuda, dtype, D):
     mask = torch.from_numpy(words_of(sets, 2)).to(cuda)
     for split in (256, 2048):
         p = lsk.AttnPlan(tab, Hq, ks, split=split)
-        want = torch.empty(len(q), Hq * D, dtype=dtype, device=cuda)
+        want = torch.empty(len(q), Hq * D, dtype=dtype, device=cuda)        # (the plan serves both)
         ws = torch.empty(max(p.ws_bytes, 1), dtype=torch.uint8, device=cuda)
         lsk.ragged_attn(q.to(cuda), ks, vs, p.blocks, p.works, p.n_works, p.groups, p.n_groups, p.n_parts, want, Hq,
                         1 / math.sqrt(D), ws, p.recs, p.n_rounds, p.n_slots, p.rows_cap)
@@ -439,12 +439,13 @@ def test_a_chain_gives_the_ragged_attentions_bits(cuda, dtype, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("kind", ["kv8", "kv8 tree", "tree"])
-def test_a_rows_result_depends_on_its_block_only(cuda, kind):
+def test_a_rows_result_depends_on_its_block_only(cuda, kind, D):
     """The same rows alone, in another order, next to others and as single tokens (causal) give the same bits; so do
     other rows-per-item caps."""
     lsk = _lsk()
-    Hq, Hkv, D = 8, 2, 128
+    Hq, Hkv = 8, 2
     blocks = [(0, 37, 9), (3, 500, 30), (1, 0, 3), (2, 900, 60)]
     tab, q, k, v = _attn_inputs(29, (Hq, Hkv, D), blocks)
     _, sets = _tree_blocks(blocks, 7)
@@ -473,7 +474,7 @@ def test_a_rows_result_depends_on_its_block_only(cuda, kind):
 
     whole = [(r, p, t, a) for (a, p, t, r) in tab]
     full, _ = run(whole)
-    for cap in (16, 32, 48):
+    for cap in (16, 32, 48)[:3 if D == 64 else 2]:
         assert torch.equal(run(whole, cap)[0], full)
     for sel in ([whole[1]], [whole[3], whole[0]], whole[::-1]):
         got, idx = run(sel)
@@ -778,7 +779,7 @@ def test_entry_points_refuse_bad_arguments():
     assert r(1, P, P, P, P, P, P, P, P, 0, 2, 64, 3, 128, None) == 0
     ok = [P, 512, 64, P, P, P, P, None, 0, P, 1, None, 0, 0, P, 1, 1, 16, P, 8, 2, 64, 128, 0.125, None, 0, None]
     k8 = lambda **kw: lib.lsk_kv8_attn(*[kw.get(f"a{i}", x) for i, x in enumerate(ok)])  # noqa: E731
-    assert k8(a0=None) == -1 and k8(a5=None) == -1 and k8(a14=None) == -1 and k8(a17=24) == -1 and k8(a7=P) == -1
+    assert k8(a0=None) == -1 and k8(a5=None) == -1 and k8(a14=None) == -1 and k8(a17=24) == -1 and k8(a17=48, a21=128) == -3 and k8(a7=P) == -1
     assert k8(a19=7) == -2 and k8(a22=96) == -2 and k8(a21=32) == -3 and k8(a3=24) == -1 and k8(a1=-1) == -2
     assert k8(a13=3) == -4 and k8(a13=3, a11=P, a24=P, a25=100) == -4          # split partials without their workspace
     assert k8(a22=1 << 25) == -2                                               # a stripe of 2 GiB and more

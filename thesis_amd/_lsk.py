@@ -664,6 +664,8 @@ class AttnPlan:
         b = b.astype(np.int32)
         self.n_slots = cu_count(self.device)
         self.rows_cap = attn_rows_cap(b, group, split, Hkv, D, self.n_slots)
+        if D == 128 and self.dtype != torch.float32:
+            self.rows_cap = min(self.rows_cap, 32)    # two tiles of accumulators are what a wave's registers hold
         works, groups, self.n_parts = attn_plan(b, group, split, self.rows_cap)
         recs, self.n_rounds = attn_schedule(works, Hkv, self.n_slots)
         self.n_works, self.n_groups = len(works), len(groups)
