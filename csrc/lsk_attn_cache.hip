@@ -233,9 +233,9 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
       }
       return bits;
     };
-    // One step over NQ tiles: 32 slots (8 per lane group) at a time.  FULL: every row reads all of them.
-    auto step = [&](auto nq_, auto full_, int sb) {
-      constexpr int NQ = decltype(nq_)::value;
+    // One step: 32 slots (8 per lane group) at a time.  FULL: every row reads all of them.  All QT tiles are computed,
+    // also those without rows (copies of the loop for fewer tiles cost more in registers than they save).
+    auto step = [&](auto full_, int sb) {
       constexpr bool FULL = decltype(full_)::value;
       // In a step that some row does not read whole, a slot whose V holds an infinity or NaN must not reach the rows
       // that do not read it (0 x NaN): the values past the item and the non-finite ones are cleared here, and the rows
@@ -279,10 +279,10 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
             for (int f = 0; f < KF; ++f) kf[a][f] = __builtin_bit_cast(lsk_bf16x8, kr[a * KF + f]);
           }
         }
-        lsk_bf16x8 pb[NQ];
-        float alpha[NQ];
+        lsk_bf16x8 pb[QT];
+        float alpha[QT];
 #pragma unroll
-        for (int qt = 0; qt < NQ; ++qt) {
+        for (int qt = 0; qt < QT; ++qt) {
           ORDER();
           // S^T = K Q^T: sacc[a][e] <-> slot s0 + 4 a + e
           lsk_f32x4 sacc[2];
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
           if constexpr (KV8) vf = codes_to_bf16(vr[c][2 * hv], vr[c][2 * hv + 1], 1.f);
           else vf = __builtin_bit_cast(lsk_bf16x8, vr[c]);
 #pragma unroll
-          for (int qt = 0; qt < NQ; ++qt) {
+          for (int qt = 0; qt < QT; ++qt) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) oacc[qt][c][i] *= alpha[qt];
             oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pb[qt], oacc[qt][c], 0, 0, 0);
@@ -349,40 +349,38 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
         if (odd) {
           // V again, as a count of its non-finite values (cnt) and their kind (sgn: +-1 for +-inf, 2^20 for NaN): of
           // those that a row reads, one kind of infinity gives that infinity, anything else NaN.
-          for (int hv = 0; hv < HV; ++hv) {
-            const int s0 = sb + 8 * HV * lg + 8 * hv;
-            lsk_bf16x8 rd[NQ];
+#pragma unroll 1
+          for (int hv = 0; hv < HV; ++hv)
 #pragma unroll
-            for (int qt = 0; qt < NQ; ++qt) {
-              const uint32_t reads = allow(qt, s0);
+            for (int qt = 0; qt < QT; ++qt) {
+              const uint32_t reads = allow(qt, sb + 8 * HV * lg + 8 * hv);
+              lsk_bf16x8 rd;
 #pragma unroll
-              for (int e = 0; e < 8; ++e) rd[qt][e] = static_cast<__bf16>((float)((reads >> e) & 1u));
-            }
+              for (int e = 0; e < 8; ++e) rd[e] = static_cast<__bf16>((float)((reads >> e) & 1u));
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-              const lsk_i32x4 x = ld(sr.v, v_vo, sb / STEP * 64 * D + c * 1024);
-              lsk_bf16x8 cnt, sgn;
+              for (int c = 0; c < CT; ++c) {
+                ORDER();
+                const lsk_i32x4 x = ld(sr.v, v_vo, sb / STEP * 64 * D + c * 1024);
+                lsk_bf16x8 cnt, sgn;
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                bool nf, nan, neg;
-                if constexpr (KV8) {
-                  const uint32_t u = (uint32_t)(hv ? x[2 + e / 4] : x[e / 4]) >> (8 * (e & 3));
-                  nf = nan = (u & 0x7fu) == 0x7fu;
-                  neg = false;
-                } else {
-                  const uint32_t u = (uint32_t)x[e / 2] >> (16 * (e & 1));
-                  nf = (u & 0x7f80u) == 0x7f80u;
-                  nan = nf && (u & 0x7fu) != 0u;
-                  neg = (u & 0x8000u) != 0u;
+                for (int e = 0; e < 8; ++e) {
+                  bool nf, nan, neg;
+                  if constexpr (KV8) {
+                    const uint32_t u = (uint32_t)(hv ? x[2 + e / 4] : x[e / 4]) >> (8 * (e & 3));
+                    nf = nan = (u & 0x7fu) == 0x7fu;
+                    neg = false;
+                  } else {
+                    const uint32_t u = (uint32_t)x[e / 2] >> (16 * (e & 1));
+                    nf = (u & 0x7f80u) == 0x7f80u;
+                    nan = nf && (u & 0x7fu) != 0u;
+                    neg = (u & 0x8000u) != 0u;
+                  }
+                  cnt[e] = static_cast<__bf16>(nf ? 1.f : 0.f);
+                  sgn[e] = static_cast<__bf16>(!nf ? 0.f : nan ? 1048576.f : neg ? -1.f : 1.f);
                 }
-                cnt[e] = static_cast<__bf16>(nf ? 1.f : 0.f);
-                sgn[e] = static_cast<__bf16>(!nf ? 0.f : nan ? 1048576.f : neg ? -1.f : 1.f);
-              }
-#pragma unroll
-              for (int qt = 0; qt < NQ; ++qt) {
                 const lsk_f32x4 z = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
-                const lsk_f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cnt, rd[qt], z, 0, 0, 0);
-                const lsk_f32x4 s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sgn, rd[qt], z, 0, 0, 0);
+                const lsk_f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cnt, rd, z, 0, 0, 0);
+                const lsk_f32x4 s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sgn, rd, z, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   const float add = s[i] == n[i] ? INFINITY : s[i] == -n[i] ? -INFINITY : __builtin_nanf("");
@@ -390,19 +388,13 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
                 }
               }
             }
-          }
         }
       }
       load_v(sr, sb + STRIDE);
     };
-    auto steps = [&](auto nq_) {
-      int sb = first_step(cur);
-      for (; sb + STEP - 1 <= full_lim; sb += STRIDE) step(nq_, std::true_type{}, sb);
-      for (; sb < kv_hi; sb += STRIDE) step(nq_, std::false_type{}, sb);
-    };
-    if (QT == 1 || nq == 1) steps(std::integral_constant<int, 1>{});
-    else if (QT == 2 || nq == 2) steps(std::integral_constant<int, (QT < 2 ? QT : 2)>{});
-    else steps(std::integral_constant<int, QT>{});
+    int sb = first_step(cur);
+    for (; sb + STEP - 1 <= full_lim; sb += STRIDE) step(std::true_type{}, sb);
+    for (; sb < kv_hi; sb += STRIDE) step(std::false_type{}, sb);
     // the next item's Q and first K / V loads fly while this item is merged
     const Item done = cur;
     cur = nxt;
