@@ -27,7 +27,10 @@
 // The 8 waves of a workgroup take the STEP-position steps of an item round robin and are merged in wave order through
 // LDS.  Which wave takes a step and every order of additions depend on absolute positions only: a row's result never
 // depends on what else is in the launch, and a chain over a bf16 cache gives the ragged attention's bits.
+#include <algorithm>
 #include <type_traits>
+#include <utility>
+#include <vector>
 
 #include "lsk_attn.h"
 #include "../include/lsk.h"
@@ -46,8 +49,9 @@ struct CacheAttnArgs {
   const int32_t* recs;
   int n_rounds;
   uint16_t* out;          // [N, Hq * D]
-  float* o_part;
+  float* o_part;          // split partials: [part][Hkv][part_rows][D], and (m, l) of each
   float* ml_part;
+  int part_rows;
   int G, Hkv, S;
   float scale_log2;
 };
@@ -86,16 +90,23 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
   constexpr int KF = D / 32;                         // K operands per 16-position tile
   constexpr int CT = D / 16;                         // 16-byte loads per lane of a step, for K and for V
   constexpr int NW = ATTN_WAVES;
-  constexpr int ROWS = 16 * QT;
-  constexpr bool QREG = QT == 1;                     // one tile: Q fragments in registers
+  constexpr int GR = 16 * QT;                        // rows of a wave
+  constexpr bool QREG = QT == 1;                     // one tile: Q fragments in registers (items of one row group)
   constexpr int MT = QT < ATTN_MERGE_TILES ? QT : ATTN_MERGE_TILES;
-  constexpr int MR = 16 * MT;
+  constexpr int MR = 16 * MT;                        // rows of a wave merged per pass
+  constexpr int QROWS = QREG ? 0 : TREE ? NW * GR : GR;  // rows of an item at most
   constexpr int QLD = D + 8;                         // 16 rows' 16-byte reads hit distinct banks
   constexpr int QCH = D / 8;
-  constexpr int QPT = (ROWS * QCH + 64 * NW - 1) / (64 * NW);
-  __shared__ float s_ml[NW][2][ROWS];
-  __shared__ __attribute__((aligned(16))) float s_o[NW][MR][D + 4];
-  __shared__ __attribute__((aligned(16))) uint16_t s_q[QREG ? 1 : ROWS][QLD];
+  constexpr int QPT = QREG ? 1 : (QROWS * QCH + 64 * NW - 1) / (64 * NW);
+  // Q of the next item waits in registers during the merge, where they hold it (a tree's items, of up to 256 rows, are
+  // few per workgroup: theirs is fetched after it)
+  constexpr bool QAHEAD = !TREE;
+  constexpr int O_BYTES = NW * MR * (D + 4) * 4, Q_BYTES = QROWS * QLD * 2;
+  // Q is in LDS during an item's steps, the waves' partial outputs during its merge: one buffer holds both in turn
+  __shared__ __attribute__((aligned(16))) char s_buf[O_BYTES > Q_BYTES ? O_BYTES : Q_BYTES];
+  __shared__ float s_ml[NW][2][GR];
+  float (*s_o)[MR][D + 4] = (float (*)[MR][D + 4])s_buf;
+  uint16_t (*s_q)[QLD] = (uint16_t (*)[QLD])s_buf;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -103,8 +114,9 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
   const int G = A.G, Hkv = A.Hkv, S = A.S, Hq = Hkv * G;
   const int32_t* my_recs = A.recs + (long)blockIdx.x * A.n_rounds * 8;
 
+  // lr: log2 of the item's row groups; the waves of a row group share the item's steps
   struct Item {
-    int q_start, row0, nrows, kv_lo, kv_hi, part, pos0, crow, kvh;
+    int q_start, row0, nrows, lr, kv_lo, kv_hi, part, pos0, crow, kvh;
   };
   auto fetch = [&](int r) {
     Item it;
@@ -113,10 +125,11 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
       return it;
     }
     const int32_t* wk = my_recs + (long)r * 8;
-    it.q_start = wk[0]; it.row0 = wk[1]; it.nrows = wk[2] & 255; it.kvh = wk[2] >> 8; it.kv_lo = wk[3];
-    it.kv_hi = wk[4]; it.part = wk[5]; it.pos0 = wk[6]; it.crow = wk[7];
+    it.q_start = wk[0]; it.row0 = wk[1]; it.nrows = wk[2] & 1023; it.lr = (wk[2] >> 10) & 3; it.kvh = wk[2] >> 12;
+    it.kv_lo = wk[3]; it.kv_hi = wk[4]; it.part = wk[5]; it.pos0 = wk[6]; it.crow = wk[7];
     return it;
   };
+  auto row_base = [&](const Item& it) { return TREE ? (wave & ((1 << it.lr) - 1)) * GR : 0; };  // the wave's first row
   // Q: row rl of an item -> 8 elements from d; operand f's k index 8 lg + e stands for d = q_dim(f) + e
   auto q_dim = [&](int f) { return KV8 ? 64 * (f >> 1) + 16 * lg + 8 * (f & 1) : 32 * f + 8 * lg; };
   auto q_ptr = [&](const Item& it, int rl) {
@@ -124,34 +137,41 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
     return A.q + (long)(it.q_start + t) * A.q_st + (long)(it.kvh * G + g) * A.q_sh;
   };
   auto ldq = [&](const uint16_t* p) { return __builtin_bit_cast(lsk_bf16x8, *(const lsk_u32x4_u*)p); };
-  lsk_bf16x8 qst[QPT];
+  lsk_bf16x8 qst[QAHEAD ? QPT : 1];
   lsk_bf16x8 qreg[KF];
+  auto q_chunk = [&](const Item& it, int c) {        // 8 elements of a row, zeros past the rows
+    const int r = c / QCH, c8 = c - r * QCH;
+    return r < it.nrows ? ldq(q_ptr(it, r) + 8 * c8) : (lsk_bf16x8){};
+  };
+  auto q_put = [&](int c, lsk_bf16x8 v) {
+    const int r = c / QCH, c8 = c - r * QCH;
+    if (r < QROWS) *(lsk_bf16x8*)(&s_q[r][8 * c8]) = v;
+  };
   auto q_load = [&](const Item& it) {
     if constexpr (QREG) {
       const bool valid = l16 < it.nrows;
       const uint16_t* p = q_ptr(it, valid ? l16 : 0);
 #pragma unroll
       for (int f = 0; f < KF; ++f) qreg[f] = valid ? ldq(p + q_dim(f)) : (lsk_bf16x8){};
-    } else {
+    } else if constexpr (QAHEAD) {
 #pragma unroll
-      for (int i = 0; i < QPT; ++i) {
-        const int c = tid + i * 64 * NW, r = c / QCH, c8 = c - r * QCH;
-        qst[i] = r < it.nrows ? ldq(q_ptr(it, r) + 8 * c8) : (lsk_bf16x8){};
-      }
+      for (int i = 0; i < QPT; ++i) qst[i] = q_chunk(it, tid + i * 64 * NW);
     }
   };
-  auto q_store = [&]() {
-    if constexpr (!QREG) {
+  auto q_store = [&](const Item& it) {
+    if constexpr (!QREG && QAHEAD) {
 #pragma unroll
-      for (int i = 0; i < QPT; ++i) {
-        const int c = tid + i * 64 * NW, r = c / QCH, c8 = c - r * QCH;
-        if (r < ROWS) *(lsk_bf16x8*)(&s_q[r][8 * c8]) = qst[i];
-      }
+      for (int i = 0; i < QPT; ++i) q_put(tid + i * 64 * NW, qst[i]);
+    } else if constexpr (!QREG) {
+      int t0 = tid;
+      asm volatile("" : "+v"(t0));                   // (the chunks' offsets are not kept across the items: they spilled)
+#pragma unroll
+      for (int i = 0; i < QPT; ++i) q_put(t0 + i * 64 * NW, q_chunk(it, t0 + i * 64 * NW));
     }
   };
   // K / V through buffer loads over the item's (row, KV head) stripe, whose range ends with the block that holds the
   // item's last position: loads past it give zeros without touching memory, so the next step's are unconditional
-  // (under a branch the compiler would wait for them early).  Non-temporal: read once per launch.
+  // (under a branch the compiler would wait for them early).  Non-temporal where each byte is read once per launch.
   struct Stripe {
     __amdgpu_buffer_rsrc_t k, v, ks, vs;
   };
@@ -171,10 +191,9 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
     return s;
   };
   auto ld = [&](__amdgpu_buffer_rsrc_t rs, int vo, int so) -> lsk_i32x4 {
-    return __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, vo, so, 2));
+    return __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, vo, so, TREE ? 0 : 2));
   };
   const int k_vo = 16 * lane, v_vo = 64 * l16 + 16 * lg;
-  constexpr int STRIDE = STEP * NW;
   lsk_i32x4 kr[CT], vr[CT], ksr, vsr;                // this step's K and V as loaded
   auto load_k = [&](const Stripe& s, int sb) {
 #pragma unroll
@@ -186,7 +205,10 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
     for (int c = 0; c < CT; ++c) vr[c] = ld(s.v, v_vo, sb / STEP * 64 * D + c * 1024);
     if constexpr (KV8) vsr = ld(s.vs, 16 * lg, sb);
   };
-  auto first_step = [&](const Item& it) { return it.kv_lo + STEP * wave; };
+  // a wave without rows starts past the stripe
+  auto first_step = [&](const Item& it) {
+    return row_base(it) < it.nrows ? it.kv_lo + STEP * (TREE ? wave >> it.lr : wave) : S;
+  };
   auto issue_first = [&](const Item& it) {
     q_load(it);
     const Stripe s = stripe(it);
@@ -199,17 +221,17 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
   issue_first(cur);
   Item nxt = fetch(1);
   if constexpr (!QREG) {
-    q_store();
+    q_store(cur);
     __syncthreads();
   }
   for (int r = 0; cur.nrows > 0; ++r) {
-    const int nq = (cur.nrows + 15) >> 4;
-    const int kv_hi = cur.kv_hi;
+    const int kv_hi = cur.kv_hi, rb = row_base(cur);
+    const int stride = STEP * (TREE ? NW >> cur.lr : NW);
     const Stripe sr = stripe(cur);
     int qpos[QT];                                    // the row's own slot; -1: no such row
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      const int rl = 16 * qt + l16;
+      const int rl = rb + 16 * qt + l16;
       qpos[qt] = rl < cur.nrows ? cur.pos0 + (cur.row0 + rl) / G : -1;
     }
     // slots that every row of the item reads
@@ -289,7 +311,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
           lsk_bf16x8 qf[KF];
 #pragma unroll
           for (int f = 0; f < KF; ++f)
-            qf[f] = QREG ? qreg[f] : *(const lsk_bf16x8*)(&s_q[16 * qt + l16][q_dim(f)]);
+            qf[f] = QREG ? qreg[f] : *(const lsk_bf16x8*)(&s_q[rb + 16 * qt + l16][q_dim(f)]);
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
             sacc[a] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
@@ -329,7 +351,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
           m_run[qt] = m_new;
         }
         ORDER();
-        if (hv == HV - 1) load_k(sr, sb + STRIDE);   // the next step's K streams in during this step's P V
+        if (hv == HV - 1) load_k(sr, sb + stride);   // the next step's K streams in during this step's P V
         // O^T = alpha O^T + V^T P^T
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
@@ -390,11 +412,11 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
             }
         }
       }
-      load_v(sr, sb + STRIDE);
+      load_v(sr, sb + stride);
     };
     int sb = first_step(cur);
-    for (; sb + STEP - 1 <= full_lim; sb += STRIDE) step(std::true_type{}, sb);
-    for (; sb < kv_hi; sb += STRIDE) step(std::false_type{}, sb);
+    for (; sb + STEP - 1 <= full_lim; sb += stride) step(std::true_type{}, sb);
+    for (; sb < kv_hi; sb += stride) step(std::false_type{}, sb);
     // the next item's Q and first K / V loads fly while this item is merged
     const Item done = cur;
     cur = nxt;
@@ -402,35 +424,35 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
       issue_first(cur);
       nxt = fetch(r + 2);
     }
-    // merge the waves in order: M = max m_w, e_w = exp2(m_w - M), L = sum e_w l_w, O = sum e_w O_w
+    // merge a row group's waves in order: M = max m_w, e_w = exp2(m_w - M), L = sum e_w l_w, O = sum e_w O_w
+    const int nr = 1 << done.lr, ranks = NW >> done.lr;
+    if (!QREG) __syncthreads();                      // every wave is past its reads of Q
 #pragma unroll
     for (int p0 = 0; p0 < QT; p0 += MT) {
-      if (p0 >= nq) break;
+      if (16 * p0 >= done.nrows) break;
 #pragma unroll
       for (int qt = p0; qt < p0 + MT && qt < QT; ++qt) {
-        if (qt < nq) {
-          if (lg == 0) {
-            s_ml[wave][0][16 * qt + l16] = m_run[qt];
-            s_ml[wave][1][16 * qt + l16] = l_run[qt];
-          }
-#pragma unroll
-          for (int c = 0; c < CT; ++c)
-            *(float4*)(&s_o[wave][16 * (qt - p0) + l16][16 * c + 4 * lg]) =
-                make_float4(oacc[qt][c][0], oacc[qt][c][1], oacc[qt][c][2], oacc[qt][c][3]);
+        if (lg == 0) {
+          s_ml[wave][0][16 * qt + l16] = m_run[qt];
+          s_ml[wave][1][16 * qt + l16] = l_run[qt];
         }
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+          *(float4*)(&s_o[wave][16 * (qt - p0) + l16][16 * c + 4 * lg]) =
+              make_float4(oacc[qt][c][0], oacc[qt][c][1], oacc[qt][c][2], oacc[qt][c][3]);
       }
       __syncthreads();
-      const int pr = min(done.nrows - 16 * p0, MR);
-      for (int e = tid; e < pr * (D / 4); e += 64 * NW) {
-        const int ql = e / (D / 4), d = 4 * (e - ql * (D / 4));
-        const int qr = 16 * p0 + ql;
+      for (int e = tid; e < nr * MR * (D / 4); e += 64 * NW) {
+        const int x = e / (D / 4), d = 4 * (e - x * (D / 4));
+        const int rg = x / MR, ql = x - rg * MR, qr = 16 * p0 + ql;  // row group, row of the pass, row of the group
+        const int row = rg * GR + qr;                                // row of the item
+        if (qr >= GR || row >= done.nrows) continue;
         float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, s_ml[w][0][qr]);
+        for (int k = 0; k < ranks; ++k) M = fmaxf(M, s_ml[(k << done.lr) + rg][0][qr]);
         float L = 0.f;
         float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
+        for (int k = 0; k < ranks; ++k) {
+          const int w = (k << done.lr) + rg;
           const float mw = s_ml[w][0][qr];
           const float ew = (mw == -INFINITY) ? 0.f : ((mw == M) ? 1.f : fast_exp2(mw - M));
           L = L + ew * s_ml[w][1][qr];
@@ -440,7 +462,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
           O.z = O.z + ew * ow.z;
           O.w = O.w + ew * ow.w;
         }
-        const int rr = done.row0 + qr;
+        const int rr = done.row0 + row;
         const int tt = rr / G, gg = rr - tt * G;
         if (done.part < 0) {
           if (TREE && L == 0.f) L = 1.f;             // nothing read: O is 0
@@ -449,7 +471,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
           pk[1] = (uint32_t)f2bf(O.z / L) | ((uint32_t)f2bf(O.w / L) << 16);
           *(lsk_u32x2_u*)(A.out + ((long)(done.q_start + tt) * Hq + done.kvh * G + gg) * D + d) = pk;
         } else {
-          const long slot = ((long)done.part * Hkv + done.kvh) * ATTN_ROWS + qr;
+          const long slot = ((long)done.part * Hkv + done.kvh) * A.part_rows + row;
           *(float4*)(A.o_part + slot * D + d) = O;
           if (d == 0) {
             A.ml_part[slot * 2 + 0] = M;
@@ -457,59 +479,71 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
           }
         }
       }
-      if (p0 == 0 && cur.nrows > 0) q_store();
+      __syncthreads();
+    }
+    if (!QREG && cur.nrows > 0) {
+      q_store(cur);
       __syncthreads();
     }
   }
 }
 
-// Merge the splits of one query group in split order: M = max_s m_s, w_s = exp2(m_s - M), out = sum w_s O_s / sum w_s l_s
-// (zeros where no split read anything).
+// Merge the splits of a row in split order: M = max_s m_s, w_s = exp2(m_s - M), out = sum w_s O_s / sum w_s l_s (zeros
+// where no split read anything).  A wave per row: the lanes take the splits' statistics side by side, then each its dims
+// of the partial outputs, 16 splits' loads in flight.  (One workgroup per group of rows with a split after the other:
+// 25 us more for 5 tokens over 100000 positions in 98 splits.)
 template <int D>
-__global__ __launch_bounds__(256) void cache_combine_kernel(const int32_t* __restrict__ blocks,
-                                                            const int32_t* __restrict__ groups,
+__global__ __launch_bounds__(256) void cache_combine_kernel(const int32_t* __restrict__ groups,
                                                             const float* __restrict__ o_part,
                                                             const float* __restrict__ ml_part,
-                                                            uint16_t* __restrict__ out, int G, int Hkv) {
-  __shared__ float s_w[ATTN_ROWS][ATTN_MAX_SPLITS];
-  __shared__ float s_L[ATTN_ROWS];
+                                                            uint16_t* __restrict__ out, int G, int Hkv, int part_rows) {
+  constexpr int PER = D / 64, AHEAD = 16;
+  __shared__ float s_w[4][ATTN_MAX_SPLITS], s_l[4][ATTN_MAX_SPLITS];
   const int32_t* gp = groups + (long)blockIdx.x * 8;
-  const int blk = gp[0], row0 = gp[1], nrows = gp[2], pf = gp[3], ns = gp[4];
-  const int kvh = blockIdx.y;
-  const int q_start = blocks[(long)blk * 4 + 0];
-  const int tid = threadIdx.x;
-  if (tid < nrows) {
-    float M = -INFINITY;
-    for (int s = 0; s < ns; ++s) M = fmaxf(M, ml_part[(((long)(pf + s) * Hkv + kvh) * ATTN_ROWS + tid) * 2]);
-    float L = 0.f;
-    for (int s = 0; s < ns; ++s) {
-      const long slot = ((long)(pf + s) * Hkv + kvh) * ATTN_ROWS + tid;
-      const float ms = ml_part[slot * 2], ls = ml_part[slot * 2 + 1];
-      const float w = (ms == -INFINITY) ? 0.f : ((ms == M) ? 1.f : fast_exp2(ms - M));
-      s_w[tid][s] = w;
-      L = L + w * ls;
-    }
-    s_L[tid] = L == 0.f ? 1.f : L;
+  const int q_start = gp[0], row0 = gp[1], nrows = gp[2], pf = gp[3], ns = gp[4];
+  const int kvh = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int rl = blockIdx.z * 4 + wave;
+  if (rl >= nrows) return;                           // (no barrier below: a wave's LDS is its own)
+  const long slot0 = ((long)pf * Hkv + kvh) * part_rows + rl, step = (long)Hkv * part_rows;
+  float m[2], M = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int s = lane + 64 * i;
+    m[i] = s < ns ? ml_part[(slot0 + s * step) * 2] : -INFINITY;
+    M = fmaxf(M, m[i]);
+    if (s < ns) s_l[wave][s] = ml_part[(slot0 + s * step) * 2 + 1];
   }
-  __syncthreads();
-  for (int e = tid; e < nrows * (D / 4); e += 256) {
-    const int rl = e / (D / 4), d = 4 * (e - rl * (D / 4));
-    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < ns; ++s) {
-      const float w = s_w[rl][s];
-      const float4 v = *(const float4*)(o_part + (((long)(pf + s) * Hkv + kvh) * ATTN_ROWS + rl) * D + d);
-      O.x = O.x + w * v.x;
-      O.y = O.y + w * v.y;
-      O.z = O.z + w * v.z;
-      O.w = O.w + w * v.w;
-    }
-    const float L = s_L[rl];
-    const int r = row0 + rl, t = r / G, g = r - t * G;
-    lsk_u32x2_u pk;
-    pk[0] = (uint32_t)f2bf(O.x / L) | ((uint32_t)f2bf(O.y / L) << 16);
-    pk[1] = (uint32_t)f2bf(O.z / L) | ((uint32_t)f2bf(O.w / L) << 16);
-    *(lsk_u32x2_u*)(out + ((long)(q_start + t) * G * Hkv + kvh * G + g) * D + d) = pk;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (lane + 64 * i < ns)
+      s_w[wave][lane + 64 * i] = (m[i] == -INFINITY) ? 0.f : ((m[i] == M) ? 1.f : fast_exp2(m[i] - M));
+  __builtin_amdgcn_wave_barrier();
+  float L = 0.f, O[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) O[i] = 0.f;
+  for (int s0 = 0; s0 < ns; s0 += AHEAD) {
+    float v[AHEAD][PER];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        v[j][i] = s0 + j < ns ? o_part[(slot0 + (s0 + j) * step) * D + lane * PER + i] : 0.f;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (s0 + j < ns) {
+        const float w = s_w[wave][s0 + j];
+        L = L + w * s_l[wave][s0 + j];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) O[i] = O[i] + w * v[j][i];
+      }
   }
+  if (L == 0.f) L = 1.f;
+  const int r = row0 + rl, t = r / G, g = r - t * G;
+  uint16_t* o = out + ((long)(q_start + t) * G * Hkv + kvh * G + g) * D + lane * PER;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) o[i] = f2bf(O[i] / L);
 }
 
 // ----------------------------------------------------------------------------- fp32 trees
@@ -613,111 +647,225 @@ __global__ __launch_bounds__(256) void tree_attn_f32_kernel(const float* __restr
   }
 }
 
-// ----------------------------------------------------------------------------- entry points
+// ----------------------------------------------------------------------------- host planner
 
-#define ATTN_CACHE_ALIGN 16
-
-static bool aligned16(const void* p) { return ((uintptr_t)p & (ATTN_CACHE_ALIGN - 1)) == 0; }
-
-// Checks and launches shared by the two entry points; kv8 = the cache is 8-bit.
-static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t* blocks, int n_works,
-                      const int32_t* groups, int n_groups, int n_parts, int n_slots, int rows_cap, int n_heads,
-                      int head_dim, float scale, void* workspace, size_t ws_bytes, hipStream_t s) {
+// Work items of one launch: 32 rows (token x query head of the group) of a block per wave, 16 where no block has more,
+// 48 for causal launches over 64 dims with larger blocks; the context in splits at absolute multiples of `split`.
+//   causal  an item is one row group: 8 waves share its steps.
+//   tree    a block of more than 32 rows gives an item 2, 4 or 8 row groups (up to 256 rows), whose 8, 4 .. waves each
+//           walk more of the positions: K / V come from memory once for all of them and fewer partial outputs are
+//           merged (32 trees of 45 nodes, 8B heads, 700 positions: one group 83 us, up to eight 29).  row_groups limits
+//           it, for caches of few stripes, whose launches have too few items otherwise.
+// The number of row groups follows from the block's rows and the cache alone, so it never makes a row's result depend on
+// the batch.  Items go longest first to the least-loaded of n_slots persistent workgroups, as in lsk_attn_schedule.
+extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int n_kv_heads, int head_dim,
+                                   int kv8, int tree, int row_groups, int n_slots, int32_t* meta, long meta_cap,
+                                   long* counts) {
+  const char* what = "lsk_cache_attn_plan";
+  LSK_REQUIRE(counts && (blocks || nb == 0), LSK_EARG, "%s: null pointer", what);
+  LSK_REQUIRE(nb >= 0 && group > 0 && split >= ATTN_TILE && split % ATTN_TILE == 0 && n_kv_heads > 0 &&
+                  n_kv_heads < (1 << 19) && n_slots > 0 &&
+                  (row_groups == 1 || row_groups == 2 || row_groups == 4 || row_groups == 8),
+              LSK_ESHAPE, "%s: bad arguments (split a multiple of %d, row_groups 1, 2, 4 or 8)", what, ATTN_TILE);
   LSK_REQUIRE(head_dim == 64 || head_dim == 128, LSK_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128)", what,
               head_dim);
+  const int step = kv8 ? 64 : 32;
+  long most = 0, n_tokens = 0;
+  for (int b = 0; b < nb; ++b) {
+    const long pos0 = blocks[b * 4 + 1], T = blocks[b * 4 + 2];
+    LSK_REQUIRE(T >= 0 && pos0 >= 0 && pos0 + T <= 0x7fffffffL - split && T * group < (1L << 31), LSK_ESHAPE,
+                "%s: block %d has T=%ld pos0=%ld", what, b, T, pos0);
+    LSK_REQUIRE((pos0 + T + split - 1) / split <= ATTN_MAX_SPLITS, LSK_ESHAPE,
+                "%s: block %d needs more than %d splits of %d positions", what, b, ATTN_MAX_SPLITS, split);
+    most = T * group > most ? T * group : most;
+    n_tokens += T;
+  }
+  const int tiles = most <= 16 ? 1 : most <= 32 || tree || head_dim == 128 ? 2 : 3;
+  struct It { int32_t rec[8]; int cost; };
+  thread_local std::vector<It> items;
+  thread_local std::vector<int32_t> groups;
+  items.clear();
+  groups.clear();
+  long np = 0;
+  int part_rows = 16 * tiles, used = 1;
+  for (int b = 0; b < nb; ++b) {
+    const int32_t* bm = blocks + (long)b * 4;
+    const int pos0 = bm[1];
+    const long rows = (long)bm[2] * group;
+    int lr = 0;
+    while (tree && (1 << lr) < row_groups && rows > (32L << lr)) ++lr;
+    used = (1 << lr) > used ? 1 << lr : used;
+    const int cap = (16 * tiles) << lr;
+    for (long row0 = 0; row0 < rows; row0 += cap) {
+      const int nrows = (int)(rows - row0 < cap ? rows - row0 : cap);
+      const int end = (int)(pos0 + (row0 + nrows - 1) / group + 1);
+      const int ns = (end + split - 1) / split;
+      if (ns > 1) {
+        const int32_t g[8] = {bm[0], (int32_t)row0, nrows, (int32_t)np, ns, 0, 0, 0};
+        groups.insert(groups.end(), g, g + 8);
+        part_rows = cap > part_rows ? cap : part_rows;
+      }
+      for (int sp = 0; sp < ns; ++sp) {
+        const int lo = sp * split, hi = lo + split < end ? lo + split : end;
+        // in tenths of a one-tile step: a wave's steps, 1.5 times as long per further tile, and the item's own cost
+        const int steps = (hi - lo + step * (ATTN_WAVES >> lr) - 1) / (step * (ATTN_WAVES >> lr));
+        const int cost = steps * (10 + 5 * (tiles - 1)) + 20 + 6 * (tiles - 1);
+        for (int h = 0; h < n_kv_heads; ++h)
+          items.push_back({{bm[0], (int32_t)row0, nrows | (lr << 10) | (h << 12), lo, hi,
+                            ns > 1 ? (int32_t)(np + sp) : -1, pos0, bm[3]}, cost});
+      }
+      if (ns > 1) np += ns;
+    }
+  }
+  LSK_REQUIRE(np < (1L << 24) && (long)items.size() < (1L << 28), LSK_ESHAPE, "%s: too many work items", what);
+  std::stable_sort(items.begin(), items.end(), [](const It& a, const It& b) { return a.cost > b.cost; });
+  thread_local std::vector<std::pair<long, int>> heap;
+  thread_local std::vector<int> slot_of, rank, count;
+  heap.clear();
+  for (int sl = 0; sl < n_slots; ++sl) heap.push_back({0, sl});
+  const auto later = [](const std::pair<long, int>& a, const std::pair<long, int>& b) { return a > b; };
+  slot_of.resize(items.size());
+  rank.resize(items.size());
+  count.assign(n_slots, 0);
+  int rounds = 0;
+  for (size_t i = 0; i < items.size(); ++i) {
+    std::pop_heap(heap.begin(), heap.end(), later);
+    auto& top = heap.back();
+    slot_of[i] = top.second;
+    rank[i] = count[top.second]++;
+    rounds = count[top.second] > rounds ? count[top.second] : rounds;
+    top.first += items[i].cost;
+    std::push_heap(heap.begin(), heap.end(), later);
+  }
+  const long len = (long)groups.size() + 8L * n_slots * rounds;
+  counts[0] = n_tokens; counts[1] = (long)groups.size() / 8; counts[2] = np; counts[3] = rounds; counts[4] = tiles;
+  counts[5] = part_rows; counts[6] = len; counts[7] = used;
+  if (meta == nullptr) return 0;
+  LSK_REQUIRE(len <= meta_cap, LSK_EWORKSPACE, "%s: %ld metadata words > %ld", what, len, meta_cap);
+  std::copy(groups.begin(), groups.end(), meta);
+  int32_t* recs = meta + groups.size();
+  std::fill(recs, recs + 8L * n_slots * rounds, 0);
+  for (size_t i = 0; i < items.size(); ++i)
+    std::copy(items[i].rec, items[i].rec + 8, recs + ((long)slot_of[i] * rounds + rank[i]) * 8);
+  return 0;
+}
+
+extern "C" size_t lsk_cache_attn_workspace_bytes(int n_parts, int n_kv_heads, int part_rows, int head_dim) {
+  const size_t rows = (size_t)n_parts * n_kv_heads * part_rows;
+  return lsk_align_up(rows * head_dim * sizeof(float), 256) + lsk_align_up(rows * 2 * sizeof(float), 256);
+}
+
+// ----------------------------------------------------------------------------- entry points
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Checks and launches shared by the two entry points; kv8: the cache is 8-bit.
+static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t* groups, int n_groups, int n_parts,
+                      int n_slots, int tiles, int row_groups, int head_dim, float scale, void* workspace, size_t ws_bytes,
+                      hipStream_t s) {
+  LSK_REQUIRE(head_dim == 64 || head_dim == 128, LSK_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128)", what,
+              head_dim);
+  LSK_REQUIRE(tiles == 1 || tiles == 2 || (tiles == 3 && head_dim == 64 && a.mask == nullptr), LSK_EARG,
+              "%s: a plan of %d tiles", what, tiles);
+  LSK_REQUIRE(row_groups == 1 || a.mask != nullptr, LSK_EARG, "%s: a tree's plan (%d row groups) without a mask", what,
+              row_groups);
+  LSK_REQUIRE(n_slots > 0 && n_groups >= 0 && n_parts >= 0 && (n_groups > 0) == (n_parts > 0), LSK_EARG,
+              "%s: a plan of %d slots, %d groups and %d partial slots", what, n_slots, n_groups, n_parts);
   LSK_REQUIRE(a.S % ATTN_TILE == 0 && (long)a.S * head_dim * 2 <= 0x7fffffffL, LSK_ESHAPE,
               "%s: max_seq %d (a multiple of %d, stripes below 2 GiB)", what, a.S, ATTN_TILE);
   LSK_REQUIRE(aligned16(a.kc) && aligned16(a.vc) && (!kv8 || (aligned16(a.ks) && aligned16(a.vs))), LSK_EARG,
               "%s: the cache tensors start at multiples of 16 bytes", what);
-  LSK_REQUIRE(head_dim == 64 || rows_cap <= 32, LSK_EUNSUPPORTED, "%s: rows_cap %d (head_dim 128: 16 or 32)", what,
-              rows_cap);
   if (n_parts > 0) {
-    const size_t need = lsk_attn_workspace_bytes(n_parts, a.Hkv, head_dim);
-    LSK_REQUIRE(workspace != nullptr && aligned16(workspace) && ws_bytes >= need && groups != nullptr && blocks != nullptr,
-                LSK_EWORKSPACE, "%s: an aligned workspace of %zu bytes needed, %zu given", what, need, ws_bytes);
+    LSK_REQUIRE(a.part_rows >= 16 * tiles && a.part_rows <= 128 * tiles, LSK_EARG, "%s: a plan of %d rows per partial",
+                what, a.part_rows);
+    const size_t need = lsk_cache_attn_workspace_bytes(n_parts, a.Hkv, a.part_rows, head_dim);
+    LSK_REQUIRE(workspace != nullptr && aligned16(workspace) && ws_bytes >= need && groups != nullptr, LSK_EWORKSPACE,
+                "%s: an aligned workspace of %zu bytes needed, %zu given", what, need, ws_bytes);
     a.o_part = (float*)workspace;
     a.ml_part = (float*)((char*)workspace +
-                         lsk_align_up((size_t)n_parts * a.Hkv * ATTN_ROWS * head_dim * sizeof(float), 256));
+                         lsk_align_up((size_t)n_parts * a.Hkv * a.part_rows * head_dim * sizeof(float), 256));
   }
   a.scale_log2 = scale * 1.4426950408889634f;
-#define LSK_CACHE_ATTN(DD, QT, K8, TR) \
-  cache_attn_kernel<DD, QT, K8, TR><<<n_slots, 64 * ATTN_WAVES, 0, s>>>(a)
-#define LSK_CACHE_ATTN_D(K8, TR)                                                            \
-  do {                                                                                      \
-    if (head_dim == 128 && rows_cap == 16) LSK_CACHE_ATTN(128, 1, K8, TR);                  \
-    else if (head_dim == 128) LSK_CACHE_ATTN(128, 2, K8, TR);                               \
-    else if (rows_cap == 16) LSK_CACHE_ATTN(64, 1, K8, TR);                                 \
-    else LSK_CACHE_ATTN(64, ATTN_QT, K8, TR);                                               \
+#define LSK_CACHE_ATTN(DD, QT, K8, TR) cache_attn_kernel<DD, QT, K8, TR><<<n_slots, 64 * ATTN_WAVES, 0, s>>>(a)
+#define LSK_CACHE_ATTN_D(K8, TR)                                            \
+  do {                                                                      \
+    if (head_dim == 128 && tiles == 1) LSK_CACHE_ATTN(128, 1, K8, TR);      \
+    else if (head_dim == 128) LSK_CACHE_ATTN(128, 2, K8, TR);               \
+    else if (tiles == 1) LSK_CACHE_ATTN(64, 1, K8, TR);                     \
+    else if (tiles == 2) LSK_CACHE_ATTN(64, 2, K8, TR);                     \
   } while (0)
   if (!kv8) LSK_CACHE_ATTN_D(false, true);
   else if (a.mask != nullptr) LSK_CACHE_ATTN_D(true, true);
+  else if (tiles == 3) LSK_CACHE_ATTN(64, 3, true, false);
   else LSK_CACHE_ATTN_D(true, false);
 #undef LSK_CACHE_ATTN_D
 #undef LSK_CACHE_ATTN
   int rc = lsk_check_launch(what);
   if (rc || n_groups == 0) return rc;
-  const dim3 cg(n_groups, a.Hkv);
+  const dim3 cg(n_groups, a.Hkv, (a.part_rows + 3) / 4);
   if (head_dim == 128)
-    cache_combine_kernel<128><<<cg, 256, 0, s>>>(blocks, groups, a.o_part, a.ml_part, a.out, a.G, a.Hkv);
+    cache_combine_kernel<128><<<cg, 256, 0, s>>>(groups, a.o_part, a.ml_part, a.out, a.G, a.Hkv, a.part_rows);
   else
-    cache_combine_kernel<64><<<cg, 256, 0, s>>>(blocks, groups, a.o_part, a.ml_part, a.out, a.G, a.Hkv);
+    cache_combine_kernel<64><<<cg, 256, 0, s>>>(groups, a.o_part, a.ml_part, a.out, a.G, a.Hkv, a.part_rows);
   return lsk_check_launch(what);
 }
 
-static int plan_args(const char* what, const void* q, const void* kc, const void* vc, const void* out, int n_works,
-                     int n_groups, int n_parts, int rows_cap, int n_heads, int n_kv_heads, int head_dim, int max_seq,
-                     long q_st, long q_sh) {
+static int shape_args(const char* what, const void* q, const void* kc, const void* vc, const void* out, int n_heads,
+                      int n_kv_heads, int head_dim, int max_seq, long q_st, long q_sh) {
   LSK_REQUIRE(q && kc && vc && out, LSK_EARG, "%s: null pointer", what);
-  LSK_REQUIRE(rows_cap > 0 && rows_cap % 16 == 0 && rows_cap <= ATTN_ROWS, LSK_EARG,
-              "%s: rows_cap %d (the plan's rows per item: 16, 32 or %d)", what, rows_cap, ATTN_ROWS);
-  LSK_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && head_dim > 0 && max_seq > 0 &&
-                  n_works >= 0 && n_groups >= 0 && n_parts >= 0 && q_st >= 0 && q_sh >= 0,
+  LSK_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_kv_heads <= 65535 && n_heads % n_kv_heads == 0 && head_dim > 0 &&
+                  max_seq > 0 && q_st >= 0 && q_sh >= 0,
               LSK_ESHAPE, "%s: bad shape", what);
   return 0;
 }
 
 extern "C" int lsk_kv8_attn(const void* q, long q_stride_t, long q_stride_h, const void* k8, const void* v8,
                             const void* k_exp, const void* v_exp, const uint32_t* mask, int mask_words,
-                            const int32_t* blocks, int n_works, const int32_t* groups, int n_groups, int n_parts,
-                            const int32_t* recs, int n_rounds, int n_slots, int rows_cap, void* out, int n_heads,
-                            int n_kv_heads, int head_dim, int max_seq, float scale, void* workspace, size_t ws_bytes,
-                            void* stream) {
+                            const int32_t* groups, int n_groups, int n_parts, const int32_t* recs, int n_rounds,
+                            int n_slots, int tiles, int row_groups, int part_rows, void* out, int n_heads, int n_kv_heads, int head_dim,
+                            int max_seq, float scale, void* workspace, size_t ws_bytes, void* stream) {
   const char* what = "lsk_kv8_attn";
-  if (int rc = plan_args(what, q, k8, v8, out, n_works, n_groups, n_parts, rows_cap, n_heads, n_kv_heads, head_dim,
-                         max_seq, q_stride_t, q_stride_h)) return rc;
-  LSK_REQUIRE(k_exp && v_exp && (mask == nullptr || mask_words > 0), LSK_EARG, "%s: null scales or an empty mask", what);
-  if (n_works == 0) return 0;
-  LSK_REQUIRE(recs && n_rounds > 0 && n_slots > 0, LSK_EARG, "%s: a schedule is needed (lsk_attn_schedule)", what);
-  CacheAttnArgs a = {(const uint16_t*)q, q_stride_t, q_stride_h, k8, v8, (const uint8_t*)k_exp, (const uint8_t*)v_exp,
-                     mask, mask_words, recs, n_rounds, (uint16_t*)out, nullptr, nullptr, n_heads / n_kv_heads, n_kv_heads,
-                     max_seq, 0.f};
-  return cache_attn(what, true, a, blocks, n_works, groups, n_groups, n_parts, n_slots, rows_cap, n_heads, head_dim,
-                    scale, workspace, ws_bytes, (hipStream_t)stream);
+  if (int rc = shape_args(what, q, k8, v8, out, n_heads, n_kv_heads, head_dim, max_seq, q_stride_t, q_stride_h))
+    return rc;
+  LSK_REQUIRE(k_exp && v_exp && (mask == nullptr || mask_words > 0), LSK_EARG, "%s: null scales or an empty mask",
+              what);
+  LSK_REQUIRE(n_rounds >= 0, LSK_EARG, "%s: a plan of %d rounds", what, n_rounds);
+  if (n_rounds == 0) return 0;
+  LSK_REQUIRE(recs != nullptr, LSK_EARG, "%s: null pointer", what);
+  const CacheAttnArgs a = {(const uint16_t*)q, q_stride_t, q_stride_h, k8, v8, (const uint8_t*)k_exp,
+                           (const uint8_t*)v_exp, mask, mask_words, recs, n_rounds, (uint16_t*)out, nullptr, nullptr,
+                           part_rows, n_heads / n_kv_heads, n_kv_heads, max_seq, 0.f};
+  return cache_attn(what, true, a, groups, n_groups, n_parts, n_slots, tiles, row_groups, head_dim, scale, workspace,
+                    ws_bytes, (hipStream_t)stream);
 }
 
 extern "C" int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_stride_h, const void* kcache,
-                             const void* vcache, const uint32_t* mask, int mask_words, const int32_t* blocks,
-                             const int32_t* works, int n_works, const int32_t* groups, int n_groups, int n_parts,
-                             const int32_t* recs, int n_rounds, int n_slots, int rows_cap, void* out, int n_heads,
+                             const void* vcache, const uint32_t* mask, int mask_words, const int32_t* works, int n_works,
+                             int rows_cap, const int32_t* groups, int n_groups, int n_parts, const int32_t* recs,
+                             int n_rounds, int n_slots, int tiles, int row_groups, int part_rows, void* out, int n_heads,
                              int n_kv_heads, int head_dim, int max_seq, float scale, void* workspace, size_t ws_bytes,
                              void* stream) {
   const char* what = "lsk_tree_attn";
-  if (int rc = plan_args(what, q, kcache, vcache, out, n_works, n_groups, n_parts, rows_cap, n_heads, n_kv_heads,
-                         head_dim, max_seq, q_stride_t, q_stride_h)) return rc;
+  if (int rc = shape_args(what, q, kcache, vcache, out, n_heads, n_kv_heads, head_dim, max_seq, q_stride_t,
+                          q_stride_h)) return rc;
   LSK_REQUIRE(mask && mask_words > 0, LSK_EARG, "%s: no mask", what);
   LSK_REQUIRE(dtype == LSK_DTYPE_BF16 || dtype == LSK_DTYPE_F32, LSK_EUNSUPPORTED, "%s: dtype %d", what, dtype);
-  if (n_works == 0) return 0;
   hipStream_t s = (hipStream_t)stream;
   const int G = n_heads / n_kv_heads;
   if (dtype == LSK_DTYPE_BF16) {
-    LSK_REQUIRE(recs && n_rounds > 0 && n_slots > 0, LSK_EARG, "%s: a schedule is needed (lsk_attn_schedule)", what);
-    CacheAttnArgs a = {(const uint16_t*)q, q_stride_t, q_stride_h, kcache, vcache, nullptr, nullptr, mask, mask_words,
-                       recs, n_rounds, (uint16_t*)out, nullptr, nullptr, G, n_kv_heads, max_seq, 0.f};
-    return cache_attn(what, false, a, blocks, n_works, groups, n_groups, n_parts, n_slots, rows_cap, n_heads, head_dim,
-                      scale, workspace, ws_bytes, s);
+    LSK_REQUIRE(n_rounds >= 0, LSK_EARG, "%s: a plan of %d rounds", what, n_rounds);
+    if (n_rounds == 0) return 0;
+    LSK_REQUIRE(recs != nullptr, LSK_EARG, "%s: null pointer", what);
+    const CacheAttnArgs a = {(const uint16_t*)q, q_stride_t, q_stride_h, kcache, vcache, nullptr, nullptr, mask,
+                             mask_words, recs, n_rounds, (uint16_t*)out, nullptr, nullptr, part_rows, G, n_kv_heads,
+                             max_seq, 0.f};
+    return cache_attn(what, false, a, groups, n_groups, n_parts, n_slots, tiles, row_groups, head_dim, scale, workspace,
+                      ws_bytes, s);
   }
+  LSK_REQUIRE(n_works >= 0 && rows_cap > 0 && rows_cap % 16 == 0 && rows_cap <= ATTN_ROWS, LSK_EARG,
+              "%s: a plan of %d works of up to %d rows (16, 32 or %d)", what, n_works, rows_cap, ATTN_ROWS);
+  if (n_works == 0) return 0;
   LSK_REQUIRE(works != nullptr, LSK_EARG, "%s: null pointer", what);
-  LSK_REQUIRE(n_parts == 0, LSK_EARG, "%s: the fp32 path takes unsplit plans", what);
   LSK_REQUIRE(max_seq % 32 == 0, LSK_ESHAPE, "%s: max_seq %d", what, max_seq);
   const dim3 grid(n_works, n_kv_heads, rows_cap / 4);
 #define LSK_TREE_F32(DD)                                                                                           \

@@ -10,6 +10,7 @@ fp32: the sums of n positions and D products, one after the other: (n + D + 64) 
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import numpy as np
@@ -303,11 +304,11 @@ def _tree_blocks(blocks, seed):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("split", [None, 64])
+@pytest.mark.parametrize("split,row_groups", [(None, None), (64, 1), (64, 8), (1024, 2), (128, 4)])
 @pytest.mark.parametrize("blocks", BLOCKS)
 @pytest.mark.parametrize("kind,heads", [("bf16", "gqa128"), ("bf16", "gqa64"), ("bf16", "mqa128"), ("kv8", "gqa128"),
                                         ("kv8", "mha64"), ("fp32", "gqa64"), ("fp32", "mqa128")])
-def test_tree_attention_matches_64_bits(cuda, kind, heads, blocks, split):
+def test_tree_attention_matches_64_bits(cuda, kind, heads, blocks, split, row_groups):
     lsk = _lsk()
     Hq, Hkv, D = _heads(heads)
     dtype = F32 if kind == "fp32" else BF16
@@ -316,11 +317,12 @@ def test_tree_attention_matches_64_bits(cuda, kind, heads, blocks, split):
     mask = torch.from_numpy(words_of(sets, (max(t for _, _, t in BLOCKS[blocks]) + 31) // 32)).to(cuda)
     if kind == "kv8":
         cache = kv8_from(lsk, cuda, k, v)
-        got = lsk.kv8_attn(q.to(cuda), cache, lsk.AttnPlan(tab, Hq, cache, split=split), mask)
+        got = lsk.kv8_attn(q.to(cuda), cache, lsk.AttnPlan(tab, Hq, cache, split, row_groups), mask)
         k, v = held(k), held(v)
     else:
         ks = (lsk.k_to_frag(k) if kind == "bf16" else k).to(cuda)
-        got = lsk.tree_attn(q.to(cuda), ks, lsk.v_to_blocked(v).to(cuda), lsk.AttnPlan(tab, Hq, ks, split=split), mask)
+        plan = lsk.AttnPlan(tab, Hq, ks, split, row_groups)
+        got = lsk.tree_attn(q.to(cuda), ks, lsk.v_to_blocked(v).to(cuda), plan, mask)
     ref, mag, big = attention(q.double(), k.double(), v.double(), tab, 1 / math.sqrt(D), sets)
     if kind == "fp32":
         assert_close_f32(got, ref, mag, 1088, D, big)
@@ -348,20 +350,20 @@ def test_masks_of_any_kind_and_rows_that_read_nothing(cuda, kind):
     if kind == "kv8":
         cache = kv8_from(lsk, cuda, k, v)
 
-        def run(split):
-            return lsk.kv8_attn(q.to(cuda), cache, lsk.AttnPlan(tab, Hq, cache, split=split), mask)
+        def run(split, rg):
+            return lsk.kv8_attn(q.to(cuda), cache, lsk.AttnPlan(tab, Hq, cache, split, rg), mask)
 
         k, v = held(k), held(v)
     else:
         ks = (lsk.k_to_frag(k) if kind == "bf16" else k).to(cuda)
         vs = lsk.v_to_blocked(v).to(cuda)
 
-        def run(split):
-            return lsk.tree_attn(q.to(cuda), ks, vs, lsk.AttnPlan(tab, Hq, ks, split=split), mask)
+        def run(split, rg):
+            return lsk.tree_attn(q.to(cuda), ks, vs, lsk.AttnPlan(tab, Hq, ks, split, rg), mask)
 
     ref, mag, big = attention(q.double(), k.double(), v.double(), tab, 1 / math.sqrt(D), sets)
-    for split in (None, 64):
-        got = run(split)
+    for split, rg in ((None, 1), (64, 1), (None, 8), (64, 8)):
+        got = run(split, rg)
         assert (got[:5] == 0).all() and (got[n - 1] == 0).all()
         if kind == "fp32":
             assert_close_f32(got, ref, mag, 192, D, big)
@@ -370,9 +372,10 @@ def test_masks_of_any_kind_and_rows_that_read_nothing(cuda, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("row_groups", [1, 8])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("kind", ["bf16", "kv8", "kv8 causal", "fp32"])
-def test_values_that_a_row_does_not_read_never_reach_it(cuda, kind, bad):
+def test_values_that_a_row_does_not_read_never_reach_it(cuda, kind, bad, row_groups):
     """NaN and infinities in nodes that a row does not read, in the slots behind the block and in those of other rows
     leave its bits as they are; a row that reads such a V gets what the formula gives."""
     lsk = _lsk()
@@ -392,9 +395,11 @@ def test_values_that_a_row_does_not_read_never_reach_it(cuda, kind, bad):
             if bad != bad:                                            # slots never written: any byte as a scale
                 for b, (_, p0, t, row) in enumerate(tab):
                     cache.ks[row, :, p0 + t:], cache.vs[row, :, p0 + t:] = 255, 255
-            return lsk.kv8_attn(q.to(cuda), cache, lsk.AttnPlan(tab, Hq, cache), mask if kind == "kv8" else None).cpu()
+            plan = lsk.AttnPlan(tab, Hq, cache, None, row_groups)
+            return lsk.kv8_attn(q.to(cuda), cache, plan, mask if kind == "kv8" else None).cpu()
         ks = (lsk.k_to_frag(k) if kind == "bf16" else k).to(cuda)
-        return lsk.tree_attn(q.to(cuda), ks, lsk.v_to_blocked(v).to(cuda), lsk.AttnPlan(tab, Hq, ks), mask).cpu()
+        plan = lsk.AttnPlan(tab, Hq, ks, None, row_groups)
+        return lsk.tree_attn(q.to(cuda), ks, lsk.v_to_blocked(v).to(cuda), plan, mask).cpu()
 
     clean = run(k, v)
     k2, v2 = k.clone(), v.clone()
@@ -418,32 +423,44 @@ def test_values_that_a_row_does_not_read_never_reach_it(cuda, kind, bad):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("dtype", [BF16, F32])
-def test_a_chain_gives_the_ragged_attentions_bits(cuda, dtype, D):
+@pytest.mark.parametrize("D", [16, 64, 128])
+def test_an_fp32_chain_gives_the_ragged_attentions_bits(cuda, D):
     lsk = _lsk()
     Hq, Hkv = 8, 2
     blocks = [(0, 0, 5), (2, 63, 9), (1, 700, 40), (3, 1000, 1)]
-    tab, q, k, v = _attn_inputs(23, (Hq, Hkv, D), blocks, dtype)
-    ks = (lsk.k_to_frag(k) if dtype == BF16 else k).to(cuda)
-    vs = lsk.v_to_blocked(v).to(cuda)
+    tab, q, k, v = _attn_inputs(23, (Hq, Hkv, D), blocks, F32)
+    kd, vd = k.to(cuda), lsk.v_to_blocked(v).to(cuda)
     sets = [set(range(i + 1)) for (_, _, t) in blocks for i in range(t)]
     mask = torch.from_numpy(words_of(sets, 2)).to(cuda)
-    for split in (256, 2048):
-        p = lsk.AttnPlan(tab, Hq, ks, split=split)
-        want = torch.empty(len(q), Hq * D, dtype=dtype, device=cuda)        # (the plan serves both)
-        ws = torch.empty(max(p.ws_bytes, 1), dtype=torch.uint8, device=cuda)
-        lsk.ragged_attn(q.to(cuda), ks, vs, p.blocks, p.works, p.n_works, p.groups, p.n_groups, p.n_parts, want, Hq,
-                        1 / math.sqrt(D), ws, p.recs, p.n_rounds, p.n_slots, p.rows_cap)
-        assert torch.equal(lsk.tree_attn(q.to(cuda), ks, vs, p, mask), want)
+    p = lsk.AttnPlan(tab, Hq, kd)
+    want = torch.empty(len(q), Hq * D, device=cuda)
+    b = torch.tensor(tab, dtype=torch.int32, device=cuda)
+    lsk.ragged_attn(q.to(cuda), kd, vd, b, p.works, p.n_works, None, 0, 0, want, Hq, 1 / math.sqrt(D),
+                    rows_cap=p.rows_cap)
+    assert torch.equal(lsk.tree_attn(q.to(cuda), kd, vd, p, mask), want)
 
 
 @pytest.mark.gpu
+def test_trees_of_one_node_and_causal_launches_agree(cuda):
+    """A launch with a mask gives, for blocks of up to 32 rows whose mask is the causal rule, the causal launch's bits:
+    a root without drafts is a decode step."""
+    lsk = _lsk()
+    Hq, Hkv, D = 8, 2, 128
+    blocks = [(0, 0, 1), (2, 63, 8), (1, 700, 1), (3, 1000, 5)]
+    tab, q, k, v = _attn_inputs(43, (Hq, Hkv, D), blocks)
+    cache = kv8_from(lsk, cuda, k, v)
+    mask = torch.from_numpy(words_of([set(range(i + 1)) for (_, _, t) in blocks for i in range(t)], 1)).to(cuda)
+    plan = lsk.AttnPlan(tab, Hq, cache, split=256, row_groups=8)
+    assert torch.equal(lsk.kv8_attn(q.to(cuda), cache, plan, mask), lsk.kv8_attn(q.to(cuda), cache, plan))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("row_groups", [1, 8])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("kind", ["kv8", "kv8 tree", "tree"])
-def test_a_rows_result_depends_on_its_block_only(cuda, kind, D):
-    """The same rows alone, in another order, next to others and as single tokens (causal) give the same bits; so do
-    other rows-per-item caps."""
+def test_a_rows_result_depends_on_its_block_only(cuda, kind, D, row_groups):
+    """The same rows alone, in another order, next to others (in launches of 1, 2 and 3 tiles) and as single tokens
+    (causal) give the same bits."""
     lsk = _lsk()
     Hq, Hkv = 8, 2
     blocks = [(0, 37, 9), (3, 500, 30), (1, 0, 3), (2, 900, 60)]
@@ -454,19 +471,11 @@ def test_a_rows_result_depends_on_its_block_only(cuda, kind, D):
     cache = kv8_from(lsk, cuda, k, v)
     kf, vf = lsk.k_to_frag(k).to(cuda), lsk.v_to_blocked(v).to(cuda)
 
-    def run(sel, cap=None):
+    def run(sel):
         """sel: [(row, pos0, T, first token)]"""
         tab, _ = pack_blocks([s[:3] for s in sel])
         idx = torch.cat([torch.arange(s[3], s[3] + s[2]) for s in sel]).to(cuda)
-        plan = lsk.AttnPlan(tab, Hq, kf if kind == "tree" else cache, split=256)
-        if cap:
-            b = np.array(tab, dtype=np.int32)
-            works, groups, plan.n_parts = lsk.attn_plan(b, Hq // Hkv, 256, cap)
-            recs, plan.n_rounds = lsk.attn_schedule(works, Hkv, plan.n_slots)
-            up = [torch.from_numpy(x.ravel().copy()).to(cuda) for x in (works, groups, recs)]
-            plan.works, plan.groups, plan.recs = up
-            plan.n_works, plan.n_groups, plan.rows_cap = len(works), len(groups), cap
-            plan.ws_bytes = lsk.attn_workspace_bytes(plan.n_parts, Hkv, D)
+        plan = lsk.AttnPlan(tab, Hq, kf if kind == "tree" else cache, split=256, row_groups=row_groups)
         m = words[idx].contiguous()
         if kind == "tree":
             return lsk.tree_attn(qd[idx], kf, vf, plan, m), idx
@@ -474,9 +483,7 @@ def test_a_rows_result_depends_on_its_block_only(cuda, kind, D):
 
     whole = [(r, p, t, a) for (a, p, t, r) in tab]
     full, _ = run(whole)
-    for cap in (16, 32, 48)[:3 if D == 64 else 2]:
-        assert torch.equal(run(whole, cap)[0], full)
-    for sel in ([whole[1]], [whole[3], whole[0]], whole[::-1]):
+    for sel in ([whole[1]], [whole[2]], [whole[3], whole[0]], whole[::-1]):
         got, idx = run(sel)
         assert torch.equal(got, full[idx])
     if kind == "kv8":
@@ -527,7 +534,7 @@ def test_attention_scale_streams_and_graph_replays(cuda):
     cache = kv8_from(lsk, cuda, k, v)
     kf, vf = lsk.k_to_frag(k).to(cuda), lsk.v_to_blocked(v).to(cuda)
     p8, pt = lsk.AttnPlan(tab, Hq, cache, split=256), lsk.AttnPlan(tab, Hq, kf, split=256)
-    assert p8.n_parts > 0 and pt.n_parts > 0
+    assert p8.causal.n_parts > 0 and pt.tree.n_parts > 0
     qd = q.to(cuda)
     ref, mag, _ = attention(q.double(), held(k), held(v), tab, 0.03)
     assert_close_bf16(lsk.kv8_attn(qd, cache, p8, scale=0.03), ref, mag)
@@ -777,17 +784,34 @@ def test_entry_points_refuse_bad_arguments():
     assert r(1, P, P, P, P, P, P, P, None, 4, 2, 64, 3, 128, None) == -1
     assert r(1, P, P, P, P, P, P, P, P, 4, 2, 32, 3, 128, None) == -3
     assert r(1, P, P, P, P, P, P, P, P, 0, 2, 64, 3, 128, None) == 0
-    ok = [P, 512, 64, P, P, P, P, None, 0, P, 1, None, 0, 0, P, 1, 1, 16, P, 8, 2, 64, 128, 0.125, None, 0, None]
+    # q, strides, k8, v8, exponents, mask, words | groups, n_groups, n_parts, recs, rounds, slots, tiles, row groups, part
+    # rows | out, heads, KV heads, D, S, scale, workspace, bytes, stream
+    ok = [P, 512, 64, P, P, P, P, None, 0, None, 0, 0, P, 1, 1, 1, 1, 16, P, 8, 2, 64, 128, 0.125, None, 0, None]
     k8 = lambda **kw: lib.lsk_kv8_attn(*[kw.get(f"a{i}", x) for i, x in enumerate(ok)])  # noqa: E731
-    assert k8(a0=None) == -1 and k8(a5=None) == -1 and k8(a14=None) == -1 and k8(a17=24) == -1 and k8(a17=48, a21=128) == -3 and k8(a7=P) == -1
+    assert k8(a0=None) == -1 and k8(a5=None) == -1 and k8(a12=None) == -1 and k8(a7=P) == -1 and k8(a18=None) == -1
+    assert k8(a15=4) == -1 and k8(a15=3, a21=128) == -1 and k8(a15=3, a7=P, a8=1) == -1 and k8(a16=2) == -1
+    assert k8(a14=0) == -1 and k8(a10=1) == -1 and k8(a13=-1) == -1
     assert k8(a19=7) == -2 and k8(a22=96) == -2 and k8(a21=32) == -3 and k8(a3=24) == -1 and k8(a1=-1) == -2
-    assert k8(a13=3) == -4 and k8(a13=3, a11=P, a24=P, a25=100) == -4          # split partials without their workspace
-    assert k8(a22=1 << 25) == -2                                               # a stripe of 2 GiB and more
-    assert k8(a10=0) == 0
-    ok2 = [1, P, 512, 64, P, P, P, 1, P, P, 1, None, 0, 0, P, 1, 1, 16, P, 8, 2, 64, 128, 0.125, None, 0, None]
+    assert k8(a10=1, a11=3) == -4 and k8(a10=1, a11=3, a9=P, a24=P, a25=100) == -4   # partials without their workspace
+    assert k8(a10=1, a11=3, a9=P, a24=P, a25=1 << 20, a17=8) == -1                   # rows per partial below a tile
+    assert k8(a22=1 << 25) == -2                                                     # a stripe of 2 GiB and more
+    assert k8(a13=0) == 0
+    ok2 = [1, P, 512, 64, P, P, P, 1, None, 0, 0, None, 0, 0, P, 1, 1, 1, 1, 16, P, 8, 2, 64, 128, 0.125, None, 0, None]
     tr = lambda **kw: lib.lsk_tree_attn(*[kw.get(f"a{i}", x) for i, x in enumerate(ok2)])  # noqa: E731
-    assert tr(a6=None) == -1 and tr(a7=0) == -1 and tr(a0=2) == -3 and tr(a14=None) == -1 and tr(a21=96) == -3
-    assert tr(a0=0, a13=2) == -1 and tr(a0=0, a21=80) == -3 and tr(a0=0, a9=None) == -1 and tr(a10=0) == 0
+    assert tr(a6=None) == -1 and tr(a7=0) == -1 and tr(a0=2) == -3 and tr(a14=None) == -1 and tr(a23=96) == -3
+    assert tr(a0=0) == -1 and tr(a0=0, a9=1, a10=16) == -1 and tr(a0=0, a9=1, a10=24, a8=P) == -1
+    assert tr(a0=0, a9=1, a10=16, a8=P, a23=80) == -3 and tr(a0=0, a10=16) == 0 and tr(a15=0) == 0
+    cnt = (ctypes.c_long * 8)()
+    blk = (ctypes.c_int32 * 4)(0, 700, 40, 0)
+    plan = lambda **kw: lib.lsk_cache_attn_plan(*[kw.get(f"a{i}", x) for i, x in enumerate(  # noqa: E731
+        [blk, 1, 4, 256, 2, 128, 1, 1, 8, 256, None, 0, cnt])])
+    assert plan() == 0 and list(cnt)[:3] == [40, 1, 3] and cnt[4] == 2 and cnt[7] == 8
+    assert plan(a3=100) == -2 and plan(a8=3) == -2 and plan(a5=96) == -3 and plan(a0=None) == -1 and plan(a12=None) == -1
+    assert plan(a10=blk, a11=4) == -4 and plan(a1=0) == 0 and cnt[3] == 0
+    blk[1] = 64 * 128
+    assert plan(a3=64) == -2                                                         # more than 128 splits
+    blk[1] = -1
+    assert plan() == -2
     m = lib.lsk_tree_masks
     assert m(None, P, P, 1, 4, 4, P, 1, None, None) == -1 and m(P, P, P, 1, 4, 33, P, 1, None, None) == -2
     assert m(P, P, P, 0, 4, 4, P, 1, None, None) == 0 and m(P, P, P, 1, 0, 4, P, 1, None, None) == 0
@@ -807,7 +831,7 @@ def test_plans_refuse_blocks_outside_the_cache():
     lsk = _lsk()
     cache = lsk.KV8.zeros(2, 2, 128, 64, "cpu")
     plan = lsk.AttnPlan([(0, 3, 2, 1), (2, 0, 0, 0), (2, 127, 1, 0)], 4, cache)
-    assert plan.n_tokens == 3 and plan.n_works > 0 and plan.split == 512
+    assert plan.n_tokens == 3 and plan.causal.n_rounds > 0 and plan.tree.n_rounds > 0 and plan.split == 512
     for b in ([(0, 3, 2, 2)], [(0, 3, 2, -1)], [(0, 127, 2, 0)], [(0, -1, 2, 0)], [(1, 0, 2, 0)], [(0, 0, -1, 0)]):
         with pytest.raises(ValueError):
             lsk.AttnPlan(b, 4, cache)
@@ -819,8 +843,63 @@ def test_plans_refuse_blocks_outside_the_cache():
         lsk.KV8.zeros(2, 2, 100, 64, "cpu")
     with pytest.raises(ValueError):
         lsk.KV8.zeros(2, 2, 128, 96, "cpu")
-    assert lsk.AttnPlan([], 4, cache).n_works == 0
-    assert lsk.cache_attn_split(1, 8, 131072) * 128 >= 131072 and lsk.cache_attn_split(256, 8, 8192) == 8192
+    assert lsk.AttnPlan([], 4, cache).causal.n_rounds == 0
+    assert lsk.AttnPlan([], 4, cache, tree=True).causal is None and lsk.AttnPlan([], 4, cache, tree=False).tree is None
+    with pytest.raises(lsk.LskError):
+        lsk.AttnPlan([(0, 0, 1, 0)], 4, cache, row_groups=3)
+    for b, s in ((1, 131072), (256, 8192), (32, 2048), (3, 64)):
+        split = lsk.cache_attn_split(b, 8, s)
+        assert split % 64 == 0 and 512 <= split <= 8192 and split * 128 >= s
+
+
+def _items(plan, launch):
+    """(row group rows, wave rows) of every work item of a plan: [(q_start, row0, nrows, groups, kvh, lo, hi, part)]"""
+    recs = launch.recs.numpy().reshape(launch.n_slots, launch.n_rounds, 8)
+    out = []
+    for slot in recs:
+        live = [r for r in slot if r[2] & 1023]
+        assert all((r[2] & 1023) == 0 for r in slot[len(live):])      # a slot's items come first
+        out += [(r[0], r[1], r[2] & 1023, 1 << (r[2] >> 10 & 3), r[2] >> 12, r[3], r[4], r[5]) for r in live]
+    return out
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("G,split,T_hi", [(4, 256, 9), (1, 64, 70), (8, 8192, 40), (3, 128, 130), (4, 512, 1)])
+def test_cache_attention_plans_cover_every_row_and_position_once(G, split, T_hi, tree, D):
+    lsk = _lsk()
+    rng = np.random.default_rng(T_hi)
+    B, Hkv, S = 6, 3, 1024
+    cache = lsk.KV8.zeros(B, Hkv, S, D, "cpu")
+    blocks = [(r, int(rng.integers(0, S - T_hi)), int(rng.integers(0, T_hi + 1))) for r in range(B)]
+    tab, n = pack_blocks(blocks)
+    plan = lsk.AttnPlan(tab, G * Hkv, cache, split=split, row_groups=8, tree=tree)
+    p = plan.tree if tree else plan.causal
+    items = _items(plan, p)
+    most = max(t for _, _, t in blocks) * G
+    assert p.tiles == (1 if most <= 16 else 2 if most <= 32 or tree or D == 128 else 3)
+    parts = [i for i in items if i[7] >= 0]
+    assert len({(i[4], i[7]) for i in parts}) == len(parts) == p.n_parts * Hkv
+    groups = {tuple(g[:5]) for g in p.groups.numpy().reshape(-1, 8)}
+    for (q0, p0, t, row) in tab:
+        rows = t * G
+        want = 1
+        while tree and want < 8 and rows > 32 * want:
+            want *= 2
+        mine = [i for i in items if i[0] == q0] if t else []
+        for h in range(Hkv):
+            covered = np.zeros((rows, S + 1), dtype=int)
+            for (_, r0, nr, g, kvh, lo, hi, part) in mine:
+                if kvh == h:
+                    assert g == want and nr <= 16 * p.tiles * g and lo % split == 0
+                    covered[r0:r0 + nr, lo:hi] += 1
+            for r in range(rows):
+                assert (covered[r, :p0 + r // G + 1] == 1).all()      # what the causal rule lets the row read
+        for (_, r0, nr, g, kvh, lo, hi, part) in mine:
+            ns = -(-(p0 + (r0 + nr - 1) // G + 1) // split)
+            assert (part >= 0) == (ns > 1)
+            if part >= 0:
+                assert (q0, r0, nr, part - lo // split, ns) in groups and nr <= p.part_rows
 
 
 def test_wrappers_refuse_tensors_off_the_gpu():

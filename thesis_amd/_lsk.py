@@ -79,10 +79,12 @@ _SIGS = {
                                 ctypes.c_double, ctypes.c_double, _P]),
     "lsk_kv8_append": (_I, [_I, _P, _P, _L, _L] + [_P] * 6 + [_I] * 5 + [_P]),
     "lsk_kv8_read": (_I, [_I] + [_P] * 8 + [_I] * 5 + [_P]),
-    "lsk_kv8_attn": (_I, [_P, _L, _L] + [_P] * 5 + [_I, _P, _I, _P, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _I, _F, _P,
-                          _Z, _P]),
-    "lsk_tree_attn": (_I, [_I, _P, _L, _L, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _I,
-                           _F, _P, _Z, _P]),
+    "lsk_cache_attn_plan": (_I, [_P] + [_I] * 9 + [_P, _L, _P]),
+    "lsk_cache_attn_workspace_bytes": (_Z, [_I, _I, _I, _I]),
+    "lsk_kv8_attn": (_I, [_P, _L, _L] + [_P] * 5 + [_I, _P, _I, _I, _P] + [_I] * 5 + [_P] + [_I] * 4 + [_F, _P, _Z,
+                          _P]),
+    "lsk_tree_attn": (_I, [_I, _P, _L, _L, _P, _P, _P, _I, _P, _I, _I, _P, _I, _I, _P] + [_I] * 5 + [_P] + [_I] * 4 +
+                      [_F, _P, _Z, _P]),
     "lsk_tree_masks": (_I, [_P, _P, _P, _I, _I, _I, _P, _I, _P, _P]),
     "lsk_tree_accept": (_I, [_P] * 5 + [_I, _I, _I] + [_P] * 4),
     "lsk_kv_compact": (_I, [_I] + [_P] * 4 + [_I] + [_P] * 4 + [_I] * 6 + [_P]),
@@ -630,22 +632,46 @@ def kv8_read(cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor, dtype: t
 
 def cache_attn_split(max_batch: int, n_kv_heads: int, max_seq: int) -> int:
     """KV positions per attention split of a cache: fixed by the cache, so that a row's result never depends on the
-    batch it is in.  Caches of many (row, KV head) stripes keep a context whole; with fewer, a context is shared by
-    several workgroups.  At most 128 splits per context."""
+    batch it is in.  About as many splits of the longest context as make one work item per CU out of the cache's
+    (row, KV head) stripes; 512 to 8192 positions, at most 128 splits."""
+    split = min(max(max_seq * max_batch * n_kv_heads // 256, 512), ATTN_SPLIT)
+    return (max(split, -(-max_seq // 128)) + 63) // 64 * 64
+
+
+def cache_attn_row_groups(max_batch: int, n_kv_heads: int) -> int:
+    """Row groups of a tree's work items at most (lsk_cache_attn_plan), fixed by the cache as the split is: caches of
+    few stripes keep the rows on as many CUs as there are."""
     stripes = max_batch * n_kv_heads
-    split = ATTN_SPLIT if stripes >= 1024 else 2048 if stripes >= 256 else 512
-    return max(split, (max_seq + 128 * 64 - 1) // (128 * 64) * 64)
+    return 8 if stripes >= 128 else 4 if stripes >= 64 else 2 if stripes >= 32 else 1
+
+
+class _Launch(NamedTuple):
+    """One lsk_cache_attn_plan on the device."""
+    groups: torch.Tensor
+    recs: torch.Tensor
+    n_groups: int
+    n_parts: int
+    n_rounds: int
+    n_slots: int
+    tiles: int
+    row_groups: int
+    part_rows: int
+    ws_bytes: int
 
 
 class AttnPlan:
-    """The plan of an attention launch over packed blocks, shared by the layers of a segment (lsk_attn_plan and
-    lsk_attn_schedule, on the device).  blocks: int [nb, 4] = (q_start, pos0, T, row) with q_start the running sum of
-    T; cache: a layer's KV8, or the K storage of a bf16 or fp32 cache.  split: KV positions per split (fp32: unsplit)."""
+    """The plan of attention launches over packed blocks, shared by the layers of a segment.  blocks: int [nb, 4] =
+    (q_start, pos0, T, row) with q_start the running sum of T; cache: a layer's KV8, or the K storage of a bf16 or fp32
+    cache.  split: KV positions per split (cache_attn_split unless given; fp32 does not split); row_groups:
+    cache_attn_row_groups unless given.  tree: which launches it is for, with a mask (True), without (False) or, over an
+    8-bit cache, either (None)."""
 
-    def __init__(self, blocks, n_heads: int, cache, split: int | None = None):
-        kcache = cache.k if isinstance(cache, KV8) else cache
-        self.dims = B, Hkv, S, D = cache.dims if isinstance(cache, KV8) else k_dims(cache)
-        self.kv8, self.dtype = isinstance(cache, KV8), kcache.dtype
+    def __init__(self, blocks, n_heads: int, cache, split: int | None = None, row_groups: int | None = None,
+                 tree: bool | None = None):
+        self.kv8 = isinstance(cache, KV8)
+        kcache = cache.k if self.kv8 else cache
+        self.dims = B, Hkv, S, D = cache.dims if self.kv8 else k_dims(cache)
+        self.dtype, self.device = kcache.dtype, kcache.device
         if n_heads <= 0 or n_heads % Hkv:
             raise ValueError(f"{n_heads} query heads over {Hkv} KV heads")
         b = np.asarray(blocks, dtype=np.int64).reshape(-1, 4)
@@ -655,33 +681,47 @@ class AttnPlan:
             raise ValueError(f"a block lies outside the cache's {B} rows x {S} positions")
         if (split is not None and (split < 64 or split % 64)) or len(b) and int(b[:, 2].sum()) >= 1 << 30:
             raise ValueError(f"a split of {split} positions (a multiple of 64), or too many tokens")
+        self.n_heads, self.n_tokens = n_heads, int(b[:, 2].sum())
+        b = np.ascontiguousarray(b, dtype=np.int32)
+        group, n_slots = n_heads // Hkv, cu_count(self.device)
+        self.works = self.causal = self.tree = None
+        self.rows_cap = self.n_works = 0
         if self.dtype == torch.float32:
-            split = 1 << 30
-        elif split is None:
-            split = cache_attn_split(B, Hkv, S)
-        self.n_heads, self.split, self.n_tokens = n_heads, split, int(b[:, 2].sum())
-        self.device, group = kcache.device, n_heads // Hkv
-        b = b.astype(np.int32)
-        self.n_slots = cu_count(self.device)
-        self.rows_cap = attn_rows_cap(b, group, split, Hkv, D, self.n_slots)
-        if D == 128 and self.dtype != torch.float32:
-            self.rows_cap = min(self.rows_cap, 32)    # two tiles of accumulators are what a wave's registers hold
-        works, groups, self.n_parts = attn_plan(b, group, split, self.rows_cap)
-        recs, self.n_rounds = attn_schedule(works, Hkv, self.n_slots)
-        self.n_works, self.n_groups = len(works), len(groups)
-        parts = [b.ravel(), works.ravel(), groups.ravel(), recs]
-        meta = torch.from_numpy(np.concatenate(parts).astype(np.int32))
-        if self.device.type == "cuda":
-            meta = meta.pin_memory().to(self.device, non_blocking=True)
-        self.blocks, self.works, self.groups, self.recs = meta.split([len(p) for p in parts])
-        self.ws_bytes = attn_workspace_bytes(self.n_parts, Hkv, D) if self.n_parts else 0
+            self.split, self.rows_cap = 1 << 30, 16
+            works, _, _ = attn_plan(b, group, self.split, self.rows_cap)
+            self.works, self.n_works = self._upload(works.ravel()), len(works)
+            return
+        self.split = cache_attn_split(B, Hkv, S) if split is None else split
+        rg = cache_attn_row_groups(B, Hkv) if row_groups is None else row_groups
+        if self.kv8 and not tree:
+            self.causal = self._plan(b, group, Hkv, D, False, 1, n_slots)
+        if tree or tree is None:
+            self.tree = self._plan(b, group, Hkv, D, True, rg, n_slots)
+
+    def _upload(self, words: np.ndarray) -> torch.Tensor:
+        t = torch.from_numpy(words)
+        return t.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else t
+
+    def _plan(self, b: np.ndarray, group: int, Hkv: int, D: int, tree: bool, row_groups: int, n_slots: int) -> _Launch:
+        lib, cnt = load(), np.zeros(8, dtype=np.int64)
+        args = (b.ctypes.data if len(b) else None, len(b), group, self.split, Hkv, D, int(self.kv8), int(tree),
+                row_groups, n_slots)
+        _check(lib.lsk_cache_attn_plan(*args, None, 0, cnt.ctypes.data), "lsk_cache_attn_plan")
+        meta = np.zeros(max(int(cnt[6]), 1), dtype=np.int32)
+        _check(lib.lsk_cache_attn_plan(*args, meta.ctypes.data, meta.size, cnt.ctypes.data), "lsk_cache_attn_plan")
+        _, ng, parts, rounds, tiles, part_rows, _, used = (int(x) for x in cnt)
+        dev = self._upload(meta)
+        ws = int(lib.lsk_cache_attn_workspace_bytes(parts, Hkv, part_rows, D)) if parts else 0
+        return _Launch(dev[:ng * 8], dev[ng * 8:], ng, parts, rounds, n_slots, tiles, used, part_rows, ws)
 
 
-def _plan_call(what: str, q: torch.Tensor, plan: AttnPlan, dims: tuple, kv8: bool, dtype: torch.dtype, mask, scale, out,
-               workspace):
+def _plan_call(what: str, q: torch.Tensor, plan: AttnPlan, launch, dims: tuple, kv8: bool, dtype: torch.dtype, mask,
+               scale, out, workspace):
     """Checks shared by kv8_attn and tree_attn; returns (scale, out, workspace, its bytes)."""
     if plan.dims != dims or plan.kv8 != kv8 or plan.dtype != dtype:
         raise LskError(f"{what}: the plan was made for another cache ({plan.dims} {plan.dtype})")
+    if launch is None and dtype != torch.float32:
+        raise LskError(f"{what}: the plan was made for launches {'without' if mask is not None else 'with'} a mask")
     _, Hkv, _, D = dims
     want = torch.bfloat16 if kv8 else dtype
     if q.shape != (plan.n_tokens, plan.n_heads, D) or q.dtype != want or (q.numel() and q.stride(2) != 1):
@@ -693,9 +733,10 @@ def _plan_call(what: str, q: torch.Tensor, plan: AttnPlan, dims: tuple, kv8: boo
         _want(what, "mask", mask, torch.int32, (plan.n_tokens, mask.shape[1]))
     if out is None:
         out = torch.empty(plan.n_tokens, plan.n_heads * D, dtype=want, device=q.device)
-    _want(what, "out", out, want, (plan.n_tokens, plan.n_heads * D))
-    if workspace is None and plan.ws_bytes:
-        workspace = torch.empty(plan.ws_bytes, dtype=torch.uint8, device=q.device)
+    else:
+        _want(what, "out", out, want, (plan.n_tokens, plan.n_heads * D))
+    if workspace is None and launch is not None and launch.ws_bytes:
+        workspace = torch.empty(launch.ws_bytes, dtype=torch.uint8, device=q.device)
     ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
     return 1.0 / math.sqrt(D) if scale is None else float(scale), out, workspace, ws_bytes
 
@@ -705,18 +746,19 @@ def kv8_attn(q: torch.Tensor, cache: KV8, plan: AttnPlan, mask: torch.Tensor | N
     """Ragged verify / decode attention over a layer's 8-bit cache (lsk_kv8_attn): q [N, Hq, D] bf16 -> [N, Hq * D].
     mask (int32 [N, words], tree_masks): blocks are trees of drafted tokens.  scale: 1 / sqrt(D) unless given.  Without
     a workspace one is taken from torch's allocator for the call."""
-    dev = _one_device(q, *cache, plan.recs, mask, out, workspace)
+    p = plan.causal if mask is None else plan.tree
+    dev = _one_device(q, *cache, p.recs if p is not None else None, mask, out, workspace)
     cache.check("kv8_attn")
-    scale, out, workspace, ws = _plan_call("kv8_attn", q, plan, cache.dims, True, cache.k.dtype, mask, scale, out,
+    scale, out, workspace, ws = _plan_call("kv8_attn", q, plan, p, cache.dims, True, cache.k.dtype, mask, scale, out,
                                            workspace)
-    if plan.n_works:
+    if p.n_rounds:
         _, Hkv, S, D = cache.dims
         with _current(dev):
             _check(load().lsk_kv8_attn(_ptr(q), q.stride(0), q.stride(1), *map(_ptr, cache), _ptr(mask),
-                                       mask.shape[1] if mask is not None else 0, _ptr(plan.blocks), plan.n_works,
-                                       _ptr(plan.groups), plan.n_groups, plan.n_parts, _ptr(plan.recs), plan.n_rounds,
-                                       plan.n_slots, plan.rows_cap, _ptr(out), plan.n_heads, Hkv, D, S, scale,
-                                       _ptr(workspace), ws, _stream()), "lsk_kv8_attn")
+                                       mask.shape[1] if mask is not None else 0, _ptr(p.groups), p.n_groups, p.n_parts,
+                                       _ptr(p.recs), p.n_rounds, p.n_slots, p.tiles, p.row_groups, p.part_rows,
+                                       _ptr(out), plan.n_heads, Hkv, D, S, scale, _ptr(workspace), ws, _stream()),
+                   "lsk_kv8_attn")
     return out
 
 
@@ -726,21 +768,24 @@ def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, plan:
     """Attention of trees of drafted tokens over a layer's bf16 or fp32 cache (lsk_tree_attn): q [N, Hq, D] ->
     [N, Hq * D].  kcache: K cache storage (k_dims); vcache: the blocked-transposed V storage; mask: int32 [N, words]
     (tree_masks).  scale: 1 / sqrt(D) unless given."""
-    dev = _one_device(q, kcache, vcache, plan.recs, mask, out, workspace)
+    p = plan.tree
+    dev = _one_device(q, kcache, vcache, p.recs if p is not None else plan.works, mask, out, workspace)
     _check_kcache(kcache.dtype, kcache)
     code = dtype_code(kcache.dtype)
     dims = B, Hkv, S, D = k_dims(kcache)
     if not kcache.is_contiguous():
         raise LskError("tree_attn: the K cache must be contiguous")
     _want("tree_attn", "V cache", vcache, kcache.dtype, (B, Hkv, S // 32, D, 32))
-    scale, out, workspace, ws = _plan_call("tree_attn", q, plan, dims, False, kcache.dtype, mask, scale, out, workspace)
-    if plan.n_works:
+    scale, out, workspace, ws = _plan_call("tree_attn", q, plan, p, dims, False, kcache.dtype, mask, scale, out,
+                                           workspace)
+    if p.n_rounds if p is not None else plan.n_works:
+        launch = (_ptr(p.groups), p.n_groups, p.n_parts, _ptr(p.recs), p.n_rounds, p.n_slots, p.tiles, p.row_groups,
+                  p.part_rows) if p is not None else (None, 0, 0, None, 0, 0, 0, 0, 0)
         with _current(dev):
             _check(load().lsk_tree_attn(code, _ptr(q), q.stride(0), q.stride(1), _ptr(kcache), _ptr(vcache), _ptr(mask),
-                                        mask.shape[1], _ptr(plan.blocks), _ptr(plan.works), plan.n_works,
-                                        _ptr(plan.groups), plan.n_groups, plan.n_parts, _ptr(plan.recs), plan.n_rounds,
-                                        plan.n_slots, plan.rows_cap, _ptr(out), plan.n_heads, Hkv, D, S, scale,
-                                        _ptr(workspace), ws, _stream()), "lsk_tree_attn")
+                                        mask.shape[1], _ptr(plan.works), plan.n_works, plan.rows_cap, *launch,
+                                        _ptr(out), plan.n_heads, Hkv, D, S, scale, _ptr(workspace), ws, _stream()),
+                   "lsk_tree_attn")
     return out
 
 
