@@ -425,7 +425,6 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
       nxt = fetch(r + 2);
     }
     // merge a row group's waves in order: M = max m_w, e_w = exp2(m_w - M), L = sum e_w l_w, O = sum e_w O_w
-    const int nr = 1 << done.lr, ranks = NW >> done.lr;
     if (!QREG) __syncthreads();                      // every wave is past its reads of Q
 #pragma unroll
     for (int p0 = 0; p0 < QT; p0 += MT) {
@@ -442,43 +441,52 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
               make_float4(oacc[qt][c][0], oacc[qt][c][1], oacc[qt][c][2], oacc[qt][c][3]);
       }
       __syncthreads();
-      for (int e = tid; e < nr * MR * (D / 4); e += 64 * NW) {
-        const int x = e / (D / 4), d = 4 * (e - x * (D / 4));
-        const int rg = x / MR, ql = x - rg * MR, qr = 16 * p0 + ql;  // row group, row of the pass, row of the group
-        const int row = rg * GR + qr;                                // row of the item
-        if (qr >= GR || row >= done.nrows) continue;
-        float M = -INFINITY;
-        for (int k = 0; k < ranks; ++k) M = fmaxf(M, s_ml[(k << done.lr) + rg][0][qr]);
-        float L = 0.f;
-        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < ranks; ++k) {
-          const int w = (k << done.lr) + rg;
-          const float mw = s_ml[w][0][qr];
-          const float ew = (mw == -INFINITY) ? 0.f : ((mw == M) ? 1.f : fast_exp2(mw - M));
-          L = L + ew * s_ml[w][1][qr];
-          const float4 ow = *(const float4*)(&s_o[w][ql][d]);
-          O.x = O.x + ew * ow.x;
-          O.y = O.y + ew * ow.y;
-          O.z = O.z + ew * ow.z;
-          O.w = O.w + ew * ow.w;
-        }
-        const int rr = done.row0 + row;
-        const int tt = rr / G, gg = rr - tt * G;
-        if (done.part < 0) {
-          if (TREE && L == 0.f) L = 1.f;             // nothing read: O is 0
-          lsk_u32x2_u pk;
-          pk[0] = (uint32_t)f2bf(O.x / L) | ((uint32_t)f2bf(O.y / L) << 16);
-          pk[1] = (uint32_t)f2bf(O.z / L) | ((uint32_t)f2bf(O.w / L) << 16);
-          *(lsk_u32x2_u*)(A.out + ((long)(done.q_start + tt) * Hq + done.kvh * G + gg) * D + d) = pk;
-        } else {
-          const long slot = ((long)done.part * Hkv + done.kvh) * A.part_rows + row;
-          *(float4*)(A.o_part + slot * D + d) = O;
-          if (d == 0) {
-            A.ml_part[slot * 2 + 0] = M;
-            A.ml_part[slot * 2 + 1] = L;
+      // 4 consecutive d of one row per thread; RANKS waves hold a part of it
+      auto merge = [&](auto ranks_) {
+        constexpr int RANKS = decltype(ranks_)::value, NR = NW / RANKS;
+        for (int e = tid; e < NR * MR * (D / 4); e += 64 * NW) {
+          const int x = e / (D / 4), d = 4 * (e - x * (D / 4));
+          const int rg = x / MR, ql = x - rg * MR, qr = 16 * p0 + ql;  // row group, row of the pass, row of the group
+          const int row = rg * GR + qr;                                // row of the item
+          if (qr >= GR || row >= done.nrows) continue;
+          float M = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < RANKS; ++k) M = fmaxf(M, s_ml[k * NR + rg][0][qr]);
+          float L = 0.f;
+          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < RANKS; ++k) {
+            const float mw = s_ml[k * NR + rg][0][qr];
+            const float ew = (mw == -INFINITY) ? 0.f : ((mw == M) ? 1.f : fast_exp2(mw - M));
+            L = L + ew * s_ml[k * NR + rg][1][qr];
+            const float4 ow = *(const float4*)(&s_o[k * NR + rg][ql][d]);
+            O.x = O.x + ew * ow.x;
+            O.y = O.y + ew * ow.y;
+            O.z = O.z + ew * ow.z;
+            O.w = O.w + ew * ow.w;
+          }
+          const int rr = done.row0 + row;
+          const int tt = rr / G, gg = rr - tt * G;
+          if (done.part < 0) {
+            if (TREE && L == 0.f) L = 1.f;           // nothing read: O is 0
+            lsk_u32x2_u pk;
+            pk[0] = (uint32_t)f2bf(O.x / L) | ((uint32_t)f2bf(O.y / L) << 16);
+            pk[1] = (uint32_t)f2bf(O.z / L) | ((uint32_t)f2bf(O.w / L) << 16);
+            *(lsk_u32x2_u*)(A.out + ((long)(done.q_start + tt) * Hq + done.kvh * G + gg) * D + d) = pk;
+          } else {
+            const long slot = ((long)done.part * Hkv + done.kvh) * A.part_rows + row;
+            *(float4*)(A.o_part + slot * D + d) = O;
+            if (d == 0) {
+              A.ml_part[slot * 2 + 0] = M;
+              A.ml_part[slot * 2 + 1] = L;
+            }
           }
         }
-      }
+      };
+      if (QREG || !TREE || done.lr == 0) merge(std::integral_constant<int, NW>{});
+      else if (done.lr == 1) merge(std::integral_constant<int, NW / 2>{});
+      else if (done.lr == 2) merge(std::integral_constant<int, NW / 4>{});
+      else merge(std::integral_constant<int, NW / 8>{});
       __syncthreads();
     }
     if (!QREG && cur.nrows > 0) {
