@@ -81,7 +81,8 @@ __device__ __forceinline__ float exp_bits(uint32_t byte) { return __uint_as_floa
 
 }  // namespace
 
-#define ORDER() __builtin_amdgcn_sched_barrier(0)
+#define ORDER() __builtin_amdgcn_sched_barrier(0)  // (keeps the loads and conversions where their registers are free)
+#define LAG 8.0f
 
 template <int D, int QT, bool KV8, bool TREE>
 __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const CacheAttnArgs A) {
@@ -301,43 +302,59 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
             for (int f = 0; f < KF; ++f) kf[a][f] = __builtin_bit_cast(lsk_bf16x8, kr[a * KF + f]);
           }
         }
-        lsk_bf16x8 pb[QT];
-        float alpha[QT];
+        // S^T = K Q^T: sacc[qt][a][e] <-> slot s0 + 4 a + e
+        lsk_f32x4 sacc[QT][2];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
-          ORDER();
-          // S^T = K Q^T: sacc[a][e] <-> slot s0 + 4 a + e
-          lsk_f32x4 sacc[2];
           lsk_bf16x8 qf[KF];
 #pragma unroll
           for (int f = 0; f < KF; ++f)
             qf[f] = QREG ? qreg[f] : *(const lsk_bf16x8*)(&s_q[rb + 16 * qt + l16][q_dim(f)]);
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
-            sacc[a] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
+            sacc[qt][a] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int f = 0; f < KF; ++f)
-              sacc[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a][f], qf[f], sacc[a], 0, 0, 0);
+              sacc[qt][a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a][f], qf[f], sacc[qt][a], 0, 0, 0);
           }
+        }
+        ORDER();
+        if (hv == HV - 1) load_k(sr, sb + stride);   // the next step's K streams in from here on
+        // The online softmax of each tile's 16 query columns.  A row's m only moves when a score passes it by more than
+        // LAG (weights up to 2^LAG; each row for itself, so the rows of a tile stay independent), which is seldom after
+        // the first step: then no maximum crosses lanes and nothing is rescaled.  Each lane sums its own slots' weights.
+        lsk_bf16x8 pb[QT];
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          ORDER();
           uint32_t reads = 0xffu;
           if constexpr (!FULL) reads = allow(qt, s0);
-          // the online softmax of the tile's 16 query columns
           float sv[8];
-          float mt = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            float sc = sacc[i >> 2][i & 3] * A.scale_log2;
-            if constexpr (!FULL) sc = (reads >> i) & 1u ? sc : -INFINITY;
-            sv[i] = sc;
-            mt = fmaxf(mt, sc);
+            sv[i] = sacc[qt][i >> 2][i & 3];
+            if constexpr (!FULL) sv[i] = (reads >> i) & 1u ? sv[i] : -INFINITY;
           }
-          mt = rows_max(mt);
-          const float m_new = fmaxf(m_run[qt], mt);
-          alpha[qt] = (m_new == m_run[qt]) ? 1.f : fast_exp2(m_run[qt] - m_new);
+          float mt = sv[0];
+#pragma unroll
+          for (int i = 1; i < 8; ++i) mt = fmaxf(mt, sv[i]);
+          mt *= A.scale_log2;
+          if (__builtin_amdgcn_ballot_w64(mt > m_run[qt] + LAG) != 0ull) {
+            mt = rows_max(mt);
+            const bool up = mt > m_run[qt] + LAG;
+            const float alpha = up ? fast_exp2(m_run[qt] - mt) : 1.f;
+            m_run[qt] = up ? mt : m_run[qt];
+            l_run[qt] *= alpha;
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) oacc[qt][c][i] *= alpha;
+          }
           float rs = 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float pe = (sv[i] == -INFINITY) ? 0.f : fast_exp2(sv[i] - m_new);
+            float pe = fast_exp2(__builtin_fmaf(sv[i], A.scale_log2, -m_run[qt]));
+            if constexpr (!FULL) pe = (reads >> i) & 1u ? pe : 0.f;
             rs += pe;
             float pv = pe;
             if constexpr (KV8) {
@@ -346,13 +363,10 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
             }
             pb[qt][i] = static_cast<__bf16>(pv);
           }
-          rs = rows_sum(rs);
-          l_run[qt] = l_run[qt] * alpha[qt] + rs;
-          m_run[qt] = m_new;
+          l_run[qt] += rs;
         }
         ORDER();
-        if (hv == HV - 1) load_k(sr, sb + stride);   // the next step's K streams in during this step's P V
-        // O^T = alpha O^T + V^T P^T
+        // O^T += V^T P^T
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
           if (c % 2 == 0) ORDER();
@@ -360,11 +374,8 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
           if constexpr (KV8) vf = codes_to_bf16(vr[c][2 * hv], vr[c][2 * hv + 1], 1.f);
           else vf = __builtin_bit_cast(lsk_bf16x8, vr[c]);
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) oacc[qt][c][i] *= alpha[qt];
+          for (int qt = 0; qt < QT; ++qt)
             oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pb[qt], oacc[qt][c], 0, 0, 0);
-          }
         }
       }
       if constexpr (!FULL) {
@@ -431,9 +442,10 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
       if (16 * p0 >= done.nrows) break;
 #pragma unroll
       for (int qt = p0; qt < p0 + MT && qt < QT; ++qt) {
+        const float l = rows_sum(l_run[qt]);
         if (lg == 0) {
           s_ml[wave][0][16 * qt + l16] = m_run[qt];
-          s_ml[wave][1][16 * qt + l16] = l_run[qt];
+          s_ml[wave][1][16 * qt + l16] = l;
         }
 #pragma unroll
         for (int c = 0; c < CT; ++c)
@@ -793,6 +805,7 @@ static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t
     a.ml_part = (float*)((char*)workspace +
                          lsk_align_up((size_t)n_parts * a.Hkv * a.part_rows * head_dim * sizeof(float), 256));
   }
+  LSK_REQUIRE(scale >= 0.f && scale <= 1e30f, LSK_EARG, "%s: scale %g (not negative)", what, (double)scale);
   a.scale_log2 = scale * 1.4426950408889634f;
 #define LSK_CACHE_ATTN(DD, QT, K8, TR) cache_attn_kernel<DD, QT, K8, TR><<<n_slots, 64 * ATTN_WAVES, 0, s>>>(a)
 #define LSK_CACHE_ATTN_D(K8, TR)                                            \
