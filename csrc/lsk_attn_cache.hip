@@ -88,6 +88,8 @@ template <int D, int QT, bool KV8, bool TREE>
 __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const CacheAttnArgs A) {
   constexpr int STEP = KV8 ? 64 : 32;                // positions per step of a wave
   constexpr int HV = STEP / 32;                      // 32-position halves of a step; a lane group has 8 slots of each
+  constexpr int NE = 8 * HV;                         // slots of a lane group: NE consecutive ones
+  constexpr uint32_t ALL = NE == 16 ? 0xffffu : 0xffu;
   constexpr int KF = D / 32;                         // K operands per 16-position tile
   constexpr int CT = D / 16;                         // 16-byte loads per lane of a step, for K and for V
   constexpr int NW = ATTN_WAVES;
@@ -196,14 +198,16 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
   };
   const int k_vo = 16 * lane, v_vo = 64 * l16 + 16 * lg;
   lsk_i32x4 kr[CT], vr[CT], ksr, vsr;                // this step's K and V as loaded
-  auto load_k = [&](const Stripe& s, int sb) {
+  constexpr int KL = CT / (2 * HV);                  // K loads of 16 slots
+  auto load_k = [&](const Stripe& s, int sb, int a) {
 #pragma unroll
-    for (int i = 0; i < CT; ++i) kr[i] = ld(s.k, k_vo, sb / STEP * 64 * D + i * 1024);
-    if constexpr (KV8) ksr = ld(s.ks, 16 * (l16 >> 2), sb);
+    for (int i = a * KL; i < (a + 1) * KL; ++i) kr[i] = ld(s.k, k_vo, sb / STEP * 64 * D + i * 1024);
+    if constexpr (KV8) {
+      if (a == 2 * HV - 1) ksr = ld(s.ks, 16 * (l16 >> 2), sb);
+    }
   };
-  auto load_v = [&](const Stripe& s, int sb) {
-#pragma unroll
-    for (int c = 0; c < CT; ++c) vr[c] = ld(s.v, v_vo, sb / STEP * 64 * D + c * 1024);
+  auto load_v = [&](const Stripe& s, int sb, int c) { vr[c] = ld(s.v, v_vo, sb / STEP * 64 * D + c * 1024); };
+  auto load_vs = [&](const Stripe& s, int sb) {
     if constexpr (KV8) vsr = ld(s.vs, 16 * lg, sb);
   };
   // a wave without rows starts past the stripe
@@ -213,8 +217,12 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
   auto issue_first = [&](const Item& it) {
     q_load(it);
     const Stripe s = stripe(it);
-    load_k(s, first_step(it));
-    load_v(s, first_step(it));
+    const int sb = first_step(it);
+#pragma unroll
+    for (int a = 0; a < 2 * HV; ++a) load_k(s, sb, a);
+    load_vs(s, sb);
+#pragma unroll
+    for (int c = 0; c < CT; ++c) load_v(s, sb, c);
   };
 
   Item cur = fetch(0);
@@ -246,184 +254,186 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
 #pragma unroll
       for (int c = 0; c < CT; ++c) oacc[qt][c] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    // bit e: row l16 of tile qt reads slot s0 + e
+    // bit e: row l16 of tile qt reads slot s0 + e, e < NE
     auto allow = [&](int qt, int s0) {
       const int n = min(kv_hi - 1, qpos[qt]) - s0 + 1;
-      uint32_t bits = n >= 8 ? 0xffu : n <= 0 ? 0u : (1u << n) - 1u;
+      uint32_t bits = n >= NE ? ALL : n <= 0 ? 0u : (1u << n) - 1u;
       if constexpr (TREE) {
         const int t = max(qpos[qt] - cur.pos0, 0);
         bits &= mask_window(A.mask + (long)(cur.q_start + t) * A.W, A.W, s0 - cur.pos0);
       }
       return bits;
     };
-    // One step: 32 slots (8 per lane group) at a time.  FULL: every row reads all of them.  All QT tiles are computed,
+    // One step.  FULL: every row reads all of its slots.  All QT tiles are computed,
     // also those without rows (copies of the loop for fewer tiles cost more in registers than they save).
     auto step = [&](auto full_, int sb) {
       constexpr bool FULL = decltype(full_)::value;
       // In a step that some row does not read whole, a slot whose V holds an infinity or NaN must not reach the rows
       // that do not read it (0 x NaN): the values past the item and the non-finite ones are cleared here, and the rows
       // that do read such a value get it after the products (below).
-      bool odd = false;
+      uint64_t odd = 0;                              // bit u: slot sb + u holds a non-finite value
       if constexpr (!FULL) {
-        constexpr int PER = 2 * HV;                  // slots of a dword
-        const int nk = kv_hi - (sb + 8 * HV * lg);   // slots of this lane that the item covers
-        uint32_t any = 0;
+        constexpr int PER = 2 * HV, BITS = 32 / PER; // slots of a dword, bits of a value
+        const int nk = kv_hi - (sb + NE * lg);       // slots of this lane that the item covers
+        uint32_t any[4];                             // the top bits of this lane's non-finite values
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int m = nk - PER * w;
-          const uint32_t keep = m >= PER ? 0xffffffffu : m <= 0 ? 0u : (1u << (32 / PER * m)) - 1u;
+          const uint32_t keep = m >= PER ? 0xffffffffu : m <= 0 ? 0u : (1u << (BITS * m)) - 1u;
+          any[w] = 0;
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
             const uint32_t x = (uint32_t)vr[c][w] & keep;
             const uint32_t nf = KV8 ? ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u
-                                    : ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;  // the top bits of its slots
-            vr[c][w] = (int)(x & ~((nf - (nf >> (KV8 ? 7 : 15))) | nf));
-            any |= nf;
+                                    : ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+            vr[c][w] = (int)(x & ~((nf - (nf >> (BITS - 1))) | nf));
+            any[w] |= nf;
           }
         }
-        odd = __builtin_amdgcn_ballot_w64(any != 0u) != 0ull;
+        if (__builtin_amdgcn_ballot_w64((any[0] | any[1] | any[2] | any[3]) != 0u) != 0ull) {
+#pragma unroll
+          for (int e = 0; e < NE; ++e) {
+            const uint64_t lanes = __builtin_amdgcn_ballot_w64((any[e / PER] >> (BITS * (e % PER) + BITS - 1)) & 1u);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) odd |= ((lanes >> (16 * g)) & 0xffffull) ? 1ull << (NE * g + e) : 0ull;
+          }
+        }
       }
+      // S^T = K Q^T, 16 slots at a time: sacc[qt][a][e] <-> slot s0 + 4 a + e.  The registers of a converted K take the
+      // next step's at once.
+      const int s0 = sb + NE * lg, sn = sb + stride;
+      lsk_f32x4 sacc[QT][2 * HV];
 #pragma unroll
-      for (int hv = 0; hv < HV; ++hv) {
-        const int s0 = sb + 8 * HV * lg + 8 * hv;    // this lane group's 8 slots
+      for (int a = 0; a < 2 * HV; ++a) {
         ORDER();
-        lsk_bf16x8 kf[2][KF];
+        lsk_bf16x8 kf[KF];
+        if constexpr (KV8) {
+          const float sc = exp_bits(((uint32_t)ksr[a] >> (8 * (l16 & 3))) & 255u);
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          if constexpr (KV8) {
-            const float sc = exp_bits(((uint32_t)ksr[2 * hv + a] >> (8 * (l16 & 3))) & 255u);
-#pragma unroll
-            for (int f = 0; f < KF; ++f) {
-              const lsk_i32x4 x = kr[(2 * hv + a) * (KF / 2) + (f >> 1)];
-              kf[a][f] = codes_to_bf16(x[2 * (f & 1)], x[2 * (f & 1) + 1], sc);
-            }
-          } else {
-#pragma unroll
-            for (int f = 0; f < KF; ++f) kf[a][f] = __builtin_bit_cast(lsk_bf16x8, kr[a * KF + f]);
+          for (int f = 0; f < KF; ++f) {
+            const lsk_i32x4 x = kr[a * (KF / 2) + (f >> 1)];
+            kf[f] = codes_to_bf16(x[2 * (f & 1)], x[2 * (f & 1) + 1], sc);
           }
-        }
-        // S^T = K Q^T: sacc[qt][a][e] <-> slot s0 + 4 a + e
-        lsk_f32x4 sacc[QT][2];
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-          lsk_bf16x8 qf[KF];
-#pragma unroll
-          for (int f = 0; f < KF; ++f)
-            qf[f] = QREG ? qreg[f] : *(const lsk_bf16x8*)(&s_q[rb + 16 * qt + l16][q_dim(f)]);
-#pragma unroll
-          for (int a = 0; a < 2; ++a) {
-            sacc[qt][a] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int f = 0; f < KF; ++f)
-              sacc[qt][a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a][f], qf[f], sacc[qt][a], 0, 0, 0);
-          }
-        }
-        ORDER();
-        if (hv == HV - 1) load_k(sr, sb + stride);   // the next step's K streams in from here on
-        // The online softmax of each tile's 16 query columns.  A row's m only moves when a score passes it by more than
-        // LAG (weights up to 2^LAG; each row for itself, so the rows of a tile stay independent), which is seldom after
-        // the first step: then no maximum crosses lanes and nothing is rescaled.  Each lane sums its own slots' weights.
-        lsk_bf16x8 pb[QT];
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
           ORDER();
-          uint32_t reads = 0xffu;
-          if constexpr (!FULL) reads = allow(qt, s0);
-          float sv[8];
+          load_k(sr, sn, a);
+        } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            sv[i] = sacc[qt][i >> 2][i & 3];
-            if constexpr (!FULL) sv[i] = (reads >> i) & 1u ? sv[i] : -INFINITY;
-          }
-          float mt = sv[0];
-#pragma unroll
-          for (int i = 1; i < 8; ++i) mt = fmaxf(mt, sv[i]);
-          mt *= A.scale_log2;
-          if (__builtin_amdgcn_ballot_w64(mt > m_run[qt] + LAG) != 0ull) {
-            mt = rows_max(mt);
-            const bool up = mt > m_run[qt] + LAG;
-            const float alpha = up ? fast_exp2(m_run[qt] - mt) : 1.f;
-            m_run[qt] = up ? mt : m_run[qt];
-            l_run[qt] *= alpha;
-#pragma unroll
-            for (int c = 0; c < CT; ++c)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) oacc[qt][c][i] *= alpha;
-          }
-          float rs = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float pe = fast_exp2(__builtin_fmaf(sv[i], A.scale_log2, -m_run[qt]));
-            if constexpr (!FULL) pe = (reads >> i) & 1u ? pe : 0.f;
-            rs += pe;
-            float pv = pe;
-            if constexpr (KV8) {
-              pv = pe * exp_bits(((uint32_t)vsr[2 * hv + (i >> 2)] >> (8 * (i & 3))) & 255u);
-              if constexpr (!FULL) pv = (reads >> i) & 1u ? pv : 0.f;  // (a slot never written: any exponent)
-            }
-            pb[qt][i] = static_cast<__bf16>(pv);
-          }
-          l_run[qt] += rs;
+          for (int f = 0; f < KF; ++f) kf[f] = __builtin_bit_cast(lsk_bf16x8, kr[a * KF + f]);
         }
-        ORDER();
-        // O^T += V^T P^T
 #pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          if (c % 2 == 0) ORDER();
-          lsk_bf16x8 vf;
-          if constexpr (KV8) vf = codes_to_bf16(vr[c][2 * hv], vr[c][2 * hv + 1], 1.f);
-          else vf = __builtin_bit_cast(lsk_bf16x8, vr[c]);
+        for (int qt = 0; qt < QT; ++qt) {
+          lsk_f32x4 acc = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int f = 0; f < KF; ++f) {
+            const lsk_bf16x8 qf =
+                QREG ? qreg[f] : *(const lsk_bf16x8*)(&s_q[rb + 16 * qt + l16][q_dim(f)]);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[f], qf, acc, 0, 0, 0);
+          }
+          sacc[qt][a] = acc;
+        }
+      }
+      ORDER();
+      if constexpr (!KV8) {
+#pragma unroll
+        for (int a = 0; a < 2 * HV; ++a) load_k(sr, sn, a);
+      }
+      // The online softmax of each tile's 16 query columns.  A row's m only moves when a score passes it by more than
+      // LAG (weights up to 2^LAG; each row for itself, so the rows of a tile stay independent), which is seldom after
+      // the first step: then no maximum crosses lanes and nothing is rescaled.  Each lane sums its own slots' weights.
+      lsk_bf16x8 pb[QT][HV];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        ORDER();
+        uint32_t reads = ALL;
+        if constexpr (!FULL) reads = allow(qt, s0);
+        float mt = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+          if constexpr (!FULL) sacc[qt][i >> 2][i & 3] = (reads >> i) & 1u ? sacc[qt][i >> 2][i & 3] : -INFINITY;
+          mt = fmaxf(mt, sacc[qt][i >> 2][i & 3]);
+        }
+        mt *= A.scale_log2;
+        if (__builtin_amdgcn_ballot_w64(mt > m_run[qt] + LAG) != 0ull) {
+          mt = rows_max(mt);
+          const bool up = mt > m_run[qt] + LAG;
+          const float alpha = up ? fast_exp2(m_run[qt] - mt) : 1.f;
+          m_run[qt] = up ? mt : m_run[qt];
+          l_run[qt] *= alpha;
+#pragma unroll
+          for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) oacc[qt][c][i] *= alpha;
+        }
+        float rs = 0.f;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+          float pe = fast_exp2(__builtin_fmaf(sacc[qt][i >> 2][i & 3], A.scale_log2, -m_run[qt]));
+          if constexpr (!FULL) pe = (reads >> i) & 1u ? pe : 0.f;
+          rs += pe;
+          float pv = pe;
+          if constexpr (KV8) {
+            pv = pe * exp_bits(((uint32_t)vsr[i >> 2] >> (8 * (i & 3))) & 255u);
+            if constexpr (!FULL) pv = (reads >> i) & 1u ? pv : 0.f;  // (a slot never written: any exponent)
+          }
+          pb[qt][i >> 3][i & 7] = static_cast<__bf16>(pv);
+        }
+        l_run[qt] += rs;
+      }
+      ORDER();
+      load_vs(sr, sn);
+      // O^T += V^T P^T; V's registers take the next step's V one by one
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        lsk_bf16x8 vf[HV];
+        if constexpr (KV8) {
+#pragma unroll
+          for (int hv = 0; hv < HV; ++hv) vf[hv] = codes_to_bf16(vr[c][2 * hv], vr[c][2 * hv + 1], 1.f);
+        } else {
+          vf[0] = __builtin_bit_cast(lsk_bf16x8, vr[c]);
+        }
+#pragma unroll
+        for (int hv = 0; hv < HV; ++hv)
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt)
-            oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pb[qt], oacc[qt][c], 0, 0, 0);
-        }
+            oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[hv], pb[qt][hv], oacc[qt][c], 0, 0, 0);
+        load_v(sr, sn, c);
+        ORDER();
       }
       if constexpr (!FULL) {
-        if (odd) {
-          // V again, as a count of its non-finite values (cnt) and their kind (sgn: +-1 for +-inf, 2^20 for NaN): of
-          // those that a row reads, one kind of infinity gives that infinity, anything else NaN.
-#pragma unroll 1
-          for (int hv = 0; hv < HV; ++hv)
+        while (odd != 0ull) {                        // (rare: one slot after the other, few registers)
+          const int u = __builtin_ctzll(odd), kp = sb + u;
+          odd &= odd - 1;
+          bool reads[QT];
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-              const uint32_t reads = allow(qt, sb + 8 * HV * lg + 8 * hv);
-              lsk_bf16x8 rd;
+          for (int qt = 0; qt < QT; ++qt) {
+            reads[qt] = kp <= qpos[qt];
+            if constexpr (TREE) {
+              const int t = max(qpos[qt] - cur.pos0, 0);
+              reads[qt] = reads[qt] &&
+                          (mask_window(A.mask + (long)(cur.q_start + t) * A.W, A.W, kp - cur.pos0) & 1u);
+            }
+          }
 #pragma unroll
-              for (int e = 0; e < 8; ++e) rd[e] = static_cast<__bf16>((float)((reads >> e) & 1u));
+          for (int c = 0; c < CT; ++c)
 #pragma unroll
-              for (int c = 0; c < CT; ++c) {
-                ORDER();
-                const lsk_i32x4 x = ld(sr.v, v_vo, sb / STEP * 64 * D + c * 1024);
-                lsk_bf16x8 cnt, sgn;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  bool nf, nan, neg;
-                  if constexpr (KV8) {
-                    const uint32_t u = (uint32_t)(hv ? x[2 + e / 4] : x[e / 4]) >> (8 * (e & 3));
-                    nf = nan = (u & 0x7fu) == 0x7fu;
-                    neg = false;
-                  } else {
-                    const uint32_t u = (uint32_t)x[e / 2] >> (16 * (e & 1));
-                    nf = (u & 0x7f80u) == 0x7f80u;
-                    nan = nf && (u & 0x7fu) != 0u;
-                    neg = (u & 0x8000u) != 0u;
-                  }
-                  cnt[e] = static_cast<__bf16>(nf ? 1.f : 0.f);
-                  sgn[e] = static_cast<__bf16>(!nf ? 0.f : nan ? 1048576.f : neg ? -1.f : 1.f);
-                }
-                const lsk_f32x4 z = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
-                const lsk_f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cnt, rd, z, 0, 0, 0);
-                const lsk_f32x4 s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sgn, rd, z, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float add = s[i] == n[i] ? INFINITY : s[i] == -n[i] ? -INFINITY : __builtin_nanf("");
-                  oacc[qt][c][i] = n[i] > 0.f ? oacc[qt][c][i] + add : oacc[qt][c][i];
-                }
+            for (int i = 0; i < 4; ++i) {
+              ORDER();
+              // V[kp][16 c + 4 lg + i]: a dim's slots of a block are 64 bytes in both formats
+              const int so = sb / STEP * 64 * D + (16 * c + i) * 64 + u * (KV8 ? 1 : 2);
+              float x;
+              if constexpr (KV8) {
+                const uint32_t b = __builtin_amdgcn_raw_buffer_load_b8(sr.v, 256 * lg, so, 0);
+                x = (b & 0x7fu) == 0x7fu ? __builtin_nanf("") : 0.f;
+              } else {
+                x = bf2f((uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr.v, 256 * lg, so, 0));
+                x = (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? x : 0.f;
               }
+#pragma unroll
+              for (int qt = 0; qt < QT; ++qt)
+                if (reads[qt]) oacc[qt][c][i] += x;
             }
         }
       }
-      load_v(sr, sb + stride);
     };
     int sb = first_step(cur);
     for (; sb + STEP - 1 <= full_lim; sb += stride) step(std::true_type{}, sb);
@@ -437,26 +447,29 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
     }
     // merge a row group's waves in order: M = max m_w, e_w = exp2(m_w - M), L = sum e_w l_w, O = sum e_w O_w
     if (!QREG) __syncthreads();                      // every wave is past its reads of Q
+    int tm = tid;
+    asm volatile("" : "+v"(tm));                     // (no address of the merge is kept in registers across the steps)
+    const int m16 = tm & 15, mg = (tm & 63) >> 4;
 #pragma unroll
     for (int p0 = 0; p0 < QT; p0 += MT) {
       if (16 * p0 >= done.nrows) break;
 #pragma unroll
       for (int qt = p0; qt < p0 + MT && qt < QT; ++qt) {
         const float l = rows_sum(l_run[qt]);
-        if (lg == 0) {
-          s_ml[wave][0][16 * qt + l16] = m_run[qt];
-          s_ml[wave][1][16 * qt + l16] = l;
+        if (mg == 0) {
+          s_ml[wave][0][16 * qt + m16] = m_run[qt];
+          s_ml[wave][1][16 * qt + m16] = l;
         }
 #pragma unroll
         for (int c = 0; c < CT; ++c)
-          *(float4*)(&s_o[wave][16 * (qt - p0) + l16][16 * c + 4 * lg]) =
+          *(float4*)(&s_o[wave][16 * (qt - p0) + m16][16 * c + 4 * mg]) =
               make_float4(oacc[qt][c][0], oacc[qt][c][1], oacc[qt][c][2], oacc[qt][c][3]);
       }
       __syncthreads();
       // 4 consecutive d of one row per thread; RANKS waves hold a part of it
       auto merge = [&](auto ranks_) {
         constexpr int RANKS = decltype(ranks_)::value, NR = NW / RANKS;
-        for (int e = tid; e < NR * MR * (D / 4); e += 64 * NW) {
+        for (int e = tm; e < NR * MR * (D / 4); e += 64 * NW) {
           const int x = e / (D / 4), d = 4 * (e - x * (D / 4));
           const int rg = x / MR, ql = x - rg * MR, qr = 16 * p0 + ql;  // row group, row of the pass, row of the group
           const int row = rg * GR + qr;                                // row of the item
