@@ -105,11 +105,14 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
   // few per workgroup: theirs is fetched after it)
   constexpr bool QAHEAD = !TREE;
   constexpr int O_BYTES = NW * MR * (D + 4) * 4, Q_BYTES = QROWS * QLD * 2;
-  // Q is in LDS during an item's steps, the waves' partial outputs during its merge: one buffer holds both in turn
-  __shared__ __attribute__((aligned(16))) char s_buf[O_BYTES > Q_BYTES ? O_BYTES : Q_BYTES];
+  // Q is in LDS during an item's steps, the waves' partial outputs during its merge.  A tree's (up to 256 rows) share one
+  // buffer in turn; else there is room for both, which saves two barriers an item.
+  constexpr bool SHARED = TREE && !QREG;
+  __shared__ __attribute__((aligned(16))) char s_buf[SHARED && Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
+  __shared__ __attribute__((aligned(16))) char s_qbuf[SHARED || QREG ? 16 : Q_BYTES];
   __shared__ float s_ml[NW][2][GR];
   float (*s_o)[MR][D + 4] = (float (*)[MR][D + 4])s_buf;
-  uint16_t (*s_q)[QLD] = (uint16_t (*)[QLD])s_buf;
+  uint16_t (*s_q)[QLD] = (uint16_t (*)[QLD])(SHARED ? s_buf : s_qbuf);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -446,7 +449,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
       nxt = fetch(r + 2);
     }
     // merge a row group's waves in order: M = max m_w, e_w = exp2(m_w - M), L = sum e_w l_w, O = sum e_w O_w
-    if (!QREG) __syncthreads();                      // every wave is past its reads of Q
+    if (SHARED) __syncthreads();                     // every wave is past its reads of Q
     int tm = tid;
     asm volatile("" : "+v"(tm));                     // (no address of the merge is kept in registers across the steps)
     const int m16 = tm & 15, mg = (tm & 63) >> 4;
@@ -460,10 +463,12 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
           s_ml[wave][0][16 * qt + m16] = m_run[qt];
           s_ml[wave][1][16 * qt + m16] = l;
         }
+        if (16 * qt < done.nrows - rb) {             // (a tile with rows)
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
-          *(float4*)(&s_o[wave][16 * (qt - p0) + m16][16 * c + 4 * mg]) =
-              make_float4(oacc[qt][c][0], oacc[qt][c][1], oacc[qt][c][2], oacc[qt][c][3]);
+          for (int c = 0; c < CT; ++c)
+            *(float4*)(&s_o[wave][16 * (qt - p0) + m16][16 * c + 4 * mg]) =
+                make_float4(oacc[qt][c][0], oacc[qt][c][1], oacc[qt][c][2], oacc[qt][c][3]);
+        }
       }
       __syncthreads();
       // 4 consecutive d of one row per thread; RANKS waves hold a part of it
@@ -512,9 +517,10 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
       else if (done.lr == 1) merge(std::integral_constant<int, NW / 2>{});
       else if (done.lr == 2) merge(std::integral_constant<int, NW / 4>{});
       else merge(std::integral_constant<int, NW / 8>{});
+      if (!SHARED && p0 == 0 && cur.nrows > 0) q_store(cur);  // (every wave is past its steps)
       __syncthreads();
     }
-    if (!QREG && cur.nrows > 0) {
+    if (SHARED && cur.nrows > 0) {
       q_store(cur);
       __syncthreads();
     }
