@@ -305,10 +305,13 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
       // S^T = K Q^T, 16 slots at a time: sacc[qt][a][e] <-> slot s0 + 4 a + e.  The registers of a converted K take the
       // next step's at once.
       const int s0 = sb + NE * lg, sn = sb + stride;
+      uint32_t reads[QT];                            // (the mask's words are asked for before the products)
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) reads[qt] = FULL ? ALL : allow(qt, s0);
       lsk_f32x4 sacc[QT][2 * HV];
 #pragma unroll
       for (int a = 0; a < 2 * HV; ++a) {
-        ORDER();
+        if constexpr (KV8) ORDER();
         lsk_bf16x8 kf[KF];
         if constexpr (KV8) {
           const float sc = exp_bits(((uint32_t)ksr[a] >> (8 * (l16 & 3))) & 255u);
@@ -346,13 +349,11 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
       lsk_bf16x8 pb[QT][HV];
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
-        ORDER();
-        uint32_t reads = ALL;
-        if constexpr (!FULL) reads = allow(qt, s0);
+        if constexpr (KV8) ORDER();
         float mt = -INFINITY;
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
-          if constexpr (!FULL) sacc[qt][i >> 2][i & 3] = (reads >> i) & 1u ? sacc[qt][i >> 2][i & 3] : -INFINITY;
+          if constexpr (!FULL) sacc[qt][i >> 2][i & 3] = (reads[qt] >> i) & 1u ? sacc[qt][i >> 2][i & 3] : -INFINITY;
           mt = fmaxf(mt, sacc[qt][i >> 2][i & 3]);
         }
         mt *= A.scale_log2;
@@ -371,12 +372,12 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
           float pe = fast_exp2(__builtin_fmaf(sacc[qt][i >> 2][i & 3], A.scale_log2, -m_run[qt]));
-          if constexpr (!FULL) pe = (reads >> i) & 1u ? pe : 0.f;
+          if constexpr (!FULL) pe = (reads[qt] >> i) & 1u ? pe : 0.f;
           rs += pe;
           float pv = pe;
           if constexpr (KV8) {
             pv = pe * exp_bits(((uint32_t)vsr[i >> 2] >> (8 * (i & 3))) & 255u);
-            if constexpr (!FULL) pv = (reads >> i) & 1u ? pv : 0.f;  // (a slot never written: any exponent)
+            if constexpr (!FULL) pv = (reads[qt] >> i) & 1u ? pv : 0.f;  // (a slot never written: any exponent)
           }
           pb[qt][i >> 3][i & 7] = static_cast<__bf16>(pv);
         }
@@ -406,14 +407,13 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
         while (odd != 0ull) {                        // (rare: one slot after the other, few registers)
           const int u = __builtin_ctzll(odd), kp = sb + u;
           odd &= odd - 1;
-          bool reads[QT];
+          bool hit[QT];
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) {
-            reads[qt] = kp <= qpos[qt];
+            hit[qt] = kp <= qpos[qt];
             if constexpr (TREE) {
               const int t = max(qpos[qt] - cur.pos0, 0);
-              reads[qt] = reads[qt] &&
-                          (mask_window(A.mask + (long)(cur.q_start + t) * A.W, A.W, kp - cur.pos0) & 1u);
+              hit[qt] = hit[qt] && (mask_window(A.mask + (long)(cur.q_start + t) * A.W, A.W, kp - cur.pos0) & 1u);
             }
           }
 #pragma unroll
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
               }
 #pragma unroll
               for (int qt = 0; qt < QT; ++qt)
-                if (reads[qt]) oacc[qt][c][i] += x;
+                if (hit[qt]) oacc[qt][c][i] += x;
             }
         }
       }
@@ -449,13 +449,44 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
       nxt = fetch(r + 2);
     }
     // merge a row group's waves in order: M = max m_w, e_w = exp2(m_w - M), L = sum e_w l_w, O = sum e_w O_w
+    // (a wave that has its rows to itself writes them out as they are)
+    const bool alone = SHARED && (NW >> done.lr) == 1;
+    if (alone) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        const float l = rows_sum(l_run[qt]);
+        const int row = rb + 16 * qt + l16;
+        if (row < done.nrows) {
+          const int rr = done.row0 + row, tt = rr / G, gg = rr - tt * G;
+          const float L = l == 0.f ? 1.f : l;
+          const long slot = ((long)done.part * Hkv + done.kvh) * A.part_rows + row;
+          uint16_t* o = A.out + ((long)(done.q_start + tt) * Hq + done.kvh * G + gg) * D + 4 * lg;
+#pragma unroll
+          for (int c = 0; c < CT; ++c) {
+            const lsk_f32x4 v = oacc[qt][c];
+            if (done.part < 0) {
+              lsk_u32x2_u pk;
+              pk[0] = (uint32_t)f2bf(v[0] / L) | ((uint32_t)f2bf(v[1] / L) << 16);
+              pk[1] = (uint32_t)f2bf(v[2] / L) | ((uint32_t)f2bf(v[3] / L) << 16);
+              *(lsk_u32x2_u*)(o + 16 * c) = pk;
+            } else {
+              *(lsk_f32x4*)(A.o_part + slot * D + 16 * c + 4 * lg) = v;
+            }
+          }
+          if (done.part >= 0 && lg == 0) {
+            A.ml_part[slot * 2 + 0] = m_run[qt];
+            A.ml_part[slot * 2 + 1] = l;
+          }
+        }
+      }
+    }
     if (SHARED) __syncthreads();                     // every wave is past its reads of Q
     int tm = tid;
     asm volatile("" : "+v"(tm));                     // (no address of the merge is kept in registers across the steps)
     const int m16 = tm & 15, mg = (tm & 63) >> 4;
 #pragma unroll
     for (int p0 = 0; p0 < QT; p0 += MT) {
-      if (16 * p0 >= done.nrows) break;
+      if (alone || 16 * p0 >= done.nrows) break;
 #pragma unroll
       for (int qt = p0; qt < p0 + MT && qt < QT; ++qt) {
         const float l = rows_sum(l_run[qt]);
@@ -515,8 +546,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
       };
       if (QREG || !TREE || done.lr == 0) merge(std::integral_constant<int, NW>{});
       else if (done.lr == 1) merge(std::integral_constant<int, NW / 2>{});
-      else if (done.lr == 2) merge(std::integral_constant<int, NW / 4>{});
-      else merge(std::integral_constant<int, NW / 8>{});
+      else merge(std::integral_constant<int, NW / 4>{});
       if (!SHARED && p0 == 0 && cur.nrows > 0) q_store(cur);  // (every wave is past its steps)
       __syncthreads();
     }
