@@ -50,14 +50,101 @@ __device__ __forceinline__ void values4(uint32_t c, float scale, float* o) {
   o[0] = a[0] * scale; o[1] = a[1] * scale; o[2] = b[0] * scale; o[3] = b[1] * scale;
 }
 
-#define KV8_TOKENS 16  // tokens of a workgroup: 16 threads each
+// 4 consecutive elements at any address that aligns one of them
+__device__ __forceinline__ void load4(const uint16_t* p, float* x) {
+  const lsk_u32x2_u u = *(const lsk_u32x2_u*)p;
+  x[0] = __uint_as_float(u[0] << 16); x[1] = __uint_as_float(u[0] & 0xffff0000u);
+  x[2] = __uint_as_float(u[1] << 16); x[3] = __uint_as_float(u[1] & 0xffff0000u);
+}
+__device__ __forceinline__ void load4(const float* p, float* x) {
+  const lsk_f32x4_u u = *(const lsk_f32x4_u*)p;
+  x[0] = u[0]; x[1] = u[1]; x[2] = u[2]; x[3] = u[3];
+}
+__device__ __forceinline__ void store4(uint16_t* p, const float* x) {
+  lsk_u32x2_u u;
+  u[0] = (uint32_t)f2bf(x[0]) | ((uint32_t)f2bf(x[1]) << 16);
+  u[1] = (uint32_t)f2bf(x[2]) | ((uint32_t)f2bf(x[3]) << 16);
+  *(lsk_u32x2_u*)p = u;
+}
+__device__ __forceinline__ void store4(float* p, const float* x) { *(lsk_f32x4_u*)p = (lsk_f32x4_u){x[0], x[1], x[2], x[3]}; }
+
+// Four dwords of four bytes, turned: byte j of a[i] <-> byte i of a[j]
+__device__ __forceinline__ void turn4(uint32_t* a) {
+  const uint32_t l0 = __builtin_amdgcn_perm(a[1], a[0], 0x05010400), h0 = __builtin_amdgcn_perm(a[1], a[0], 0x07030602);
+  const uint32_t l1 = __builtin_amdgcn_perm(a[3], a[2], 0x05010400), h1 = __builtin_amdgcn_perm(a[3], a[2], 0x07030602);
+  a[0] = __builtin_amdgcn_perm(l1, l0, 0x05040100);
+  a[1] = __builtin_amdgcn_perm(l1, l0, 0x07060302);
+  a[2] = __builtin_amdgcn_perm(h1, h0, 0x05040100);
+  a[3] = __builtin_amdgcn_perm(h1, h0, 0x07060302);
+}
+
+// the largest finite magnitude (bits) of the vector that 16 threads hold
+template <int PER>
+__device__ __forceinline__ uint32_t vector_max(const float* x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
+    m = u < 0x7f800000u && u > m ? u : m;
+  }
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) {
+    const uint32_t y = (uint32_t)__shfl_xor((int)m, o, 16);
+    m = y > m ? y : m;
+  }
+  return m;
+}
+
 #define KV8_THREADS 256
+#define KV8_TOKENS 64  // tokens of a workgroup of V, and of four workgroups of K: 16 threads hold a token's vector
+#define KV8_LD 17      // dwords of a dim's row of the V tile in LDS (64 tokens from any position: 17 dwords of slots)
+
+// Whether the V workgroup's nt tokens are a run of one cache row (consecutive positions, inside the cache), from every
+// wave's own look at them.
+__device__ __forceinline__ bool kv8_run(const int32_t* rows, const int32_t* pos, int t0, int nt, int max_batch, int S) {
+  const int l = threadIdx.x & 63, i = min(l, nt - 1);
+  const int r = rows[t0 + i], p = pos[t0 + i];
+  const int r0 = __shfl(r, 0, 64), p0 = __shfl(p, 0, 64);
+  const bool ok = r >= 0 && r < max_batch && p >= 0 && p < S && r == r0 &&
+                  (uint32_t)p - (uint32_t)p0 == (uint32_t)i;
+  return __builtin_amdgcn_ballot_w64(ok) == ~0ull;
+}
+
+// A workgroup's tokens one by one: f(d, token, address of its byte in the V codes), lanes side by side over the tokens.
+template <int D, typename F>
+__device__ __forceinline__ void kv8_each(const int32_t* rows, const int32_t* pos, int t0, int nt, int h, int Hkv,
+                                         int max_batch, int S, F f) {
+  const int lg = nt > 1 ? 32 - __builtin_clz(nt - 1) : 0;              // 2^lg >= nt
+  const int tj = threadIdx.x & ((1 << lg) - 1);
+  if (tj >= nt) return;
+  const int r = rows[t0 + tj], p = pos[t0 + tj];
+  if (r < 0 || r >= max_batch || p < 0 || p >= S) return;
+  const long at = ((long)r * Hkv + h) * (long)S * D + (long)(p >> 6) * 64 * D + (p & 63);
+  for (int d = threadIdx.x >> lg; d < D; d += KV8_THREADS >> lg) f(d, tj, at + d * 64);
+}
+
+// A run's dwords of V codes: f(d, its index in the LDS row, address), over the 64-position blocks that it touches.
+template <int D, typename F>
+__device__ __forceinline__ void kv8_dwords(long stripe, int p0, int nt, F f) {
+  const int q0 = p0 & ~3, n = (p0 + nt - q0 + 3) >> 2;                 // <= 17
+  for (int i = threadIdx.x; i < D * 16; i += KV8_THREADS) {
+    const int d = i >> 4, w = i & 15, q = q0 + 4 * w;
+    if (w < n) f(d, w, stripe * D + (long)(q >> 6) * 64 * D + d * 64 + (q & 63));
+  }
+  if (n == 17 && threadIdx.x < D) {
+    const int d = threadIdx.x, q = q0 + 64;
+    f(d, 16, stripe * D + (long)(q >> 6) * 64 * D + d * 64 + (q & 63));
+  }
+}
 
 }  // namespace
 
-// A workgroup quantises 16 tokens of one KV head, K then V; 16 threads hold a token's vector, D / 16 consecutive
-// elements each, and find its largest magnitude by shuffles.  K goes straight to its place; V is turned in LDS so that
-// a dim's positions land side by side.
+// Workgroups 0 .. 3 of blockIdx.z quantise 16 tokens of one KV head's K each, workgroup 4 the 64 tokens' V.  16 threads
+// hold a token's vector, D / 16 consecutive elements each, and find its largest magnitude by shuffles.  K goes straight
+// to its place.  V is turned, 4 x 4 in registers and the rest in LDS: a run of positions (a prompt's tokens) is written
+// a dword at a time, whole 64-byte sectors from one workgroup; other tokens byte by byte.
+// Latency-bound for a decode step's tokens; a long prompt moves 3 D bytes a token and head (4001 tokens of 8 heads of
+// 128: 13.4 us; with 16 tokens to every workgroup, so that four share a sector of V, 16.9; bytes alone 18.6).
 template <typename T, int D>
 __global__ __launch_bounds__(KV8_THREADS) void kv8_append_kernel(const T* __restrict__ k, const T* __restrict__ v,
                                                                  long st_t, long st_h, uint8_t* __restrict__ kc,
@@ -67,50 +154,77 @@ __global__ __launch_bounds__(KV8_THREADS) void kv8_append_kernel(const T* __rest
                                                                  const int32_t* __restrict__ pos, int N, int Hkv,
                                                                  int max_batch, int S) {
   constexpr int PER = D / 16;
-  __shared__ uint8_t s_v[KV8_TOKENS][D + 4];
-  const int t0 = blockIdx.x * KV8_TOKENS, h = blockIdx.y;
-  const int j = threadIdx.x >> 4, part = threadIdx.x & 15;
-  const int t = t0 + j;
-  const int row = t < N ? rows[t] : -1, p = t < N ? pos[t] : -1;
-  const bool ok = row >= 0 && row < max_batch && p >= 0 && p < S;
-  const long stripe = ((long)row * Hkv + h) * (long)S;
-#pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
+  __shared__ uint32_t s_v[D * KV8_LD];
+  const int h = blockIdx.y, j = threadIdx.x >> 4, part = threadIdx.x & 15;
+  if (blockIdx.z < 4) {
+    const int t = blockIdx.x * KV8_TOKENS + blockIdx.z * 16 + j;
+    if (t >= N) return;                              // (16 threads at a time)
     float x[PER];
-    uint32_t m = 0;
+    const T* src = k + (long)t * st_t + (long)h * st_h + part * PER;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      x[i] = ok ? Elem<T>::ld((kv ? v : k) + (long)t * st_t + (long)h * st_h + part * PER + i) : 0.f;
-      const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
-      m = u < 0x7f800000u && u > m ? u : m;
-    }
-#pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) {
-      const uint32_t y = (uint32_t)__shfl_xor((int)m, o, 16);
-      m = y > m ? y : m;
-    }
-    const int e = biased_exponent(m);
+    for (int i = 0; i < PER; i += 4) load4(src + i, x + i);
+    const int row = rows[t], p = pos[t];
+    const int e = biased_exponent(vector_max<PER>(x));
     const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
-    if (ok) {
-      if (part == 0) (kv ? vs : ks)[stripe + p] = (uint8_t)e;
+    if (row < 0 || row >= max_batch || p < 0 || p >= S) return;
+    const long stripe = ((long)row * Hkv + h) * (long)S;
+    uint32_t* dst = (uint32_t*)(kc + stripe * D + kv8_k_offset(p, part * PER, D));
 #pragma unroll
-      for (int i = 0; i < PER; i += 4) {
-        const uint32_t c = codes4(x + i, inv);
-        if (kv == 0) *(uint32_t*)(kc + stripe * D + kv8_k_offset(p, part * PER + i, D)) = c;
-        else *(uint32_t*)(&s_v[j][part * PER + i]) = c;
-      }
+    for (int i = 0; i < PER / 4; ++i) dst[i] = codes4(x + 4 * i, inv);
+    if (part == 0) ks[stripe + p] = (uint8_t)e;
+    return;
+  }
+  const int t0 = blockIdx.x * KV8_TOKENS, nt = min(KV8_TOKENS, N - t0);
+  float x[4][PER];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int tj = min(4 * j + c, nt - 1);           // (tokens behind the last one: its copies, never written)
+    const T* src = v + (long)(t0 + tj) * st_t + (long)h * st_h + part * PER;
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) load4(src + i, &x[c][i]);
+  }
+  uint32_t w[PER / 4][4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int e = biased_exponent(vector_max<PER>(x[c]));
+    const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < PER / 4; ++i) w[i][c] = codes4(&x[c][4 * i], inv);
+    if (part == 0 && 4 * j + c < nt) {
+      const int row = rows[t0 + 4 * j + c], p = pos[t0 + 4 * j + c];
+      if (row >= 0 && row < max_batch && p >= 0 && p < S) vs[((long)row * Hkv + h) * (long)S + p] = (uint8_t)e;
     }
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < KV8_TOKENS * D; i += KV8_THREADS) {
-    const int tj = i % KV8_TOKENS, d = i / KV8_TOKENS, tt = t0 + tj;
-    if (tt >= N) continue;
-    const int r = rows[tt], pp = pos[tt];
-    if (r < 0 || r >= max_batch || pp < 0 || pp >= S) continue;
-    vc[((long)r * Hkv + h) * (long)S * D + (long)(pp >> 6) * 64 * D + d * 64 + (pp & 63)] = s_v[tj][d];
+#pragma unroll
+  for (int i = 0; i < PER / 4; ++i) {
+    turn4(w[i]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s_v[(part * PER + 4 * i + c) * KV8_LD + j] = w[i][c];
   }
+  const bool run = kv8_run(rows, pos, t0, nt, max_batch, S);
+  __syncthreads();
+  if (!run) {
+    kv8_each<D>(rows, pos, t0, nt, h, Hkv, max_batch, S, [&](int d, int tj, long at) {
+      vc[at] = (uint8_t)(s_v[d * KV8_LD + (tj >> 2)] >> (8 * (tj & 3)));
+    });
+    return;
+  }
+  const int p0 = pos[t0], sh = p0 & 3;
+  kv8_dwords<D>(((long)rows[t0] * Hkv + h) * (long)S, p0, nt, [&](int d, int i, long at) {
+    const uint32_t* r = s_v + d * KV8_LD;            // slots 4 i .. + 3 of the run's: tokens 4 i - sh .. + 3
+    const uint32_t u = sh == 0 ? r[i] : __builtin_amdgcn_alignbyte(r[i], r[max(i - 1, 0)], 4 - sh);
+    const int tj = 4 * i - sh;
+    if (tj >= 0 && tj + 3 < nt) {
+      *(uint32_t*)(vc + at) = u;
+    } else {
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (tj + b >= 0 && tj + b < nt) vc[at + b] = (uint8_t)(u >> (8 * b));
+    }
+  });
 }
 
+// The way back, in the same shape (4001 tokens of 8 heads of 128: 11.2 us; 12.7 with 16 tokens to a workgroup).
 template <typename T, int D>
 __global__ __launch_bounds__(KV8_THREADS) void kv8_read_kernel(const uint8_t* __restrict__ kc,
                                                                const uint8_t* __restrict__ vc,
@@ -121,37 +235,61 @@ __global__ __launch_bounds__(KV8_THREADS) void kv8_read_kernel(const uint8_t* __
                                                                T* __restrict__ v, int N, int Hkv, int max_batch,
                                                                int S) {
   constexpr int PER = D / 16;
-  __shared__ uint8_t s_v[KV8_TOKENS][D + 4];
-  const int t0 = blockIdx.x * KV8_TOKENS, h = blockIdx.y;
-  for (int i = threadIdx.x; i < KV8_TOKENS * D; i += KV8_THREADS) {
-    const int tj = i % KV8_TOKENS, d = i / KV8_TOKENS, tt = t0 + tj;
-    if (tt >= N) continue;
-    const int r = rows[tt], pp = pos[tt];
-    if (r < 0 || r >= max_batch || pp < 0 || pp >= S) continue;
-    s_v[tj][d] = vc[((long)r * Hkv + h) * (long)S * D + (long)(pp >> 6) * 64 * D + d * 64 + (pp & 63)];
+  __shared__ uint32_t s_v[D * KV8_LD];
+  const int h = blockIdx.y, j = threadIdx.x >> 4, part = threadIdx.x & 15;
+  if (blockIdx.z < 4) {
+    const int t = blockIdx.x * KV8_TOKENS + blockIdx.z * 16 + j;
+    if (t >= N) return;
+    const int row = rows[t], p = pos[t];
+    const bool ok = row >= 0 && row < max_batch && p >= 0 && p < S;
+    const long stripe = ((long)row * Hkv + h) * (long)S;
+    const uint32_t* src = (const uint32_t*)(kc + stripe * D + kv8_k_offset(p, part * PER, D));
+    T* dst = k + ((long)t * Hkv + h) * D + part * PER;
+    const float scale = ok ? __uint_as_float((uint32_t)ks[stripe + p] << 23) : 0.f;
+#pragma unroll
+    for (int i = 0; i < PER / 4; ++i) {
+      float o[4];
+      values4(ok ? src[i] : 0u, scale, o);
+      store4(dst + 4 * i, o);
+    }
+    return;
+  }
+  const int t0 = blockIdx.x * KV8_TOKENS, nt = min(KV8_TOKENS, N - t0);
+  const bool run = kv8_run(rows, pos, t0, nt, max_batch, S);
+  int sh = 0;
+  if (run) {
+    const int p0 = pos[t0];
+    sh = p0 & 3;
+    kv8_dwords<D>(((long)rows[t0] * Hkv + h) * (long)S, p0, nt,
+                  [&](int d, int i, long at) { s_v[d * KV8_LD + i] = *(const uint32_t*)(vc + at); });
+  } else {
+    kv8_each<D>(rows, pos, t0, nt, h, Hkv, max_batch, S,
+                [&](int d, int tj, long at) { ((uint8_t*)(s_v + d * KV8_LD))[tj] = vc[at]; });
   }
   __syncthreads();
-  const int j = threadIdx.x >> 4, part = threadIdx.x & 15;
-  const int t = t0 + j;
-  if (t >= N) return;
-  const int row = rows[t], p = pos[t];
-  const bool ok = row >= 0 && row < max_batch && p >= 0 && p < S;
-  const long stripe = ((long)row * Hkv + h) * (long)S;
-  const float sk = ok ? __uint_as_float((uint32_t)ks[stripe + p] << 23) : 0.f;
-  const float sv = ok ? __uint_as_float((uint32_t)vs[stripe + p] << 23) : 0.f;
+  uint32_t w[PER / 4][4];
 #pragma unroll
-  for (int i = 0; i < PER; i += 4) {
-    const int d = part * PER + i;
-    const long o = ((long)t * Hkv + h) * D + d;
-    float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-    if (ok) {
-      values4(*(const uint32_t*)(kc + stripe * D + kv8_k_offset(p, d, D)), sk, a);
-      values4(*(const uint32_t*)(&s_v[j][d]), sv, b);
+  for (int i = 0; i < PER / 4; ++i) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t* r = s_v + (part * PER + 4 * i + c) * KV8_LD + j;
+      w[i][c] = __builtin_amdgcn_alignbyte(r[1], r[0], sh);
     }
+    turn4(w[i]);
+  }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      Elem<T>::st(k + o + q, a[q]);
-      Elem<T>::st(v + o + q, b[q]);
+  for (int c = 0; c < 4; ++c) {
+    const int t = t0 + 4 * j + c;
+    if (4 * j + c >= nt) break;
+    const int row = rows[t], p = pos[t];
+    const bool ok = row >= 0 && row < max_batch && p >= 0 && p < S;
+    const float scale = ok ? __uint_as_float((uint32_t)vs[((long)row * Hkv + h) * (long)S + p] << 23) : 0.f;
+    T* dst = v + ((long)t * Hkv + h) * D + part * PER;
+#pragma unroll
+    for (int i = 0; i < PER / 4; ++i) {
+      float o[4];
+      values4(ok ? w[i][c] : 0u, scale, o);
+      store4(dst + 4 * i, o);
     }
   }
 }
@@ -183,7 +321,7 @@ extern "C" int lsk_kv8_append(int dtype, const void* k, const void* v, long stri
                         max_seq)) return rc;
   LSK_REQUIRE(stride_t >= 0 && stride_h >= 0, LSK_ESHAPE, "%s: negative strides", what);
   if (n_tokens == 0) return 0;
-  const dim3 grid((n_tokens + KV8_TOKENS - 1) / KV8_TOKENS, n_kv_heads);
+  const dim3 grid((n_tokens + KV8_TOKENS - 1) / KV8_TOKENS, n_kv_heads, 5);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == LSK_DTYPE_BF16)
     KV8_LAUNCH(kv8_append_kernel, uint16_t, (const uint16_t*)k, (const uint16_t*)v, stride_t, stride_h, (uint8_t*)k8,
@@ -201,7 +339,7 @@ extern "C" int lsk_kv8_read(int dtype, const void* k8, const void* v8, const voi
   if (int rc = kv8_args(what, dtype, k, v, k8, v8, k_exp, v_exp, rows, pos, n_tokens, n_kv_heads, head_dim, max_batch,
                         max_seq)) return rc;
   if (n_tokens == 0) return 0;
-  const dim3 grid((n_tokens + KV8_TOKENS - 1) / KV8_TOKENS, n_kv_heads);
+  const dim3 grid((n_tokens + KV8_TOKENS - 1) / KV8_TOKENS, n_kv_heads, 5);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == LSK_DTYPE_BF16)
     KV8_LAUNCH(kv8_read_kernel, uint16_t, (const uint8_t*)k8, (const uint8_t*)v8, (const uint8_t*)k_exp,

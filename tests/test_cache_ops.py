@@ -211,6 +211,35 @@ def test_kv8_append_and_read_are_exact(cuda, dtype, D, n, h):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_kv8_runs_of_positions_from_any_start(cuda, D):
+    """Prompts from any position, next to each other, across 64-position blocks and up to the cache's end, between
+    single tokens: every token's values, and nothing of its neighbours."""
+    lsk = _lsk()
+    g = _gen(31)
+    B, h, S = 6, 2, 256
+    runs = [(0, 1, 16), (1, 2, 33), (2, 57, 31), (2, 88, 40), (3, 240, 16), (4, 3, 1), (0, 61, 5), (5, 255, 1), (5, 0, 96),
+            (4, 130, 29)]
+    rows = torch.cat([torch.full((n,), r) for (r, _, n) in runs])
+    pos = torch.cat([torch.arange(p, p + n) for (_, p, n) in runs])
+    for shift in (0, 3):                              # (the second time the workgroups hold other runs)
+        rows, pos = rows.roll(shift), pos.roll(shift)
+        n = len(rows)
+        k, v = (torch.randn(n, h, D, generator=g).to(BF16) for _ in range(2))
+        cache = lsk.KV8.zeros(B, h, S, D, cuda)
+        for x in (cache.k, cache.v):
+            x.view(torch.uint8).fill_(57)             # (1.125 everywhere else)
+        lsk.kv8_append(k.to(cuda), v.to(cuda), cache, _i32(rows, cuda), _i32(pos, cuda))
+        allrows, allpos = torch.arange(B).repeat_interleave(S), torch.arange(S).repeat(B)
+        for got, x in zip(lsk.kv8_read(cache, _i32(allrows, cuda), _i32(allpos, cuda), F32), (k, v)):
+            want = torch.full((B, S, h, D), 1.125, dtype=torch.float64)
+            want[rows, pos] = held(x)
+            assert torch.equal(got.cpu().double().view(B, S, h, D), want)
+        for got, x in zip(lsk.kv8_read(cache, _i32(rows, cuda), _i32(pos, cuda), F32), (k, v)):
+            assert torch.equal(got.cpu().double(), held(x))
+
+
+@pytest.mark.gpu
 def test_kv8_rounds_every_bf16_value_to_the_nearest_code(cuda):
     """All finite bf16 values with a fixed largest value in the vector: the code is the nearest e4m3 value, ties to
     even (torch's own conversion of the scaled value)."""
