@@ -7,7 +7,6 @@ There is no fallback: a missing or stale library raises at the first call.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 import os
@@ -521,36 +520,51 @@ def shift_segment_positions(meta, n_tokens: int, nb: int, n_works: int, n_groups
 
 # ----------------------------------------------------------------------------- 8-bit cache and trees of drafted tokens
 
-def _one_device(*ts) -> torch.device:
-    """The device that all the tensors are on (None is skipped); LskError otherwise."""
-    _dev(*ts)
-    devs = {t.device for t in ts if t is not None}
-    if len(devs) != 1:
-        raise LskError(f"tensors on different devices: {sorted(map(str, devs))}")
-    return devs.pop()
+def _one_device(*ts) -> int:
+    """The index of the device that all the tensors are on (None is skipped); LskError otherwise."""
+    dev = None
+    for t in ts:
+        if t is not None:
+            i = t.get_device()
+            if i != dev:
+                if dev is not None or i < 0:
+                    _dev(*ts)
+                    raise LskError(f"tensors on different devices: "
+                                   f"{sorted({str(t.device) for t in ts if t is not None})}")
+                dev = i
+    return dev
 
 
-def _current(device: torch.device):
-    """A context in which `device` is the current one (its current stream takes the launch)."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _launch(dev: int, what: str, *args) -> None:
+    """Calls `what` with args and device dev's current stream; dev is the current device for the call."""
+    fn = getattr(load(), what)
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, _stream())
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream())
+    _check(rc, what)
 
 
 def _want(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
         raise LskError(f"{what}: {name} must be a contiguous {list(shape)} {dtype} tensor, got {list(t.shape)} {t.dtype}"
                        f"{'' if t.is_contiguous() else ', not contiguous'}")
 
 
-class KV8(NamedTuple):
-    """An 8-bit K / V cache (lsk_kv8_append): e4m3 codes and one power-of-two scale per position and KV head, the byte
-    e + 127.  A layer's tensors, or with a leading layer axis those of several:
-      k [B, Hkv, S/64, 4, D/64, 64, 16] and v [B, Hkv, S/64, D, 64] float8_e4m3fn, ks and vs [B, Hkv, S] uint8."""
+class _KV8(NamedTuple):
     k: torch.Tensor
     v: torch.Tensor
     ks: torch.Tensor
     vs: torch.Tensor
+
+
+class KV8(_KV8):
+    """An 8-bit K / V cache (lsk_kv8_append): e4m3 codes and one power-of-two scale per position and KV head, the byte
+    e + 127.  A layer's tensors, or with a leading layer axis those of several:
+      k [B, Hkv, S/64, 4, D/64, 64, 16] and v [B, Hkv, S/64, D, 64] float8_e4m3fn, ks and vs [B, Hkv, S] uint8.
+    The tensors' types and shapes are checked by the object's first use; they have to stay as they are."""
+    _checked = None                                   # (layers, dims) that the tensors were found to fit
 
     @classmethod
     def zeros(cls, max_batch: int, n_kv_heads: int, max_seq: int, head_dim: int, device, layers: int | None = None):
@@ -572,26 +586,31 @@ class KV8(NamedTuple):
         *_, B, Hkv, S = self.ks.shape
         return B, Hkv, S, self.v.shape[-2]
 
-    def check(self, what: str, layers: bool = False) -> None:
-        n = 1 if layers else 0
-        if self.ks.dim() != 3 + n or self.v.dim() != 5 + n:
+    def check(self, what: str, layers: bool = False) -> tuple:
+        """(B, Hkv, S, D) of a cache of the documented storage; LskError otherwise."""
+        if self._checked is not None and self._checked[0] == layers:
+            return self._checked[1]
+        k, v, ks, vs = self
+        lead, n = tuple(ks.shape), 4 if layers else 3
+        if len(lead) != n or v.dim() != n + 2:
             raise LskError(f"{what}: an 8-bit cache of {'several layers' if layers else 'one layer'} is needed")
-        lead = tuple(self.ks.shape[:2 + n])
-        _, _, S, D = self.dims
+        S, D = lead[-1], v.shape[-2]
         if D not in (64, 128) or S % 64 or S == 0:
             raise LskError(f"{what}: 8-bit caches need head_dim 64 or 128 and max_seq a multiple of 64 (got {D}, {S})")
-        _want(what, "k codes", self.k, torch.float8_e4m3fn, (*lead, S // 64, 4, D // 64, 64, 16))
-        _want(what, "v codes", self.v, torch.float8_e4m3fn, (*lead, S // 64, D, 64))
-        _want(what, "k exponents", self.ks, torch.uint8, (*lead, S))
-        _want(what, "v exponents", self.vs, torch.uint8, (*lead, S))
+        blocks = (*lead[:-1], S // 64)
+        _want(what, "k codes", k, torch.float8_e4m3fn, (*blocks, 4, D // 64, 64, 16))
+        _want(what, "v codes", v, torch.float8_e4m3fn, (*blocks, D, 64))
+        _want(what, "k exponents", ks, torch.uint8, lead)
+        _want(what, "v exponents", vs, torch.uint8, lead)
+        self._checked = layers, (lead[-3], lead[-2], S, D)
+        return self._checked[1]
 
 
 def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor) -> None:
     """k, v [N, Hkv, D] (bf16 or fp32, of equal strides; dims contiguous) quantised into a layer's 8-bit cache at
     (rows, pos).  Tokens outside the cache are skipped; the (row, position) pairs of a call have to differ."""
     dev = _one_device(k, v, *cache, rows_i32, pos_i32)
-    cache.check("kv8_append")
-    B, Hkv, S, D = cache.dims
+    B, Hkv, S, D = cache.check("kv8_append")
     n = k.shape[0]
     if k.shape != (n, Hkv, D) or v.shape != k.shape or v.dtype != k.dtype:
         raise LskError(f"kv8_append: k and v must be [N, {Hkv}, {D}] of one dtype, got {list(k.shape)} {k.dtype} and "
@@ -603,9 +622,8 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: KV8, rows_i32: torch.Ten
     code = dtype_code(k.dtype)
     if n == 0:
         return
-    with _current(dev):
-        _check(load().lsk_kv8_append(code, _ptr(k), _ptr(v), k.stride(0), k.stride(1), *map(_ptr, cache), _ptr(rows_i32),
-                                     _ptr(pos_i32), n, Hkv, D, B, S, _stream()), "lsk_kv8_append")
+    _launch(dev, "lsk_kv8_append", code, _ptr(k), _ptr(v), k.stride(0), k.stride(1), *map(_ptr, cache), _ptr(rows_i32),
+            _ptr(pos_i32), n, Hkv, D, B, S)
 
 
 def kv8_read(cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
@@ -613,20 +631,19 @@ def kv8_read(cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor, dtype: t
     """The K and V that a layer's 8-bit cache holds at (rows, pos): two [N, Hkv, D] tensors (bf16: exactly); zeros for
     tokens outside the cache."""
     dev = _one_device(*cache, rows_i32, pos_i32, *(out or ()))
-    cache.check("kv8_read")
-    B, Hkv, S, D = cache.dims
+    B, Hkv, S, D = cache.check("kv8_read")
     n = rows_i32.numel()
     _want("kv8_read", "rows", rows_i32, torch.int32, (n,))
     _want("kv8_read", "pos", pos_i32, torch.int32, (n,))
     code = dtype_code(dtype if out is None else out[0].dtype)
     if out is None:
-        out = tuple(torch.empty(n, Hkv, D, dtype=dtype, device=dev) for _ in range(2))
-    for t in out:
-        _want("kv8_read", "out", t, out[0].dtype, (n, Hkv, D))
+        out = tuple(cache.ks.new_empty((n, Hkv, D), dtype=dtype) for _ in range(2))
+    else:
+        for t in out:
+            _want("kv8_read", "out", t, out[0].dtype, (n, Hkv, D))
     if n:
-        with _current(dev):
-            _check(load().lsk_kv8_read(code, *map(_ptr, cache), _ptr(rows_i32), _ptr(pos_i32), _ptr(out[0]),
-                                       _ptr(out[1]), n, Hkv, D, B, S, _stream()), "lsk_kv8_read")
+        _launch(dev, "lsk_kv8_read", code, *map(_ptr, cache), _ptr(rows_i32), _ptr(pos_i32), _ptr(out[0]), _ptr(out[1]),
+                n, Hkv, D, B, S)
     return out
 
 
@@ -645,18 +662,15 @@ def cache_attn_row_groups(max_batch: int, n_kv_heads: int) -> int:
     return 8 if stripes >= 128 else 4 if stripes >= 64 else 2 if stripes >= 32 else 1
 
 
-class _Launch(NamedTuple):
-    """One lsk_cache_attn_plan on the device."""
-    groups: torch.Tensor
-    recs: torch.Tensor
-    n_groups: int
-    n_parts: int
-    n_rounds: int
-    n_slots: int
-    tiles: int
-    row_groups: int
-    part_rows: int
-    ws_bytes: int
+class _Launch:
+    """One lsk_cache_attn_plan on the device, and its arguments of a launch."""
+
+    def __init__(self, groups: torch.Tensor, recs: torch.Tensor, n_groups: int, n_parts: int, n_rounds: int, n_slots: int,
+                 tiles: int, row_groups: int, part_rows: int, ws_bytes: int):
+        self.groups, self.recs, self.n_groups, self.n_parts, self.n_rounds = groups, recs, n_groups, n_parts, n_rounds
+        self.n_slots, self.tiles, self.row_groups, self.part_rows, self.ws_bytes = \
+            n_slots, tiles, row_groups, part_rows, ws_bytes
+        self.args = (_ptr(groups), n_groups, n_parts, _ptr(recs), n_rounds, n_slots, tiles, row_groups, part_rows)
 
 
 class AttnPlan:
@@ -732,12 +746,12 @@ def _plan_call(what: str, q: torch.Tensor, plan: AttnPlan, launch, dims: tuple, 
     if mask is not None:
         _want(what, "mask", mask, torch.int32, (plan.n_tokens, mask.shape[1]))
     if out is None:
-        out = torch.empty(plan.n_tokens, plan.n_heads * D, dtype=want, device=q.device)
+        out = q.new_empty((plan.n_tokens, plan.n_heads * D))
     else:
         _want(what, "out", out, want, (plan.n_tokens, plan.n_heads * D))
     if workspace is None and launch is not None and launch.ws_bytes:
-        workspace = torch.empty(launch.ws_bytes, dtype=torch.uint8, device=q.device)
-    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+        workspace = q.new_empty((launch.ws_bytes,), dtype=torch.uint8)
+    ws_bytes = workspace.nbytes if workspace is not None else 0
     return 1.0 / math.sqrt(D) if scale is None else float(scale), out, workspace, ws_bytes
 
 
@@ -748,17 +762,12 @@ def kv8_attn(q: torch.Tensor, cache: KV8, plan: AttnPlan, mask: torch.Tensor | N
     a workspace one is taken from torch's allocator for the call."""
     p = plan.causal if mask is None else plan.tree
     dev = _one_device(q, *cache, p.recs if p is not None else None, mask, out, workspace)
-    cache.check("kv8_attn")
-    scale, out, workspace, ws = _plan_call("kv8_attn", q, plan, p, cache.dims, True, cache.k.dtype, mask, scale, out,
-                                           workspace)
+    dims = _, Hkv, S, D = cache.check("kv8_attn")
+    scale, out, workspace, ws = _plan_call("kv8_attn", q, plan, p, dims, True, cache.k.dtype, mask, scale, out, workspace)
     if p.n_rounds:
-        _, Hkv, S, D = cache.dims
-        with _current(dev):
-            _check(load().lsk_kv8_attn(_ptr(q), q.stride(0), q.stride(1), *map(_ptr, cache), _ptr(mask),
-                                       mask.shape[1] if mask is not None else 0, _ptr(p.groups), p.n_groups, p.n_parts,
-                                       _ptr(p.recs), p.n_rounds, p.n_slots, p.tiles, p.row_groups, p.part_rows,
-                                       _ptr(out), plan.n_heads, Hkv, D, S, scale, _ptr(workspace), ws, _stream()),
-                   "lsk_kv8_attn")
+        _launch(dev, "lsk_kv8_attn", _ptr(q), q.stride(0), q.stride(1), *map(_ptr, cache), _ptr(mask),
+                mask.shape[1] if mask is not None else 0, *p.args, _ptr(out), plan.n_heads, Hkv, D, S, scale,
+                _ptr(workspace), ws)
     return out
 
 
@@ -779,13 +788,10 @@ def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, plan:
     scale, out, workspace, ws = _plan_call("tree_attn", q, plan, p, dims, False, kcache.dtype, mask, scale, out,
                                            workspace)
     if p.n_rounds if p is not None else plan.n_works:
-        launch = (_ptr(p.groups), p.n_groups, p.n_parts, _ptr(p.recs), p.n_rounds, p.n_slots, p.tiles, p.row_groups,
-                  p.part_rows) if p is not None else (None, 0, 0, None, 0, 0, 0, 0, 0)
-        with _current(dev):
-            _check(load().lsk_tree_attn(code, _ptr(q), q.stride(0), q.stride(1), _ptr(kcache), _ptr(vcache), _ptr(mask),
-                                        mask.shape[1], _ptr(plan.works), plan.n_works, plan.rows_cap, *launch,
-                                        _ptr(out), plan.n_heads, Hkv, D, S, scale, _ptr(workspace), ws, _stream()),
-                   "lsk_tree_attn")
+        args = p.args if p is not None else (None, 0, 0, None, 0, 0, 0, 0, 0)
+        _launch(dev, "lsk_tree_attn", code, _ptr(q), q.stride(0), q.stride(1), _ptr(kcache), _ptr(vcache), _ptr(mask),
+                mask.shape[1], _ptr(plan.works), plan.n_works, plan.rows_cap, *args, _ptr(out), plan.n_heads, Hkv, D, S,
+                scale, _ptr(workspace), ws)
     return out
 
 
@@ -798,12 +804,10 @@ def tree_masks(parents: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, 
     for name, t, k in (("parents", parents, n), ("starts", starts, nb), ("lens", lens, nb)):
         _want("tree_masks", name, t, torch.int32, (k,))
     words = max(1, (max_nodes + 31) // 32)
-    mask = torch.zeros(n, words, dtype=torch.int32, device=dev)
-    depth = torch.zeros(n, dtype=torch.int32, device=dev)
+    mask, depth = parents.new_zeros((n, words)), parents.new_zeros((n,))
     if n and nb:
-        with _current(dev):
-            _check(load().lsk_tree_masks(_ptr(parents), _ptr(starts), _ptr(lens), nb, n, max_nodes, _ptr(mask), words,
-                                         _ptr(depth), _stream()), "lsk_tree_masks")
+        _launch(dev, "lsk_tree_masks", _ptr(parents), _ptr(starts), _ptr(lens), nb, n, max_nodes, _ptr(mask), words,
+                _ptr(depth))
     return mask, depth
 
 
@@ -820,15 +824,12 @@ def tree_accept(Yv: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, s
         _want("tree_accept", name, t, dt, (k,))
     if max_nodes < 1:
         raise LskError(f"tree_accept: max_nodes {max_nodes}")
-    acc = torch.empty(nb, dtype=torch.int64, device=dev)
-    path = torch.empty(nb, max_nodes, dtype=torch.int32, device=dev)
-    out = torch.empty(nb, max_nodes, dtype=torch.int64, device=dev)
+    acc, path, out = Yv.new_empty((nb,)), parents.new_empty((nb, max_nodes)), Yv.new_empty((nb, max_nodes))
     if nb and n == 0:
         acc.fill_(-1), path.fill_(-1), out.fill_(-1)
     elif nb:
-        with _current(dev):
-            _check(load().lsk_tree_accept(_ptr(Yv), _ptr(tokens), _ptr(parents), _ptr(starts), _ptr(lens), nb, n,
-                                          max_nodes, _ptr(acc), _ptr(path), _ptr(out), _stream()), "lsk_tree_accept")
+        _launch(dev, "lsk_tree_accept", _ptr(Yv), _ptr(tokens), _ptr(parents), _ptr(starts), _ptr(lens), nb, n, max_nodes,
+                _ptr(acc), _ptr(path), _ptr(out))
     return acc, path, out
 
 
@@ -843,10 +844,8 @@ def _compact(what, code, k, v, ks, vs, layers, dims, rows_i32, pos0_i32, accepte
         raise LskError(f"{what}: path must be [{nb}, max_nodes]")
     _want(what, "path", path, torch.int32, (nb, path.shape[1]))
     if nb and layers:
-        with _current(dev):
-            _check(load().lsk_kv_compact(code, _ptr(k), _ptr(v), _ptr(ks), _ptr(vs), layers, _ptr(rows_i32),
-                                         _ptr(pos0_i32), _ptr(accepted), _ptr(path), nb, path.shape[1], Hkv, D, B, S,
-                                         _stream()), "lsk_kv_compact")
+        _launch(dev, "lsk_kv_compact", code, _ptr(k), _ptr(v), _ptr(ks), _ptr(vs), layers, _ptr(rows_i32), _ptr(pos0_i32),
+                _ptr(accepted), _ptr(path), nb, path.shape[1], Hkv, D, B, S)
 
 
 def kv_compact(k: torch.Tensor, v: torch.Tensor, rows_i32, pos0_i32, accepted, path) -> None:
@@ -855,8 +854,9 @@ def kv_compact(k: torch.Tensor, v: torch.Tensor, rows_i32, pos0_i32, accepted, p
     or a run of their layers); path and accepted: tree_accept's; rows, pos0 int32 [nb], the rows different."""
     if k.dim() not in (5, 7) or not k.is_contiguous():
         raise LskError("kv_compact: the K storage of several layers is needed, contiguous")
-    _check_kcache(k.dtype, k[0] if k.shape[0] else k.new_empty(k.shape[1:]))
     code = dtype_code(k.dtype)
+    if (k.dim() == 7) != (code == DTYPE_BF16):
+        raise LskError("kv_compact: fragment-major bf16 K storage or row-major fp32 is needed")
     B, Hkv = k.shape[1:3]
     S, D = (k.shape[3] * 32, k.shape[4] * 16) if k.dim() == 7 else (k.shape[3], k.shape[4])
     _want("kv_compact", "V storage", v, k.dtype, (k.shape[0], B, Hkv, S // 32, D, 32))
@@ -865,9 +865,8 @@ def kv_compact(k: torch.Tensor, v: torch.Tensor, rows_i32, pos0_i32, accepted, p
 
 def kv8_compact(cache: KV8, rows_i32, pos0_i32, accepted, path) -> None:
     """kv_compact for the layers of an 8-bit cache (tensors with a leading layer axis)."""
-    cache.check("kv8_compact", layers=True)
-    _compact("kv8_compact", DTYPE_KV8, cache.k, cache.v, cache.ks, cache.vs, cache.k.shape[0], cache.dims, rows_i32,
-             pos0_i32, accepted, path)
+    dims = cache.check("kv8_compact", layers=True)
+    _compact("kv8_compact", DTYPE_KV8, *cache, cache.k.shape[0], dims, rows_i32, pos0_i32, accepted, path)
 
 
 # ----------------------------------------------------------------------------- layer-range runner
