@@ -84,6 +84,145 @@ __device__ __forceinline__ float exp_bits(uint32_t byte) { return __uint_as_floa
 #define ORDER() __builtin_amdgcn_sched_barrier(0)  // (keeps the loads and conversions where their registers are free)
 #define LAG 8.0f
 
+// K / V through buffer loads over an item's (row, KV head) stripe, whose range ends with the block that holds the item's
+// last position: loads past it give zeros without touching memory, so the next step's are unconditional (under a branch
+// the compiler would wait for them early).
+struct Stripe {
+  __amdgpu_buffer_rsrc_t k, v, ks, vs;
+};
+template <int D, bool KV8>
+__device__ __forceinline__ Stripe cache_stripe(const CacheAttnArgs& A, int crow, int kvh, int kv_hi) {
+  constexpr int STEP = KV8 ? 64 : 32;
+  const long st = (long)crow * A.Hkv + kvh;
+  const long bytes = (long)(A.S / STEP) * 64 * D;    // of a whole stripe
+  const int end = min(A.S, (kv_hi + STEP - 1) / STEP * STEP);
+  Stripe s;
+  s.k = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)A.kc + st * bytes), (short)0, end / STEP * 64 * D,
+                                          LSK_BUFFER_RSRC_WORD3);
+  s.v = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)A.vc + st * bytes), (short)0, end / STEP * 64 * D,
+                                          LSK_BUFFER_RSRC_WORD3);
+  if constexpr (KV8) {
+    s.ks = __builtin_amdgcn_make_buffer_rsrc((void*)(A.ks + st * A.S), (short)0, end, LSK_BUFFER_RSRC_WORD3);
+    s.vs = __builtin_amdgcn_make_buffer_rsrc((void*)(A.vs + st * A.S), (short)0, end, LSK_BUFFER_RSRC_WORD3);
+  }
+  return s;
+}
+
+// A step's V as loaded (row d = 16 c + l16, this lane's slots): clears the values past the first nk slots and the
+// non-finite ones; bit u of the result: slot u of the step holds a non-finite value.
+template <bool KV8, int CT>
+__device__ __forceinline__ uint64_t clear_odd(lsk_i32x4 (&vr)[CT], int nk) {
+  constexpr int PER = KV8 ? 4 : 2, BITS = 32 / PER;  // slots of a dword, bits of a value
+  constexpr int NE = 4 * PER;
+  uint32_t any[4];                                   // the top bits of this lane's non-finite values
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int m = nk - PER * w;
+    const uint32_t keep = m >= PER ? 0xffffffffu : m <= 0 ? 0u : (1u << (BITS * m)) - 1u;
+    any[w] = 0;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const uint32_t x = (uint32_t)vr[c][w] & keep;
+      const uint32_t nf = KV8 ? ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u
+                              : ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+      vr[c][w] = (int)(x & ~((nf - (nf >> (BITS - 1))) | nf));
+      any[w] |= nf;
+    }
+  }
+  uint64_t odd = 0;
+  if (__builtin_amdgcn_ballot_w64((any[0] | any[1] | any[2] | any[3]) != 0u) != 0ull) {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const uint64_t lanes = __builtin_amdgcn_ballot_w64((any[e / PER] >> (BITS * (e % PER) + BITS - 1)) & 1u);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) odd |= ((lanes >> (16 * g)) & 0xffffull) ? 1ull << (NE * g + e) : 0ull;
+    }
+  }
+  return odd;
+}
+
+// The non-finite values of V that clear_odd took out, for the rows that read them.
+template <bool KV8, bool TREE, int QT, int CT>
+__device__ __forceinline__ void add_odd(const CacheAttnArgs& A, __amdgpu_buffer_rsrc_t v, uint64_t odd, int sb,
+                                        int q_start, int pos0, const int (&qpos)[QT], lsk_f32x4 (&oacc)[QT][CT]) {
+  constexpr int STEP = KV8 ? 64 : 32, D = 16 * CT;
+  const int lg = (threadIdx.x & 63) >> 4;
+  while (odd != 0ull) {                              // (rare: one slot after the other, few registers)
+    const int u = __builtin_ctzll(odd), kp = sb + u;
+    odd &= odd - 1;
+    bool hit[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      hit[qt] = kp <= qpos[qt];
+      if constexpr (TREE) {
+        const int t = max(qpos[qt] - pos0, 0);
+        hit[qt] = hit[qt] && (mask_window(A.mask + (long)(q_start + t) * A.W, A.W, kp - pos0) & 1u);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ORDER();
+        // V[kp][16 c + 4 lg + i]: a dim's slots of a block are 64 bytes in both formats
+        const int so = sb / STEP * 64 * D + (16 * c + i) * 64 + u * (KV8 ? 1 : 2);
+        float x;
+        if constexpr (KV8) {
+          const uint32_t b = __builtin_amdgcn_raw_buffer_load_b8(v, 256 * lg, so, 0);
+          x = (b & 0x7fu) == 0x7fu ? __builtin_nanf("") : 0.f;
+        } else {
+          x = bf2f((uint16_t)__builtin_amdgcn_raw_buffer_load_b16(v, 256 * lg, so, 0));
+          x = (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? x : 0.f;
+        }
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+          if (hit[qt]) oacc[qt][c][i] += x;
+      }
+  }
+}
+
+// The online softmax of one tile's 16 query columns over a step: s[a][e] are the scores of this lane's slots 4 a + e, of
+// which `reads` says what the column reads (FULL: all), vsr V's exponents of the slots (8-bit); pb the weights for the
+// second product.  A row's m only moves when a score passes it by more than LAG (weights up to 2^LAG; each row for
+// itself, so the rows of a tile stay independent), which is seldom after the first step: then no maximum crosses lanes
+// and nothing is rescaled.  Each lane sums its own slots' weights.
+template <bool KV8, bool FULL, int NA, int CT, int HV>
+__device__ __forceinline__ void softmax_tile(lsk_f32x4 (&s)[NA], uint32_t reads, lsk_i32x4 vsr, float scale_log2, float& m,
+                                             float& l, lsk_f32x4 (&o)[CT], lsk_bf16x8 (&pb)[HV]) {
+  float mt = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 4 * NA; ++i) {
+    if constexpr (!FULL) s[i >> 2][i & 3] = (reads >> i) & 1u ? s[i >> 2][i & 3] : -INFINITY;
+    mt = fmaxf(mt, s[i >> 2][i & 3]);
+  }
+  mt *= scale_log2;
+  if (__builtin_amdgcn_ballot_w64(mt > m + LAG) != 0ull) {
+    mt = rows_max(mt);
+    const bool up = mt > m + LAG;
+    const float alpha = up ? fast_exp2(m - mt) : 1.f;
+    m = up ? mt : m;
+    l *= alpha;
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[c][i] *= alpha;
+  }
+  float rs = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4 * NA; ++i) {
+    float pe = fast_exp2(__builtin_fmaf(s[i >> 2][i & 3], scale_log2, -m));
+    if constexpr (!FULL) pe = (reads >> i) & 1u ? pe : 0.f;
+    rs += pe;
+    float pv = pe;
+    if constexpr (KV8) {
+      pv = pe * exp_bits(((uint32_t)vsr[i >> 2] >> (8 * (i & 3))) & 255u);
+      if constexpr (!FULL) pv = (reads >> i) & 1u ? pv : 0.f;  // (a slot never written: any exponent)
+    }
+    pb[i >> 3][i & 7] = static_cast<__bf16>(pv);
+  }
+  l += rs;
+}
+
 template <int D, int QT, bool KV8, bool TREE>
 __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const CacheAttnArgs A) {
   constexpr int STEP = KV8 ? 64 : 32;                // positions per step of a wave
@@ -97,22 +236,13 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
   constexpr bool QREG = QT == 1;                     // one tile: Q fragments in registers (items of one row group)
   constexpr int MT = QT < ATTN_MERGE_TILES ? QT : ATTN_MERGE_TILES;
   constexpr int MR = 16 * MT;                        // rows of a wave merged per pass
-  constexpr int QROWS = QREG ? 0 : TREE ? NW * GR : GR;  // rows of an item at most
+  constexpr int QROWS = QREG ? 0 : TREE ? 2 * GR : GR;  // rows of an item at most
   constexpr int QLD = D + 8;                         // 16 rows' 16-byte reads hit distinct banks
   constexpr int QCH = D / 8;
   constexpr int QPT = QREG ? 1 : (QROWS * QCH + 64 * NW - 1) / (64 * NW);
-  // Q of the next item waits in registers during the merge, where they hold it (a tree's items, of up to 256 rows, are
-  // few per workgroup: theirs is fetched after it)
-  constexpr bool QAHEAD = !TREE;
-  constexpr int O_BYTES = NW * MR * (D + 4) * 4, Q_BYTES = QROWS * QLD * 2;
-  // Q is in LDS during an item's steps, the waves' partial outputs during its merge.  A tree's (up to 256 rows) share one
-  // buffer in turn; else there is room for both, which saves two barriers an item.
-  constexpr bool SHARED = TREE && !QREG;
-  __shared__ __attribute__((aligned(16))) char s_buf[SHARED && Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
-  __shared__ __attribute__((aligned(16))) char s_qbuf[SHARED || QREG ? 16 : Q_BYTES];
+  __shared__ __attribute__((aligned(16))) float s_o[NW][MR][D + 4];
+  __shared__ __attribute__((aligned(16))) uint16_t s_q[QREG ? 1 : QROWS][QLD];
   __shared__ float s_ml[NW][2][GR];
-  float (*s_o)[MR][D + 4] = (float (*)[MR][D + 4])s_buf;
-  uint16_t (*s_q)[QLD] = (uint16_t (*)[QLD])(SHARED ? s_buf : s_qbuf);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -143,16 +273,14 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
     return A.q + (long)(it.q_start + t) * A.q_st + (long)(it.kvh * G + g) * A.q_sh;
   };
   auto ldq = [&](const uint16_t* p) { return __builtin_bit_cast(lsk_bf16x8, *(const lsk_u32x4_u*)p); };
+  // Q of the next item waits in registers during the merge; a tree's (twice the registers, which spilled) comes after it
+  constexpr bool QAHEAD = !TREE;
   lsk_bf16x8 qst[QAHEAD ? QPT : 1];
-  lsk_bf16x8 qreg[KF];
   auto q_chunk = [&](const Item& it, int c) {        // 8 elements of a row, zeros past the rows
-    const int r = c / QCH, c8 = c - r * QCH;
-    return r < it.nrows ? ldq(q_ptr(it, r) + 8 * c8) : (lsk_bf16x8){};
+    const int row = c / QCH;
+    return row < it.nrows ? ldq(q_ptr(it, row) + 8 * (c - row * QCH)) : (lsk_bf16x8){};
   };
-  auto q_put = [&](int c, lsk_bf16x8 v) {
-    const int r = c / QCH, c8 = c - r * QCH;
-    if (r < QROWS) *(lsk_bf16x8*)(&s_q[r][8 * c8]) = v;
-  };
+  lsk_bf16x8 qreg[KF];
   auto q_load = [&](const Item& it) {
     if constexpr (QREG) {
       const bool valid = l16 < it.nrows;
@@ -165,37 +293,17 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
     }
   };
   auto q_store = [&](const Item& it) {
-    if constexpr (!QREG && QAHEAD) {
-#pragma unroll
-      for (int i = 0; i < QPT; ++i) q_put(tid + i * 64 * NW, qst[i]);
-    } else if constexpr (!QREG) {
+    if constexpr (!QREG) {
       int t0 = tid;
       asm volatile("" : "+v"(t0));                   // (the chunks' offsets are not kept across the items: they spilled)
 #pragma unroll
-      for (int i = 0; i < QPT; ++i) q_put(t0 + i * 64 * NW, q_chunk(it, t0 + i * 64 * NW));
+      for (int i = 0; i < QPT; ++i) {
+        const int c = t0 + i * 64 * NW, row = c / QCH;
+        if (row < QROWS) *(lsk_bf16x8*)(&s_q[row][8 * (c - row * QCH)]) = QAHEAD ? qst[QAHEAD ? i : 0] : q_chunk(it, c);
+      }
     }
   };
-  // K / V through buffer loads over the item's (row, KV head) stripe, whose range ends with the block that holds the
-  // item's last position: loads past it give zeros without touching memory, so the next step's are unconditional
-  // (under a branch the compiler would wait for them early).  Non-temporal where each byte is read once per launch.
-  struct Stripe {
-    __amdgpu_buffer_rsrc_t k, v, ks, vs;
-  };
-  auto stripe = [&](const Item& it) {
-    const long st = (long)it.crow * Hkv + it.kvh;
-    const long bytes = (long)(S / STEP) * 64 * D;    // of a whole stripe
-    const int end = min(S, (it.kv_hi + STEP - 1) / STEP * STEP);
-    Stripe s;
-    s.k = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)A.kc + st * bytes), (short)0, end / STEP * 64 * D,
-                                            LSK_BUFFER_RSRC_WORD3);
-    s.v = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)A.vc + st * bytes), (short)0, end / STEP * 64 * D,
-                                            LSK_BUFFER_RSRC_WORD3);
-    if constexpr (KV8) {
-      s.ks = __builtin_amdgcn_make_buffer_rsrc((void*)(A.ks + st * S), (short)0, end, LSK_BUFFER_RSRC_WORD3);
-      s.vs = __builtin_amdgcn_make_buffer_rsrc((void*)(A.vs + st * S), (short)0, end, LSK_BUFFER_RSRC_WORD3);
-    }
-    return s;
-  };
+  auto stripe = [&](const Item& it) { return cache_stripe<D, KV8>(A, it.crow, it.kvh, it.kv_hi); };
   auto ld = [&](__amdgpu_buffer_rsrc_t rs, int vo, int so) -> lsk_i32x4 {
     return __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, vo, so, TREE ? 0 : 2));
   };
@@ -276,31 +384,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
       // that do read such a value get it after the products (below).
       uint64_t odd = 0;                              // bit u: slot sb + u holds a non-finite value
       if constexpr (!FULL) {
-        constexpr int PER = 2 * HV, BITS = 32 / PER; // slots of a dword, bits of a value
-        const int nk = kv_hi - (sb + NE * lg);       // slots of this lane that the item covers
-        uint32_t any[4];                             // the top bits of this lane's non-finite values
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int m = nk - PER * w;
-          const uint32_t keep = m >= PER ? 0xffffffffu : m <= 0 ? 0u : (1u << (BITS * m)) - 1u;
-          any[w] = 0;
-#pragma unroll
-          for (int c = 0; c < CT; ++c) {
-            const uint32_t x = (uint32_t)vr[c][w] & keep;
-            const uint32_t nf = KV8 ? ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u
-                                    : ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-            vr[c][w] = (int)(x & ~((nf - (nf >> (BITS - 1))) | nf));
-            any[w] |= nf;
-          }
-        }
-        if (__builtin_amdgcn_ballot_w64((any[0] | any[1] | any[2] | any[3]) != 0u) != 0ull) {
-#pragma unroll
-          for (int e = 0; e < NE; ++e) {
-            const uint64_t lanes = __builtin_amdgcn_ballot_w64((any[e / PER] >> (BITS * (e % PER) + BITS - 1)) & 1u);
-#pragma unroll
-            for (int g = 0; g < 4; ++g) odd |= ((lanes >> (16 * g)) & 0xffffull) ? 1ull << (NE * g + e) : 0ull;
-          }
-        }
+        odd = clear_odd<KV8>(vr, kv_hi - (sb + NE * lg));
       }
       // S^T = K Q^T, 16 slots at a time: sacc[qt][a][e] <-> slot s0 + 4 a + e.  The registers of a converted K take the
       // next step's at once.
@@ -343,45 +427,11 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
 #pragma unroll
         for (int a = 0; a < 2 * HV; ++a) load_k(sr, sn, a);
       }
-      // The online softmax of each tile's 16 query columns.  A row's m only moves when a score passes it by more than
-      // LAG (weights up to 2^LAG; each row for itself, so the rows of a tile stay independent), which is seldom after
-      // the first step: then no maximum crosses lanes and nothing is rescaled.  Each lane sums its own slots' weights.
       lsk_bf16x8 pb[QT][HV];
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
         if constexpr (KV8) ORDER();
-        float mt = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < NE; ++i) {
-          if constexpr (!FULL) sacc[qt][i >> 2][i & 3] = (reads[qt] >> i) & 1u ? sacc[qt][i >> 2][i & 3] : -INFINITY;
-          mt = fmaxf(mt, sacc[qt][i >> 2][i & 3]);
-        }
-        mt *= A.scale_log2;
-        if (__builtin_amdgcn_ballot_w64(mt > m_run[qt] + LAG) != 0ull) {
-          mt = rows_max(mt);
-          const bool up = mt > m_run[qt] + LAG;
-          const float alpha = up ? fast_exp2(m_run[qt] - mt) : 1.f;
-          m_run[qt] = up ? mt : m_run[qt];
-          l_run[qt] *= alpha;
-#pragma unroll
-          for (int c = 0; c < CT; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) oacc[qt][c][i] *= alpha;
-        }
-        float rs = 0.f;
-#pragma unroll
-        for (int i = 0; i < NE; ++i) {
-          float pe = fast_exp2(__builtin_fmaf(sacc[qt][i >> 2][i & 3], A.scale_log2, -m_run[qt]));
-          if constexpr (!FULL) pe = (reads[qt] >> i) & 1u ? pe : 0.f;
-          rs += pe;
-          float pv = pe;
-          if constexpr (KV8) {
-            pv = pe * exp_bits(((uint32_t)vsr[i >> 2] >> (8 * (i & 3))) & 255u);
-            if constexpr (!FULL) pv = (reads[qt] >> i) & 1u ? pv : 0.f;  // (a slot never written: any exponent)
-          }
-          pb[qt][i >> 3][i & 7] = static_cast<__bf16>(pv);
-        }
-        l_run[qt] += rs;
+        softmax_tile<KV8, FULL>(sacc[qt], reads[qt], vsr, A.scale_log2, m_run[qt], l_run[qt], oacc[qt], pb[qt]);
       }
       ORDER();
       load_vs(sr, sn);
@@ -404,38 +454,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
         ORDER();
       }
       if constexpr (!FULL) {
-        while (odd != 0ull) {                        // (rare: one slot after the other, few registers)
-          const int u = __builtin_ctzll(odd), kp = sb + u;
-          odd &= odd - 1;
-          bool hit[QT];
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) {
-            hit[qt] = kp <= qpos[qt];
-            if constexpr (TREE) {
-              const int t = max(qpos[qt] - cur.pos0, 0);
-              hit[qt] = hit[qt] && (mask_window(A.mask + (long)(cur.q_start + t) * A.W, A.W, kp - cur.pos0) & 1u);
-            }
-          }
-#pragma unroll
-          for (int c = 0; c < CT; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              ORDER();
-              // V[kp][16 c + 4 lg + i]: a dim's slots of a block are 64 bytes in both formats
-              const int so = sb / STEP * 64 * D + (16 * c + i) * 64 + u * (KV8 ? 1 : 2);
-              float x;
-              if constexpr (KV8) {
-                const uint32_t b = __builtin_amdgcn_raw_buffer_load_b8(sr.v, 256 * lg, so, 0);
-                x = (b & 0x7fu) == 0x7fu ? __builtin_nanf("") : 0.f;
-              } else {
-                x = bf2f((uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr.v, 256 * lg, so, 0));
-                x = (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? x : 0.f;
-              }
-#pragma unroll
-              for (int qt = 0; qt < QT; ++qt)
-                if (hit[qt]) oacc[qt][c][i] += x;
-            }
-        }
+        add_odd<KV8, TREE>(A, sr.v, odd, sb, cur.q_start, cur.pos0, qpos, oacc);
       }
     };
     int sb = first_step(cur);
@@ -449,44 +468,12 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
       nxt = fetch(r + 2);
     }
     // merge a row group's waves in order: M = max m_w, e_w = exp2(m_w - M), L = sum e_w l_w, O = sum e_w O_w
-    // (a wave that has its rows to itself writes them out as they are)
-    const bool alone = SHARED && (NW >> done.lr) == 1;
-    if (alone) {
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt) {
-        const float l = rows_sum(l_run[qt]);
-        const int row = rb + 16 * qt + l16;
-        if (row < done.nrows) {
-          const int rr = done.row0 + row, tt = rr / G, gg = rr - tt * G;
-          const float L = l == 0.f ? 1.f : l;
-          const long slot = ((long)done.part * Hkv + done.kvh) * A.part_rows + row;
-          uint16_t* o = A.out + ((long)(done.q_start + tt) * Hq + done.kvh * G + gg) * D + 4 * lg;
-#pragma unroll
-          for (int c = 0; c < CT; ++c) {
-            const lsk_f32x4 v = oacc[qt][c];
-            if (done.part < 0) {
-              lsk_u32x2_u pk;
-              pk[0] = (uint32_t)f2bf(v[0] / L) | ((uint32_t)f2bf(v[1] / L) << 16);
-              pk[1] = (uint32_t)f2bf(v[2] / L) | ((uint32_t)f2bf(v[3] / L) << 16);
-              *(lsk_u32x2_u*)(o + 16 * c) = pk;
-            } else {
-              *(lsk_f32x4*)(A.o_part + slot * D + 16 * c + 4 * lg) = v;
-            }
-          }
-          if (done.part >= 0 && lg == 0) {
-            A.ml_part[slot * 2 + 0] = m_run[qt];
-            A.ml_part[slot * 2 + 1] = l;
-          }
-        }
-      }
-    }
-    if (SHARED) __syncthreads();                     // every wave is past its reads of Q
     int tm = tid;
     asm volatile("" : "+v"(tm));                     // (no address of the merge is kept in registers across the steps)
     const int m16 = tm & 15, mg = (tm & 63) >> 4;
 #pragma unroll
     for (int p0 = 0; p0 < QT; p0 += MT) {
-      if (alone || 16 * p0 >= done.nrows) break;
+      if (16 * p0 >= done.nrows) break;
 #pragma unroll
       for (int qt = p0; qt < p0 + MT && qt < QT; ++qt) {
         const float l = rows_sum(l_run[qt]);
@@ -545,14 +532,235 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
         }
       };
       if (QREG || !TREE || done.lr == 0) merge(std::integral_constant<int, NW>{});
-      else if (done.lr == 1) merge(std::integral_constant<int, NW / 2>{});
-      else merge(std::integral_constant<int, NW / 4>{});
-      if (!SHARED && p0 == 0 && cur.nrows > 0) q_store(cur);  // (every wave is past its steps)
+      else merge(std::integral_constant<int, NW / 2>{});
+      if (p0 == 0 && cur.nrows > 0) q_store(cur);       // (every wave is past its steps)
       __syncthreads();
     }
-    if (SHARED && cur.nrows > 0) {
-      q_store(cur);
-      __syncthreads();
+  }
+}
+
+// Trees of more rows: an item of four or eight row groups of 32 rows, whose waves read the same K and V.  Two steps' at a
+// time go through LDS, in two buffers: each wave reading them for itself takes up to eight times the 64 bytes per clock
+// of the CU's cache (32 trees of 64 nodes, 8B heads: OLDSTEP us per 32 positions against NEWSTEP).  Q stays in registers.
+// A wave with eight row groups takes both steps, with four every other one; then the two waves of a row group are merged.
+template <int D, bool KV8>
+__global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_tree_kernel(const CacheAttnArgs A,
+                                                                        const int32_t* __restrict__ items) {
+  constexpr int STEP = KV8 ? 64 : 32, HV = STEP / 32, NE = 8 * HV, KF = D / 32, CT = D / 16, NW = ATTN_WAVES, QT = 2;
+  constexpr uint32_t ALL = NE == 16 ? 0xffffu : 0xffu;
+  constexpr int UNITS = 2 * CT, UPW = 2 * UNITS / NW;  // 1 KiB fragments of a step, K's then V's; of two steps, per wave
+  constexpr int BUF = 2 * UNITS * 1024;
+  __shared__ __attribute__((aligned(16))) char s_buf[2 * BUF];
+  __shared__ float s_ml[4][2][16 * QT];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = A.G, Hkv = A.Hkv;
+  const int32_t* wk = items + (long)blockIdx.x * 8;
+  const int q_start = wk[0], row0 = wk[1], nrows = wk[2] & 1023, lr = (wk[2] >> 10) & 3, kvh = wk[2] >> 12;
+  const int kv_lo = wk[3], kv_hi = wk[4], part = wk[5], pos0 = wk[6], crow = wk[7];
+  const int rb = (wave & ((1 << lr) - 1)) * 16 * QT, rank = wave >> lr;
+  const int own = lr == 3 ? 1 : 2;                   // steps from one of a wave's to the next
+  const Stripe sr = cache_stripe<D, KV8>(A, crow, kvh, kv_hi);
+  auto ld = [&](__amdgpu_buffer_rsrc_t rs, int vo, int so) -> lsk_i32x4 {
+    return __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, vo, so, 0));
+  };
+  lsk_i32x4 st[UPW], ksr, vsr;
+  auto st_load = [&](int sb) {
+#pragma unroll
+    for (int i = 0; i < UPW; ++i) {
+      const int u = wave * UPW + i, w = u % UNITS;   // (a wave's fragments are all of K or all of V)
+      const int so = (sb / STEP + u / UNITS) * 64 * D + w % CT * 1024;
+      st[i] = ld(w < CT ? sr.k : sr.v, w < CT ? 16 * lane : 64 * l16 + 16 * lg, so);
+    }
+  };
+  auto st_write = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < UPW; ++i) *(lsk_i32x4*)(s_buf + buf * BUF + (wave * UPW + i) * 1024 + 16 * lane) = st[i];
+  };
+  auto load_ks = [&](int sb) {
+    if constexpr (KV8) ksr = ld(sr.ks, 16 * (l16 >> 2), sb);
+  };
+  auto load_vs = [&](int sb) {
+    if constexpr (KV8) vsr = ld(sr.vs, 16 * lg, sb);
+  };
+  st_load(kv_lo);
+  load_ks(kv_lo + STEP * rank);
+  load_vs(kv_lo + STEP * rank);
+  lsk_bf16x8 qf[QT][KF];
+  int qpos[QT];                                      // the row's own slot; -1: no such row
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int rl = rb + 16 * qt + l16, r = row0 + min(rl, nrows - 1), t = r / G, g = r - t * G;
+    const uint16_t* q = A.q + (long)(q_start + t) * A.q_st + (long)(kvh * G + g) * A.q_sh;
+    qpos[qt] = rl < nrows ? pos0 + t : -1;
+#pragma unroll
+    for (int f = 0; f < KF; ++f)
+      qf[qt][f] = __builtin_bit_cast(lsk_bf16x8,
+                                     *(const lsk_u32x4_u*)(q + (KV8 ? 64 * (f >> 1) + 16 * lg + 8 * (f & 1) : 32 * f + 8 * lg)));
+  }
+  lsk_f32x4 oacc[QT][CT];
+  float m_run[QT], l_run[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    m_run[qt] = -INFINITY;
+    l_run[qt] = 0.f;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) oacc[qt][c] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  // one step from LDS (as in cache_attn_kernel)
+  auto step = [&](auto full_, int sb, const char* src) {
+    constexpr bool FULL = decltype(full_)::value;
+    lsk_i32x4 vr[CT];
+    auto get_v = [&]() {
+#pragma unroll
+      for (int c = 0; c < CT; ++c) vr[c] = *(const lsk_i32x4*)(src + (CT + c) * 1024 + 16 * lane);
+    };
+    uint64_t odd = 0;
+    uint32_t reads[QT];
+    if constexpr (!FULL) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        const int s0 = sb + NE * lg, n = min(kv_hi - 1, qpos[qt]) - s0 + 1, t = max(qpos[qt] - pos0, 0);
+        reads[qt] = (n >= NE ? ALL : n <= 0 ? 0u : (1u << n) - 1u) &
+                    mask_window(A.mask + (long)(q_start + t) * A.W, A.W, s0 - pos0);
+      }
+    }
+    constexpr int AT = KV8 ? 1 : 2;                  // 16-slot tiles at a time: their products are independent chains
+    lsk_f32x4 sacc[QT][2 * HV];
+#pragma unroll
+    for (int a0 = 0; a0 < 2 * HV; a0 += AT) {
+      ORDER();
+      lsk_bf16x8 kf[AT][KF];
+#pragma unroll
+      for (int a = 0; a < AT; ++a) {
+        if constexpr (KV8) {
+          const float sc = exp_bits(((uint32_t)ksr[a0 + a] >> (8 * (l16 & 3))) & 255u);
+#pragma unroll
+          for (int f = 0; f < KF; f += 2) {
+            const lsk_i32x4 x = *(const lsk_i32x4*)(src + ((a0 + a) * (KF / 2) + (f >> 1)) * 1024 + 16 * lane);
+            kf[a][f] = codes_to_bf16(x[0], x[1], sc);
+            kf[a][f + 1] = codes_to_bf16(x[2], x[3], sc);
+          }
+        } else {
+#pragma unroll
+          for (int f = 0; f < KF; ++f) kf[a][f] = *(const lsk_bf16x8*)(src + ((a0 + a) * KF + f) * 1024 + 16 * lane);
+        }
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) sacc[qt][a0 + a] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int f = 0; f < KF; ++f)
+#pragma unroll
+        for (int a = 0; a < AT; ++a)
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+            sacc[qt][a0 + a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a][f], qf[qt][f], sacc[qt][a0 + a], 0, 0, 0);
+    }
+    ORDER();
+    load_ks(sb + own * STEP);
+    if constexpr (!KV8) get_v();                     // (8-bit: two more tiles of scores are live)
+    lsk_bf16x8 pb[QT][HV];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      if constexpr (KV8) ORDER();
+      softmax_tile<KV8, FULL>(sacc[qt], FULL ? ALL : reads[qt], vsr, A.scale_log2, m_run[qt], l_run[qt], oacc[qt], pb[qt]);
+    }
+    load_vs(sb + own * STEP);
+    if constexpr (KV8) {
+      ORDER();
+      get_v();
+    }
+    if constexpr (!FULL) odd = clear_odd<KV8>(vr, kv_hi - (sb + NE * lg));
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      lsk_bf16x8 vf[HV];
+      if constexpr (KV8) {
+#pragma unroll
+        for (int hv = 0; hv < HV; ++hv) vf[hv] = codes_to_bf16(vr[c][2 * hv], vr[c][2 * hv + 1], 1.f);
+      } else {
+        vf[0] = __builtin_bit_cast(lsk_bf16x8, vr[c]);
+      }
+#pragma unroll
+      for (int hv = 0; hv < HV; ++hv)
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+          oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[hv], pb[qt][hv], oacc[qt][c], 0, 0, 0);
+    }
+    if constexpr (!FULL) add_odd<KV8, true>(A, sr.v, odd, sb, q_start, pos0, qpos, oacc);
+  };
+  st_write(0);
+  st_load(kv_lo + 2 * STEP);
+  int s2 = kv_lo, buf = 0;
+  auto pairs = [&](auto full_, int end) {            // the pairs of steps that start before `end`
+    for (; s2 < end; s2 += 2 * STEP, buf ^= 1) {
+      __syncthreads();                               // (the other buffer's readers are done, this one is written)
+      for (int j = rank; j < 2; j += own) {
+        const int sb = s2 + j * STEP;
+        if (sb >= kv_hi || rb >= nrows) break;
+        step(full_, sb, s_buf + buf * BUF + j * UNITS * 1024);
+      }
+      st_write(buf ^ 1);
+      st_load(s2 + 4 * STEP);
+    }
+  };
+  pairs(std::true_type{}, min(kv_hi, pos0) - 2 * STEP + 1);  // (every row reads them whole)
+  pairs(std::false_type{}, kv_hi);
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) l_run[qt] = rows_sum(l_run[qt]);
+  if (lr == 2) {                                     // O = e_0 O_0 + e_1 O_1, e_w = exp2(m_w - max m), l likewise
+    __syncthreads();
+    lsk_f32x4* so = (lsk_f32x4*)s_buf + (wave & 3) * QT * CT * 64 + lane;
+    if (rank == 1) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        if (lg == 0) {
+          s_ml[wave & 3][0][16 * qt + l16] = m_run[qt];
+          s_ml[wave & 3][1][16 * qt + l16] = l_run[qt];
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) so[(qt * CT + c) * 64] = oacc[qt][c];
+      }
+    }
+    __syncthreads();
+    if (rank == 1) return;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const float m1 = s_ml[wave & 3][0][16 * qt + l16], M = fmaxf(m_run[qt], m1);
+      const float e0 = m_run[qt] == -INFINITY ? 0.f : m_run[qt] == M ? 1.f : fast_exp2(m_run[qt] - M);
+      const float e1 = m1 == -INFINITY ? 0.f : m1 == M ? 1.f : fast_exp2(m1 - M);
+      m_run[qt] = M;
+      l_run[qt] = e0 * l_run[qt] + e1 * s_ml[wave & 3][1][16 * qt + l16];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        const lsk_f32x4 o1 = so[(qt * CT + c) * 64];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) oacc[qt][c][i] = e0 * oacc[qt][c][i] + e1 * o1[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int rl = rb + 16 * qt + l16;
+    if (rl >= nrows) continue;
+    const int r = row0 + rl, t = r / G, g = r - t * G;
+    const float L = l_run[qt] == 0.f ? 1.f : l_run[qt];  // (nothing read: O is 0)
+    const long slot = ((long)part * Hkv + kvh) * A.part_rows + rl;
+    uint16_t* o = A.out + ((long)(q_start + t) * G * Hkv + kvh * G + g) * D + 4 * lg;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const lsk_f32x4 v = oacc[qt][c];
+      if (part < 0) {
+        lsk_u32x2_u pk;
+        pk[0] = (uint32_t)f2bf(v[0] / L) | ((uint32_t)f2bf(v[1] / L) << 16);
+        pk[1] = (uint32_t)f2bf(v[2] / L) | ((uint32_t)f2bf(v[3] / L) << 16);
+        *(lsk_u32x2_u*)(o + 16 * c) = pk;
+      } else {
+        *(lsk_f32x4*)(A.o_part + slot * D + 16 * c + 4 * lg) = v;
+      }
+    }
+    if (part >= 0 && lg == 0) {
+      A.ml_part[slot * 2 + 0] = m_run[qt];
+      A.ml_part[slot * 2 + 1] = l_run[qt];
     }
   }
 }
@@ -775,9 +983,10 @@ extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int
   }
   const int tiles = most <= 16 ? 1 : most <= 32 || tree || head_dim == 128 ? 2 : 3;
   struct It { int32_t rec[8]; int cost; };
-  thread_local std::vector<It> items;
+  thread_local std::vector<It> items, shared;
   thread_local std::vector<int32_t> groups;
   items.clear();
+  shared.clear();
   groups.clear();
   long np = 0;
   int part_rows = 16 * tiles, used = 1;
@@ -804,14 +1013,16 @@ extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int
         const int steps = (hi - lo + step * (ATTN_WAVES >> lr) - 1) / (step * (ATTN_WAVES >> lr));
         const int cost = steps * (10 + 5 * (tiles - 1)) + 20 + 6 * (tiles - 1);
         for (int h = 0; h < n_kv_heads; ++h)
-          items.push_back({{bm[0], (int32_t)row0, nrows | (lr << 10) | (h << 12), lo, hi,
+          (lr < 2 ? items : shared).push_back({{bm[0], (int32_t)row0, nrows | (lr << 10) | (h << 12), lo, hi,
                             ns > 1 ? (int32_t)(np + sp) : -1, pos0, bm[3]}, cost});
       }
       if (ns > 1) np += ns;
     }
   }
-  LSK_REQUIRE(np < (1L << 24) && (long)items.size() < (1L << 28), LSK_ESHAPE, "%s: too many work items", what);
-  std::stable_sort(items.begin(), items.end(), [](const It& a, const It& b) { return a.cost > b.cost; });
+  LSK_REQUIRE(np < (1L << 24) && (long)(items.size() + shared.size()) < (1L << 28), LSK_ESHAPE, "%s: too many work items", what);
+  const auto longer = [](const It& a, const It& b) { return a.cost > b.cost; };
+  std::stable_sort(items.begin(), items.end(), longer);
+  std::stable_sort(shared.begin(), shared.end(), longer);
   thread_local std::vector<std::pair<long, int>> heap;
   thread_local std::vector<int> slot_of, rank, count;
   heap.clear();
@@ -830,9 +1041,9 @@ extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int
     top.first += items[i].cost;
     std::push_heap(heap.begin(), heap.end(), later);
   }
-  const long len = (long)groups.size() + 8L * n_slots * rounds;
+  const long len = (long)groups.size() + 8L * n_slots * rounds + 8L * (long)shared.size();
   counts[0] = n_tokens; counts[1] = (long)groups.size() / 8; counts[2] = np; counts[3] = rounds; counts[4] = tiles;
-  counts[5] = part_rows; counts[6] = len; counts[7] = used;
+  counts[5] = part_rows; counts[6] = len; counts[7] = used; counts[8] = (long)shared.size();
   if (meta == nullptr) return 0;
   LSK_REQUIRE(len <= meta_cap, LSK_EWORKSPACE, "%s: %ld metadata words > %ld", what, len, meta_cap);
   std::copy(groups.begin(), groups.end(), meta);
@@ -840,6 +1051,8 @@ extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int
   std::fill(recs, recs + 8L * n_slots * rounds, 0);
   for (size_t i = 0; i < items.size(); ++i)
     std::copy(items[i].rec, items[i].rec + 8, recs + ((long)slot_of[i] * rounds + rank[i]) * 8);
+  for (size_t i = 0; i < shared.size(); ++i)
+    std::copy(shared[i].rec, shared[i].rec + 8, recs + ((long)n_slots * rounds + (long)i) * 8);
   return 0;
 }
 
@@ -854,14 +1067,14 @@ static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Checks and launches shared by the two entry points; kv8: the cache is 8-bit.
 static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t* groups, int n_groups, int n_parts,
-                      int n_slots, int tiles, int row_groups, int head_dim, float scale, void* workspace, size_t ws_bytes,
+                      int n_slots, int n_shared, int tiles, int row_groups, int head_dim, float scale, void* workspace, size_t ws_bytes,
                       hipStream_t s) {
   LSK_REQUIRE(head_dim == 64 || head_dim == 128, LSK_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128)", what,
               head_dim);
   LSK_REQUIRE(tiles == 1 || tiles == 2 || (tiles == 3 && head_dim == 64 && a.mask == nullptr), LSK_EARG,
               "%s: a plan of %d tiles", what, tiles);
-  LSK_REQUIRE(row_groups == 1 || a.mask != nullptr, LSK_EARG, "%s: a tree's plan (%d row groups) without a mask", what,
-              row_groups);
+  LSK_REQUIRE((row_groups == 1 && n_shared == 0) || a.mask != nullptr, LSK_EARG,
+              "%s: a tree's plan (%d row groups) without a mask", what, row_groups);
   LSK_REQUIRE(n_slots > 0 && n_groups >= 0 && n_parts >= 0 && (n_groups > 0) == (n_parts > 0), LSK_EARG,
               "%s: a plan of %d slots, %d groups and %d partial slots", what, n_slots, n_groups, n_parts);
   LSK_REQUIRE(a.S % ATTN_TILE == 0 && (long)a.S * head_dim * 2 <= 0x7fffffffL, LSK_ESHAPE,
@@ -880,6 +1093,7 @@ static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t
   }
   LSK_REQUIRE(scale >= 0.f && scale <= 1e30f, LSK_EARG, "%s: scale %g (not negative)", what, (double)scale);
   a.scale_log2 = scale * 1.4426950408889634f;
+  int rc = 0;
 #define LSK_CACHE_ATTN(DD, QT, K8, TR) cache_attn_kernel<DD, QT, K8, TR><<<n_slots, 64 * ATTN_WAVES, 0, s>>>(a)
 #define LSK_CACHE_ATTN_D(K8, TR)                                            \
   do {                                                                      \
@@ -888,14 +1102,23 @@ static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t
     else if (tiles == 1) LSK_CACHE_ATTN(64, 1, K8, TR);                     \
     else if (tiles == 2) LSK_CACHE_ATTN(64, 2, K8, TR);                     \
   } while (0)
-  if (!kv8) LSK_CACHE_ATTN_D(false, true);
+  if (a.n_rounds == 0) ;
+  else if (!kv8) LSK_CACHE_ATTN_D(false, true);
   else if (a.mask != nullptr) LSK_CACHE_ATTN_D(true, true);
   else if (tiles == 3) LSK_CACHE_ATTN(64, 3, true, false);
   else LSK_CACHE_ATTN_D(true, false);
 #undef LSK_CACHE_ATTN_D
 #undef LSK_CACHE_ATTN
-  int rc = lsk_check_launch(what);
-  if (rc || n_groups == 0) return rc;
+  if (a.n_rounds > 0 && (rc = lsk_check_launch(what))) return rc;
+  if (n_shared > 0) {
+    const int32_t* items = a.recs + 8L * n_slots * a.n_rounds;
+    if (head_dim == 128 && kv8) cache_tree_kernel<128, true><<<n_shared, 64 * ATTN_WAVES, 0, s>>>(a, items);
+    else if (head_dim == 128) cache_tree_kernel<128, false><<<n_shared, 64 * ATTN_WAVES, 0, s>>>(a, items);
+    else if (kv8) cache_tree_kernel<64, true><<<n_shared, 64 * ATTN_WAVES, 0, s>>>(a, items);
+    else cache_tree_kernel<64, false><<<n_shared, 64 * ATTN_WAVES, 0, s>>>(a, items);
+    if ((rc = lsk_check_launch(what))) return rc;
+  }
+  if (n_groups == 0) return 0;
   const dim3 cg(n_groups, a.Hkv, (a.part_rows + 3) / 4);
   if (head_dim == 128)
     cache_combine_kernel<128><<<cg, 256, 0, s>>>(groups, a.o_part, a.ml_part, a.out, a.G, a.Hkv, a.part_rows);
@@ -916,27 +1139,28 @@ static int shape_args(const char* what, const void* q, const void* kc, const voi
 extern "C" int lsk_kv8_attn(const void* q, long q_stride_t, long q_stride_h, const void* k8, const void* v8,
                             const void* k_exp, const void* v_exp, const uint32_t* mask, int mask_words,
                             const int32_t* groups, int n_groups, int n_parts, const int32_t* recs, int n_rounds,
-                            int n_slots, int tiles, int row_groups, int part_rows, void* out, int n_heads, int n_kv_heads, int head_dim,
+                            int n_slots, int n_shared, int tiles, int row_groups, int part_rows, void* out, int n_heads, int n_kv_heads, int head_dim,
                             int max_seq, float scale, void* workspace, size_t ws_bytes, void* stream) {
   const char* what = "lsk_kv8_attn";
   if (int rc = shape_args(what, q, k8, v8, out, n_heads, n_kv_heads, head_dim, max_seq, q_stride_t, q_stride_h))
     return rc;
   LSK_REQUIRE(k_exp && v_exp && (mask == nullptr || mask_words > 0), LSK_EARG, "%s: null scales or an empty mask",
               what);
-  LSK_REQUIRE(n_rounds >= 0, LSK_EARG, "%s: a plan of %d rounds", what, n_rounds);
-  if (n_rounds == 0) return 0;
+  LSK_REQUIRE(n_rounds >= 0 && n_shared >= 0, LSK_EARG, "%s: a plan of %d rounds and %d shared items", what, n_rounds,
+              n_shared);
+  if (n_rounds == 0 && n_shared == 0) return 0;
   LSK_REQUIRE(recs != nullptr, LSK_EARG, "%s: null pointer", what);
   const CacheAttnArgs a = {(const uint16_t*)q, q_stride_t, q_stride_h, k8, v8, (const uint8_t*)k_exp,
                            (const uint8_t*)v_exp, mask, mask_words, recs, n_rounds, (uint16_t*)out, nullptr, nullptr,
                            part_rows, n_heads / n_kv_heads, n_kv_heads, max_seq, 0.f};
-  return cache_attn(what, true, a, groups, n_groups, n_parts, n_slots, tiles, row_groups, head_dim, scale, workspace,
+  return cache_attn(what, true, a, groups, n_groups, n_parts, n_slots, n_shared, tiles, row_groups, head_dim, scale, workspace,
                     ws_bytes, (hipStream_t)stream);
 }
 
 extern "C" int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_stride_h, const void* kcache,
                              const void* vcache, const uint32_t* mask, int mask_words, const int32_t* works, int n_works,
                              int rows_cap, const int32_t* groups, int n_groups, int n_parts, const int32_t* recs,
-                             int n_rounds, int n_slots, int tiles, int row_groups, int part_rows, void* out, int n_heads,
+                             int n_rounds, int n_slots, int n_shared, int tiles, int row_groups, int part_rows, void* out, int n_heads,
                              int n_kv_heads, int head_dim, int max_seq, float scale, void* workspace, size_t ws_bytes,
                              void* stream) {
   const char* what = "lsk_tree_attn";
@@ -947,13 +1171,14 @@ extern "C" int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_s
   hipStream_t s = (hipStream_t)stream;
   const int G = n_heads / n_kv_heads;
   if (dtype == LSK_DTYPE_BF16) {
-    LSK_REQUIRE(n_rounds >= 0, LSK_EARG, "%s: a plan of %d rounds", what, n_rounds);
-    if (n_rounds == 0) return 0;
+    LSK_REQUIRE(n_rounds >= 0 && n_shared >= 0, LSK_EARG, "%s: a plan of %d rounds and %d shared items", what, n_rounds,
+                n_shared);
+    if (n_rounds == 0 && n_shared == 0) return 0;
     LSK_REQUIRE(recs != nullptr, LSK_EARG, "%s: null pointer", what);
     const CacheAttnArgs a = {(const uint16_t*)q, q_stride_t, q_stride_h, kcache, vcache, nullptr, nullptr, mask,
                              mask_words, recs, n_rounds, (uint16_t*)out, nullptr, nullptr, part_rows, G, n_kv_heads,
                              max_seq, 0.f};
-    return cache_attn(what, false, a, groups, n_groups, n_parts, n_slots, tiles, row_groups, head_dim, scale, workspace,
+    return cache_attn(what, false, a, groups, n_groups, n_parts, n_slots, n_shared, tiles, row_groups, head_dim, scale, workspace,
                       ws_bytes, s);
   }
   LSK_REQUIRE(n_works >= 0 && rows_cap > 0 && rows_cap % 16 == 0 && rows_cap <= ATTN_ROWS, LSK_EARG,

@@ -813,30 +813,31 @@ def test_entry_points_refuse_bad_arguments():
     assert r(1, P, P, P, P, P, P, P, None, 4, 2, 64, 3, 128, None) == -1
     assert r(1, P, P, P, P, P, P, P, P, 4, 2, 32, 3, 128, None) == -3
     assert r(1, P, P, P, P, P, P, P, P, 0, 2, 64, 3, 128, None) == 0
-    # q, strides, k8, v8, exponents, mask, words | groups, n_groups, n_parts, recs, rounds, slots, tiles, row groups, part
-    # rows | out, heads, KV heads, D, S, scale, workspace, bytes, stream
-    ok = [P, 512, 64, P, P, P, P, None, 0, None, 0, 0, P, 1, 1, 1, 1, 16, P, 8, 2, 64, 128, 0.125, None, 0, None]
+    # q, strides, k8, v8, exponents, mask, words | groups, n_groups, n_parts, recs, rounds, slots, shared, tiles, row
+    # groups, part rows | out, heads, KV heads, D, S, scale, workspace, bytes, stream
+    ok = [P, 512, 64, P, P, P, P, None, 0, None, 0, 0, P, 1, 1, 0, 1, 1, 16, P, 8, 2, 64, 128, 0.125, None, 0, None]
     k8 = lambda **kw: lib.lsk_kv8_attn(*[kw.get(f"a{i}", x) for i, x in enumerate(ok)])  # noqa: E731
-    assert k8(a0=None) == -1 and k8(a5=None) == -1 and k8(a12=None) == -1 and k8(a7=P) == -1 and k8(a18=None) == -1
-    assert k8(a15=4) == -1 and k8(a15=3, a21=128) == -1 and k8(a15=3, a7=P, a8=1) == -1 and k8(a16=2) == -1
+    assert k8(a0=None) == -1 and k8(a5=None) == -1 and k8(a12=None) == -1 and k8(a7=P) == -1 and k8(a19=None) == -1
+    assert k8(a16=4) == -1 and k8(a16=3, a22=128) == -1 and k8(a16=3, a7=P, a8=1) == -1 and k8(a17=2) == -1
+    assert k8(a15=1) == -1 and k8(a15=-1) == -1 and k8(a24=-0.5) == -1 and k8(a24=math.nan) == -1
     assert k8(a14=0) == -1 and k8(a10=1) == -1 and k8(a13=-1) == -1
-    assert k8(a19=7) == -2 and k8(a22=96) == -2 and k8(a21=32) == -3 and k8(a3=24) == -1 and k8(a1=-1) == -2
-    assert k8(a10=1, a11=3) == -4 and k8(a10=1, a11=3, a9=P, a24=P, a25=100) == -4   # partials without their workspace
-    assert k8(a10=1, a11=3, a9=P, a24=P, a25=1 << 20, a17=8) == -1                   # rows per partial below a tile
-    assert k8(a22=1 << 25) == -2                                                     # a stripe of 2 GiB and more
+    assert k8(a20=7) == -2 and k8(a23=96) == -2 and k8(a22=32) == -3 and k8(a3=24) == -1 and k8(a1=-1) == -2
+    assert k8(a10=1, a11=3) == -4 and k8(a10=1, a11=3, a9=P, a25=P, a26=100) == -4   # partials without their workspace
+    assert k8(a10=1, a11=3, a9=P, a25=P, a26=1 << 20, a18=8) == -1                   # rows per partial below a tile
+    assert k8(a23=1 << 25) == -2                                                     # a stripe of 2 GiB and more
     assert k8(a13=0) == 0
-    ok2 = [1, P, 512, 64, P, P, P, 1, None, 0, 0, None, 0, 0, P, 1, 1, 1, 1, 16, P, 8, 2, 64, 128, 0.125, None, 0, None]
+    ok2 = [1, P, 512, 64, P, P, P, 1, None, 0, 0, None, 0, 0, P, 1, 1, 0, 1, 1, 16, P, 8, 2, 64, 128, 0.125, None, 0, None]
     tr = lambda **kw: lib.lsk_tree_attn(*[kw.get(f"a{i}", x) for i, x in enumerate(ok2)])  # noqa: E731
-    assert tr(a6=None) == -1 and tr(a7=0) == -1 and tr(a0=2) == -3 and tr(a14=None) == -1 and tr(a23=96) == -3
+    assert tr(a6=None) == -1 and tr(a7=0) == -1 and tr(a0=2) == -3 and tr(a14=None) == -1 and tr(a24=96) == -3
     assert tr(a0=0) == -1 and tr(a0=0, a9=1, a10=16) == -1 and tr(a0=0, a9=1, a10=24, a8=P) == -1
-    assert tr(a0=0, a9=1, a10=16, a8=P, a23=80) == -3 and tr(a0=0, a10=16) == 0 and tr(a15=0) == 0
-    cnt = (ctypes.c_long * 8)()
+    assert tr(a0=0, a9=1, a10=16, a8=P, a24=80) == -3 and tr(a0=0, a10=16) == 0 and tr(a15=0) == 0
+    cnt = (ctypes.c_long * 9)()
     blk = (ctypes.c_int32 * 4)(0, 700, 40, 0)
     plan = lambda **kw: lib.lsk_cache_attn_plan(*[kw.get(f"a{i}", x) for i, x in enumerate(  # noqa: E731
         [blk, 1, 4, 256, 2, 128, 1, 1, 8, 256, None, 0, cnt])])
-    assert plan() == 0 and list(cnt)[:3] == [40, 1, 3] and cnt[4] == 2 and cnt[7] == 8
+    assert plan() == 0 and list(cnt)[:3] == [40, 1, 3] and cnt[4] == 2 and cnt[7] == 8 and cnt[8] == 6
     assert plan(a3=100) == -2 and plan(a8=3) == -2 and plan(a5=96) == -3 and plan(a0=None) == -1 and plan(a12=None) == -1
-    assert plan(a10=blk, a11=4) == -4 and plan(a1=0) == 0 and cnt[3] == 0
+    assert plan(a10=blk, a11=4) == -4 and plan(a1=0) == 0 and cnt[3] == cnt[8] == 0
     blk[1] = 64 * 128
     assert plan(a3=64) == -2                                                         # more than 128 splits
     blk[1] = -1
@@ -860,7 +861,7 @@ def test_plans_refuse_blocks_outside_the_cache():
     lsk = _lsk()
     cache = lsk.KV8.zeros(2, 2, 128, 64, "cpu")
     plan = lsk.AttnPlan([(0, 3, 2, 1), (2, 0, 0, 0), (2, 127, 1, 0)], 4, cache)
-    assert plan.n_tokens == 3 and plan.causal.n_rounds > 0 and plan.tree.n_rounds > 0 and plan.split == 512
+    assert plan.n_tokens == 3 and plan.causal.n_items > 0 and plan.tree.n_items > 0 and plan.split == 512
     for b in ([(0, 3, 2, 2)], [(0, 3, 2, -1)], [(0, 127, 2, 0)], [(0, -1, 2, 0)], [(1, 0, 2, 0)], [(0, 0, -1, 0)]):
         with pytest.raises(ValueError):
             lsk.AttnPlan(b, 4, cache)
@@ -883,11 +884,15 @@ def test_plans_refuse_blocks_outside_the_cache():
 
 def _items(plan, launch):
     """(row group rows, wave rows) of every work item of a plan: [(q_start, row0, nrows, groups, kvh, lo, hi, part)]"""
-    recs = launch.recs.numpy().reshape(launch.n_slots, launch.n_rounds, 8)
-    out = []
+    one = launch.n_slots * launch.n_rounds * 8
+    recs = launch.recs.numpy()[:one].reshape(launch.n_slots, launch.n_rounds, 8)
+    shared = launch.recs.numpy()[one:].reshape(launch.n_shared, 8)     # items of four or eight row groups
+    assert all(r[2] >> 10 & 3 >= 2 for r in shared)
+    out = [(r[0], r[1], r[2] & 1023, 1 << (r[2] >> 10 & 3), r[2] >> 12, r[3], r[4], r[5]) for r in shared]
     for slot in recs:
         live = [r for r in slot if r[2] & 1023]
         assert all((r[2] & 1023) == 0 for r in slot[len(live):])      # a slot's items come first
+        assert all(r[2] >> 10 & 3 < 2 for r in live)
         out += [(r[0], r[1], r[2] & 1023, 1 << (r[2] >> 10 & 3), r[2] >> 12, r[3], r[4], r[5]) for r in live]
     return out
 

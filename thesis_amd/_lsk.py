@@ -80,9 +80,9 @@ _SIGS = {
     "lsk_kv8_read": (_I, [_I] + [_P] * 8 + [_I] * 5 + [_P]),
     "lsk_cache_attn_plan": (_I, [_P] + [_I] * 9 + [_P, _L, _P]),
     "lsk_cache_attn_workspace_bytes": (_Z, [_I, _I, _I, _I]),
-    "lsk_kv8_attn": (_I, [_P, _L, _L] + [_P] * 5 + [_I, _P, _I, _I, _P] + [_I] * 5 + [_P] + [_I] * 4 + [_F, _P, _Z,
+    "lsk_kv8_attn": (_I, [_P, _L, _L] + [_P] * 5 + [_I, _P, _I, _I, _P] + [_I] * 6 + [_P] + [_I] * 4 + [_F, _P, _Z,
                           _P]),
-    "lsk_tree_attn": (_I, [_I, _P, _L, _L, _P, _P, _P, _I, _P, _I, _I, _P, _I, _I, _P] + [_I] * 5 + [_P] + [_I] * 4 +
+    "lsk_tree_attn": (_I, [_I, _P, _L, _L, _P, _P, _P, _I, _P, _I, _I, _P, _I, _I, _P] + [_I] * 6 + [_P] + [_I] * 4 +
                       [_F, _P, _Z, _P]),
     "lsk_tree_masks": (_I, [_P, _P, _P, _I, _I, _I, _P, _I, _P, _P]),
     "lsk_tree_accept": (_I, [_P] * 5 + [_I, _I, _I] + [_P] * 4),
@@ -666,11 +666,13 @@ class _Launch:
     """One lsk_cache_attn_plan on the device, and its arguments of a launch."""
 
     def __init__(self, groups: torch.Tensor, recs: torch.Tensor, n_groups: int, n_parts: int, n_rounds: int, n_slots: int,
-                 tiles: int, row_groups: int, part_rows: int, ws_bytes: int):
+                 n_shared: int, tiles: int, row_groups: int, part_rows: int, ws_bytes: int):
         self.groups, self.recs, self.n_groups, self.n_parts, self.n_rounds = groups, recs, n_groups, n_parts, n_rounds
-        self.n_slots, self.tiles, self.row_groups, self.part_rows, self.ws_bytes = \
-            n_slots, tiles, row_groups, part_rows, ws_bytes
-        self.args = (_ptr(groups), n_groups, n_parts, _ptr(recs), n_rounds, n_slots, tiles, row_groups, part_rows)
+        self.n_slots, self.n_shared, self.tiles, self.row_groups, self.part_rows, self.ws_bytes = \
+            n_slots, n_shared, tiles, row_groups, part_rows, ws_bytes
+        self.n_items = n_rounds + n_shared           # (0: nothing to launch)
+        self.args = (_ptr(groups), n_groups, n_parts, _ptr(recs), n_rounds, n_slots, n_shared, tiles, row_groups,
+                     part_rows)
 
 
 class AttnPlan:
@@ -717,16 +719,17 @@ class AttnPlan:
         return t.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else t
 
     def _plan(self, b: np.ndarray, group: int, Hkv: int, D: int, tree: bool, row_groups: int, n_slots: int) -> _Launch:
-        lib, cnt = load(), np.zeros(8, dtype=np.int64)
+        lib, cnt = load(), np.zeros(9, dtype=np.int64)
         args = (b.ctypes.data if len(b) else None, len(b), group, self.split, Hkv, D, int(self.kv8), int(tree),
                 row_groups, n_slots)
         _check(lib.lsk_cache_attn_plan(*args, None, 0, cnt.ctypes.data), "lsk_cache_attn_plan")
         meta = np.zeros(max(int(cnt[6]), 1), dtype=np.int32)
         _check(lib.lsk_cache_attn_plan(*args, meta.ctypes.data, meta.size, cnt.ctypes.data), "lsk_cache_attn_plan")
-        _, ng, parts, rounds, tiles, part_rows, _, used = (int(x) for x in cnt)
+        _, ng, parts, rounds, tiles, part_rows, _, used, shared = (int(x) for x in cnt)
         dev = self._upload(meta)
         ws = int(lib.lsk_cache_attn_workspace_bytes(parts, Hkv, part_rows, D)) if parts else 0
-        return _Launch(dev[:ng * 8], dev[ng * 8:], ng, parts, rounds, n_slots, tiles, used, part_rows, ws)
+        return _Launch(dev[:ng * 8], dev[ng * 8:], ng, parts, rounds, n_slots, shared, tiles, used, part_rows,
+                       ws)
 
 
 def _plan_call(what: str, q: torch.Tensor, plan: AttnPlan, launch, dims: tuple, kv8: bool, dtype: torch.dtype, mask,
@@ -764,7 +767,7 @@ def kv8_attn(q: torch.Tensor, cache: KV8, plan: AttnPlan, mask: torch.Tensor | N
     dev = _one_device(q, *cache, p.recs if p is not None else None, mask, out, workspace)
     dims = _, Hkv, S, D = cache.check("kv8_attn")
     scale, out, workspace, ws = _plan_call("kv8_attn", q, plan, p, dims, True, cache.k.dtype, mask, scale, out, workspace)
-    if p.n_rounds:
+    if p.n_items:
         _launch(dev, "lsk_kv8_attn", _ptr(q), q.stride(0), q.stride(1), *map(_ptr, cache), _ptr(mask),
                 mask.shape[1] if mask is not None else 0, *p.args, _ptr(out), plan.n_heads, Hkv, D, S, scale,
                 _ptr(workspace), ws)
@@ -787,8 +790,8 @@ def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, plan:
     _want("tree_attn", "V cache", vcache, kcache.dtype, (B, Hkv, S // 32, D, 32))
     scale, out, workspace, ws = _plan_call("tree_attn", q, plan, p, dims, False, kcache.dtype, mask, scale, out,
                                            workspace)
-    if p.n_rounds if p is not None else plan.n_works:
-        args = p.args if p is not None else (None, 0, 0, None, 0, 0, 0, 0, 0)
+    if p.n_items if p is not None else plan.n_works:
+        args = p.args if p is not None else (None, 0, 0, None, 0, 0, 0, 0, 0, 0)
         _launch(dev, "lsk_tree_attn", code, _ptr(q), q.stride(0), q.stride(1), _ptr(kcache), _ptr(vcache), _ptr(mask),
                 mask.shape[1], _ptr(plan.works), plan.n_works, plan.rows_cap, *args, _ptr(out), plan.n_heads, Hkv, D, S,
                 scale, _ptr(workspace), ws)
