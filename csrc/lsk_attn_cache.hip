@@ -8,8 +8,9 @@
 //
 //   out = sum_p w_p v_p / sum_p w_p,   w_p = exp2(s_p - max s),   s_p = scale log2(e) (q . k_p)
 //
-// Work items, records, splits and their merge are those of the ragged attention (lsk_attn_plan, lsk_attn_schedule): a
-// mask only takes away from the causal rule, so the same plan serves both.
+// Work items, their records and the splits of long contexts are lsk_cache_attn_plan's (below).  Two kernels walk them:
+// cache_attn_kernel, whose waves share the positions of up to two row groups of 32 rows, and cache_tree_kernel for trees
+// of more rows, whose waves share K and V.
 //
 // Both cache formats are read as 1 KiB fragments in lane order, 64 D bytes per block of STEP positions:
 //   bf16   STEP = 32: K fragment (a, f), lane 16 lg + l16: position 8 (l16 / 4) + 4 a + l16 % 4, d = 32 f + 8 lg .. + 7;
@@ -24,9 +25,9 @@
 // The weights are rounded to bf16 for the second product (relative 2^-9 each, independent of one another: it adds about
 // as much error as the rounding of the bf16 output); the sum of the weights is taken before that rounding.
 //
-// The 8 waves of a workgroup take the STEP-position steps of an item round robin and are merged in wave order through
-// LDS.  Which wave takes a step and every order of additions depend on absolute positions only: a row's result never
-// depends on what else is in the launch, and a chain over a bf16 cache gives the ragged attention's bits.
+// The waves of a row group take the steps round robin and are merged in wave order.  Which wave takes a step and every
+// order of additions depend on absolute positions only: a row's result never depends on what else is in the launch.  An
+// fp32 chain (every ancestor's bit set) gives the ragged attention's bits.
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -144,11 +145,12 @@ __device__ __forceinline__ uint64_t clear_odd(lsk_i32x4 (&vr)[CT], int nk) {
 // The non-finite values of V that clear_odd took out, for the rows that read them.
 template <bool KV8, bool TREE, int QT, int CT>
 __device__ __forceinline__ void add_odd(const CacheAttnArgs& A, __amdgpu_buffer_rsrc_t v, uint64_t odd, int sb,
-                                        int q_start, int pos0, const int (&qpos)[QT], lsk_f32x4 (&oacc)[QT][CT]) {
+                                        int q_start, int pos0, const int (&qpos)[QT], lsk_f32x4 (&oacc)[QT][CT],
+                                        int wide = 0) {
   constexpr int STEP = KV8 ? 64 : 32, D = 16 * CT;
   const int lg = (threadIdx.x & 63) >> 4;
   while (odd != 0ull) {                              // (rare: one slot after the other, few registers)
-    const int u = __builtin_ctzll(odd), kp = sb + u;
+    const int u = __builtin_ctzll(odd), kp = sb + u + (u & wide);  // (wide 0x18: groups of 8 slots, 16 apart)
     odd &= odd - 1;
     bool hit[QT];
 #pragma unroll
@@ -165,7 +167,7 @@ __device__ __forceinline__ void add_odd(const CacheAttnArgs& A, __amdgpu_buffer_
       for (int i = 0; i < 4; ++i) {
         ORDER();
         // V[kp][16 c + 4 lg + i]: a dim's slots of a block are 64 bytes in both formats
-        const int so = sb / STEP * 64 * D + (16 * c + i) * 64 + u * (KV8 ? 1 : 2);
+        const int so = kp / STEP * 64 * D + (16 * c + i) * 64 + kp % STEP * (KV8 ? 1 : 2);
         float x;
         if constexpr (KV8) {
           const uint32_t b = __builtin_amdgcn_raw_buffer_load_b8(v, 256 * lg, so, 0);
@@ -541,16 +543,22 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
 
 // Trees of more rows: an item of four or eight row groups of 32 rows, whose waves read the same K and V.  Two steps' at a
 // time go through LDS, in two buffers: each wave reading them for itself takes up to eight times the 64 bytes per clock
-// of the CU's cache (32 trees of 64 nodes, 8B heads: OLDSTEP us per 32 positions against NEWSTEP).  Q stays in registers.
+// of the CU's cache (32 trees of 64 nodes, 8B heads, 960
+// positions: 45 us; without LDS 67).  8-bit codes become bf16 on the way, once for all the waves.  Q stays in registers.
 // A wave with eight row groups takes both steps, with four every other one; then the two waves of a row group are merged.
+// Bound by the softmax's vector instructions beside the products: 32 positions of 256 rows take 0.9 us, of which the
+// matrix instructions are half.
 template <int D, bool KV8>
 __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_tree_kernel(const CacheAttnArgs A,
                                                                         const int32_t* __restrict__ items) {
-  constexpr int STEP = KV8 ? 64 : 32, HV = STEP / 32, NE = 8 * HV, KF = D / 32, CT = D / 16, NW = ATTN_WAVES, QT = 2;
-  constexpr uint32_t ALL = NE == 16 ? 0xffffu : 0xffu;
-  constexpr int UNITS = 2 * CT, UPW = 2 * UNITS / NW;  // 1 KiB fragments of a step, K's then V's; of two steps, per wave
-  constexpr int BUF = 2 * UNITS * 1024;
+  constexpr int KF = D / 32, CT = D / 16, NW = ATTN_WAVES, QT = 2;
+  constexpr int PAIR = 64, NE = 8;                   // positions of a pair of steps; slots of a lane in a step
+  constexpr uint32_t ALL = 0xffu;
+  constexpr int UNITS = 2 * CT;                      // 1 KiB bf16 fragments of a step: K's (a, f), then V's
+  constexpr int UPW = (KV8 ? 1 : 2) * UNITS / NW;    // fragments of a pair, as they are in the cache, per wave
+  constexpr int HALF = UNITS * 1024, BUF = 2 * HALF;
   __shared__ __attribute__((aligned(16))) char s_buf[2 * BUF];
+  __shared__ __attribute__((aligned(16))) uint8_t s_vs[2][PAIR];
   __shared__ float s_ml[4][2][16 * QT];
   const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -561,31 +569,41 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_tree_kernel(const Ca
   const int rb = (wave & ((1 << lr) - 1)) * 16 * QT, rank = wave >> lr;
   const int own = lr == 3 ? 1 : 2;                   // steps from one of a wave's to the next
   const Stripe sr = cache_stripe<D, KV8>(A, crow, kvh, kv_hi);
-  auto ld = [&](__amdgpu_buffer_rsrc_t rs, int vo, int so) -> lsk_i32x4 {
-    return __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, vo, so, 0));
-  };
-  lsk_i32x4 st[UPW], ksr, vsr;
+  lsk_i32x4 st[UPW];                                 // the wave's part of the next pair, in flight
+  uint32_t st_ks[UPW], st_vs;                        // 8-bit: exponents of this lane's K, and of position `lane`
   auto st_load = [&](int sb) {
 #pragma unroll
-    for (int i = 0; i < UPW; ++i) {
-      const int u = wave * UPW + i, w = u % UNITS;   // (a wave's fragments are all of K or all of V)
-      const int so = (sb / STEP + u / UNITS) * 64 * D + w % CT * 1024;
-      st[i] = ld(w < CT ? sr.k : sr.v, w < CT ? 16 * lane : 64 * l16 + 16 * lg, so);
+    for (int i = 0; i < UPW; ++i) {                  // (a wave's fragments are all of K or all of V)
+      const int u = wave * UPW + i, w = u % UNITS;
+      const int so = (sb + u / UNITS * 32) * 2 * D / (KV8 ? 2 : 1) + w % CT * 1024;
+      st[i] = __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                w < CT ? sr.k : sr.v, w < CT ? 16 * lane : 64 * l16 + 16 * lg, so, 0));
+      if constexpr (KV8)
+        st_ks[i] = __builtin_amdgcn_raw_buffer_load_b8(sr.ks, 16 * (l16 >> 2) + (l16 & 3),
+                                                       sb + 4 * (w % CT / (KF / 2)), 0);
     }
+    if constexpr (KV8) st_vs = __builtin_amdgcn_raw_buffer_load_b8(sr.vs, lane, sb, 0);
   };
   auto st_write = [&](int buf) {
+    char* to = s_buf + buf * BUF + 16 * lane;
 #pragma unroll
-    for (int i = 0; i < UPW; ++i) *(lsk_i32x4*)(s_buf + buf * BUF + (wave * UPW + i) * 1024 + 16 * lane) = st[i];
-  };
-  auto load_ks = [&](int sb) {
-    if constexpr (KV8) ksr = ld(sr.ks, 16 * (l16 >> 2), sb);
-  };
-  auto load_vs = [&](int sb) {
-    if constexpr (KV8) vsr = ld(sr.vs, 16 * lg, sb);
+    for (int i = 0; i < UPW; ++i) {
+      const int u = wave * UPW + i;
+      if constexpr (KV8) {                           // codes -> bf16, K with its scale: once for all the waves
+        const float sc = u < CT ? exp_bits(st_ks[i]) : 1.f;
+        const int a = u / (KF / 2), f = 2 * (u % (KF / 2));
+        char* lo = to + (u < CT ? (a >> 1) * HALF + ((a & 1) * KF + f) * 1024 : u * 1024);
+        *(lsk_bf16x8*)lo = codes_to_bf16(st[i][0], st[i][1], sc);
+        *(lsk_bf16x8*)(lo + (u < CT ? 1024 : HALF)) = codes_to_bf16(st[i][2], st[i][3], sc);
+      } else {
+        *(lsk_i32x4*)(to + u * 1024) = st[i];
+      }
+    }
+    if constexpr (KV8) {
+      if (wave == 0) s_vs[buf][lane] = (uint8_t)st_vs;
+    }
   };
   st_load(kv_lo);
-  load_ks(kv_lo + STEP * rank);
-  load_vs(kv_lo + STEP * rank);
   lsk_bf16x8 qf[QT][KF];
   int qpos[QT];                                      // the row's own slot; -1: no such row
 #pragma unroll
@@ -594,9 +612,10 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_tree_kernel(const Ca
     const uint16_t* q = A.q + (long)(q_start + t) * A.q_st + (long)(kvh * G + g) * A.q_sh;
     qpos[qt] = rl < nrows ? pos0 + t : -1;
 #pragma unroll
-    for (int f = 0; f < KF; ++f)
-      qf[qt][f] = __builtin_bit_cast(lsk_bf16x8,
-                                     *(const lsk_u32x4_u*)(q + (KV8 ? 64 * (f >> 1) + 16 * lg + 8 * (f & 1) : 32 * f + 8 * lg)));
+    for (int f = 0; f < KF; ++f) {
+      const int d = KV8 ? 64 * (f >> 1) + 16 * lg + 8 * (f & 1) : 32 * f + 8 * lg;
+      qf[qt][f] = __builtin_bit_cast(lsk_bf16x8, *(const lsk_u32x4_u*)(q + d));
+    }
   }
   lsk_f32x4 oacc[QT][CT];
   float m_run[QT], l_run[QT];
@@ -607,103 +626,76 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_tree_kernel(const Ca
 #pragma unroll
     for (int c = 0; c < CT; ++c) oacc[qt][c] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  // one step from LDS (as in cache_attn_kernel)
-  auto step = [&](auto full_, int sb, const char* src) {
+  // Step j of the pair at s2 (as in cache_attn_kernel): this lane's slots are s0 .. s0 + 7.
+  auto step = [&](auto full_, int s2, int j, int buf) {
     constexpr bool FULL = decltype(full_)::value;
-    lsk_i32x4 vr[CT];
-    auto get_v = [&]() {
-#pragma unroll
-      for (int c = 0; c < CT; ++c) vr[c] = *(const lsk_i32x4*)(src + (CT + c) * 1024 + 16 * lane);
-    };
-    uint64_t odd = 0;
+    const char* src = s_buf + buf * BUF + j * HALF + 16 * lane;
+    const int s0 = s2 + (KV8 ? 16 * lg + 8 * j : 32 * j + 8 * lg);
     uint32_t reads[QT];
-    if constexpr (!FULL) {
 #pragma unroll
-      for (int qt = 0; qt < QT; ++qt) {
-        const int s0 = sb + NE * lg, n = min(kv_hi - 1, qpos[qt]) - s0 + 1, t = max(qpos[qt] - pos0, 0);
+    for (int qt = 0; qt < QT; ++qt) {
+      reads[qt] = ALL;
+      if constexpr (!FULL) {
+        const int n = min(kv_hi - 1, qpos[qt]) - s0 + 1, t = max(qpos[qt] - pos0, 0);
         reads[qt] = (n >= NE ? ALL : n <= 0 ? 0u : (1u << n) - 1u) &
                     mask_window(A.mask + (long)(q_start + t) * A.W, A.W, s0 - pos0);
       }
     }
-    constexpr int AT = KV8 ? 1 : 2;                  // 16-slot tiles at a time: their products are independent chains
-    lsk_f32x4 sacc[QT][2 * HV];
+    lsk_f32x4 sacc[QT][2];
+    lsk_bf16x8 kf[2][KF];
 #pragma unroll
-    for (int a0 = 0; a0 < 2 * HV; a0 += AT) {
-      ORDER();
-      lsk_bf16x8 kf[AT][KF];
+    for (int a = 0; a < 2; ++a) {
 #pragma unroll
-      for (int a = 0; a < AT; ++a) {
-        if constexpr (KV8) {
-          const float sc = exp_bits(((uint32_t)ksr[a0 + a] >> (8 * (l16 & 3))) & 255u);
+      for (int f = 0; f < KF; ++f) kf[a][f] = *(const lsk_bf16x8*)(src + (a * KF + f) * 1024);
 #pragma unroll
-          for (int f = 0; f < KF; f += 2) {
-            const lsk_i32x4 x = *(const lsk_i32x4*)(src + ((a0 + a) * (KF / 2) + (f >> 1)) * 1024 + 16 * lane);
-            kf[a][f] = codes_to_bf16(x[0], x[1], sc);
-            kf[a][f + 1] = codes_to_bf16(x[2], x[3], sc);
-          }
-        } else {
-#pragma unroll
-          for (int f = 0; f < KF; ++f) kf[a][f] = *(const lsk_bf16x8*)(src + ((a0 + a) * KF + f) * 1024 + 16 * lane);
-        }
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) sacc[qt][a0 + a] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
-      }
-#pragma unroll
-      for (int f = 0; f < KF; ++f)
-#pragma unroll
-        for (int a = 0; a < AT; ++a)
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
-            sacc[qt][a0 + a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a][f], qf[qt][f], sacc[qt][a0 + a], 0, 0, 0);
+      for (int qt = 0; qt < QT; ++qt) sacc[qt][a] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    ORDER();
-    load_ks(sb + own * STEP);
-    if constexpr (!KV8) get_v();                     // (8-bit: two more tiles of scores are live)
-    lsk_bf16x8 pb[QT][HV];
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      if constexpr (KV8) ORDER();
-      softmax_tile<KV8, FULL>(sacc[qt], FULL ? ALL : reads[qt], vsr, A.scale_log2, m_run[qt], l_run[qt], oacc[qt], pb[qt]);
-    }
-    load_vs(sb + own * STEP);
-    if constexpr (KV8) {
-      ORDER();
-      get_v();
-    }
-    if constexpr (!FULL) odd = clear_odd<KV8>(vr, kv_hi - (sb + NE * lg));
+    for (int f = 0; f < KF; ++f)                     // (four independent chains)
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      lsk_bf16x8 vf[HV];
-      if constexpr (KV8) {
-#pragma unroll
-        for (int hv = 0; hv < HV; ++hv) vf[hv] = codes_to_bf16(vr[c][2 * hv], vr[c][2 * hv + 1], 1.f);
-      } else {
-        vf[0] = __builtin_bit_cast(lsk_bf16x8, vr[c]);
-      }
-#pragma unroll
-      for (int hv = 0; hv < HV; ++hv)
+      for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
-          oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[hv], pb[qt][hv], oacc[qt][c], 0, 0, 0);
+          sacc[qt][a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a][f], qf[qt][f], sacc[qt][a], 0, 0, 0);
+    ORDER();
+    lsk_i32x4 vr[CT], vsr = {0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < CT; ++c) vr[c] = *(const lsk_i32x4*)(src + (CT + c) * 1024);
+    if constexpr (KV8) {
+      const uint2 e = *(const uint2*)(s_vs[buf] + 16 * lg + 8 * j);
+      vsr[0] = (int)e.x;
+      vsr[1] = (int)e.y;
     }
-    if constexpr (!FULL) add_odd<KV8, true>(A, sr.v, odd, sb, q_start, pos0, qpos, oacc);
+    lsk_bf16x8 pb[QT][1];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+      softmax_tile<KV8, FULL>(sacc[qt], reads[qt], vsr, A.scale_log2, m_run[qt], l_run[qt], oacc[qt], pb[qt]);
+    uint64_t odd = 0;                                // (V is bf16 here in both formats)
+    if constexpr (!FULL) odd = clear_odd<false>(vr, kv_hi - s0);
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt)
+        oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lsk_bf16x8, vr[c]), pb[qt][0],
+                                                              oacc[qt][c], 0, 0, 0);
+    if constexpr (!FULL)
+      add_odd<KV8, true>(A, sr.v, odd, s2 + (KV8 ? 8 : 32) * j, q_start, pos0, qpos, oacc, KV8 ? 0x18 : 0);
   };
   st_write(0);
-  st_load(kv_lo + 2 * STEP);
+  st_load(kv_lo + PAIR);
   int s2 = kv_lo, buf = 0;
   auto pairs = [&](auto full_, int end) {            // the pairs of steps that start before `end`
-    for (; s2 < end; s2 += 2 * STEP, buf ^= 1) {
+    for (; s2 < end; s2 += PAIR, buf ^= 1) {
       __syncthreads();                               // (the other buffer's readers are done, this one is written)
       for (int j = rank; j < 2; j += own) {
-        const int sb = s2 + j * STEP;
-        if (sb >= kv_hi || rb >= nrows) break;
-        step(full_, sb, s_buf + buf * BUF + j * UNITS * 1024);
+        if (s2 + (KV8 ? 8 : 32) * j >= kv_hi || rb >= nrows) break;
+        step(full_, s2, j, buf);
       }
       st_write(buf ^ 1);
-      st_load(s2 + 4 * STEP);
+      st_load(s2 + 2 * PAIR);
     }
   };
-  pairs(std::true_type{}, min(kv_hi, pos0) - 2 * STEP + 1);  // (every row reads them whole)
+  pairs(std::true_type{}, min(kv_hi, pos0) - PAIR + 1);  // (every row reads them whole)
   pairs(std::false_type{}, kv_hi);
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) l_run[qt] = rows_sum(l_run[qt]);
@@ -955,8 +947,10 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 //   causal  an item is one row group: 8 waves share its steps.
 //   tree    a block of more than 32 rows gives an item 2, 4 or 8 row groups (up to 256 rows), whose 8, 4 .. waves each
 //           walk more of the positions: K / V come from memory once for all of them and fewer partial outputs are
-//           merged (32 trees of 45 nodes, 8B heads, 700 positions: one group 83 us, up to eight 29).  row_groups limits
-//           it, for caches of few stripes, whose launches have too few items otherwise.
+//           merged.  Items of 4 and 8 are cache_tree_kernel's, one workgroup each, longest first.  row_groups limits
+//           it, for caches of few stripes, whose launches have too few items otherwise (64-node trees, 8B heads, 960
+//           positions, at most 8 / 4 / 2 row groups: 8 trees 39 / 27 / 21 us, 16 trees 40 / 28 / 37, 64 trees
+//           96 / 109 / 170; 32 trees of 25 to 64 nodes over 128 to 1280 positions 52 / 45 / 55).
 // The number of row groups follows from the block's rows and the cache alone, so it never makes a row's result depend on
 // the batch.  Items go longest first to the least-loaded of n_slots persistent workgroups, as in lsk_attn_schedule.
 extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int n_kv_heads, int head_dim,
