@@ -225,18 +225,23 @@ __device__ __forceinline__ void softmax_tile(lsk_f32x4 (&s)[NA], uint32_t reads,
   l += rs;
 }
 
+// A workgroup has four waves, and each CU two workgroups (n_slots): one's first loads and merge fall into the other's
+// steps.  Against one workgroup of eight waves (8B heads, 8-bit, decode): 256 requests of 250 positions 28 us against 46,
+// of 960 81 against 91, of 4000 313 against 311; 7B heads, 16 trees of 30 nodes and 960 positions 30 against 36; one
+// request of 100000 positions, 1B heads, 25 against 23.
+#define CACHE_WAVES 4
 template <int D, int QT, bool KV8, bool TREE>
-__global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const CacheAttnArgs A) {
+__global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const CacheAttnArgs A) {
   constexpr int STEP = KV8 ? 64 : 32;                // positions per step of a wave
   constexpr int HV = STEP / 32;                      // 32-position halves of a step; a lane group has 8 slots of each
   constexpr int NE = 8 * HV;                         // slots of a lane group: NE consecutive ones
   constexpr uint32_t ALL = NE == 16 ? 0xffffu : 0xffu;
   constexpr int KF = D / 32;                         // K operands per 16-position tile
   constexpr int CT = D / 16;                         // 16-byte loads per lane of a step, for K and for V
-  constexpr int NW = ATTN_WAVES;
+  constexpr int NW = CACHE_WAVES;
   constexpr int GR = 16 * QT;                        // rows of a wave
   constexpr bool QREG = QT == 1;                     // one tile: Q fragments in registers (items of one row group)
-  constexpr int MT = QT < ATTN_MERGE_TILES ? QT : ATTN_MERGE_TILES;
+  constexpr int MT = TREE || QT < ATTN_MERGE_TILES ? 1 : ATTN_MERGE_TILES;  // (two workgroups' LDS fits a CU's)
   constexpr int MR = 16 * MT;                        // rows of a wave merged per pass
   constexpr int QROWS = QREG ? 0 : TREE ? 2 * GR : GR;  // rows of an item at most
   constexpr int QLD = D + 8;                         // 16 rows' 16-byte reads hit distinct banks
@@ -548,10 +553,11 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_attn_kernel(const Ca
 // A wave with eight row groups takes both steps, with four every other one; then the two waves of a row group are merged.
 // Bound by the softmax's vector instructions beside the products: 32 positions of 256 rows take 0.9 us, of which the
 // matrix instructions are half.
+#define TREE_WAVES 8
 template <int D, bool KV8>
-__global__ __launch_bounds__(64 * ATTN_WAVES, 1) void cache_tree_kernel(const CacheAttnArgs A,
+__global__ __launch_bounds__(64 * TREE_WAVES, 1) void cache_tree_kernel(const CacheAttnArgs A,
                                                                         const int32_t* __restrict__ items) {
-  constexpr int KF = D / 32, CT = D / 16, NW = ATTN_WAVES, QT = 2;
+  constexpr int KF = D / 32, CT = D / 16, NW = TREE_WAVES, QT = 2;
   constexpr int PAIR = 64, NE = 8;                   // positions of a pair of steps; slots of a lane in a step
   constexpr uint32_t ALL = 0xffu;
   constexpr int UNITS = 2 * CT;                      // 1 KiB bf16 fragments of a step: K's (a, f), then V's
@@ -944,9 +950,9 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 
 // Work items of one launch: 32 rows (token x query head of the group) of a block per wave, 16 where no block has more,
 // 48 for causal launches over 64 dims with larger blocks; the context in splits at absolute multiples of `split`.
-//   causal  an item is one row group: 8 waves share its steps.
-//   tree    a block of more than 32 rows gives an item 2, 4 or 8 row groups (up to 256 rows), whose 8, 4 .. waves each
-//           walk more of the positions: K / V come from memory once for all of them and fewer partial outputs are
+//   causal  an item is one row group: 4 waves share its steps.
+//   tree    a block of more than 32 rows gives an item 2, 4 or 8 row groups (up to 256 rows), whose waves each walk
+//           more of the positions: K / V come from memory once for all of them and fewer partial outputs are
 //           merged.  Items of 4 and 8 are cache_tree_kernel's, one workgroup each, longest first.  row_groups limits
 //           it, for caches of few stripes, whose launches have too few items otherwise (64-node trees, 8B heads, 960
 //           positions, at most 8 / 4 / 2 row groups: 8 trees 39 / 27 / 21 us, 16 trees 40 / 28 / 37, 64 trees
@@ -1004,7 +1010,7 @@ extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int
       for (int sp = 0; sp < ns; ++sp) {
         const int lo = sp * split, hi = lo + split < end ? lo + split : end;
         // in tenths of a one-tile step: a wave's steps, 1.5 times as long per further tile, and the item's own cost
-        const int steps = (hi - lo + step * (ATTN_WAVES >> lr) - 1) / (step * (ATTN_WAVES >> lr));
+        const int share = step * ((lr < 2 ? CACHE_WAVES : TREE_WAVES) >> lr), steps = (hi - lo + share - 1) / share;
         const int cost = steps * (10 + 5 * (tiles - 1)) + 20 + 6 * (tiles - 1);
         for (int h = 0; h < n_kv_heads; ++h)
           (lr < 2 ? items : shared).push_back({{bm[0], (int32_t)row0, nrows | (lr << 10) | (h << 12), lo, hi,
@@ -1088,7 +1094,7 @@ static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t
   LSK_REQUIRE(scale >= 0.f && scale <= 1e30f, LSK_EARG, "%s: scale %g (not negative)", what, (double)scale);
   a.scale_log2 = scale * 1.4426950408889634f;
   int rc = 0;
-#define LSK_CACHE_ATTN(DD, QT, K8, TR) cache_attn_kernel<DD, QT, K8, TR><<<n_slots, 64 * ATTN_WAVES, 0, s>>>(a)
+#define LSK_CACHE_ATTN(DD, QT, K8, TR) cache_attn_kernel<DD, QT, K8, TR><<<n_slots, 64 * CACHE_WAVES, 0, s>>>(a)
 #define LSK_CACHE_ATTN_D(K8, TR)                                            \
   do {                                                                      \
     if (head_dim == 128 && tiles == 1) LSK_CACHE_ATTN(128, 1, K8, TR);      \
@@ -1106,10 +1112,10 @@ static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t
   if (a.n_rounds > 0 && (rc = lsk_check_launch(what))) return rc;
   if (n_shared > 0) {
     const int32_t* items = a.recs + 8L * n_slots * a.n_rounds;
-    if (head_dim == 128 && kv8) cache_tree_kernel<128, true><<<n_shared, 64 * ATTN_WAVES, 0, s>>>(a, items);
-    else if (head_dim == 128) cache_tree_kernel<128, false><<<n_shared, 64 * ATTN_WAVES, 0, s>>>(a, items);
-    else if (kv8) cache_tree_kernel<64, true><<<n_shared, 64 * ATTN_WAVES, 0, s>>>(a, items);
-    else cache_tree_kernel<64, false><<<n_shared, 64 * ATTN_WAVES, 0, s>>>(a, items);
+    if (head_dim == 128 && kv8) cache_tree_kernel<128, true><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
+    else if (head_dim == 128) cache_tree_kernel<128, false><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
+    else if (kv8) cache_tree_kernel<64, true><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
+    else cache_tree_kernel<64, false><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
     if ((rc = lsk_check_launch(what))) return rc;
   }
   if (n_groups == 0) return 0;

@@ -699,7 +699,7 @@ class AttnPlan:
             raise ValueError(f"a split of {split} positions (a multiple of 64), or too many tokens")
         self.n_heads, self.n_tokens = n_heads, int(b[:, 2].sum())
         b = np.ascontiguousarray(b, dtype=np.int32)
-        group, n_slots = n_heads // Hkv, cu_count(self.device)
+        group, n_slots = n_heads // Hkv, 2 * cu_count(self.device)    # (two workgroups fit a CU)
         self.works = self.causal = self.tree = None
         self.rows_cap = self.n_works = 0
         if self.dtype == torch.float32:
