@@ -139,12 +139,14 @@ __device__ __forceinline__ void kv8_dwords(long stripe, int p0, int nt, F f) {
 
 }  // namespace
 
-// Workgroups 0 .. 3 of blockIdx.z quantise 16 tokens of one KV head's K each, workgroup 4 the 64 tokens' V.  16 threads
+// Workgroup 0 of blockIdx.z quantises 64 tokens' V of one KV head (it takes longest and starts first), workgroups 1 .. 4
+// 16 tokens' K each.  16 threads
 // hold a token's vector, D / 16 consecutive elements each, and find its largest magnitude by shuffles.  K goes straight
 // to its place.  V is turned, 4 x 4 in registers and the rest in LDS: a run of positions (a prompt's tokens) is written
 // a dword at a time, whole 64-byte sectors from one workgroup; other tokens byte by byte.
 // Latency-bound for a decode step's tokens; a long prompt moves 3 D bytes a token and head (4001 tokens of 8 heads of
-// 128: 13.4 us; with 16 tokens to every workgroup, so that four share a sector of V, 16.9; bytes alone 18.6).
+// 128: 11.8 us; with the V workgroups last 13.4; with 16 tokens to every workgroup, so that four share a sector of V,
+// 16.9).
 template <typename T, int D>
 __global__ __launch_bounds__(KV8_THREADS) void kv8_append_kernel(const T* __restrict__ k, const T* __restrict__ v,
                                                                  long st_t, long st_h, uint8_t* __restrict__ kc,
@@ -156,8 +158,8 @@ __global__ __launch_bounds__(KV8_THREADS) void kv8_append_kernel(const T* __rest
   constexpr int PER = D / 16;
   __shared__ uint32_t s_v[D * KV8_LD];
   const int h = blockIdx.y, j = threadIdx.x >> 4, part = threadIdx.x & 15;
-  if (blockIdx.z < 4) {
-    const int t = blockIdx.x * KV8_TOKENS + blockIdx.z * 16 + j;
+  if (blockIdx.z > 0) {
+    const int t = blockIdx.x * KV8_TOKENS + (blockIdx.z - 1) * 16 + j;
     if (t >= N) return;                              // (16 threads at a time)
     float x[PER];
     const T* src = k + (long)t * st_t + (long)h * st_h + part * PER;
@@ -224,7 +226,7 @@ __global__ __launch_bounds__(KV8_THREADS) void kv8_append_kernel(const T* __rest
   });
 }
 
-// The way back, in the same shape (4001 tokens of 8 heads of 128: 11.2 us; 12.7 with 16 tokens to a workgroup).
+// The way back, in the same shape (4001 tokens of 8 heads of 128: 10.1 us).
 template <typename T, int D>
 __global__ __launch_bounds__(KV8_THREADS) void kv8_read_kernel(const uint8_t* __restrict__ kc,
                                                                const uint8_t* __restrict__ vc,
@@ -237,8 +239,8 @@ __global__ __launch_bounds__(KV8_THREADS) void kv8_read_kernel(const uint8_t* __
   constexpr int PER = D / 16;
   __shared__ uint32_t s_v[D * KV8_LD];
   const int h = blockIdx.y, j = threadIdx.x >> 4, part = threadIdx.x & 15;
-  if (blockIdx.z < 4) {
-    const int t = blockIdx.x * KV8_TOKENS + blockIdx.z * 16 + j;
+  if (blockIdx.z > 0) {
+    const int t = blockIdx.x * KV8_TOKENS + (blockIdx.z - 1) * 16 + j;
     if (t >= N) return;
     const int row = rows[t], p = pos[t];
     const bool ok = row >= 0 && row < max_batch && p >= 0 && p < S;

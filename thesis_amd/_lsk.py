@@ -552,6 +552,9 @@ def _want(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tupl
                        f"{'' if t.is_contiguous() else ', not contiguous'}")
 
 
+_E4M3 = torch.float8_e4m3fn
+
+
 class _KV8(NamedTuple):
     k: torch.Tensor
     v: torch.Tensor
@@ -598,10 +601,14 @@ class KV8(_KV8):
         if D not in (64, 128) or S % 64 or S == 0:
             raise LskError(f"{what}: 8-bit caches need head_dim 64 or 128 and max_seq a multiple of 64 (got {D}, {S})")
         blocks = (*lead[:-1], S // 64)
-        _want(what, "k codes", k, torch.float8_e4m3fn, (*blocks, 4, D // 64, 64, 16))
-        _want(what, "v codes", v, torch.float8_e4m3fn, (*blocks, D, 64))
-        _want(what, "k exponents", ks, torch.uint8, lead)
-        _want(what, "v exponents", vs, torch.uint8, lead)
+        k_shape, v_shape = (*blocks, 4, D // 64, 64, 16), (*blocks, D, 64)
+        if not (k.shape == k_shape and v.shape == v_shape and vs.shape == lead and k.dtype is v.dtype is _E4M3 and
+                ks.dtype is vs.dtype is torch.uint8 and k.is_contiguous() and v.is_contiguous() and
+                ks.is_contiguous() and vs.is_contiguous()):
+            _want(what, "k codes", k, _E4M3, k_shape)
+            _want(what, "v codes", v, _E4M3, v_shape)
+            _want(what, "k exponents", ks, torch.uint8, lead)
+            _want(what, "v exponents", vs, torch.uint8, lead)
         self._checked = layers, (lead[-3], lead[-2], S, D)
         return self._checked[1]
 
