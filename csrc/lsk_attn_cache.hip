@@ -312,8 +312,11 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
     }
   };
   auto stripe = [&](const Item& it) { return cache_stripe<D, KV8>(A, it.crow, it.kvh, it.kv_hi); };
+  // Non-temporal where each byte is read once (32 trees of 16 nodes, 7B heads, 960 positions of bf16: 95 us against 80);
+  // not where two row groups read it (39 nodes: 111 us against 118)
+  constexpr int AUX = TREE && QT == 2 ? 0 : 2;
   auto ld = [&](__amdgpu_buffer_rsrc_t rs, int vo, int so) -> lsk_i32x4 {
-    return __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, vo, so, TREE ? 0 : 2));
+    return __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, vo, so, AUX));
   };
   const int k_vo = 16 * lane, v_vo = 64 * l16 + 16 * lg;
   lsk_i32x4 kr[CT], vr[CT], ksr, vsr;                // this step's K and V as loaded
