@@ -143,6 +143,15 @@ extern "C" int lsk_tree_accept(const int64_t* Yv, const int64_t* tokens, const i
 #define COMPACT_CHUNK 16
 #define COMPACT_THREADS 256
 
+// f over the 16 lanes of a row, in all of them (f associative, commutative and idempotent)
+template <typename U, typename F>
+__device__ __forceinline__ U row_reduce(U x, F f) {
+#define ROW_ROR(N) x = f(x, (U)__builtin_amdgcn_mov_dpp((int)x, 0x120 + N, 0xf, 0xf, false))
+  ROW_ROR(8); ROW_ROR(4); ROW_ROR(2); ROW_ROR(1);
+#undef ROW_ROR
+  return x;
+}
+
 template <int FMT> struct CompactElem;                // element, and a 16-byte piece at any address that aligns one
 template <> struct CompactElem<0> { using T = uint32_t; using Piece = lsk_f32x4_u; };
 template <> struct CompactElem<1> { using T = uint16_t; using Piece = lsk_u32x4_u; };
@@ -156,15 +165,11 @@ __device__ __forceinline__ long compact_k(int p, int ch, int D) {
   const int pp = p & 63, a = (pp >> 2) & 3, l16 = ((pp >> 4) << 2) | (pp & 3);
   return (long)(p >> 6) * 64 * D + (long)((a * (D >> 6) + (ch >> 2)) * 64 + (ch & 3) * 16 + l16) * 16;
 }
-template <int FMT>
-__device__ __forceinline__ long compact_v(int p, int d, int D) {
-  constexpr int B = FMT == 2 ? 64 : 32;
-  return (long)(p / B) * B * D + (long)d * B + p % B;
-}
-
-// Bound by the memory's sectors: a slot's K is D / 8 pieces (bf16) and its V one element of each of D rows, so every
-// moved slot costs whole sectors.  K moves in 16-byte pieces and the path is read once per chunk: 32 requests of 32 layers
-// of 8 heads of 128 take 59 us (element by element, the path read for each: 70).
+// K moves in 16-byte pieces of a slot.  V^T has a slot's values 64 bytes (fp32: 128) apart, D of them: the chunk's blocks
+// are turned in LDS, read and written in 16-byte pieces of eight (four, sixteen) slots, so that the memory sees a request
+// per dim and piece and not one per moved value, which bounded it (130 slots of 32 requests, 32 layers of 8 heads of
+// 128: 42 us against 59).  Only pieces that hold a source or a destination are touched; a piece's other slots
+// are written back as they were.
 template <int FMT, int D>
 __global__ __launch_bounds__(COMPACT_THREADS) void kv_compact_kernel(
     void* kc_, void* vc_, uint8_t* ks, uint8_t* vs, const int32_t* __restrict__ rows, const int32_t* __restrict__ pos0,
@@ -174,7 +179,13 @@ __global__ __launch_bounds__(COMPACT_THREADS) void kv_compact_kernel(
   constexpr int KCH = D * (int)sizeof(T) / 16;       // pieces of a slot's K
   constexpr int KPER = (COMPACT_CHUNK * KCH + COMPACT_THREADS - 1) / COMPACT_THREADS;
   constexpr int VPER = COMPACT_CHUNK * D / COMPACT_THREADS;
-  __shared__ int s_from[COMPACT_CHUNK];              // slot that slot p0 + j0 + i takes its contents from; -1: it stays
+  constexpr int B = FMT == 2 ? 64 : 32;              // slots of a V block
+  constexpr int PS = 16 / (int)sizeof(T), PPR = B / PS;  // slots of a piece, pieces of a dim's row
+  constexpr int LD = B * (int)sizeof(T) / 4 + 1;     // dwords of a row in LDS
+  constexpr int PROWS = COMPACT_THREADS / PPR, NP = (D + PROWS - 1) / PROWS;
+  constexpr int none = 0x7fffffff;
+  __shared__ int s_from[COMPACT_CHUNK];              // slot that slot to + j takes its contents from; -1: it stays
+  __shared__ uint32_t s_v[3][D * LD];                // the two blocks the chunk's destinations may lie in, and one other
   const int b = blockIdx.x, h = blockIdx.y, layer = blockIdx.z;
   const int row = rows[b], p0 = pos0[b];
   const int n = (int)min(acc[b], (int64_t)(max_nodes - 1));
@@ -182,47 +193,112 @@ __global__ __launch_bounds__(COMPACT_THREADS) void kv_compact_kernel(
   const long stripe = (((long)layer * max_batch + row) * Hkv + h) * (long)S;
   T* kc = (T*)kc_ + stripe * D;
   T* vc = (T*)vc_ + stripe * D;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, vd = tid % D, vj = tid / D, pc = tid % PPR, pr = tid / PPR;
   for (int j0 = 1; j0 <= n; j0 += COMPACT_CHUNK) {
-    bool moves = false;
-    if (tid < COMPACT_CHUNK) {
-      const int j = j0 + tid, node = j <= n ? path[(long)b * max_nodes + j] : -1;
-      moves = node > j && node < S - p0;
-      s_from[tid] = moves ? p0 + node : -1;
+    const int to = p0 + j0, db = to / B;
+    // Every wave's lanes look at the chunk's 16 slots: which pieces of the two destination blocks hold a source or a
+    // destination (bytes 0 and 1), a destination (2 and 3), and which later block is the first with a source.
+    const int l16 = tid & 15, j = j0 + l16, node = j <= n ? path[(long)b * max_nodes + j] : -1;
+    const bool moves = node > j && node < S - p0;
+    const int from = moves ? p0 + node : -1;
+    uint32_t bits = 0;
+    int other = none;
+    if (moves) {
+      const int src = from / B - db, dst = (to + l16) / B - db;
+      bits = 0x10001u << (8 * dst + (to + l16) % B / PS);
+      if (src < 2) bits |= 1u << (8 * src + from % B / PS);
+      else other = from / B;
     }
-    if (!__syncthreads_or(moves)) continue;
+    bits = __builtin_amdgcn_readfirstlane(row_reduce(bits, [](uint32_t x, uint32_t y) { return x | y; }));
+    if (bits == 0) continue;                         // nothing moves (as every wave finds)
+    auto least = [](int x, int y) { return min(x, y); };
+    other = __builtin_amdgcn_readfirstlane(row_reduce(other, least));
+    auto pieces_of = [&](int blk) {                  // pieces of a later block that hold a source
+      const uint32_t u = from >= 0 && from / B == blk ? 1u << (from % B / PS) : 0u;
+      return (uint32_t)__builtin_amdgcn_readfirstlane(row_reduce(u, [](uint32_t x, uint32_t y) { return x | y; }));
+    };
+    if (tid < COMPACT_CHUNK) s_from[tid] = from;
+    __syncthreads();
     Piece kx[KPER];
-    T vx[VPER];
-    uint8_t ek = 0, ev = 0;
 #pragma unroll
     for (int i = 0; i < KPER; ++i) {
       const int e = tid + i * COMPACT_THREADS, j = e / KCH, from = j < COMPACT_CHUNK ? s_from[j] : -1;
       if (from >= 0) kx[i] = *(const Piece*)(kc + compact_k<FMT>(from, e % KCH, D));
     }
-#pragma unroll
-    for (int i = 0; i < VPER; ++i) {
-      const int e = tid + i * COMPACT_THREADS, from = s_from[e / D];
-      if (from >= 0) vx[i] = vc[compact_v<FMT>(from, e % D, D)];
-    }
+    uint8_t ek = 0, ev = 0;
     if (FMT == 2 && tid < COMPACT_CHUNK && moves) {
       ek = ks[stripe + s_from[tid]];
       ev = vs[stripe + s_from[tid]];
     }
-    __syncthreads();                                 // (the loads' values are in before any slot is written)
-    const int to = p0 + j0;
+    auto fetch = [&](uint32_t* v, int blk, uint32_t need) {
+      if (need == 0) return;
+      Piece x[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int d = pr + i * PROWS;
+        if (d < D && (need >> pc & 1u)) x[i] = *(const Piece*)(vc + (long)blk * B * D + d * B + pc * PS);
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int d = pr + i * PROWS;
+        if (d < D && (need >> pc & 1u)) {
+          const lsk_i32x4 u = __builtin_bit_cast(lsk_i32x4, x[i]);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) v[d * LD + pc * 4 + w] = (uint32_t)u[w];
+        }
+      }
+    };
+    T vx[VPER];
+    auto take = [&](int buf, int blk) {              // this thread's values of dim vd whose source is in block blk
+#pragma unroll
+      for (int i = 0; i < VPER; ++i) {
+        const int from = s_from[vj * VPER + i];
+        if (from >= 0 && from / B == blk) vx[i] = ((const T*)(s_v[buf] + vd * LD))[from % B];
+      }
+    };
+    fetch(s_v[0], db, bits & 255u);
+    fetch(s_v[1], db + 1, bits >> 8 & 255u);
+    if (other != none) fetch(s_v[2], other, pieces_of(other));
+    __syncthreads();
+    take(0, db);
+    take(1, db + 1);
+    while (other != none) {
+      take(2, other);
+      other = __builtin_amdgcn_readfirstlane(row_reduce(from / B > other ? from / B : none, least));
+      if (other == none) break;
+      __syncthreads();
+      fetch(s_v[2], other, pieces_of(other));
+      __syncthreads();
+    }
+    __syncthreads();                                 // (every source is in registers)
+#pragma unroll
+    for (int i = 0; i < VPER; ++i) {
+      const int j = vj * VPER + i;
+      if (s_from[j] >= 0) ((T*)(s_v[(to + j) / B - db] + vd * LD))[(to + j) % B] = vx[i];
+    }
 #pragma unroll
     for (int i = 0; i < KPER; ++i) {
       const int e = tid + i * COMPACT_THREADS, j = e / KCH;
       if (j < COMPACT_CHUNK && s_from[j] >= 0) *(Piece*)(kc + compact_k<FMT>(to + j, e % KCH, D)) = kx[i];
     }
-#pragma unroll
-    for (int i = 0; i < VPER; ++i) {
-      const int e = tid + i * COMPACT_THREADS, j = e / D;
-      if (s_from[j] >= 0) vc[compact_v<FMT>(to + j, e % D, D)] = vx[i];
-    }
     if (FMT == 2 && tid < COMPACT_CHUNK && moves) {
       ks[stripe + to + tid] = ek;
       vs[stripe + to + tid] = ev;
+    }
+    __syncthreads();
+    for (int d = 0; d < 2; ++d) {
+      const uint32_t dirty = bits >> (16 + 8 * d) & 255u;
+      if (dirty == 0) continue;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int row_d = pr + i * PROWS;
+        if (row_d < D && (dirty >> pc & 1u)) {
+          lsk_i32x4 u;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) u[w] = (int)s_v[d][row_d * LD + pc * 4 + w];
+          *(Piece*)(vc + (long)(db + d) * B * D + row_d * B + pc * PS) = __builtin_bit_cast(Piece, u);
+        }
+      }
     }
     __syncthreads();
   }
