@@ -520,30 +520,29 @@ def shift_segment_positions(meta, n_tokens: int, nb: int, n_works: int, n_groups
 
 # ----------------------------------------------------------------------------- 8-bit cache and trees of drafted tokens
 
-def _one_device(*ts) -> int:
+def _one_device(first: torch.Tensor, *ts) -> int:
     """The index of the device that all the tensors are on (None is skipped); LskError otherwise."""
-    dev = None
+    dev = first.get_device()
     for t in ts:
-        if t is not None:
-            i = t.get_device()
-            if i != dev:
-                if dev is not None or i < 0:
-                    _dev(*ts)
-                    raise LskError(f"tensors on different devices: "
-                                   f"{sorted({str(t.device) for t in ts if t is not None})}")
-                dev = i
+        if t is not None and t.get_device() != dev:
+            dev = -1
+            break
+    if dev < 0:
+        _dev(first, *ts)
+        raise LskError(f"tensors on different devices: {sorted({str(t.device) for t in (first, *ts) if t is not None})}")
     return dev
 
 
 def _launch(dev: int, what: str, *args) -> None:
     """Calls `what` with args and device dev's current stream; dev is the current device for the call."""
     fn = getattr(load(), what)
-    if torch.cuda.current_device() == dev:
+    if torch._C._cuda_getDevice() == dev:
         rc = fn(*args, _stream())
     else:
         with torch.cuda.device(dev):
             rc = fn(*args, _stream())
-    _check(rc, what)
+    if rc:
+        _check(rc, what)
 
 
 def _want(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
@@ -589,6 +588,10 @@ class KV8(_KV8):
         *_, B, Hkv, S = self.ks.shape
         return B, Hkv, S, self.v.shape[-2]
 
+    def ptrs(self) -> tuple:
+        k, v, ks, vs = self
+        return k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
+
     def check(self, what: str, layers: bool = False) -> tuple:
         """(B, Hkv, S, D) of a cache of the documented storage; LskError otherwise."""
         if self._checked is not None and self._checked[0] == layers:
@@ -622,15 +625,16 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: KV8, rows_i32: torch.Ten
     if k.shape != (n, Hkv, D) or v.shape != k.shape or v.dtype != k.dtype:
         raise LskError(f"kv8_append: k and v must be [N, {Hkv}, {D}] of one dtype, got {list(k.shape)} {k.dtype} and "
                        f"{list(v.shape)} {v.dtype}")
-    if n and (k.stride(2) != 1 or v.stride(2) != 1 or k.stride() != v.stride()):
+    st_t, st_h, st_d = k.stride()
+    if n and (st_d != 1 or v.stride() != (st_t, st_h, st_d)):
         raise LskError("kv8_append: k and v need contiguous dims and the same strides")
     _want("kv8_append", "rows", rows_i32, torch.int32, (n,))
     _want("kv8_append", "pos", pos_i32, torch.int32, (n,))
     code = dtype_code(k.dtype)
     if n == 0:
         return
-    _launch(dev, "lsk_kv8_append", code, _ptr(k), _ptr(v), k.stride(0), k.stride(1), *map(_ptr, cache), _ptr(rows_i32),
-            _ptr(pos_i32), n, Hkv, D, B, S)
+    _launch(dev, "lsk_kv8_append", code, k.data_ptr(), v.data_ptr(), st_t, st_h, *cache.ptrs(), rows_i32.data_ptr(),
+            pos_i32.data_ptr(), n, Hkv, D, B, S)
 
 
 def kv8_read(cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
@@ -644,13 +648,13 @@ def kv8_read(cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor, dtype: t
     _want("kv8_read", "pos", pos_i32, torch.int32, (n,))
     code = dtype_code(dtype if out is None else out[0].dtype)
     if out is None:
-        out = tuple(cache.ks.new_empty((n, Hkv, D), dtype=dtype) for _ in range(2))
+        out = cache.ks.new_empty(n, Hkv, D, dtype=dtype), cache.ks.new_empty(n, Hkv, D, dtype=dtype)
     else:
         for t in out:
             _want("kv8_read", "out", t, out[0].dtype, (n, Hkv, D))
     if n:
-        _launch(dev, "lsk_kv8_read", code, *map(_ptr, cache), _ptr(rows_i32), _ptr(pos_i32), _ptr(out[0]), _ptr(out[1]),
-                n, Hkv, D, B, S)
+        _launch(dev, "lsk_kv8_read", code, *cache.ptrs(), rows_i32.data_ptr(), pos_i32.data_ptr(), out[0].data_ptr(),
+                out[1].data_ptr(), n, Hkv, D, B, S)
     return out
 
 
@@ -705,6 +709,8 @@ class AttnPlan:
         if (split is not None and (split < 64 or split % 64)) or len(b) and int(b[:, 2].sum()) >= 1 << 30:
             raise ValueError(f"a split of {split} positions (a multiple of 64), or too many tokens")
         self.n_heads, self.n_tokens = n_heads, int(b[:, 2].sum())
+        self.q_shape, self.width, self.scale = (self.n_tokens, n_heads, D), n_heads * D, 1.0 / math.sqrt(D)
+        self.index = self.device.index if self.device.index is not None else -1
         b = np.ascontiguousarray(b, dtype=np.int32)
         group, n_slots = n_heads // Hkv, 2 * cu_count(self.device)    # (two workgroups fit a CU)
         self.works = self.causal = self.tree = None
@@ -739,30 +745,34 @@ class AttnPlan:
                        ws)
 
 
-def _plan_call(what: str, q: torch.Tensor, plan: AttnPlan, launch, dims: tuple, kv8: bool, dtype: torch.dtype, mask,
-               scale, out, workspace):
+def _plan_call(what: str, dev: int, q: torch.Tensor, plan: AttnPlan, launch, dims: tuple, kv8: bool,
+               dtype: torch.dtype, mask, scale, out, workspace):
     """Checks shared by kv8_attn and tree_attn; returns (scale, out, workspace, its bytes)."""
-    if plan.dims != dims or plan.kv8 != kv8 or plan.dtype != dtype:
+    if dev != plan.index:
+        raise LskError(f"{what}: the plan is on {plan.device}, the tensors on cuda:{dev}")
+    if plan.dims != dims or plan.kv8 != kv8 or plan.dtype is not dtype:
         raise LskError(f"{what}: the plan was made for another cache ({plan.dims} {plan.dtype})")
     if launch is None and dtype != torch.float32:
         raise LskError(f"{what}: the plan was made for launches {'without' if mask is not None else 'with'} a mask")
-    _, Hkv, _, D = dims
     want = torch.bfloat16 if kv8 else dtype
-    if q.shape != (plan.n_tokens, plan.n_heads, D) or q.dtype != want or (q.numel() and q.stride(2) != 1):
-        raise LskError(f"{what}: q must be [{plan.n_tokens}, {plan.n_heads}, {D}] {want} with contiguous dims, got "
-                       f"{list(q.shape)} {q.dtype}")
-    if mask is not None and (mask.dim() != 2 or mask.shape[1] < 1):
-        raise LskError(f"{what}: mask must be [{plan.n_tokens}, words]")
+    n, width = plan.n_tokens, plan.width
+    if q.shape != plan.q_shape or q.dtype is not want or (n and q.stride(2) != 1):
+        raise LskError(f"{what}: q must be {list(plan.q_shape)} {want} with contiguous dims, got {list(q.shape)} {q.dtype}")
     if mask is not None:
-        _want(what, "mask", mask, torch.int32, (plan.n_tokens, mask.shape[1]))
+        if mask.dim() != 2 or mask.shape[1] < 1:
+            raise LskError(f"{what}: mask must be [{n}, words]")
+        _want(what, "mask", mask, torch.int32, (n, mask.shape[1]))
     if out is None:
-        out = q.new_empty((plan.n_tokens, plan.n_heads * D))
+        out = q.new_empty(n, width)
     else:
-        _want(what, "out", out, want, (plan.n_tokens, plan.n_heads * D))
-    if workspace is None and launch is not None and launch.ws_bytes:
-        workspace = q.new_empty((launch.ws_bytes,), dtype=torch.uint8)
+        _want(what, "out", out, want, (n, width))
+    if workspace is None:
+        if launch is not None and launch.ws_bytes:
+            workspace = q.new_empty(launch.ws_bytes, dtype=torch.uint8)
+    elif not workspace.is_contiguous():
+        raise LskError(f"{what}: the workspace must be contiguous")
     ws_bytes = workspace.nbytes if workspace is not None else 0
-    return 1.0 / math.sqrt(D) if scale is None else float(scale), out, workspace, ws_bytes
+    return plan.scale if scale is None else float(scale), out, workspace, ws_bytes
 
 
 def kv8_attn(q: torch.Tensor, cache: KV8, plan: AttnPlan, mask: torch.Tensor | None = None, scale: float | None = None,
@@ -771,13 +781,14 @@ def kv8_attn(q: torch.Tensor, cache: KV8, plan: AttnPlan, mask: torch.Tensor | N
     mask (int32 [N, words], tree_masks): blocks are trees of drafted tokens.  scale: 1 / sqrt(D) unless given.  Without
     a workspace one is taken from torch's allocator for the call."""
     p = plan.causal if mask is None else plan.tree
-    dev = _one_device(q, *cache, p.recs if p is not None else None, mask, out, workspace)
+    dev = _one_device(q, *cache, mask, out, workspace)
     dims = _, Hkv, S, D = cache.check("kv8_attn")
-    scale, out, workspace, ws = _plan_call("kv8_attn", q, plan, p, dims, True, cache.k.dtype, mask, scale, out, workspace)
+    scale, out, workspace, ws = _plan_call("kv8_attn", dev, q, plan, p, dims, True, _E4M3, mask, scale, out, workspace)
     if p.n_items:
-        _launch(dev, "lsk_kv8_attn", _ptr(q), q.stride(0), q.stride(1), *map(_ptr, cache), _ptr(mask),
-                mask.shape[1] if mask is not None else 0, *p.args, _ptr(out), plan.n_heads, Hkv, D, S, scale,
-                _ptr(workspace), ws)
+        st_t, st_h, _ = q.stride()
+        masked = (None, 0) if mask is None else (mask.data_ptr(), mask.shape[1])
+        _launch(dev, "lsk_kv8_attn", q.data_ptr(), st_t, st_h, *cache.ptrs(), *masked, *p.args, out.data_ptr(),
+                plan.n_heads, Hkv, D, S, scale, _ptr(workspace), ws)
     return out
 
 
@@ -788,20 +799,21 @@ def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, plan:
     [N, Hq * D].  kcache: K cache storage (k_dims); vcache: the blocked-transposed V storage; mask: int32 [N, words]
     (tree_masks).  scale: 1 / sqrt(D) unless given."""
     p = plan.tree
-    dev = _one_device(q, kcache, vcache, p.recs if p is not None else plan.works, mask, out, workspace)
+    dev = _one_device(q, kcache, vcache, mask, out, workspace)
     _check_kcache(kcache.dtype, kcache)
     code = dtype_code(kcache.dtype)
     dims = B, Hkv, S, D = k_dims(kcache)
     if not kcache.is_contiguous():
         raise LskError("tree_attn: the K cache must be contiguous")
     _want("tree_attn", "V cache", vcache, kcache.dtype, (B, Hkv, S // 32, D, 32))
-    scale, out, workspace, ws = _plan_call("tree_attn", q, plan, p, dims, False, kcache.dtype, mask, scale, out,
+    scale, out, workspace, ws = _plan_call("tree_attn", dev, q, plan, p, dims, False, kcache.dtype, mask, scale, out,
                                            workspace)
     if p.n_items if p is not None else plan.n_works:
         args = p.args if p is not None else (None, 0, 0, None, 0, 0, 0, 0, 0, 0)
-        _launch(dev, "lsk_tree_attn", code, _ptr(q), q.stride(0), q.stride(1), _ptr(kcache), _ptr(vcache), _ptr(mask),
-                mask.shape[1], _ptr(plan.works), plan.n_works, plan.rows_cap, *args, _ptr(out), plan.n_heads, Hkv, D, S,
-                scale, _ptr(workspace), ws)
+        st_t, st_h, _ = q.stride()
+        _launch(dev, "lsk_tree_attn", code, q.data_ptr(), st_t, st_h, kcache.data_ptr(), vcache.data_ptr(),
+                mask.data_ptr(), mask.shape[1], _ptr(plan.works), plan.n_works, plan.rows_cap, *args, out.data_ptr(),
+                plan.n_heads, Hkv, D, S, scale, _ptr(workspace), ws)
     return out
 
 
@@ -834,7 +846,7 @@ def tree_accept(Yv: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, s
         _want("tree_accept", name, t, dt, (k,))
     if max_nodes < 1:
         raise LskError(f"tree_accept: max_nodes {max_nodes}")
-    acc, path, out = Yv.new_empty((nb,)), parents.new_empty((nb, max_nodes)), Yv.new_empty((nb, max_nodes))
+    acc, path, out = Yv.new_empty(nb), parents.new_empty(nb, max_nodes), Yv.new_empty(nb, max_nodes)
     if nb and n == 0:
         acc.fill_(-1), path.fill_(-1), out.fill_(-1)
     elif nb:
@@ -845,32 +857,31 @@ def tree_accept(Yv: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, s
 
 def _compact(what, code, k, v, ks, vs, layers, dims, rows_i32, pos0_i32, accepted, path) -> None:
     dev = _one_device(k, v, ks, vs, rows_i32, pos0_i32, accepted, path)
-    nb = rows_i32.numel()
-    B, Hkv, S, D = dims
+    nb, (B, Hkv, S, D) = rows_i32.numel(), dims
     _want(what, "rows", rows_i32, torch.int32, (nb,))
     _want(what, "pos0", pos0_i32, torch.int32, (nb,))
     _want(what, "accepted", accepted, torch.int64, (nb,))
-    if path.dim() != 2 or path.shape[1] < 1:
+    most = path.shape[1] if path.dim() == 2 else 0
+    if most < 1:
         raise LskError(f"{what}: path must be [{nb}, max_nodes]")
-    _want(what, "path", path, torch.int32, (nb, path.shape[1]))
+    _want(what, "path", path, torch.int32, (nb, most))
     if nb and layers:
-        _launch(dev, "lsk_kv_compact", code, _ptr(k), _ptr(v), _ptr(ks), _ptr(vs), layers, _ptr(rows_i32), _ptr(pos0_i32),
-                _ptr(accepted), _ptr(path), nb, path.shape[1], Hkv, D, B, S)
+        _launch(dev, "lsk_kv_compact", code, k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), layers, rows_i32.data_ptr(),
+                pos0_i32.data_ptr(), accepted.data_ptr(), path.data_ptr(), nb, most, Hkv, D, B, S)
 
 
 def kv_compact(k: torch.Tensor, v: torch.Tensor, rows_i32, pos0_i32, accepted, path) -> None:
     """The accepted paths' K / V move to consecutive slots in every layer (lsk_kv_compact): slot pos0 + j of a cache row
     takes slot pos0 + path[j], j = 1 .. accepted.  k, v: the layers' storage (KVCache.kf_all or fp32 rows, and vb_all;
     or a run of their layers); path and accepted: tree_accept's; rows, pos0 int32 [nb], the rows different."""
-    if k.dim() not in (5, 7) or not k.is_contiguous():
-        raise LskError("kv_compact: the K storage of several layers is needed, contiguous")
-    code = dtype_code(k.dtype)
-    if (k.dim() == 7) != (code == DTYPE_BF16):
-        raise LskError("kv_compact: fragment-major bf16 K storage or row-major fp32 is needed")
-    B, Hkv = k.shape[1:3]
-    S, D = (k.shape[3] * 32, k.shape[4] * 16) if k.dim() == 7 else (k.shape[3], k.shape[4])
-    _want("kv_compact", "V storage", v, k.dtype, (k.shape[0], B, Hkv, S // 32, D, 32))
-    _compact("kv_compact", code, k, v, None, None, k.shape[0], (B, Hkv, S, D), rows_i32, pos0_i32, accepted, path)
+    shape, code = tuple(k.shape), dtype_code(k.dtype)
+    if len(shape) != (7 if code == DTYPE_BF16 else 5) or not k.is_contiguous():
+        raise LskError("kv_compact: the K storage of several layers is needed, contiguous: fragment-major bf16 or row-major "
+                       "fp32")
+    L, B, Hkv = shape[:3]
+    S, D = (shape[3] * 32, shape[4] * 16) if code == DTYPE_BF16 else shape[3:]
+    _want("kv_compact", "V storage", v, k.dtype, (L, B, Hkv, S // 32, D, 32))
+    _compact("kv_compact", code, k, v, None, None, L, (B, Hkv, S, D), rows_i32, pos0_i32, accepted, path)
 
 
 def kv8_compact(cache: KV8, rows_i32, pos0_i32, accepted, path) -> None:
