@@ -452,6 +452,56 @@ def test_values_that_a_row_does_not_read_never_reach_it(cuda, kind, bad, row_gro
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("kind", ["bf16", "kv8"])
+def test_bad_values_in_trees_of_many_rows_stay_with_their_readers(cuda, kind, bad, D):
+    """The same for trees of 80 to 180 rows, whose waves share K and V."""
+    lsk = _lsk()
+    Hq, Hkv = 8, 2
+    blocks = [(0, 70, 20), (2, 64, 45), (1, 131, 33)]
+    tab, q, k, v = _attn_inputs(47, (Hq, Hkv, D), blocks, S=256, B=3)
+    v[0, :, 77, D - 1] = 5.0                                          # (the largest also without the dims below)
+    v[2, :, 104, D - 1] = 5.0
+    parents, sets = _tree_blocks(blocks, 5)
+    mask = torch.from_numpy(words_of(sets, 2)).to(cuda)
+
+    def run(k, v):
+        if kind == "kv8":
+            cache = kv8_from(lsk, cuda, k, v)
+            for (_, p0, t, row) in tab:                               # slots never written: any byte as a scale
+                cache.ks[row, :, p0 + t:], cache.vs[row, :, p0 + t:] = 255, 255
+            plan = lsk.AttnPlan(tab, Hq, cache, None, 8)
+            assert plan.tree.n_shared == 3 * Hkv and plan.tree.n_rounds == 0
+            return lsk.kv8_attn(q.to(cuda), cache, plan, mask).cpu()
+        ks = lsk.k_to_frag(k).to(cuda)
+        return lsk.tree_attn(q.to(cuda), ks, lsk.v_to_blocked(v).to(cuda), lsk.AttnPlan(tab, Hq, ks, None, 8), mask).cpu()
+
+    clean = run(k, v)
+    k2, v2 = k.clone(), v.clone()
+    for (_, p0, t, row) in tab:
+        k2[row, :, p0 + t:], v2[row, :, p0 + t:] = bad, bad
+    assert torch.equal(run(k2, v2), clean)
+    reads = torch.zeros(len(q), dtype=torch.bool)
+    for (b, node) in ((0, 7), (1, 40)):
+        q0, p0, t, row = tab[b]
+        v2[row, :, p0 + node, :10], v2[row, :, p0 + node, 40] = bad, bad
+        reads |= torch.tensor([q0 <= i < q0 + t and node in sets[i] for i in range(len(q))])
+    assert reads[:20].any() and reads[20:65].any() and not reads[:20].all() and not reads[20:65].all()
+    hit = torch.zeros(D, dtype=torch.bool)
+    hit[:10], hit[40] = True, True
+    got, clean = run(torch.where(torch.isfinite(k2), k2, k), v2).view(-1, Hq, D), clean.view(-1, Hq, D)
+    assert torch.equal(got[~reads], clean[~reads])
+    assert torch.equal(got[reads][..., ~hit], clean[reads][..., ~hit])
+    want = torch.full_like(got[reads][..., hit], math.nan if kind == "kv8" else bad)
+    assert torch.equal(got[reads][..., hit].nan_to_num(7.0), want.nan_to_num(7.0))
+    for (b, node) in ((0, 7), (1, 40)):
+        k2[tab[b][3], :, tab[b][1] + node] = bad
+    got = run(k2, v).view(-1, Hq, D)
+    assert torch.equal(got[~reads], clean[~reads]) and torch.isnan(got[reads]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D", [16, 64, 128])
 def test_an_fp32_chain_gives_the_ragged_attentions_bits(cuda, D):
     lsk = _lsk()
@@ -615,6 +665,35 @@ def test_attention_of_offsets_past_32_bits(cuda):
     assert_close_bf16(got, ref, mag)
 
 
+@pytest.mark.gpu
+def test_trees_and_compaction_past_32_bits(cuda):
+    """A tree of many rows in a bf16 cache row whose first byte lies past 4 GiB: attended to, accepted and compacted."""
+    lsk = _lsk()
+    Hq, Hkv, D, S = 8, 1, 128, 32768
+    B = (5 << 30) // (S * D * 2)
+    kf = torch.zeros(1, B, Hkv, S // 32, D // 16, 64, 8, dtype=BF16, device=cuda)
+    vb = torch.zeros(1, B, Hkv, S // 32, D, 32, dtype=BF16, device=cuda)
+    g, rng = _gen(53), np.random.default_rng(53)
+    p0, T, row = 100, 40, B - 1
+    n = p0 + T
+    k, v = (torch.randn(n, Hkv, D, generator=g).to(BF16) for _ in range(2))
+    lsk.kv_append(k.to(cuda), v.to(cuda), kf[0], vb[0], _i32(np.full(n, row), cuda), _i32(np.arange(n), cuda))
+    parents = random_tree(rng, T)
+    tab, q = [(0, p0, T, row)], torch.randn(T, Hq, D, generator=g).to(BF16)
+    sets = ancestors(parents)
+    mask = torch.from_numpy(words_of(sets, 2)).to(cuda)
+    got = lsk.tree_attn(q.to(cuda), kf[0], vb[0], lsk.AttnPlan(tab, Hq, kf[0]), mask)
+    dense = lambda x: x.double().permute(1, 0, 2)[None].expand(row + 1, -1, -1, -1)  # noqa: E731
+    ref, mag, _ = attention(q.double(), dense(k), dense(v), tab, 1 / math.sqrt(D), sets)
+    assert_close_bf16(got, ref, mag)
+    path = [0] + sorted(rng.choice(np.arange(1, T), 12, replace=False).tolist())
+    lsk.kv_compact(kf, vb, _i32([row], cuda), _i32([p0], cuda), torch.tensor([12], device=cuda), _i32([path], cuda))
+    src = list(range(p0)) + [p0 + j for j in path]
+    for got, x in ((lsk.k_from_frag(kf[0, row].cpu()), k), (lsk.v_from_blocked(vb[0, row].cpu()), v)):
+        assert torch.equal(got[0, :len(src)], x[src, 0]) and torch.equal(got[0, len(src):n], x[len(src):, 0])
+        assert (got[0, n:] == 0).all()
+
+
 # ----------------------------------------------------------------------------- masks, acceptance, compaction
 
 def accept(parents, tokens, y):
@@ -731,6 +810,104 @@ def test_compaction_moves_the_accepted_paths_and_nothing_else(cuda, fmt, D):
             x[:, r, :, p0:p0 + len(p)] = x[:, r][:, :, src].clone()
     got = _dense(lsk, cuda, fmt, cache, (L, B, H, S, D))
     assert torch.equal(got[0].double(), k.double()) and torch.equal(got[1].double(), v.double())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,D", [("bf16", 128), ("bf16", 64), ("fp32", 16), ("fp32", 128), ("kv8", 128), ("kv8", 64)])
+def test_compaction_of_long_paths_from_far_nodes(cuda, fmt, D):
+    """Paths of several chunks of 16 whose sources lie in many blocks, consecutive runs between them, and a count past
+    the path's end (it stops there)."""
+    lsk = _lsk()
+    L, B, H, S = 1, 4, 1, 1024
+    cache, k, v = _caches(lsk, cuda, fmt, L, B, H, S, D, _gen(D + 1))
+    rng = np.random.default_rng(D)
+    rows, pos0 = [2, 0, 1, 3], [3, 31, 32, 500]
+    paths = [[0] + sorted(rng.choice(np.arange(1, 900), 70, replace=False).tolist()),
+             [0] + list(range(1, 20)) + [300, 301, 302, 640],
+             [0, 959] + [-1] * 3, [0] + list(range(5, 75)) + [523]]
+    most = max(len(p) for p in paths) + 1
+    path = np.full((len(paths), most), -1)
+    for i, p in enumerate(paths):
+        path[i, :len(p)] = p
+    acc = [70, 1000, 1, 71]
+    args = (_i32(rows, cuda), _i32(pos0, cuda), torch.tensor(acc, device=cuda), _i32(path, cuda))
+    (lsk.kv8_compact(cache, *args) if fmt == "kv8" else lsk.kv_compact(*cache, *args))
+    for r, p0, p in zip(rows, pos0, paths):
+        src = [p0 + i for i in p if i >= 0]
+        for x in (k, v):
+            x[:, r, :, p0:p0 + len(src)] = x[:, r][:, :, src].clone()
+    got = _dense(lsk, cuda, fmt, cache, (L, B, H, S, D))
+    assert torch.equal(got[0].double(), k.double()) and torch.equal(got[1].double(), v.double())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "kv8"])
+def test_a_tree_step_captured_in_two_graphs(cuda, fmt):
+    """Masks, write, attention, acceptance and compaction as a captured step, replayed with new inputs between eager
+    steps; two graphs of the same step, whose partial outputs are their own."""
+    lsk = _lsk()
+    L, B, Hq, Hkv, D, S = 2, 3, 8, 2, 128, 512
+    sizes, pos0, rows = [40, 5, 21], [300, 64, 7], [1, 2, 0]
+    tab, n = pack_blocks(list(zip(rows, pos0, sizes)))
+    (cache, _, _) = _caches(lsk, cuda, fmt, L, B, Hkv, S, D, _gen(59))
+    layers = [cache.layer(i) for i in range(L)] if fmt == "kv8" else [(cache[0][i], cache[1][i]) for i in range(L)]
+    flat = [t.view(torch.uint8) if t.dtype == E4M3 else t for t in cache]
+    saved = [t.clone() for t in flat]
+    plan = lsk.AttnPlan(tab, Hq, layers[0] if fmt == "kv8" else layers[0][0], split=128, row_groups=8)
+    assert plan.tree.n_parts > 0 and plan.tree.n_shared > 0 and plan.tree.n_rounds > 0
+    starts, lens = _i32([b[0] for b in tab], cuda), _i32(sizes, cuda)
+    trow, tpos = _i32(np.repeat(rows, sizes), cuda), _i32(np.concatenate([p + np.arange(t) for p, t in zip(pos0, sizes)]), cuda)
+    r_t, p_t = _i32(rows, cuda), _i32(pos0, cuda)
+    par, tok, y = _i32(np.zeros(n), cuda), torch.zeros(n, dtype=torch.int64, device=cuda), torch.zeros(
+        n, dtype=torch.int64, device=cuda)
+    q, k, v = (torch.zeros(n, h, D, dtype=BF16, device=cuda) for h in (Hq, Hkv, Hkv))
+
+    def step():
+        mask, depth = lsk.tree_masks(par, starts, lens, max(sizes))
+        out = []
+        for c in layers:
+            if fmt == "kv8":
+                lsk.kv8_append(k, v, c, trow, tpos)
+                out.append(lsk.kv8_attn(q, c, plan, mask))
+            else:
+                lsk.kv_append(k, v, c[0], c[1], trow, tpos)
+                out.append(lsk.tree_attn(q, c[0], c[1], plan, mask))
+        acc, path, new = lsk.tree_accept(y, tok, par, starts, lens, max(sizes))
+        lsk.kv8_compact(cache, r_t, p_t, acc, path) if fmt == "kv8" else lsk.kv_compact(*cache, r_t, p_t, acc, path)
+        return [*out, mask, depth, acc, path, new]
+
+    def fresh(i):
+        parents, tokens, greedy = _forest(60 + i, sizes, vocab=2)
+        for t, x in ((par, parents), (tok, tokens), (y, greedy)):
+            t.copy_(_cat(x, t.dtype, cuda))
+        for j, t in enumerate((q, k, v)):
+            t.copy_(torch.randn(t.shape, generator=_gen(70 + 3 * i + j)).to(BF16))
+
+    def reset():
+        for t, x in zip(flat, saved):
+            t.copy_(x)
+
+    fresh(0)
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = step()
+        graphs.append((g, outs))
+    for i in range(4):
+        fresh(i)
+        reset()
+        want = step()
+        held_after = [t.clone() for t in flat]
+        assert (want[-3] > 0).any()
+        for g, outs in graphs:
+            reset()
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+            assert all(torch.equal(a, b) for a, b in zip(flat, held_after))
 
 
 @pytest.mark.gpu
