@@ -9,21 +9,21 @@
 //   out = sum_p w_p v_p / sum_p w_p,   w_p = exp2(s_p - max s),   s_p = scale log2(e) (q . k_p)
 //
 // Work items, their records and the splits of long contexts are lsk_cache_attn_plan's (below).  Two kernels walk them:
-// cache_attn_kernel, whose waves share the positions of up to two row groups of 32 rows, and cache_tree_kernel for trees
-// of more rows, whose waves share K and V.
+// cache_attn_kernel, whose waves share the positions of up to two row groups of 32 rows, and cache_tree_kernel for
+// trees of more rows, whose waves share K and V.
 //
 // Both cache formats are read as 1 KiB fragments in lane order, 64 D bytes per block of STEP positions:
-//   bf16   STEP = 32: K fragment (a, f), lane 16 lg + l16: position 8 (l16 / 4) + 4 a + l16 % 4, d = 32 f + 8 lg .. + 7;
-//          V^T: row d, positions 8 lg .. + 7.
+//   bf16   STEP = 32: K fragment (a, f), lane 16 lg + l16: position 8 (l16 / 4) + 4 a + l16 % 4,
+//          d = 32 f + 8 lg .. + 7; V^T: row d, positions 8 lg .. + 7.
 //   8-bit  STEP = 64: e4m3 codes; K fragment (a, j): position 16 (l16 / 4) + 4 a + l16 % 4, d = 64 j + 16 lg .. + 15
 //          (two MFMA operands of 8 d each); V^T: row d, positions 16 lg .. + 15 (two operands of 8 positions each).
 //          A position's K and V are its codes times 2^(ks - 127) and 2^(vs - 127).
 // Per step of a wave (v_mfma_f32_16x16x32_bf16): S^T[pos][q] = K Q^T, whose rows are mapped to positions so that lane
 // group lg ends up with the consecutive positions its V^T load needs; online softmax with fp32 statistics;
-// O^T[d][q] += V^T P^T.  e4m3 values times a power of two are bf16 values, so the conversions in registers are exact and
-// K's scale costs nothing (the conversion takes one); V's scale, which differs per position, multiplies the weights.
-// The weights are rounded to bf16 for the second product (relative 2^-9 each, independent of one another: it adds about
-// as much error as the rounding of the bf16 output); the sum of the weights is taken before that rounding.
+// O^T[d][q] += V^T P^T.  e4m3 values times a power of two are bf16 values, so the conversions in registers are exact
+// and K's scale costs nothing (the conversion takes one); V's scale, which differs per position, multiplies the
+// weights.  The weights are rounded to bf16 for the second product (by at most 2^-8 each, independent of one another:
+// it adds about as much error as the rounding of the bf16 output); the sum of the weights is taken before that rounding.
 //
 // The waves of a row group take the steps round robin and are merged in wave order.  Which wave takes a step and every
 // order of additions depend on absolute positions only: a row's result never depends on what else is in the launch.  An
@@ -85,9 +85,9 @@ __device__ __forceinline__ float exp_bits(uint32_t byte) { return __uint_as_floa
 #define ORDER() __builtin_amdgcn_sched_barrier(0)  // (keeps the loads and conversions where their registers are free)
 #define LAG 8.0f
 
-// K / V through buffer loads over an item's (row, KV head) stripe, whose range ends with the block that holds the item's
-// last position: loads past it give zeros without touching memory, so the next step's are unconditional (under a branch
-// the compiler would wait for them early).
+// K / V through buffer loads over an item's (row, KV head) stripe, whose range ends with the block that holds the
+// item's last position: loads past it give zeros without touching memory, so the next step's are unconditional (under
+// a branch the compiler would wait for them early).
 struct Stripe {
   __amdgpu_buffer_rsrc_t k, v, ks, vs;
 };
@@ -183,14 +183,14 @@ __device__ __forceinline__ void add_odd(const CacheAttnArgs& A, __amdgpu_buffer_
   }
 }
 
-// The online softmax of one tile's 16 query columns over a step: s[a][e] are the scores of this lane's slots 4 a + e, of
-// which `reads` says what the column reads (FULL: all), vsr V's exponents of the slots (8-bit); pb the weights for the
-// second product.  A row's m only moves when a score passes it by more than LAG (weights up to 2^LAG; each row for
+// The online softmax of one tile's 16 query columns over a step: s[a][e] are the scores of this lane's slots 4 a + e,
+// of which `reads` says what the column reads (FULL: all), vsr V's exponents of the slots (8-bit); pb the weights for
+// the second product.  A row's m only moves when a score passes it by more than LAG (weights up to 2^LAG; each row for
 // itself, so the rows of a tile stay independent), which is seldom after the first step: then no maximum crosses lanes
 // and nothing is rescaled.  Each lane sums its own slots' weights.
 template <bool KV8, bool FULL, int NA, int CT, int HV>
-__device__ __forceinline__ void softmax_tile(lsk_f32x4 (&s)[NA], uint32_t reads, lsk_i32x4 vsr, float scale_log2, float& m,
-                                             float& l, lsk_f32x4 (&o)[CT], lsk_bf16x8 (&pb)[HV]) {
+__device__ __forceinline__ void softmax_tile(lsk_f32x4 (&s)[NA], uint32_t reads, lsk_i32x4 vsr, float scale_log2,
+                                             float& m, float& l, lsk_f32x4 (&o)[CT], lsk_bf16x8 (&pb)[HV]) {
   float mt = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 4 * NA; ++i) {
@@ -226,9 +226,9 @@ __device__ __forceinline__ void softmax_tile(lsk_f32x4 (&s)[NA], uint32_t reads,
 }
 
 // A workgroup has four waves, and each CU two workgroups (n_slots): one's first loads and merge fall into the other's
-// steps.  Against one workgroup of eight waves (8B heads, 8-bit, decode): 256 requests of 250 positions 28 us against 46,
-// of 960 81 against 91, of 4000 313 against 311; 7B heads, 16 trees of 30 nodes and 960 positions 30 against 36; one
-// request of 100000 positions, 1B heads, 25 against 23.
+// steps.  Against one workgroup of eight waves (8B heads, 8-bit, decode): 256 requests of 250 positions 28 us against
+// 46, of 960 81 against 91, of 4000 313 against 311; 7B heads, 16 trees of 30 nodes and 960 positions 30 against 36;
+// one request of 100000 positions, 1B heads, 25 against 23.
 #define CACHE_WAVES 4
 template <int D, int QT, bool KV8, bool TREE>
 __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const CacheAttnArgs A) {
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
   auto q_store = [&](const Item& it) {
     if constexpr (!QREG) {
       int t0 = tid;
-      asm volatile("" : "+v"(t0));                   // (the chunks' offsets are not kept across the items: they spilled)
+      asm volatile("" : "+v"(t0));                   // (the chunks' offsets, kept across the items, spilled)
 #pragma unroll
       for (int i = 0; i < QPT; ++i) {
         const int c = t0 + i * 64 * NW, row = c / QCH;
@@ -312,8 +312,8 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
     }
   };
   auto stripe = [&](const Item& it) { return cache_stripe<D, KV8>(A, it.crow, it.kvh, it.kv_hi); };
-  // Non-temporal where each byte is read once (32 trees of 16 nodes, 7B heads, 960 positions of bf16: 95 us against 80);
-  // not where two row groups read it (39 nodes: 111 us against 118)
+  // Non-temporal where each byte is read once (32 trees of 16 nodes, 7B heads, 960 positions of bf16: 95 us against
+  // 80); not where two row groups read it (39 nodes: 111 us against 118)
   constexpr int AUX = TREE && QT == 2 ? 0 : 2;
   auto ld = [&](__amdgpu_buffer_rsrc_t rs, int vo, int so) -> lsk_i32x4 {
     return __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, vo, so, AUX));
@@ -550,13 +550,13 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
   }
 }
 
-// Trees of more rows: an item of four or eight row groups of 32 rows, whose waves read the same K and V.  Two steps' at a
-// time go through LDS, in two buffers: each wave reading them for itself takes up to eight times the 64 bytes per clock
-// of the CU's cache (32 trees of 64 nodes, 8B heads, 960
-// positions: 45 us; without LDS 67).  8-bit codes become bf16 on the way, once for all the waves.  Q stays in registers.
-// A wave with eight row groups takes both steps, with four every other one; then the two waves of a row group are merged.
-// Bound by the softmax's vector instructions beside the products: 32 positions of 256 rows take 0.9 us, of which the
-// matrix instructions are half.
+// Trees of more rows: an item of four or eight row groups of 32 rows, whose waves read the same K and V.  Two steps'
+// at a time go through LDS, in two buffers: each wave reading them for itself takes up to eight times the 64 bytes per
+// clock of the CU's cache (32 trees of 25 to 64 nodes, 8B heads, 128 to 1280 positions: 67 us without LDS, 52 with it,
+// 45 with at most four row groups).  8-bit codes become bf16 on the way, once for all the waves.  Q stays in registers.
+// A wave with eight row groups takes both steps, with four every other one; then the two waves of a row group are
+// merged.  Bound by the softmax's vector instructions beside the products: 32 positions of 256 rows take 0.9 us, of
+// which the matrix instructions are half.
 #define TREE_WAVES 8
 template <int D, bool KV8>
 __global__ __launch_bounds__(64 * TREE_WAVES, 1) void cache_tree_kernel(const CacheAttnArgs A,
@@ -768,9 +768,9 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 1) void cache_tree_kernel(const Ca
 }
 
 // Merge the splits of a row in split order: M = max_s m_s, w_s = exp2(m_s - M), out = sum w_s O_s / sum w_s l_s (zeros
-// where no split read anything).  A wave per row: the lanes take the splits' statistics side by side, then each its dims
-// of the partial outputs, 16 splits' loads in flight.  (One workgroup per group of rows with a split after the other:
-// 25 us more for 5 tokens over 100000 positions in 98 splits.)
+// where no split read anything).  A wave per row: the lanes take the splits' statistics side by side, then each its
+// dims of the partial outputs, 16 splits' loads in flight.  (One workgroup per group of rows with a split after the
+// other: 25 us more for 5 tokens over 100000 positions in 98 splits.)
 template <int D>
 __global__ __launch_bounds__(256) void cache_combine_kernel(const int32_t* __restrict__ groups,
                                                             const float* __restrict__ o_part,
@@ -826,11 +826,11 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(const int32_t* __res
 }
 
 // ----------------------------------------------------------------------------- fp32 trees
-// The token-identity model's kernel: a wave per query row walks the row's slots in 64-position chunks (lane = slot, then
-// lane = dim), in the ragged attention's order of additions (a chain gives its bits), skipping the slots the row does not
-// read.  The four rows of a workgroup share the chunk's K and V in LDS, fetched in whole lines while the chunk before is
-// worked on: a wave that reads K for itself touches 64 lines with every load, which bounded it (4 trees of 12 nodes, 1B
-// heads, 192 positions: 23.7 us against 11.3).  Bound by the chain of a row's additions.
+// The token-identity model's kernel: a wave per query row walks the row's slots in 64-position chunks (lane = slot,
+// then lane = dim), in the ragged attention's order of additions (a chain gives its bits), skipping the slots the row
+// does not read.  The four rows of a workgroup share the chunk's K and V in LDS, fetched in whole lines while the
+// chunk before is worked on: a wave that reads K for itself touches 64 lines with every load, which bounded it (4
+// trees of 12 nodes, 1B heads, 192 positions: 23.7 us against 11.3).  Bound by the chain of a row's additions.
 #define F32_ROWS 4
 // x[i] + x[i ^ 32], then ^ 16, 8, 4, 2, 1 (or the maxima): rotations by 8 and 4 within rows of 16 lanes equal the
 // exchanges, the values having that period by then
@@ -852,8 +852,8 @@ __device__ __forceinline__ float wave_reduce(float x, F f) {
 template <int D>
 __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
     const float* __restrict__ q, long q_st, long q_sh, const float* __restrict__ kc, const float* __restrict__ vc,
-    const uint32_t* __restrict__ mask, int W, const int32_t* __restrict__ works, float* __restrict__ out, int G, int Hkv,
-    int S, float scale) {
+    const uint32_t* __restrict__ mask, int W, const int32_t* __restrict__ works, float* __restrict__ out, int G,
+    int Hkv, int S, float scale) {
   constexpr int DPL = (D + 63) / 64;
   constexpr int KLD = D + 4, VLD = 68;               // floats of an LDS row of K (a position), of V (a dim)
   constexpr int NT = 64 * F32_ROWS, PER = 64 * D / 4 / NT;
@@ -961,8 +961,8 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 //           it, for caches of few stripes, whose launches have too few items otherwise (64-node trees, 8B heads, 960
 //           positions, at most 8 / 4 / 2 row groups: 8 trees 39 / 27 / 21 us, 16 trees 40 / 28 / 37, 64 trees
 //           96 / 109 / 170; 32 trees of 25 to 64 nodes over 128 to 1280 positions 52 / 45 / 55).
-// The number of row groups follows from the block's rows and the cache alone, so it never makes a row's result depend on
-// the batch.  Items go longest first to the least-loaded of n_slots persistent workgroups, as in lsk_attn_schedule.
+// The number of row groups follows from the block's rows and the cache alone, so it never makes a row's result depend
+// on the batch.  Items go longest first to the least-loaded of n_slots persistent workgroups, as in lsk_attn_schedule.
 extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int n_kv_heads, int head_dim,
                                    int kv8, int tree, int row_groups, int n_slots, int32_t* meta, long meta_cap,
                                    long* counts) {
@@ -1023,7 +1023,8 @@ extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int
       if (ns > 1) np += ns;
     }
   }
-  LSK_REQUIRE(np < (1L << 24) && (long)(items.size() + shared.size()) < (1L << 28), LSK_ESHAPE, "%s: too many work items", what);
+  LSK_REQUIRE(np < (1L << 24) && (long)(items.size() + shared.size()) < (1L << 28), LSK_ESHAPE,
+              "%s: too many work items", what);
   const auto longer = [](const It& a, const It& b) { return a.cost > b.cost; };
   std::stable_sort(items.begin(), items.end(), longer);
   std::stable_sort(shared.begin(), shared.end(), longer);
@@ -1071,8 +1072,8 @@ static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Checks and launches shared by the two entry points; kv8: the cache is 8-bit.
 static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t* groups, int n_groups, int n_parts,
-                      int n_slots, int n_shared, int tiles, int row_groups, int head_dim, float scale, void* workspace, size_t ws_bytes,
-                      hipStream_t s) {
+                      int n_slots, int n_shared, int tiles, int row_groups, int head_dim, float scale, void* workspace,
+                      size_t ws_bytes, hipStream_t s) {
   LSK_REQUIRE(head_dim == 64 || head_dim == 128, LSK_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128)", what,
               head_dim);
   LSK_REQUIRE(tiles == 1 || tiles == 2 || (tiles == 3 && head_dim == 64 && a.mask == nullptr), LSK_EARG,
@@ -1143,8 +1144,9 @@ static int shape_args(const char* what, const void* q, const void* kc, const voi
 extern "C" int lsk_kv8_attn(const void* q, long q_stride_t, long q_stride_h, const void* k8, const void* v8,
                             const void* k_exp, const void* v_exp, const uint32_t* mask, int mask_words,
                             const int32_t* groups, int n_groups, int n_parts, const int32_t* recs, int n_rounds,
-                            int n_slots, int n_shared, int tiles, int row_groups, int part_rows, void* out, int n_heads, int n_kv_heads, int head_dim,
-                            int max_seq, float scale, void* workspace, size_t ws_bytes, void* stream) {
+                            int n_slots, int n_shared, int tiles, int row_groups, int part_rows, void* out, int n_heads,
+                            int n_kv_heads, int head_dim, int max_seq, float scale, void* workspace, size_t ws_bytes,
+                            void* stream) {
   const char* what = "lsk_kv8_attn";
   if (int rc = shape_args(what, q, k8, v8, out, n_heads, n_kv_heads, head_dim, max_seq, q_stride_t, q_stride_h))
     return rc;
@@ -1157,16 +1159,16 @@ extern "C" int lsk_kv8_attn(const void* q, long q_stride_t, long q_stride_h, con
   const CacheAttnArgs a = {(const uint16_t*)q, q_stride_t, q_stride_h, k8, v8, (const uint8_t*)k_exp,
                            (const uint8_t*)v_exp, mask, mask_words, recs, n_rounds, (uint16_t*)out, nullptr, nullptr,
                            part_rows, n_heads / n_kv_heads, n_kv_heads, max_seq, 0.f};
-  return cache_attn(what, true, a, groups, n_groups, n_parts, n_slots, n_shared, tiles, row_groups, head_dim, scale, workspace,
-                    ws_bytes, (hipStream_t)stream);
+  return cache_attn(what, true, a, groups, n_groups, n_parts, n_slots, n_shared, tiles, row_groups, head_dim, scale,
+                    workspace, ws_bytes, (hipStream_t)stream);
 }
 
 extern "C" int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_stride_h, const void* kcache,
-                             const void* vcache, const uint32_t* mask, int mask_words, const int32_t* works, int n_works,
-                             int rows_cap, const int32_t* groups, int n_groups, int n_parts, const int32_t* recs,
-                             int n_rounds, int n_slots, int n_shared, int tiles, int row_groups, int part_rows, void* out, int n_heads,
-                             int n_kv_heads, int head_dim, int max_seq, float scale, void* workspace, size_t ws_bytes,
-                             void* stream) {
+                             const void* vcache, const uint32_t* mask, int mask_words, const int32_t* works,
+                             int n_works, int rows_cap, const int32_t* groups, int n_groups, int n_parts,
+                             const int32_t* recs, int n_rounds, int n_slots, int n_shared, int tiles, int row_groups,
+                             int part_rows, void* out, int n_heads, int n_kv_heads, int head_dim, int max_seq,
+                             float scale, void* workspace, size_t ws_bytes, void* stream) {
   const char* what = "lsk_tree_attn";
   if (int rc = shape_args(what, q, kcache, vcache, out, n_heads, n_kv_heads, head_dim, max_seq, q_stride_t,
                           q_stride_h)) return rc;
@@ -1182,8 +1184,8 @@ extern "C" int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_s
     const CacheAttnArgs a = {(const uint16_t*)q, q_stride_t, q_stride_h, kcache, vcache, nullptr, nullptr, mask,
                              mask_words, recs, n_rounds, (uint16_t*)out, nullptr, nullptr, part_rows, G, n_kv_heads,
                              max_seq, 0.f};
-    return cache_attn(what, false, a, groups, n_groups, n_parts, n_slots, n_shared, tiles, row_groups, head_dim, scale, workspace,
-                      ws_bytes, s);
+    return cache_attn(what, false, a, groups, n_groups, n_parts, n_slots, n_shared, tiles, row_groups, head_dim, scale,
+                      workspace, ws_bytes, s);
   }
   LSK_REQUIRE(n_works >= 0 && rows_cap > 0 && rows_cap % 16 == 0 && rows_cap <= ATTN_ROWS, LSK_EARG,
               "%s: a plan of %d works of up to %d rows (16, 32 or %d)", what, n_works, rows_cap, ATTN_ROWS);
@@ -1192,9 +1194,10 @@ extern "C" int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_s
   LSK_REQUIRE(max_seq % 32 == 0, LSK_ESHAPE, "%s: max_seq %d", what, max_seq);
   const dim3 grid(n_works, n_kv_heads, rows_cap / F32_ROWS);
 #define LSK_TREE_F32(DD)                                                                                           \
-  tree_attn_f32_kernel<DD><<<grid, 64 * F32_ROWS, 0, s>>>((const float*)q, q_stride_t, q_stride_h, (const float*)kcache,     \
-                                                (const float*)vcache, mask, mask_words, works, (float*)out, G,     \
-                                                n_kv_heads, max_seq, scale)
+  tree_attn_f32_kernel<DD><<<grid, 64 * F32_ROWS, 0, s>>>((const float*)q, q_stride_t, q_stride_h,                 \
+                                                          (const float*)kcache, (const float*)vcache, mask,        \
+                                                          mask_words, works, (float*)out, G, n_kv_heads, max_seq,  \
+                                                          scale)
   switch (head_dim) {
     case 16: LSK_TREE_F32(16); break;
     case 32: LSK_TREE_F32(32); break;

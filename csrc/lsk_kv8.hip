@@ -2,11 +2,11 @@
 //
 // Each token's K (and V) of one KV head is D e4m3 codes and one power-of-two scale 2^e, held as the biased exponent
 // e + 127 in a byte:
-//   amax = the largest finite |x|,  e = the smallest integer >= -117 with amax <= 448 * 2^e  (448: e4m3's largest value),
+//   amax = the largest finite |x|,  e = the smallest integer >= -117 with amax <= 448 * 2^e  (448 is e4m3's largest),
 //   code = rne_e4m3(x * 2^-e),  the cache stands for code * 2^e.  NaN and infinities become NaN codes; amax = 0: e = 0.
 // With e >= -117 every value is zero or a normal number (e4m3's smallest is 2^-9), in bf16 as in fp32.
-// The product x * 2^-e is exact (a value far below amax may underflow, where its code is 0 anyway), so the only rounding
-// is the one to e4m3: at most 2^-4 of the value, or 2^-10 * 2^e for values below 2^-6 * 2^e.
+// The product x * 2^-e is exact (a value far below amax may underflow, where its code is 0 anyway), so the only
+// rounding is the one to e4m3: at most 2^-4 of the value, or 2^-10 * 2^e for values below 2^-6 * 2^e.
 //
 // Storage of one (row, KV head) stripe of S positions (S a multiple of 64), 64-position blocks of 64 D bytes:
 //   K  fragments (a, j) of 16 positions x 64 d, 1 KiB in lane order: lane 16 lg + l16 holds position
@@ -66,7 +66,9 @@ __device__ __forceinline__ void store4(uint16_t* p, const float* x) {
   u[1] = (uint32_t)f2bf(x[2]) | ((uint32_t)f2bf(x[3]) << 16);
   *(lsk_u32x2_u*)p = u;
 }
-__device__ __forceinline__ void store4(float* p, const float* x) { *(lsk_f32x4_u*)p = (lsk_f32x4_u){x[0], x[1], x[2], x[3]}; }
+__device__ __forceinline__ void store4(float* p, const float* x) {
+  *(lsk_f32x4_u*)p = (lsk_f32x4_u){x[0], x[1], x[2], x[3]};
+}
 
 // Four dwords of four bytes, turned: byte j of a[i] <-> byte i of a[j]
 __device__ __forceinline__ void turn4(uint32_t* a) {
@@ -139,11 +141,11 @@ __device__ __forceinline__ void kv8_dwords(long stripe, int p0, int nt, F f) {
 
 }  // namespace
 
-// Workgroup 0 of blockIdx.z quantises 64 tokens' V of one KV head (it takes longest and starts first), workgroups 1 .. 4
-// 16 tokens' K each.  16 threads
-// hold a token's vector, D / 16 consecutive elements each, and find its largest magnitude by shuffles.  K goes straight
-// to its place.  V is turned, 4 x 4 in registers and the rest in LDS: a run of positions (a prompt's tokens) is written
-// a dword at a time, whole 64-byte sectors from one workgroup; other tokens byte by byte.
+// Workgroup 0 of blockIdx.z quantises 64 tokens' V of one KV head (it takes longest and starts first), workgroups 1 to 4
+// quantise 16 tokens' K each.  16 threads hold a token's vector, D / 16 consecutive elements each, and find its largest
+// magnitude by shuffles.  K goes straight to its place.  V is turned, 4 x 4 in registers and the rest in LDS: a run of
+// positions (a prompt's tokens) is written a dword at a time, whole 64-byte sectors from one workgroup; other tokens
+// byte by byte.
 // Latency-bound for a decode step's tokens; a long prompt moves 3 D bytes a token and head (4001 tokens of 8 heads of
 // 128: 11.8 us; with the V workgroups last 13.4; with 16 tokens to every workgroup, so that four share a sector of V,
 // 16.9).
@@ -304,8 +306,8 @@ static int kv8_args(const char* what, int dtype, const void* k, const void* v, c
   LSK_REQUIRE(d == 64 || d == 128, LSK_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128)", what, d);
   LSK_REQUIRE(n >= 0 && hkv > 0 && hkv <= 65535 && b > 0 && s > 0 && s % 64 == 0, LSK_ESHAPE,
               "%s: bad shape (max_seq %% 64 == 0)", what);
-  LSK_REQUIRE((((uintptr_t)kc | (uintptr_t)vc) & 15) == 0, LSK_EARG, "%s: the cache tensors start at multiples of 16 bytes",
-              what);
+  LSK_REQUIRE((((uintptr_t)kc | (uintptr_t)vc) & 15) == 0, LSK_EARG,
+              "%s: the cache tensors start at multiples of 16 bytes", what);
   return 0;
 }
 

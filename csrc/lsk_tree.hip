@@ -130,15 +130,16 @@ extern "C" int lsk_tree_accept(const int64_t* Yv, const int64_t* tokens, const i
               "%s: null pointer", what);
   LSK_REQUIRE(nb >= 0 && n_tokens >= 0 && max_nodes > 0, LSK_ESHAPE, "%s: bad shape", what);
   if (nb == 0) return 0;
-  tree_accept_kernel<<<nb, 64, 0, (hipStream_t)stream>>>(Yv, tokens, parents, starts, lens, n_tokens, max_nodes, acc_out,
-                                                         path_out, tokens_out);
+  tree_accept_kernel<<<nb, 64, 0, (hipStream_t)stream>>>(Yv, tokens, parents, starts, lens, n_tokens, max_nodes,
+                                                         acc_out, path_out, tokens_out);
   return lsk_check_launch(what);
 }
 
-// Slot pos0 + j takes what slot pos0 + path[j] holds, for the accepted j = 1 .. acc, in every layer: the accepted path's
-// K / V become consecutive and the committed length is pos0 + acc + 1.  Sources lie at or after their destinations
-// (path is increasing, path[j] >= j) and later destinations never reach an earlier chunk's sources, so a workgroup reads
-// 16 slots of one (layer, block, KV head), waits, and writes them, chunk after chunk.  Slots that stay are skipped.
+// Slot pos0 + j takes what slot pos0 + path[j] holds, for the accepted j = 1 .. acc, in every layer: the accepted
+// path's K / V become consecutive and the committed length is pos0 + acc + 1.  Sources lie at or after their
+// destinations (path is increasing, path[j] >= j) and later destinations never reach an earlier chunk's sources, so a
+// workgroup reads 16 slots of one (layer, block, KV head), waits, and writes them, chunk after chunk.  Slots that stay
+// are skipped.
 // FMT: 0 fp32 (K [S, D], V in 32-position blocks), 1 bf16 (fragment-major K, V in 32-position blocks), 2 8-bit.
 #define COMPACT_CHUNK 16
 #define COMPACT_THREADS 256
@@ -165,10 +166,11 @@ __device__ __forceinline__ long compact_k(int p, int ch, int D) {
   const int pp = p & 63, a = (pp >> 2) & 3, l16 = ((pp >> 4) << 2) | (pp & 3);
   return (long)(p >> 6) * 64 * D + (long)((a * (D >> 6) + (ch >> 2)) * 64 + (ch & 3) * 16 + l16) * 16;
 }
-// K moves in 16-byte pieces of a slot.  V^T has a slot's values 64 bytes (fp32: 128) apart, D of them: the chunk's blocks
-// are turned in LDS, read and written in 16-byte pieces of eight (four, sixteen) slots, so that the memory sees a request
-// per dim and piece and not one per moved value, which bounded it (130 slots of 32 requests, 32 layers of 8 heads of
-// 128: 42 us against 59).  Only pieces that hold a source or a destination are touched; a piece's other slots
+
+// K moves in 16-byte pieces of a slot.  V^T has a slot's values 64 bytes (fp32: 128) apart, D of them: the chunk's
+// blocks are turned in LDS, read and written in 16-byte pieces of eight (four, sixteen) slots, so that the memory sees
+// a request per dim and piece and not one per moved value, which bounded it (130 slots of 32 requests, 32 layers of 8
+// heads of 128: 42 us against 59).  Only pieces that hold a source or a destination are touched; a piece's other slots
 // are written back as they were.
 template <int FMT, int D>
 __global__ __launch_bounds__(COMPACT_THREADS) void kv_compact_kernel(
@@ -185,7 +187,7 @@ __global__ __launch_bounds__(COMPACT_THREADS) void kv_compact_kernel(
   constexpr int PROWS = COMPACT_THREADS / PPR, NP = (D + PROWS - 1) / PROWS;
   constexpr int none = 0x7fffffff;
   __shared__ int s_from[COMPACT_CHUNK];              // slot that slot to + j takes its contents from; -1: it stays
-  __shared__ uint32_t s_v[3][D * LD];                // the two blocks the chunk's destinations may lie in, and one other
+  __shared__ uint32_t s_v[3][D * LD];                // the two blocks the destinations may lie in, and one other
   const int b = blockIdx.x, h = blockIdx.y, layer = blockIdx.z;
   const int row = rows[b], p0 = pos0[b];
   const int n = (int)min(acc[b], (int64_t)(max_nodes - 1));

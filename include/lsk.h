@@ -304,35 +304,39 @@ int lsk_kv8_read(int dtype, const void* k8, const void* v8, const void* k_exp, c
  * mask (uint32 [n_tokens][mask_words]), of the block's own slots only those whose bit is set: bit j % 32 of word j / 32
  * for node j; bits of later nodes and bits past the words count as 0.  A row that reads nothing gives zeros.  Values in
  * slots that a row does not read never reach it, whatever they are.
- * groups .. part_rows: lsk_cache_attn_plan's (fp32 trees: works, n_works, rows_cap of an unsplit lsk_attn_plan instead).
+ * groups .. part_rows: lsk_cache_attn_plan's (fp32 trees: works, n_works, rows_cap of an unsplit lsk_attn_plan).
  * workspace >= lsk_cache_attn_workspace_bytes(n_parts, n_kv_heads, part_rows, head_dim), 16-byte aligned, and a call's
- * own.  head_dim 64 or 128 (fp32 also 16 and 32).  A row's result depends on its own block (with a mask: also on the
- * plan's row_groups) and the split only, not on the rest of the launch; an fp32 chain (every ancestor's bit set) gives
- * lsk_ragged_attn's bits.
+ * own (one that two captured graphs share is written by both).  head_dim 64 or 128 (fp32 also 16 and 32); scale not
+ * negative; bf16 and 8-bit: max_seq a multiple of 64, a (row, KV head) stripe below 2 GiB.  A row's result depends on
+ * its own block (with a mask: also on the plan's row_groups) and the split only, not on the rest of the launch; an fp32
+ * chain (every ancestor's bit set) gives lsk_ragged_attn's bits.
  * Beside lsk_ragged_attn (solutions/packed.py:142-166).
  *
- * lsk_cache_attn_plan (host pointers, no GPU work): blocks int32 [nb][4] = {q_start, pos0, T, row}; split: positions per
- * split, a multiple of 64, at most 128 splits per context.  tree: the launch has a mask; then blocks of many rows share
- * K / V among up to row_groups (1, 2, 4, 8) groups of waves.  meta = [groups int32 n_groups*8][recs
- * n_slots*n_rounds*8, then n_shared*8]; counts[9] = {tokens, n_groups, n_parts, n_rounds, tiles, part_rows, words of
- * meta, row_groups used, n_shared}.  meta == NULL: counts only; meta_cap too small: LSK_EWORKSPACE with counts written. */
+ * lsk_cache_attn_plan (host pointers, no GPU work): blocks int32 [nb][4] = {q_start, pos0, T, row}; split: positions
+ * per split, a multiple of 64, at most 128 splits per context.  tree: the launch has a mask; then blocks of many rows
+ * share K / V among up to row_groups (1, 2, 4, 8) groups of 32 rows.  n_slots: persistent workgroups, two per CU; recs:
+ * their items, and behind them the n_shared items of four and eight row groups (a workgroup each).  meta = [groups
+ * int32 n_groups*8][recs n_slots*n_rounds*8, then n_shared*8]; counts[9] = {tokens, n_groups, n_parts, n_rounds, tiles,
+ * part_rows, words of meta, row_groups used, n_shared}.  meta == NULL: counts only; meta_cap too small: LSK_EWORKSPACE
+ * with counts written. */
 int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int n_kv_heads, int head_dim, int kv8,
                         int tree, int row_groups, int n_slots, int32_t* meta, long meta_cap, long* counts);
 size_t lsk_cache_attn_workspace_bytes(int n_parts, int n_kv_heads, int part_rows, int head_dim);
 int lsk_kv8_attn(const void* q, long q_stride_t, long q_stride_h, const void* k8, const void* v8, const void* k_exp,
                  const void* v_exp, const uint32_t* mask, int mask_words, const int32_t* groups, int n_groups,
-                 int n_parts, const int32_t* recs, int n_rounds, int n_slots, int n_shared, int tiles, int row_groups, int part_rows,
-                 void* out, int n_heads, int n_kv_heads, int head_dim, int max_seq, float scale, void* workspace,
-                 size_t ws_bytes, void* stream);
+                 int n_parts, const int32_t* recs, int n_rounds, int n_slots, int n_shared, int tiles, int row_groups,
+                 int part_rows, void* out, int n_heads, int n_kv_heads, int head_dim, int max_seq, float scale,
+                 void* workspace, size_t ws_bytes, void* stream);
 int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_stride_h, const void* kcache, const void* vcache,
                   const uint32_t* mask, int mask_words, const int32_t* works, int n_works, int rows_cap,
                   const int32_t* groups, int n_groups, int n_parts, const int32_t* recs, int n_rounds, int n_slots,
-                  int n_shared, int tiles, int row_groups, int part_rows, void* out, int n_heads, int n_kv_heads, int head_dim,
-                  int max_seq, float scale, void* workspace, size_t ws_bytes, void* stream);
+                  int n_shared, int tiles, int row_groups, int part_rows, void* out, int n_heads, int n_kv_heads,
+                  int head_dim, int max_seq, float scale, void* workspace, size_t ws_bytes, void* stream);
 
 /* ---- trees of drafted tokens (the reference drafts chains) ----
  * A block's nodes are its tokens 0 .. lens[b] - 1 from starts[b]; node 0 is the root (the last committed token),
- * parents[starts[b] + i] < i the parent of node i (anything outside [0, i): none).  Node i's K / V sit in slot pos0 + i.
+ * parents[starts[b] + i] < i the parent of node i (anything outside [0, i): none).  Node i's K / V sit in slot
+ * pos0 + i.
  *
  * lsk_tree_masks: mask [n_tokens][mask_words] (32 * mask_words >= max_nodes >= every len) = the bits of each node's
  * ancestors and its own; depth [n_tokens] (optional) = its number of ancestors (its RoPE position is pos0 + depth).
@@ -347,7 +351,8 @@ int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_stride_h, co
  * lsk_kv_compact: slot pos0[b] + j of cache row rows[b] takes what slot pos0[b] + path[b][j] holds, j = 1 ..
  * accepted[b], in every layer and KV head (caches [n_layers, max_batch, ...], contiguous; k_exp, v_exp for
  * LSK_DTYPE_KV8, else NULL); then lsk_kv_rollback's pointer update holds as for a chain.  path as lsk_tree_accept
- * writes it (increasing); the rows of a call have to differ.  Blocks outside the cache are skipped. */
+ * writes it (increasing); the rows of a call have to differ.  Blocks outside the cache are skipped.  V's neighbouring
+ * slots of a moved one (16 bytes) are written back as they were. */
 int lsk_tree_masks(const int32_t* parents, const int32_t* starts, const int32_t* lens, int nb, int n_tokens,
                    int max_nodes, uint32_t* mask, int mask_words, int32_t* depth, void* stream);
 int lsk_tree_accept(const int64_t* Yv, const int64_t* tokens, const int32_t* parents, const int32_t* starts,

@@ -218,8 +218,8 @@ def test_kv8_runs_of_positions_from_any_start(cuda, D):
     lsk = _lsk()
     g = _gen(31)
     B, h, S = 6, 2, 256
-    runs = [(0, 1, 16), (1, 2, 33), (2, 57, 31), (2, 88, 40), (3, 240, 16), (4, 3, 1), (0, 61, 5), (5, 255, 1), (5, 0, 96),
-            (4, 130, 29)]
+    runs = [(0, 1, 16), (1, 2, 33), (2, 57, 31), (2, 88, 40), (3, 240, 16), (4, 3, 1), (0, 61, 5), (5, 255, 1),
+            (5, 0, 96), (4, 130, 29)]
     rows = torch.cat([torch.full((n,), r) for (r, _, n) in runs])
     pos = torch.cat([torch.arange(p, p + n) for (_, p, n) in runs])
     for shift in (0, 3):                              # (the second time the workgroups hold other runs)
@@ -475,7 +475,8 @@ def test_bad_values_in_trees_of_many_rows_stay_with_their_readers(cuda, kind, ba
             assert plan.tree.n_shared == 3 * Hkv and plan.tree.n_rounds == 0
             return lsk.kv8_attn(q.to(cuda), cache, plan, mask).cpu()
         ks = lsk.k_to_frag(k).to(cuda)
-        return lsk.tree_attn(q.to(cuda), ks, lsk.v_to_blocked(v).to(cuda), lsk.AttnPlan(tab, Hq, ks, None, 8), mask).cpu()
+        plan = lsk.AttnPlan(tab, Hq, ks, None, 8)
+        return lsk.tree_attn(q.to(cuda), ks, lsk.v_to_blocked(v).to(cuda), plan, mask).cpu()
 
     clean = run(k, v)
     k2, v2 = k.clone(), v.clone()
@@ -856,7 +857,8 @@ def test_a_tree_step_captured_in_two_graphs(cuda, fmt):
     plan = lsk.AttnPlan(tab, Hq, layers[0] if fmt == "kv8" else layers[0][0], split=128, row_groups=8)
     assert plan.tree.n_parts > 0 and plan.tree.n_shared > 0 and plan.tree.n_rounds > 0
     starts, lens = _i32([b[0] for b in tab], cuda), _i32(sizes, cuda)
-    trow, tpos = _i32(np.repeat(rows, sizes), cuda), _i32(np.concatenate([p + np.arange(t) for p, t in zip(pos0, sizes)]), cuda)
+    trow = _i32(np.repeat(rows, sizes), cuda)
+    tpos = _i32(np.concatenate([p + np.arange(t) for p, t in zip(pos0, sizes)]), cuda)
     r_t, p_t = _i32(rows, cuda), _i32(pos0, cuda)
     par, tok, y = _i32(np.zeros(n), cuda), torch.zeros(n, dtype=torch.int64, device=cuda), torch.zeros(
         n, dtype=torch.int64, device=cuda)
@@ -1003,7 +1005,8 @@ def test_entry_points_refuse_bad_arguments():
     assert k8(a10=1, a11=3, a9=P, a25=P, a26=1 << 20, a18=8) == -1                   # rows per partial below a tile
     assert k8(a23=1 << 25) == -2                                                     # a stripe of 2 GiB and more
     assert k8(a13=0) == 0
-    ok2 = [1, P, 512, 64, P, P, P, 1, None, 0, 0, None, 0, 0, P, 1, 1, 0, 1, 1, 16, P, 8, 2, 64, 128, 0.125, None, 0, None]
+    ok2 = [1, P, 512, 64, P, P, P, 1, None, 0, 0, None, 0, 0, P, 1, 1, 0, 1, 1, 16, P, 8, 2, 64, 128, 0.125, None, 0,
+           None]
     tr = lambda **kw: lib.lsk_tree_attn(*[kw.get(f"a{i}", x) for i, x in enumerate(ok2)])  # noqa: E731
     assert tr(a6=None) == -1 and tr(a7=0) == -1 and tr(a0=2) == -3 and tr(a14=None) == -1 and tr(a24=96) == -3
     assert tr(a0=0) == -1 and tr(a0=0, a9=1, a10=16) == -1 and tr(a0=0, a9=1, a10=24, a8=P) == -1
@@ -1013,7 +1016,8 @@ def test_entry_points_refuse_bad_arguments():
     plan = lambda **kw: lib.lsk_cache_attn_plan(*[kw.get(f"a{i}", x) for i, x in enumerate(  # noqa: E731
         [blk, 1, 4, 256, 2, 128, 1, 1, 8, 256, None, 0, cnt])])
     assert plan() == 0 and list(cnt)[:3] == [40, 1, 3] and cnt[4] == 2 and cnt[7] == 8 and cnt[8] == 6
-    assert plan(a3=100) == -2 and plan(a8=3) == -2 and plan(a5=96) == -3 and plan(a0=None) == -1 and plan(a12=None) == -1
+    assert plan(a3=100) == -2 and plan(a8=3) == -2 and plan(a5=96) == -3 and plan(a0=None) == -1
+    assert plan(a12=None) == -1
     assert plan(a10=blk, a11=4) == -4 and plan(a1=0) == 0 and cnt[3] == cnt[8] == 0
     blk[1] = 64 * 128
     assert plan(a3=64) == -2                                                         # more than 128 splits

@@ -529,7 +529,8 @@ def _one_device(first: torch.Tensor, *ts) -> int:
             break
     if dev < 0:
         _dev(first, *ts)
-        raise LskError(f"tensors on different devices: {sorted({str(t.device) for t in (first, *ts) if t is not None})}")
+        devs = {str(t.device) for t in (first, *ts) if t is not None}
+        raise LskError(f"tensors on different devices: {sorted(devs)}")
     return dev
 
 
@@ -547,8 +548,8 @@ def _launch(dev: int, what: str, *args) -> None:
 
 def _want(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
     if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
-        raise LskError(f"{what}: {name} must be a contiguous {list(shape)} {dtype} tensor, got {list(t.shape)} {t.dtype}"
-                       f"{'' if t.is_contiguous() else ', not contiguous'}")
+        raise LskError(f"{what}: {name} must be a contiguous {list(shape)} {dtype} tensor, got {list(t.shape)} "
+                       f"{t.dtype}{'' if t.is_contiguous() else ', not contiguous'}")
 
 
 _E4M3 = torch.float8_e4m3fn
@@ -676,8 +677,8 @@ def cache_attn_row_groups(max_batch: int, n_kv_heads: int) -> int:
 class _Launch:
     """One lsk_cache_attn_plan on the device, and its arguments of a launch."""
 
-    def __init__(self, groups: torch.Tensor, recs: torch.Tensor, n_groups: int, n_parts: int, n_rounds: int, n_slots: int,
-                 n_shared: int, tiles: int, row_groups: int, part_rows: int, ws_bytes: int):
+    def __init__(self, groups: torch.Tensor, recs: torch.Tensor, n_groups: int, n_parts: int, n_rounds: int,
+                 n_slots: int, n_shared: int, tiles: int, row_groups: int, part_rows: int, ws_bytes: int):
         self.groups, self.recs, self.n_groups, self.n_parts, self.n_rounds = groups, recs, n_groups, n_parts, n_rounds
         self.n_slots, self.n_shared, self.tiles, self.row_groups, self.part_rows, self.ws_bytes = \
             n_slots, n_shared, tiles, row_groups, part_rows, ws_bytes
@@ -757,7 +758,8 @@ def _plan_call(what: str, dev: int, q: torch.Tensor, plan: AttnPlan, launch, dim
     want = torch.bfloat16 if kv8 else dtype
     n, width = plan.n_tokens, plan.width
     if q.shape != plan.q_shape or q.dtype is not want or (n and q.stride(2) != 1):
-        raise LskError(f"{what}: q must be {list(plan.q_shape)} {want} with contiguous dims, got {list(q.shape)} {q.dtype}")
+        raise LskError(f"{what}: q must be {list(plan.q_shape)} {want} with contiguous dims, got {list(q.shape)} "
+                       f"{q.dtype}")
     if mask is not None:
         if mask.dim() != 2 or mask.shape[1] < 1:
             raise LskError(f"{what}: mask must be [{n}, words]")
@@ -850,8 +852,8 @@ def tree_accept(Yv: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, s
     if nb and n == 0:
         acc.fill_(-1), path.fill_(-1), out.fill_(-1)
     elif nb:
-        _launch(dev, "lsk_tree_accept", _ptr(Yv), _ptr(tokens), _ptr(parents), _ptr(starts), _ptr(lens), nb, n, max_nodes,
-                _ptr(acc), _ptr(path), _ptr(out))
+        _launch(dev, "lsk_tree_accept", Yv.data_ptr(), tokens.data_ptr(), parents.data_ptr(), starts.data_ptr(),
+                lens.data_ptr(), nb, n, max_nodes, acc.data_ptr(), path.data_ptr(), out.data_ptr())
     return acc, path, out
 
 
@@ -866,8 +868,8 @@ def _compact(what, code, k, v, ks, vs, layers, dims, rows_i32, pos0_i32, accepte
         raise LskError(f"{what}: path must be [{nb}, max_nodes]")
     _want(what, "path", path, torch.int32, (nb, most))
     if nb and layers:
-        _launch(dev, "lsk_kv_compact", code, k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), layers, rows_i32.data_ptr(),
-                pos0_i32.data_ptr(), accepted.data_ptr(), path.data_ptr(), nb, most, Hkv, D, B, S)
+        _launch(dev, "lsk_kv_compact", code, k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), layers,
+                rows_i32.data_ptr(), pos0_i32.data_ptr(), accepted.data_ptr(), path.data_ptr(), nb, most, Hkv, D, B, S)
 
 
 def kv_compact(k: torch.Tensor, v: torch.Tensor, rows_i32, pos0_i32, accepted, path) -> None:
@@ -876,8 +878,8 @@ def kv_compact(k: torch.Tensor, v: torch.Tensor, rows_i32, pos0_i32, accepted, p
     or a run of their layers); path and accepted: tree_accept's; rows, pos0 int32 [nb], the rows different."""
     shape, code = tuple(k.shape), dtype_code(k.dtype)
     if len(shape) != (7 if code == DTYPE_BF16 else 5) or not k.is_contiguous():
-        raise LskError("kv_compact: the K storage of several layers is needed, contiguous: fragment-major bf16 or row-major "
-                       "fp32")
+        raise LskError("kv_compact: the K storage of several layers is needed, contiguous: fragment-major bf16 or "
+                       "row-major fp32")
     L, B, Hkv = shape[:3]
     S, D = (shape[3] * 32, shape[4] * 16) if code == DTYPE_BF16 else shape[3:]
     _want("kv_compact", "V storage", v, k.dtype, (L, B, Hkv, S // 32, D, 32))
