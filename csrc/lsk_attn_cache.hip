@@ -550,42 +550,41 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
   }
 }
 
-// Trees of more rows: an item of four or eight row groups of 32 rows, whose waves read the same K and V.  Two steps'
-// at a time go through LDS, in two buffers: each wave reading them for itself takes up to eight times the 64 bytes per
-// clock of the CU's cache (32 trees of 25 to 64 nodes, 8B heads, 128 to 1280 positions: 67 us without LDS, 52 with it,
-// 45 with at most four row groups).  8-bit codes become bf16 on the way, once for all the waves.  Q stays in registers.
-// A wave with eight row groups takes both steps, with four every other one; then the two waves of a row group are
-// merged.  Bound by the softmax's vector instructions beside the products: 32 positions of 256 rows take 0.9 us, of
-// which the matrix instructions are half.
-#define TREE_WAVES 8
+// Trees of more rows: an item of four row groups of 32 rows, a wave each, which read the same K and V.  These go through
+// LDS, a step's at a time (8-bit: two steps'), in two buffers: a wave that reads them for itself takes its share of the
+// CU's 64 bytes per clock (32 trees of 25 to 64 nodes, 8B heads, 128 to 1280 positions: 67 us without LDS, 42 with it).
+// 8-bit codes become bf16 on the way, once for all the waves.  Q stays in registers.  Two workgroups fit a CU, so that
+// one's waits fall into the other's steps (one of eight waves, merged at the end: 45 us).
+// Bound by the softmax's vector instructions beside the products and the reads of LDS: 32 positions of 256 rows take
+// 1.3 us of a CU, of which the matrix instructions are 0.5.
+#define TREE_WAVES 4
 template <int D, bool KV8>
-__global__ __launch_bounds__(64 * TREE_WAVES, 1) void cache_tree_kernel(const CacheAttnArgs A,
+__global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const CacheAttnArgs A,
                                                                         const int32_t* __restrict__ items) {
   constexpr int KF = D / 32, CT = D / 16, NW = TREE_WAVES, QT = 2;
-  constexpr int PAIR = 64, NE = 8;                   // positions of a pair of steps; slots of a lane in a step
+  constexpr int STEPS = KV8 ? 2 : 1, CHUNK = 32 * STEPS;  // steps and positions that go through LDS at a time
+  constexpr int NE = 8;                              // slots of a lane in a step
   constexpr uint32_t ALL = 0xffu;
   constexpr int UNITS = 2 * CT;                      // 1 KiB bf16 fragments of a step: K's (a, f), then V's
-  constexpr int UPW = (KV8 ? 1 : 2) * UNITS / NW;    // fragments of a pair, as they are in the cache, per wave
-  constexpr int HALF = UNITS * 1024, BUF = 2 * HALF;
+  constexpr int UPW = UNITS / NW;                    // fragments of a chunk, as they are in the cache, per wave
+  constexpr int HALF = UNITS * 1024, BUF = STEPS * HALF;
   __shared__ __attribute__((aligned(16))) char s_buf[2 * BUF];
-  __shared__ __attribute__((aligned(16))) uint8_t s_vs[2][PAIR];
-  __shared__ float s_ml[4][2][16 * QT];
+  __shared__ __attribute__((aligned(16))) uint8_t s_vs[2][64];
   const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = A.G, Hkv = A.Hkv;
   const int32_t* wk = items + (long)blockIdx.x * 8;
-  const int q_start = wk[0], row0 = wk[1], nrows = wk[2] & 1023, lr = (wk[2] >> 10) & 3, kvh = wk[2] >> 12;
+  const int q_start = wk[0], row0 = wk[1], nrows = wk[2] & 1023, kvh = wk[2] >> 12;
   const int kv_lo = wk[3], kv_hi = wk[4], part = wk[5], pos0 = wk[6], crow = wk[7];
-  const int rb = (wave & ((1 << lr) - 1)) * 16 * QT, rank = wave >> lr;
-  const int own = lr == 3 ? 1 : 2;                   // steps from one of a wave's to the next
+  const int rb = wave * 16 * QT;
   const Stripe sr = cache_stripe<D, KV8>(A, crow, kvh, kv_hi);
-  lsk_i32x4 st[UPW];                                 // the wave's part of the next pair, in flight
+  lsk_i32x4 st[UPW];                                 // the wave's part of the next chunk, in flight
   uint32_t st_ks[UPW], st_vs;                        // 8-bit: exponents of this lane's K, and of position `lane`
   auto st_load = [&](int sb) {
 #pragma unroll
     for (int i = 0; i < UPW; ++i) {                  // (a wave's fragments are all of K or all of V)
-      const int u = wave * UPW + i, w = u % UNITS;
-      const int so = (sb + u / UNITS * 32) * 2 * D / (KV8 ? 2 : 1) + w % CT * 1024;
+      const int w = wave * UPW + i;
+      const int so = sb * (KV8 ? 1 : 2) * D + w % CT * 1024;
       st[i] = __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(
                                                 w < CT ? sr.k : sr.v, w < CT ? 16 * lane : 64 * l16 + 16 * lg, so, 0));
       if constexpr (KV8)
@@ -636,7 +635,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 1) void cache_tree_kernel(const Ca
 #pragma unroll
     for (int c = 0; c < CT; ++c) oacc[qt][c] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  // Step j of the pair at s2 (as in cache_attn_kernel): this lane's slots are s0 .. s0 + 7.
+  // Step j of the chunk at s2 (as in cache_attn_kernel): this lane's slots are s0 .. s0 + 7.
   auto step = [&](auto full_, int s2, int j, int buf) {
     constexpr bool FULL = decltype(full_)::value;
     const char* src = s_buf + buf * BUF + j * HALF + 16 * lane;
@@ -692,54 +691,24 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 1) void cache_tree_kernel(const Ca
       add_odd<KV8, true>(A, sr.v, odd, s2 + (KV8 ? 8 : 32) * j, q_start, pos0, qpos, oacc, KV8 ? 0x18 : 0);
   };
   st_write(0);
-  st_load(kv_lo + PAIR);
+  st_load(kv_lo + CHUNK);
   int s2 = kv_lo, buf = 0;
-  auto pairs = [&](auto full_, int end) {            // the pairs of steps that start before `end`
-    for (; s2 < end; s2 += PAIR, buf ^= 1) {
+  auto chunks = [&](auto full_, int end) {           // those that start before `end`
+    for (; s2 < end; s2 += CHUNK, buf ^= 1) {
       __syncthreads();                               // (the other buffer's readers are done, this one is written)
-      for (int j = rank; j < 2; j += own) {
-        if (s2 + (KV8 ? 8 : 32) * j >= kv_hi || rb >= nrows) break;
+#pragma nounroll
+      for (int j = 0; j < STEPS; ++j) {
+        if (s2 + 8 * j >= kv_hi || rb >= nrows) break;
         step(full_, s2, j, buf);
       }
       st_write(buf ^ 1);
-      st_load(s2 + 2 * PAIR);
+      st_load(s2 + 2 * CHUNK);
     }
   };
-  pairs(std::true_type{}, min(kv_hi, pos0) - PAIR + 1);  // (every row reads them whole)
-  pairs(std::false_type{}, kv_hi);
+  chunks(std::true_type{}, min(kv_hi, pos0) - CHUNK + 1);  // (every row reads them whole)
+  chunks(std::false_type{}, kv_hi);
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) l_run[qt] = rows_sum(l_run[qt]);
-  if (lr == 2) {                                     // O = e_0 O_0 + e_1 O_1, e_w = exp2(m_w - max m), l likewise
-    __syncthreads();
-    lsk_f32x4* so = (lsk_f32x4*)s_buf + (wave & 3) * QT * CT * 64 + lane;
-    if (rank == 1) {
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt) {
-        if (lg == 0) {
-          s_ml[wave & 3][0][16 * qt + l16] = m_run[qt];
-          s_ml[wave & 3][1][16 * qt + l16] = l_run[qt];
-        }
-#pragma unroll
-        for (int c = 0; c < CT; ++c) so[(qt * CT + c) * 64] = oacc[qt][c];
-      }
-    }
-    __syncthreads();
-    if (rank == 1) return;
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      const float m1 = s_ml[wave & 3][0][16 * qt + l16], M = fmaxf(m_run[qt], m1);
-      const float e0 = m_run[qt] == -INFINITY ? 0.f : m_run[qt] == M ? 1.f : fast_exp2(m_run[qt] - M);
-      const float e1 = m1 == -INFINITY ? 0.f : m1 == M ? 1.f : fast_exp2(m1 - M);
-      m_run[qt] = M;
-      l_run[qt] = e0 * l_run[qt] + e1 * s_ml[wave & 3][1][16 * qt + l16];
-#pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        const lsk_f32x4 o1 = so[(qt * CT + c) * 64];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) oacc[qt][c][i] = e0 * oacc[qt][c][i] + e1 * o1[i];
-      }
-    }
-  }
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const int rl = rb + 16 * qt + l16;
@@ -955,12 +924,11 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 // Work items of one launch: 32 rows (token x query head of the group) of a block per wave, 16 where no block has more,
 // 48 for causal launches over 64 dims with larger blocks; the context in splits at absolute multiples of `split`.
 //   causal  an item is one row group: 4 waves share its steps.
-//   tree    a block of more than 32 rows gives an item 2, 4 or 8 row groups (up to 256 rows), whose waves each walk
-//           more of the positions: K / V come from memory once for all of them and fewer partial outputs are
-//           merged.  Items of 4 and 8 are cache_tree_kernel's, one workgroup each, longest first.  row_groups limits
-//           it, for caches of few stripes, whose launches have too few items otherwise (64-node trees, 8B heads, 960
-//           positions, at most 8 / 4 / 2 row groups: 8 trees 39 / 27 / 21 us, 16 trees 40 / 28 / 37, 64 trees
-//           96 / 109 / 170; 32 trees of 25 to 64 nodes over 128 to 1280 positions 52 / 45 / 55).
+//   tree    a block of more than 32 rows gives an item 2 or 4 row groups (up to 128 rows), whose waves each walk more
+//           of the positions: K / V come from memory once for all of them and fewer partial outputs are merged.  Items
+//           of 4 are cache_tree_kernel's, one workgroup each, longest first.  row_groups limits it, for caches of few
+//           stripes, whose launches have too few items otherwise (64-node trees, 8B heads, 960 positions, at most
+//           4 / 2 row groups: 8 trees 30 / 23 us, 16 trees 32 / 34, 32 trees 46 / 59, 64 trees 104 / 144).
 // The number of row groups follows from the block's rows and the cache alone, so it never makes a row's result depend
 // on the batch.  Items go longest first to the least-loaded of n_slots persistent workgroups, as in lsk_attn_schedule.
 extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int n_kv_heads, int head_dim,
@@ -970,8 +938,8 @@ extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int
   LSK_REQUIRE(counts && (blocks || nb == 0), LSK_EARG, "%s: null pointer", what);
   LSK_REQUIRE(nb >= 0 && group > 0 && split >= ATTN_TILE && split % ATTN_TILE == 0 && n_kv_heads > 0 &&
                   n_kv_heads < (1 << 19) && n_slots > 0 &&
-                  (row_groups == 1 || row_groups == 2 || row_groups == 4 || row_groups == 8),
-              LSK_ESHAPE, "%s: bad arguments (split a multiple of %d, row_groups 1, 2, 4 or 8)", what, ATTN_TILE);
+                  (row_groups == 1 || row_groups == 2 || row_groups == 4),
+              LSK_ESHAPE, "%s: bad arguments (split a multiple of %d, row_groups 1, 2 or 4)", what, ATTN_TILE);
   LSK_REQUIRE(head_dim == 64 || head_dim == 128, LSK_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128)", what,
               head_dim);
   const int step = kv8 ? 64 : 32;
@@ -1014,7 +982,7 @@ extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int
       for (int sp = 0; sp < ns; ++sp) {
         const int lo = sp * split, hi = lo + split < end ? lo + split : end;
         // in tenths of a one-tile step: a wave's steps, 1.5 times as long per further tile, and the item's own cost
-        const int share = step * ((lr < 2 ? CACHE_WAVES : TREE_WAVES) >> lr), steps = (hi - lo + share - 1) / share;
+        const int share = step * (CACHE_WAVES >> lr), steps = (hi - lo + share - 1) / share;
         const int cost = steps * (10 + 5 * (tiles - 1)) + 20 + 6 * (tiles - 1);
         for (int h = 0; h < n_kv_heads; ++h)
           (lr < 2 ? items : shared).push_back({{bm[0], (int32_t)row0, nrows | (lr << 10) | (h << 12), lo, hi,
@@ -1087,7 +1055,7 @@ static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t
   LSK_REQUIRE(aligned16(a.kc) && aligned16(a.vc) && (!kv8 || (aligned16(a.ks) && aligned16(a.vs))), LSK_EARG,
               "%s: the cache tensors start at multiples of 16 bytes", what);
   if (n_parts > 0) {
-    LSK_REQUIRE(a.part_rows >= 16 * tiles && a.part_rows <= 128 * tiles, LSK_EARG, "%s: a plan of %d rows per partial",
+    LSK_REQUIRE(a.part_rows >= 16 * tiles && a.part_rows <= 64 * tiles, LSK_EARG, "%s: a plan of %d rows per partial",
                 what, a.part_rows);
     const size_t need = lsk_cache_attn_workspace_bytes(n_parts, a.Hkv, a.part_rows, head_dim);
     LSK_REQUIRE(workspace != nullptr && aligned16(workspace) && ws_bytes >= need && groups != nullptr, LSK_EWORKSPACE,

@@ -333,7 +333,7 @@ def _tree_blocks(blocks, seed):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("split,row_groups", [(None, None), (64, 1), (64, 8), (1024, 2), (128, 4)])
+@pytest.mark.parametrize("split,row_groups", [(None, None), (64, 1), (64, 4), (1024, 2), (128, 4)])
 @pytest.mark.parametrize("blocks", BLOCKS)
 @pytest.mark.parametrize("kind,heads", [("bf16", "gqa128"), ("bf16", "gqa64"), ("bf16", "mqa128"), ("kv8", "gqa128"),
                                         ("kv8", "mha64"), ("fp32", "gqa64"), ("fp32", "mqa128")])
@@ -391,7 +391,7 @@ def test_masks_of_any_kind_and_rows_that_read_nothing(cuda, kind):
             return lsk.tree_attn(q.to(cuda), ks, vs, lsk.AttnPlan(tab, Hq, ks, split, rg), mask)
 
     ref, mag, big = attention(q.double(), k.double(), v.double(), tab, 1 / math.sqrt(D), sets)
-    for split, rg in ((None, 1), (64, 1), (None, 8), (64, 8)):
+    for split, rg in ((None, 1), (64, 1), (None, 4), (64, 4)):
         got = run(split, rg)
         assert (got[:5] == 0).all() and (got[n - 1] == 0).all()
         if kind == "fp32":
@@ -401,7 +401,7 @@ def test_masks_of_any_kind_and_rows_that_read_nothing(cuda, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("row_groups", [1, 8])
+@pytest.mark.parametrize("row_groups", [1, 4])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("kind", ["bf16", "kv8", "kv8 causal", "fp32"])
 def test_values_that_a_row_does_not_read_never_reach_it(cuda, kind, bad, row_groups):
@@ -471,11 +471,11 @@ def test_bad_values_in_trees_of_many_rows_stay_with_their_readers(cuda, kind, ba
             cache = kv8_from(lsk, cuda, k, v)
             for (_, p0, t, row) in tab:                               # slots never written: any byte as a scale
                 cache.ks[row, :, p0 + t:], cache.vs[row, :, p0 + t:] = 255, 255
-            plan = lsk.AttnPlan(tab, Hq, cache, None, 8)
-            assert plan.tree.n_shared == 3 * Hkv and plan.tree.n_rounds == 0
+            plan = lsk.AttnPlan(tab, Hq, cache, None, 4)
+            assert plan.tree.n_shared == 5 * Hkv and plan.tree.n_rounds == 0
             return lsk.kv8_attn(q.to(cuda), cache, plan, mask).cpu()
         ks = lsk.k_to_frag(k).to(cuda)
-        plan = lsk.AttnPlan(tab, Hq, ks, None, 8)
+        plan = lsk.AttnPlan(tab, Hq, ks, None, 4)
         return lsk.tree_attn(q.to(cuda), ks, lsk.v_to_blocked(v).to(cuda), plan, mask).cpu()
 
     clean = run(k, v)
@@ -530,12 +530,12 @@ def test_trees_of_one_node_and_causal_launches_agree(cuda):
     tab, q, k, v = _attn_inputs(43, (Hq, Hkv, D), blocks)
     cache = kv8_from(lsk, cuda, k, v)
     mask = torch.from_numpy(words_of([set(range(i + 1)) for (_, _, t) in blocks for i in range(t)], 1)).to(cuda)
-    plan = lsk.AttnPlan(tab, Hq, cache, split=256, row_groups=8)
+    plan = lsk.AttnPlan(tab, Hq, cache, split=256, row_groups=4)
     assert torch.equal(lsk.kv8_attn(q.to(cuda), cache, plan, mask), lsk.kv8_attn(q.to(cuda), cache, plan))
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("row_groups", [1, 8])
+@pytest.mark.parametrize("row_groups", [1, 4])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("kind", ["kv8", "kv8 tree", "tree"])
 def test_a_rows_result_depends_on_its_block_only(cuda, kind, D, row_groups):
@@ -854,7 +854,7 @@ def test_a_tree_step_captured_in_two_graphs(cuda, fmt):
     layers = [cache.layer(i) for i in range(L)] if fmt == "kv8" else [(cache[0][i], cache[1][i]) for i in range(L)]
     flat = [t.view(torch.uint8) if t.dtype == E4M3 else t for t in cache]
     saved = [t.clone() for t in flat]
-    plan = lsk.AttnPlan(tab, Hq, layers[0] if fmt == "kv8" else layers[0][0], split=128, row_groups=8)
+    plan = lsk.AttnPlan(tab, Hq, layers[0] if fmt == "kv8" else layers[0][0], split=128, row_groups=4)
     assert plan.tree.n_parts > 0 and plan.tree.n_shared > 0 and plan.tree.n_rounds > 0
     starts, lens = _i32([b[0] for b in tab], cuda), _i32(sizes, cuda)
     trow = _i32(np.repeat(rows, sizes), cuda)
@@ -1014,8 +1014,9 @@ def test_entry_points_refuse_bad_arguments():
     cnt = (ctypes.c_long * 9)()
     blk = (ctypes.c_int32 * 4)(0, 700, 40, 0)
     plan = lambda **kw: lib.lsk_cache_attn_plan(*[kw.get(f"a{i}", x) for i, x in enumerate(  # noqa: E731
-        [blk, 1, 4, 256, 2, 128, 1, 1, 8, 256, None, 0, cnt])])
-    assert plan() == 0 and list(cnt)[:3] == [40, 1, 3] and cnt[4] == 2 and cnt[7] == 8 and cnt[8] == 6
+        [blk, 1, 4, 256, 2, 128, 1, 1, 4, 256, None, 0, cnt])])
+    assert plan() == 0 and list(cnt)[:3] == [40, 2, 6] and cnt[4] == 2 and cnt[7] == 4 and cnt[8] == 12
+    assert plan(a8=8) == -2
     assert plan(a3=100) == -2 and plan(a8=3) == -2 and plan(a5=96) == -3 and plan(a0=None) == -1
     assert plan(a12=None) == -1
     assert plan(a10=blk, a11=4) == -4 and plan(a1=0) == 0 and cnt[3] == cnt[8] == 0
@@ -1067,8 +1068,8 @@ def _items(plan, launch):
     """(row group rows, wave rows) of every work item of a plan: [(q_start, row0, nrows, groups, kvh, lo, hi, part)]"""
     one = launch.n_slots * launch.n_rounds * 8
     recs = launch.recs.numpy()[:one].reshape(launch.n_slots, launch.n_rounds, 8)
-    shared = launch.recs.numpy()[one:].reshape(launch.n_shared, 8)     # items of four or eight row groups
-    assert all(r[2] >> 10 & 3 >= 2 for r in shared)
+    shared = launch.recs.numpy()[one:].reshape(launch.n_shared, 8)     # items of four row groups
+    assert all(r[2] >> 10 & 3 == 2 for r in shared)
     out = [(r[0], r[1], r[2] & 1023, 1 << (r[2] >> 10 & 3), r[2] >> 12, r[3], r[4], r[5]) for r in shared]
     for slot in recs:
         live = [r for r in slot if r[2] & 1023]
@@ -1088,7 +1089,7 @@ def test_cache_attention_plans_cover_every_row_and_position_once(G, split, T_hi,
     cache = lsk.KV8.zeros(B, Hkv, S, D, "cpu")
     blocks = [(r, int(rng.integers(0, S - T_hi)), int(rng.integers(0, T_hi + 1))) for r in range(B)]
     tab, n = pack_blocks(blocks)
-    plan = lsk.AttnPlan(tab, G * Hkv, cache, split=split, row_groups=8, tree=tree)
+    plan = lsk.AttnPlan(tab, G * Hkv, cache, split=split, row_groups=4, tree=tree)
     p = plan.tree if tree else plan.causal
     items = _items(plan, p)
     most = max(t for _, _, t in blocks) * G
@@ -1099,7 +1100,7 @@ def test_cache_attention_plans_cover_every_row_and_position_once(G, split, T_hi,
     for (q0, p0, t, row) in tab:
         rows = t * G
         want = 1
-        while tree and want < 8 and rows > 32 * want:
+        while tree and want < 4 and rows > 32 * want:
             want *= 2
         mine = [i for i in items if i[0] == q0] if t else []
         for h in range(Hkv):

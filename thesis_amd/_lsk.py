@@ -671,7 +671,7 @@ def cache_attn_row_groups(max_batch: int, n_kv_heads: int) -> int:
     """Row groups of a tree's work items at most (lsk_cache_attn_plan), fixed by the cache as the split is: caches of
     few stripes keep the rows on as many CUs as there are."""
     stripes = max_batch * n_kv_heads
-    return 8 if stripes >= 512 else 4 if stripes >= 128 else 2 if stripes >= 64 else 1
+    return 4 if stripes >= 128 else 2 if stripes >= 64 else 1
 
 
 class _Launch:
