@@ -926,20 +926,22 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 //   causal  an item is one row group: 4 waves share its steps.
 //   tree    a block of more than 32 rows gives an item 2 or 4 row groups (up to 128 rows), whose waves each walk more
 //           of the positions: K / V come from memory once for all of them and fewer partial outputs are merged.  Items
-//           of 4 are cache_tree_kernel's, one workgroup each, longest first.  row_groups limits it, for caches of few
-//           stripes, whose launches have too few items otherwise (64-node trees, 8B heads, 960 positions, at most
-//           4 / 2 row groups: 8 trees 30 / 23 us, 16 trees 32 / 34, 32 trees 46 / 59, 64 trees 104 / 144).
+//           of 4 are cache_tree_kernel's, one workgroup each, longest first.  Where the cache's (row, KV head) stripes
+//           times the block's tiles of 32 rows are at most n_slots, each tile is an item instead (8B heads, 960
+//           positions, 4 / 2 / 1 row groups: 64 stripes, 64-node trees 30 / 22 / 21 us; 128 stripes, 32 nodes
+//           29 / 22 / 21, 64 nodes 32 / 34 / 37; 256 stripes, 16 nodes - / 29 / 26, 32 nodes 31 / 34 / 37, 64 nodes
+//           46 / 60 / 69).
 // The number of row groups follows from the block's rows and the cache alone, so it never makes a row's result depend
 // on the batch.  Items go longest first to the least-loaded of n_slots persistent workgroups, as in lsk_attn_schedule.
-extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int n_kv_heads, int head_dim,
-                                   int kv8, int tree, int row_groups, int n_slots, int32_t* meta, long meta_cap,
-                                   long* counts) {
+extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int max_batch, int n_kv_heads,
+                                   int head_dim, int kv8, int tree, int row_groups, int n_slots, int32_t* meta,
+                                   long meta_cap, long* counts) {
   const char* what = "lsk_cache_attn_plan";
   LSK_REQUIRE(counts && (blocks || nb == 0), LSK_EARG, "%s: null pointer", what);
   LSK_REQUIRE(nb >= 0 && group > 0 && split >= ATTN_TILE && split % ATTN_TILE == 0 && n_kv_heads > 0 &&
-                  n_kv_heads < (1 << 19) && n_slots > 0 &&
-                  (row_groups == 1 || row_groups == 2 || row_groups == 4),
-              LSK_ESHAPE, "%s: bad arguments (split a multiple of %d, row_groups 1, 2 or 4)", what, ATTN_TILE);
+                  n_kv_heads < (1 << 19) && max_batch > 0 && n_slots > 0 &&
+                  (row_groups == 0 || row_groups == 1 || row_groups == 2 || row_groups == 4),
+              LSK_ESHAPE, "%s: bad arguments (split a multiple of %d, row_groups 0, 1, 2 or 4)", what, ATTN_TILE);
   LSK_REQUIRE(head_dim == 64 || head_dim == 128, LSK_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128)", what,
               head_dim);
   const int step = kv8 ? 64 : 32;
@@ -967,7 +969,8 @@ extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int
     const int pos0 = bm[1];
     const long rows = (long)bm[2] * group;
     int lr = 0;
-    while (tree && (1 << lr) < row_groups && rows > (32L << lr)) ++lr;
+    const int most_groups = row_groups ? row_groups : (long)max_batch * n_kv_heads * ((rows + 31) / 32) <= n_slots ? 1 : 4;
+    while (tree && (1 << lr) < most_groups && rows > (32L << lr)) ++lr;
     used = (1 << lr) > used ? 1 << lr : used;
     const int cap = (16 * tiles) << lr;
     for (long row0 = 0; row0 < rows; row0 += cap) {

@@ -1014,12 +1014,13 @@ def test_entry_points_refuse_bad_arguments():
     cnt = (ctypes.c_long * 9)()
     blk = (ctypes.c_int32 * 4)(0, 700, 40, 0)
     plan = lambda **kw: lib.lsk_cache_attn_plan(*[kw.get(f"a{i}", x) for i, x in enumerate(  # noqa: E731
-        [blk, 1, 4, 256, 2, 128, 1, 1, 4, 256, None, 0, cnt])])
+        [blk, 1, 4, 256, 2, 2, 128, 1, 1, 4, 256, None, 0, cnt])])
     assert plan() == 0 and list(cnt)[:3] == [40, 2, 6] and cnt[4] == 2 and cnt[7] == 4 and cnt[8] == 12
-    assert plan(a8=8) == -2
-    assert plan(a3=100) == -2 and plan(a8=3) == -2 and plan(a5=96) == -3 and plan(a0=None) == -1
-    assert plan(a12=None) == -1
-    assert plan(a10=blk, a11=4) == -4 and plan(a1=0) == 0 and cnt[3] == cnt[8] == 0
+    assert plan(a9=0) == 0 and cnt[7] == 1 and plan(a9=0, a4=300) == 0 and cnt[7] == 4     # 2 x 2 x 5 tiles; 600 x 5
+    assert plan(a9=8) == -2 and plan(a4=0) == -2 and plan(a8=0) == 0 and cnt[7] == 1
+    assert plan(a3=100) == -2 and plan(a9=3) == -2 and plan(a6=96) == -3 and plan(a0=None) == -1
+    assert plan(a13=None) == -1
+    assert plan(a11=blk, a12=4) == -4 and plan(a1=0) == 0 and cnt[3] == cnt[8] == 0
     blk[1] = 64 * 128
     assert plan(a3=64) == -2                                                         # more than 128 splits
     blk[1] = -1

@@ -78,7 +78,7 @@ _SIGS = {
                                 ctypes.c_double, ctypes.c_double, _P]),
     "lsk_kv8_append": (_I, [_I, _P, _P, _L, _L] + [_P] * 6 + [_I] * 5 + [_P]),
     "lsk_kv8_read": (_I, [_I] + [_P] * 8 + [_I] * 5 + [_P]),
-    "lsk_cache_attn_plan": (_I, [_P] + [_I] * 9 + [_P, _L, _P]),
+    "lsk_cache_attn_plan": (_I, [_P] + [_I] * 10 + [_P, _L, _P]),
     "lsk_cache_attn_workspace_bytes": (_Z, [_I, _I, _I, _I]),
     "lsk_kv8_attn": (_I, [_P, _L, _L] + [_P] * 5 + [_I, _P, _I, _I, _P] + [_I] * 6 + [_P] + [_I] * 4 + [_F, _P, _Z,
                           _P]),
@@ -667,13 +667,6 @@ def cache_attn_split(max_batch: int, n_kv_heads: int, max_seq: int) -> int:
     return (max(split, -(-max_seq // 128)) + 63) // 64 * 64
 
 
-def cache_attn_row_groups(max_batch: int, n_kv_heads: int) -> int:
-    """Row groups of a tree's work items at most (lsk_cache_attn_plan), fixed by the cache as the split is: caches of
-    few stripes keep the rows on as many CUs as there are."""
-    stripes = max_batch * n_kv_heads
-    return 4 if stripes >= 128 else 2 if stripes >= 64 else 1
-
-
 class _Launch:
     """One lsk_cache_attn_plan on the device, and its arguments of a launch."""
 
@@ -690,8 +683,8 @@ class _Launch:
 class AttnPlan:
     """The plan of attention launches over packed blocks, shared by the layers of a segment.  blocks: int [nb, 4] =
     (q_start, pos0, T, row) with q_start the running sum of T; cache: a layer's KV8, or the K storage of a bf16 or fp32
-    cache.  split: KV positions per split (cache_attn_split unless given; fp32 does not split); row_groups:
-    cache_attn_row_groups unless given.  tree: which launches it is for, with a mask (True), without (False) or, over an
+    cache.  split: KV positions per split (cache_attn_split unless given; fp32 does not split); row_groups: a
+    tree's at most (by the cache and the block unless given).  tree: which launches it is for, with a mask (True), without (False) or, over an
     8-bit cache, either (None)."""
 
     def __init__(self, blocks, n_heads: int, cache, split: int | None = None, row_groups: int | None = None,
@@ -722,19 +715,20 @@ class AttnPlan:
             self.works, self.n_works = self._upload(works.ravel()), len(works)
             return
         self.split = cache_attn_split(B, Hkv, S) if split is None else split
-        rg = cache_attn_row_groups(B, Hkv) if row_groups is None else row_groups
+        rg = 0 if row_groups is None else row_groups
         if self.kv8 and not tree:
-            self.causal = self._plan(b, group, Hkv, D, False, 1, n_slots)
+            self.causal = self._plan(b, group, B, Hkv, D, False, 1, n_slots)
         if tree or tree is None:
-            self.tree = self._plan(b, group, Hkv, D, True, rg, n_slots)
+            self.tree = self._plan(b, group, B, Hkv, D, True, rg, n_slots)
 
     def _upload(self, words: np.ndarray) -> torch.Tensor:
         t = torch.from_numpy(words)
         return t.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else t
 
-    def _plan(self, b: np.ndarray, group: int, Hkv: int, D: int, tree: bool, row_groups: int, n_slots: int) -> _Launch:
+    def _plan(self, b: np.ndarray, group: int, B: int, Hkv: int, D: int, tree: bool, row_groups: int,
+              n_slots: int) -> _Launch:
         lib, cnt = load(), np.zeros(9, dtype=np.int64)
-        args = (b.ctypes.data if len(b) else None, len(b), group, self.split, Hkv, D, int(self.kv8), int(tree),
+        args = (b.ctypes.data if len(b) else None, len(b), group, self.split, B, Hkv, D, int(self.kv8), int(tree),
                 row_groups, n_slots)
         _check(lib.lsk_cache_attn_plan(*args, None, 0, cnt.ctypes.data), "lsk_cache_attn_plan")
         meta = np.zeros(max(int(cnt[6]), 1), dtype=np.int32)
