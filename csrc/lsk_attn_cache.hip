@@ -29,6 +29,7 @@
 // order of additions depend on absolute positions only: a row's result never depends on what else is in the launch.  An
 // fp32 chain (every ancestor's bit set) gives the ragged attention's bits.
 #include <algorithm>
+#include <exception>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -933,13 +934,12 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 //           46 / 60 / 69).
 // The number of row groups follows from the block's rows and the cache alone, so it never makes a row's result depend
 // on the batch.  Items go longest first to the least-loaded of n_slots persistent workgroups, as in lsk_attn_schedule.
-extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int max_batch, int n_kv_heads,
-                                   int head_dim, int kv8, int tree, int row_groups, int n_slots, int32_t* meta,
-                                   long meta_cap, long* counts) {
-  const char* what = "lsk_cache_attn_plan";
+static int cache_plan(const char* what, const int32_t* blocks, int nb, int group, int split, int max_batch,
+                      int n_kv_heads, int head_dim, int kv8, int tree, int row_groups, int n_slots, int32_t* meta,
+                      long meta_cap, long* counts) {
   LSK_REQUIRE(counts && (blocks || nb == 0), LSK_EARG, "%s: null pointer", what);
   LSK_REQUIRE(nb >= 0 && group > 0 && split >= ATTN_TILE && split % ATTN_TILE == 0 && n_kv_heads > 0 &&
-                  n_kv_heads < (1 << 19) && max_batch > 0 && n_slots > 0 &&
+                  n_kv_heads < (1 << 19) && max_batch > 0 && n_slots > 0 && n_slots <= (1 << 16) &&
                   (row_groups == 0 || row_groups == 1 || row_groups == 2 || row_groups == 4),
               LSK_ESHAPE, "%s: bad arguments (split a multiple of %d, row_groups 0, 1, 2 or 4)", what, ATTN_TILE);
   LSK_REQUIRE(head_dim == 64 || head_dim == 128, LSK_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128)", what,
@@ -982,6 +982,8 @@ extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int
         groups.insert(groups.end(), g, g + 8);
         part_rows = cap > part_rows ? cap : part_rows;
       }
+      LSK_REQUIRE((long)(items.size() + shared.size()) + (long)ns * n_kv_heads < (1L << 24), LSK_ESHAPE,
+                  "%s: too many work items", what);
       for (int sp = 0; sp < ns; ++sp) {
         const int lo = sp * split, hi = lo + split < end ? lo + split : end;
         // in tenths of a one-tile step: a wave's steps, 1.5 times as long per further tile, and the item's own cost
@@ -994,8 +996,6 @@ extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int
       if (ns > 1) np += ns;
     }
   }
-  LSK_REQUIRE(np < (1L << 24) && (long)(items.size() + shared.size()) < (1L << 28), LSK_ESHAPE,
-              "%s: too many work items", what);
   const auto longer = [](const It& a, const It& b) { return a.cost > b.cost; };
   std::stable_sort(items.begin(), items.end(), longer);
   std::stable_sort(shared.begin(), shared.end(), longer);
@@ -1030,6 +1030,18 @@ extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int
   for (size_t i = 0; i < shared.size(); ++i)
     std::copy(shared[i].rec, shared[i].rec + 8, recs + ((long)n_slots * rounds + (long)i) * 8);
   return 0;
+}
+
+extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int max_batch, int n_kv_heads,
+                                   int head_dim, int kv8, int tree, int row_groups, int n_slots, int32_t* meta,
+                                   long meta_cap, long* counts) {
+  const char* what = "lsk_cache_attn_plan";
+  try {
+    return cache_plan(what, blocks, nb, group, split, max_batch, n_kv_heads, head_dim, kv8, tree, row_groups, n_slots,
+                      meta, meta_cap, counts);
+  } catch (const std::exception&) {
+    LSK_REQUIRE(false, LSK_EWORKSPACE, "%s: out of host memory", what);
+  }
 }
 
 extern "C" size_t lsk_cache_attn_workspace_bytes(int n_parts, int n_kv_heads, int part_rows, int head_dim) {

@@ -1021,6 +1021,9 @@ def test_entry_points_refuse_bad_arguments():
     assert plan(a3=100) == -2 and plan(a9=3) == -2 and plan(a6=96) == -3 and plan(a0=None) == -1
     assert plan(a13=None) == -1
     assert plan(a11=blk, a12=4) == -4 and plan(a1=0) == 0 and cnt[3] == cnt[8] == 0
+    blk[2] = 1 << 20
+    assert plan(a5=1 << 18) == -2 and plan(a10=1 << 30) == -2                        # more items than a plan holds
+    blk[2] = 40
     blk[1] = 64 * 128
     assert plan(a3=64) == -2                                                         # more than 128 splits
     blk[1] = -1
