@@ -304,6 +304,8 @@ int lsk_kv8_read(int dtype, const void* k8, const void* v8, const void* k_exp, c
  * mask (uint32 [n_tokens][mask_words]), of the block's own slots only those whose bit is set: bit j % 32 of word j / 32
  * for node j; bits of later nodes and bits past the words count as 0.  A row that reads nothing gives zeros.  Values in
  * slots that a row does not read never reach it, whatever they are.
+ * Weights are relative to a running maximum that may lag by 2^8 and are summed in fp32 before the division: 2^8 |V|
+ * times the positions read has to stay below 2^128.
  * groups .. part_rows: lsk_cache_attn_plan's (fp32 trees: works, n_works, rows_cap of an unsplit lsk_attn_plan).
  * workspace >= lsk_cache_attn_workspace_bytes(n_parts, n_kv_heads, part_rows, head_dim), 16-byte aligned, and a call's
  * own (one that two captured graphs share is written by both).  head_dim 64 or 128 (fp32 also 16 and 32); scale not
