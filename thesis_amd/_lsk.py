@@ -659,11 +659,20 @@ def kv8_read(cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor, dtype: t
     return out
 
 
-def cache_attn_split(max_batch: int, n_kv_heads: int, max_seq: int) -> int:
+def cache_attn_split(max_batch: int, n_kv_heads: int, max_seq: int, tree: bool = False) -> int:
     """KV positions per attention split of a cache: fixed by the cache, so that a row's result never depends on the
-    batch it is in.  About as many splits of the longest context as make one work item per CU out of the cache's
-    (row, KV head) stripes; 512 to 8192 positions, at most 128 splits."""
-    split = min(max(max_seq * max_batch * n_kv_heads // 256, 512), ATTN_SPLIT)
+    batch it is in.  The longest context in as many splits as make about one work item per CU out of the cache's
+    (row, KV head) stripes, but each long enough to pay for the merge: 800 positions, 2048 from 128 stripes on (32 / 8
+    heads of 64, one token, 1 request: 1000 positions 7.2 us whole, 11.0 in two; 5000 positions 15.8 whole, 10.8 in
+    five).  Trees, whose partial outputs are many rows: a quarter of the items, 1280 positions, 2048 from 32 stripes on
+    (64 nodes, 32 / 8 heads of 128, 1000 positions, 4 requests: 14 us whole, 32 in two; 1 request of 5000 positions 33
+    whole, 23 in three).  512 to 8192 positions, at most 128 splits."""
+    stripes = max_batch * n_kv_heads
+    if tree:
+        n = min(64 // stripes, max_seq // (1280 if stripes < 32 else 2048))
+    else:
+        n = min(256 // stripes, max_seq // (800 if stripes < 128 else 2048))
+    split = min(max(-(-max_seq // max(n, 1)), 512), ATTN_SPLIT)
     return (max(split, -(-max_seq // 128)) + 63) // 64 * 64
 
 
@@ -683,9 +692,9 @@ class _Launch:
 class AttnPlan:
     """The plan of attention launches over packed blocks, shared by the layers of a segment.  blocks: int [nb, 4] =
     (q_start, pos0, T, row) with q_start the running sum of T; cache: a layer's KV8, or the K storage of a bf16 or fp32
-    cache.  split: KV positions per split (cache_attn_split unless given; fp32 does not split); row_groups: a
-    tree's at most (by the cache and the block unless given).  tree: which launches it is for, with a mask (True), without (False) or, over an
-    8-bit cache, either (None)."""
+    cache.  split: KV positions per split (cache_attn_split unless given; fp32 does not split); row_groups: a tree's at
+    most (by the cache and the block unless given).  tree: which launches it is for, with a mask (True), without (False)
+    or, over an 8-bit cache, either (None)."""
 
     def __init__(self, blocks, n_heads: int, cache, split: int | None = None, row_groups: int | None = None,
                  tree: bool | None = None):
@@ -714,22 +723,22 @@ class AttnPlan:
             works, _, _ = attn_plan(b, group, self.split, self.rows_cap)
             self.works, self.n_works = self._upload(works.ravel()), len(works)
             return
-        self.split = cache_attn_split(B, Hkv, S) if split is None else split
+        self.split, self.tree_split = (cache_attn_split(B, Hkv, S, t) if split is None else split for t in (False, True))
         rg = 0 if row_groups is None else row_groups
         if self.kv8 and not tree:
-            self.causal = self._plan(b, group, B, Hkv, D, False, 1, n_slots)
+            self.causal = self._plan(b, group, self.split, False, 1, n_slots)
         if tree or tree is None:
-            self.tree = self._plan(b, group, B, Hkv, D, True, rg, n_slots)
+            self.tree = self._plan(b, group, self.tree_split, True, rg, n_slots)
 
     def _upload(self, words: np.ndarray) -> torch.Tensor:
         t = torch.from_numpy(words)
         return t.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else t
 
-    def _plan(self, b: np.ndarray, group: int, B: int, Hkv: int, D: int, tree: bool, row_groups: int,
-              n_slots: int) -> _Launch:
+    def _plan(self, b: np.ndarray, group: int, split: int, tree: bool, row_groups: int, n_slots: int) -> _Launch:
         lib, cnt = load(), np.zeros(9, dtype=np.int64)
-        args = (b.ctypes.data if len(b) else None, len(b), group, self.split, B, Hkv, D, int(self.kv8), int(tree),
-                row_groups, n_slots)
+        B, Hkv, _, D = self.dims
+        args = (b.ctypes.data if len(b) else None, len(b), group, split, B, Hkv, D, int(self.kv8), int(tree), row_groups,
+                n_slots)
         _check(lib.lsk_cache_attn_plan(*args, None, 0, cnt.ctypes.data), "lsk_cache_attn_plan")
         meta = np.zeros(max(int(cnt[6]), 1), dtype=np.int32)
         _check(lib.lsk_cache_attn_plan(*args, meta.ctypes.data, meta.size, cnt.ctypes.data), "lsk_cache_attn_plan")
