@@ -738,61 +738,81 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
 }
 
 // Merge the splits of a row in split order: M = max_s m_s, w_s = exp2(m_s - M), out = sum w_s O_s / sum w_s l_s (zeros
-// where no split read anything).  A wave per row: the lanes take the splits' statistics side by side, then each its
-// dims of the partial outputs, 16 splits' loads in flight.  (One workgroup per group of rows with a split after the
-// other: 25 us more for 5 tokens over 100000 positions in 98 splits.)
+// where no split read anything).  16 lanes per row: they take the splits' statistics side by side, then each D / 16 dims
+// of the partial outputs, AHEAD splits' loads in flight, the first ones beside the statistics'.  (A wave per row with
+// the loads behind the statistics: 32 trees of 64 nodes in three splits 57 us, now 20.)
+#define COMBINE_ROWS 16
 template <int D>
 __global__ __launch_bounds__(256) void cache_combine_kernel(const int32_t* __restrict__ groups,
                                                             const float* __restrict__ o_part,
                                                             const float* __restrict__ ml_part,
                                                             uint16_t* __restrict__ out, int G, int Hkv, int part_rows) {
-  constexpr int PER = D / 64, AHEAD = 16;
-  __shared__ float s_w[4][ATTN_MAX_SPLITS], s_l[4][ATTN_MAX_SPLITS];
+  constexpr int PER = D / 16, AHEAD = D == 64 ? 16 : 8, MS = ATTN_MAX_SPLITS / 16;
   const int32_t* gp = groups + (long)blockIdx.x * 8;
   const int q_start = gp[0], row0 = gp[1], nrows = gp[2], pf = gp[3], ns = gp[4];
-  const int kvh = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int rl = blockIdx.z * 4 + wave;
-  if (rl >= nrows) return;                           // (no barrier below: a wave's LDS is its own)
+  const int kvh = blockIdx.y, l16 = threadIdx.x & 15;
+  const int rl = blockIdx.z * COMBINE_ROWS + (threadIdx.x >> 4);
+  if (rl >= nrows) return;                           // (no barrier: a row's lanes are its own)
   const long slot0 = ((long)pf * Hkv + kvh) * part_rows + rl, step = (long)Hkv * part_rows;
-  float m[2], M = -INFINITY;
+  float m[MS], l[MS], w[MS], M = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int s = lane + 64 * i;
-    m[i] = s < ns ? ml_part[(slot0 + s * step) * 2] : -INFINITY;
-    M = fmaxf(M, m[i]);
-    if (s < ns) s_l[wave][s] = ml_part[(slot0 + s * step) * 2 + 1];
+  for (int i = 0; i < MS; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+    if (16 * i < ns && l16 + 16 * i < ns) {
+      const float* p = ml_part + (slot0 + (l16 + 16 * i) * step) * 2;
+      m[i] = p[0];
+      l[i] = p[1];
+    }
   }
+  lsk_f32x4 v[AHEAD][PER / 4];
+  auto fetch = [&](int s0) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    for (int j = 0; j < AHEAD; ++j)
+      if (s0 + j < ns)
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (lane + 64 * i < ns)
-      s_w[wave][lane + 64 * i] = (m[i] == -INFINITY) ? 0.f : ((m[i] == M) ? 1.f : fast_exp2(m[i] - M));
-  __builtin_amdgcn_wave_barrier();
+        for (int i = 0; i < PER / 4; ++i)
+          v[j][i] = *(const lsk_f32x4*)(o_part + (slot0 + (s0 + j) * step) * D + l16 * PER + 4 * i);
+  };
+  fetch(0);
+#pragma unroll
+  for (int i = 0; i < MS; ++i) M = fmaxf(M, m[i]);
+#define COMBINE_ROR(N) \
+  M = fmaxf(M, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(M), 0x120 + N, 0xf, 0xf, false)))
+  COMBINE_ROR(8); COMBINE_ROR(4); COMBINE_ROR(2); COMBINE_ROR(1);
+#undef COMBINE_ROR
+#pragma unroll
+  for (int i = 0; i < MS; ++i) w[i] = m[i] == -INFINITY ? 0.f : m[i] == M ? 1.f : fast_exp2(m[i] - M);
   float L = 0.f, O[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) O[i] = 0.f;
-  for (int s0 = 0; s0 < ns; s0 += AHEAD) {
-    float v[AHEAD][PER];
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        v[j][i] = s0 + j < ns ? o_part[(slot0 + (s0 + j) * step) * D + lane * PER + i] : 0.f;
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-      if (s0 + j < ns) {
-        const float w = s_w[wave][s0 + j];
-        L = L + w * s_l[wave][s0 + j];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) O[i] = O[i] + w * v[j][i];
-      }
+  for (int i = 0; i < MS; ++i) {
+    if (16 * i >= ns) break;
+    // lane j of the row to all of them
+#define COMBINE_STEP(J)                                                                                             \
+  if (16 * i + J < ns) {                                                                                            \
+    const float wj = __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(w[i]), 0x150 + J, 0xf, 0xf, false));  \
+    const float lj = __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(l[i]), 0x150 + J, 0xf, 0xf, false));  \
+    L = L + wj * lj;                                                                                                \
+    _Pragma("unroll") for (int d = 0; d < PER; ++d) O[d] = O[d] + wj * v[J % AHEAD][d / 4][d % 4];                  \
+    if (J % AHEAD == AHEAD - 1) fetch(16 * i + J + 1);                                                              \
+  }
+    COMBINE_STEP(0) COMBINE_STEP(1) COMBINE_STEP(2) COMBINE_STEP(3) COMBINE_STEP(4) COMBINE_STEP(5) COMBINE_STEP(6)
+    COMBINE_STEP(7) COMBINE_STEP(8) COMBINE_STEP(9) COMBINE_STEP(10) COMBINE_STEP(11) COMBINE_STEP(12)
+    COMBINE_STEP(13) COMBINE_STEP(14) COMBINE_STEP(15)
+#undef COMBINE_STEP
   }
   if (L == 0.f) L = 1.f;
   const int r = row0 + rl, t = r / G, g = r - t * G;
-  uint16_t* o = out + ((long)(q_start + t) * G * Hkv + kvh * G + g) * D + lane * PER;
+  uint16_t* o = out + ((long)(q_start + t) * G * Hkv + kvh * G + g) * D + l16 * PER;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) o[i] = f2bf(O[i] / L);
+  for (int i = 0; i < PER; i += 4) {
+    lsk_u32x2_u pk;
+    pk[0] = (uint32_t)f2bf(O[i] / L) | ((uint32_t)f2bf(O[i + 1] / L) << 16);
+    pk[1] = (uint32_t)f2bf(O[i + 2] / L) | ((uint32_t)f2bf(O[i + 3] / L) << 16);
+    *(lsk_u32x2_u*)(o + i) = pk;
+  }
 }
 
 // ----------------------------------------------------------------------------- fp32 trees
@@ -1107,7 +1127,7 @@ static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t
     if ((rc = lsk_check_launch(what))) return rc;
   }
   if (n_groups == 0) return 0;
-  const dim3 cg(n_groups, a.Hkv, (a.part_rows + 3) / 4);
+  const dim3 cg(n_groups, a.Hkv, (a.part_rows + COMBINE_ROWS - 1) / COMBINE_ROWS);
   if (head_dim == 128)
     cache_combine_kernel<128><<<cg, 256, 0, s>>>(groups, a.o_part, a.ml_part, a.out, a.G, a.Hkv, a.part_rows);
   else

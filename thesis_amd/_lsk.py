@@ -664,12 +664,12 @@ def cache_attn_split(max_batch: int, n_kv_heads: int, max_seq: int, tree: bool =
     batch it is in.  The longest context in as many splits as make about one work item per CU out of the cache's
     (row, KV head) stripes, but each long enough to pay for the merge: 800 positions, 2048 from 128 stripes on (32 / 8
     heads of 64, one token, 1 request: 1000 positions 7.2 us whole, 11.0 in two; 5000 positions 15.8 whole, 10.8 in
-    five).  Trees, whose partial outputs are many rows: a quarter of the items, 1280 positions, 2048 from 32 stripes on
-    (64 nodes, 32 / 8 heads of 128, 1000 positions, 4 requests: 14 us whole, 32 in two; 1 request of 5000 positions 33
-    whole, 23 in three).  512 to 8192 positions, at most 128 splits."""
+    five).  Trees, whose partial outputs are many rows: 1280 positions, 2048 from 32 stripes on (64 nodes, 32 / 8 heads
+    of 128: 4 requests of 1000 positions 14 us whole, 28 in two, of 5000 positions 37 and 42 in three; 1 request of 5000
+    positions 33 whole, 21 in three).  512 to 8192 positions, at most 128 splits."""
     stripes = max_batch * n_kv_heads
     if tree:
-        n = min(64 // stripes, max_seq // (1280 if stripes < 32 else 2048))
+        n = min(256 // stripes, max_seq // (1280 if stripes < 32 else 2048))
     else:
         n = min(256 // stripes, max_seq // (800 if stripes < 128 else 2048))
     split = min(max(-(-max_seq // max(n, 1)), 512), ATTN_SPLIT)
