@@ -326,6 +326,26 @@ def test_kv8_attention_matches_64_bits(cuda, heads, blocks, split):
     assert_close_bf16(got, ref, mag)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("split", [64, 128, 512])
+def test_attention_merges_up_to_128_splits(cuda, D, split):
+    """A long context in as many splits as a plan takes (and one that ends with the last of them), beside short ones."""
+    lsk = _lsk()
+    Hq, Hkv = 4, 1
+    blocks = [(0, 8187, 5), (1, 8000, 1), (2, 1020, 9), (3, 63, 2)]
+    tab, q, k, v = _attn_inputs(61, (Hq, Hkv, D), blocks, S=8192)
+    ref, mag, _ = attention(q.double(), held(k), held(v), tab, 1 / math.sqrt(D))
+    cache = kv8_from(lsk, cuda, k, v)
+    plan = lsk.AttnPlan(tab, Hq, cache, split=split)
+    assert plan.causal.n_parts >= 8192 // split
+    assert_close_bf16(lsk.kv8_attn(q.to(cuda), cache, plan), ref, mag)
+    mask = torch.from_numpy(words_of([set(range(i + 1)) for (_, _, t, _) in tab for i in range(t)], 1)).to(cuda)
+    ref, mag, _ = attention(q.double(), k.double(), v.double(), tab, 1 / math.sqrt(D))
+    kf, vf = lsk.k_to_frag(k).to(cuda), lsk.v_to_blocked(v).to(cuda)
+    assert_close_bf16(lsk.tree_attn(q.to(cuda), kf, vf, lsk.AttnPlan(tab, Hq, kf, split=split), mask), ref, mag)
+
+
 def _tree_blocks(blocks, seed):
     rng = np.random.default_rng(seed)
     parents = [random_tree(rng, t) if t else [] for (_, _, t) in blocks]
@@ -1159,7 +1179,9 @@ def test_wrappers_refuse_what_does_not_fit(cuda):
              lambda: lsk.tree_attn(q, kf, vf, pt, m.cpu()),
              lambda: lsk.kv_compact(kf, vf, i[:1], i[:1], a, m[:1]),
              lambda: lsk.kv_compact(kf[None], vf[None], i[:1], i[:1], a[:0], m[:1]),
-             lambda: lsk.kv8_compact(cache, i[:1], i[:1], a, m[:1]),
+             lambda: lsk.kv8_compact(cache, i[:1], i[:1], a, m[:1]), lambda: lsk.kv8_read(cache, i, i, out=(x,)),
+             lambda: lsk.kv8_attn(q, cache, plan, workspace=torch.zeros(8, 2, device=cuda)[:, 0]),
+             lambda: lsk.kv8_attn(q, cache, plan, scale=-1.0),
              lambda: lsk.tree_accept(a, a, i, i[:1], i[:1], 1)]
     for f in calls:
         with pytest.raises(lsk.LskError):

@@ -651,6 +651,8 @@ def kv8_read(cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor, dtype: t
     if out is None:
         out = cache.ks.new_empty(n, Hkv, D, dtype=dtype), cache.ks.new_empty(n, Hkv, D, dtype=dtype)
     else:
+        if len(out) != 2:
+            raise LskError("kv8_read: out is a pair of tensors")
         for t in out:
             _want("kv8_read", "out", t, out[0].dtype, (n, Hkv, D))
     if n:
