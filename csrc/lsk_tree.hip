@@ -232,14 +232,15 @@ __global__ __launch_bounds__(COMPACT_THREADS) void kv_compact_kernel(
       ek = ks[stripe + s_from[tid]];
       ev = vs[stripe + s_from[tid]];
     }
-    auto fetch = [&](uint32_t* v, int blk, uint32_t need) {
-      if (need == 0) return;
-      Piece x[NP];
+    // the pieces `need` of block blk: asked for, and put into LDS
+    auto fetch = [&](Piece (&x)[NP], int blk, uint32_t need) {
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const int d = pr + i * PROWS;
         if (d < D && (need >> pc & 1u)) x[i] = *(const Piece*)(vc + (long)blk * B * D + d * B + pc * PS);
       }
+    };
+    auto put = [&](uint32_t* v, const Piece (&x)[NP], uint32_t need) {
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const int d = pr + i * PROWS;
@@ -258,9 +259,14 @@ __global__ __launch_bounds__(COMPACT_THREADS) void kv_compact_kernel(
         if (from >= 0 && from / B == blk) vx[i] = ((const T*)(s_v[buf] + vd * LD))[from % B];
       }
     };
-    fetch(s_v[0], db, bits & 255u);
-    fetch(s_v[1], db + 1, bits >> 8 & 255u);
-    if (other != none) fetch(s_v[2], other, pieces_of(other));
+    Piece x0[NP], x1[NP], x2[NP];
+    uint32_t need = pieces_of(other);                // (0: there is none)
+    fetch(x0, db, bits & 255u);
+    fetch(x1, db + 1, bits >> 8 & 255u);
+    fetch(x2, other, need);
+    put(s_v[0], x0, bits & 255u);
+    put(s_v[1], x1, bits >> 8 & 255u);
+    put(s_v[2], x2, need);
     __syncthreads();
     take(0, db);
     take(1, db + 1);
@@ -268,8 +274,10 @@ __global__ __launch_bounds__(COMPACT_THREADS) void kv_compact_kernel(
       take(2, other);
       other = __builtin_amdgcn_readfirstlane(row_reduce(from / B > other ? from / B : none, least));
       if (other == none) break;
+      need = pieces_of(other);
+      fetch(x2, other, need);
       __syncthreads();
-      fetch(s_v[2], other, pieces_of(other));
+      put(s_v[2], x2, need);
       __syncthreads();
     }
     __syncthreads();                                 // (every source is in registers)
