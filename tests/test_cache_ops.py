@@ -862,6 +862,30 @@ def test_compaction_of_long_paths_from_far_nodes(cuda, fmt, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("L", [33, 65])
+@pytest.mark.parametrize("fmt,D", [("bf16", 64), ("fp32", 16)])
+def test_compaction_of_many_layers(cuda, fmt, D, L):
+    """Every layer of a large batch, each with its own slots moved."""
+    lsk = _lsk()
+    B, H, S = 16, 8, 96
+    dt = F32 if fmt == "fp32" else BF16
+    g, rng = _gen(L), np.random.default_rng(L)
+    k, v = (torch.randn(L, B, H, S, D, generator=g).to(dt) for _ in range(2))
+    kc, vc = (lsk.k_to_frag(k) if fmt == "bf16" else k).to(cuda), lsk.v_to_blocked(v).to(cuda)
+    pos0 = rng.integers(0, 40, B)
+    path = np.stack([np.concatenate([[0], np.sort(rng.choice(np.arange(1, 56), 20, replace=False))]) for _ in range(B)])
+    acc = rng.integers(0, 21, B)
+    rows = rng.permutation(B)
+    lsk.kv_compact(kc, vc, _i32(rows, cuda), _i32(pos0, cuda), torch.from_numpy(acc).to(cuda), _i32(path, cuda))
+    for i, r in enumerate(rows):
+        src = (pos0[i] + path[i, :acc[i] + 1]).tolist()
+        for x in (k, v):
+            x[:, r, :, pos0[i]:pos0[i] + len(src)] = x[:, r][:, :, src].clone()
+    assert torch.equal((lsk.k_from_frag(kc.cpu()) if fmt == "bf16" else kc.cpu()), k)
+    assert torch.equal(lsk.v_from_blocked(vc.cpu()), v)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["bf16", "kv8"])
 def test_a_tree_step_captured_in_two_graphs(cuda, fmt):
     """Masks, write, attention, acceptance and compaction as a captured step, replayed with new inputs between eager
