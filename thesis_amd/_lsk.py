@@ -598,19 +598,19 @@ class KV8(_KV8):
         if self._checked is not None and self._checked[0] == layers:
             return self._checked[1]
         k, v, ks, vs = self
-        lead, n = tuple(ks.shape), 4 if layers else 3
-        if len(lead) != n or v.dim() != n + 2:
+        lead, v_shape, n = ks.shape, v.shape, 4 if layers else 3
+        if len(lead) != n or len(v_shape) != n + 2:
             raise LskError(f"{what}: an 8-bit cache of {'several layers' if layers else 'one layer'} is needed")
-        S, D = lead[-1], v.shape[-2]
+        S, D = lead[-1], v_shape[-2]
         if D not in (64, 128) or S % 64 or S == 0:
             raise LskError(f"{what}: 8-bit caches need head_dim 64 or 128 and max_seq a multiple of 64 (got {D}, {S})")
         blocks = (*lead[:-1], S // 64)
-        k_shape, v_shape = (*blocks, 4, D // 64, 64, 16), (*blocks, D, 64)
-        if not (k.shape == k_shape and v.shape == v_shape and vs.shape == lead and k.dtype is v.dtype is _E4M3 and
+        want_k, want_v = (*blocks, 4, D // 64, 64, 16), (*blocks, D, 64)
+        if not (k.shape == want_k and v_shape == want_v and vs.shape == lead and k.dtype is v.dtype is _E4M3 and
                 ks.dtype is vs.dtype is torch.uint8 and k.is_contiguous() and v.is_contiguous() and
                 ks.is_contiguous() and vs.is_contiguous()):
-            _want(what, "k codes", k, _E4M3, k_shape)
-            _want(what, "v codes", v, _E4M3, v_shape)
+            _want(what, "k codes", k, _E4M3, want_k)
+            _want(what, "v codes", v, _E4M3, want_v)
             _want(what, "k exponents", ks, torch.uint8, lead)
             _want(what, "v exponents", vs, torch.uint8, lead)
         self._checked = layers, (lead[-3], lead[-2], S, D)
