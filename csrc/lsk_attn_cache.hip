@@ -69,6 +69,13 @@ __device__ __forceinline__ uint32_t mask_window(const uint32_t* words, int W, in
   return bits;
 }
 
+// Whether token t of a block reads a slot at all: one before the block, or a node whose bit is set.
+__device__ __forceinline__ bool reads_any(const uint32_t* words, int W, int t, int pos0) {
+  uint32_t any = pos0 > 0 ? 1u : 0u;
+  for (int w = 0; w < W && 32 * w <= t; ++w) any |= words[w] & (t - 32 * w >= 31 ? ~0u : (2u << (t - 32 * w)) - 1u);
+  return any != 0u;
+}
+
 // 8 e4m3 codes -> bf16, times a power of two (exact)
 __device__ __forceinline__ lsk_bf16x8 codes_to_bf16(uint32_t x, uint32_t y, float scale) {
   typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
@@ -931,7 +938,7 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
     __builtin_amdgcn_wave_barrier();
   }
   if (!active) return;
-  if (l_run == 0.f) l_run = 1.f;
+  if (l_run == 0.f && !reads_any(words, W, t, pos0)) l_run = 1.f;
   float* orow = out + ((long)(q_start + t) * Hkv * G + kvh * G + g) * D;
 #pragma unroll
   for (int i = 0; i < DPL; ++i) {

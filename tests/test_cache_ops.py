@@ -522,6 +522,35 @@ def test_bad_values_in_trees_of_many_rows_stay_with_their_readers(cuda, kind, ba
     assert torch.equal(got[~reads], clean[~reads]) and torch.isnan(got[reads]).all()
 
 
+def _minus_infinity(kind, q, k, at):
+    """Makes the scores of the slots at [(row, slice)] -infinity: one dim of K, against queries of a fixed sign there.
+    An 8-bit cache holds no infinity: there q . k overflows fp32."""
+    q[..., 3] = 1000.0 if kind.startswith("kv8") else q[..., 3].abs() + 0.5
+    k[..., 3] = 0.0                                                   # (elsewhere the dim adds nothing)
+    for row, slots in at:
+        if kind.startswith("kv8"):
+            k[row, :, slots] = 0.0
+        k[row, :, slots, 3] = -3e38 if kind.startswith("kv8") else -math.inf
+
+
+@pytest.mark.gpu
+def test_an_fp32_chain_of_minus_infinity_is_the_ragged_attentions(cuda):
+    lsk = _lsk()
+    Hq, Hkv, D = 8, 2, 64
+    tab, q, k, v = _attn_inputs(79, (Hq, Hkv, D), [(0, 0, 5), (1, 40, 2)], F32, S=128)
+    _minus_infinity("fp32", q, k, [(0, slice(0, 2)), (1, slice(0, 42))])
+    kd, vd = k.to(cuda), lsk.v_to_blocked(v).to(cuda)
+    mask = torch.from_numpy(words_of([set(range(i + 1)) for t in (5, 2) for i in range(t)], 1)).to(cuda)
+    p = lsk.AttnPlan(tab, Hq, kd)
+    want = torch.empty(len(q), Hq * D, device=cuda)
+    b = torch.tensor(tab, dtype=torch.int32, device=cuda)
+    lsk.ragged_attn(q.to(cuda), kd, vd, b, p.works, p.n_works, None, 0, 0, want, Hq, 1 / math.sqrt(D),
+                    rows_cap=p.rows_cap)
+    got = lsk.tree_attn(q.to(cuda), kd, vd, p, mask)
+    assert torch.isnan(want[[0, 1, 5, 6]]).all() and torch.isfinite(want[2:5]).all()
+    assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("D", [16, 64, 128])
 def test_an_fp32_chain_gives_the_ragged_attentions_bits(cuda, D):
