@@ -92,6 +92,9 @@ __device__ __forceinline__ float exp_bits(uint32_t byte) { return __uint_as_floa
 
 #define ORDER() __builtin_amdgcn_sched_barrier(0)  // (keeps the loads and conversions where their registers are free)
 #define LAG 8.0f
+// A row's running maximum before its first score: finite, so that a score of -infinity gets the weight 0 also where the
+// row has read no other (against a maximum of -infinity it would be exp2(NaN)); no finite score lies below it.
+#define M_NONE (-3.4028234663852886e38f)
 
 // K / V through buffer loads over an item's (row, KV head) stripe, whose range ends with the block that holds the
 // item's last position: loads past it give zeros without touching memory, so the next step's are unconditional (under
@@ -379,7 +382,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
     float m_run[QT], l_run[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      m_run[qt] = -INFINITY;
+      m_run[qt] = M_NONE;
       l_run[qt] = 0.f;
 #pragma unroll
       for (int c = 0; c < CT; ++c) oacc[qt][c] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
@@ -516,7 +519,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
           const int rg = x / MR, ql = x - rg * MR, qr = 16 * p0 + ql;  // row group, row of the pass, row of the group
           const int row = rg * GR + qr;                                // row of the item
           if (qr >= GR || row >= done.nrows) continue;
-          float M = -INFINITY;
+          float M = M_NONE;
 #pragma unroll
           for (int k = 0; k < RANKS; ++k) M = fmaxf(M, s_ml[k * NR + rg][0][qr]);
           float L = 0.f;
@@ -524,7 +527,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
 #pragma unroll
           for (int k = 0; k < RANKS; ++k) {
             const float mw = s_ml[k * NR + rg][0][qr];
-            const float ew = (mw == -INFINITY) ? 0.f : ((mw == M) ? 1.f : fast_exp2(mw - M));
+            const float ew = mw == M ? 1.f : fast_exp2(mw - M);
             L = L + ew * s_ml[k * NR + rg][1][qr];
             const float4 ow = *(const float4*)(&s_o[k * NR + rg][ql][d]);
             O.x = O.x + ew * ow.x;
@@ -535,7 +538,10 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
           const int rr = done.row0 + row;
           const int tt = rr / G, gg = rr - tt * G;
           if (done.part < 0) {
-            if (TREE && L == 0.f) L = 1.f;           // nothing read: O is 0
+            if constexpr (TREE) {                    // (0 / 0 stays where every score is -infinity)
+              const uint32_t* words = A.mask + (long)(done.q_start + tt) * A.W;
+              if (L == 0.f && !reads_any(words, A.W, tt, done.pos0)) L = 1.f;
+            }
             lsk_u32x2_u pk;
             pk[0] = (uint32_t)f2bf(O.x / L) | ((uint32_t)f2bf(O.y / L) << 16);
             pk[1] = (uint32_t)f2bf(O.z / L) | ((uint32_t)f2bf(O.w / L) << 16);
@@ -638,7 +644,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
   float m_run[QT], l_run[QT];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
-    m_run[qt] = -INFINITY;
+    m_run[qt] = M_NONE;
     l_run[qt] = 0.f;
 #pragma unroll
     for (int c = 0; c < CT; ++c) oacc[qt][c] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
@@ -722,7 +728,8 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
     const int rl = rb + 16 * qt + l16;
     if (rl >= nrows) continue;
     const int r = row0 + rl, t = r / G, g = r - t * G;
-    const float L = l_run[qt] == 0.f ? 1.f : l_run[qt];  // (nothing read: O is 0)
+    float L = l_run[qt];
+    if (L == 0.f && part < 0 && !reads_any(A.mask + (long)(q_start + t) * A.W, A.W, t, pos0)) L = 1.f;
     const long slot = ((long)part * Hkv + kvh) * A.part_rows + rl;
     uint16_t* o = A.out + ((long)(q_start + t) * G * Hkv + kvh * G + g) * D + 4 * lg;
 #pragma unroll
@@ -753,18 +760,19 @@ template <int D>
 __global__ __launch_bounds__(256) void cache_combine_kernel(const int32_t* __restrict__ groups,
                                                             const float* __restrict__ o_part,
                                                             const float* __restrict__ ml_part,
+                                                            const uint32_t* __restrict__ mask, int W,
                                                             uint16_t* __restrict__ out, int G, int Hkv, int part_rows) {
   constexpr int PER = D / 16, AHEAD = D == 64 ? 16 : 8, MS = ATTN_MAX_SPLITS / 16;
   const int32_t* gp = groups + (long)blockIdx.x * 8;
-  const int q_start = gp[0], row0 = gp[1], nrows = gp[2], pf = gp[3], ns = gp[4];
+  const int q_start = gp[0], row0 = gp[1], nrows = gp[2], pf = gp[3], ns = gp[4], pos0 = gp[5];
   const int kvh = blockIdx.y, l16 = threadIdx.x & 15;
   const int rl = blockIdx.z * COMBINE_ROWS + (threadIdx.x >> 4);
   if (rl >= nrows) return;                           // (no barrier: a row's lanes are its own)
   const long slot0 = ((long)pf * Hkv + kvh) * part_rows + rl, step = (long)Hkv * part_rows;
-  float m[MS], l[MS], w[MS], M = -INFINITY;
+  float m[MS], l[MS], w[MS], M = M_NONE;
 #pragma unroll
   for (int i = 0; i < MS; ++i) {
-    m[i] = -INFINITY;
+    m[i] = M_NONE;
     l[i] = 0.f;
     if (16 * i < ns && l16 + 16 * i < ns) {
       const float* p = ml_part + (slot0 + (l16 + 16 * i) * step) * 2;
@@ -789,7 +797,7 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(const int32_t* __res
   COMBINE_ROR(8); COMBINE_ROR(4); COMBINE_ROR(2); COMBINE_ROR(1);
 #undef COMBINE_ROR
 #pragma unroll
-  for (int i = 0; i < MS; ++i) w[i] = m[i] == -INFINITY ? 0.f : m[i] == M ? 1.f : fast_exp2(m[i] - M);
+  for (int i = 0; i < MS; ++i) w[i] = m[i] == M ? 1.f : fast_exp2(m[i] - M);
   float L = 0.f, O[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) O[i] = 0.f;
@@ -810,8 +818,8 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(const int32_t* __res
     COMBINE_STEP(13) COMBINE_STEP(14) COMBINE_STEP(15)
 #undef COMBINE_STEP
   }
-  if (L == 0.f) L = 1.f;
   const int r = row0 + rl, t = r / G, g = r - t * G;
+  if (L == 0.f && mask != nullptr && !reads_any(mask + (long)(q_start + t) * W, W, t, pos0)) L = 1.f;
   uint16_t* o = out + ((long)(q_start + t) * G * Hkv + kvh * G + g) * D + l16 * PER;
 #pragma unroll
   for (int i = 0; i < PER; i += 4) {
@@ -1005,7 +1013,7 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
       const int end = (int)(pos0 + (row0 + nrows - 1) / group + 1);
       const int ns = (end + split - 1) / split;
       if (ns > 1) {
-        const int32_t g[8] = {bm[0], (int32_t)row0, nrows, (int32_t)np, ns, 0, 0, 0};
+        const int32_t g[8] = {bm[0], (int32_t)row0, nrows, (int32_t)np, ns, pos0, 0, 0};
         groups.insert(groups.end(), g, g + 8);
         part_rows = cap > part_rows ? cap : part_rows;
       }
@@ -1136,9 +1144,10 @@ static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t
   if (n_groups == 0) return 0;
   const dim3 cg(n_groups, a.Hkv, (a.part_rows + COMBINE_ROWS - 1) / COMBINE_ROWS);
   if (head_dim == 128)
-    cache_combine_kernel<128><<<cg, 256, 0, s>>>(groups, a.o_part, a.ml_part, a.out, a.G, a.Hkv, a.part_rows);
+    cache_combine_kernel<128><<<cg, 256, 0, s>>>(groups, a.o_part, a.ml_part, a.mask, a.W, a.out, a.G, a.Hkv,
+                                                 a.part_rows);
   else
-    cache_combine_kernel<64><<<cg, 256, 0, s>>>(groups, a.o_part, a.ml_part, a.out, a.G, a.Hkv, a.part_rows);
+    cache_combine_kernel<64><<<cg, 256, 0, s>>>(groups, a.o_part, a.ml_part, a.mask, a.W, a.out, a.G, a.Hkv, a.part_rows);
   return lsk_check_launch(what);
 }
 

@@ -522,6 +522,26 @@ def test_bad_values_in_trees_of_many_rows_stay_with_their_readers(cuda, kind, ba
     assert torch.equal(got[~reads], clean[~reads]) and torch.isnan(got[reads]).all()
 
 
+def _run_kind(lsk, cuda, kind, q, k, v, tab, mask, split=None, row_groups=None):
+    """One attention launch of a kind (bf16, fp32: trees; kv8: a tree; kv8 causal: no mask) over dense k, v."""
+    Hq = q.shape[1]
+    if kind.startswith("kv8"):
+        cache = kv8_from(lsk, cuda, k, v)
+        plan = lsk.AttnPlan(tab, Hq, cache, split, row_groups)
+        return lsk.kv8_attn(q.to(cuda), cache, plan, mask if kind == "kv8" else None).cpu()
+    ks = (lsk.k_to_frag(k) if kind == "bf16" else k).to(cuda)
+    plan = lsk.AttnPlan(tab, Hq, ks, split, row_groups)
+    return lsk.tree_attn(q.to(cuda), ks, lsk.v_to_blocked(v).to(cuda), plan, mask).cpu()
+
+
+def _compare(kind, got, ref, mag, big, D, rows=slice(None)):
+    if kind == "fp32":
+        assert torch.equal(torch.isnan(got[rows]), torch.isnan(ref[rows]))
+        assert_close_f32(got[rows].nan_to_num(0), ref[rows].nan_to_num(0), mag[rows].nan_to_num(0), 1088, D, big)
+    else:
+        assert_close_bf16(got[rows], ref[rows], mag[rows])
+
+
 def _minus_infinity(kind, q, k, at):
     """Makes the scores of the slots at [(row, slice)] -infinity: one dim of K, against queries of a fixed sign there.
     An 8-bit cache holds no infinity: there q . k overflows fp32."""
@@ -531,6 +551,60 @@ def _minus_infinity(kind, q, k, at):
         if kind.startswith("kv8"):
             k[row, :, slots] = 0.0
         k[row, :, slots, 3] = -3e38 if kind.startswith("kv8") else -math.inf
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [None, 64])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kind", ["bf16", "kv8", "kv8 causal", "fp32"])
+def test_scores_of_minus_infinity_have_weight_zero(cuda, kind, D, split):
+    """Slots with a score of -infinity where a row reads no other slot of a wave's step, of its first step or of a
+    split: before the block, and as the block's first nodes."""
+    lsk = _lsk()
+    Hq, Hkv = 8, 2
+    dtype = F32 if kind == "fp32" else BF16
+    blocks = [(0, 32, 3), (1, 64, 3), (2, 128, 45), (3, 96, 7), (0, 200, 20)]
+    tab, q, k, v = _attn_inputs(71, (Hq, Hkv, D), blocks, dtype, S=256)
+    _minus_infinity(kind, q, k, [(0, slice(32, 33)), (1, slice(64, 65)), (2, slice(0, 64)), (3, slice(0, 96))])
+    # each node reads the root and itself
+    sets = [set(range(i + 1)) if kind == "kv8 causal" else {0, i} for (_, _, t) in blocks for i in range(t)]
+    mask = torch.from_numpy(words_of(sets, 2)).to(cuda)
+    got = _run_kind(lsk, cuda, kind, q, k, v, tab, mask, split, 4)
+    if kind.startswith("kv8"):
+        k, v = held(k), held(v)
+    ref, mag, big = attention(q.double(), k.double(), v.double(), tab, 1 / math.sqrt(D), sets)
+    assert torch.isfinite(ref).all()
+    _compare(kind, got, ref, mag, big, D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [None, 64])
+@pytest.mark.parametrize("row_groups", [1, 4])
+@pytest.mark.parametrize("kind", ["bf16", "kv8", "fp32"])
+def test_rows_of_minus_infinity_only_and_rows_that_read_nothing(cuda, kind, row_groups, split):
+    """A row that reads nothing gives zeros; one whose scores are all -infinity NaN, as the formula does (over an 8-bit
+    cache, where fp32 overflows: the same); nodes whose parent scores -infinity their own V."""
+    lsk = _lsk()
+    Hq, Hkv, D = 8, 2, 64
+    dtype = F32 if kind == "fp32" else BF16
+    blocks = [(0, 0, 100), (1, 0, 9), (2, 0, 70)]
+    tab, q, k, v = _attn_inputs(73, (Hq, Hkv, D), blocks, dtype, S=128)
+    sets = [{0, i} for (_, _, t) in blocks for i in range(t)]
+    _minus_infinity(kind, q, k, [(0, slice(0, 1)), (1, slice(0, 1)), (2, slice(0, 1))])
+    first = [a for (a, _, _, _) in tab]
+    nothing = [first[0] + 5, first[0] + 99, first[1] + 8, first[2] + 66]
+    for i in nothing:
+        sets[i] = set()
+    mask = torch.from_numpy(words_of(sets, 4)).to(cuda)
+    mask[first[2] + 66, 2] = 1 << 3                                   # (a later node's bit does not count)
+    got = _run_kind(lsk, cuda, kind, q, k, v, tab, mask, split, row_groups)
+    assert (got[nothing] == 0).all() and torch.isnan(got[first]).all()
+    if kind.startswith("kv8"):
+        k, v = held(k), held(v)
+    ref, mag, big = attention(q.double(), k.double(), v.double(), tab, 1 / math.sqrt(D), sets)
+    rest = [i for i in range(len(q)) if i not in first]
+    assert torch.isfinite(ref[rest]).all()
+    _compare(kind, got, ref, mag, big, D, rest)
 
 
 @pytest.mark.gpu
