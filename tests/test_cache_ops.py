@@ -1190,6 +1190,17 @@ def test_entry_points_refuse_bad_arguments():
     assert c(1, P, P, None, None, 0, P, P, P, P, 1, 4, 2, 64, 3, 128, None) == 0
 
 
+def test_the_planner_refuses_rows_outside_the_cache():
+    """A launch takes a block's cache row and first token from the plan: the planner refuses what lies outside."""
+    lib = _lsk().load()
+    cnt = (ctypes.c_long * 9)()
+    for kv8, tree in ((1, 0), (1, 1), (0, 1)):
+        for q_start, row, T, want in ((0, 0, 3, 0), (7, 1, 3, 0), (0, 2, 3, -2), (0, -1, 3, -2), (-1, 0, 3, -2),
+                                      (0, 1 << 30, 0, -2), ((1 << 31) - 3, 0, 3, -2)):
+            blk = (ctypes.c_int32 * 8)(0, 5, 0, 0, q_start, 40, T, row)
+            assert lib.lsk_cache_attn_plan(blk, 2, 4, 256, 2, 2, 128, kv8, tree, 0, 256, None, 0, cnt) == want
+
+
 def test_plans_refuse_blocks_outside_the_cache():
     lsk = _lsk()
     cache = lsk.KV8.zeros(2, 2, 128, 64, "cpu")
