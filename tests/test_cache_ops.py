@@ -769,6 +769,74 @@ def test_attention_scale_streams_and_graph_replays(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["kv8", "kv8 causal", "bf16", "fp32"])
+def test_a_plan_serves_launches_on_other_streams(cuda, kind):
+    """A plan whose upload waits behind its stream's work, used on another stream at once, and dropped before that
+    stream's launch has run, while its own stream takes new memory: the launch's records stay what they are."""
+    lsk = _lsk()
+    Hq, Hkv, D = 8, 2, 64
+    blocks = [(0, 200, 9), (1, 130, 40), (2, 0, 1)]
+    tab, q, k, v = _attn_inputs(83, (Hq, Hkv, D), blocks, F32 if kind == "fp32" else BF16, S=256, B=3)
+    mask = torch.from_numpy(words_of(_tree_blocks(blocks, 9)[1], 2)).to(cuda)
+    if kind.startswith("kv8"):
+        cache = kv8_from(lsk, cuda, k, v)
+        call = lambda plan: lsk.kv8_attn(qd, cache, plan, mask if kind == "kv8" else None)  # noqa: E731
+    else:
+        cache = (lsk.k_to_frag(k) if kind == "bf16" else k).to(cuda)
+        vs = lsk.v_to_blocked(v).to(cuda)
+        call = lambda plan: lsk.tree_attn(qd, cache, vs, plan, mask)  # noqa: E731
+    qd = q.to(cuda)
+    want = call(lsk.AttnPlan(tab, Hq, cache, None if kind == "fp32" else 64))
+    torch.cuda.synchronize()
+    own, other = torch.cuda.Stream(), torch.cuda.Stream()
+    for late_upload in (True, False):
+        with torch.cuda.stream(own):
+            if late_upload:
+                torch.cuda._sleep(20_000_000)
+            plan = lsk.AttnPlan(tab, Hq, cache, None if kind == "fp32" else 64)
+        sizes = [t.numel() for t in plan._buffers]
+        with torch.cuda.stream(other):
+            if not late_upload:
+                torch.cuda._sleep(20_000_000)
+            got = call(plan)
+            again = call(plan)
+        del plan
+        with torch.cuda.stream(own):
+            fresh = [torch.zeros(n, dtype=torch.int32, device=cuda) for n in sizes for _ in range(4)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(again, want) and len(fresh) == 4 * len(sizes)
+
+
+@pytest.mark.gpu
+def test_plans_and_captures(cuda):
+    """A plan is not made inside a capture, nor used there while its upload may still be on its way."""
+    lsk = _lsk()
+    tab, q, k, v = _attn_inputs(89, (8, 2, 64), [(0, 200, 9), (1, 130, 4)], S=256, B=2)
+    cache, qd = kv8_from(lsk, cuda, k, v), q.to(cuda)
+    plan = lsk.AttnPlan(tab, 8, cache)
+    want = lsk.kv8_attn(qd, cache, plan)
+
+    class Pending:
+        def query(self):
+            return False
+
+    uploaded, g = plan._uploaded, torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(lsk.LskError):
+            lsk.AttnPlan(tab, 8, cache)
+        plan._uploaded = Pending()
+        with pytest.raises(lsk.LskError):
+            lsk.kv8_attn(qd, cache, plan)
+        plan._uploaded = uploaded
+        got = lsk.kv8_attn(qd, cache, plan)
+    for i in range(3):
+        got.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(lsk.kv8_attn(qd, cache, plan), want)
+
+
+@pytest.mark.gpu
 def test_attention_of_offsets_past_32_bits(cuda):
     """Cache rows whose first byte lies past 4 GiB: appended, read and attended to."""
     lsk = _lsk()

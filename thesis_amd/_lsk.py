@@ -138,11 +138,11 @@ def _ptr(t) -> int | None:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _stream() -> int:
-    """The current HIP stream of the current device (raw handle; the cheap query when torch has it)."""
+def _stream(dev: int | None = None) -> int:
+    """The current HIP stream of device dev (or the current device): raw handle, by the cheap query when torch has it."""
     if _raw_stream is not None:
-        return _raw_stream(torch._C._cuda_getDevice())
-    return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(torch._C._cuda_getDevice() if dev is None else dev)
+    return torch.cuda.current_stream(dev).cuda_stream
 
 
 def k_to_frag(k: torch.Tensor) -> torch.Tensor:
@@ -696,7 +696,10 @@ class AttnPlan:
     (q_start, pos0, T, row) with q_start the running sum of T; cache: a layer's KV8, or the K storage of a bf16 or fp32
     cache.  split: KV positions per split (cache_attn_split unless given; fp32 does not split); row_groups: a tree's at
     most (by the cache and the block unless given).  tree: which launches it is for, with a mask (True), without (False)
-    or, over an 8-bit cache, either (None)."""
+    or, over an 8-bit cache, either (None).
+    Its records go to the GPU on the current stream.  A launch on another stream waits for them, and they outlive it
+    when the plan is dropped; a captured launch reads them with every replay: the plan is made before the capture and
+    kept as long as the graph."""
 
     def __init__(self, blocks, n_heads: int, cache, split: int | None = None, row_groups: int | None = None,
                  tree: bool | None = None):
@@ -718,12 +721,14 @@ class AttnPlan:
         self.index = self.device.index if self.device.index is not None else -1
         b = np.ascontiguousarray(b, dtype=np.int32)
         group, n_slots = n_heads // Hkv, 2 * cu_count(self.device)    # (two workgroups fit a CU)
+        self._buffers, self._uploaded, self._streams = [], None, set()
         self.works = self.causal = self.tree = None
         self.rows_cap = self.n_works = 0
         if self.dtype == torch.float32:
             self.split, self.rows_cap = 1 << 30, 16
             works, _, _ = attn_plan(b, group, self.split, self.rows_cap)
             self.works, self.n_works = self._upload(works.ravel()), len(works)
+            self._mark_uploaded()
             return
         self.split, self.tree_split = (cache_attn_split(B, Hkv, S, t) if split is None else split for t in (False, True))
         rg = 0 if row_groups is None else row_groups
@@ -731,10 +736,37 @@ class AttnPlan:
             self.causal = self._plan(b, group, self.split, False, 1, n_slots)
         if tree or tree is None:
             self.tree = self._plan(b, group, self.tree_split, True, rg, n_slots)
+        self._mark_uploaded()
 
     def _upload(self, words: np.ndarray) -> torch.Tensor:
         t = torch.from_numpy(words)
-        return t.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else t
+        if self.device.type != "cuda":
+            return t
+        if torch.cuda.is_current_stream_capturing():
+            raise LskError("a plan is made before a capture begins (its upload would be replayed from freed memory)")
+        self._buffers.append(t.pin_memory().to(self.device, non_blocking=True))
+        return self._buffers[-1]
+
+    def _mark_uploaded(self) -> None:
+        if self.device.type == "cuda":
+            stream = torch.cuda.current_stream(self.device)
+            self._uploaded = stream.record_event()
+            self._streams.add(stream.cuda_stream)
+
+    def _join(self, dev: int) -> None:
+        """Before a launch on device dev's current stream: that stream waits for the records, and they outlive it."""
+        if _stream(dev) in self._streams:
+            return
+        with torch.cuda.device(dev):
+            if torch.cuda.is_current_stream_capturing():
+                if not self._uploaded.query():       # (a capture cannot wait for work outside it)
+                    raise LskError("the plan's upload has not ended: synchronize before the capture begins")
+                return
+            stream = torch.cuda.current_stream()
+            stream.wait_event(self._uploaded)
+            for t in self._buffers:
+                t.record_stream(stream)
+            self._streams.add(stream.cuda_stream)
 
     def _plan(self, b: np.ndarray, group: int, split: int, tree: bool, row_groups: int, n_slots: int) -> _Launch:
         lib, cnt = load(), np.zeros(9, dtype=np.int64)
@@ -753,7 +785,7 @@ class AttnPlan:
 
 def _plan_call(what: str, dev: int, q: torch.Tensor, plan: AttnPlan, launch, dims: tuple, kv8: bool,
                dtype: torch.dtype, mask, scale, out, workspace):
-    """Checks shared by kv8_attn and tree_attn; returns (scale, out, workspace, its bytes)."""
+    """Checks shared by kv8_attn and tree_attn, and the plan joined; returns (scale, out, workspace, its bytes)."""
     if dev != plan.index:
         raise LskError(f"{what}: the plan is on {plan.device}, the tensors on cuda:{dev}")
     if plan.dims != dims or plan.kv8 != kv8 or plan.dtype is not dtype:
@@ -779,6 +811,7 @@ def _plan_call(what: str, dev: int, q: torch.Tensor, plan: AttnPlan, launch, dim
     elif not workspace.is_contiguous():
         raise LskError(f"{what}: the workspace must be contiguous")
     ws_bytes = workspace.nbytes if workspace is not None else 0
+    plan._join(dev)
     return plan.scale if scale is None else float(scale), out, workspace, ws_bytes
 
 
