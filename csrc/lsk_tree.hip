@@ -190,7 +190,7 @@ __global__ __launch_bounds__(COMPACT_THREADS) void kv_compact_kernel(
   __shared__ uint32_t s_v[3][D * LD];                // the two blocks the destinations may lie in, and one other
   const int b = blockIdx.x, h = blockIdx.y, layer = blockIdx.z;
   const int row = rows[b], p0 = pos0[b];
-  const int n = (int)min(acc[b], (int64_t)(max_nodes - 1));
+  const int n = (int)min(max(acc[b], (int64_t)0), (int64_t)(max_nodes - 1));
   if (row < 0 || row >= max_batch || p0 < 0 || p0 >= S) return;
   const long stripe = (((long)layer * max_batch + row) * Hkv + h) * (long)S;
   T* kc = (T*)kc_ + stripe * D;

@@ -1057,6 +1057,21 @@ def test_compaction_of_many_layers(cuda, fmt, D, L):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "fp32", "kv8"])
+def test_compaction_of_negative_counts_moves_nothing(cuda, fmt):
+    """Also counts whose low 32 bits are positive."""
+    lsk = _lsk()
+    L, B, H, S, D = 1, 4, 2, 64, 64
+    cache, _, _ = _caches(lsk, cuda, fmt, L, B, H, S, D, _gen(97))
+    before = [t.clone() for t in cache]
+    acc = torch.tensor([-1, -(1 << 32) + 5, -(1 << 40) + 3, -(1 << 63)], device=cuda)
+    args = (_i32(range(B), cuda), _i32([0, 3, 20, 7], cuda), acc, _i32([[0, 2, 4, 6, 8, 10, 12, 14]] * B, cuda))
+    lsk.kv8_compact(cache, *args) if fmt == "kv8" else lsk.kv_compact(*cache, *args)
+    bits = lambda t: t.view(torch.uint8).cpu()                        # noqa: E731
+    assert all(torch.equal(bits(a), bits(b)) for a, b in zip(cache, before))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["bf16", "kv8"])
 def test_a_tree_step_captured_in_two_graphs(cuda, fmt):
     """Masks, write, attention, acceptance and compaction as a captured step, replayed with new inputs between eager
