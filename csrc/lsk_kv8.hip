@@ -4,6 +4,7 @@
 // e + 127 in a byte:
 //   amax = the largest finite |x|,  e = the smallest integer >= -117 with amax <= 448 * 2^e  (448 is e4m3's largest),
 //   code = rne_e4m3(x * 2^-e),  the cache stands for code * 2^e.  NaN and infinities become NaN codes; amax = 0: e = 0.
+// At the largest e, 120, a code is at most 240 (the next one, 256, would stand for 2^128; still within 2^-4 of x).
 // With e >= -117 every value is zero or a normal number (e4m3's smallest is 2^-9), in bf16 as in fp32.
 // The product x * 2^-e is exact (a value far below amax may underflow, where its code is 0 anyway), so the only
 // rounding is the one to e4m3: at most 2^-4 of the value, or 2^-10 * 2^e for values below 2^-6 * 2^e.
@@ -32,11 +33,15 @@ __device__ __forceinline__ int biased_exponent(uint32_t m) {
   return e < 10 ? 10 : e;
 }
 
-// four floats -> four e4m3 codes, after the exact scaling by inv; non-finite values -> NaN codes
-__device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
+// four floats -> four e4m3 codes, after the exact scaling by 2^(127 - e); non-finite values -> NaN codes
+__device__ __forceinline__ uint32_t codes4(const float* x, int e) {
+  const float inv = __uint_as_float((uint32_t)(254 - e) << 23), top = e == 247 ? 240.f : 448.f;
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_fmed3f(x[i] * inv, -top, top);
   uint32_t r = 0;
-  r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, (int)r, false);
-  r = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, (int)r, true);
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], (int)r, false);
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], (int)r, true);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if ((__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u) r |= 0x7fu << (8 * i);
@@ -169,12 +174,11 @@ __global__ __launch_bounds__(KV8_THREADS) void kv8_append_kernel(const T* __rest
     for (int i = 0; i < PER; i += 4) load4(src + i, x + i);
     const int row = rows[t], p = pos[t];
     const int e = biased_exponent(vector_max<PER>(x));
-    const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
     if (row < 0 || row >= max_batch || p < 0 || p >= S) return;
     const long stripe = ((long)row * Hkv + h) * (long)S;
     uint32_t* dst = (uint32_t*)(kc + stripe * D + kv8_k_offset(p, part * PER, D));
 #pragma unroll
-    for (int i = 0; i < PER / 4; ++i) dst[i] = codes4(x + 4 * i, inv);
+    for (int i = 0; i < PER / 4; ++i) dst[i] = codes4(x + 4 * i, e);
     if (part == 0) ks[stripe + p] = (uint8_t)e;
     return;
   }
@@ -191,9 +195,8 @@ __global__ __launch_bounds__(KV8_THREADS) void kv8_append_kernel(const T* __rest
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const int e = biased_exponent(vector_max<PER>(x[c]));
-    const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
 #pragma unroll
-    for (int i = 0; i < PER / 4; ++i) w[i][c] = codes4(&x[c][4 * i], inv);
+    for (int i = 0; i < PER / 4; ++i) w[i][c] = codes4(&x[c][4 * i], e);
     if (part == 0 && 4 * j + c < nt) {
       const int row = rows[t0 + 4 * j + c], p = pos[t0 + 4 * j + c];
       if (row >= 0 && row < max_batch && p >= 0 && p < S) vs[((long)row * Hkv + h) * (long)S + p] = (uint8_t)e;

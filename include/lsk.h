@@ -278,7 +278,8 @@ int lsk_shift_segment_positions(int32_t* meta, int n_tokens, int nb, int n_works
 /* ---- 8-bit KV cache (no counterpart in the reference, whose cache is the model's dtype) ----
  * One token's K (V) of one KV head: head_dim e4m3 codes and a power-of-two scale 2^e held as the byte e + 127:
  *   amax = largest finite |x|, e = smallest integer >= -117 with amax <= 448 * 2^e (0 for amax = 0),
- *   code = x * 2^-e rounded to e4m3, nearest even (NaN and infinities: NaN), value = code * 2^e.
+ *   code = x * 2^-e rounded to e4m3, nearest even (at e = 120 at most 240; NaN and infinities: NaN),
+ *   value = code * 2^e: finite for every finite x.
  * Storage of a layer (head_dim 64 or 128, S = max_seq a multiple of 64, tensors at multiples of 16 bytes):
  *   k8 [B, Hkv, S/64, 4, D/64, 64, 16] bytes: lane 16 lg + l16 of fragment (a, j) of a 64-position block holds position
  *      16 (l16 / 4) + 4 a + l16 % 4 and d = 64 j + 16 lg .. + 15;

@@ -283,6 +283,38 @@ def test_kv8_append_takes_strides_and_non_finite_values(cuda):
     assert torch.isnan(held(view(buf, 1))).sum() == 3
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_largest_finite_values_stay_finite(cuda, dtype, D):
+    """At e = 120 the e4m3 value 256 would stand for 2^128: codes end at 240, within 2^-4 of the value.  A query of
+    zeros weighs such keys equally."""
+    lsk = _lsk()
+    top = torch.finfo(dtype).max
+    x = torch.randn(6, 2, D, generator=_gen(7)).to(dtype)
+    x[0, :, :4] = torch.tensor([top, -top, top / 2, top / 300], dtype=dtype)
+    x[1, :, 5], x[2, :, 5], x[3, :, 5] = 248 * 2.0 ** 120, -247 * 2.0 ** 120, 2.0 ** 127
+    x[4] = top * torch.linspace(-1, 1, D, dtype=torch.float64).to(dtype)
+    v = torch.randn(6, 2, D, generator=_gen(8)).to(dtype)
+    cache = lsk.KV8.zeros(1, 2, 64, D, cuda)
+    rows, pos = _i32(np.zeros(6), cuda), _i32(np.arange(6), cuda)
+    for k_, v_ in ((x, v), (v, x)):
+        lsk.kv8_append(k_.to(cuda), v_.to(cuda), cache, rows, pos)
+        want = held(x).clamp(-240 * 2.0 ** 120, 240 * 2.0 ** 120)
+        assert ((want - x.double()).abs() <= 2.0 ** -4 * x.double().abs() + 2.0 ** -10 * 2.0 ** 120).all()
+        for out in (F32, BF16):
+            got = lsk.kv8_read(cache, rows, pos, out)[0 if k_ is x else 1]
+            assert torch.equal(got.double().cpu(), want)
+        if k_ is x:
+            assert cache.ks[0, :, 0].tolist() == [247, 247]
+            tab = [(0, 5, 1, 0)]
+            got = lsk.kv8_attn(torch.zeros(1, 2, D, dtype=BF16, device=cuda), cache, lsk.AttnPlan(tab, 2, cache))
+            dense = lambda t: held(t).permute(1, 0, 2)[None]          # noqa: E731
+            zero = torch.zeros(1, 2, D, dtype=torch.float64)
+            ref, mag, _ = attention(zero, torch.zeros_like(dense(v)), dense(v), tab, 1.0)
+            assert_close_bf16(got, ref, mag)
+
+
 # ----------------------------------------------------------------------------- attention
 
 def _heads(case):
