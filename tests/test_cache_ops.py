@@ -585,6 +585,82 @@ def _minus_infinity(kind, q, k, at):
         k[row, :, slots, 3] = -3e38 if kind.startswith("kv8") else -math.inf
 
 
+def _rising(seed, heads, blocks, S=1088, B=4):
+    """Inputs whose scores (in log2 units, scale ln 2) climb along the context by steps of 3 to 12, each row at its own
+    rate: downwards, not at all, slowly and fast, so that the rows of a tile pass their maxima at different steps."""
+    Hq, Hkv, D = heads
+    tab, q, k, v = _attn_inputs(seed, heads, blocks, S=S, B=B)
+    g, n = _gen(seed + 1), len(q)
+    q, k = q * 0.1, k * 0.5
+    climb = torch.where(torch.rand(B, Hkv, S, generator=g) < 0.02, 3.0 + 9.0 * torch.rand(B, Hkv, S, generator=g), 0.0)
+    k[..., 3] = (climb.cumsum(-1) - climb.sum(-1, keepdim=True) / 2).to(BF16)
+    rate = torch.tensor([1.0, -0.5, 0.0, 0.25, 0.75, 1.5])[torch.arange(n * Hq).view(n, Hq) % 6]
+    q[..., 3] = rate.to(BF16)
+    return tab, q, k, v
+
+
+def _passes(q, k, tab, sets, step, ways, split, limit):
+    """For every row (64 bits): how often a step's maximum passes a finite running one by more than `limit` (log2
+    units), and how often by less, with the steps of each split taken by `ways` waves in turn."""
+    N, Hq, D = q.shape
+    G = Hq // k.shape[1]
+    far, near = torch.zeros(N, Hq, dtype=torch.int64), torch.zeros(N, Hq, dtype=torch.int64)
+    for (qs, p0, T, row) in tab:
+        for t in range(T):
+            s = (q[qs + t].view(-1, G, D) @ k[row, :, :p0 + t + 1].transpose(-1, -2)).reshape(Hq, -1)
+            if sets is not None:
+                skip = [p0 + j for j in range(t + 1) if j not in sets[qs + t]]
+                s[:, skip] = -math.inf
+            for lo in range(0, s.shape[1], split):
+                tiles = [x.amax(-1) for x in s[:, lo:lo + split].split(step, -1)]
+                for w in range(ways):
+                    m = torch.full((Hq,), -math.inf, dtype=torch.float64)
+                    for x in tiles[w::ways]:
+                        over = x - m
+                        far[qs + t] += torch.isfinite(m) & (over > limit)
+                        near[qs + t] += torch.isfinite(m) & (over > 0) & (over <= limit)
+                        m = torch.where((over > limit) | torch.isneginf(m), x, m)
+    return far, near
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [64, 512, 2048])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kind,row_groups", [("kv8 causal", None), ("kv8", 1), ("kv8", 2), ("kv8", 4), ("bf16", 1),
+                                             ("bf16", 2), ("bf16", 4)])
+def test_running_maxima_that_are_passed_again_and_again(cuda, kind, row_groups, D, split):
+    """The running maximum moves when it is passed by more than 2^8, and stays when by less: scores that climb by both,
+    waves and splits whose maxima lie tens apart.  A score is off by (D + 4) 2^-24 sum |q k| scale at most, which moves
+    its weight and the sum of the weights by as much relatively (the sum is `big`)."""
+    lsk = _lsk()
+    Hq, Hkv = 8, 2
+    blocks = [(0, 600, 9), (1, 900, 1), (2, 700, 40), (3, 333, 12), (0, 1050, 20)]
+    tab, q, k, v = _rising(101, (Hq, Hkv, D), blocks)
+    sets = None if kind == "kv8 causal" else _tree_blocks(blocks, 13)[1]
+    mask = None if sets is None else torch.from_numpy(words_of(sets, 2)).to(cuda)
+    if kind == "bf16":
+        ks, vs = lsk.k_to_frag(k).to(cuda), lsk.v_to_blocked(v).to(cuda)
+        got = lsk.tree_attn(q.to(cuda), ks, vs, lsk.AttnPlan(tab, Hq, ks, split, row_groups), mask, math.log(2.0))
+    else:
+        cache = kv8_from(lsk, cuda, k, v)
+        got = lsk.kv8_attn(q.to(cuda), cache, lsk.AttnPlan(tab, Hq, cache, split, row_groups), mask, math.log(2.0))
+        if sets is None:                              # the same rows as single tokens: the same bits
+            one = [(i, p0 + t, 1, row) for (qs, p0, T, row) in tab for t, i in enumerate(range(qs, qs + T))]
+            alone = lsk.kv8_attn(q.to(cuda), cache, lsk.AttnPlan(one, Hq, cache, split), None, math.log(2.0))
+            assert torch.equal(alone, got)
+        k, v = held(k), held(v)
+    q, k, v = q.double(), k.double(), v.double()
+    ref, mag, big = attention(q, k, v, tab, math.log(2.0), sets)
+    got = got.double().cpu()
+    tol = 1.01 * 2.0 ** -8 * (ref.abs() + mag) + (2.0 ** -12 + 2 * (D + 4) * 2.0 ** -24 * big) * mag + 1e-30
+    assert ((got - ref).abs() <= tol).all(), ((got - ref).abs() / tol).max()
+    if split > 64:                                    # (at 64 positions a wave has one step or two)
+        step, ways = 32 if row_groups == 4 or kind == "bf16" else 64, 4 // (row_groups or 1)   # of blocks of many rows
+        far, near = _passes(q, k, tab, sets, step, ways, split, 8.0)
+        tile = far[10:14].reshape(-1)                 # 16 query rows per KV head and tile: four tokens
+        assert (far > 0).sum() > 100 and (near > 0).sum() > 100 and len(set(tile.tolist())) > 1
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("split", [None, 64])
 @pytest.mark.parametrize("D", [64, 128])
