@@ -378,6 +378,20 @@ def test_attention_merges_up_to_128_splits(cuda, D, split):
     assert_close_bf16(lsk.tree_attn(q.to(cuda), kf, vf, lsk.AttnPlan(tab, Hq, kf, split=split), mask), ref, mag)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [None, 128])
+@pytest.mark.parametrize("heads", ["gqa128", "gqa64"])
+def test_kv8_attention_of_prompts(cuda, heads, split):
+    """Whole prompts and a prompt behind a committed prefix, several hundred tokens a block, beside a decode step."""
+    lsk = _lsk()
+    Hq, Hkv, D = _heads(heads)
+    tab, q, k, v = _attn_inputs(107, (Hq, Hkv, D), [(1, 0, 333), (0, 97, 250), (2, 400, 1)], S=448, B=3)
+    cache = kv8_from(lsk, cuda, k, v)
+    got = lsk.kv8_attn(q.to(cuda), cache, lsk.AttnPlan(tab, Hq, cache, split, tree=False))
+    ref, mag, _ = attention(q.double(), held(k), held(v), tab, 1 / math.sqrt(D))
+    assert_close_bf16(got, ref, mag)
+
+
 def _tree_blocks(blocks, seed):
     rng = np.random.default_rng(seed)
     parents = [random_tree(rng, t) if t else [] for (_, _, t) in blocks]
@@ -1162,6 +1176,47 @@ def test_compaction_of_many_layers(cuda, fmt, D, L):
             x[:, r, :, pos0[i]:pos0[i] + len(src)] = x[:, r][:, :, src].clone()
     assert torch.equal((lsk.k_from_frag(kc.cpu()) if fmt == "bf16" else kc.cpu()), k)
     assert torch.equal(lsk.v_from_blocked(vc.cpu()), v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_compaction_of_an_engines_cache(cuda, dtype):
+    """KVCache's own storage, all layers at once, and a run of them; attention over a layer of it before and after."""
+    from thesis_amd.common.model import KVCache, ModelConfig
+
+    lsk = _lsk()
+    cfg = ModelConfig(64, 256, 3, 4, 2, 64, 256)
+    L, B, H, S, D = 3, 2, 2, 128, cfg.head_dim
+    kv = KVCache(cfg, B, S, dtype, cuda)
+    g = _gen(109)
+    dense = [torch.randn(L, B, H, S, D, generator=g).to(dtype) for _ in range(2)]
+    kstore = kv.kf_all if dtype == BF16 else kv.k_all
+    kstore.copy_(lsk.k_to_frag(dense[0]) if dtype == BF16 else dense[0])
+    kv.vb_all.copy_(lsk.v_to_blocked(dense[1]))
+    q = torch.randn(1, 4, D, generator=g).to(dtype)
+    tab, sets = [(0, 43, 1, 1)], [{0}]
+    mask = torch.from_numpy(words_of(sets, 1)).to(cuda)
+
+    def attend(layer):
+        plan = lsk.AttnPlan(tab, 4, kv.kstore[layer], tree=True)
+        got = lsk.tree_attn(q.to(cuda), kv.kstore[layer], kv.vb[layer], plan, mask)
+        ref, mag, big = attention(q.double(), dense[0][layer].double(), dense[1][layer].double(), tab, 1 / math.sqrt(D),
+                                  sets)
+        assert_close_f32(got, ref, mag, S, D, big) if dtype == F32 else assert_close_bf16(got, ref, mag)
+
+    path = [0, 2, 5, 9]
+    args = (_i32([1], cuda), _i32([40], cuda), torch.tensor([3], device=cuda), _i32([path], cuda))
+    attend(1)
+    lsk.kv_compact(kstore[1:], kv.vb_all[1:], *args)
+    for x in dense:
+        x[1:, 1, :, 40:44] = x[1:, 1][:, :, [40 + j for j in path]].clone()
+    assert torch.equal(kv.k_all.cpu(), dense[0]) and torch.equal(kv.v_all.cpu(), dense[1])
+    attend(1)
+    lsk.kv_compact(kstore, kv.vb_all, *args)
+    for x in dense:
+        x[:, 1, :, 40:44] = x[:, 1][:, :, [40 + j for j in path]].clone()
+    assert torch.equal(kv.k_all.cpu(), dense[0]) and torch.equal(kv.v_all.cpu(), dense[1])
+    attend(0)
 
 
 @pytest.mark.gpu
