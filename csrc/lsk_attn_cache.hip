@@ -19,11 +19,12 @@
 //          (two MFMA operands of 8 d each); V^T: row d, positions 16 lg .. + 15 (two operands of 8 positions each).
 //          A position's K and V are its codes times 2^(ks - 127) and 2^(vs - 127).
 // Per step of a wave (v_mfma_f32_16x16x32_bf16): S^T[pos][q] = K Q^T, whose rows are mapped to positions so that lane
-// group lg ends up with the consecutive positions its V^T load needs; online softmax with fp32 statistics;
-// O^T[d][q] += V^T P^T.  e4m3 values times a power of two are bf16 values, so the conversions in registers are exact
-// and K's scale costs nothing (the conversion takes one); V's scale, which differs per position, multiplies the
-// weights.  The weights are rounded to bf16 for the second product (by at most 2^-8 each, independent of one another:
-// it adds about as much error as the rounding of the bf16 output); the sum of the weights is taken before that rounding.
+// group lg ends up with the consecutive positions its V^T load needs; online softmax with fp32 statistics; O^T[d][q] +=
+// V^T P^T.  e4m3 values times a power of two are bf16 values, so the conversions in registers are exact and K's scale
+// costs nothing (the conversion takes one); V's scale, which differs per position, multiplies the weights.  The weights
+// are rounded to bf16 for the second product, as the ragged attention's are (by at most 2^-8 each, independent of one
+// another: with the bf16 output's rounding the error against 64 bits is 0.0021 to 0.0023 of the outputs' size, where
+// fp32 weights leave 0.0017); the sum of the weights is taken before that rounding.
 //
 // The waves of a row group take the steps round robin and are merged in wave order.  Which wave takes a step and every
 // order of additions depend on absolute positions only: a row's result never depends on what else is in the launch.  An
@@ -564,13 +565,15 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
   }
 }
 
-// Trees of more rows: an item of four row groups of 32 rows, a wave each, which read the same K and V.  These go through
-// LDS, a step's at a time (8-bit: two steps'), in two buffers: a wave that reads them for itself takes its share of the
-// CU's 64 bytes per clock (32 trees of 25 to 64 nodes, 8B heads, 128 to 1280 positions: 67 us without LDS, 42 with it).
-// 8-bit codes become bf16 on the way, once for all the waves.  Q stays in registers.  Two workgroups fit a CU, so that
-// one's waits fall into the other's steps (one of eight waves, merged at the end: 45 us).
-// Bound by the softmax's vector instructions beside the products and the reads of LDS: 32 positions of 256 rows take
-// 1.3 us of a CU, of which the matrix instructions are 0.5.
+// Trees of more rows: an item of four row groups of 32 rows, a wave each, which read the same K and V.  These go
+// through LDS, a step's at a time (8-bit: two steps'), in two buffers: a wave that reads them for itself takes its
+// share of the CU's 64 bytes per clock (32 trees of 25 to 64 nodes, 8B heads, 128 to 1280 positions: 67 us without LDS,
+// 42 with it). 8-bit codes become bf16 on the way, once for all the waves.  Q stays in registers.  Two workgroups fit a
+// CU, so that one's waits fall into the other's steps (one of eight waves, merged at the end: 45 us).
+// A CU is bound by the softmax's vector instructions beside the products and the reads of LDS: 32 positions of 256 rows
+// take 1.3 us of it, of which the matrix instructions are 0.5.  The launch is bound by its fullest CU: every item is a
+// workgroup of its own and all are resident at once (those 32 trees: 480 items, 23 to 28 us of such work a CU, 40 on
+// the fullest).
 #define TREE_WAVES 4
 template <int D, bool KV8>
 __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const CacheAttnArgs A,
@@ -752,7 +755,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
 }
 
 // Merge the splits of a row in split order: M = max_s m_s, w_s = exp2(m_s - M), out = sum w_s O_s / sum w_s l_s (zeros
-// where no split read anything).  16 lanes per row: they take the splits' statistics side by side, then each D / 16 dims
+// where the row reads nothing).  16 lanes per row: they take the splits' statistics side by side, then each D / 16 dims
 // of the partial outputs, AHEAD splits' loads in flight, the first ones beside the statistics'.  (A wave per row with
 // the loads behind the statistics: 32 trees of 64 nodes in three splits 57 us, now 20.)
 #define COMBINE_ROWS 16
@@ -1007,7 +1010,8 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
     const int pos0 = bm[1];
     const long rows = (long)bm[2] * group;
     int lr = 0;
-    const int most_groups = row_groups ? row_groups : (long)max_batch * n_kv_heads * ((rows + 31) / 32) <= n_slots ? 1 : 4;
+    const bool few = (long)max_batch * n_kv_heads * ((rows + 31) / 32) <= n_slots;
+    const int most_groups = row_groups ? row_groups : few ? 1 : 4;
     while (tree && (1 << lr) < most_groups && rows > (32L << lr)) ++lr;
     used = (1 << lr) > used ? 1 << lr : used;
     const int cap = (16 * tiles) << lr;
@@ -1150,7 +1154,8 @@ static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t
     cache_combine_kernel<128><<<cg, 256, 0, s>>>(groups, a.o_part, a.ml_part, a.mask, a.W, a.out, a.G, a.Hkv,
                                                  a.part_rows);
   else
-    cache_combine_kernel<64><<<cg, 256, 0, s>>>(groups, a.o_part, a.ml_part, a.mask, a.W, a.out, a.G, a.Hkv, a.part_rows);
+    cache_combine_kernel<64><<<cg, 256, 0, s>>>(groups, a.o_part, a.ml_part, a.mask, a.W, a.out, a.G, a.Hkv,
+                                                a.part_rows);
   return lsk_check_launch(what);
 }
 

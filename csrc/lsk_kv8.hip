@@ -146,14 +146,15 @@ __device__ __forceinline__ void kv8_dwords(long stripe, int p0, int nt, F f) {
 
 }  // namespace
 
-// Workgroup 0 of blockIdx.z quantises 64 tokens' V of one KV head (it takes longest and starts first), workgroups 1 to 4
-// quantise 16 tokens' K each.  16 threads hold a token's vector, D / 16 consecutive elements each, and find its largest
-// magnitude by shuffles.  K goes straight to its place.  V is turned, 4 x 4 in registers and the rest in LDS: a run of
-// positions (a prompt's tokens) is written a dword at a time, whole 64-byte sectors from one workgroup; other tokens
-// byte by byte.
-// Latency-bound for a decode step's tokens; a long prompt moves 3 D bytes a token and head (4001 tokens of 8 heads of
-// 128: 11.8 us; with the V workgroups last 13.4; with 16 tokens to every workgroup, so that four share a sector of V,
-// 16.9).
+// Workgroup 0 of blockIdx.z quantises 64 tokens' V of one KV head (it takes longest and starts first), workgroups 1 to
+// 4 quantise 16 tokens' K each.  16 threads hold a token's vector, D / 16 consecutive elements each, and find its
+// largest magnitude by shuffles.  K goes straight to its place.  V is turned, 4 x 4 in registers and the rest in LDS: a
+// run of positions (a prompt's tokens) is written a dword at a time, whole 64-byte sectors from one workgroup; other
+// tokens byte by byte.
+// Bound by a workgroup's chain of loading, reducing, converting, turning and storing: 6.9 us for a decode step's
+// tokens, whose V asks for rows and positions behind the conversion and is stored byte by byte; a prompt moves 3 D
+// bytes a token and head (4001 tokens of 8 heads of 128: 11.3 us, 4.8 by their bytes; with the V workgroups last 13.4;
+// with 16 tokens to every workgroup, so that four share a sector of V, 16.9).
 template <typename T, int D>
 __global__ __launch_bounds__(KV8_THREADS) void kv8_append_kernel(const T* __restrict__ k, const T* __restrict__ v,
                                                                  long st_t, long st_h, uint8_t* __restrict__ kc,
@@ -231,7 +232,7 @@ __global__ __launch_bounds__(KV8_THREADS) void kv8_append_kernel(const T* __rest
   });
 }
 
-// The way back, in the same shape (4001 tokens of 8 heads of 128: 10.1 us).
+// The way back, in the same shape and bound alike (4001 tokens of 8 heads of 128: 10.2 us).
 template <typename T, int D>
 __global__ __launch_bounds__(KV8_THREADS) void kv8_read_kernel(const uint8_t* __restrict__ kc,
                                                                const uint8_t* __restrict__ vc,

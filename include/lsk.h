@@ -285,9 +285,9 @@ int lsk_shift_segment_positions(int32_t* meta, int n_tokens, int nb, int n_works
  *      16 (l16 / 4) + 4 a + l16 % 4 and d = 64 j + 16 lg .. + 15;
  *   v8 [B, Hkv, S/64, D, 64] bytes: blocks transposed;   k_exp, v_exp [B, Hkv, S] bytes.
  *
- * lsk_kv8_append: k, v [n_tokens, n_kv_heads, head_dim] (bf16 or fp32; strides in elements, dims contiguous) go to
- * (rows[t], pos[t]).  A token outside [0, max_batch) x [0, max_seq) is skipped.  The (row, position) pairs of a call
- * have to differ: of equal ones, one token's codes may meet the other's scale.
+ * lsk_kv8_append: k, v [n_tokens, n_kv_heads, head_dim] (bf16 or fp32; strides in elements, dims contiguous), k with
+ * its RoPE rotation, go to (rows[t], pos[t]).  A token outside [0, max_batch) x [0, max_seq) is skipped.  The (row,
+ * position) pairs of a call have to differ: of equal ones, one token's codes may meet the other's scale.
  * lsk_kv8_read: the values at (rows[t], pos[t]) as contiguous k, v [n_tokens, n_kv_heads, head_dim] (bf16 exactly, or
  * fp32); zeros for a token outside the cache.
  * Beside lsk_kv_append (solutions/packed.py:180-181). */
@@ -303,25 +303,27 @@ int lsk_kv8_read(int dtype, const void* k8, const void* v8, const void* k_exp, c
  * trees), any strides in elements, dims contiguous; out [n_tokens, n_heads * head_dim] contiguous, q's dtype.
  * Token t of block {q_start, pos0, T, row} sits in slot pos0 + t of its cache row and reads slots 0 .. pos0 + t; with a
  * mask (uint32 [n_tokens][mask_words]), of the block's own slots only those whose bit is set: bit j % 32 of word j / 32
- * for node j; bits of later nodes and bits past the words count as 0.  A row that reads nothing gives zeros.  Values in
- * slots that a row does not read never reach it, whatever they are.
+ * for node j; bits of later nodes and bits past the words count as 0.  A row that reads nothing gives zeros, one whose
+ * scores are all -infinity NaN.  Values in slots that a row does not read never reach it, whatever they are.
+ * bf16 and 8-bit: scores, statistics and sums are fp32; the weights are rounded to bf16 for their product with V, as
+ * lsk_ragged_attn's are.
  * Weights are relative to a running maximum that may lag by 2^8 and are summed in fp32 before the division: 2^8 |V|
  * times the positions read has to stay below 2^128.
  * groups .. part_rows: lsk_cache_attn_plan's (fp32 trees: works, n_works, rows_cap of an unsplit lsk_attn_plan).
  * workspace >= lsk_cache_attn_workspace_bytes(n_parts, n_kv_heads, part_rows, head_dim), 16-byte aligned, and a call's
  * own (one that two captured graphs share is written by both).  head_dim 64 or 128 (fp32 also 16 and 32); scale not
- * negative; bf16 and 8-bit: max_seq a multiple of 64, a (row, KV head) stripe below 2 GiB.  A row's result depends on
+ * negative; bf16 and 8-bit: max_seq a multiple of 64, max_seq * head_dim below 2^30.  A row's result depends on
  * its own block (with a mask: also on the plan's row_groups) and the split only, not on the rest of the launch; an fp32
  * chain (every ancestor's bit set) gives lsk_ragged_attn's bits.
  * Beside lsk_ragged_attn (solutions/packed.py:142-166).
  *
  * lsk_cache_attn_plan (host pointers, no GPU work): blocks int32 [nb][4] = {q_start, pos0, T, row}, a row of the
- * cache's max_batch; split: positions per split, a multiple of 64, at most 128 splits per context.  tree: the launch has
- * a mask; then blocks of many rows share K / V among up to row_groups (1, 2, 4; 0: by the cache and the block) groups
- * of 32 rows.  n_slots: persistent workgroups, two per CU; recs: their items, and behind them the n_shared items of four
- * row groups (a workgroup each).  meta = [groups int32 n_groups*8][recs n_slots*n_rounds*8, then n_shared*8]; counts[9]
- * = {tokens, n_groups, n_parts, n_rounds, tiles, part_rows, words of meta, row_groups used, n_shared}.  meta == NULL:
- * counts only; meta_cap too small: LSK_EWORKSPACE with counts written. */
+ * cache's max_batch; split: positions per split, a multiple of 64, at most 128 splits per context.  tree: the launch
+ * has a mask; then blocks of many rows share K / V among up to row_groups (1, 2, 4; 0: by the cache and the block)
+ * groups of 32 rows.  n_slots: persistent workgroups, two per CU; recs: their items, and behind them the n_shared items
+ * of four row groups (a workgroup each).  meta = [groups int32 n_groups*8][recs n_slots*n_rounds*8, then n_shared*8];
+ * counts[9] = {tokens, n_groups, n_parts, n_rounds, tiles, part_rows, words of meta, row_groups used, n_shared}.  meta
+ * == NULL: counts only; meta_cap too small: LSK_EWORKSPACE with counts written. */
 int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int max_batch, int n_kv_heads,
                         int head_dim, int kv8, int tree, int row_groups, int n_slots, int32_t* meta, long meta_cap,
                         long* counts);
@@ -339,8 +341,10 @@ int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_stride_h, co
 
 /* ---- trees of drafted tokens (the reference drafts chains) ----
  * A block's nodes are its tokens 0 .. lens[b] - 1 from starts[b]; node 0 is the root (the last committed token),
- * parents[starts[b] + i] < i the parent of node i (anything outside [0, i): none).  Node i's K / V sit in slot
- * pos0 + i.
+ * parents[starts[b] + i] < i the parent of node i (anything outside [0, i): none).  Node i's K / V sit in slot pos0 +
+ * i, K rotated for position pos0 + depth.  The launches that rotate and append (lsk_rope_append,
+ * lsk_rope_append_partial, lsk_gemm_qkv_rope) take one position for both: a node beside a chain is rotated by the
+ * caller and written by lsk_kv_append or lsk_kv8_append.
  *
  * lsk_tree_masks: mask [n_tokens][mask_words] (32 * mask_words >= max_nodes >= every len) = the bits of each node's
  * ancestors and its own; depth [n_tokens] (optional) = its number of ancestors (its RoPE position is pos0 + depth).
@@ -353,8 +357,8 @@ int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_stride_h, co
  * (solutions/engine.py:461-476).
  *
  * lsk_kv_compact: slot pos0[b] + j of cache row rows[b] takes what slot pos0[b] + path[b][j] holds, j = 1 ..
- * accepted[b], in every layer and KV head (caches [n_layers, max_batch, ...], contiguous; k_exp, v_exp for
- * LSK_DTYPE_KV8, else NULL); then lsk_kv_rollback's pointer update holds as for a chain.  path as lsk_tree_accept
+ * accepted[b] (negative: none), in every layer and KV head (caches [n_layers, max_batch, ...], contiguous; k_exp, v_exp
+ * for LSK_DTYPE_KV8, else NULL); then lsk_kv_rollback's pointer update holds as for a chain.  path as lsk_tree_accept
  * writes it (increasing); the rows of a call have to differ.  Blocks outside the cache are skipped.  V's neighbouring
  * slots of a moved one (16 bytes) are written back as they were. */
 int lsk_tree_masks(const int32_t* parents, const int32_t* starts, const int32_t* lens, int nb, int n_tokens,

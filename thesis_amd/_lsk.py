@@ -139,7 +139,8 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _stream(dev: int | None = None) -> int:
-    """The current HIP stream of device dev (or the current device): raw handle, by the cheap query when torch has it."""
+    """The current HIP stream of device dev, or of the current device (raw handle; the cheap query when torch has it).
+    """
     if _raw_stream is not None:
         return _raw_stream(torch._C._cuda_getDevice() if dev is None else dev)
     return torch.cuda.current_stream(dev).cuda_stream
@@ -668,7 +669,10 @@ def cache_attn_split(max_batch: int, n_kv_heads: int, max_seq: int, tree: bool =
     heads of 64, one token, 1 request: 1000 positions 7.2 us whole, 11.0 in two; 5000 positions 15.8 whole, 10.8 in
     five).  Trees, whose partial outputs are many rows: 1280 positions, 2048 from 32 stripes on (64 nodes, 32 / 8 heads
     of 128: 4 requests of 1000 positions 14 us whole, 28 in two, of 5000 positions 37 and 42 in three; 1 request of 5000
-    positions 33 whole, 21 in three).  512 to 8192 positions, at most 128 splits."""
+    positions 33 whole, 21 in three).  512 to 8192 positions, at most 128 splits.  256: MI355X's CUs, as a constant, so
+    that a row's bits are the same on every device.  The rule does not see a prompt, whose many rows need no splits: its
+    plan is better given one (one prompt of 4001 tokens in a cache of its own, 32 / 8 heads of 128: 396 us and a
+    workspace of 181 MB at 832 positions, 248 us and none at 8192)."""
     stripes = max_batch * n_kv_heads
     if tree:
         n = min(256 // stripes, max_seq // (1280 if stripes < 32 else 2048))
@@ -696,7 +700,7 @@ class AttnPlan:
     (q_start, pos0, T, row) with q_start the running sum of T; cache: a layer's KV8, or the K storage of a bf16 or fp32
     cache.  split: KV positions per split (cache_attn_split unless given; fp32 does not split); row_groups: a tree's at
     most (by the cache and the block unless given).  tree: which launches it is for, with a mask (True), without (False)
-    or, over an 8-bit cache, either (None).
+    or, over an 8-bit cache, either (None), which takes twice as long (256 requests: 333 us for 129).
     Its records go to the GPU on the current stream.  A launch on another stream waits for them, and they outlive it
     when the plan is dropped; a captured launch reads them with every replay: the plan is made before the capture and
     kept as long as the graph."""
@@ -730,7 +734,8 @@ class AttnPlan:
             self.works, self.n_works = self._upload(works.ravel()), len(works)
             self._mark_uploaded()
             return
-        self.split, self.tree_split = (cache_attn_split(B, Hkv, S, t) if split is None else split for t in (False, True))
+        self.split, self.tree_split = (split if split is not None else cache_attn_split(B, Hkv, S, t)
+                                       for t in (False, True))
         rg = 0 if row_groups is None else row_groups
         if self.kv8 and not tree:
             self.causal = self._plan(b, group, self.split, False, 1, n_slots)
@@ -771,8 +776,8 @@ class AttnPlan:
     def _plan(self, b: np.ndarray, group: int, split: int, tree: bool, row_groups: int, n_slots: int) -> _Launch:
         lib, cnt = load(), np.zeros(9, dtype=np.int64)
         B, Hkv, _, D = self.dims
-        args = (b.ctypes.data if len(b) else None, len(b), group, split, B, Hkv, D, int(self.kv8), int(tree), row_groups,
-                n_slots)
+        args = (b.ctypes.data if len(b) else None, len(b), group, split, B, Hkv, D, int(self.kv8), int(tree),
+                row_groups, n_slots)
         _check(lib.lsk_cache_attn_plan(*args, None, 0, cnt.ctypes.data), "lsk_cache_attn_plan")
         meta = np.zeros(max(int(cnt[6]), 1), dtype=np.int32)
         _check(lib.lsk_cache_attn_plan(*args, meta.ctypes.data, meta.size, cnt.ctypes.data), "lsk_cache_attn_plan")
