@@ -989,7 +989,7 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
     const long q_start = bm[0], pos0 = bm[1], T = bm[2];
     LSK_REQUIRE(T >= 0 && pos0 >= 0 && pos0 + T <= 0x7fffffffL - split && T * group < (1L << 31), LSK_ESHAPE,
                 "%s: block %d has T=%ld pos0=%ld", what, b, T, pos0);
-    LSK_REQUIRE(q_start >= 0 && q_start + T <= 0x7fffffffL && bm[3] >= 0 && bm[3] < max_batch, LSK_ESHAPE,
+    LSK_REQUIRE(T == 0 || (q_start >= 0 && q_start + T <= 0x7fffffffL && bm[3] >= 0 && bm[3] < max_batch), LSK_ESHAPE,
                 "%s: block %d starts at token %ld and is in row %d of %d", what, b, q_start, bm[3], max_batch);
     LSK_REQUIRE((pos0 + T + split - 1) / split <= ATTN_MAX_SPLITS, LSK_ESHAPE,
                 "%s: block %d needs more than %d splits of %d positions", what, b, ATTN_MAX_SPLITS, split);

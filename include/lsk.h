@@ -318,12 +318,12 @@ int lsk_kv8_read(int dtype, const void* k8, const void* v8, const void* k_exp, c
  * Beside lsk_ragged_attn (solutions/packed.py:142-166).
  *
  * lsk_cache_attn_plan (host pointers, no GPU work): blocks int32 [nb][4] = {q_start, pos0, T, row}, a row of the
- * cache's max_batch; split: positions per split, a multiple of 64, at most 128 splits per context.  tree: the launch
- * has a mask; then blocks of many rows share K / V among up to row_groups (1, 2, 4; 0: by the cache and the block)
- * groups of 32 rows.  n_slots: persistent workgroups, two per CU; recs: their items, and behind them the n_shared items
- * of four row groups (a workgroup each).  meta = [groups int32 n_groups*8][recs n_slots*n_rounds*8, then n_shared*8];
- * counts[9] = {tokens, n_groups, n_parts, n_rounds, tiles, part_rows, words of meta, row_groups used, n_shared}.  meta
- * == NULL: counts only; meta_cap too small: LSK_EWORKSPACE with counts written. */
+ * cache's max_batch (where T = 0 any); split: positions per split, a multiple of 64, at most 128 splits per context.
+ * tree: the launch has a mask; then blocks of many rows share K / V among up to row_groups (1, 2, 4; 0: by the cache
+ * and the block) groups of 32 rows.  n_slots: persistent workgroups, two per CU; recs: their items, and behind them the
+ * n_shared items of four row groups (a workgroup each).  meta = [groups int32 n_groups*8][recs n_slots*n_rounds*8, then
+ * n_shared*8]; counts[9] = {tokens, n_groups, n_parts, n_rounds, tiles, part_rows, words of meta, row_groups used,
+ * n_shared}.  meta == NULL: counts only; meta_cap too small: LSK_EWORKSPACE with counts written. */
 int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int max_batch, int n_kv_heads,
                         int head_dim, int kv8, int tree, int row_groups, int n_slots, int32_t* meta, long meta_cap,
                         long* counts);

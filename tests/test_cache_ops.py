@@ -1442,7 +1442,7 @@ def test_the_planner_refuses_rows_outside_the_cache():
     cnt = (ctypes.c_long * 9)()
     for kv8, tree in ((1, 0), (1, 1), (0, 1)):
         for q_start, row, T, want in ((0, 0, 3, 0), (7, 1, 3, 0), (0, 2, 3, -2), (0, -1, 3, -2), (-1, 0, 3, -2),
-                                      (0, 1 << 30, 0, -2), ((1 << 31) - 3, 0, 3, -2)):
+                                      (0, 1 << 30, 3, -2), ((1 << 31) - 3, 0, 3, -2), (-1, -1, 0, 0)):
             blk = (ctypes.c_int32 * 8)(0, 5, 0, 0, q_start, 40, T, row)
             assert lib.lsk_cache_attn_plan(blk, 2, 4, 256, 2, 2, 128, kv8, tree, 0, 256, None, 0, cnt) == want
 
