@@ -759,9 +759,8 @@ class AttnPlan:
             self._streams.add(stream.cuda_stream)
 
     def _join(self, dev: int) -> None:
-        """Before a launch on device dev's current stream: that stream waits for the records, and they outlive it."""
-        if _stream(dev) in self._streams:
-            return
+        """Before a first launch on device dev's current stream: that stream waits for the records, and they outlive it.
+        """
         with torch.cuda.device(dev):
             if torch.cuda.is_current_stream_capturing():
                 if not self._uploaded.query():       # (a capture cannot wait for work outside it)
@@ -816,7 +815,8 @@ def _plan_call(what: str, dev: int, q: torch.Tensor, plan: AttnPlan, launch, dim
     elif not workspace.is_contiguous():
         raise LskError(f"{what}: the workspace must be contiguous")
     ws_bytes = workspace.nbytes if workspace is not None else 0
-    plan._join(dev)
+    if _stream(dev) not in plan._streams:
+        plan._join(dev)
     return plan.scale if scale is None else float(scale), out, workspace, ws_bytes
 
 
