@@ -1,4 +1,4 @@
-// Verify / decode attention over an 8-bit KV cache, and over trees of drafted tokens.
+// Verify / decode attention over an 8-bit or 4-bit KV cache, and over trees of drafted tokens.
 //
 // Rule: token t of a block {q_start, pos0, T, row} sits in slot pos0 + t of its cache row (this call's K / V already
 // appended) and reads the slots 0 .. pos0 + t.  With a mask it reads, of the block's own slots pos0 .. pos0 + t, only
@@ -12,16 +12,19 @@
 // cache_attn_kernel, whose waves share the positions of up to two row groups of 32 rows, and cache_tree_kernel for
 // trees of more rows, whose waves share K and V.
 //
-// Both cache formats are read as 1 KiB fragments in lane order, 64 D bytes per block of STEP positions:
+// The cache formats are read as 1 KiB fragments in lane order, 64 D (4-bit: 32 D) bytes per block of STEP positions:
 //   bf16   STEP = 32: K fragment (a, f), lane 16 lg + l16: position 8 (l16 / 4) + 4 a + l16 % 4,
 //          d = 32 f + 8 lg .. + 7; V^T: row d, positions 8 lg .. + 7.
 //   8-bit  STEP = 64: e4m3 codes; K fragment (a, j): position 16 (l16 / 4) + 4 a + l16 % 4, d = 64 j + 16 lg .. + 15
 //          (two MFMA operands of 8 d each); V^T: row d, positions 16 lg .. + 15 (two operands of 8 positions each).
 //          A position's K and V are its codes times 2^(ks - 127) and 2^(vs - 127).
+//   4-bit  STEP = 64: e2m1 codes, a scale per 32 dims; the same positions, lane group lg of K with d = D / 4 lg .. + D / 4 -
+//          1 (D / 32 operands of 8 d each); V^T: rows d = 32 c + l16 and 32 c + 16 + l16, positions 16 lg .. + 15 of each.
 // Per step of a wave (v_mfma_f32_16x16x32_bf16): S^T[pos][q] = K Q^T, whose rows are mapped to positions so that lane
 // group lg ends up with the consecutive positions its V^T load needs; online softmax with fp32 statistics; O^T[d][q] +=
 // V^T P^T.  e4m3 values times a power of two are bf16 values, so the conversions in registers are exact and K's scale
-// costs nothing (the conversion takes one); V's scale, which differs per position, multiplies the weights.  The weights
+// costs nothing (the conversion takes one); V's scale, which differs per position, multiplies the weights (4-bit: once
+// for every 32 dims).  The weights
 // are rounded to bf16 for the second product, as the ragged attention's are (by at most 2^-8 each, independent of one
 // another: with the bf16 output's rounding the error against 64 bits is 0.0021 to 0.0023 of the outputs' size, where
 // fp32 weights leave 0.0017); the sum of the weights is taken before that rounding.
@@ -45,7 +48,7 @@ struct CacheAttnArgs {
   long q_st, q_sh;        // elements between tokens and between heads
   const void* kc;         // K and V cache of the layer
   const void* vc;
-  const uint8_t* ks;      // [B, Hkv, S] biased exponents (8-bit cache)
+  const uint8_t* ks;      // biased exponents: [B, Hkv, S] (8-bit cache), [B, Hkv, S / 64, D / 32, 64] (4-bit)
   const uint8_t* vs;
   const uint32_t* mask;   // [N, W]
   int W;
@@ -87,7 +90,41 @@ __device__ __forceinline__ lsk_bf16x8 codes_to_bf16(uint32_t x, uint32_t y, floa
   return (lsk_bf16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// 8 e2m1 codes -> bf16, times a power of two (exact; an exponent byte of 255 gives NaN)
+__device__ __forceinline__ lsk_bf16x8 codes4_to_bf16(uint32_t x, float scale) {
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  const bf2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, scale, 0);
+  const bf2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, scale, 1);
+  const bf2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, scale, 2);
+  const bf2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, scale, 3);
+  return (lsk_bf16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
 __device__ __forceinline__ float exp_bits(uint32_t byte) { return __uint_as_float(byte << 23); }
+// the exponent that byte i of four dwords holds
+__device__ __forceinline__ float exp_of(const lsk_i32x4& b, int i) {
+  return exp_bits(((uint32_t)b[i >> 2] >> (8 * (i & 3))) & 255u);
+}
+// 8 e2m1 codes of consecutive positions -> bf16, each times its own power of two (bytes 8 hv .. of b)
+__device__ __forceinline__ lsk_bf16x8 codes4_to_bf16(uint32_t x, const lsk_i32x4& b, int hv) {
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  lsk_bf16x8 r;
+#define CODES4_PAIR(I)                                                                            \
+  {                                                                                               \
+    const bf2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, exp_of(b, 8 * hv + 2 * I), I);     \
+    const bf2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, exp_of(b, 8 * hv + 2 * I + 1), I); \
+    r[2 * I] = lo[0];                                                                             \
+    r[2 * I + 1] = hi[1];                                                                         \
+  }
+  CODES4_PAIR(0) CODES4_PAIR(1) CODES4_PAIR(2) CODES4_PAIR(3)
+#undef CODES4_PAIR
+  return r;
+}
+
+// Cache formats, as lsk_cache_attn_plan numbers them
+#define FMT_BF16 0
+#define FMT_KV8 1
+#define FMT_KV4 2
 
 }  // namespace
 
@@ -103,20 +140,23 @@ __device__ __forceinline__ float exp_bits(uint32_t byte) { return __uint_as_floa
 struct Stripe {
   __amdgpu_buffer_rsrc_t k, v, ks, vs;
 };
-template <int D, bool KV8>
+template <int D, int FMT>
 __device__ __forceinline__ Stripe cache_stripe(const CacheAttnArgs& A, int crow, int kvh, int kv_hi) {
-  constexpr int STEP = KV8 ? 64 : 32;
+  constexpr int STEP = FMT == FMT_BF16 ? 32 : 64, BLK = (FMT == FMT_KV4 ? 32 : 64) * D;
+  constexpr int SPP = FMT == FMT_KV4 ? D / 32 : 1;   // scales of a position
   const long st = (long)crow * A.Hkv + kvh;
-  const long bytes = (long)(A.S / STEP) * 64 * D;    // of a whole stripe
+  const long bytes = (long)(A.S / STEP) * BLK;       // of a whole stripe
   const int end = min(A.S, (kv_hi + STEP - 1) / STEP * STEP);
   Stripe s;
-  s.k = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)A.kc + st * bytes), (short)0, end / STEP * 64 * D,
+  s.k = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)A.kc + st * bytes), (short)0, end / STEP * BLK,
                                           LSK_BUFFER_RSRC_WORD3);
-  s.v = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)A.vc + st * bytes), (short)0, end / STEP * 64 * D,
+  s.v = __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)A.vc + st * bytes), (short)0, end / STEP * BLK,
                                           LSK_BUFFER_RSRC_WORD3);
-  if constexpr (KV8) {
-    s.ks = __builtin_amdgcn_make_buffer_rsrc((void*)(A.ks + st * A.S), (short)0, end, LSK_BUFFER_RSRC_WORD3);
-    s.vs = __builtin_amdgcn_make_buffer_rsrc((void*)(A.vs + st * A.S), (short)0, end, LSK_BUFFER_RSRC_WORD3);
+  if constexpr (FMT != FMT_BF16) {
+    s.ks = __builtin_amdgcn_make_buffer_rsrc((void*)(A.ks + st * A.S * SPP), (short)0, end * SPP,
+                                             LSK_BUFFER_RSRC_WORD3);
+    s.vs = __builtin_amdgcn_make_buffer_rsrc((void*)(A.vs + st * A.S * SPP), (short)0, end * SPP,
+                                             LSK_BUFFER_RSRC_WORD3);
   }
   return s;
 }
@@ -155,11 +195,11 @@ __device__ __forceinline__ uint64_t clear_odd(lsk_i32x4 (&vr)[CT], int nk) {
 }
 
 // The non-finite values of V that clear_odd took out, for the rows that read them.
-template <bool KV8, bool TREE, int QT, int CT>
-__device__ __forceinline__ void add_odd(const CacheAttnArgs& A, __amdgpu_buffer_rsrc_t v, uint64_t odd, int sb,
+template <int FMT, bool TREE, int QT, int CT>
+__device__ __forceinline__ void add_odd(const CacheAttnArgs& A, const Stripe& st, uint64_t odd, int sb,
                                         int q_start, int pos0, const int (&qpos)[QT], lsk_f32x4 (&oacc)[QT][CT],
                                         int wide = 0) {
-  constexpr int STEP = KV8 ? 64 : 32, D = 16 * CT;
+  constexpr int STEP = FMT == FMT_BF16 ? 32 : 64, D = 16 * CT;
   const int lg = (threadIdx.x & 63) >> 4;
   while (odd != 0ull) {                              // (rare: one slot after the other, few registers)
     const int u = __builtin_ctzll(odd), kp = sb + u + (u & wide);  // (wide 0x18: groups of 8 slots, 16 apart)
@@ -178,14 +218,17 @@ __device__ __forceinline__ void add_odd(const CacheAttnArgs& A, __amdgpu_buffer_
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         ORDER();
-        // V[kp][16 c + 4 lg + i]: a dim's slots of a block are 64 bytes in both formats
-        const int so = kp / STEP * 64 * D + (16 * c + i) * 64 + kp % STEP * (KV8 ? 1 : 2);
+        // V[kp][16 c + 4 lg + i]: a dim's slots of a block are 64 bytes in bf16 and in 8 bits; in 4 bits NaN is a scale's
+        const int so = kp / STEP * 64 * D + (16 * c + i) * 64 + kp % STEP * (FMT == FMT_KV8 ? 1 : 2);
         float x;
-        if constexpr (KV8) {
-          const uint32_t b = __builtin_amdgcn_raw_buffer_load_b8(v, 256 * lg, so, 0);
+        if constexpr (FMT == FMT_KV4) {
+          const uint32_t b = __builtin_amdgcn_raw_buffer_load_b8(st.vs, 0, (kp / 64 * (D / 32) + c / 2) * 64 + kp % 64, 0);
+          x = b == 255u ? __builtin_nanf("") : 0.f;
+        } else if constexpr (FMT == FMT_KV8) {
+          const uint32_t b = __builtin_amdgcn_raw_buffer_load_b8(st.v, 256 * lg, so, 0);
           x = (b & 0x7fu) == 0x7fu ? __builtin_nanf("") : 0.f;
         } else {
-          x = bf2f((uint16_t)__builtin_amdgcn_raw_buffer_load_b16(v, 256 * lg, so, 0));
+          x = bf2f((uint16_t)__builtin_amdgcn_raw_buffer_load_b16(st.v, 256 * lg, so, 0));
           x = (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? x : 0.f;
         }
 #pragma unroll
@@ -197,10 +240,10 @@ __device__ __forceinline__ void add_odd(const CacheAttnArgs& A, __amdgpu_buffer_
 
 // The online softmax of one tile's 16 query columns over a step: s[a][e] are the scores of this lane's slots 4 a + e,
 // of which `reads` says what the column reads (FULL: all), vsr V's exponents of the slots (8-bit); pb the weights for
-// the second product.  A row's m only moves when a score passes it by more than LAG (weights up to 2^LAG; each row for
+// the second product (4-bit: s takes them, before V's scales).  A row's m only moves when a score passes it by more than LAG (weights up to 2^LAG; each row for
 // itself, so the rows of a tile stay independent), which is seldom after the first step: then no maximum crosses lanes
 // and nothing is rescaled.  Each lane sums its own slots' weights.
-template <bool KV8, bool FULL, int NA, int CT, int HV>
+template <int FMT, bool FULL, int NA, int CT, int HV>
 __device__ __forceinline__ void softmax_tile(lsk_f32x4 (&s)[NA], uint32_t reads, lsk_i32x4 vsr, float scale_log2,
                                              float& m, float& l, lsk_f32x4 (&o)[CT], lsk_bf16x8 (&pb)[HV]) {
   float mt = -INFINITY;
@@ -227,8 +270,12 @@ __device__ __forceinline__ void softmax_tile(lsk_f32x4 (&s)[NA], uint32_t reads,
     float pe = fast_exp2(__builtin_fmaf(s[i >> 2][i & 3], scale_log2, -m));
     if constexpr (!FULL) pe = (reads >> i) & 1u ? pe : 0.f;
     rs += pe;
+    if constexpr (FMT == FMT_KV4) {
+      s[i >> 2][i & 3] = pe;
+      continue;
+    }
     float pv = pe;
-    if constexpr (KV8) {
+    if constexpr (FMT == FMT_KV8) {
       pv = pe * exp_bits(((uint32_t)vsr[i >> 2] >> (8 * (i & 3))) & 255u);
       if constexpr (!FULL) pv = (reads >> i) & 1u ? pv : 0.f;  // (a slot never written: any exponent)
     }
@@ -242,14 +289,17 @@ __device__ __forceinline__ void softmax_tile(lsk_f32x4 (&s)[NA], uint32_t reads,
 // 46, of 960 81 against 91, of 4000 313 against 311; 7B heads, 16 trees of 30 nodes and 960 positions 30 against 36;
 // one request of 100000 positions, 1B heads, 25 against 23.
 #define CACHE_WAVES 4
-template <int D, int QT, bool KV8, bool TREE>
+template <int D, int QT, int FMT, bool TREE>
 __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const CacheAttnArgs A) {
-  constexpr int STEP = KV8 ? 64 : 32;                // positions per step of a wave
+  constexpr bool KV8 = FMT == FMT_KV8, KV4 = FMT == FMT_KV4, CODES = KV8 || KV4;
+  constexpr int STEP = CODES ? 64 : 32;              // positions per step of a wave
+  constexpr int BLK = (KV4 ? 32 : 64) * D;           // bytes of a step's K, and of its V
   constexpr int HV = STEP / 32;                      // 32-position halves of a step; a lane group has 8 slots of each
   constexpr int NE = 8 * HV;                         // slots of a lane group: NE consecutive ones
   constexpr uint32_t ALL = NE == 16 ? 0xffffu : 0xffu;
   constexpr int KF = D / 32;                         // K operands per 16-position tile
-  constexpr int CT = D / 16;                         // 16-byte loads per lane of a step, for K and for V
+  constexpr int CT = D / 16;                         // 16-row tiles of O^T
+  constexpr int LT = KV4 ? CT / 2 : CT;              // 16-byte loads per lane of a step, for K and for V
   constexpr int NW = CACHE_WAVES;
   constexpr int GR = 16 * QT;                        // rows of a wave
   constexpr bool QREG = QT == 1;                     // one tile: Q fragments in registers (items of one row group)
@@ -286,7 +336,9 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
   };
   auto row_base = [&](const Item& it) { return TREE ? (wave & ((1 << it.lr) - 1)) * GR : 0; };  // the wave's first row
   // Q: row rl of an item -> 8 elements from d; operand f's k index 8 lg + e stands for d = q_dim(f) + e
-  auto q_dim = [&](int f) { return KV8 ? 64 * (f >> 1) + 16 * lg + 8 * (f & 1) : 32 * f + 8 * lg; };
+  auto q_dim = [&](int f) {
+    return KV4 ? D / 4 * lg + 8 * f : KV8 ? 64 * (f >> 1) + 16 * lg + 8 * (f & 1) : 32 * f + 8 * lg;
+  };
   auto q_ptr = [&](const Item& it, int rl) {
     const int r = it.row0 + rl, t = r / G, g = r - t * G;
     return A.q + (long)(it.q_start + t) * A.q_st + (long)(it.kvh * G + g) * A.q_sh;
@@ -323,26 +375,34 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
       }
     }
   };
-  auto stripe = [&](const Item& it) { return cache_stripe<D, KV8>(A, it.crow, it.kvh, it.kv_hi); };
+  auto stripe = [&](const Item& it) { return cache_stripe<D, FMT>(A, it.crow, it.kvh, it.kv_hi); };
   // Non-temporal where each byte is read once (32 trees of 16 nodes, 7B heads, 960 positions of bf16: 95 us against
   // 80); not where two row groups read it (39 nodes: 111 us against 118)
   constexpr int AUX = TREE && QT == 2 ? 0 : 2;
   auto ld = [&](__amdgpu_buffer_rsrc_t rs, int vo, int so) -> lsk_i32x4 {
     return __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, vo, so, AUX));
   };
-  const int k_vo = 16 * lane, v_vo = 64 * l16 + 16 * lg;
-  lsk_i32x4 kr[CT], vr[CT], ksr, vsr;                // this step's K and V as loaded
-  constexpr int KL = CT / (2 * HV);                  // K loads of 16 slots
+  const int k_vo = 16 * lane, v_vo = KV4 ? 16 * lane : 64 * l16 + 16 * lg;
+  lsk_i32x4 kr[LT], vr[LT], ksr, vsr[KV4 ? D / 32 : 1];  // this step's K and V as loaded
+  // the K loads that the 16 slots of tile a are the last to need
   auto load_k = [&](const Stripe& s, int sb, int a) {
+    constexpr int PER = 2 * HV;                      // tiles of a step
 #pragma unroll
-    for (int i = a * KL; i < (a + 1) * KL; ++i) kr[i] = ld(s.k, k_vo, sb / STEP * 64 * D + i * 1024);
+    for (int i = a * LT / PER; i < (a + 1) * LT / PER; ++i) kr[i] = ld(s.k, k_vo, sb / STEP * BLK + i * 1024);
     if constexpr (KV8) {
       if (a == 2 * HV - 1) ksr = ld(s.ks, 16 * (l16 >> 2), sb);
     }
+    if constexpr (KV4) {                             // (a byte of the dword for each tile)
+      if (a == 2 * HV - 1)
+        ksr[0] = __builtin_amdgcn_raw_buffer_load_b32(s.ks, 64 * (D == 128 ? lg : lg >> 1) + 4 * l16, sb * (D / 32), AUX);
+    }
   };
-  auto load_v = [&](const Stripe& s, int sb, int c) { vr[c] = ld(s.v, v_vo, sb / STEP * 64 * D + c * 1024); };
+  auto load_v = [&](const Stripe& s, int sb, int c) { vr[c] = ld(s.v, v_vo, sb / STEP * BLK + c * 1024); };
   auto load_vs = [&](const Stripe& s, int sb) {
-    if constexpr (KV8) vsr = ld(s.vs, 16 * lg, sb);
+    if constexpr (KV8) vsr[0] = ld(s.vs, 16 * lg, sb);
+    if constexpr (KV4)
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) vsr[b] = ld(s.vs, 64 * b + 16 * lg, sb * (D / 32));
   };
   // a wave without rows starts past the stripe
   auto first_step = [&](const Item& it) {
@@ -356,7 +416,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
     for (int a = 0; a < 2 * HV; ++a) load_k(s, sb, a);
     load_vs(s, sb);
 #pragma unroll
-    for (int c = 0; c < CT; ++c) load_v(s, sb, c);
+    for (int c = 0; c < LT; ++c) load_v(s, sb, c);
   };
 
   Item cur = fetch(0);
@@ -405,8 +465,9 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
       // In a step that some row does not read whole, a slot whose V holds an infinity or NaN must not reach the rows
       // that do not read it (0 x NaN): the values past the item and the non-finite ones are cleared here, and the rows
       // that do read such a value get it after the products (below).
+      // (4-bit codes are finite: only a scale can be NaN, and it goes through the weights.)
       uint64_t odd = 0;                              // bit u: slot sb + u holds a non-finite value
-      if constexpr (!FULL) {
+      if constexpr (!FULL && !KV4) {
         odd = clear_odd<KV8>(vr, kv_hi - (sb + NE * lg));
       }
       // S^T = K Q^T, 16 slots at a time: sacc[qt][a][e] <-> slot s0 + 4 a + e.  The registers of a converted K take the
@@ -418,7 +479,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
       lsk_f32x4 sacc[QT][2 * HV];
 #pragma unroll
       for (int a = 0; a < 2 * HV; ++a) {
-        if constexpr (KV8) ORDER();
+        if constexpr (CODES) ORDER();
         lsk_bf16x8 kf[KF];
         if constexpr (KV8) {
           const float sc = exp_bits(((uint32_t)ksr[a] >> (8 * (l16 & 3))) & 255u);
@@ -427,6 +488,12 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
             const lsk_i32x4 x = kr[a * (KF / 2) + (f >> 1)];
             kf[f] = codes_to_bf16(x[2 * (f & 1)], x[2 * (f & 1) + 1], sc);
           }
+          ORDER();
+          load_k(sr, sn, a);
+        } else if constexpr (KV4) {
+          const float sc = exp_bits(((uint32_t)ksr[0] >> (8 * a)) & 255u);
+#pragma unroll
+          for (int f = 0; f < KF; ++f) kf[f] = codes4_to_bf16((uint32_t)kr[(a * KF + f) >> 2][(a * KF + f) & 3], sc);
           ORDER();
           load_k(sr, sn, a);
         } else {
@@ -446,23 +513,36 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
         }
       }
       ORDER();
-      if constexpr (!KV8) {
+      if constexpr (!CODES) {
 #pragma unroll
         for (int a = 0; a < 2 * HV; ++a) load_k(sr, sn, a);
       }
       lsk_bf16x8 pb[QT][HV];
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
-        if constexpr (KV8) ORDER();
-        softmax_tile<KV8, FULL>(sacc[qt], reads[qt], vsr, A.scale_log2, m_run[qt], l_run[qt], oacc[qt], pb[qt]);
+        if constexpr (CODES) ORDER();
+        softmax_tile<FMT, FULL>(sacc[qt], reads[qt], vsr[0], A.scale_log2, m_run[qt], l_run[qt], oacc[qt], pb[qt]);
       }
       ORDER();
-      load_vs(sr, sn);
+      if constexpr (!KV4) load_vs(sr, sn);
       // O^T += V^T P^T; V's registers take the next step's V one by one
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         lsk_bf16x8 vf[HV];
-        if constexpr (KV8) {
+        if constexpr (KV4) {
+          if (c % 2 == 0) {                          // the weights times the scales of these 32 dims
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+              for (int i = 0; i < NE; ++i) {
+                float pv = sacc[qt][i >> 2][i & 3] * exp_of(vsr[c / 2], i);
+                if constexpr (!FULL) pv = (reads[qt] >> i) & 1u ? pv : 0.f;  // (a slot not read: any scale)
+                pb[qt][i >> 3][i & 7] = static_cast<__bf16>(pv);
+              }
+          }
+#pragma unroll
+          for (int hv = 0; hv < HV; ++hv) vf[hv] = codes4_to_bf16((uint32_t)vr[c / 2][2 * (c & 1) + hv], 1.f);
+        } else if constexpr (KV8) {
 #pragma unroll
           for (int hv = 0; hv < HV; ++hv) vf[hv] = codes_to_bf16(vr[c][2 * hv], vr[c][2 * hv + 1], 1.f);
         } else {
@@ -473,11 +553,13 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt)
             oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[hv], pb[qt][hv], oacc[qt][c], 0, 0, 0);
-        load_v(sr, sn, c);
+        if constexpr (!KV4) load_v(sr, sn, c);
+        else if (c % 2 == 1) load_v(sr, sn, c / 2);
         ORDER();
       }
-      if constexpr (!FULL) {
-        add_odd<KV8, TREE>(A, sr.v, odd, sb, cur.q_start, cur.pos0, qpos, oacc);
+      if constexpr (KV4) load_vs(sr, sn);
+      if constexpr (!FULL && !KV4) {
+        add_odd<FMT, TREE>(A, sr, odd, sb, cur.q_start, cur.pos0, qpos, oacc);
       }
     };
     int sb = first_step(cur);
@@ -575,15 +657,17 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
 // workgroup of its own and all are resident at once (those 32 trees: 480 items, 23 to 28 us of such work a CU, 40 on
 // the fullest).
 #define TREE_WAVES 4
-template <int D, bool KV8>
+template <int D, int FMT>
 __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const CacheAttnArgs A,
                                                                         const int32_t* __restrict__ items) {
   constexpr int KF = D / 32, CT = D / 16, NW = TREE_WAVES, QT = 2;
-  constexpr int STEPS = KV8 ? 2 : 1, CHUNK = 32 * STEPS;  // steps and positions that go through LDS at a time
+  constexpr bool KV8 = FMT == FMT_KV8, KV4 = FMT == FMT_KV4, CODES = KV8 || KV4;
+  constexpr int STEPS = CODES ? 2 : 1, CHUNK = 32 * STEPS;  // steps and positions that go through LDS at a time
   constexpr int NE = 8;                              // slots of a lane in a step
   constexpr uint32_t ALL = 0xffu;
   constexpr int UNITS = 2 * CT;                      // 1 KiB bf16 fragments of a step: K's (a, f), then V's
-  constexpr int UPW = UNITS / NW;                    // fragments of a chunk, as they are in the cache, per wave
+  constexpr int LT = KV4 ? CT / 2 : CT;              // fragments of a chunk's K, and of its V, as they are in the cache
+  constexpr int UPW = 2 * LT / NW;                   // those of a wave
   constexpr int HALF = UNITS * 1024, BUF = STEPS * HALF;
   __shared__ __attribute__((aligned(16))) char s_buf[2 * BUF];
   __shared__ __attribute__((aligned(16))) uint8_t s_vs[2][64];
@@ -594,16 +678,26 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
   const int q_start = wk[0], row0 = wk[1], nrows = wk[2] & 1023, kvh = wk[2] >> 12;
   const int kv_lo = wk[3], kv_hi = wk[4], part = wk[5], pos0 = wk[6], crow = wk[7];
   const int rb = wave * 16 * QT;
-  const Stripe sr = cache_stripe<D, KV8>(A, crow, kvh, kv_hi);
+  const Stripe sr = cache_stripe<D, FMT>(A, crow, kvh, kv_hi);
   lsk_i32x4 st[UPW];                                 // the wave's part of the next chunk, in flight
   uint32_t st_ks[UPW], st_vs;                        // 8-bit: exponents of this lane's K, and of position `lane`
+  lsk_i32x4 st_s[UPW];                               // 4-bit: exponents of this lane's K (a dword) or V
   auto st_load = [&](int sb) {
 #pragma unroll
     for (int i = 0; i < UPW; ++i) {                  // (a wave's fragments are all of K or all of V)
       const int w = wave * UPW + i;
-      const int so = sb * (KV8 ? 1 : 2) * D + w % CT * 1024;
+      const int so = (KV4 ? sb / 2 : KV8 ? sb : 2 * sb) * D + w % LT * 1024;
       st[i] = __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                w < CT ? sr.k : sr.v, w < CT ? 16 * lane : 64 * l16 + 16 * lg, so, 0));
+                                                w < LT ? sr.k : sr.v, w < LT || KV4 ? 16 * lane : 64 * l16 + 16 * lg, so,
+                                                0));
+      if constexpr (KV4) {
+        if (w < LT)
+          st_s[i][0] = __builtin_amdgcn_raw_buffer_load_b32(sr.ks, 64 * (D == 128 ? lg : lg >> 1) + 4 * l16,
+                                                            sb * (D / 32), 0);
+        else
+          st_s[i] = __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                      sr.vs, 16 * lg, sb * (D / 32) + 64 * (w - LT), 0));
+      }
       if constexpr (KV8)
         st_ks[i] = __builtin_amdgcn_raw_buffer_load_b8(sr.ks, 16 * (l16 >> 2) + (l16 & 3),
                                                        sb + 4 * (w % CT / (KF / 2)), 0);
@@ -615,7 +709,20 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
 #pragma unroll
     for (int i = 0; i < UPW; ++i) {
       const int u = wave * UPW + i;
-      if constexpr (KV8) {                           // codes -> bf16, K with its scale: once for all the waves
+      if constexpr (KV4) {                           // both with their scales
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t x = (uint32_t)st[i][w];
+          if (u < LT) {                              // dword w: tile g / KF, operand g % KF
+            const int g = 4 * u + w, a = g / KF;
+            *(lsk_bf16x8*)(to + (a >> 1) * HALF + ((a & 1) * KF + g % KF) * 1024) =
+                codes4_to_bf16(x, exp_bits(((uint32_t)st_s[i][0] >> (8 * a)) & 255u));
+          } else {                                   // rows 32 (u - LT) + 16 (w / 2) + l16, positions 16 lg + 8 (w % 2) ..
+            *(lsk_bf16x8*)(to + (w & 1) * HALF + (CT + 2 * (u - LT) + (w >> 1)) * 1024) =
+                codes4_to_bf16(x, st_s[i], w & 1);
+          }
+        }
+      } else if constexpr (KV8) {                    // codes -> bf16, K with its scale: once for all the waves
         const float sc = u < CT ? exp_bits(st_ks[i]) : 1.f;
         const int a = u / (KF / 2), f = 2 * (u % (KF / 2));
         char* lo = to + (u < CT ? (a >> 1) * HALF + ((a & 1) * KF + f) * 1024 : u * 1024);
@@ -639,7 +746,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
     qpos[qt] = rl < nrows ? pos0 + t : -1;
 #pragma unroll
     for (int f = 0; f < KF; ++f) {
-      const int d = KV8 ? 64 * (f >> 1) + 16 * lg + 8 * (f & 1) : 32 * f + 8 * lg;
+      const int d = KV4 ? D / 4 * lg + 8 * f : KV8 ? 64 * (f >> 1) + 16 * lg + 8 * (f & 1) : 32 * f + 8 * lg;
       qf[qt][f] = __builtin_bit_cast(lsk_bf16x8, *(const lsk_u32x4_u*)(q + d));
     }
   }
@@ -656,7 +763,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
   auto step = [&](auto full_, int s2, int j, int buf) {
     constexpr bool FULL = decltype(full_)::value;
     const char* src = s_buf + buf * BUF + j * HALF + 16 * lane;
-    const int s0 = s2 + (KV8 ? 16 * lg + 8 * j : 32 * j + 8 * lg);
+    const int s0 = s2 + (CODES ? 16 * lg + 8 * j : 32 * j + 8 * lg);
     uint32_t reads[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
@@ -695,8 +802,8 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
     lsk_bf16x8 pb[QT][1];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
-      softmax_tile<KV8, FULL>(sacc[qt], reads[qt], vsr, A.scale_log2, m_run[qt], l_run[qt], oacc[qt], pb[qt]);
-    uint64_t odd = 0;                                // (V is bf16 here in both formats)
+      softmax_tile<KV4 ? FMT_BF16 : FMT, FULL>(sacc[qt], reads[qt], vsr, A.scale_log2, m_run[qt], l_run[qt], oacc[qt], pb[qt]);
+    uint64_t odd = 0;                                // (V is bf16 here in all formats)
     if constexpr (!FULL) odd = clear_odd<false>(vr, kv_hi - s0);
 #pragma unroll
     for (int c = 0; c < CT; ++c)
@@ -705,7 +812,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
         oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lsk_bf16x8, vr[c]), pb[qt][0],
                                                               oacc[qt][c], 0, 0, 0);
     if constexpr (!FULL)
-      add_odd<KV8, true>(A, sr.v, odd, s2 + (KV8 ? 8 : 32) * j, q_start, pos0, qpos, oacc, KV8 ? 0x18 : 0);
+      add_odd<FMT, true>(A, sr, odd, s2 + (CODES ? 8 : 32) * j, q_start, pos0, qpos, oacc, CODES ? 0x18 : 0);
   };
   st_write(0);
   st_load(kv_lo + CHUNK);
@@ -973,16 +1080,17 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 // The number of row groups follows from the block's rows and the cache alone, so it never makes a row's result depend
 // on the batch.  Items go longest first to the least-loaded of n_slots persistent workgroups, as in lsk_attn_schedule.
 static int cache_plan(const char* what, const int32_t* blocks, int nb, int group, int split, int max_batch,
-                      int n_kv_heads, int head_dim, int kv8, int tree, int row_groups, int n_slots, int32_t* meta,
+                      int n_kv_heads, int head_dim, int format, int tree, int row_groups, int n_slots, int32_t* meta,
                       long meta_cap, long* counts) {
   LSK_REQUIRE(counts && (blocks || nb == 0), LSK_EARG, "%s: null pointer", what);
   LSK_REQUIRE(nb >= 0 && group > 0 && split >= ATTN_TILE && split % ATTN_TILE == 0 && n_kv_heads > 0 &&
                   n_kv_heads < (1 << 19) && max_batch > 0 && n_slots > 0 && n_slots <= (1 << 16) &&
+                  format >= FMT_BF16 && format <= FMT_KV4 &&
                   (row_groups == 0 || row_groups == 1 || row_groups == 2 || row_groups == 4),
               LSK_ESHAPE, "%s: bad arguments (split a multiple of %d, row_groups 0, 1, 2 or 4)", what, ATTN_TILE);
   LSK_REQUIRE(head_dim == 64 || head_dim == 128, LSK_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128)", what,
               head_dim);
-  const int step = kv8 ? 64 : 32;
+  const int step = format == FMT_BF16 ? 32 : 64;
   long most = 0, n_tokens = 0;
   for (int b = 0; b < nb; ++b) {
     const int32_t* bm = blocks + (long)b * 4;
@@ -1075,11 +1183,11 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
 }
 
 extern "C" int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int max_batch, int n_kv_heads,
-                                   int head_dim, int kv8, int tree, int row_groups, int n_slots, int32_t* meta,
+                                   int head_dim, int format, int tree, int row_groups, int n_slots, int32_t* meta,
                                    long meta_cap, long* counts) {
   const char* what = "lsk_cache_attn_plan";
   try {
-    return cache_plan(what, blocks, nb, group, split, max_batch, n_kv_heads, head_dim, kv8, tree, row_groups, n_slots,
+    return cache_plan(what, blocks, nb, group, split, max_batch, n_kv_heads, head_dim, format, tree, row_groups, n_slots,
                       meta, meta_cap, counts);
   } catch (const std::exception&) {
     LSK_REQUIRE(false, LSK_EWORKSPACE, "%s: out of host memory", what);
@@ -1095,8 +1203,8 @@ extern "C" size_t lsk_cache_attn_workspace_bytes(int n_parts, int n_kv_heads, in
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// Checks and launches shared by the two entry points; kv8: the cache is 8-bit.
-static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t* groups, int n_groups, int n_parts,
+// Checks and launches shared by the entry points.
+static int cache_attn(const char* what, int format, CacheAttnArgs a, const int32_t* groups, int n_groups, int n_parts,
                       int n_slots, int n_shared, int tiles, int row_groups, int head_dim, float scale, void* workspace,
                       size_t ws_bytes, hipStream_t s) {
   LSK_REQUIRE(head_dim == 64 || head_dim == 128, LSK_EUNSUPPORTED, "%s: head_dim %d (supported: 64, 128)", what,
@@ -1109,7 +1217,7 @@ static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t
               "%s: a plan of %d slots, %d groups and %d partial slots", what, n_slots, n_groups, n_parts);
   LSK_REQUIRE(a.S % ATTN_TILE == 0 && (long)a.S * head_dim * 2 <= 0x7fffffffL, LSK_ESHAPE,
               "%s: max_seq %d (a multiple of %d, stripes below 2 GiB)", what, a.S, ATTN_TILE);
-  LSK_REQUIRE(aligned16(a.kc) && aligned16(a.vc) && (!kv8 || (aligned16(a.ks) && aligned16(a.vs))), LSK_EARG,
+  LSK_REQUIRE(aligned16(a.kc) && aligned16(a.vc) && (format == FMT_BF16 || (aligned16(a.ks) && aligned16(a.vs))), LSK_EARG,
               "%s: the cache tensors start at multiples of 16 bytes", what);
   if (n_parts > 0) {
     LSK_REQUIRE(a.part_rows >= 16 * tiles && a.part_rows <= 64 * tiles, LSK_EARG, "%s: a plan of %d rows per partial",
@@ -1124,28 +1232,36 @@ static int cache_attn(const char* what, bool kv8, CacheAttnArgs a, const int32_t
   LSK_REQUIRE(scale >= 0.f && scale <= 1e30f, LSK_EARG, "%s: scale %g (not negative)", what, (double)scale);
   a.scale_log2 = scale * 1.4426950408889634f;
   int rc = 0;
-#define LSK_CACHE_ATTN(DD, QT, K8, TR) cache_attn_kernel<DD, QT, K8, TR><<<n_slots, 64 * CACHE_WAVES, 0, s>>>(a)
-#define LSK_CACHE_ATTN_D(K8, TR)                                            \
-  do {                                                                      \
-    if (head_dim == 128 && tiles == 1) LSK_CACHE_ATTN(128, 1, K8, TR);      \
-    else if (head_dim == 128) LSK_CACHE_ATTN(128, 2, K8, TR);               \
-    else if (tiles == 1) LSK_CACHE_ATTN(64, 1, K8, TR);                     \
-    else if (tiles == 2) LSK_CACHE_ATTN(64, 2, K8, TR);                     \
+#define LSK_CACHE_ATTN(DD, QT, F, TR) cache_attn_kernel<DD, QT, F, TR><<<n_slots, 64 * CACHE_WAVES, 0, s>>>(a)
+#define LSK_CACHE_ATTN_D(F, TR)                                            \
+  do {                                                                     \
+    if (head_dim == 128 && tiles == 1) LSK_CACHE_ATTN(128, 1, F, TR);      \
+    else if (head_dim == 128) LSK_CACHE_ATTN(128, 2, F, TR);               \
+    else if (tiles == 1) LSK_CACHE_ATTN(64, 1, F, TR);                     \
+    else if (tiles == 2) LSK_CACHE_ATTN(64, 2, F, TR);                     \
   } while (0)
   if (a.n_rounds == 0) ;
-  else if (!kv8) LSK_CACHE_ATTN_D(false, true);
-  else if (a.mask != nullptr) LSK_CACHE_ATTN_D(true, true);
-  else if (tiles == 3) LSK_CACHE_ATTN(64, 3, true, false);
-  else LSK_CACHE_ATTN_D(true, false);
+  else if (format == FMT_BF16) LSK_CACHE_ATTN_D(FMT_BF16, true);
+  else if (format == FMT_KV8 && a.mask != nullptr) LSK_CACHE_ATTN_D(FMT_KV8, true);
+  else if (format == FMT_KV4 && a.mask != nullptr) LSK_CACHE_ATTN_D(FMT_KV4, true);
+  else if (format == FMT_KV8 && tiles == 3) LSK_CACHE_ATTN(64, 3, FMT_KV8, false);
+  else if (format == FMT_KV8) LSK_CACHE_ATTN_D(FMT_KV8, false);
+  else if (tiles == 3) LSK_CACHE_ATTN(64, 3, FMT_KV4, false);
+  else LSK_CACHE_ATTN_D(FMT_KV4, false);
 #undef LSK_CACHE_ATTN_D
 #undef LSK_CACHE_ATTN
   if (a.n_rounds > 0 && (rc = lsk_check_launch(what))) return rc;
   if (n_shared > 0) {
     const int32_t* items = a.recs + 8L * n_slots * a.n_rounds;
-    if (head_dim == 128 && kv8) cache_tree_kernel<128, true><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
-    else if (head_dim == 128) cache_tree_kernel<128, false><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
-    else if (kv8) cache_tree_kernel<64, true><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
-    else cache_tree_kernel<64, false><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
+#define LSK_CACHE_TREE(F)                                                                            \
+  do {                                                                                               \
+    if (head_dim == 128) cache_tree_kernel<128, F><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);   \
+    else cache_tree_kernel<64, F><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);                    \
+  } while (0)
+    if (format == FMT_BF16) LSK_CACHE_TREE(FMT_BF16);
+    else if (format == FMT_KV8) LSK_CACHE_TREE(FMT_KV8);
+    else LSK_CACHE_TREE(FMT_KV4);
+#undef LSK_CACHE_TREE
     if ((rc = lsk_check_launch(what))) return rc;
   }
   if (n_groups == 0) return 0;
@@ -1168,26 +1284,46 @@ static int shape_args(const char* what, const void* q, const void* kc, const voi
   return 0;
 }
 
-extern "C" int lsk_kv8_attn(const void* q, long q_stride_t, long q_stride_h, const void* k8, const void* v8,
-                            const void* k_exp, const void* v_exp, const uint32_t* mask, int mask_words,
-                            const int32_t* groups, int n_groups, int n_parts, const int32_t* recs, int n_rounds,
-                            int n_slots, int n_shared, int tiles, int row_groups, int part_rows, void* out, int n_heads,
-                            int n_kv_heads, int head_dim, int max_seq, float scale, void* workspace, size_t ws_bytes,
-                            void* stream) {
-  const char* what = "lsk_kv8_attn";
-  if (int rc = shape_args(what, q, k8, v8, out, n_heads, n_kv_heads, head_dim, max_seq, q_stride_t, q_stride_h))
-    return rc;
+// lsk_kv8_attn and lsk_kv4_attn
+static int codes_attn(const char* what, int format, const void* q, long q_st, long q_sh, const void* kc, const void* vc,
+                      const void* k_exp, const void* v_exp, const uint32_t* mask, int mask_words, const int32_t* groups,
+                      int n_groups, int n_parts, const int32_t* recs, int n_rounds, int n_slots, int n_shared, int tiles,
+                      int row_groups, int part_rows, void* out, int n_heads, int n_kv_heads, int head_dim, int max_seq,
+                      float scale, void* workspace, size_t ws_bytes, void* stream) {
+  if (int rc = shape_args(what, q, kc, vc, out, n_heads, n_kv_heads, head_dim, max_seq, q_st, q_sh)) return rc;
   LSK_REQUIRE(k_exp && v_exp && (mask == nullptr || mask_words > 0), LSK_EARG, "%s: null scales or an empty mask",
               what);
   LSK_REQUIRE(n_rounds >= 0 && n_shared >= 0, LSK_EARG, "%s: a plan of %d rounds and %d shared items", what, n_rounds,
               n_shared);
   if (n_rounds == 0 && n_shared == 0) return 0;
   LSK_REQUIRE(recs != nullptr, LSK_EARG, "%s: null pointer", what);
-  const CacheAttnArgs a = {(const uint16_t*)q, q_stride_t, q_stride_h, k8, v8, (const uint8_t*)k_exp,
-                           (const uint8_t*)v_exp, mask, mask_words, recs, n_rounds, (uint16_t*)out, nullptr, nullptr,
-                           part_rows, n_heads / n_kv_heads, n_kv_heads, max_seq, 0.f};
-  return cache_attn(what, true, a, groups, n_groups, n_parts, n_slots, n_shared, tiles, row_groups, head_dim, scale,
+  const CacheAttnArgs a = {(const uint16_t*)q, q_st, q_sh, kc, vc, (const uint8_t*)k_exp, (const uint8_t*)v_exp, mask,
+                           mask_words, recs, n_rounds, (uint16_t*)out, nullptr, nullptr, part_rows,
+                           n_heads / n_kv_heads, n_kv_heads, max_seq, 0.f};
+  return cache_attn(what, format, a, groups, n_groups, n_parts, n_slots, n_shared, tiles, row_groups, head_dim, scale,
                     workspace, ws_bytes, (hipStream_t)stream);
+}
+
+extern "C" int lsk_kv8_attn(const void* q, long q_stride_t, long q_stride_h, const void* k8, const void* v8,
+                            const void* k_exp, const void* v_exp, const uint32_t* mask, int mask_words,
+                            const int32_t* groups, int n_groups, int n_parts, const int32_t* recs, int n_rounds,
+                            int n_slots, int n_shared, int tiles, int row_groups, int part_rows, void* out, int n_heads,
+                            int n_kv_heads, int head_dim, int max_seq, float scale, void* workspace, size_t ws_bytes,
+                            void* stream) {
+  return codes_attn("lsk_kv8_attn", FMT_KV8, q, q_stride_t, q_stride_h, k8, v8, k_exp, v_exp, mask, mask_words, groups,
+                    n_groups, n_parts, recs, n_rounds, n_slots, n_shared, tiles, row_groups, part_rows, out, n_heads,
+                    n_kv_heads, head_dim, max_seq, scale, workspace, ws_bytes, stream);
+}
+
+extern "C" int lsk_kv4_attn(const void* q, long q_stride_t, long q_stride_h, const void* k4, const void* v4,
+                            const void* k_exp, const void* v_exp, const uint32_t* mask, int mask_words,
+                            const int32_t* groups, int n_groups, int n_parts, const int32_t* recs, int n_rounds,
+                            int n_slots, int n_shared, int tiles, int row_groups, int part_rows, void* out, int n_heads,
+                            int n_kv_heads, int head_dim, int max_seq, float scale, void* workspace, size_t ws_bytes,
+                            void* stream) {
+  return codes_attn("lsk_kv4_attn", FMT_KV4, q, q_stride_t, q_stride_h, k4, v4, k_exp, v_exp, mask, mask_words, groups,
+                    n_groups, n_parts, recs, n_rounds, n_slots, n_shared, tiles, row_groups, part_rows, out, n_heads,
+                    n_kv_heads, head_dim, max_seq, scale, workspace, ws_bytes, stream);
 }
 
 extern "C" int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_stride_h, const void* kcache,
@@ -1211,7 +1347,7 @@ extern "C" int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_s
     const CacheAttnArgs a = {(const uint16_t*)q, q_stride_t, q_stride_h, kcache, vcache, nullptr, nullptr, mask,
                              mask_words, recs, n_rounds, (uint16_t*)out, nullptr, nullptr, part_rows, G, n_kv_heads,
                              max_seq, 0.f};
-    return cache_attn(what, false, a, groups, n_groups, n_parts, n_slots, n_shared, tiles, row_groups, head_dim, scale,
+    return cache_attn(what, FMT_BF16, a, groups, n_groups, n_parts, n_slots, n_shared, tiles, row_groups, head_dim, scale,
                       workspace, ws_bytes, s);
   }
   LSK_REQUIRE(n_works >= 0 && rows_cap > 0 && rows_cap % 16 == 0 && rows_cap <= ATTN_ROWS, LSK_EARG,

@@ -13,6 +13,7 @@
 #define LSK_DTYPE_F32 0
 #define LSK_DTYPE_BF16 1
 #define LSK_DTYPE_KV8 2  // an 8-bit KV cache (lsk_kv8_append); not a tensor dtype
+#define LSK_DTYPE_KV4 4  // a 4-bit KV cache (lsk_kv4_append); not a tensor dtype
 
 typedef __bf16 lsk_bf16x8 __attribute__((ext_vector_type(8)));
 typedef short lsk_s16x4 __attribute__((ext_vector_type(4)));
@@ -159,6 +160,10 @@ int lsk_gemm_partial_af(const void* A, const void* W, float* P, int M, int N, in
 // 16-token groups) for the w2 launch.
 int lsk_gemm_silu_af(const void* A, const void* W, void* H, int h_frag, int M, int ffn, int K, void* stream);
 bool lsk_gemm_residual_covers(int M, int N, int K, int ks);
+// lsk_kv_compact's launch for a 4-bit cache, arguments checked
+int lsk_kv4_compact(void* kc, void* vc, void* ks, void* vs, int n_layers, const int32_t* rows, const int32_t* pos0,
+                    const int64_t* acc, const int32_t* path, int nb, int max_nodes, int n_kv_heads, int head_dim,
+                    int max_batch, int max_seq, hipStream_t s);
 int lsk_ragged_attn_impl(int dtype, const void* q, const void* kcache, const void* vcache, const int32_t* blocks,
                          const int32_t* works, int n_works, const int32_t* groups, int n_groups, int n_parts,
                          const int32_t* recs, int n_rounds, int n_slots, int rows_cap, void* out, int out_frag,

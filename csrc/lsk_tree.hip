@@ -321,13 +321,13 @@ extern "C" int lsk_kv_compact(int dtype, void* kcache, void* vcache, void* k_exp
                               void* stream) {
   const char* what = "lsk_kv_compact";
   LSK_REQUIRE(kcache && vcache && rows && pos0 && accepted && path, LSK_EARG, "%s: null pointer", what);
-  LSK_REQUIRE(dtype == LSK_DTYPE_F32 || dtype == LSK_DTYPE_BF16 || dtype == LSK_DTYPE_KV8, LSK_EUNSUPPORTED,
-              "%s: dtype %d", what, dtype);
-  LSK_REQUIRE(dtype != LSK_DTYPE_KV8 || (k_exp && v_exp), LSK_EARG, "%s: null exponents", what);
+  const bool codes = dtype == LSK_DTYPE_KV8 || dtype == LSK_DTYPE_KV4;
+  LSK_REQUIRE(dtype == LSK_DTYPE_F32 || dtype == LSK_DTYPE_BF16 || codes, LSK_EUNSUPPORTED, "%s: dtype %d", what, dtype);
+  LSK_REQUIRE(!codes || (k_exp && v_exp), LSK_EARG, "%s: null exponents", what);
   LSK_REQUIRE(n_layers >= 0 && n_layers <= 65535 && nb >= 0 && max_nodes > 0 && n_kv_heads > 0 && n_kv_heads <= 65535 &&
-                  max_batch > 0 && max_seq > 0 && max_seq % (dtype == LSK_DTYPE_KV8 ? 64 : 32) == 0,
+                  max_batch > 0 && max_seq > 0 && max_seq % (codes ? 64 : 32) == 0,
               LSK_ESHAPE, "%s: bad shape", what);
-  LSK_REQUIRE(dtype != LSK_DTYPE_KV8 || (((uintptr_t)kcache | (uintptr_t)vcache) & 15) == 0, LSK_EARG,
+  LSK_REQUIRE(!codes || (((uintptr_t)kcache | (uintptr_t)vcache) & 15) == 0, LSK_EARG,
               "%s: the cache tensors start at multiples of 16 bytes", what);
   if (nb == 0 || n_layers == 0) return 0;
   const dim3 grid(nb, n_kv_heads, n_layers);
@@ -348,7 +348,9 @@ extern "C" int lsk_kv_compact(int dtype, void* kcache, void* vcache, void* k_exp
     LSK_REQUIRE(head_dim == 64 || head_dim == 128, LSK_EUNSUPPORTED, "%s: head_dim %d", what, head_dim);
     if (dtype == LSK_DTYPE_F32) LSK_COMPACT_D(0);
     else if (dtype == LSK_DTYPE_BF16) LSK_COMPACT_D(1);
-    else LSK_COMPACT_D(2);
+    else if (dtype == LSK_DTYPE_KV8) LSK_COMPACT_D(2);
+    else return lsk_kv4_compact(kcache, vcache, k_exp, v_exp, n_layers, rows, pos0, accepted, path, nb, max_nodes,
+                                n_kv_heads, head_dim, max_batch, max_seq, s);
   }
 #undef LSK_COMPACT_D
 #undef LSK_COMPACT

@@ -5,7 +5,7 @@
  *
  * Conventions
  *   - dtype codes: LSK_DTYPE_F32 (0) and LSK_DTYPE_BF16 (1); bf16 is torch.bfloat16 storage.  lsk_kv_compact also
- *     takes LSK_DTYPE_KV8 (2), the 8-bit KV cache.
+ *     takes LSK_DTYPE_KV8 (2) and LSK_DTYPE_KV4 (4), the 8-bit and 4-bit KV caches.
  *   - All pointers are device pointers unless stated; the library never allocates or frees
  *     device memory: tensors and workspaces belong to the caller (the PyTorch caching allocator).
  *   - `stream` is a hipStream_t; every call is asynchronous on it, nothing synchronises inside.
@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define LSK_ABI_VERSION 14
+#define LSK_ABI_VERSION 15
 
 #define LSK_EPI_NONE 0     /* C = rnd(A W^T)                                   */
 #define LSK_EPI_RESIDUAL 1 /* C = rnd(R + rnd(A W^T))                          */
@@ -319,13 +319,13 @@ int lsk_kv8_read(int dtype, const void* k8, const void* v8, const void* k_exp, c
  *
  * lsk_cache_attn_plan (host pointers, no GPU work): blocks int32 [nb][4] = {q_start, pos0, T, row}, a row of the
  * cache's max_batch (where T = 0 any); split: positions per split, a multiple of 64, at most 128 splits per context.
- * tree: the launch has a mask; then blocks of many rows share K / V among up to row_groups (1, 2, 4; 0: by the cache
+ * format: 0 for bf16, 1 for 8-bit and 2 for 4-bit caches.  tree: the launch has a mask; then blocks of many rows share K / V among up to row_groups (1, 2, 4; 0: by the cache
  * and the block) groups of 32 rows.  n_slots: persistent workgroups, two per CU; recs: their items, and behind them the
  * n_shared items of four row groups (a workgroup each).  meta = [groups int32 n_groups*8][recs n_slots*n_rounds*8, then
  * n_shared*8]; counts[9] = {tokens, n_groups, n_parts, n_rounds, tiles, part_rows, words of meta, row_groups used,
  * n_shared}.  meta == NULL: counts only; meta_cap too small: LSK_EWORKSPACE with counts written. */
 int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int max_batch, int n_kv_heads,
-                        int head_dim, int kv8, int tree, int row_groups, int n_slots, int32_t* meta, long meta_cap,
+                        int head_dim, int format, int tree, int row_groups, int n_slots, int32_t* meta, long meta_cap,
                         long* counts);
 size_t lsk_cache_attn_workspace_bytes(int n_parts, int n_kv_heads, int part_rows, int head_dim);
 int lsk_kv8_attn(const void* q, long q_stride_t, long q_stride_h, const void* k8, const void* v8, const void* k_exp,
@@ -338,6 +338,69 @@ int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_stride_h, co
                   const int32_t* groups, int n_groups, int n_parts, const int32_t* recs, int n_rounds, int n_slots,
                   int n_shared, int tiles, int row_groups, int part_rows, void* out, int n_heads, int n_kv_heads,
                   int head_dim, int max_seq, float scale, void* workspace, size_t ws_bytes, void* stream);
+
+/* ---- 4-bit KV cache (no counterpart in the reference, whose cache is the model's dtype) ----
+ * 32 consecutive dims of one token's K (V) of one KV head: 32 e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives) and a power-of-two scale 2^e held as the byte e + 127:
+ *   amax = largest |x|, e = smallest integer >= -125 with amax <= 7 * 2^e (0 for amax = 0),
+ *   code = x * 2^-e rounded to e2m1, nearest even, at most 6 (at e = 126 at most 3),  value = code * 2^e: finite for
+ *   finite x.  32 dims that hold a NaN or an infinity are NaN as a whole (the byte 255, zero codes).
+ * Storage of a layer (head_dim D = 64 or 128, S = max_seq a multiple of 64, k4 and v4 at multiples of 16 bytes, for
+ * lsk_kv4_attn the exponents too); of two codes in a byte the lower half comes first:
+ *   k4 [B, Hkv, S/64, D/32, 64, 16] bytes: position 16 q + 4 a + r of a 64-position block, dims D/4 lg .. D/4 (lg + 1) - 1
+ *      are the 16 bytes of lane 16 lg + 4 q + r in fragment a (D = 128), or half a % 2 of them in fragment a / 2 (D = 64);
+ *   v4 [B, Hkv, S/64, D/32, 64, 16] bytes: positions 16 lg .. + 15 of dim 32 c + 16 h + l are half h of lane 16 lg + l's
+ *      bytes in fragment c;
+ *   k_exp [B, Hkv, S/64, D/32, 16, 4] bytes: [4 q + r][a];   v_exp [B, Hkv, S/64, D/32, 64]: [position].
+ *
+ * lsk_kv4_append, lsk_kv4_read: as lsk_kv8_append and lsk_kv8_read.  Two positions share a byte of V: tokens written side
+ * by side in one call do not disturb each other; calls that overlap (on two streams) have to write different 16-position
+ * groups of a row.
+ * lsk_kv4_attn: lsk_kv8_attn over a layer's 4-bit cache, with a plan of format 2.  A NaN in 32 dims of V reaches those
+ * dims of the rows that read it, one of K the rows.  lsk_kv_compact takes LSK_DTYPE_KV4.
+ * Beside lsk_kv_append and lsk_ragged_attn (solutions/packed.py:142-166, 180-181). */
+int lsk_kv4_append(int dtype, const void* k, const void* v, long stride_t, long stride_h, void* k4, void* v4,
+                   void* k_exp, void* v_exp, const int32_t* rows, const int32_t* pos, int n_tokens, int n_kv_heads,
+                   int head_dim, int max_batch, int max_seq, void* stream);
+int lsk_kv4_read(int dtype, const void* k4, const void* v4, const void* k_exp, const void* v_exp, const int32_t* rows,
+                 const int32_t* pos, void* k, void* v, int n_tokens, int n_kv_heads, int head_dim, int max_batch,
+                 int max_seq, void* stream);
+int lsk_kv4_attn(const void* q, long q_stride_t, long q_stride_h, const void* k4, const void* v4, const void* k_exp,
+                 const void* v_exp, const uint32_t* mask, int mask_words, const int32_t* groups, int n_groups,
+                 int n_parts, const int32_t* recs, int n_rounds, int n_slots, int n_shared, int tiles, int row_groups,
+                 int part_rows, void* out, int n_heads, int n_kv_heads, int head_dim, int max_seq, float scale,
+                 void* workspace, size_t ws_bytes, void* stream);
+
+/* ---- norms of queries and keys (the reference's models have none) ----
+ * qkv: rows of (n_heads + 2 n_kv_heads) head_dim elements, ld apart.  Every query and key head is normalised
+ * (x * rsqrt(mean(x^2) + eps) * w, w_q and w_k [head_dim] of qkv's dtype) and rotated by its position's rows of the fp32
+ * tables [tab_len, head_dim]; fp32 until the one rounding of the result.  q_out [n_tokens, n_heads, head_dim].  Either
+ * k_out [n_tokens, n_kv_heads, head_dim] (rows and the caches NULL; values are not read), or K and the values go to
+ * (rows[t], pos[t]) of the caches in lsk_rope_append's layouts.  A token outside the tables or the cache writes nothing.
+ * head_dim 32, 64, 128 or 256; max_seq a multiple of 32.  All tensors may start at any address that aligns their elements.
+ * Beside lsk_rope_append (solutions/packed.py:176-181). */
+int lsk_qk_norm_rope(int dtype, const void* qkv, long ld, const void* w_q, const void* w_k, float eps,
+                     const float* cos_tab, const float* sin_tab, int tab_len, const int32_t* rows, const int32_t* pos,
+                     int n_tokens, int n_heads, int n_kv_heads, int head_dim, void* q_out, void* k_out, void* kcache,
+                     void* vcache, int max_batch, int max_seq, void* stream);
+
+/* ---- 8-bit integer projections (the reference multiplies in the model's dtype) ----
+ * A row x of K values (a token's activations, an output channel's weights): amax = max |x|, codes rne(x fl(127 / amax)),
+ * scale fl(amax / 127); a row that holds a NaN or an infinity has the scale NaN, one with amax < 2^-100 the scale 0.
+ * Packed codes of R rows: (R+15)/16 * (K+63)/64 fragments of 1 KiB at a multiple of 16 bytes; lane 16 lg + l16 of
+ * fragment (g, j) = row 16 g + l16, k = 64 j + 16 lg .. + 15; fragments ordered [g][j].  K <= 131072.
+ *
+ * lsk_quant_rows_i8: x [M, K] (bf16 or fp32, ldx) -> packed codes (zeros past K; rows past M in the last group are not
+ * written) and scales [M].  lsk_pack_i8 / lsk_unpack_i8: codes [N, K] row-major <-> packed (zeros past N and K).
+ * lsk_gemm_i8: C[m][n] = epilogue(a_scales[m] w_scales[n] sum_k A[m][k] W[n][k]), the sum exact, the rest fp32 with one
+ * rounding: LSK_EPI_NONE, LSK_EPI_RESIDUAL (+ R) or LSK_EPI_SILU_MUL (W of 2 ffn rows [gate; up], N == ffn a multiple of
+ * 16: silu(g) u).  C and R [M, N] of `dtype`.  A result does not depend on what else is in the launch.
+ * Beside lsk_gemm (solutions/packed.py:175, 182-185). */
+int lsk_quant_rows_i8(int dtype, const void* x, long ldx, void* codes, float* scales, int M, int K, void* stream);
+int lsk_pack_i8(const void* codes, long ld, void* packed, int N, int K, void* stream);
+int lsk_unpack_i8(const void* packed, void* codes, long ld, int N, int K, void* stream);
+int lsk_gemm_i8(int dtype, const void* A, const float* a_scales, const void* W, const float* w_scales, void* C, long ldc,
+                const void* R, long ldr, int M, int N, int K, int epilogue, int ffn, void* stream);
 
 /* ---- trees of drafted tokens (the reference drafts chains) ----
  * A block's nodes are its tokens 0 .. lens[b] - 1 from starts[b]; node 0 is the root (the last committed token),
@@ -358,7 +421,7 @@ int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_stride_h, co
  *
  * lsk_kv_compact: slot pos0[b] + j of cache row rows[b] takes what slot pos0[b] + path[b][j] holds, j = 1 ..
  * accepted[b] (negative: none), in every layer and KV head (caches [n_layers, max_batch, ...], contiguous; k_exp, v_exp
- * for LSK_DTYPE_KV8, else NULL); then lsk_kv_rollback's pointer update holds as for a chain.  path as lsk_tree_accept
+ * for LSK_DTYPE_KV8 and LSK_DTYPE_KV4, else NULL); then lsk_kv_rollback's pointer update holds as for a chain.  path as lsk_tree_accept
  * writes it (increasing); the rows of a call have to differ.  Blocks outside the cache are skipped.  V's neighbouring
  * slots of a moved one (16 bytes) are written back as they were. */
 int lsk_tree_masks(const int32_t* parents, const int32_t* starts, const int32_t* lens, int nb, int n_tokens,

@@ -21,11 +21,12 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liblsk.so"
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_KV8 = 2             # an 8-bit KV cache, where an entry point takes one
+DTYPE_KV4 = 4             # a 4-bit KV cache
 EPI_NONE, EPI_RESIDUAL, EPI_SILU_MUL = 0, 1, 2
 EPI_PARTIAL, EPI_ARGMAX, EPI_QKV_ROPE = 3, 4, 5   # launch kinds known to lsk_gemm_wide_config
 ATTN_SPLIT = 8192         # LSK_ATTN_SPLIT
 ATTN_ROWS = 48            # query rows per attention work item (csrc/lsk_attention.hip ATTN_ROWS)
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 # name -> (restype, argtypes)
 _P, _I, _L, _F, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float, ctypes.c_size_t
@@ -84,6 +85,15 @@ _SIGS = {
                           _P]),
     "lsk_tree_attn": (_I, [_I, _P, _L, _L, _P, _P, _P, _I, _P, _I, _I, _P, _I, _I, _P] + [_I] * 6 + [_P] + [_I] * 4 +
                       [_F, _P, _Z, _P]),
+    "lsk_kv4_append": (_I, [_I, _P, _P, _L, _L] + [_P] * 6 + [_I] * 5 + [_P]),
+    "lsk_kv4_read": (_I, [_I] + [_P] * 8 + [_I] * 5 + [_P]),
+    "lsk_kv4_attn": (_I, [_P, _L, _L] + [_P] * 5 + [_I, _P, _I, _I, _P] + [_I] * 6 + [_P] + [_I] * 4 + [_F, _P, _Z,
+                          _P]),
+    "lsk_qk_norm_rope": (_I, [_I, _P, _L, _P, _P, _F, _P, _P, _I, _P, _P] + [_I] * 4 + [_P] * 4 + [_I, _I, _P]),
+    "lsk_quant_rows_i8": (_I, [_I, _P, _L, _P, _P, _I, _I, _P]),
+    "lsk_pack_i8": (_I, [_P, _L, _P, _I, _I, _P]),
+    "lsk_unpack_i8": (_I, [_P, _P, _L, _I, _I, _P]),
+    "lsk_gemm_i8": (_I, [_I] + [_P] * 5 + [_L, _P, _L] + [_I] * 5 + [_P]),
     "lsk_tree_masks": (_I, [_P, _P, _P, _I, _I, _I, _P, _I, _P, _P]),
     "lsk_tree_accept": (_I, [_P] * 5 + [_I, _I, _I] + [_P] * 4),
     "lsk_kv_compact": (_I, [_I] + [_P] * 4 + [_I] + [_P] * 4 + [_I] * 6 + [_P]),
@@ -618,48 +628,133 @@ class KV8(_KV8):
         return self._checked[1]
 
 
-def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor) -> None:
-    """k, v [N, Hkv, D] (bf16 or fp32, of equal strides; dims contiguous) quantised into a layer's 8-bit cache at
-    (rows, pos).  Tokens outside the cache are skipped; the (row, position) pairs of a call have to differ."""
+class _KV4(NamedTuple):
+    k: torch.Tensor
+    v: torch.Tensor
+    ks: torch.Tensor
+    vs: torch.Tensor
+
+
+class KV4(_KV4):
+    """A 4-bit K / V cache (lsk_kv4_append): e2m1 codes and one power-of-two scale per position, KV head and 32 dims, the
+    byte e + 127.  A layer's tensors, or with a leading layer axis those of several, all uint8:
+      k and v [B, Hkv, S/64, D/32, 64, 16], ks [B, Hkv, S/64, D/32, 16, 4] and vs [B, Hkv, S/64, D/32, 64].
+    The tensors' types and shapes are checked by the object's first use; they have to stay as they are."""
+    _checked = None                                   # (layers, dims) that the tensors were found to fit
+
+    @classmethod
+    def zeros(cls, max_batch: int, n_kv_heads: int, max_seq: int, head_dim: int, device, layers: int | None = None):
+        if head_dim not in (64, 128) or max_seq % 64 or max_seq <= 0:
+            raise ValueError(f"4-bit caches need head_dim 64 or 128 and max_seq a multiple of 64 (got {head_dim}, "
+                             f"{max_seq})")
+        lead = (max_batch, n_kv_heads) if layers is None else (layers, max_batch, n_kv_heads)
+        lead = (*lead, max_seq // 64, head_dim // 32)
+        byte = dict(dtype=torch.uint8, device=device)
+        return cls(torch.zeros(*lead, 64, 16, **byte), torch.zeros(*lead, 64, 16, **byte),
+                   torch.full((*lead, 16, 4), 127, **byte), torch.full((*lead, 64), 127, **byte))
+
+    def layer(self, i: int) -> "KV4":
+        return KV4(self.k[i], self.v[i], self.ks[i], self.vs[i])
+
+    @property
+    def dims(self) -> tuple:
+        """(B, Hkv, S, D)"""
+        *_, B, Hkv, nb, nd, _ = self.vs.shape
+        return B, Hkv, nb * 64, nd * 32
+
+    def ptrs(self) -> tuple:
+        k, v, ks, vs = self
+        return k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
+
+    def check(self, what: str, layers: bool = False) -> tuple:
+        """(B, Hkv, S, D) of a cache of the documented storage; LskError otherwise."""
+        if self._checked is not None and self._checked[0] == layers:
+            return self._checked[1]
+        k, v, ks, vs = self
+        lead = vs.shape[:-1]
+        if len(lead) != (5 if layers else 4):
+            raise LskError(f"{what}: a 4-bit cache of {'several layers' if layers else 'one layer'} is needed")
+        if lead[-1] not in (2, 4) or lead[-2] == 0:
+            raise LskError(f"{what}: 4-bit caches need head_dim 64 or 128 and at least 64 positions (got "
+                           f"{32 * lead[-1]}, {64 * lead[-2]})")
+        _want(what, "k codes", k, torch.uint8, (*lead, 64, 16))
+        _want(what, "v codes", v, torch.uint8, (*lead, 64, 16))
+        _want(what, "k exponents", ks, torch.uint8, (*lead, 16, 4))
+        _want(what, "v exponents", vs, torch.uint8, (*lead, 64))
+        self._checked = layers, (lead[-4], lead[-3], lead[-2] * 64, lead[-1] * 32)
+        return self._checked[1]
+
+
+def _want_cache(name: str, cache, kind) -> None:
+    if not isinstance(cache, kind):
+        raise LskError(f"{name}: a {kind.__name__} cache is needed, got {type(cache).__name__}")
+
+
+def _codes_append(name: str, k, v, cache, rows_i32, pos_i32) -> None:
     dev = _one_device(k, v, *cache, rows_i32, pos_i32)
-    B, Hkv, S, D = cache.check("kv8_append")
+    B, Hkv, S, D = cache.check(name)
     n = k.shape[0]
     if k.shape != (n, Hkv, D) or v.shape != k.shape or v.dtype != k.dtype:
-        raise LskError(f"kv8_append: k and v must be [N, {Hkv}, {D}] of one dtype, got {list(k.shape)} {k.dtype} and "
+        raise LskError(f"{name}: k and v must be [N, {Hkv}, {D}] of one dtype, got {list(k.shape)} {k.dtype} and "
                        f"{list(v.shape)} {v.dtype}")
     st_t, st_h, st_d = k.stride()
     if n and (st_d != 1 or v.stride() != (st_t, st_h, st_d)):
-        raise LskError("kv8_append: k and v need contiguous dims and the same strides")
-    _want("kv8_append", "rows", rows_i32, torch.int32, (n,))
-    _want("kv8_append", "pos", pos_i32, torch.int32, (n,))
+        raise LskError(f"{name}: k and v need contiguous dims and the same strides")
+    _want(name, "rows", rows_i32, torch.int32, (n,))
+    _want(name, "pos", pos_i32, torch.int32, (n,))
     code = dtype_code(k.dtype)
     if n == 0:
         return
-    _launch(dev, "lsk_kv8_append", code, k.data_ptr(), v.data_ptr(), st_t, st_h, *cache.ptrs(), rows_i32.data_ptr(),
+    _launch(dev, "lsk_" + name, code, k.data_ptr(), v.data_ptr(), st_t, st_h, *cache.ptrs(), rows_i32.data_ptr(),
             pos_i32.data_ptr(), n, Hkv, D, B, S)
+
+
+def _codes_read(name: str, cache, rows_i32, pos_i32, dtype, out) -> tuple:
+    dev = _one_device(*cache, rows_i32, pos_i32, *(out or ()))
+    B, Hkv, S, D = cache.check(name)
+    n = rows_i32.numel()
+    _want(name, "rows", rows_i32, torch.int32, (n,))
+    _want(name, "pos", pos_i32, torch.int32, (n,))
+    code = dtype_code(dtype if out is None else out[0].dtype)
+    if out is None:
+        out = cache.ks.new_empty(n, Hkv, D, dtype=dtype), cache.ks.new_empty(n, Hkv, D, dtype=dtype)
+    else:
+        if len(out) != 2:
+            raise LskError(f"{name}: out is a pair of tensors")
+        for t in out:
+            _want(name, "out", t, out[0].dtype, (n, Hkv, D))
+    if n:
+        _launch(dev, "lsk_" + name, code, *cache.ptrs(), rows_i32.data_ptr(), pos_i32.data_ptr(), out[0].data_ptr(),
+                out[1].data_ptr(), n, Hkv, D, B, S)
+    return out
+
+
+def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor) -> None:
+    """k, v [N, Hkv, D] (bf16 or fp32, of equal strides; dims contiguous) quantised into a layer's 8-bit cache at
+    (rows, pos).  Tokens outside the cache are skipped; the (row, position) pairs of a call have to differ."""
+    _want_cache("kv8_append", cache, KV8)
+    _codes_append("kv8_append", k, v, cache, rows_i32, pos_i32)
 
 
 def kv8_read(cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
              out: tuple | None = None) -> tuple:
     """The K and V that a layer's 8-bit cache holds at (rows, pos): two [N, Hkv, D] tensors (bf16: exactly); zeros for
     tokens outside the cache."""
-    dev = _one_device(*cache, rows_i32, pos_i32, *(out or ()))
-    B, Hkv, S, D = cache.check("kv8_read")
-    n = rows_i32.numel()
-    _want("kv8_read", "rows", rows_i32, torch.int32, (n,))
-    _want("kv8_read", "pos", pos_i32, torch.int32, (n,))
-    code = dtype_code(dtype if out is None else out[0].dtype)
-    if out is None:
-        out = cache.ks.new_empty(n, Hkv, D, dtype=dtype), cache.ks.new_empty(n, Hkv, D, dtype=dtype)
-    else:
-        if len(out) != 2:
-            raise LskError("kv8_read: out is a pair of tensors")
-        for t in out:
-            _want("kv8_read", "out", t, out[0].dtype, (n, Hkv, D))
-    if n:
-        _launch(dev, "lsk_kv8_read", code, *cache.ptrs(), rows_i32.data_ptr(), pos_i32.data_ptr(), out[0].data_ptr(),
-                out[1].data_ptr(), n, Hkv, D, B, S)
-    return out
+    _want_cache("kv8_read", cache, KV8)
+    return _codes_read("kv8_read", cache, rows_i32, pos_i32, dtype, out)
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: KV4, rows_i32: torch.Tensor, pos_i32: torch.Tensor) -> None:
+    """kv8_append for a layer's 4-bit cache."""
+    _want_cache("kv4_append", cache, KV4)
+    _codes_append("kv4_append", k, v, cache, rows_i32, pos_i32)
+
+
+def kv4_read(cache: KV4, rows_i32: torch.Tensor, pos_i32: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
+             out: tuple | None = None) -> tuple:
+    """kv8_read for a layer's 4-bit cache."""
+    _want_cache("kv4_read", cache, KV4)
+    return _codes_read("kv4_read", cache, rows_i32, pos_i32, dtype, out)
 
 
 def cache_attn_split(max_batch: int, n_kv_heads: int, max_seq: int, tree: bool = False) -> int:
@@ -697,19 +792,19 @@ class _Launch:
 
 class AttnPlan:
     """The plan of attention launches over packed blocks, shared by the layers of a segment.  blocks: int [nb, 4] =
-    (q_start, pos0, T, row) with q_start the running sum of T; cache: a layer's KV8, or the K storage of a bf16 or fp32
-    cache.  split: KV positions per split (cache_attn_split unless given; fp32 does not split); row_groups: a tree's at
+    (q_start, pos0, T, row) with q_start the running sum of T; cache: a layer's KV8 or KV4, or the K storage of a bf16 or
+    fp32 cache.  split: KV positions per split (cache_attn_split unless given; fp32 does not split); row_groups: a tree's at
     most (by the cache and the block unless given).  tree: which launches it is for, with a mask (True), without (False)
-    or, over an 8-bit cache, either (None), which takes twice as long (256 requests: 333 us for 129).
+    or, over an 8-bit or 4-bit cache, either (None), which takes twice as long (256 requests: 333 us for 129).
     Its records go to the GPU on the current stream.  A launch on another stream waits for them, and they outlive it
     when the plan is dropped; a captured launch reads them with every replay: the plan is made before the capture and
     kept as long as the graph."""
 
     def __init__(self, blocks, n_heads: int, cache, split: int | None = None, row_groups: int | None = None,
                  tree: bool | None = None):
-        self.kv8 = isinstance(cache, KV8)
-        kcache = cache.k if self.kv8 else cache
-        self.dims = B, Hkv, S, D = cache.dims if self.kv8 else k_dims(cache)
+        self.format = 1 if isinstance(cache, KV8) else 2 if isinstance(cache, KV4) else 0
+        kcache = cache.k if self.format else cache
+        self.dims = B, Hkv, S, D = cache.dims if self.format else k_dims(cache)
         self.dtype, self.device = kcache.dtype, kcache.device
         if n_heads <= 0 or n_heads % Hkv:
             raise ValueError(f"{n_heads} query heads over {Hkv} KV heads")
@@ -737,7 +832,7 @@ class AttnPlan:
         self.split, self.tree_split = (split if split is not None else cache_attn_split(B, Hkv, S, t)
                                        for t in (False, True))
         rg = 0 if row_groups is None else row_groups
-        if self.kv8 and not tree:
+        if self.format and not tree:
             self.causal = self._plan(b, group, self.split, False, 1, n_slots)
         if tree or tree is None:
             self.tree = self._plan(b, group, self.tree_split, True, rg, n_slots)
@@ -775,7 +870,7 @@ class AttnPlan:
     def _plan(self, b: np.ndarray, group: int, split: int, tree: bool, row_groups: int, n_slots: int) -> _Launch:
         lib, cnt = load(), np.zeros(9, dtype=np.int64)
         B, Hkv, _, D = self.dims
-        args = (b.ctypes.data if len(b) else None, len(b), group, split, B, Hkv, D, int(self.kv8), int(tree),
+        args = (b.ctypes.data if len(b) else None, len(b), group, split, B, Hkv, D, self.format, int(tree),
                 row_groups, n_slots)
         _check(lib.lsk_cache_attn_plan(*args, None, 0, cnt.ctypes.data), "lsk_cache_attn_plan")
         meta = np.zeros(max(int(cnt[6]), 1), dtype=np.int32)
@@ -787,16 +882,16 @@ class AttnPlan:
                        ws)
 
 
-def _plan_call(what: str, dev: int, q: torch.Tensor, plan: AttnPlan, launch, dims: tuple, kv8: bool,
+def _plan_call(what: str, dev: int, q: torch.Tensor, plan: AttnPlan, launch, dims: tuple, fmt: int,
                dtype: torch.dtype, mask, scale, out, workspace):
-    """Checks shared by kv8_attn and tree_attn, and the plan joined; returns (scale, out, workspace, its bytes)."""
+    """Checks shared by the attention calls, and the plan joined; returns (scale, out, workspace, its bytes)."""
     if dev != plan.index:
         raise LskError(f"{what}: the plan is on {plan.device}, the tensors on cuda:{dev}")
-    if plan.dims != dims or plan.kv8 != kv8 or plan.dtype is not dtype:
+    if plan.dims != dims or plan.format != fmt or plan.dtype is not dtype:
         raise LskError(f"{what}: the plan was made for another cache ({plan.dims} {plan.dtype})")
     if launch is None and dtype != torch.float32:
         raise LskError(f"{what}: the plan was made for launches {'without' if mask is not None else 'with'} a mask")
-    want = torch.bfloat16 if kv8 else dtype
+    want = torch.bfloat16 if fmt else dtype
     n, width = plan.n_tokens, plan.width
     if q.shape != plan.q_shape or q.dtype is not want or (n and q.stride(2) != 1):
         raise LskError(f"{what}: q must be {list(plan.q_shape)} {want} with contiguous dims, got {list(q.shape)} "
@@ -825,14 +920,26 @@ def kv8_attn(q: torch.Tensor, cache: KV8, plan: AttnPlan, mask: torch.Tensor | N
     """Ragged verify / decode attention over a layer's 8-bit cache (lsk_kv8_attn): q [N, Hq, D] bf16 -> [N, Hq * D].
     mask (int32 [N, words], tree_masks): blocks are trees of drafted tokens.  scale: 1 / sqrt(D) unless given.  Without
     a workspace one is taken from torch's allocator for the call."""
+    _want_cache("kv8_attn", cache, KV8)
+    return _codes_attn("kv8_attn", 1, q, cache, plan, mask, scale, out, workspace)
+
+
+def kv4_attn(q: torch.Tensor, cache: KV4, plan: AttnPlan, mask: torch.Tensor | None = None, scale: float | None = None,
+             out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """kv8_attn over a layer's 4-bit cache (lsk_kv4_attn)."""
+    _want_cache("kv4_attn", cache, KV4)
+    return _codes_attn("kv4_attn", 2, q, cache, plan, mask, scale, out, workspace)
+
+
+def _codes_attn(name: str, fmt: int, q, cache, plan: AttnPlan, mask, scale, out, workspace) -> torch.Tensor:
     p = plan.causal if mask is None else plan.tree
     dev = _one_device(q, *cache, mask, out, workspace)
-    dims = _, Hkv, S, D = cache.check("kv8_attn")
-    scale, out, workspace, ws = _plan_call("kv8_attn", dev, q, plan, p, dims, True, _E4M3, mask, scale, out, workspace)
+    dims = _, Hkv, S, D = cache.check(name)
+    scale, out, workspace, ws = _plan_call(name, dev, q, plan, p, dims, fmt, cache.k.dtype, mask, scale, out, workspace)
     if p.n_items:
         st_t, st_h, _ = q.stride()
         masked = (None, 0) if mask is None else (mask.data_ptr(), mask.shape[1])
-        _launch(dev, "lsk_kv8_attn", q.data_ptr(), st_t, st_h, *cache.ptrs(), *masked, *p.args, out.data_ptr(),
+        _launch(dev, "lsk_" + name, q.data_ptr(), st_t, st_h, *cache.ptrs(), *masked, *p.args, out.data_ptr(),
                 plan.n_heads, Hkv, D, S, scale, _ptr(workspace), ws)
     return out
 
@@ -851,7 +958,7 @@ def tree_attn(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, plan:
     if not kcache.is_contiguous():
         raise LskError("tree_attn: the K cache must be contiguous")
     _want("tree_attn", "V cache", vcache, kcache.dtype, (B, Hkv, S // 32, D, 32))
-    scale, out, workspace, ws = _plan_call("tree_attn", dev, q, plan, p, dims, False, kcache.dtype, mask, scale, out,
+    scale, out, workspace, ws = _plan_call("tree_attn", dev, q, plan, p, dims, 0, kcache.dtype, mask, scale, out,
                                            workspace)
     if p.n_items if p is not None else plan.n_works:
         args = p.args if p is not None else (None, 0, 0, None, 0, 0, 0, 0, 0, 0)
@@ -931,8 +1038,167 @@ def kv_compact(k: torch.Tensor, v: torch.Tensor, rows_i32, pos0_i32, accepted, p
 
 def kv8_compact(cache: KV8, rows_i32, pos0_i32, accepted, path) -> None:
     """kv_compact for the layers of an 8-bit cache (tensors with a leading layer axis)."""
+    _want_cache("kv8_compact", cache, KV8)
     dims = cache.check("kv8_compact", layers=True)
     _compact("kv8_compact", DTYPE_KV8, *cache, cache.k.shape[0], dims, rows_i32, pos0_i32, accepted, path)
+
+
+def kv4_compact(cache: KV4, rows_i32, pos0_i32, accepted, path) -> None:
+    """kv_compact for the layers of a 4-bit cache (tensors with a leading layer axis)."""
+    _want_cache("kv4_compact", cache, KV4)
+    dims = cache.check("kv4_compact", layers=True)
+    _compact("kv4_compact", DTYPE_KV4, *cache, cache.k.shape[0], dims, rows_i32, pos0_i32, accepted, path)
+
+
+# ----------------------------------------------------------------------------- query and key norms with rotation
+
+def _norm_rope(name: str, qkv, w_q, w_k, eps, cos_tab, sin_tab, pos_i32, n_heads, n_kv_heads, head_dim, q_out, k_out,
+               rows_i32, kcache, vcache, max_batch, max_seq) -> None:
+    dev = _one_device(qkv, w_q, w_k, cos_tab, sin_tab, pos_i32, q_out, k_out, rows_i32, kcache, vcache)
+    n, code = qkv.shape[0], dtype_code(qkv.dtype)
+    if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or (n and qkv.stride(1) != 1):
+        raise LskError(f"{name}: qkv must be [N, {(n_heads + 2 * n_kv_heads) * head_dim}] with contiguous rows, got "
+                       f"{list(qkv.shape)}")
+    _want(name, "w_q", w_q, qkv.dtype, (head_dim,))
+    _want(name, "w_k", w_k, qkv.dtype, (head_dim,))
+    _want(name, "cos", cos_tab, torch.float32, (cos_tab.shape[0], head_dim))
+    _want(name, "sin", sin_tab, torch.float32, tuple(cos_tab.shape))
+    _want(name, "pos", pos_i32, torch.int32, (n,))
+    _want(name, "q_out", q_out, qkv.dtype, (n, n_heads, head_dim))
+    if n:
+        _launch(dev, "lsk_qk_norm_rope", code, qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), w_q.data_ptr(),
+                w_k.data_ptr(), float(eps), cos_tab.data_ptr(), sin_tab.data_ptr(), cos_tab.shape[0], _ptr(rows_i32),
+                pos_i32.data_ptr(), n, n_heads, n_kv_heads, head_dim, q_out.data_ptr(), _ptr(k_out), _ptr(kcache),
+                _ptr(vcache), max_batch, max_seq)
+
+
+def qk_norm_rope(qkv: torch.Tensor, w_q: torch.Tensor, w_k: torch.Tensor, eps: float, cos_tab: torch.Tensor,
+                 sin_tab: torch.Tensor, pos_i32: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
+                 out: tuple | None = None) -> tuple:
+    """Queries and keys of fused rows qkv [N, (Hq + 2 Hkv) D], normalised head by head (weights w_q, w_k [D]) and rotated
+    to their positions (lsk_qk_norm_rope) -> (q [N, Hq, D], k [N, Hkv, D]).  A position outside the tables leaves its
+    rows of the outputs as they were.  For caches that are written by kv8_append or kv4_append."""
+    n = qkv.shape[0]
+    if out is None:
+        out = qkv.new_empty(n, n_heads, head_dim), qkv.new_empty(n, n_kv_heads, head_dim)
+    elif len(out) != 2:
+        raise LskError("qk_norm_rope: out is a pair of tensors")
+    _want("qk_norm_rope", "k", out[1], qkv.dtype, (n, n_kv_heads, head_dim))
+    _norm_rope("qk_norm_rope", qkv, w_q, w_k, eps, cos_tab, sin_tab, pos_i32, n_heads, n_kv_heads, head_dim, out[0],
+               out[1], None, None, None, 0, 0)
+    return out
+
+
+def qk_norm_rope_append(qkv: torch.Tensor, q_out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor,
+                        w_q: torch.Tensor, w_k: torch.Tensor, eps: float, cos_tab: torch.Tensor, sin_tab: torch.Tensor,
+                        rows_i32: torch.Tensor, pos_i32: torch.Tensor, n_heads: int, n_kv_heads: int,
+                        head_dim: int) -> None:
+    """rope_append for models that normalise queries and keys head by head (qk_norm_rope); K and V go to (rows, pos) of
+    a layer's bf16 or fp32 cache.  A token outside the cache or the tables writes nothing."""
+    _check_kcache(qkv.dtype, kcache)
+    B, Hkv, S, D = k_dims(kcache)
+    if (Hkv, D) != (n_kv_heads, head_dim) or not kcache.is_contiguous() or kcache.dtype != qkv.dtype:
+        raise LskError(f"qk_norm_rope_append: a contiguous {qkv.dtype} K cache of {n_kv_heads} heads of {head_dim} is "
+                       f"needed, got {Hkv} of {D} {kcache.dtype}")
+    _want("qk_norm_rope_append", "V cache", vcache, qkv.dtype, (B, Hkv, S // 32, D, 32))
+    _want("qk_norm_rope_append", "rows", rows_i32, torch.int32, (qkv.shape[0],))
+    _norm_rope("qk_norm_rope_append", qkv, w_q, w_k, eps, cos_tab, sin_tab, pos_i32, n_heads, n_kv_heads, head_dim,
+               q_out, None, rows_i32, kcache, vcache, B, S)
+
+
+# ----------------------------------------------------------------------------- 8-bit integer projections
+
+def _i8_bytes(rows: int, k: int) -> int:
+    return (rows + 15) // 16 * ((k + 63) // 64) * 1024
+
+
+class RowsI8:
+    """Activations [M, K] as 8-bit integers with a scale per row (quant_rows_i8), in the matrix instructions' order."""
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, shape: tuple, dtype: torch.dtype):
+        self.data, self.scales, self.shape, self.dtype = data, scales, shape, dtype
+
+
+def quant_rows_i8(x: torch.Tensor, out: RowsI8 | None = None) -> RowsI8:
+    """Quantises the rows of x [M, K] (bf16 or fp32) to 8-bit integers (lsk_quant_rows_i8): codes round(x 127 / amax),
+    scales amax / 127.  A row that holds a NaN or an infinity gets the scale NaN.  out: buffers to write again."""
+    if x.dim() != 2 or (x.numel() and x.stride(1) != 1):
+        raise LskError(f"quant_rows_i8: a 2-D tensor with contiguous rows is needed, got {list(x.shape)}")
+    M, K = x.shape
+    code = dtype_code(x.dtype)
+    if out is None:
+        out = RowsI8(x.new_empty(_i8_bytes(M, K), dtype=torch.int8), x.new_empty(M, dtype=torch.float32), (M, K), x.dtype)
+    elif out.shape != (M, K) or out.dtype != x.dtype:
+        raise LskError(f"quant_rows_i8: out holds {out.shape} of {out.dtype}")
+    dev = _one_device(x, out.data, out.scales)
+    if M:
+        _launch(dev, "lsk_quant_rows_i8", code, x.data_ptr(), max(x.stride(0), K), out.data.data_ptr(),
+                out.scales.data_ptr(), M, K)
+    return out
+
+
+class PackedWeightI8:
+    """A weight [N, K] (F.linear's [out, in]) as 8-bit integers with a scale per output channel, in the matrix
+    instructions' order: a bf16 or fp32 tensor, quantised as quant_rows_i8 does, or int8 codes [N, K] with their fp32
+    scales [N].  unpack() gives the codes [N, K] back."""
+
+    def __init__(self, w: torch.Tensor, scales: torch.Tensor | None = None):
+        if w.dim() != 2 or w.stride(1) != 1 or 0 in w.shape:
+            raise LskError(f"PackedWeightI8: a 2-D tensor with contiguous rows is needed, got {list(w.shape)}")
+        N, K = self.shape = tuple(w.shape)
+        self.device = w.device
+        if w.dtype == torch.int8:
+            if scales is None:
+                raise LskError("PackedWeightI8: codes without scales")
+            _want("PackedWeightI8", "scales", scales, torch.float32, (N,))
+            dev = _one_device(w, scales)
+            self.data, self.scales = w.new_empty(_i8_bytes(N, K)), scales.clone()
+            _launch(dev, "lsk_pack_i8", w.data_ptr(), max(w.stride(0), K), self.data.data_ptr(), N, K)
+        else:
+            if scales is not None:
+                raise LskError("PackedWeightI8: scales belong to int8 codes")
+            _one_device(w)
+            q = quant_rows_i8(w, RowsI8(w.new_zeros(_i8_bytes(N, K), dtype=torch.int8),
+                                        w.new_empty(N, dtype=torch.float32), (N, K), w.dtype))
+            self.data, self.scales = q.data, q.scales
+
+    def unpack(self) -> torch.Tensor:
+        N, K = self.shape
+        out = self.data.new_empty(N, K)
+        _launch(_one_device(self.data), "lsk_unpack_i8", self.data.data_ptr(), out.data_ptr(), K, N, K)
+        return out
+
+    def __repr__(self) -> str:
+        return f"PackedWeightI8(shape={self.shape}, device={self.device})"
+
+
+def gemm_i8(a: RowsI8, w: PackedWeightI8, out: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+            epilogue: int = EPI_NONE) -> torch.Tensor:
+    """gemm over 8-bit integers (lsk_gemm_i8): out[m, n] = epilogue(scale_m scale_n sum_k a w) of a's dtype, fp32 until
+    its one rounding.  EPI_RESIDUAL adds residual [M, N]; for EPI_SILU_MUL w holds [gate; up]."""
+    if a.shape[1] != w.shape[1]:
+        raise LskError(f"gemm_i8: {a.shape} against a weight of {w.shape}")
+    M, K = a.shape
+    N = w.shape[0]
+    if epilogue == EPI_SILU_MUL:
+        if N % 32:
+            raise LskError(f"gemm_i8: silu-mul needs gate and up of a multiple of 16 rows, got {N} together")
+        N //= 2
+    if (residual is not None) != (epilogue == EPI_RESIDUAL):
+        raise LskError("gemm_i8: a residual is what EPI_RESIDUAL takes")
+    dev = _one_device(a.data, a.scales, w.data, w.scales, out, residual)
+    if out is None:
+        out = torch.empty(M, N, dtype=a.dtype, device=a.data.device)
+    for t in (out, residual):
+        if t is not None and (t.shape != (M, N) or t.dtype != a.dtype or (t.numel() and t.stride(1) != 1)):
+            raise LskError(f"gemm_i8: out and residual must be {[M, N]} {a.dtype} with contiguous rows, got "
+                           f"{list(t.shape)} {t.dtype}")
+    if M:
+        ldr = max(residual.stride(0), N) if residual is not None else 0
+        _launch(dev, "lsk_gemm_i8", dtype_code(a.dtype), a.data.data_ptr(), a.scales.data_ptr(), w.data.data_ptr(),
+                w.scales.data_ptr(), out.data_ptr(), max(out.stride(0), N), _ptr(residual), ldr, M, N, K, epilogue,
+                N if epilogue == EPI_SILU_MUL else 0)
+    return out
 
 
 # ----------------------------------------------------------------------------- layer-range runner
