@@ -614,9 +614,9 @@ def test_quant_rows_i8_is_exact(cuda, dtype, M, K):
     a = lsk.quant_rows_i8(view)
     assert torch.equal(a.scales.cpu().nan_to_num(-1), scales.nan_to_num(-1))
     live = torch.isfinite(scales)
-    assert torch.equal(unpacked(a.data, M, K)[live].double(), codes[live])
+    assert torch.equal(unpacked(a.codes, M, K)[live].double(), codes[live])
     nks = (K + 63) // 64
-    pad = a.data.cpu().view(-1, nks, 64, 16)[:, -1]                   # zeros past K in the rows that are there
+    pad = a.codes.cpu().view(-1, nks, 64, 16)[:, -1]                   # zeros past K in the rows that are there
     for r in range(M):
         tail = pad[r // 16].view(4, 16, 16)[:, r % 16].reshape(-1)[K - 64 * (nks - 1):]
         assert (tail == 0).all()

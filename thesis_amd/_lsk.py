@@ -205,6 +205,9 @@ def v_from_blocked(vb: torch.Tensor) -> torch.Tensor:
     return vb.transpose(-1, -2).reshape(*lead, nb * b, D)
 
 
+_CODES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
+
+
 def dtype_code(dtype: torch.dtype) -> int:
     if dtype == torch.bfloat16:
         return DTYPE_BF16
@@ -547,14 +550,23 @@ def _one_device(first: torch.Tensor, *ts) -> int:
 
 def _launch(dev: int, what: str, *args) -> None:
     """Calls `what` with args and device dev's current stream; dev is the current device for the call."""
-    fn = getattr(load(), what)
+    fn = getattr(_lib or load(), what)
     if torch._C._cuda_getDevice() == dev:
-        rc = fn(*args, _stream())
+        rc = fn(*args, _stream(dev))
     else:
         with torch.cuda.device(dev):
             rc = fn(*args, _stream())
     if rc:
         _check(rc, what)
+
+
+def _same_device(first: torch.Tensor, *ts) -> int:
+    """The index of the device that all the tensors are on, -1 where there is none."""
+    dev = first.get_device()
+    for t in ts:
+        if t.get_device() != dev:
+            return -1
+    return dev
 
 
 def _want(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
@@ -577,8 +589,8 @@ class KV8(_KV8):
     """An 8-bit K / V cache (lsk_kv8_append): e4m3 codes and one power-of-two scale per position and KV head, the byte
     e + 127.  A layer's tensors, or with a leading layer axis those of several:
       k [B, Hkv, S/64, 4, D/64, 64, 16] and v [B, Hkv, S/64, D, 64] float8_e4m3fn, ks and vs [B, Hkv, S] uint8.
-    The tensors' types and shapes are checked by the object's first use; they have to stay as they are."""
-    _checked = None                                   # (layers, dims) that the tensors were found to fit
+    The tensors' types, shapes and devices are checked by the object's first use; they have to stay as they are."""
+    _checked = None                                   # (layers, dims, device, addresses) that the tensors were found with
 
     @classmethod
     def zeros(cls, max_batch: int, n_kv_heads: int, max_seq: int, head_dim: int, device, layers: int | None = None):
@@ -624,7 +636,7 @@ class KV8(_KV8):
             _want(what, "v codes", v, _E4M3, want_v)
             _want(what, "k exponents", ks, torch.uint8, lead)
             _want(what, "v exponents", vs, torch.uint8, lead)
-        self._checked = layers, (lead[-3], lead[-2], S, D)
+        self._checked = layers, (lead[-3], lead[-2], S, D), _same_device(k, v, ks, vs), self.ptrs()
         return self._checked[1]
 
 
@@ -639,8 +651,8 @@ class KV4(_KV4):
     """A 4-bit K / V cache (lsk_kv4_append): e2m1 codes and one power-of-two scale per position, KV head and 32 dims, the
     byte e + 127.  A layer's tensors, or with a leading layer axis those of several, all uint8:
       k and v [B, Hkv, S/64, D/32, 64, 16], ks [B, Hkv, S/64, D/32, 16, 4] and vs [B, Hkv, S/64, D/32, 64].
-    The tensors' types and shapes are checked by the object's first use; they have to stay as they are."""
-    _checked = None                                   # (layers, dims) that the tensors were found to fit
+    The tensors' types, shapes and devices are checked by the object's first use; they have to stay as they are."""
+    _checked = None                                   # (layers, dims, device, addresses) that the tensors were found with
 
     @classmethod
     def zeros(cls, max_batch: int, n_kv_heads: int, max_seq: int, head_dim: int, device, layers: int | None = None):
@@ -671,50 +683,72 @@ class KV4(_KV4):
         if self._checked is not None and self._checked[0] == layers:
             return self._checked[1]
         k, v, ks, vs = self
-        lead = vs.shape[:-1]
+        shape = vs.shape
+        lead = shape[:-1]
         if len(lead) != (5 if layers else 4):
             raise LskError(f"{what}: a 4-bit cache of {'several layers' if layers else 'one layer'} is needed")
         if lead[-1] not in (2, 4) or lead[-2] == 0:
             raise LskError(f"{what}: 4-bit caches need head_dim 64 or 128 and at least 64 positions (got "
                            f"{32 * lead[-1]}, {64 * lead[-2]})")
-        _want(what, "k codes", k, torch.uint8, (*lead, 64, 16))
-        _want(what, "v codes", v, torch.uint8, (*lead, 64, 16))
-        _want(what, "k exponents", ks, torch.uint8, (*lead, 16, 4))
-        _want(what, "v exponents", vs, torch.uint8, (*lead, 64))
-        self._checked = layers, (lead[-4], lead[-3], lead[-2] * 64, lead[-1] * 32)
+        codes = (*lead, 64, 16)
+        if not (k.shape == v.shape == codes and ks.shape == (*lead, 16, 4) and shape[-1] == 64 and
+                k.dtype is v.dtype is ks.dtype is vs.dtype is torch.uint8 and k.is_contiguous() and
+                v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+            _want(what, "k codes", k, torch.uint8, codes)
+            _want(what, "v codes", v, torch.uint8, codes)
+            _want(what, "k exponents", ks, torch.uint8, (*lead, 16, 4))
+            _want(what, "v exponents", vs, torch.uint8, (*lead, 64))
+        self._checked = layers, (lead[-4], lead[-3], lead[-2] * 64, lead[-1] * 32), _same_device(k, v, ks, vs), \
+            self.ptrs()
         return self._checked[1]
 
 
-def _want_cache(name: str, cache, kind) -> None:
+def _want_kind(name: str, cache, kind) -> None:
     if not isinstance(cache, kind):
         raise LskError(f"{name}: a {kind.__name__} cache is needed, got {type(cache).__name__}")
 
 
-def _codes_append(name: str, k, v, cache, rows_i32, pos_i32) -> None:
-    dev = _one_device(k, v, *cache, rows_i32, pos_i32)
-    B, Hkv, S, D = cache.check(name)
-    n = k.shape[0]
-    if k.shape != (n, Hkv, D) or v.shape != k.shape or v.dtype != k.dtype:
-        raise LskError(f"{name}: k and v must be [N, {Hkv}, {D}] of one dtype, got {list(k.shape)} {k.dtype} and "
-                       f"{list(v.shape)} {v.dtype}")
-    st_t, st_h, st_d = k.stride()
-    if n and (st_d != 1 or v.stride() != (st_t, st_h, st_d)):
-        raise LskError(f"{name}: k and v need contiguous dims and the same strides")
-    _want(name, "rows", rows_i32, torch.int32, (n,))
-    _want(name, "pos", pos_i32, torch.int32, (n,))
-    code = dtype_code(k.dtype)
+def _cache_of(name: str, cache, kind) -> tuple:
+    """(dims, device, addresses) of a layer's cache of that kind; LskError otherwise."""
+    _want_kind(name, cache, kind)
+    cache.check(name)
+    return cache._checked[1:]
+
+
+def _codes_append(name: str, kind, k, v, cache, rows_i32, pos_i32) -> None:
+    dims, dev, ptrs = _cache_of(name, cache, kind)
+    B, Hkv, S, D = dims
+    shape, dtype, strides = k.shape, k.dtype, k.stride()
+    n, code = shape[0], _CODES.get(dtype)
+    if not (shape == (n, Hkv, D) and v.shape == shape and v.dtype is dtype and code is not None and strides[-1] == 1 and
+            v.stride() == strides and rows_i32.shape == pos_i32.shape == (n,) and
+            rows_i32.dtype is pos_i32.dtype is torch.int32 and rows_i32.is_contiguous() and pos_i32.is_contiguous() and
+            dev >= 0 and _same_device(k, v, rows_i32, pos_i32) == dev):
+        _one_device(k, v, *cache, rows_i32, pos_i32)
+        if shape != (n, Hkv, D) or v.shape != shape or v.dtype != dtype:
+            raise LskError(f"{name}: k and v must be [N, {Hkv}, {D}] of one dtype, got {list(shape)} {dtype} and "
+                           f"{list(v.shape)} {v.dtype}")
+        if n and (strides[2] != 1 or v.stride() != strides):
+            raise LskError(f"{name}: k and v need contiguous dims and the same strides")
+        _want(name, "rows", rows_i32, torch.int32, (n,))
+        _want(name, "pos", pos_i32, torch.int32, (n,))
+        dtype_code(dtype)
     if n == 0:
         return
-    _launch(dev, "lsk_" + name, code, k.data_ptr(), v.data_ptr(), st_t, st_h, *cache.ptrs(), rows_i32.data_ptr(),
+    _launch(dev, "lsk_" + name, code, k.data_ptr(), v.data_ptr(), strides[0], strides[1], *ptrs, rows_i32.data_ptr(),
             pos_i32.data_ptr(), n, Hkv, D, B, S)
 
 
-def _codes_read(name: str, cache, rows_i32, pos_i32, dtype, out) -> tuple:
-    dev = _one_device(*cache, rows_i32, pos_i32, *(out or ()))
-    B, Hkv, S, D = cache.check(name)
+def _codes_read(name: str, kind, cache, rows_i32, pos_i32, dtype, out) -> tuple:
+    dims, dev, ptrs = _cache_of(name, cache, kind)
+    B, Hkv, S, D = dims
     n = rows_i32.numel()
-    _want(name, "rows", rows_i32, torch.int32, (n,))
-    _want(name, "pos", pos_i32, torch.int32, (n,))
+    if not (rows_i32.shape == pos_i32.shape == (n,) and rows_i32.dtype is pos_i32.dtype is torch.int32 and
+            rows_i32.is_contiguous() and pos_i32.is_contiguous() and dev >= 0 and
+            _same_device(rows_i32, pos_i32, *(out or ())) == dev):
+        _one_device(*cache, rows_i32, pos_i32, *(out or ()))
+        _want(name, "rows", rows_i32, torch.int32, (n,))
+        _want(name, "pos", pos_i32, torch.int32, (n,))
     code = dtype_code(dtype if out is None else out[0].dtype)
     if out is None:
         out = cache.ks.new_empty(n, Hkv, D, dtype=dtype), cache.ks.new_empty(n, Hkv, D, dtype=dtype)
@@ -724,7 +758,7 @@ def _codes_read(name: str, cache, rows_i32, pos_i32, dtype, out) -> tuple:
         for t in out:
             _want(name, "out", t, out[0].dtype, (n, Hkv, D))
     if n:
-        _launch(dev, "lsk_" + name, code, *cache.ptrs(), rows_i32.data_ptr(), pos_i32.data_ptr(), out[0].data_ptr(),
+        _launch(dev, "lsk_" + name, code, *ptrs, rows_i32.data_ptr(), pos_i32.data_ptr(), out[0].data_ptr(),
                 out[1].data_ptr(), n, Hkv, D, B, S)
     return out
 
@@ -732,29 +766,25 @@ def _codes_read(name: str, cache, rows_i32, pos_i32, dtype, out) -> tuple:
 def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor) -> None:
     """k, v [N, Hkv, D] (bf16 or fp32, of equal strides; dims contiguous) quantised into a layer's 8-bit cache at
     (rows, pos).  Tokens outside the cache are skipped; the (row, position) pairs of a call have to differ."""
-    _want_cache("kv8_append", cache, KV8)
-    _codes_append("kv8_append", k, v, cache, rows_i32, pos_i32)
+    _codes_append("kv8_append", KV8, k, v, cache, rows_i32, pos_i32)
 
 
 def kv8_read(cache: KV8, rows_i32: torch.Tensor, pos_i32: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
              out: tuple | None = None) -> tuple:
     """The K and V that a layer's 8-bit cache holds at (rows, pos): two [N, Hkv, D] tensors (bf16: exactly); zeros for
     tokens outside the cache."""
-    _want_cache("kv8_read", cache, KV8)
-    return _codes_read("kv8_read", cache, rows_i32, pos_i32, dtype, out)
+    return _codes_read("kv8_read", KV8, cache, rows_i32, pos_i32, dtype, out)
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: KV4, rows_i32: torch.Tensor, pos_i32: torch.Tensor) -> None:
     """kv8_append for a layer's 4-bit cache."""
-    _want_cache("kv4_append", cache, KV4)
-    _codes_append("kv4_append", k, v, cache, rows_i32, pos_i32)
+    _codes_append("kv4_append", KV4, k, v, cache, rows_i32, pos_i32)
 
 
 def kv4_read(cache: KV4, rows_i32: torch.Tensor, pos_i32: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
              out: tuple | None = None) -> tuple:
     """kv8_read for a layer's 4-bit cache."""
-    _want_cache("kv4_read", cache, KV4)
-    return _codes_read("kv4_read", cache, rows_i32, pos_i32, dtype, out)
+    return _codes_read("kv4_read", KV4, cache, rows_i32, pos_i32, dtype, out)
 
 
 def cache_attn_split(max_batch: int, n_kv_heads: int, max_seq: int, tree: bool = False) -> int:
@@ -920,27 +950,26 @@ def kv8_attn(q: torch.Tensor, cache: KV8, plan: AttnPlan, mask: torch.Tensor | N
     """Ragged verify / decode attention over a layer's 8-bit cache (lsk_kv8_attn): q [N, Hq, D] bf16 -> [N, Hq * D].
     mask (int32 [N, words], tree_masks): blocks are trees of drafted tokens.  scale: 1 / sqrt(D) unless given.  Without
     a workspace one is taken from torch's allocator for the call."""
-    _want_cache("kv8_attn", cache, KV8)
-    return _codes_attn("kv8_attn", 1, q, cache, plan, mask, scale, out, workspace)
+    return _codes_attn("kv8_attn", KV8, 1, q, cache, plan, mask, scale, out, workspace)
 
 
 def kv4_attn(q: torch.Tensor, cache: KV4, plan: AttnPlan, mask: torch.Tensor | None = None, scale: float | None = None,
              out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """kv8_attn over a layer's 4-bit cache (lsk_kv4_attn)."""
-    _want_cache("kv4_attn", cache, KV4)
-    return _codes_attn("kv4_attn", 2, q, cache, plan, mask, scale, out, workspace)
+    return _codes_attn("kv4_attn", KV4, 2, q, cache, plan, mask, scale, out, workspace)
 
 
-def _codes_attn(name: str, fmt: int, q, cache, plan: AttnPlan, mask, scale, out, workspace) -> torch.Tensor:
+def _codes_attn(name: str, kind, fmt: int, q, cache, plan: AttnPlan, mask, scale, out, workspace) -> torch.Tensor:
     p = plan.causal if mask is None else plan.tree
-    dev = _one_device(q, *cache, mask, out, workspace)
-    dims = _, Hkv, S, D = cache.check(name)
+    dims, dev, ptrs = _cache_of(name, cache, kind)
+    if q.get_device() != dev or dev < 0 or mask is not None or out is not None or workspace is not None:
+        dev = _one_device(q, *cache, mask, out, workspace)
     scale, out, workspace, ws = _plan_call(name, dev, q, plan, p, dims, fmt, cache.k.dtype, mask, scale, out, workspace)
     if p.n_items:
         st_t, st_h, _ = q.stride()
         masked = (None, 0) if mask is None else (mask.data_ptr(), mask.shape[1])
-        _launch(dev, "lsk_" + name, q.data_ptr(), st_t, st_h, *cache.ptrs(), *masked, *p.args, out.data_ptr(),
-                plan.n_heads, Hkv, D, S, scale, _ptr(workspace), ws)
+        _launch(dev, "lsk_" + name, q.data_ptr(), st_t, st_h, *ptrs, *masked, *p.args, out.data_ptr(), plan.n_heads,
+                dims[1], dims[3], dims[2], scale, _ptr(workspace), ws)
     return out
 
 
@@ -1038,14 +1067,14 @@ def kv_compact(k: torch.Tensor, v: torch.Tensor, rows_i32, pos0_i32, accepted, p
 
 def kv8_compact(cache: KV8, rows_i32, pos0_i32, accepted, path) -> None:
     """kv_compact for the layers of an 8-bit cache (tensors with a leading layer axis)."""
-    _want_cache("kv8_compact", cache, KV8)
+    _want_kind("kv8_compact", cache, KV8)
     dims = cache.check("kv8_compact", layers=True)
     _compact("kv8_compact", DTYPE_KV8, *cache, cache.k.shape[0], dims, rows_i32, pos0_i32, accepted, path)
 
 
 def kv4_compact(cache: KV4, rows_i32, pos0_i32, accepted, path) -> None:
     """kv_compact for the layers of a 4-bit cache (tensors with a leading layer axis)."""
-    _want_cache("kv4_compact", cache, KV4)
+    _want_kind("kv4_compact", cache, KV4)
     dims = cache.check("kv4_compact", layers=True)
     _compact("kv4_compact", DTYPE_KV4, *cache, cache.k.shape[0], dims, rows_i32, pos0_i32, accepted, path)
 
@@ -1054,22 +1083,31 @@ def kv4_compact(cache: KV4, rows_i32, pos0_i32, accepted, path) -> None:
 
 def _norm_rope(name: str, qkv, w_q, w_k, eps, cos_tab, sin_tab, pos_i32, n_heads, n_kv_heads, head_dim, q_out, k_out,
                rows_i32, kcache, vcache, max_batch, max_seq) -> None:
-    dev = _one_device(qkv, w_q, w_k, cos_tab, sin_tab, pos_i32, q_out, k_out, rows_i32, kcache, vcache)
-    n, code = qkv.shape[0], dtype_code(qkv.dtype)
-    if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or (n and qkv.stride(1) != 1):
-        raise LskError(f"{name}: qkv must be [N, {(n_heads + 2 * n_kv_heads) * head_dim}] with contiguous rows, got "
-                       f"{list(qkv.shape)}")
-    _want(name, "w_q", w_q, qkv.dtype, (head_dim,))
-    _want(name, "w_k", w_k, qkv.dtype, (head_dim,))
-    _want(name, "cos", cos_tab, torch.float32, (cos_tab.shape[0], head_dim))
-    _want(name, "sin", sin_tab, torch.float32, tuple(cos_tab.shape))
-    _want(name, "pos", pos_i32, torch.int32, (n,))
-    _want(name, "q_out", q_out, qkv.dtype, (n, n_heads, head_dim))
+    n, dtype, width, table = qkv.shape[0], qkv.dtype, (n_heads + 2 * n_kv_heads) * head_dim, cos_tab.shape
+    code, dev, strides = _CODES.get(dtype), qkv.get_device(), qkv.stride()
+    others = (k_out,) if k_out is not None else (rows_i32, kcache, vcache)
+    if not (qkv.shape == (n, width) and strides[1] == 1 and code is not None and w_q.shape == w_k.shape == (head_dim,) and
+            w_q.dtype is w_k.dtype is q_out.dtype is dtype and len(table) == 2 and table[1] == head_dim and
+            sin_tab.shape == table and cos_tab.dtype is sin_tab.dtype is torch.float32 and pos_i32.shape == (n,) and
+            pos_i32.dtype is torch.int32 and q_out.shape == (n, n_heads, head_dim) and w_q.is_contiguous() and
+            w_k.is_contiguous() and cos_tab.is_contiguous() and sin_tab.is_contiguous() and pos_i32.is_contiguous() and
+            q_out.is_contiguous() and dev >= 0 and
+            _same_device(qkv, w_q, w_k, cos_tab, sin_tab, pos_i32, q_out, *others) == dev):
+        _one_device(qkv, w_q, w_k, cos_tab, sin_tab, pos_i32, q_out, *others)
+        dtype_code(dtype)
+        if qkv.dim() != 2 or qkv.shape[1] != width or (n and strides[1] != 1):
+            raise LskError(f"{name}: qkv must be [N, {width}] with contiguous rows, got {list(qkv.shape)}")
+        _want(name, "w_q", w_q, dtype, (head_dim,))
+        _want(name, "w_k", w_k, dtype, (head_dim,))
+        _want(name, "cos", cos_tab, torch.float32, (table[0], head_dim))
+        _want(name, "sin", sin_tab, torch.float32, tuple(table))
+        _want(name, "pos", pos_i32, torch.int32, (n,))
+        _want(name, "q_out", q_out, dtype, (n, n_heads, head_dim))
     if n:
-        _launch(dev, "lsk_qk_norm_rope", code, qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), w_q.data_ptr(),
-                w_k.data_ptr(), float(eps), cos_tab.data_ptr(), sin_tab.data_ptr(), cos_tab.shape[0], _ptr(rows_i32),
-                pos_i32.data_ptr(), n, n_heads, n_kv_heads, head_dim, q_out.data_ptr(), _ptr(k_out), _ptr(kcache),
-                _ptr(vcache), max_batch, max_seq)
+        _launch(dev, "lsk_qk_norm_rope", code, qkv.data_ptr(), max(strides[0], width), w_q.data_ptr(), w_k.data_ptr(),
+                float(eps), cos_tab.data_ptr(), sin_tab.data_ptr(), table[0], _ptr(rows_i32), pos_i32.data_ptr(), n,
+                n_heads, n_kv_heads, head_dim, q_out.data_ptr(), _ptr(k_out), _ptr(kcache), _ptr(vcache), max_batch,
+                max_seq)
 
 
 def qk_norm_rope(qkv: torch.Tensor, w_q: torch.Tensor, w_k: torch.Tensor, eps: float, cos_tab: torch.Tensor,
@@ -1113,27 +1151,42 @@ def _i8_bytes(rows: int, k: int) -> int:
 
 
 class RowsI8:
-    """Activations [M, K] as 8-bit integers with a scale per row (quant_rows_i8), in the matrix instructions' order."""
+    """Activations [M, K] as 8-bit integers with a scale per row (quant_rows_i8), in the matrix instructions' order: data
+    holds the codes and, behind them, the fp32 scales."""
+    __slots__ = ("data", "offset", "shape", "dtype")
 
-    def __init__(self, data: torch.Tensor, scales: torch.Tensor, shape: tuple, dtype: torch.dtype):
-        self.data, self.scales, self.shape, self.dtype = data, scales, shape, dtype
+    def __init__(self, data: torch.Tensor, shape: tuple, dtype: torch.dtype):
+        self.data, self.offset, self.shape, self.dtype = data, _i8_bytes(*shape), shape, dtype
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self.data[:self.offset]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self.data[self.offset:].view(torch.float32)
 
 
 def quant_rows_i8(x: torch.Tensor, out: RowsI8 | None = None) -> RowsI8:
     """Quantises the rows of x [M, K] (bf16 or fp32) to 8-bit integers (lsk_quant_rows_i8): codes round(x 127 / amax),
     scales amax / 127.  A row that holds a NaN or an infinity gets the scale NaN.  out: buffers to write again."""
-    if x.dim() != 2 or (x.numel() and x.stride(1) != 1):
-        raise LskError(f"quant_rows_i8: a 2-D tensor with contiguous rows is needed, got {list(x.shape)}")
-    M, K = x.shape
-    code = dtype_code(x.dtype)
+    shape, dtype = x.shape, x.dtype
+    if len(shape) != 2 or (x.stride(1) != 1 and x.numel()):
+        raise LskError(f"quant_rows_i8: a 2-D tensor with contiguous rows is needed, got {list(shape)}")
+    M, K = shape
+    code = dtype_code(dtype)
     if out is None:
-        out = RowsI8(x.new_empty(_i8_bytes(M, K), dtype=torch.int8), x.new_empty(M, dtype=torch.float32), (M, K), x.dtype)
-    elif out.shape != (M, K) or out.dtype != x.dtype:
-        raise LskError(f"quant_rows_i8: out holds {out.shape} of {out.dtype}")
-    dev = _one_device(x, out.data, out.scales)
+        out = RowsI8(x.new_empty(_i8_bytes(M, K) + 4 * M, dtype=torch.int8), (M, K), dtype)
+        dev = x.get_device()
+        if dev < 0:
+            _dev(x)
+    else:
+        if out.shape != (M, K) or out.dtype != dtype:
+            raise LskError(f"quant_rows_i8: out holds {out.shape} of {out.dtype}")
+        dev = _one_device(x, out.data)
     if M:
-        _launch(dev, "lsk_quant_rows_i8", code, x.data_ptr(), max(x.stride(0), K), out.data.data_ptr(),
-                out.scales.data_ptr(), M, K)
+        codes = out.data.data_ptr()
+        _launch(dev, "lsk_quant_rows_i8", code, x.data_ptr(), max(x.stride(0), K), codes, codes + out.offset, M, K)
     return out
 
 
@@ -1158,9 +1211,8 @@ class PackedWeightI8:
             if scales is not None:
                 raise LskError("PackedWeightI8: scales belong to int8 codes")
             _one_device(w)
-            q = quant_rows_i8(w, RowsI8(w.new_zeros(_i8_bytes(N, K), dtype=torch.int8),
-                                        w.new_empty(N, dtype=torch.float32), (N, K), w.dtype))
-            self.data, self.scales = q.data, q.scales
+            q = quant_rows_i8(w, RowsI8(w.new_zeros(_i8_bytes(N, K) + 4 * N, dtype=torch.int8), (N, K), w.dtype))
+            self.data, self.scales = q.codes, q.scales
 
     def unpack(self) -> torch.Tensor:
         N, K = self.shape
@@ -1186,18 +1238,24 @@ def gemm_i8(a: RowsI8, w: PackedWeightI8, out: torch.Tensor | None = None, resid
         N //= 2
     if (residual is not None) != (epilogue == EPI_RESIDUAL):
         raise LskError("gemm_i8: a residual is what EPI_RESIDUAL takes")
-    dev = _one_device(a.data, a.scales, w.data, w.scales, out, residual)
+    dtype, dev = a.dtype, _one_device(a.data, w.data, w.scales, out, residual)
     if out is None:
-        out = torch.empty(M, N, dtype=a.dtype, device=a.data.device)
+        out = torch.empty((M, N), dtype=dtype, device=a.data.device)
+    ldr = 0
     for t in (out, residual):
-        if t is not None and (t.shape != (M, N) or t.dtype != a.dtype or (t.numel() and t.stride(1) != 1)):
-            raise LskError(f"gemm_i8: out and residual must be {[M, N]} {a.dtype} with contiguous rows, got "
-                           f"{list(t.shape)} {t.dtype}")
+        if t is not None:
+            ld, one = t.stride() if t.dim() == 2 else (0, 0)
+            if t.shape != (M, N) or t.dtype is not dtype or (one != 1 and t.numel()):
+                raise LskError(f"gemm_i8: out and residual must be {[M, N]} {dtype} with contiguous rows, got "
+                               f"{list(t.shape)} {t.dtype}")
+            if t is out:
+                ldc = max(ld, N)
+            else:
+                ldr = max(ld, N)
     if M:
-        ldr = max(residual.stride(0), N) if residual is not None else 0
-        _launch(dev, "lsk_gemm_i8", dtype_code(a.dtype), a.data.data_ptr(), a.scales.data_ptr(), w.data.data_ptr(),
-                w.scales.data_ptr(), out.data_ptr(), max(out.stride(0), N), _ptr(residual), ldr, M, N, K, epilogue,
-                N if epilogue == EPI_SILU_MUL else 0)
+        codes = a.data.data_ptr()
+        _launch(dev, "lsk_gemm_i8", dtype_code(dtype), codes, codes + a.offset, w.data.data_ptr(), w.scales.data_ptr(),
+                out.data_ptr(), ldc, _ptr(residual), ldr, M, N, K, epilogue, N if epilogue == EPI_SILU_MUL else 0)
     return out
 
 
