@@ -71,19 +71,84 @@ __device__ __forceinline__ void load2(const float* p, float* x) { x[0] = p[0]; x
 __device__ __forceinline__ void store2(uint16_t* p, const float* x) { p[0] = f2bf(x[0]); p[1] = f2bf(x[1]); }
 __device__ __forceinline__ void store2(float* p, const float* x) { p[0] = x[0]; p[1] = x[1]; }
 
-// Replaces 4 of a dword's bits: another thread may be replacing others of them.
+// The bits of `mask` of a dword become those of x: other threads may be replacing others of its bits.
+__device__ __forceinline__ void put_bits(uint32_t* w, uint32_t x, uint32_t mask) {
+  const uint32_t old = __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if ((old ^ x) & mask) __hip_atomic_fetch_xor(w, (old ^ x) & mask, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 __device__ __forceinline__ void put_nibble(uint8_t* codes, long at, int odd, uint32_t code) {
-  uint32_t* w = (uint32_t*)(codes + (at & ~3l));
   const int sh = 8 * (int)(at & 3) + 4 * odd;
-  const uint32_t old = __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) >> sh & 15u;
-  if (old != code) __hip_atomic_fetch_xor(w, (old ^ code) << sh, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  put_bits((uint32_t*)(codes + (at & ~3l)), code << sh, 15u << sh);
+}
+
+// 32 consecutive elements (at any address that aligns one of them): their largest magnitude's exponent and their codes
+__device__ __forceinline__ void load32(const uint16_t* p, float* x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const lsk_u32x4_u u = *(const lsk_u32x4_u*)(p + 8 * i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
+      x[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+    }
+  }
+}
+__device__ __forceinline__ void load32(const float* p, float* x) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const lsk_f32x4_u u = *(const lsk_f32x4_u*)(p + 4 * i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[4 * i + j] = u[j];
+  }
+}
+template <typename T>
+__device__ __forceinline__ int quantise32(const T* p, uint32_t* codes) {
+  float x[32];
+  load32(p, x);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+  const int e = kv4_exponent(m);
+  const float scale = __uint_as_float((uint32_t)e << 23);
+  if (e == 253) {                                    // (as kv4_byte)
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = __builtin_amdgcn_fmed3f(x[i], -0x1.8p127f, 0x1.8p127f);
+  }
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t c = 0;
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[8 * w], x[8 * w + 1], scale, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[8 * w + 2], x[8 * w + 3], scale, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[8 * w + 4], x[8 * w + 5], scale, 2);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[8 * w + 6], x[8 * w + 7], scale, 3);
+    codes[w] = e == 255 ? 0u : c;
+  }
+  return e;
+}
+
+// 8 codes (pairs in bytes) -> values, stored (at any address that aligns one of them)
+__device__ __forceinline__ void store8(uint16_t* p, uint32_t c, float scale) {
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  const bf2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1);
+  const bf2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3);
+  *(lsk_u32x4_u*)p = __builtin_bit_cast(lsk_u32x4_u, (lsk_bf16x8){a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]});
+}
+__device__ __forceinline__ void store8(float* p, uint32_t c, float scale) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  const f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 1);
+  const f2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 3);
+  *(lsk_f32x4_u*)p = (lsk_f32x4_u){a[0], a[1], b[0], b[1]};
+  *(lsk_f32x4_u*)(p + 4) = (lsk_f32x4_u){d[0], d[1], e[0], e[1]};
 }
 
 }  // namespace
 
 #define KV4_THREADS 256
+// Tokens times KV heads from which the kernels for many tokens run (8 heads of 128, a prompt of 1024 / 4001 tokens, append:
+// 5.7 / 7.7 us against 6.2 / 22; single tokens of 32 rows 8.5 us against 3.2)
+#define KV4_MANY 8192
 
-// D / 2 threads a token and head, two dims each; 16 of them find their 32 dims' largest magnitude.
+// Few tokens: D / 2 threads a token and head, two dims each; 16 of them find their 32 dims' largest magnitude.
 template <typename T, int D>
 __global__ __launch_bounds__(KV4_THREADS) void kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v,
                                                                  long st_t, long st_h, uint8_t* __restrict__ kc,
@@ -117,7 +182,186 @@ __global__ __launch_bounds__(KV4_THREADS) void kv4_append_kernel(const T* __rest
   }
 }
 
-// The way back, in the same shape.
+// A workgroup's tokens as groups: runs of positions within 16 aligned ones of a cache row.  first[g] .. first[g + 1] - 1
+// are group g's tokens; returns the number of groups.  row and pos: this thread's token (row -1: outside the cache), held
+// by the first of its NB threads.
+template <int TOK, int NB>
+struct Kv4Groups {
+  int row[TOK], pos[TOK], first[TOK + 1], n;
+  __device__ __forceinline__ void put(int tj, int b, int row_, int pos_) {
+    if (b == 0) {
+      row[tj] = row_;
+      pos[tj] = pos_;
+    }
+  }
+  __device__ __forceinline__ void find(int nt) {     // after put and a barrier, before another; the first wave's work
+    const int l = threadIdx.x;
+    if (l >= 64) return;
+    int at = 0;
+#pragma unroll
+    for (int u = 0; u < TOK; u += 64) {
+      const int j = u + l;
+      const bool begins = j < nt && (j == 0 || row[j] != row[j - 1] || pos[j] != pos[j - 1] + 1 || (pos[j] & 15) == 0);
+      const uint64_t m = __builtin_amdgcn_ballot_w64(begins);
+      if (begins) first[at + __builtin_popcountll(m & ((1ull << l) - 1))] = j;
+      at += __builtin_popcountll(m);
+    }
+    if (l == 0) {
+      first[at] = nt;
+      n = at;
+    }
+  }
+};
+
+// Many tokens: a thread takes 32 dims of a token.  K's codes go straight to their place, 16 bytes (D = 64: twice 8).  V's
+// go through LDS: a workgroup's tokens fall into groups, runs of positions within 16 aligned ones of a cache row (a
+// prompt's groups are whole, a decode step's single tokens), and a wave writes a group at a time, a lane the bytes of two
+// dims.  A dword that other tokens share is put together by an atomic xor of the bits that change.
+template <typename T, int D>
+__global__ __launch_bounds__(KV4_THREADS) void kv4_append_many_kernel(
+    const T* __restrict__ k, const T* __restrict__ v, long st_t, long st_h, uint8_t* __restrict__ kc,
+    uint8_t* __restrict__ vc, uint8_t* __restrict__ ks, uint8_t* __restrict__ vs, const int32_t* __restrict__ rows,
+    const int32_t* __restrict__ pos, int N, int Hkv, int max_batch, int S) {
+  constexpr int NB = D / 32, TOK = KV4_THREADS / NB;  // blocks of 32 dims of a token, tokens of a workgroup
+  constexpr int LD = D / 8 + 1;                       // dwords of a token's codes in LDS
+  __shared__ uint32_t s_c[TOK * LD];
+  __shared__ Kv4Groups<TOK, NB> s_g;
+  const int tid = threadIdx.x, tj = tid / NB, b = tid % NB, h = blockIdx.y, t0 = blockIdx.x * TOK, t = t0 + tj;
+  const int nt = min(TOK, N - t0);
+  int row = -1, p = -1, e = 0;
+  uint32_t c[4] = {0, 0, 0, 0};
+  if (t < N) {
+    row = rows[t];
+    p = pos[t];
+    e = quantise32((blockIdx.z ? k : v) + (long)t * st_t + (long)h * st_h + 32 * b, c);
+  }
+  const bool ok = row >= 0 && row < max_batch && p >= 0 && p < S;
+  const long stripe = ((long)row * Hkv + h) * (long)S;
+  if (blockIdx.z) {                                  // (V's workgroups take longer and start first)
+    if (!ok) return;
+    uint8_t* to = kc + stripe * (D / 2) + kv4_k_offset(p, 32 * b, D);
+    if constexpr (D == 128) {
+      *(lsk_i32x4*)to = (lsk_i32x4){(int)c[0], (int)c[1], (int)c[2], (int)c[3]};
+    } else {                                         // (the next lane group's 16 dims lie 256 bytes on)
+      *(uint2*)to = make_uint2(c[0], c[1]);
+      *(uint2*)(to + 256) = make_uint2(c[2], c[3]);
+    }
+    ks[stripe * NB + kv4_ks_offset(p, 32 * b, D)] = (uint8_t)e;
+    return;
+  }
+  if (ok) vs[stripe * NB + kv4_vs_offset(p, 32 * b, D)] = (uint8_t)e;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) s_c[tj * LD + 4 * b + w] = c[w];
+  s_g.put(tj, b, ok ? row : -1, p);
+  __syncthreads();
+  s_g.find(nt);
+  __syncthreads();
+  constexpr int LANES = D / 2, PER = 64 / LANES;      // lanes of a group, groups of a wave at a time
+  const int lane = tid & 63, l = lane % LANES, fr = l >> 4, l16 = l & 15;
+  for (int g = (tid >> 6) * PER + lane / LANES; g < s_g.n; g += KV4_THREADS / LANES) {
+    const int j0 = s_g.first[g], n = s_g.first[g + 1] - j0, r = s_g.row[j0], q = s_g.pos[j0];
+    if (r < 0) continue;
+    // dims 32 fr + l16 and 16 more: positions q % 16 .. of 16, four bits each
+    uint64_t lo = 0, hi = 0;
+    const uint8_t* src = (const uint8_t*)(s_c + j0 * LD) + 16 * fr + (l16 >> 1);
+    const int odd = 4 * (l16 & 1);
+    for (int i = 0; i < n; ++i, src += 4 * LD) {
+      const int sh = 4 * ((q & 15) + i);
+      lo |= (uint64_t)(src[0] >> odd & 15u) << sh;
+      hi |= (uint64_t)(src[8] >> odd & 15u) << sh;
+    }
+    uint8_t* to = vc + ((long)r * Hkv + h) * (long)S * (D / 2) + kv4_v_offset(q & ~15, 32 * fr + l16, D);
+    if (n == 16) {
+      *(lsk_i32x4*)to = (lsk_i32x4){(int)(uint32_t)lo, (int)(lo >> 32), (int)(uint32_t)hi, (int)(hi >> 32)};
+    } else {
+      const uint64_t mask = ((1ull << (4 * n)) - 1) << (4 * (q & 15));
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t mw = (uint32_t)(mask >> (32 * w)), x = (uint32_t)(lo >> (32 * w)), y = (uint32_t)(hi >> (32 * w));
+        uint32_t* at = (uint32_t*)to + w;
+        if (mw == 0xffffffffu) {
+          at[0] = x;
+          at[2] = y;
+        } else if (mw) {
+          put_bits(at, x, mw);
+          put_bits(at + 2, y, mw);
+        }
+      }
+    }
+  }
+}
+
+// The way back: eight dims of a token a thread, so that a token's are written side by side.  V's groups go through LDS, two
+// lanes exchanging a dim each so that a byte there holds two neighbouring dims.
+template <typename T, int D>
+__global__ __launch_bounds__(KV4_THREADS) void kv4_read_many_kernel(
+    const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, const uint8_t* __restrict__ ks,
+    const uint8_t* __restrict__ vs, const int32_t* __restrict__ rows, const int32_t* __restrict__ pos, T* __restrict__ k,
+    T* __restrict__ v, int N, int Hkv, int max_batch, int S) {
+  constexpr int NB = D / 32, TOK = KV4_THREADS / NB, LD = D / 8 + 1;
+  constexpr int PARTS = D / 8, TP = KV4_THREADS / PARTS, PASSES = TOK / TP;
+  __shared__ uint32_t s_c[TOK * LD];
+  __shared__ Kv4Groups<TOK, 1> s_g;
+  const int tid = threadIdx.x, h = blockIdx.y, t0 = blockIdx.x * TOK, nt = min(TOK, N - t0), d = 8 * (tid % PARTS);
+  const bool is_k = blockIdx.z != 0;
+  uint32_t c[PASSES], e[PASSES];
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int tj = tid / PARTS + i * TP, row = tj < nt ? rows[t0 + tj] : -1, p = tj < nt ? pos[t0 + tj] : -1;
+    const bool ok = row >= 0 && row < max_batch && p >= 0 && p < S;
+    const long stripe = ((long)row * Hkv + h) * (long)S;
+    c[i] = 0;
+    e[i] = 127;
+    if (ok && is_k) {
+      c[i] = *(const uint32_t*)(kc + stripe * (D / 2) + kv4_k_offset(p, d, D));
+      e[i] = ks[stripe * NB + kv4_ks_offset(p, d, D)];
+    } else if (ok) {
+      e[i] = vs[stripe * NB + kv4_vs_offset(p, d, D)];
+    }
+    if (!is_k) {
+      if (!ok) s_c[tj * LD + (d >> 3)] = 0;          // (outside the cache: zeros)
+      s_g.put(tj, tid % PARTS, ok ? row : -1, p);
+    }
+  }
+  if (!is_k) {
+    __syncthreads();
+    s_g.find(nt);
+    __syncthreads();
+    constexpr int LANES = D / 2, PER = 64 / LANES;
+    const int lane = tid & 63, l = lane % LANES, fr = l >> 4, l16 = l & 15;
+    for (int g = (tid >> 6) * PER + lane / LANES; g < s_g.n; g += KV4_THREADS / LANES) {
+      const int j0 = s_g.first[g], n = s_g.first[g + 1] - j0, r = s_g.row[j0], q = s_g.pos[j0];
+      if (r < 0) continue;                           // (LANES lanes at a time)
+      const lsk_i32x4 u = *(const lsk_i32x4*)(vc + ((long)r * Hkv + h) * (long)S * (D / 2) +
+                                              kv4_v_offset(q & ~15, 32 * fr + l16, D));
+      // an even lane takes dims 32 fr + l16 and the next, the odd one beside it those 16 on
+      uint32_t bytes[2][2];                          // [positions 0 .. 7, 8 .. 15][even, odd]
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t mine = (uint32_t)(l16 & 1 ? u[2 + w] : u[w]), give = (uint32_t)(l16 & 1 ? u[w] : u[2 + w]);
+        const uint32_t got = __builtin_amdgcn_mov_dpp(give, 0xb1, 0xf, 0xf, false);  // quad_perm [1, 0, 3, 2]
+        const uint32_t lo = l16 & 1 ? got : mine, hi = l16 & 1 ? mine : got;
+        bytes[w][0] = (lo & 0x0f0f0f0fu) | (hi & 0x0f0f0f0fu) << 4;
+        bytes[w][1] = (lo >> 4 & 0x0f0f0f0fu) | (hi & 0xf0f0f0f0u);
+      }
+      uint8_t* to = (uint8_t*)(s_c + j0 * LD) + 16 * fr + 8 * (l16 & 1) + (l16 >> 1);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int j = i - (q & 15);
+        if (j >= 0 && j < n) to[j * 4 * LD] = (uint8_t)(bytes[i >> 3][i & 1] >> (8 * ((i & 7) >> 1)));
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) c[i] = s_c[(tid / PARTS + i * TP) * LD + (d >> 3)];
+  }
+  T* to = (is_k ? k : v) + ((long)(t0 + tid / PARTS) * Hkv + h) * D + d;
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i)
+    if (tid / PARTS + i * TP < nt) store8(to + (long)i * TP * Hkv * D, c[i], __uint_as_float(e[i] << 23));
+}
+
+// The way back for few tokens.
 template <typename T, int D>
 __global__ __launch_bounds__(KV4_THREADS) void kv4_read_kernel(const uint8_t* __restrict__ kc,
                                                                const uint8_t* __restrict__ vc,
@@ -194,10 +438,12 @@ static int kv4_args(const char* what, int dtype, const void* k, const void* v, c
   return 0;
 }
 
-#define KV4_LAUNCH(KERNEL, T, ...)                                                  \
-  do {                                                                              \
-    if (head_dim == 128) KERNEL<T, 128><<<grid, KV4_THREADS, 0, st>>>(__VA_ARGS__); \
-    else KERNEL<T, 64><<<grid, KV4_THREADS, 0, st>>>(__VA_ARGS__);                  \
+#define KV4_LAUNCH(NAME, T, ...)                                                               \
+  do {                                                                                         \
+    if (head_dim == 128 && many) NAME##_many_kernel<T, 128><<<grid, KV4_THREADS, 0, st>>>(__VA_ARGS__); \
+    else if (head_dim == 128) NAME##_kernel<T, 128><<<grid, KV4_THREADS, 0, st>>>(__VA_ARGS__); \
+    else if (many) NAME##_many_kernel<T, 64><<<grid, KV4_THREADS, 0, st>>>(__VA_ARGS__);        \
+    else NAME##_kernel<T, 64><<<grid, KV4_THREADS, 0, st>>>(__VA_ARGS__);                       \
   } while (0)
 
 extern "C" int lsk_kv4_append(int dtype, const void* k, const void* v, long stride_t, long stride_h, void* k4, void* v4,
@@ -208,14 +454,15 @@ extern "C" int lsk_kv4_append(int dtype, const void* k, const void* v, long stri
                         max_seq)) return rc;
   LSK_REQUIRE(stride_t >= 0 && stride_h >= 0, LSK_ESHAPE, "%s: negative strides", what);
   if (n_tokens == 0) return 0;
-  const int per = KV4_THREADS / (head_dim / 2);
+  const bool many = (long)n_tokens * n_kv_heads >= KV4_MANY;
+  const int per = KV4_THREADS / (many ? head_dim / 32 : head_dim / 2);
   const dim3 grid((n_tokens + per - 1) / per, n_kv_heads, 2);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == LSK_DTYPE_BF16)
-    KV4_LAUNCH(kv4_append_kernel, uint16_t, (const uint16_t*)k, (const uint16_t*)v, stride_t, stride_h, (uint8_t*)k4,
+    KV4_LAUNCH(kv4_append, uint16_t, (const uint16_t*)k, (const uint16_t*)v, stride_t, stride_h, (uint8_t*)k4,
                (uint8_t*)v4, (uint8_t*)k_exp, (uint8_t*)v_exp, rows, pos, n_tokens, n_kv_heads, max_batch, max_seq);
   else
-    KV4_LAUNCH(kv4_append_kernel, float, (const float*)k, (const float*)v, stride_t, stride_h, (uint8_t*)k4,
+    KV4_LAUNCH(kv4_append, float, (const float*)k, (const float*)v, stride_t, stride_h, (uint8_t*)k4,
                (uint8_t*)v4, (uint8_t*)k_exp, (uint8_t*)v_exp, rows, pos, n_tokens, n_kv_heads, max_batch, max_seq);
   return lsk_check_launch(what);
 }
@@ -227,14 +474,15 @@ extern "C" int lsk_kv4_read(int dtype, const void* k4, const void* v4, const voi
   if (int rc = kv4_args(what, dtype, k, v, k4, v4, k_exp, v_exp, rows, pos, n_tokens, n_kv_heads, head_dim, max_batch,
                         max_seq)) return rc;
   if (n_tokens == 0) return 0;
-  const int per = KV4_THREADS / (head_dim / 2);
+  const bool many = (long)n_tokens * n_kv_heads >= KV4_MANY;
+  const int per = KV4_THREADS / (many ? head_dim / 32 : head_dim / 2);
   const dim3 grid((n_tokens + per - 1) / per, n_kv_heads, 2);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == LSK_DTYPE_BF16)
-    KV4_LAUNCH(kv4_read_kernel, uint16_t, (const uint8_t*)k4, (const uint8_t*)v4, (const uint8_t*)k_exp,
+    KV4_LAUNCH(kv4_read, uint16_t, (const uint8_t*)k4, (const uint8_t*)v4, (const uint8_t*)k_exp,
                (const uint8_t*)v_exp, rows, pos, (uint16_t*)k, (uint16_t*)v, n_tokens, n_kv_heads, max_batch, max_seq);
   else
-    KV4_LAUNCH(kv4_read_kernel, float, (const uint8_t*)k4, (const uint8_t*)v4, (const uint8_t*)k_exp,
+    KV4_LAUNCH(kv4_read, float, (const uint8_t*)k4, (const uint8_t*)v4, (const uint8_t*)k_exp,
                (const uint8_t*)v_exp, rows, pos, (float*)k, (float*)v, n_tokens, n_kv_heads, max_batch, max_seq);
   return lsk_check_launch(what);
 }
