@@ -101,10 +101,21 @@ __device__ __forceinline__ lsk_bf16x8 codes4_to_bf16(uint32_t x, float scale) {
 }
 
 __device__ __forceinline__ float exp_bits(uint32_t byte) { return __uint_as_float(byte << 23); }
-// the exponent that byte i of four dwords holds
-__device__ __forceinline__ float exp_of(const lsk_i32x4& b, int i) {
-  return exp_bits(((uint32_t)b[i >> 2] >> (8 * (i & 3))) & 255u);
+// 2^(byte - 127) of byte k of a dword (the compiler takes two instructions for most bytes)
+__device__ __forceinline__ float exp_byte(uint32_t dw, int k) {
+  float r;
+#define EXP_BYTE(K)                                                                                                 \
+  asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_" #K : "=v"(r) \
+      : "v"(23), "v"(dw))
+  if (k == 0) EXP_BYTE(0);
+  else if (k == 1) EXP_BYTE(1);
+  else if (k == 2) EXP_BYTE(2);
+  else EXP_BYTE(3);
+#undef EXP_BYTE
+  return r;
 }
+// the scale that byte i of four dwords holds
+__device__ __forceinline__ float exp_of(const lsk_i32x4& b, int i) { return exp_byte((uint32_t)b[i >> 2], i & 3); }
 // 8 e2m1 codes of consecutive positions -> bf16, each times its own power of two (bytes 8 hv .. of b)
 __device__ __forceinline__ lsk_bf16x8 codes4_to_bf16(uint32_t x, const lsk_i32x4& b, int hv) {
   typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
@@ -240,10 +251,12 @@ __device__ __forceinline__ void add_odd(const CacheAttnArgs& A, const Stripe& st
 
 // The online softmax of one tile's 16 query columns over a step: s[a][e] are the scores of this lane's slots 4 a + e,
 // of which `reads` says what the column reads (FULL: all), vsr V's exponents of the slots (8-bit); pb the weights for
-// the second product (4-bit: s takes them, before V's scales).  A row's m only moves when a score passes it by more than LAG (weights up to 2^LAG; each row for
-// itself, so the rows of a tile stay independent), which is seldom after the first step: then no maximum crosses lanes
-// and nothing is rescaled.  Each lane sums its own slots' weights.
-template <int FMT, bool FULL, int NA, int CT, int HV>
+// the second product (4-bit: s takes them, before V's scales).  A row's m only moves when a score passes it by more
+// than LAG (weights up to 2^LAG; each row for itself, so the rows of a tile stay independent), which is seldom after the
+// first step: then no maximum crosses lanes and nothing is rescaled.  Each lane sums its own slots' weights.  FAR (4-bit
+// caches): from 2^26 on, where the rounding of m alone could lift a weight past 2^LAG, the scores are rounded before m
+// is subtracted.
+template <int FMT, bool FULL, bool FAR, int NA, int CT, int HV>
 __device__ __forceinline__ void softmax_tile(lsk_f32x4 (&s)[NA], uint32_t reads, lsk_i32x4 vsr, float scale_log2,
                                              float& m, float& l, lsk_f32x4 (&o)[CT], lsk_bf16x8 (&pb)[HV]) {
   float mt = -INFINITY;
@@ -253,21 +266,29 @@ __device__ __forceinline__ void softmax_tile(lsk_f32x4 (&s)[NA], uint32_t reads,
     mt = fmaxf(mt, s[i >> 2][i & 3]);
   }
   mt *= scale_log2;
-  if (__builtin_amdgcn_ballot_w64(mt > m + LAG) != 0ull) {
+  const bool far = FAR && fabsf(mt) > 0x1p26f;
+  float mm = m;
+  if (__builtin_amdgcn_ballot_w64(mt > m + LAG || far) != 0ull) {
     mt = rows_max(mt);
     const bool up = mt > m + LAG;
     const float alpha = up ? fast_exp2(m - mt) : 1.f;
-    m = up ? mt : m;
+    mm = m = up ? mt : m;
     l *= alpha;
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[c][i] *= alpha;
+    if constexpr (FAR)
+      if (far) {
+        mm = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4 * NA; ++i) s[i >> 2][i & 3] = (s[i >> 2][i & 3] * scale_log2 - m) * (1.f / scale_log2);
+      }
   }
   float rs = 0.f;
 #pragma unroll
   for (int i = 0; i < 4 * NA; ++i) {
-    float pe = fast_exp2(__builtin_fmaf(s[i >> 2][i & 3], scale_log2, -m));
+    float pe = fast_exp2(__builtin_fmaf(s[i >> 2][i & 3], scale_log2, -mm));
     if constexpr (!FULL) pe = (reads >> i) & 1u ? pe : 0.f;
     rs += pe;
     if constexpr (FMT == FMT_KV4) {
@@ -458,10 +479,12 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
       }
       return bits;
     };
-    // One step.  FULL: every row reads all of its slots.  All QT tiles are computed,
-    // also those without rows (copies of the loop for fewer tiles cost more in registers than they save).
-    auto step = [&](auto full_, int sb) {
+    // One step.  FULL: every row reads all of its slots.  All QT tiles are computed, also those without rows (copies of
+    // the loop for fewer tiles cost more in registers than they save); over a 4-bit cache, which leaves registers, only
+    // one for items of up to 16 rows (256 requests of 1 to 9 tokens, 8B heads: 142 us against 136).
+    auto step = [&](auto full_, auto nq_, int sb) {
       constexpr bool FULL = decltype(full_)::value;
+      constexpr int NQ = decltype(nq_)::value;
       // In a step that some row does not read whole, a slot whose V holds an infinity or NaN must not reach the rows
       // that do not read it (0 x NaN): the values past the item and the non-finite ones are cleared here, and the rows
       // that do read such a value get it after the products (below).
@@ -475,7 +498,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
       const int s0 = sb + NE * lg, sn = sb + stride;
       uint32_t reads[QT];                            // (the mask's words are asked for before the products)
 #pragma unroll
-      for (int qt = 0; qt < QT; ++qt) reads[qt] = FULL ? ALL : allow(qt, s0);
+      for (int qt = 0; qt < NQ; ++qt) reads[qt] = FULL ? ALL : allow(qt, s0);
       lsk_f32x4 sacc[QT][2 * HV];
 #pragma unroll
       for (int a = 0; a < 2 * HV; ++a) {
@@ -491,7 +514,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
           ORDER();
           load_k(sr, sn, a);
         } else if constexpr (KV4) {
-          const float sc = exp_bits(((uint32_t)ksr[0] >> (8 * a)) & 255u);
+          const float sc = exp_byte((uint32_t)ksr[0], a);
 #pragma unroll
           for (int f = 0; f < KF; ++f) kf[f] = codes4_to_bf16((uint32_t)kr[(a * KF + f) >> 2][(a * KF + f) & 3], sc);
           ORDER();
@@ -501,7 +524,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
           for (int f = 0; f < KF; ++f) kf[f] = __builtin_bit_cast(lsk_bf16x8, kr[a * KF + f]);
         }
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
+        for (int qt = 0; qt < NQ; ++qt) {
           lsk_f32x4 acc = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int f = 0; f < KF; ++f) {
@@ -519,9 +542,9 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
       }
       lsk_bf16x8 pb[QT][HV];
 #pragma unroll
-      for (int qt = 0; qt < QT; ++qt) {
+      for (int qt = 0; qt < NQ; ++qt) {
         if constexpr (CODES) ORDER();
-        softmax_tile<FMT, FULL>(sacc[qt], reads[qt], vsr[0], A.scale_log2, m_run[qt], l_run[qt], oacc[qt], pb[qt]);
+        softmax_tile<FMT, FULL, KV4>(sacc[qt], reads[qt], vsr[0], A.scale_log2, m_run[qt], l_run[qt], oacc[qt], pb[qt]);
       }
       ORDER();
       if constexpr (!KV4) load_vs(sr, sn);
@@ -532,7 +555,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
         if constexpr (KV4) {
           if (c % 2 == 0) {                          // the weights times the scales of these 32 dims
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
+            for (int qt = 0; qt < NQ; ++qt)
 #pragma unroll
               for (int i = 0; i < NE; ++i) {
                 float pv = sacc[qt][i >> 2][i & 3] * exp_of(vsr[c / 2], i);
@@ -551,7 +574,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
 #pragma unroll
         for (int hv = 0; hv < HV; ++hv)
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
+          for (int qt = 0; qt < NQ; ++qt)
             oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[hv], pb[qt][hv], oacc[qt][c], 0, 0, 0);
         if constexpr (!KV4) load_v(sr, sn, c);
         else if (c % 2 == 1) load_v(sr, sn, c / 2);
@@ -563,8 +586,12 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
       }
     };
     int sb = first_step(cur);
-    for (; sb + STEP - 1 <= full_lim; sb += stride) step(std::true_type{}, sb);
-    for (; sb < kv_hi; sb += stride) step(std::false_type{}, sb);
+    auto steps = [&](auto nq_) {
+      for (; sb + STEP - 1 <= full_lim; sb += stride) step(std::true_type{}, nq_, sb);
+      for (; sb < kv_hi; sb += stride) step(std::false_type{}, nq_, sb);
+    };
+    if (KV4 && QT > 1 && cur.nrows - rb <= 16) steps(std::integral_constant<int, 1>{});
+    else steps(std::integral_constant<int, QT>{});
     // the next item's Q and first K / V loads fly while this item is merged
     const Item done = cur;
     cur = nxt;
@@ -647,6 +674,44 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
   }
 }
 
+// The end of an item of cache_tree_kernel: a wave's rows, from rb on, or its part of them
+template <bool TREE, int QT, int CT>
+__device__ __forceinline__ void tree_store(const CacheAttnArgs& A, const lsk_f32x4 (&oacc)[QT][CT], const float (&m_run)[QT],
+                                           float (&l_run)[QT], int q_start, int row0, int nrows, int rb, int kvh, int part,
+                                           int pos0) {
+  constexpr int D = 16 * CT;
+  const int l16 = threadIdx.x & 15, lg = (threadIdx.x & 63) >> 4, G = A.G, Hkv = A.Hkv;
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) l_run[qt] = rows_sum(l_run[qt]);
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int rl = rb + 16 * qt + l16;
+    if (rl >= nrows) continue;
+    const int r = row0 + rl, t = r / G, g = r - t * G;
+    float L = l_run[qt];
+    if constexpr (TREE)
+      if (L == 0.f && part < 0 && !reads_any(A.mask + (long)(q_start + t) * A.W, A.W, t, pos0)) L = 1.f;
+    const long slot = ((long)part * Hkv + kvh) * A.part_rows + rl;
+    uint16_t* o = A.out + ((long)(q_start + t) * G * Hkv + kvh * G + g) * D + 4 * lg;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const lsk_f32x4 v = oacc[qt][c];
+      if (part < 0) {
+        lsk_u32x2_u pk;
+        pk[0] = (uint32_t)f2bf(v[0] / L) | ((uint32_t)f2bf(v[1] / L) << 16);
+        pk[1] = (uint32_t)f2bf(v[2] / L) | ((uint32_t)f2bf(v[3] / L) << 16);
+        *(lsk_u32x2_u*)(o + 16 * c) = pk;
+      } else {
+        *(lsk_f32x4*)(A.o_part + slot * D + 16 * c + 4 * lg) = v;
+      }
+    }
+    if (part >= 0 && lg == 0) {
+      A.ml_part[slot * 2 + 0] = m_run[qt];
+      A.ml_part[slot * 2 + 1] = l_run[qt];
+    }
+  }
+}
+
 // Trees of more rows: an item of four row groups of 32 rows, a wave each, which read the same K and V.  These go
 // through LDS, a step's at a time (8-bit: two steps'), in two buffers: a wave that reads them for itself takes its
 // share of the CU's 64 bytes per clock (32 trees of 25 to 64 nodes, 8B heads, 128 to 1280 positions: 67 us without LDS,
@@ -657,7 +722,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
 // workgroup of its own and all are resident at once (those 32 trees: 480 items, 23 to 28 us of such work a CU, 40 on
 // the fullest).
 #define TREE_WAVES 4
-template <int D, int FMT>
+template <int D, int FMT, bool TREE>
 __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const CacheAttnArgs A,
                                                                         const int32_t* __restrict__ items) {
   constexpr int KF = D / 32, CT = D / 16, NW = TREE_WAVES, QT = 2;
@@ -684,8 +749,8 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
   lsk_i32x4 st_s[UPW];                               // 4-bit: exponents of this lane's K (a dword) or V
   auto st_load = [&](int sb) {
 #pragma unroll
-    for (int i = 0; i < UPW; ++i) {                  // (a wave's fragments are all of K or all of V)
-      const int w = wave * UPW + i;
+    for (int i = 0; i < UPW; ++i) {                  // (all of K or all of V; 4-bit: one of each, V's cost more)
+      const int w = KV4 ? wave + NW * i : wave * UPW + i;
       const int so = (KV4 ? sb / 2 : KV8 ? sb : 2 * sb) * D + w % LT * 1024;
       st[i] = __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(
                                                 w < LT ? sr.k : sr.v, w < LT || KV4 ? 16 * lane : 64 * l16 + 16 * lg, so,
@@ -708,7 +773,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
     char* to = s_buf + buf * BUF + 16 * lane;
 #pragma unroll
     for (int i = 0; i < UPW; ++i) {
-      const int u = wave * UPW + i;
+      const int u = KV4 ? wave + NW * i : wave * UPW + i;
       if constexpr (KV4) {                           // both with their scales
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -716,7 +781,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
           if (u < LT) {                              // dword w: tile g / KF, operand g % KF
             const int g = 4 * u + w, a = g / KF;
             *(lsk_bf16x8*)(to + (a >> 1) * HALF + ((a & 1) * KF + g % KF) * 1024) =
-                codes4_to_bf16(x, exp_bits(((uint32_t)st_s[i][0] >> (8 * a)) & 255u));
+                codes4_to_bf16(x, exp_byte((uint32_t)st_s[i][0], a));
           } else {                                   // rows 32 (u - LT) + 16 (w / 2) + l16, positions 16 lg + 8 (w % 2) ..
             *(lsk_bf16x8*)(to + (w & 1) * HALF + (CT + 2 * (u - LT) + (w >> 1)) * 1024) =
                 codes4_to_bf16(x, st_s[i], w & 1);
@@ -770,8 +835,8 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
       reads[qt] = ALL;
       if constexpr (!FULL) {
         const int n = min(kv_hi - 1, qpos[qt]) - s0 + 1, t = max(qpos[qt] - pos0, 0);
-        reads[qt] = (n >= NE ? ALL : n <= 0 ? 0u : (1u << n) - 1u) &
-                    mask_window(A.mask + (long)(q_start + t) * A.W, A.W, s0 - pos0);
+        reads[qt] = n >= NE ? ALL : n <= 0 ? 0u : (1u << n) - 1u;
+        if constexpr (TREE) reads[qt] &= mask_window(A.mask + (long)(q_start + t) * A.W, A.W, s0 - pos0);
       }
     }
     lsk_f32x4 sacc[QT][2];
@@ -802,7 +867,8 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
     lsk_bf16x8 pb[QT][1];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
-      softmax_tile<KV4 ? FMT_BF16 : FMT, FULL>(sacc[qt], reads[qt], vsr, A.scale_log2, m_run[qt], l_run[qt], oacc[qt], pb[qt]);
+      softmax_tile<KV4 ? FMT_BF16 : FMT, FULL, KV4>(sacc[qt], reads[qt], vsr, A.scale_log2, m_run[qt], l_run[qt],
+                                                      oacc[qt], pb[qt]);
     uint64_t odd = 0;                                // (V is bf16 here in all formats)
     if constexpr (!FULL) odd = clear_odd<false>(vr, kv_hi - s0);
 #pragma unroll
@@ -812,8 +878,10 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
         oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lsk_bf16x8, vr[c]), pb[qt][0],
                                                               oacc[qt][c], 0, 0, 0);
     if constexpr (!FULL)
-      add_odd<FMT, true>(A, sr, odd, s2 + (CODES ? 8 : 32) * j, q_start, pos0, qpos, oacc, CODES ? 0x18 : 0);
+      add_odd<FMT, TREE>(A, sr, odd, s2 + (CODES ? 8 : 32) * j, q_start, pos0, qpos, oacc, CODES ? 0x18 : 0);
   };
+  // behind the last slot that a row of the wave reads (0: no rows)
+  const int wave_hi = rb >= nrows ? 0 : TREE ? kv_hi : min(kv_hi, pos0 + (row0 + min(rb + 16 * QT, nrows) - 1) / G + 1);
   st_write(0);
   st_load(kv_lo + CHUNK);
   int s2 = kv_lo, buf = 0;
@@ -822,43 +890,191 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
       __syncthreads();                               // (the other buffer's readers are done, this one is written)
 #pragma nounroll
       for (int j = 0; j < STEPS; ++j) {
-        if (s2 + 8 * j >= kv_hi || rb >= nrows) break;
+        if (s2 + 8 * j >= wave_hi) break;
         step(full_, s2, j, buf);
       }
       st_write(buf ^ 1);
       st_load(s2 + 2 * CHUNK);
     }
   };
-  chunks(std::true_type{}, min(kv_hi, pos0) - CHUNK + 1);  // (every row reads them whole)
+  chunks(std::true_type{}, min(kv_hi, TREE ? pos0 : pos0 + row0 / G + 1) - CHUNK + 1);  // (every row reads them whole)
   chunks(std::false_type{}, kv_hi);
+  tree_store<TREE>(A, oacc, m_run, l_run, q_start, row0, nrows, rb, kvh, part, pos0);
+}
+
+// The same over a 4-bit cache of 128 dims, without a mask (TREE false) or with one.  A lane's 32 codes of K and their scale
+// are an operand of the scaled matrix instruction (v_mfma_scale_f32_16x16x128_f8f6f4: 16 positions x 128 dims), so K is
+// neither converted nor staged.  Its partner Q is given as two e4m3 numbers per value, q = 2^e (hi + lo / 16) with a
+// power of two for every 32 dims of a row: hi holds the upper four of a bf16 value's eight bits, lo the rest, exactly
+// for values down to 2^-15 of the 32 dims' largest; below, off by at most 2^-21 of that.  An infinity becomes NaN: the
+// row's result is NaN either way.  Lane group lg's operand of Q is dims 16 lg .. + 15 and 64 + 16 lg .. + 15 (of K's codes,
+// dims 32 lg .. + 31), its scale that of dims 32 lg .. + 31.  V goes through LDS as bf16 with its scales, 64 positions at
+// a time, a quarter of the dims a wave.  (8B heads: a prompt of 1001 tokens after 1000 62 -> 56 us against the kernel
+// above over 4 bits, 32 trees of 64 nodes 55 -> 46.)
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ void split_q(const uint16_t* q, int lg, i32x8& hi, i32x8& lo, int& exps) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  int e[2];
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) l_run[qt] = rows_sum(l_run[qt]);
+  for (int hv = 0; hv < 2; ++hv) {                   // dims 64 hv + 16 lg .. + 15
+    float x[16];
+    uint32_t m = 0;
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    const int rl = rb + 16 * qt + l16;
-    if (rl >= nrows) continue;
-    const int r = row0 + rl, t = r / G, g = r - t * G;
-    float L = l_run[qt];
-    if (L == 0.f && part < 0 && !reads_any(A.mask + (long)(q_start + t) * A.W, A.W, t, pos0)) L = 1.f;
-    const long slot = ((long)part * Hkv + kvh) * A.part_rows + rl;
-    uint16_t* o = A.out + ((long)(q_start + t) * G * Hkv + kvh * G + g) * D + 4 * lg;
+    for (int i = 0; i < 2; ++i) {
+      const lsk_u32x4_u u = *(const lsk_u32x4_u*)(q + 64 * hv + 16 * lg + 8 * i);
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      const lsk_f32x4 v = oacc[qt][c];
-      if (part < 0) {
-        lsk_u32x2_u pk;
-        pk[0] = (uint32_t)f2bf(v[0] / L) | ((uint32_t)f2bf(v[1] / L) << 16);
-        pk[1] = (uint32_t)f2bf(v[2] / L) | ((uint32_t)f2bf(v[3] / L) << 16);
-        *(lsk_u32x2_u*)(o + 16 * c) = pk;
-      } else {
-        *(lsk_f32x4*)(A.o_part + slot * D + 16 * c + 4 * lg) = v;
+      for (int j = 0; j < 4; ++j) {
+        x[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
+        x[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
       }
     }
-    if (part >= 0 && lg == 0) {
-      A.ml_part[slot * 2 + 0] = m_run[qt];
-      A.ml_part[slot * 2 + 1] = l_run[qt];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));  // (32 dims are two lanes')
+    // the smallest e >= 10 - 127 with amax <= 448 * 2^e (biased; lo's is four less)
+    const bool odd = m >= 0x7f800000u;
+    e[hv] = max(odd ? 127 : (int)(m >> 23) - 8 + ((m & 0x7fffffu) > 0x600000u ? 1 : 0), 10);
+    const float inv = __uint_as_float((uint32_t)(254 - e[hv]) << 23);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = odd ? __builtin_nanf("") : x[4 * w + i] * inv;
+      int h = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+      h = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], h, true);
+      const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
+      int l = __builtin_amdgcn_cvt_pk_fp8_f32((y[0] - a[0]) * 16.f, (y[1] - a[1]) * 16.f, 0, false);
+      l = __builtin_amdgcn_cvt_pk_fp8_f32((y[2] - b[0]) * 16.f, (y[3] - b[1]) * 16.f, l, true);
+      hi[4 * hv + w] = h;
+      lo[4 * hv + w] = l;
     }
   }
+  // lane group lg gives the power of dims 32 lg .. + 31: that of lane groups 2 (lg % 2) .. + 1 in their half lg / 2
+  const int other = __shfl_xor(lg == 2 ? e[0] : e[1], 48, 64);
+  const int mine = lg == 0 ? e[0] : lg == 3 ? e[1] : other;
+  exps = mine | (mine - 4) << 8;
+}
+
+template <bool TREE>
+__global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree4_kernel(const CacheAttnArgs A,
+                                                                         const int32_t* __restrict__ items) {
+  constexpr int D = 128, CT = D / 16, QT = 2, CHUNK = 64, NE = 16;
+  constexpr uint32_t ALL = 0xffffu;
+  constexpr int HALF = CT * 1024, BUF = 2 * HALF;    // V fragments (half hv of a lane group's 16 positions, c)
+  __shared__ __attribute__((aligned(16))) char s_v[2 * BUF];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = A.G, Hkv = A.Hkv;
+  const int32_t* wk = items + (long)blockIdx.x * 8;
+  const int q_start = wk[0], row0 = wk[1], nrows = wk[2] & 1023, kvh = wk[2] >> 12;
+  const int kv_lo = wk[3], kv_hi = wk[4], part = wk[5], pos0 = wk[6], crow = wk[7];
+  const int rb = wave * 16 * QT;
+  const Stripe sr = cache_stripe<D, FMT_KV4>(A, crow, kvh, kv_hi);
+  lsk_i32x4 kr[4], vs, v;                            // K of this chunk, V of the one being staged (this wave's 32 dims)
+  int ks;
+  auto ld = [&](__amdgpu_buffer_rsrc_t rs, int vo, int so) {
+    return __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, vo, so, 0));
+  };
+  auto load_k = [&](int sb) {
+#pragma unroll
+    for (int a = 0; a < 4; ++a) kr[a] = ld(sr.k, 16 * lane, sb / 2 * D + a * 1024);
+    ks = (int)__builtin_amdgcn_raw_buffer_load_b32(sr.ks, 4 * lane, sb * (D / 32), 0);
+  };
+  auto load_v = [&](int sb) {
+    v = ld(sr.v, 16 * lane, sb / 2 * D + wave * 1024);
+    vs = ld(sr.vs, 16 * lg, sb * (D / 32) + 64 * wave);
+  };
+  auto write_v = [&](int buf) {                      // rows 32 wave + 16 (w / 2) + l16, positions 16 lg + 8 (w % 2) ..
+    char* to = s_v + buf * BUF + 16 * lane + 2 * wave * 1024;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      *(lsk_bf16x8*)(to + (w & 1) * HALF + (w >> 1) * 1024) = codes4_to_bf16((uint32_t)v[w], vs, w & 1);
+  };
+  load_v(kv_lo);
+  load_k(kv_lo);
+  i32x8 qh[QT], ql[QT];
+  int qe[QT], qpos[QT];                              // the row's own slot; -1: no such row
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int rl = rb + 16 * qt + l16, r = row0 + min(rl, nrows - 1), t = r / G, g = r - t * G;
+    qpos[qt] = rl < nrows ? pos0 + t : -1;
+    split_q(A.q + (long)(q_start + t) * A.q_st + (long)(kvh * G + g) * A.q_sh, lg, qh[qt], ql[qt], qe[qt]);
+  }
+  // behind the last slot that a row of the wave reads (0: no rows)
+  const int wave_hi = rb >= nrows ? 0 : TREE ? kv_hi : min(kv_hi, pos0 + (row0 + min(rb + 16 * QT, nrows) - 1) / G + 1);
+  lsk_f32x4 oacc[QT][CT];
+  float m_run[QT], l_run[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    m_run[qt] = M_NONE;
+    l_run[qt] = 0.f;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) oacc[qt][c] = (lsk_f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  auto step = [&](auto full_, int s2, int buf) {
+    constexpr bool FULL = decltype(full_)::value;
+    const int s0 = s2 + 16 * lg;                     // this lane's slots s0 .. s0 + 15
+    uint32_t reads[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      reads[qt] = ALL;
+      if constexpr (!FULL) {
+        const int n = min(kv_hi - 1, qpos[qt]) - s0 + 1, t = max(qpos[qt] - pos0, 0);
+        reads[qt] = n >= NE ? ALL : n <= 0 ? 0u : (1u << n) - 1u;
+        if constexpr (TREE) reads[qt] &= mask_window(A.mask + (long)(q_start + t) * A.W, A.W, s0 - pos0);
+      }
+    }
+    lsk_f32x4 sacc[QT][4];
+    const lsk_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#define TREE4_TILE(AA)                                                                                           \
+  {                                                                                                              \
+    const i32x8 k8 = __builtin_shufflevector(kr[AA], kr[AA], 0, 1, 2, 3, -1, -1, -1, -1);                          \
+    _Pragma("unroll") for (int qt = 0; qt < QT; ++qt) sacc[qt][AA] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4( \
+        k8, qh[qt], zero, 4, 0, AA, ks, 0, qe[qt]);                                                              \
+    _Pragma("unroll") for (int qt = 0; qt < QT; ++qt) sacc[qt][AA] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4( \
+        k8, ql[qt], sacc[qt][AA], 4, 0, AA, ks, 1, qe[qt]);                                                      \
+  }
+    TREE4_TILE(0) TREE4_TILE(1) TREE4_TILE(2) TREE4_TILE(3)
+#undef TREE4_TILE
+    ORDER();
+    load_k(s2 + CHUNK);
+    lsk_bf16x8 pb[QT][2];
+    lsk_i32x4 none = {0, 0, 0, 0};
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+      softmax_tile<FMT_BF16, FULL, true>(sacc[qt], reads[qt], none, A.scale_log2, m_run[qt], l_run[qt], oacc[qt], pb[qt]);
+#pragma unroll
+    for (int hv = 0; hv < 2; ++hv) {
+      const char* src = s_v + buf * BUF + hv * HALF + 16 * lane;
+      lsk_i32x4 vr[CT];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) vr[c] = *(const lsk_i32x4*)(src + c * 1024);
+      uint64_t odd = 0;
+      if constexpr (!FULL) odd = clear_odd<false>(vr, kv_hi - (s0 + 8 * hv));
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+          oacc[qt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lsk_bf16x8, vr[c]), pb[qt][hv],
+                                                                oacc[qt][c], 0, 0, 0);
+      if constexpr (!FULL) add_odd<FMT_KV4, TREE>(A, sr, odd, s2 + 8 * hv, q_start, pos0, qpos, oacc, 0x18);
+    }
+  };
+  write_v(0);
+  load_v(kv_lo + CHUNK);
+  int s2 = kv_lo, buf = 0;
+  auto chunks = [&](auto full_, int end) {           // those that start before `end`
+    for (; s2 < end; s2 += CHUNK, buf ^= 1) {
+      __syncthreads();                               // (the other buffer's readers are done, this one is written)
+      if (s2 < wave_hi) step(full_, s2, buf);
+      write_v(buf ^ 1);
+      load_v(s2 + 2 * CHUNK);
+    }
+  };
+  chunks(std::true_type{}, min(kv_hi, TREE ? pos0 : pos0 + row0 / G + 1) - CHUNK + 1);  // (every row reads them whole)
+  chunks(std::false_type{}, kv_hi);
+  tree_store<TREE>(A, oacc, m_run, l_run, q_start, row0, nrows, rb, kvh, part, pos0);
 }
 
 // Merge the splits of a row in split order: M = max_s m_s, w_s = exp2(m_s - M), out = sum w_s O_s / sum w_s l_s (zeros
@@ -1077,8 +1293,18 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 //           positions, 4 / 2 / 1 row groups: 64 stripes, 64-node trees 30 / 22 / 21 us; 128 stripes, 32 nodes
 //           29 / 22 / 21, 64 nodes 32 / 34 / 37; 256 stripes, 16 nodes - / 29 / 26, 32 nodes 31 / 34 / 37, 64 nodes
 //           46 / 60 / 69).
+//   wide    a block of more than 64 rows without a mask over a 4-bit cache (a piece of a prompt), where the cache's
+//           stripes times the block's tiles of 32 rows are more than WIDE_TILES: items of 128 rows for the tree kernels,
+//           whose waves share the conversions of K and V (8B heads after 1000 positions, wide / not, unsplit: 256 stripes
+//           of 64 tokens 52 / 83 us, 64 stripes of 256 54 / 88; equal at 1024 tiles, 64 stripes of 128 44 / 45; behind at
+//           512, 64 stripes of 64 35 / 25 and 8 of 512 40 / 26; in two splits at 512 tiles 34 / 35; 17 tokens in 256
+//           stripes 39 / 38; 1B heads: 64 stripes of 128 tokens 37 / 32, of 256 44 / 60).  The cache full of such blocks has 192 items and more, so its splits are of WIDE_SPLIT
+//           positions at least (8 stripes, a prompt of 4001 tokens: 640 positions 218 us, 1280 174, 2560 155, whole 142;
+//           the other way round for one short piece in a large cache: 256 tokens after 5000 whole 107, 2560 63).
 // The number of row groups follows from the block's rows and the cache alone, so it never makes a row's result depend
 // on the batch.  Items go longest first to the least-loaded of n_slots persistent workgroups, as in lsk_attn_schedule.
+#define WIDE_TILES(D) ((D) == 64 ? 1280 : 768)
+#define WIDE_SPLIT 4096
 static int cache_plan(const char* what, const int32_t* blocks, int nb, int group, int split, int max_batch,
                       int n_kv_heads, int head_dim, int format, int tree, int row_groups, int n_slots, int32_t* meta,
                       long meta_cap, long* counts) {
@@ -1104,6 +1330,16 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
     most = T * group > most ? T * group : most;
     n_tokens += T;
   }
+  const auto wide = [&](long rows) {
+    return format == FMT_KV4 && !tree && rows > 64 && (long)max_batch * n_kv_heads * ((rows + 31) / 32) > WIDE_TILES(head_dim);
+  };
+  if (wide(most)) {                                  // (the other blocks' tiles)
+    most = 0;
+    for (int b = 0; b < nb; ++b) {
+      const long rows = (long)blocks[(long)b * 4 + 2] * group;
+      if (!wide(rows) && rows > most) most = rows;
+    }
+  }
   const int tiles = most <= 16 ? 1 : most <= 32 || tree || head_dim == 128 ? 2 : 3;
   struct It { int32_t rec[8]; int cost; };
   thread_local std::vector<It> items, shared;
@@ -1121,12 +1357,17 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
     const bool few = (long)max_batch * n_kv_heads * ((rows + 31) / 32) <= n_slots;
     const int most_groups = row_groups ? row_groups : few ? 1 : 4;
     while (tree && (1 << lr) < most_groups && rows > (32L << lr)) ++lr;
+    int cap = (16 * tiles) << lr, bsplit = split;
+    if (wide(rows)) {
+      lr = 2;
+      cap = 128;
+      bsplit = std::max(split, WIDE_SPLIT);
+    }
     used = (1 << lr) > used ? 1 << lr : used;
-    const int cap = (16 * tiles) << lr;
     for (long row0 = 0; row0 < rows; row0 += cap) {
       const int nrows = (int)(rows - row0 < cap ? rows - row0 : cap);
       const int end = (int)(pos0 + (row0 + nrows - 1) / group + 1);
-      const int ns = (end + split - 1) / split;
+      const int ns = (end + bsplit - 1) / bsplit;
       if (ns > 1) {
         const int32_t g[8] = {bm[0], (int32_t)row0, nrows, (int32_t)np, ns, pos0, 0, 0};
         groups.insert(groups.end(), g, g + 8);
@@ -1135,7 +1376,7 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
       LSK_REQUIRE((long)(items.size() + shared.size()) + (long)ns * n_kv_heads < (1L << 24), LSK_ESHAPE,
                   "%s: too many work items", what);
       for (int sp = 0; sp < ns; ++sp) {
-        const int lo = sp * split, hi = lo + split < end ? lo + split : end;
+        const int lo = sp * bsplit, hi = lo + bsplit < end ? lo + bsplit : end;
         // in tenths of a one-tile step: a wave's steps, 1.5 times as long per further tile, and the item's own cost
         const int share = step * (CACHE_WAVES >> lr), steps = (hi - lo + share - 1) / share;
         const int cost = steps * (10 + 5 * (tiles - 1)) + 20 + 6 * (tiles - 1);
@@ -1211,7 +1452,7 @@ static int cache_attn(const char* what, int format, CacheAttnArgs a, const int32
               head_dim);
   LSK_REQUIRE(tiles == 1 || tiles == 2 || (tiles == 3 && head_dim == 64 && a.mask == nullptr), LSK_EARG,
               "%s: a plan of %d tiles", what, tiles);
-  LSK_REQUIRE((row_groups == 1 && n_shared == 0) || a.mask != nullptr, LSK_EARG,
+  LSK_REQUIRE((row_groups == 1 && n_shared == 0) || a.mask != nullptr || (format == FMT_KV4 && row_groups != 2), LSK_EARG,
               "%s: a tree's plan (%d row groups) without a mask", what, row_groups);
   LSK_REQUIRE(n_slots > 0 && n_groups >= 0 && n_parts >= 0 && (n_groups > 0) == (n_parts > 0), LSK_EARG,
               "%s: a plan of %d slots, %d groups and %d partial slots", what, n_slots, n_groups, n_parts);
@@ -1220,8 +1461,8 @@ static int cache_attn(const char* what, int format, CacheAttnArgs a, const int32
   LSK_REQUIRE(aligned16(a.kc) && aligned16(a.vc) && (format == FMT_BF16 || (aligned16(a.ks) && aligned16(a.vs))), LSK_EARG,
               "%s: the cache tensors start at multiples of 16 bytes", what);
   if (n_parts > 0) {
-    LSK_REQUIRE(a.part_rows >= 16 * tiles && a.part_rows <= 64 * tiles, LSK_EARG, "%s: a plan of %d rows per partial",
-                what, a.part_rows);
+    LSK_REQUIRE(a.part_rows >= 16 * tiles && (a.part_rows <= 64 * tiles || (n_shared > 0 && a.part_rows == 128)), LSK_EARG,
+                "%s: a plan of %d rows per partial", what, a.part_rows);
     const size_t need = lsk_cache_attn_workspace_bytes(n_parts, a.Hkv, a.part_rows, head_dim);
     LSK_REQUIRE(workspace != nullptr && aligned16(workspace) && ws_bytes >= need && groups != nullptr, LSK_EWORKSPACE,
                 "%s: an aligned workspace of %zu bytes needed, %zu given", what, need, ws_bytes);
@@ -1253,14 +1494,17 @@ static int cache_attn(const char* what, int format, CacheAttnArgs a, const int32
   if (a.n_rounds > 0 && (rc = lsk_check_launch(what))) return rc;
   if (n_shared > 0) {
     const int32_t* items = a.recs + 8L * n_slots * a.n_rounds;
-#define LSK_CACHE_TREE(F)                                                                            \
+#define LSK_CACHE_TREE(F, TR)                                                                        \
   do {                                                                                               \
-    if (head_dim == 128) cache_tree_kernel<128, F><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);   \
-    else cache_tree_kernel<64, F><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);                    \
+    if (head_dim == 128) cache_tree_kernel<128, F, TR><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items); \
+    else cache_tree_kernel<64, F, TR><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);                 \
   } while (0)
-    if (format == FMT_BF16) LSK_CACHE_TREE(FMT_BF16);
-    else if (format == FMT_KV8) LSK_CACHE_TREE(FMT_KV8);
-    else LSK_CACHE_TREE(FMT_KV4);
+    if (format == FMT_BF16) LSK_CACHE_TREE(FMT_BF16, true);
+    else if (format == FMT_KV8) LSK_CACHE_TREE(FMT_KV8, true);
+    else if (head_dim == 128 && a.mask != nullptr) cache_tree4_kernel<true><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
+    else if (head_dim == 128) cache_tree4_kernel<false><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
+    else if (a.mask != nullptr) cache_tree_kernel<64, FMT_KV4, true><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
+    else cache_tree_kernel<64, FMT_KV4, false><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
 #undef LSK_CACHE_TREE
     if ((rc = lsk_check_launch(what))) return rc;
   }

@@ -17,8 +17,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_cache_ops import (BF16, BLOCKS, F32, _cat, _gen, _heads, _i32, _lsk, accept, ancestors, assert_close_bf16,
-                            attention, pack_blocks, random_tree, words_of)
+from test_cache_ops import (BF16, BLOCKS, F32, _cat, _gen, _heads, _i32, _items, _lsk, accept, ancestors,
+                            assert_close_bf16, attention, pack_blocks, random_tree, words_of)
 
 HALF = {BF16: 2.0 ** -8, F32: 2.0 ** -24}             # eps / 2
 
@@ -343,6 +343,69 @@ def test_kv4_attention_of_large_and_small_scales(cuda, D):
         got = lsk.kv4_attn(q.to(cuda), cache, lsk.AttnPlan(tab, 4, cache, split=split, tree=False))
         ref, mag, _ = attention(q.double(), held(k), held(v), tab, 1 / math.sqrt(D))
         assert_close_bf16(got, ref, mag)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_kv4_attention_of_prompt_pieces_in_a_large_cache(cuda, D):
+    """Items of 128 rows, one of them in two splits, beside a block of few rows; NaN everywhere behind the blocks, NaN and
+    infinities in slots and a query that some rows read; a row's bits do not depend on the rest of the launch."""
+    lsk = _lsk()
+    g = _gen(D + 1)
+    B, Hkv, Hq, S = 100, 8, 32, 4288
+    real = [99, 3, 50, 51, 0]
+    blocks = [(0, 4200, 20), (1, 0, 33), (2, 31, 47), (3, 60, 17), (4, 5, 2)]      # 800 stripes
+    tab, n = pack_blocks(blocks)
+    k, v = (torch.randn(len(real), Hkv, S, D, generator=g).to(BF16) for _ in range(2))
+    k[1, 0, 20, 5], k[2, 3, 60, D - 1], v[1, 2, 32, 0], v[3, 7, 10, D - 1] = math.nan, math.inf, -math.inf, math.nan
+    q = torch.randn(n, Hq, D, generator=g).to(BF16)
+    q[30] *= 2.0 ** 40                                # (the scale of 32 of its dims; one position takes all)
+    q[31, :, :32] *= 2.0 ** -60
+    q[32, 4, 7], q[33, 5, 40] = math.inf, math.nan
+    q[34] = 0
+    cache = lsk.KV4.zeros(B, Hkv, S, D, cuda)
+    for t, fill in zip(cache, (0xF7, 0x7F, 255, 255)):
+        t.fill_(fill)
+    for (r, p0, t) in blocks:
+        m = p0 + t
+        lsk.kv4_append(k[r, :, :m].transpose(0, 1).to(cuda), v[r, :, :m].transpose(0, 1).to(cuda), cache,
+                       _i32(np.full(m, real[r]), cuda), _i32(np.arange(m), cuda))
+    where = [(a, b, c, real[r]) for (a, b, c, r) in tab]
+    plan = lsk.AttnPlan(where, Hq, cache, split=64, tree=False)
+    assert plan.causal.n_shared == (2 * 1 + 2 + 2 + 1) * Hkv and plan.causal.n_parts == 2
+    got = lsk.kv4_attn(q.to(cuda), cache, plan)
+    ref, mag, _ = attention(q.double(), held(k), held(v), tab, 1 / math.sqrt(D))
+    assert_close_bf16(got, ref, mag)
+    for i, (qs, p0, T, row) in enumerate(where):
+        alone = lsk.AttnPlan([(0, p0, T, row)], Hq, cache, split=64, tree=False)
+        one = lsk.kv4_attn(q[qs:qs + T].to(cuda), cache, alone)
+        assert torch.equal(one.view(torch.int16), got[qs:qs + T].view(torch.int16))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G,split", [(4, 64), (1, 512), (8, 8192), (3, 4160)])
+def test_kv4_plans_cover_every_row_and_position_once(G, split, D):
+    lsk = _lsk()
+    rng = np.random.default_rng(G)
+    B, Hkv, S = 90, 3, 8192
+    cache = lsk.KV4.zeros(1, 1, 64, D, "cpu")
+    cache = lsk.KV4(*(t.expand(B, Hkv, S // 64, *t.shape[3:]) for t in cache))
+    blocks = [(r, int(rng.integers(0, S - 400)), int(t)) for r, t in enumerate((400, 1, 64 // G, 65, 0, 200, 130))]
+    tab, _ = pack_blocks(blocks)
+    p = lsk.AttnPlan(tab, G * Hkv, cache, split=split, tree=False).causal
+    items, seen = _items(p, p), []
+    for (q0, p0, t, _) in tab:
+        wide = t * G > 64 and B * Hkv * -(-t * G // 32) > (768 if D == 128 else 1280)
+        covered = np.zeros((Hkv, t * G, S), dtype=np.int8)
+        for (_, r0, nr, g, h, lo, hi, part) in (i for i in items if i[0] == q0 and t):
+            assert g == (4 if wide else 1) and nr <= (128 if wide else 48) and nr <= (128 if part < 0 else p.part_rows)
+            assert lo % (max(split, 4096) if wide else split) == 0
+            assert (part >= 0) == (p0 + (r0 + nr - 1) // G + 1 > (max(split, 4096) if wide else split))
+            covered[h, r0:r0 + nr, lo:hi] += 1
+            seen += [(h, part)] if part >= 0 else []
+        for r in range(t * G):
+            assert (covered[:, r, :p0 + r // G + 1] == 1).all()
+    assert len(set(seen)) == len(seen) == p.n_parts * Hkv
 
 
 @pytest.mark.gpu

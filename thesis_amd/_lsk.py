@@ -787,14 +787,16 @@ def kv4_read(cache: KV4, rows_i32: torch.Tensor, pos_i32: torch.Tensor, dtype: t
     return _codes_read("kv4_read", KV4, cache, rows_i32, pos_i32, dtype, out)
 
 
-def cache_attn_split(max_batch: int, n_kv_heads: int, max_seq: int, tree: bool = False) -> int:
+def cache_attn_split(max_batch: int, n_kv_heads: int, max_seq: int, tree: bool = False, kv4: bool = False) -> int:
     """KV positions per attention split of a cache: fixed by the cache, so that a row's result never depends on the
     batch it is in.  The longest context in as many splits as make about one work item per CU out of the cache's
     (row, KV head) stripes, but each long enough to pay for the merge: 800 positions, 2048 from 128 stripes on (32 / 8
     heads of 64, one token, 1 request: 1000 positions 7.2 us whole, 11.0 in two; 5000 positions 15.8 whole, 10.8 in
     five).  Trees, whose partial outputs are many rows: 1280 positions, 2048 from 32 stripes on (64 nodes, 32 / 8 heads
     of 128: 4 requests of 1000 positions 14 us whole, 28 in two, of 5000 positions 37 and 42 in three; 1 request of 5000
-    positions 33 whole, 21 in three).  512 to 8192 positions, at most 128 splits.  256: MI355X's CUs, as a constant, so
+    positions 33 whole, 21 in three).  A 4-bit cache (kv4) without a mask, below 128 stripes: 512 positions where that
+    makes three splits or more (32 / 8 heads of 128, one token, 8 requests: 1000 positions 8.5 us whole, 9.4 in two,
+    2000 positions 12.5 whole, 9.8 in four).  512 to 8192 positions, at most 128 splits.  256: MI355X's CUs, as a constant, so
     that a row's bits are the same on every device.  The rule does not see a prompt, whose many rows need no splits: its
     plan is better given one (one prompt of 4001 tokens in a cache of its own, 32 / 8 heads of 128: 396 us and a
     workspace of 181 MB at 832 positions, 248 us and none at 8192)."""
@@ -802,7 +804,8 @@ def cache_attn_split(max_batch: int, n_kv_heads: int, max_seq: int, tree: bool =
     if tree:
         n = min(256 // stripes, max_seq // (1280 if stripes < 32 else 2048))
     else:
-        n = min(256 // stripes, max_seq // (800 if stripes < 128 else 2048))
+        least = 2048 if stripes >= 128 else 800 if not kv4 else 512 if max_seq >= 3 * 512 else max_seq
+        n = min(256 // stripes, max_seq // least)
     split = min(max(-(-max_seq // max(n, 1)), 512), ATTN_SPLIT)
     return (max(split, -(-max_seq // 128)) + 63) // 64 * 64
 
@@ -824,8 +827,9 @@ class AttnPlan:
     """The plan of attention launches over packed blocks, shared by the layers of a segment.  blocks: int [nb, 4] =
     (q_start, pos0, T, row) with q_start the running sum of T; cache: a layer's KV8 or KV4, or the K storage of a bf16 or
     fp32 cache.  split: KV positions per split (cache_attn_split unless given; fp32 does not split); row_groups: a tree's at
-    most (by the cache and the block unless given).  tree: which launches it is for, with a mask (True), without (False)
-    or, over an 8-bit or 4-bit cache, either (None), which takes twice as long (256 requests: 333 us for 129).
+    most (by the cache and the block unless given); prompts over a 4-bit cache take splits of 4096 positions or more.
+    tree: which launches it is for, with a mask (True), without (False) or, over an 8-bit or 4-bit cache, either (None),
+    which takes twice as long (256 requests: 333 us for 129).
     Its records go to the GPU on the current stream.  A launch on another stream waits for them, and they outlive it
     when the plan is dropped; a captured launch reads them with every replay: the plan is made before the capture and
     kept as long as the graph."""
@@ -859,7 +863,7 @@ class AttnPlan:
             self.works, self.n_works = self._upload(works.ravel()), len(works)
             self._mark_uploaded()
             return
-        self.split, self.tree_split = (split if split is not None else cache_attn_split(B, Hkv, S, t)
+        self.split, self.tree_split = (split if split is not None else cache_attn_split(B, Hkv, S, t, self.format == 2)
                                        for t in (False, True))
         rg = 0 if row_groups is None else row_groups
         if self.format and not tree:
