@@ -305,11 +305,64 @@ __device__ __forceinline__ void softmax_tile(lsk_f32x4 (&s)[NA], uint32_t reads,
   l += rs;
 }
 
+// Over a 4-bit cache of 128 dims a lane's 32 codes of K and their scale are an operand of the scaled matrix instruction
+// (v_mfma_scale_f32_16x16x128_f8f6f4: 16 positions x 128 dims) as they are.  Its partner Q is given as two e4m3 numbers
+// per value, q = 2^e (hi + lo / 16) with a power of two for every 32 dims of a row: hi holds the upper four of a bf16
+// value's eight bits, lo the rest, exactly for values down to 2^-15 of the 32 dims' largest; below, off by at most 2^-21
+// of that.  An infinity becomes NaN: the row's result is NaN either way.  Lane group lg's operand of Q is dims 16 lg ..
+// + 15 and 64 + 16 lg .. + 15 (of K's codes, dims 32 lg .. + 31), its scale that of dims 32 lg .. + 31.
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ uint32_t largest8(lsk_bf16x8 x) {  // |bits|
+  const lsk_i32x4 w = __builtin_bit_cast(lsk_i32x4, x);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, max((uint32_t)w[i] & 0x7fffu, (uint32_t)w[i] >> 16 & 0x7fffu));
+  return m;
+}
+// the smallest e >= 10 - 127 with m <= 448 * 2^e (biased; lo's is four less), 0 where m is not finite
+__device__ __forceinline__ int power_of(uint32_t m) {
+  return m >= 0x7f80u ? 127 : max((int)(m >> 7) - 8 + ((m & 0x7fu) > 0x60u ? 1 : 0), 10);
+}
+__device__ __forceinline__ int powers(int e) { return e | (e - 4) << 8; }
+// 8 values -> hi (two dwords), lo
+__device__ __forceinline__ lsk_i32x4 split8(lsk_bf16x8 x, int e, bool odd) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  const float inv = odd ? __builtin_nanf("") : __uint_as_float((uint32_t)(254 - e) << 23);
+  lsk_i32x4 r;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = (float)x[4 * w + i] * inv;
+    int h = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    h = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], h, true);
+    const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
+    int l = __builtin_amdgcn_cvt_pk_fp8_f32((y[0] - a[0]) * 16.f, (y[1] - a[1]) * 16.f, 0, false);
+    l = __builtin_amdgcn_cvt_pk_fp8_f32((y[2] - b[0]) * 16.f, (y[3] - b[1]) * 16.f, l, true);
+    r[w] = h;
+    r[2 + w] = l;
+  }
+  return r;
+}
+// S^T tiles 0 .. 3 of one query tile over 64 positions
+__device__ __forceinline__ void scores4(const lsk_i32x4 (&k)[4], int ks, const i32x8& hi, const i32x8& lo, int qe,
+                                        lsk_f32x4 (&s)[4]) {
+  const lsk_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#define SCORES4(A, Q, SEL, ACC)                                                                          \
+  s[A] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(                                               \
+      __builtin_shufflevector(k[A], k[A], 0, 1, 2, 3, -1, -1, -1, -1), Q, ACC, 4, 0, A, ks, SEL, qe);
+  SCORES4(0, hi, 0, zero) SCORES4(1, hi, 0, zero) SCORES4(2, hi, 0, zero) SCORES4(3, hi, 0, zero)
+  SCORES4(0, lo, 1, s[0]) SCORES4(1, lo, 1, s[1]) SCORES4(2, lo, 1, s[2]) SCORES4(3, lo, 1, s[3])
+#undef SCORES4
+}
+
 // A workgroup has four waves, and each CU two workgroups (n_slots): one's first loads and merge fall into the other's
 // steps.  Against one workgroup of eight waves (8B heads, 8-bit, decode): 256 requests of 250 positions 28 us against
 // 46, of 960 81 against 91, of 4000 313 against 311; 7B heads, 16 trees of 30 nodes and 960 positions 30 against 36;
 // one request of 100000 positions, 1B heads, 25 against 23.
 #define CACHE_WAVES 4
+#define PAIR_ROWS 48  // of an item of two row groups without a mask: with the merge's buffer half a CU's LDS
 template <int D, int QT, int FMT, bool TREE>
 __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const CacheAttnArgs A) {
   constexpr bool KV8 = FMT == FMT_KV8, KV4 = FMT == FMT_KV4, CODES = KV8 || KV4;
@@ -323,16 +376,20 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
   constexpr int LT = KV4 ? CT / 2 : CT;              // 16-byte loads per lane of a step, for K and for V
   constexpr int NW = CACHE_WAVES;
   constexpr int GR = 16 * QT;                        // rows of a wave
-  constexpr bool QREG = QT == 1;                     // one tile: Q fragments in registers (items of one row group)
+  constexpr bool KOP = KV4 && D == 128;              // K's codes are an operand
+  constexpr bool QREG = QT == 1 && !KOP;             // one tile: Q fragments in registers (items of one row group)
+  constexpr bool GROUPS = QT == 2 && (TREE || KOP);  // items of two row groups
   constexpr int MT = TREE || QT < ATTN_MERGE_TILES ? 1 : ATTN_MERGE_TILES;  // (two workgroups' LDS fits a CU's)
   constexpr int MR = 16 * MT;                        // rows of a wave merged per pass
-  constexpr int QROWS = QREG ? 0 : TREE ? 2 * GR : GR;  // rows of an item at most
+  // rows of an item at most
+  constexpr int QROWS = QREG ? 0 : GROUPS && TREE ? 2 * GR : GROUPS && D == 128 ? PAIR_ROWS : GR;
   constexpr int QLD = D + 8;                         // 16 rows' 16-byte reads hit distinct banks
   constexpr int QCH = D / 8;
   constexpr int QPT = QREG ? 1 : (QROWS * QCH + 64 * NW - 1) / (64 * NW);
   __shared__ __attribute__((aligned(16))) float s_o[NW][MR][D + 4];
   __shared__ __attribute__((aligned(16))) uint16_t s_q[QREG ? 1 : QROWS][QLD];
-  __shared__ float s_ml[NW][2][GR];
+  __shared__ uint16_t s_qe[KOP ? QROWS : 1][4];      // (KOP: a row is its hi, then its lo)
+  __shared__ float s_ml[KOP ? 1 : NW][2][GR];        // (KOP: behind a row of s_o)
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -355,7 +412,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
     it.kv_lo = wk[3]; it.kv_hi = wk[4]; it.part = wk[5]; it.pos0 = wk[6]; it.crow = wk[7];
     return it;
   };
-  auto row_base = [&](const Item& it) { return TREE ? (wave & ((1 << it.lr) - 1)) * GR : 0; };  // the wave's first row
+  auto row_base = [&](const Item& it) { return GROUPS ? (wave & ((1 << it.lr) - 1)) * GR : 0; };  // the wave's first row
   // Q: row rl of an item -> 8 elements from d; operand f's k index 8 lg + e stands for d = q_dim(f) + e
   auto q_dim = [&](int f) {
     return KV4 ? D / 4 * lg + 8 * f : KV8 ? 64 * (f >> 1) + 16 * lg + 8 * (f & 1) : 32 * f + 8 * lg;
@@ -367,7 +424,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
   auto ldq = [&](const uint16_t* p) { return __builtin_bit_cast(lsk_bf16x8, *(const lsk_u32x4_u*)p); };
   // Q of the next item waits in registers during the merge where they hold it (with 128 dims it spilled: 256 requests
   // of 1 to 9 tokens 199 us against 181 without; with 64 dims 53.9 against 55.2), else it comes after the merge
-  constexpr bool QAHEAD = !TREE && D == 64;
+  constexpr bool QAHEAD = !TREE && (D == 64 || QT == 1);
   lsk_bf16x8 qst[QAHEAD ? QPT : 1];
   auto q_chunk = [&](const Item& it, int c) {        // 8 elements of a row, zeros past the rows
     const int row = c / QCH;
@@ -392,14 +449,29 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
 #pragma unroll
       for (int i = 0; i < QPT; ++i) {
         const int c = t0 + i * 64 * NW, row = c / QCH;
-        if (row < QROWS) *(lsk_bf16x8*)(&s_q[row][8 * (c - row * QCH)]) = QAHEAD ? qst[QAHEAD ? i : 0] : q_chunk(it, c);
+        if (row >= QROWS) continue;
+        const lsk_bf16x8 x = QAHEAD ? qst[QAHEAD ? i : 0] : q_chunk(it, c);
+        if constexpr (KOP) {                         // (four lanes hold 32 dims)
+          uint32_t m = largest8(x);
+          m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xb1, 0xf, 0xf, false));
+          m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4e, 0xf, 0xf, false));
+          const int e = power_of(m);
+          const lsk_i32x4 w = split8(x, e, m >= 0x7f80u);
+          lsk_u32x2_u hi, lo;
+          hi[0] = w[0]; hi[1] = w[1]; lo[0] = w[2]; lo[1] = w[3];
+          *(lsk_u32x2_u*)(&s_q[row][4 * (c % QCH)]) = hi;
+          *(lsk_u32x2_u*)(&s_q[row][D / 2 + 4 * (c % QCH)]) = lo;
+          s_qe[row][c / 4 % 4] = (uint16_t)powers(e);
+        } else {
+          *(lsk_bf16x8*)(&s_q[row][8 * (c - row * QCH)]) = x;
+        }
       }
     }
   };
   auto stripe = [&](const Item& it) { return cache_stripe<D, FMT>(A, it.crow, it.kvh, it.kv_hi); };
   // Non-temporal where each byte is read once (32 trees of 16 nodes, 7B heads, 960 positions of bf16: 95 us against
   // 80); not where two row groups read it (39 nodes: 111 us against 118)
-  constexpr int AUX = TREE && QT == 2 ? 0 : 2;
+  constexpr int AUX = GROUPS ? 0 : 2;
   auto ld = [&](__amdgpu_buffer_rsrc_t rs, int vo, int so) -> lsk_i32x4 {
     return __builtin_bit_cast(lsk_i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, vo, so, AUX));
   };
@@ -427,7 +499,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
   };
   // a wave without rows starts past the stripe
   auto first_step = [&](const Item& it) {
-    return row_base(it) < it.nrows ? it.kv_lo + STEP * (TREE ? wave >> it.lr : wave) : S;
+    return row_base(it) < it.nrows ? it.kv_lo + STEP * (GROUPS ? wave >> it.lr : wave) : S;
   };
   auto issue_first = [&](const Item& it) {
     q_load(it);
@@ -450,13 +522,14 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
   }
   for (int r = 0; cur.nrows > 0; ++r) {
     const int kv_hi = cur.kv_hi, rb = row_base(cur);
-    const int stride = STEP * (TREE ? NW >> cur.lr : NW);
+    const int stride = STEP * (GROUPS ? NW >> cur.lr : NW);
     const Stripe sr = stripe(cur);
-    int qpos[QT];                                    // the row's own slot; -1: no such row
+    int qpos[QT], qe[QT];                            // the row's own slot (-1: no such row); its powers of two
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const int rl = rb + 16 * qt + l16;
       qpos[qt] = rl < cur.nrows ? cur.pos0 + (cur.row0 + rl) / G : -1;
+      qe[qt] = KOP ? s_qe[KOP ? rl : 0][lg] : 0;
     }
     // slots that every row of the item reads
     const int full_lim = min(kv_hi - 1, TREE ? cur.pos0 - 1 : cur.pos0 + cur.row0 / G);
@@ -485,6 +558,9 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
     auto step = [&](auto full_, auto nq_, int sb) {
       constexpr bool FULL = decltype(full_)::value;
       constexpr int NQ = decltype(nq_)::value;
+      // V's scales of a 4-bit cache multiply the weights, once for every 32 dims; with more than one query tile V itself
+      // (a wave's instructions per step of 64 positions and 128 dims: 160 a tile against 192)
+      constexpr bool VS = KV4 && FULL && NQ > 1;
       // In a step that some row does not read whole, a slot whose V holds an infinity or NaN must not reach the rows
       // that do not read it (0 x NaN): the values past the item and the non-finite ones are cleared here, and the rows
       // that do read such a value get it after the products (below).
@@ -500,8 +576,24 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
 #pragma unroll
       for (int qt = 0; qt < NQ; ++qt) reads[qt] = FULL ? ALL : allow(qt, s0);
       lsk_f32x4 sacc[QT][2 * HV];
+      if constexpr (KOP) {
 #pragma unroll
-      for (int a = 0; a < 2 * HV; ++a) {
+        for (int qt = 0; qt < NQ; ++qt) {
+          const uint16_t* qp = s_q[rb + 16 * qt + l16] + 8 * lg;
+          i32x8 qv[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const lsk_i32x4 x = *(const lsk_i32x4*)(qp + h * (D / 2)), y = *(const lsk_i32x4*)(qp + h * (D / 2) + 32);
+            qv[h] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+          }
+          scores4(kr, ksr[0], qv[0], qv[1], qe[qt], sacc[qt]);
+        }
+        ORDER();
+#pragma unroll
+        for (int a = 0; a < 4; ++a) load_k(sr, sn, a);
+      }
+#pragma unroll
+      for (int a = 0; a < (KOP ? 0 : 2 * HV); ++a) {
         if constexpr (CODES) ORDER();
         lsk_bf16x8 kf[KF];
         if constexpr (KV8) {
@@ -544,7 +636,8 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
 #pragma unroll
       for (int qt = 0; qt < NQ; ++qt) {
         if constexpr (CODES) ORDER();
-        softmax_tile<FMT, FULL, KV4>(sacc[qt], reads[qt], vsr[0], A.scale_log2, m_run[qt], l_run[qt], oacc[qt], pb[qt]);
+        softmax_tile<VS ? FMT_BF16 : FMT, FULL, KV4>(sacc[qt], reads[qt], vsr[0], A.scale_log2, m_run[qt], l_run[qt],
+                                                     oacc[qt], pb[qt]);
       }
       ORDER();
       if constexpr (!KV4) load_vs(sr, sn);
@@ -553,7 +646,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
       for (int c = 0; c < CT; ++c) {
         lsk_bf16x8 vf[HV];
         if constexpr (KV4) {
-          if (c % 2 == 0) {                          // the weights times the scales of these 32 dims
+          if (!VS && c % 2 == 0) {                   // the weights times the scales of these 32 dims
 #pragma unroll
             for (int qt = 0; qt < NQ; ++qt)
 #pragma unroll
@@ -564,7 +657,10 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
               }
           }
 #pragma unroll
-          for (int hv = 0; hv < HV; ++hv) vf[hv] = codes4_to_bf16((uint32_t)vr[c / 2][2 * (c & 1) + hv], 1.f);
+          for (int hv = 0; hv < HV; ++hv) {
+            const uint32_t x = (uint32_t)vr[c / 2][2 * (c & 1) + hv];
+            vf[hv] = VS ? codes4_to_bf16(x, vsr[c / 2], hv) : codes4_to_bf16(x, 1.f);
+          }
         } else if constexpr (KV8) {
 #pragma unroll
           for (int hv = 0; hv < HV; ++hv) vf[hv] = codes_to_bf16(vr[c][2 * hv], vr[c][2 * hv + 1], 1.f);
@@ -603,6 +699,10 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
     int tm = tid;
     asm volatile("" : "+v"(tm));                     // (no address of the merge is kept in registers across the steps)
     const int m16 = tm & 15, mg = (tm & 63) >> 4;
+    auto ml = [&](int w, int i, int first, int ql) -> float& {  // the maximum, the sum of row ql of a pass
+      if constexpr (KOP) return s_o[w][ql][D + i];
+      else return s_ml[w][i][first + ql];
+    };
 #pragma unroll
     for (int p0 = 0; p0 < QT; p0 += MT) {
       if (16 * p0 >= done.nrows) break;
@@ -610,8 +710,8 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
       for (int qt = p0; qt < p0 + MT && qt < QT; ++qt) {
         const float l = rows_sum(l_run[qt]);
         if (mg == 0) {
-          s_ml[wave][0][16 * qt + m16] = m_run[qt];
-          s_ml[wave][1][16 * qt + m16] = l;
+          ml(wave, 0, 16 * p0, 16 * (qt - p0) + m16) = m_run[qt];
+          ml(wave, 1, 16 * p0, 16 * (qt - p0) + m16) = l;
         }
         if (16 * qt < done.nrows - rb) {             // (a tile with rows)
 #pragma unroll
@@ -631,14 +731,14 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
           if (qr >= GR || row >= done.nrows) continue;
           float M = M_NONE;
 #pragma unroll
-          for (int k = 0; k < RANKS; ++k) M = fmaxf(M, s_ml[k * NR + rg][0][qr]);
+          for (int k = 0; k < RANKS; ++k) M = fmaxf(M, ml(k * NR + rg, 0, 16 * p0, ql));
           float L = 0.f;
           float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int k = 0; k < RANKS; ++k) {
-            const float mw = s_ml[k * NR + rg][0][qr];
+            const float mw = ml(k * NR + rg, 0, 16 * p0, ql);
             const float ew = mw == M ? 1.f : fast_exp2(mw - M);
-            L = L + ew * s_ml[k * NR + rg][1][qr];
+            L = L + ew * ml(k * NR + rg, 1, 16 * p0, ql);
             const float4 ow = *(const float4*)(&s_o[k * NR + rg][ql][d]);
             O.x = O.x + ew * ow.x;
             O.y = O.y + ew * ow.y;
@@ -666,7 +766,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
           }
         }
       };
-      if (QREG || !TREE || done.lr == 0) merge(std::integral_constant<int, NW>{});
+      if (!GROUPS || done.lr == 0) merge(std::integral_constant<int, NW>{});
       else merge(std::integral_constant<int, NW / 2>{});
       if (p0 == 0 && cur.nrows > 0) q_store(cur);       // (every wave is past its steps)
       __syncthreads();
@@ -676,9 +776,9 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
 
 // The end of an item of cache_tree_kernel: a wave's rows, from rb on, or its part of them
 template <bool TREE, int QT, int CT>
-__device__ __forceinline__ void tree_store(const CacheAttnArgs& A, const lsk_f32x4 (&oacc)[QT][CT], const float (&m_run)[QT],
-                                           float (&l_run)[QT], int q_start, int row0, int nrows, int rb, int kvh, int part,
-                                           int pos0) {
+__device__ __forceinline__ void tree_store(const CacheAttnArgs& A, const lsk_f32x4 (&oacc)[QT][CT],
+                                           const float (&m_run)[QT], float (&l_run)[QT], int q_start, int row0, int nrows,
+                                           int rb, int kvh, int part, int pos0) {
   constexpr int D = 16 * CT;
   const int l16 = threadIdx.x & 15, lg = (threadIdx.x & 63) >> 4, G = A.G, Hkv = A.Hkv;
 #pragma unroll
@@ -902,58 +1002,35 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
   tree_store<TREE>(A, oacc, m_run, l_run, q_start, row0, nrows, rb, kvh, part, pos0);
 }
 
-// The same over a 4-bit cache of 128 dims, without a mask (TREE false) or with one.  A lane's 32 codes of K and their scale
-// are an operand of the scaled matrix instruction (v_mfma_scale_f32_16x16x128_f8f6f4: 16 positions x 128 dims), so K is
-// neither converted nor staged.  Its partner Q is given as two e4m3 numbers per value, q = 2^e (hi + lo / 16) with a
-// power of two for every 32 dims of a row: hi holds the upper four of a bf16 value's eight bits, lo the rest, exactly
-// for values down to 2^-15 of the 32 dims' largest; below, off by at most 2^-21 of that.  An infinity becomes NaN: the
-// row's result is NaN either way.  Lane group lg's operand of Q is dims 16 lg .. + 15 and 64 + 16 lg .. + 15 (of K's codes,
-// dims 32 lg .. + 31), its scale that of dims 32 lg .. + 31.  V goes through LDS as bf16 with its scales, 64 positions at
-// a time, a quarter of the dims a wave.  (8B heads: a prompt of 1001 tokens after 1000 62 -> 56 us against the kernel
-// above over 4 bits, 32 trees of 64 nodes 55 -> 46.)
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
+// The same over a 4-bit cache of 128 dims, without a mask (TREE false) or with one.  K is neither converted nor staged
+// (above); each wave splits its own Q.  V goes through LDS as bf16 with its scales, 64 positions at a time, a quarter of
+// the dims a wave.  (8B heads: a prompt of 1001 tokens after 1000 62 -> 56 us against the kernel above over 4 bits, 32
+// trees of 64 nodes 55 -> 46.)
 __device__ __forceinline__ void split_q(const uint16_t* q, int lg, i32x8& hi, i32x8& lo, int& exps) {
-  typedef float f2 __attribute__((ext_vector_type(2)));
   int e[2];
 #pragma unroll
   for (int hv = 0; hv < 2; ++hv) {                   // dims 64 hv + 16 lg .. + 15
-    float x[16];
+    lsk_bf16x8 x[2];
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const lsk_u32x4_u u = *(const lsk_u32x4_u*)(q + 64 * hv + 16 * lg + 8 * i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
-        x[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-      }
+      x[i] = __builtin_bit_cast(lsk_bf16x8, *(const lsk_u32x4_u*)(q + 64 * hv + 16 * lg + 8 * i));
+      m = max(m, largest8(x[i]));
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
     m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));  // (32 dims are two lanes')
-    // the smallest e >= 10 - 127 with amax <= 448 * 2^e (biased; lo's is four less)
-    const bool odd = m >= 0x7f800000u;
-    e[hv] = max(odd ? 127 : (int)(m >> 23) - 8 + ((m & 0x7fffffu) > 0x600000u ? 1 : 0), 10);
-    const float inv = __uint_as_float((uint32_t)(254 - e[hv]) << 23);
+    e[hv] = power_of(m);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      float y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = odd ? __builtin_nanf("") : x[4 * w + i] * inv;
-      int h = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-      h = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], h, true);
-      const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
-      int l = __builtin_amdgcn_cvt_pk_fp8_f32((y[0] - a[0]) * 16.f, (y[1] - a[1]) * 16.f, 0, false);
-      l = __builtin_amdgcn_cvt_pk_fp8_f32((y[2] - b[0]) * 16.f, (y[3] - b[1]) * 16.f, l, true);
-      hi[4 * hv + w] = h;
-      lo[4 * hv + w] = l;
+    for (int i = 0; i < 2; ++i) {
+      const lsk_i32x4 w = split8(x[i], e[hv], m >= 0x7f80u);
+      hi[4 * hv + 2 * i] = w[0];
+      hi[4 * hv + 2 * i + 1] = w[1];
+      lo[4 * hv + 2 * i] = w[2];
+      lo[4 * hv + 2 * i + 1] = w[3];
     }
   }
   // lane group lg gives the power of dims 32 lg .. + 31: that of lane groups 2 (lg % 2) .. + 1 in their half lg / 2
   const int other = __shfl_xor(lg == 2 ? e[0] : e[1], 48, 64);
-  const int mine = lg == 0 ? e[0] : lg == 3 ? e[1] : other;
-  exps = mine | (mine - 4) << 8;
+  exps = powers(lg == 0 ? e[0] : lg == 3 ? e[1] : other);
 }
 
 template <bool TREE>
@@ -1026,17 +1103,8 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree4_kernel(const C
       }
     }
     lsk_f32x4 sacc[QT][4];
-    const lsk_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-#define TREE4_TILE(AA)                                                                                           \
-  {                                                                                                              \
-    const i32x8 k8 = __builtin_shufflevector(kr[AA], kr[AA], 0, 1, 2, 3, -1, -1, -1, -1);                          \
-    _Pragma("unroll") for (int qt = 0; qt < QT; ++qt) sacc[qt][AA] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4( \
-        k8, qh[qt], zero, 4, 0, AA, ks, 0, qe[qt]);                                                              \
-    _Pragma("unroll") for (int qt = 0; qt < QT; ++qt) sacc[qt][AA] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4( \
-        k8, ql[qt], sacc[qt][AA], 4, 0, AA, ks, 1, qe[qt]);                                                      \
-  }
-    TREE4_TILE(0) TREE4_TILE(1) TREE4_TILE(2) TREE4_TILE(3)
-#undef TREE4_TILE
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) scores4(kr, ks, qh[qt], ql[qt], qe[qt], sacc[qt]);
     ORDER();
     load_k(s2 + CHUNK);
     lsk_bf16x8 pb[QT][2];
@@ -1298,13 +1366,19 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 //           whose waves share the conversions of K and V (8B heads after 1000 positions, wide / not, unsplit: 256 stripes
 //           of 64 tokens 52 / 83 us, 64 stripes of 256 54 / 88; equal at 1024 tiles, 64 stripes of 128 44 / 45; behind at
 //           512, 64 stripes of 64 35 / 25 and 8 of 512 40 / 26; in two splits at 512 tiles 34 / 35; 17 tokens in 256
-//           stripes 39 / 38; 1B heads: 64 stripes of 128 tokens 37 / 32, of 256 44 / 60).  The cache full of such blocks has 192 items and more, so its splits are of WIDE_SPLIT
-//           positions at least (8 stripes, a prompt of 4001 tokens: 640 positions 218 us, 1280 174, 2560 155, whole 142;
-//           the other way round for one short piece in a large cache: 256 tokens after 5000 whole 107, 2560 63).
+//           stripes 39 / 38; 1B heads: 64 stripes of 128 tokens 37 / 32, of 256 44 / 60).  The cache full of such blocks
+//           has 192 items and more, so its splits are of WIDE_SPLIT positions at least (8 stripes, a prompt of 4001
+//           tokens: 640 positions 218 us, 1280 174, 2560 155, whole 142; the other way round for one short piece in a
+//           large cache: 256 tokens after 5000 whole 107, 2560 63).
+//   pairs   a block that is not wide, over a 4-bit cache of 128 dims, whose rows make fewer items of PAIR_ROWS than of 32,
+//           where the stripes times the tiles of 32 rows are more than PAIR_TILES: items of two row groups of two waves (8B
+//           heads after 1000 positions, pairs / not: 64 requests of 9 tokens 32 / 48 us, of 12 33 / 46, 128 of 9 62 / 93;
+//           32 of 9, 512 tiles, 25 / 24; 64 of 16, 48 + 16 rows or 32 + 32, 61 / 48).
 // The number of row groups follows from the block's rows and the cache alone, so it never makes a row's result depend
 // on the batch.  Items go longest first to the least-loaded of n_slots persistent workgroups, as in lsk_attn_schedule.
 #define WIDE_TILES(D) ((D) == 64 ? 1280 : 768)
 #define WIDE_SPLIT 4096
+#define PAIR_TILES 512
 static int cache_plan(const char* what, const int32_t* blocks, int nb, int group, int split, int max_batch,
                       int n_kv_heads, int head_dim, int format, int tree, int row_groups, int n_slots, int32_t* meta,
                       long meta_cap, long* counts) {
@@ -1331,7 +1405,13 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
     n_tokens += T;
   }
   const auto wide = [&](long rows) {
-    return format == FMT_KV4 && !tree && rows > 64 && (long)max_batch * n_kv_heads * ((rows + 31) / 32) > WIDE_TILES(head_dim);
+    return format == FMT_KV4 && !tree && rows > 64 &&
+           (long)max_batch * n_kv_heads * ((rows + 31) / 32) > WIDE_TILES(head_dim);
+  };
+  const auto pair = [&](long rows) {
+    return format == FMT_KV4 && head_dim == 128 && !tree && !wide(rows) &&
+           (rows + PAIR_ROWS - 1) / PAIR_ROWS < (rows + 31) / 32 &&
+           (long)max_batch * n_kv_heads * ((rows + 31) / 32) > PAIR_TILES;
   };
   if (wide(most)) {                                  // (the other blocks' tiles)
     most = 0;
@@ -1358,6 +1438,10 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
     const int most_groups = row_groups ? row_groups : few ? 1 : 4;
     while (tree && (1 << lr) < most_groups && rows > (32L << lr)) ++lr;
     int cap = (16 * tiles) << lr, bsplit = split;
+    if (pair(rows)) {
+      lr = 1;
+      cap = PAIR_ROWS;
+    }
     if (wide(rows)) {
       lr = 2;
       cap = 128;
@@ -1452,7 +1536,8 @@ static int cache_attn(const char* what, int format, CacheAttnArgs a, const int32
               head_dim);
   LSK_REQUIRE(tiles == 1 || tiles == 2 || (tiles == 3 && head_dim == 64 && a.mask == nullptr), LSK_EARG,
               "%s: a plan of %d tiles", what, tiles);
-  LSK_REQUIRE((row_groups == 1 && n_shared == 0) || a.mask != nullptr || (format == FMT_KV4 && row_groups != 2), LSK_EARG,
+  LSK_REQUIRE((row_groups == 1 && n_shared == 0) || a.mask != nullptr ||
+                  (format == FMT_KV4 && (row_groups != 2 || head_dim == 128)), LSK_EARG,
               "%s: a tree's plan (%d row groups) without a mask", what, row_groups);
   LSK_REQUIRE(n_slots > 0 && n_groups >= 0 && n_parts >= 0 && (n_groups > 0) == (n_parts > 0), LSK_EARG,
               "%s: a plan of %d slots, %d groups and %d partial slots", what, n_slots, n_groups, n_parts);

@@ -256,7 +256,8 @@ def test_kv4_attention(cuda, heads, blocks, split):
     ref, mag, _ = attention(q.double(), held(k), held(v), tab, 1 / math.sqrt(D))
     assert_close_bf16(got, ref, mag)
     # a chain's mask gives the causal rule, within the same bounds
-    words = words_of([set(range(t + 1)) for (_, _, T, _) in tab for t in range(T)], max(T for (_, _, T, _) in tab) // 32 + 1)
+    most = max(T for (_, _, T, _) in tab)
+    words = words_of([set(range(t + 1)) for (_, _, T, _) in tab for t in range(T)], most // 32 + 1)
     assert_close_bf16(lsk.kv4_attn(q.to(cuda), cache, plan, _i32(words, cuda)), ref, mag)
 
 
@@ -347,14 +348,16 @@ def test_kv4_attention_of_large_and_small_scales(cuda, D):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("D", [64, 128])
-def test_kv4_attention_of_prompt_pieces_in_a_large_cache(cuda, D):
-    """Items of 128 rows, one of them in two splits, beside a block of few rows; NaN everywhere behind the blocks, NaN and
-    infinities in slots and a query that some rows read; a row's bits do not depend on the rest of the launch."""
+@pytest.mark.parametrize("tokens", [(20, 33, 47, 17, 2), (12, 11, 9, 10, 2)])
+def test_kv4_attention_of_prompt_pieces_in_a_large_cache(cuda, tokens, D):
+    """Items of 128 rows (of 33 to 48), one of them in two splits, beside a block of few rows; NaN everywhere behind the
+    blocks, NaN and infinities in slots and a query that some rows read; a row's bits do not depend on the rest of the
+    launch."""
     lsk = _lsk()
     g = _gen(D + 1)
     B, Hkv, Hq, S = 100, 8, 32, 4288
     real = [99, 3, 50, 51, 0]
-    blocks = [(0, 4200, 20), (1, 0, 33), (2, 31, 47), (3, 60, 17), (4, 5, 2)]      # 800 stripes
+    blocks = [(r, p0, t) for r, (p0, t) in enumerate(zip((4200, 0, 31, 60, 5), tokens))]       # 800 stripes
     tab, n = pack_blocks(blocks)
     k, v = (torch.randn(len(real), Hkv, S, D, generator=g).to(BF16) for _ in range(2))
     k[1, 0, 20, 5], k[2, 3, 60, D - 1], v[1, 2, 32, 0], v[3, 7, 10, D - 1] = math.nan, math.inf, -math.inf, math.nan
@@ -371,13 +374,16 @@ def test_kv4_attention_of_prompt_pieces_in_a_large_cache(cuda, D):
         lsk.kv4_append(k[r, :, :m].transpose(0, 1).to(cuda), v[r, :, :m].transpose(0, 1).to(cuda), cache,
                        _i32(np.full(m, real[r]), cuda), _i32(np.arange(m), cuda))
     where = [(a, b, c, real[r]) for (a, b, c, r) in tab]
-    plan = lsk.AttnPlan(where, Hq, cache, split=64, tree=False)
-    assert plan.causal.n_shared == (2 * 1 + 2 + 2 + 1) * Hkv and plan.causal.n_parts == 2
+    wide = tokens[0] == 20
+    split = 64 if wide else 2112
+    plan = lsk.AttnPlan(where, Hq, cache, split=split, tree=False)
+    assert plan.causal.n_shared == (2 * 1 + 2 + 2 + 1) * Hkv * wide and plan.causal.n_parts == 2
+    assert plan.causal.row_groups == (4 if wide else 2 if D == 128 else 1)
     got = lsk.kv4_attn(q.to(cuda), cache, plan)
     ref, mag, _ = attention(q.double(), held(k), held(v), tab, 1 / math.sqrt(D))
     assert_close_bf16(got, ref, mag)
     for i, (qs, p0, T, row) in enumerate(where):
-        alone = lsk.AttnPlan([(0, p0, T, row)], Hq, cache, split=64, tree=False)
+        alone = lsk.AttnPlan([(0, p0, T, row)], Hq, cache, split=split, tree=False)
         one = lsk.kv4_attn(q[qs:qs + T].to(cuda), cache, alone)
         assert torch.equal(one.view(torch.int16), got[qs:qs + T].view(torch.int16))
 
@@ -396,9 +402,11 @@ def test_kv4_plans_cover_every_row_and_position_once(G, split, D):
     items, seen = _items(p, p), []
     for (q0, p0, t, _) in tab:
         wide = t * G > 64 and B * Hkv * -(-t * G // 32) > (768 if D == 128 else 1280)
+        two = D == 128 and not wide and -(-t * G // 48) < -(-t * G // 32) and B * Hkv * -(-t * G // 32) > 512
         covered = np.zeros((Hkv, t * G, S), dtype=np.int8)
         for (_, r0, nr, g, h, lo, hi, part) in (i for i in items if i[0] == q0 and t):
-            assert g == (4 if wide else 1) and nr <= (128 if wide else 48) and nr <= (128 if part < 0 else p.part_rows)
+            assert g == (4 if wide else 2 if two else 1) and nr <= (128 if wide else 48)
+            assert part < 0 or nr <= p.part_rows
             assert lo % (max(split, 4096) if wide else split) == 0
             assert (part >= 0) == (p0 + (r0 + nr - 1) // G + 1 > (max(split, 4096) if wide else split))
             covered[h, r0:r0 + nr, lo:hi] += 1
