@@ -1004,8 +1004,8 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
 
 // The same over a 4-bit cache of 128 dims, without a mask (TREE false) or with one.  K is neither converted nor staged
 // (above); each wave splits its own Q.  V goes through LDS as bf16 with its scales, 64 positions at a time, a quarter of
-// the dims a wave.  (8B heads: a prompt of 1001 tokens after 1000 62 -> 56 us against the kernel above over 4 bits, 32
-// trees of 64 nodes 55 -> 46.)
+// the dims a wave.  (8B heads, items of 128 rows: a prompt of 1001 tokens after 1000 62 -> 56 us against the kernel above
+// over 4 bits, 32 trees of 64 nodes 55 -> 46.)
 __device__ __forceinline__ void split_q(const uint16_t* q, int lg, i32x8& hi, i32x8& lo, int& exps) {
   int e[2];
 #pragma unroll
@@ -1033,10 +1033,10 @@ __device__ __forceinline__ void split_q(const uint16_t* q, int lg, i32x8& hi, i3
   exps = powers(lg == 0 ? e[0] : lg == 3 ? e[1] : other);
 }
 
-template <bool TREE>
+template <bool TREE, int QT>
 __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree4_kernel(const CacheAttnArgs A,
                                                                          const int32_t* __restrict__ items) {
-  constexpr int D = 128, CT = D / 16, QT = 2, CHUNK = 64, NE = 16;
+  constexpr int D = 128, CT = D / 16, CHUNK = 64, NE = 16;
   constexpr uint32_t ALL = 0xffffu;
   constexpr int HALF = CT * 1024, BUF = 2 * HALF;    // V fragments (half hv of a lane group's 16 positions, c)
   __shared__ __attribute__((aligned(16))) char s_v[2 * BUF];
@@ -1364,12 +1364,14 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 //   wide    a block of more than 64 rows without a mask over a 4-bit cache (a piece of a prompt), where the cache's
 //           stripes times the block's tiles of 32 rows are more than WIDE_TILES: items of 128 rows for the tree kernels,
 //           whose waves share the conversions of K and V (8B heads after 1000 positions, wide / not, unsplit: 256 stripes
-//           of 64 tokens 52 / 83 us, 64 stripes of 256 54 / 88; equal at 1024 tiles, 64 stripes of 128 44 / 45; behind at
-//           512, 64 stripes of 64 35 / 25 and 8 of 512 40 / 26; in two splits at 512 tiles 34 / 35; 17 tokens in 256
-//           stripes 39 / 38; 1B heads: 64 stripes of 128 tokens 37 / 32, of 256 44 / 60).  The cache full of such blocks
-//           has 192 items and more, so its splits are of WIDE_SPLIT positions at least (8 stripes, a prompt of 4001
-//           tokens: 640 positions 218 us, 1280 174, 2560 155, whole 142; the other way round for one short piece in a
-//           large cache: 256 tokens after 5000 whole 107, 2560 63).
+//           of 64 tokens 52 / 83 us, 64 stripes of 256 54 / 88; 1024 tiles, 64 stripes of 128, 36 / 45; behind at 512: 8
+//           of 512 tokens 29 / 26; 17 tokens in 256 stripes 39 / 38; 1B heads: 64 stripes of 128 tokens 37 / 32, of 256
+//           44 / 60).  Over 128 dims items are of 64 rows, one query tile a wave, where the launch has at most
+//           HALF_ITEMS of 128, one for each CU: it is bound by the longest item, and two workgroups' products and softmax
+//           overlap (251 items, one of 1001 tokens: 53 -> 44 us; 376, one of 1500: 69 -> 80; a row's bits are the same).
+//           The cache full of such blocks has 192 items of 128 rows and more, so its splits are of WIDE_SPLIT positions
+//           at least (8 stripes, a prompt of 4001 tokens: 640 positions 218 us, 1280 174, 2560 155, whole 142; the other
+//           way round for one short piece in a large cache: 256 tokens after 5000 whole 107, 2560 63).
 //   pairs   a block that is not wide, over a 4-bit cache of 128 dims, whose rows make fewer items of PAIR_ROWS than of 32,
 //           where the stripes times the tiles of 32 rows are more than PAIR_TILES: items of two row groups of two waves (8B
 //           heads after 1000 positions, pairs / not: 64 requests of 9 tokens 32 / 48 us, of 12 33 / 46, 128 of 9 62 / 93;
@@ -1379,6 +1381,7 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 #define WIDE_TILES(D) ((D) == 64 ? 1280 : 768)
 #define WIDE_SPLIT 4096
 #define PAIR_TILES 512
+#define HALF_ITEMS 256
 static int cache_plan(const char* what, const int32_t* blocks, int nb, int group, int split, int max_batch,
                       int n_kv_heads, int head_dim, int format, int tree, int row_groups, int n_slots, int32_t* meta,
                       long meta_cap, long* counts) {
@@ -1420,6 +1423,12 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
       if (!wide(rows) && rows > most) most = rows;
     }
   }
+  long n_wide = 0;                                   // items of 128 rows
+  for (int b = 0; b < nb; ++b) {
+    const long rows = (long)blocks[(long)b * 4 + 2] * group;
+    n_wide += wide(rows) ? (rows + 127) / 128 * n_kv_heads : 0;
+  }
+  const int wide_rows = head_dim == 128 && n_wide <= HALF_ITEMS ? 64 : 128;
   const int tiles = most <= 16 ? 1 : most <= 32 || tree || head_dim == 128 ? 2 : 3;
   struct It { int32_t rec[8]; int cost; };
   thread_local std::vector<It> items, shared;
@@ -1444,10 +1453,11 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
     }
     if (wide(rows)) {
       lr = 2;
-      cap = 128;
+      cap = wide_rows;
       bsplit = std::max(split, WIDE_SPLIT);
     }
-    used = (1 << lr) > used ? 1 << lr : used;
+    const int groups_used = wide(rows) && wide_rows == 64 ? 2 : 1 << lr;
+    used = groups_used > used ? groups_used : used;
     for (long row0 = 0; row0 < rows; row0 += cap) {
       const int nrows = (int)(rows - row0 < cap ? rows - row0 : cap);
       const int end = (int)(pos0 + (row0 + nrows - 1) / group + 1);
@@ -1584,12 +1594,15 @@ static int cache_attn(const char* what, int format, CacheAttnArgs a, const int32
     if (head_dim == 128) cache_tree_kernel<128, F, TR><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items); \
     else cache_tree_kernel<64, F, TR><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);                 \
   } while (0)
+#define LSK_CACHE_TREE4(TR, QT) cache_tree4_kernel<TR, QT><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items)
     if (format == FMT_BF16) LSK_CACHE_TREE(FMT_BF16, true);
     else if (format == FMT_KV8) LSK_CACHE_TREE(FMT_KV8, true);
-    else if (head_dim == 128 && a.mask != nullptr) cache_tree4_kernel<true><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
-    else if (head_dim == 128) cache_tree4_kernel<false><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
+    else if (head_dim == 128 && a.mask != nullptr) LSK_CACHE_TREE4(true, 2);
+    else if (head_dim == 128 && row_groups == 4) LSK_CACHE_TREE4(false, 2);
+    else if (head_dim == 128) LSK_CACHE_TREE4(false, 1);
     else if (a.mask != nullptr) cache_tree_kernel<64, FMT_KV4, true><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
     else cache_tree_kernel<64, FMT_KV4, false><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
+#undef LSK_CACHE_TREE4
 #undef LSK_CACHE_TREE
     if ((rc = lsk_check_launch(what))) return rc;
   }

@@ -377,8 +377,10 @@ def test_kv4_attention_of_prompt_pieces_in_a_large_cache(cuda, tokens, D):
     wide = tokens[0] == 20
     split = 64 if wide else 2112
     plan = lsk.AttnPlan(where, Hq, cache, split=split, tree=False)
-    assert plan.causal.n_shared == (2 * 1 + 2 + 2 + 1) * Hkv * wide and plan.causal.n_parts == 2
-    assert plan.causal.row_groups == (4 if wide else 2 if D == 128 else 1)
+    if wide:                                          # (few items of 128 dims: 64 rows each)
+        assert plan.causal.n_shared == (2 * 2 + 3 + 3 + 2 if D == 128 else 2 * 1 + 2 + 2 + 1) * Hkv
+    assert plan.causal.n_parts == (4 if wide and D == 128 else 2)
+    assert plan.causal.row_groups == (2 if D == 128 else 4 if wide else 1)
     got = lsk.kv4_attn(q.to(cuda), cache, plan)
     ref, mag, _ = attention(q.double(), held(k), held(v), tab, 1 / math.sqrt(D))
     assert_close_bf16(got, ref, mag)
@@ -386,6 +388,29 @@ def test_kv4_attention_of_prompt_pieces_in_a_large_cache(cuda, tokens, D):
         alone = lsk.AttnPlan([(0, p0, T, row)], Hq, cache, split=split, tree=False)
         one = lsk.kv4_attn(q[qs:qs + T].to(cuda), cache, alone)
         assert torch.equal(one.view(torch.int16), got[qs:qs + T].view(torch.int16))
+
+
+@pytest.mark.gpu
+def test_kv4_attention_of_many_prompt_pieces(cuda):
+    """More pieces than CUs: items of 128 rows, whose rows have the bits of those in items of 64."""
+    lsk = _lsk()
+    g = _gen(17)
+    B, Hkv, Hq, S, D, n_blocks = 100, 8, 32, 128, 128, 40
+    tab, n = pack_blocks([((7 * i) % B, (11 * i) % 60, 17 + i % 3) for i in range(n_blocks)])
+    k, v = (torch.randn(B, Hkv, S, D, generator=g).to(BF16) for _ in range(2))
+    q = torch.randn(n, Hq, D, generator=g).to(BF16)
+    cache = kv4_from(lsk, cuda, k, v)
+    plan = lsk.AttnPlan(tab, Hq, cache, tree=False)
+    assert plan.causal.row_groups == 4 and plan.causal.n_shared == n_blocks * Hkv
+    got = lsk.kv4_attn(q.to(cuda), cache, plan)
+    few = tab[:9] + tab[-2:]
+    ref, mag, _ = attention(q.double(), held(k), held(v), few, 1 / math.sqrt(D))
+    rows = torch.cat([torch.arange(qs, qs + T) for (qs, _, T, _) in few])
+    assert_close_bf16(got[rows.to(cuda)], ref[rows], mag[rows])
+    for (qs, p0, T, row) in tab:
+        alone = lsk.AttnPlan([(0, p0, T, row)], Hq, cache, tree=False)
+        assert alone.causal.row_groups == 2
+        assert torch.equal(lsk.kv4_attn(q[qs:qs + T].to(cuda), cache, alone), got[qs:qs + T])
 
 
 @pytest.mark.parametrize("D", [64, 128])
