@@ -1360,7 +1360,9 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 //           times the block's tiles of 32 rows are at most n_slots, each tile is an item instead (8B heads, 960
 //           positions, 4 / 2 / 1 row groups: 64 stripes, 64-node trees 30 / 22 / 21 us; 128 stripes, 32 nodes
 //           29 / 22 / 21, 64 nodes 32 / 34 / 37; 256 stripes, 16 nodes - / 29 / 26, 32 nodes 31 / 34 / 37, 64 nodes
-//           46 / 60 / 69).
+//           46 / 60 / 69).  A 4-bit cache of 128 dims: items of 64 rows where the launch has at most HALF_ITEMS of 128
+//           (below; 128 stripes, 64 nodes, 16 trees 40 / 36 us), and more than 64 rows are tiles up to n_slots / 2 only
+//           (128 stripes, 30 to 40 nodes 44 / 32 us, 32 stripes, 64 nodes 19 / 25).
 //   wide    a block of more than 64 rows without a mask over a 4-bit cache (a piece of a prompt), where the cache's
 //           stripes times the block's tiles of 32 rows are more than WIDE_TILES: items of 128 rows for the tree kernels,
 //           whose waves share the conversions of K and V (8B heads after 1000 positions, wide / not, unsplit: 256 stripes
@@ -1423,12 +1425,21 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
       if (!wide(rows) && rows > most) most = rows;
     }
   }
-  long n_wide = 0;                                   // items of 128 rows
+  // log2 of a tree's row groups
+  const auto tree_groups = [&](long rows) {
+    const long least = format == FMT_KV4 && head_dim == 128 && rows > 64 ? n_slots / 2 : n_slots;
+    const bool few = (long)max_batch * n_kv_heads * ((rows + 31) / 32) <= least;
+    const int most_groups = row_groups ? row_groups : few ? 1 : 4;
+    int lr = 0;
+    while ((1 << lr) < most_groups && rows > (32L << lr)) ++lr;
+    return lr;
+  };
+  long n_shared = 0;                                 // items of 128 rows
   for (int b = 0; b < nb; ++b) {
     const long rows = (long)blocks[(long)b * 4 + 2] * group;
-    n_wide += wide(rows) ? (rows + 127) / 128 * n_kv_heads : 0;
+    if (tree ? tree_groups(rows) == 2 : wide(rows)) n_shared += (rows + 127) / 128 * n_kv_heads;
   }
-  const int wide_rows = head_dim == 128 && n_wide <= HALF_ITEMS ? 64 : 128;
+  const int shared_rows = format == FMT_KV4 && head_dim == 128 && n_shared <= HALF_ITEMS ? 64 : 128;
   const int tiles = most <= 16 ? 1 : most <= 32 || tree || head_dim == 128 ? 2 : 3;
   struct It { int32_t rec[8]; int cost; };
   thread_local std::vector<It> items, shared;
@@ -1442,10 +1453,7 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
     const int32_t* bm = blocks + (long)b * 4;
     const int pos0 = bm[1];
     const long rows = (long)bm[2] * group;
-    int lr = 0;
-    const bool few = (long)max_batch * n_kv_heads * ((rows + 31) / 32) <= n_slots;
-    const int most_groups = row_groups ? row_groups : few ? 1 : 4;
-    while (tree && (1 << lr) < most_groups && rows > (32L << lr)) ++lr;
+    int lr = tree ? tree_groups(rows) : 0;
     int cap = (16 * tiles) << lr, bsplit = split;
     if (pair(rows)) {
       lr = 1;
@@ -1453,11 +1461,10 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
     }
     if (wide(rows)) {
       lr = 2;
-      cap = wide_rows;
       bsplit = std::max(split, WIDE_SPLIT);
     }
-    const int groups_used = wide(rows) && wide_rows == 64 ? 2 : 1 << lr;
-    used = groups_used > used ? groups_used : used;
+    if (lr == 2) cap = shared_rows;
+    used = std::max(used, lr == 2 && shared_rows == 64 ? 2 : 1 << lr);
     for (long row0 = 0; row0 < rows; row0 += cap) {
       const int nrows = (int)(rows - row0 < cap ? rows - row0 : cap);
       const int end = (int)(pos0 + (row0 + nrows - 1) / group + 1);
@@ -1597,8 +1604,9 @@ static int cache_attn(const char* what, int format, CacheAttnArgs a, const int32
 #define LSK_CACHE_TREE4(TR, QT) cache_tree4_kernel<TR, QT><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items)
     if (format == FMT_BF16) LSK_CACHE_TREE(FMT_BF16, true);
     else if (format == FMT_KV8) LSK_CACHE_TREE(FMT_KV8, true);
-    else if (head_dim == 128 && a.mask != nullptr) LSK_CACHE_TREE4(true, 2);
+    else if (head_dim == 128 && row_groups == 4 && a.mask != nullptr) LSK_CACHE_TREE4(true, 2);
     else if (head_dim == 128 && row_groups == 4) LSK_CACHE_TREE4(false, 2);
+    else if (head_dim == 128 && a.mask != nullptr) LSK_CACHE_TREE4(true, 1);
     else if (head_dim == 128) LSK_CACHE_TREE4(false, 1);
     else if (a.mask != nullptr) cache_tree_kernel<64, FMT_KV4, true><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);
     else cache_tree_kernel<64, FMT_KV4, false><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);

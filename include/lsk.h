@@ -323,7 +323,7 @@ int lsk_kv8_read(int dtype, const void* k8, const void* v8, const void* k_exp, c
  * K / V among up to row_groups (1, 2, 4; 0: by the cache and the block) groups of 32 rows.  Large blocks over a 4-bit
  * cache do so without a mask too (two or four groups), and the largest ones' splits are of 4096 positions at least.
  * n_slots: persistent workgroups, two per CU; recs: their items, and behind them the n_shared items of four row groups
- * (a workgroup each; without a mask of at most 64 rows where row_groups is 2).  meta = [groups int32 n_groups*8][recs
+ * (a workgroup each; over a 4-bit cache of at most 64 rows where row_groups is 2).  meta = [groups int32 n_groups*8][recs
  * n_slots*n_rounds*8, then n_shared*8]; counts[9] = {tokens, n_groups, n_parts, n_rounds, tiles, part_rows, words of
  * meta, row_groups used, n_shared}.  meta == NULL: counts only; meta_cap too small: LSK_EWORKSPACE with counts written. */
 int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int max_batch, int n_kv_heads,

@@ -414,8 +414,9 @@ def test_kv4_attention_of_many_prompt_pieces(cuda):
 
 
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("tree", [False, True])
 @pytest.mark.parametrize("G,split", [(4, 64), (1, 512), (8, 8192), (3, 4160)])
-def test_kv4_plans_cover_every_row_and_position_once(G, split, D):
+def test_kv4_plans_cover_every_row_and_position_once(G, split, tree, D):
     lsk = _lsk()
     rng = np.random.default_rng(G)
     B, Hkv, S = 90, 3, 8192
@@ -423,14 +424,16 @@ def test_kv4_plans_cover_every_row_and_position_once(G, split, D):
     cache = lsk.KV4(*(t.expand(B, Hkv, S // 64, *t.shape[3:]) for t in cache))
     blocks = [(r, int(rng.integers(0, S - 400)), int(t)) for r, t in enumerate((400, 1, 64 // G, 65, 0, 200, 130))]
     tab, _ = pack_blocks(blocks)
-    p = lsk.AttnPlan(tab, G * Hkv, cache, split=split, tree=False).causal
+    plan = lsk.AttnPlan(tab, G * Hkv, cache, split=split, tree=tree)
+    p = plan.tree if tree else plan.causal
     items, seen = _items(p, p), []
     for (q0, p0, t, _) in tab:
-        wide = t * G > 64 and B * Hkv * -(-t * G // 32) > (768 if D == 128 else 1280)
+        wide = not tree and t * G > 64 and B * Hkv * -(-t * G // 32) > (768 if D == 128 else 1280)
         two = D == 128 and not wide and -(-t * G // 48) < -(-t * G // 32) and B * Hkv * -(-t * G // 32) > 512
         covered = np.zeros((Hkv, t * G, S), dtype=np.int8)
         for (_, r0, nr, g, h, lo, hi, part) in (i for i in items if i[0] == q0 and t):
-            assert g == (4 if wide else 2 if two else 1) and nr <= (128 if wide else 48)
+            assert tree or (g == (4 if wide else 2 if two else 1) and nr <= (128 if wide else 48))
+            assert nr <= 32 * g or not tree and g < 4 and nr <= 48
             assert part < 0 or nr <= p.part_rows
             assert lo % (max(split, 4096) if wide else split) == 0
             assert (part >= 0) == (p0 + (r0 + nr - 1) // G + 1 > (max(split, 4096) if wide else split))
