@@ -35,6 +35,16 @@ extern "C" {
 const char* lsk_last_error(void);
 int lsk_abi_version(void);
 
+/* An entry point by its number, its n_args arguments in order as 64-bit words: integers and pointers as they are, a
+ * float as the bits of a double.  For bindings that pay for each argument. */
+#define LSK_CALL_KV4_APPEND 0
+#define LSK_CALL_KV4_READ 1
+#define LSK_CALL_KV4_ATTN 2
+#define LSK_CALL_QK_NORM_ROPE 3
+#define LSK_CALL_QUANT_ROWS_I8 4
+#define LSK_CALL_GEMM_I8 5
+int lsk_call(int entry, int n_args, const int64_t* args);
+
 /* RMSNorm: out = w * (x * rsqrt(mean(x^2) + eps)).to(dtype).
  * Replaces common/model.py:153-156 (rms_norm), used at solutions/packed.py:175,183 and common/model.py:330. */
 int lsk_rmsnorm(int dtype, const void* x, const void* w, void* out, int n_rows, int dim, float eps, long ldx,

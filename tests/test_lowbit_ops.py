@@ -929,6 +929,29 @@ def test_lowbit_entry_points_refuse_bad_arguments():
     assert gm(a12=2, a13=32) == -2 and gm(a12=2, a10=24, a13=24) == -2 and gm(a1=24) == -1 and gm(a9=0) == 0
 
 
+def test_calls_with_packed_arguments_are_the_same_calls():
+    lsk = _lsk()
+    lib = lsk.load()
+    P = 16
+    calls = {"lsk_kv4_append": (1, P, P, 128, 64, P, P, P, P, P, P, 0, 2, 64, 3, 128, 0),
+             "lsk_kv4_read": (1, P, P, P, P, P, P, P, P, 0, 2, 64, 3, 128, 0),
+             "lsk_kv4_attn": (P, 512, 64, P, P, P, P, 0, 0, 0, 0, 0, P, 0, 1, 0, 1, 1, 16, P, 8, 2, 64, 128, 0.125, 0, 0, 0),
+             "lsk_qk_norm_rope": (1, P, 768, P, P, 1e-5, P, P, 64, P, P, 0, 4, 4, 64, P, 0, P, P, 2, 64, 0),
+             "lsk_quant_rows_i8": (1, P, 64, P, P, 0, 64, 0),
+             "lsk_gemm_i8": (1, P, P, P, P, P, 64, 0, 0, 0, 64, 64, 0, 0, 0)}
+    assert set(calls) == set(lsk._CALLS)
+    for name, args in calls.items():
+        number, n, pack = lsk._CALLS[name]
+        assert n == len(args) and lib.lsk_call(number, n, pack(*args)) == getattr(lib, name)(*args) == 0
+        for i, x in enumerate(args):
+            bad = args[:i] + (-1.0 if isinstance(x, float) else -7,) + args[i + 1:]
+            got, text = lib.lsk_call(number, n, pack(*bad)), lib.lsk_last_error()
+            assert got == getattr(lib, name)(*bad)
+            assert got == 0 or text == lib.lsk_last_error() and text.startswith(name.encode())
+        assert lib.lsk_call(number, n - 1, pack(*args)) == -1
+    assert lib.lsk_call(len(calls), 1, bytes(8)) == lib.lsk_call(-1, 1, bytes(8)) == lib.lsk_call(0, 17, None) == -1
+
+
 def test_kv4_plans_and_caches_refuse_what_does_not_fit():
     lsk = _lsk()
     cache = lsk.KV4.zeros(2, 2, 128, 64, "cpu")

@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import struct
 from pathlib import Path
 from typing import NamedTuple
 
@@ -33,6 +34,7 @@ _P, _I, _L, _F, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_floa
 _SIGS = {
     "lsk_last_error": (ctypes.c_char_p, []),
     "lsk_abi_version": (_I, []),
+    "lsk_call": (_I, [_I, _I, ctypes.c_char_p]),
     "lsk_rmsnorm": (_I, [_I, _P, _P, _P, _I, _I, _F, _L, _L, _P]),
     "lsk_rope_append": (_I, [_I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
     "lsk_kv_append": (_I, [_I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
@@ -105,6 +107,11 @@ _SIGS = {
 PROF_CLASSES = ("rmsnorm", "gemm_qkv", "rope_append", "attention", "gemm_o", "gemm_w13", "gemm_w2", "gemm_lm_head",
                 "argmax", "glue")
 EXPORTS = tuple(_SIGS)
+# what lsk_call calls, in the order of its numbers: name -> (number, arguments, their packing)
+_CALLS = {name: (i, len(_SIGS[name][1]),
+                 struct.Struct("=" + "".join("d" if t is _F else "q" for t in _SIGS[name][1])).pack)
+          for i, name in enumerate(("lsk_kv4_append", "lsk_kv4_read", "lsk_kv4_attn", "lsk_qk_norm_rope",
+                                    "lsk_quant_rows_i8", "lsk_gemm_i8"))}
 
 _lib = None
 
@@ -139,10 +146,8 @@ def _check(rc: int, what: str) -> None:
         raise LskError(f"{what} failed ({rc}): {msg}")
 
 
-def _ptr(t) -> int | None:
-    if t is None:
-        return None
-    return t.data_ptr()
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -550,12 +555,15 @@ def _one_device(first: torch.Tensor, *ts) -> int:
 
 def _launch(dev: int, what: str, *args) -> None:
     """Calls `what` with args and device dev's current stream; dev is the current device for the call."""
-    fn = getattr(_lib or load(), what)
-    if torch._C._cuda_getDevice() == dev:
-        rc = fn(*args, _stream(dev))
-    else:
+    lib = _lib or load()
+    if torch._C._cuda_getDevice() != dev:
         with torch.cuda.device(dev):
-            rc = fn(*args, _stream())
+            rc = getattr(lib, what)(*args, _stream())
+    elif what in _CALLS:
+        number, n, pack = _CALLS[what]
+        rc = lib.lsk_call(number, n, pack(*args, _stream(dev)))
+    else:
+        rc = getattr(lib, what)(*args, _stream(dev))
     if rc:
         _check(rc, what)
 
@@ -590,7 +598,7 @@ class KV8(_KV8):
     e + 127.  A layer's tensors, or with a leading layer axis those of several:
       k [B, Hkv, S/64, 4, D/64, 64, 16] and v [B, Hkv, S/64, D, 64] float8_e4m3fn, ks and vs [B, Hkv, S] uint8.
     The tensors' types, shapes and devices are checked by the object's first use; they have to stay as they are."""
-    _checked = None                                   # (layers, dims, device, addresses) that the tensors were found with
+    _checked = None                                   # (layers, dims, device) that the tensors were found with
 
     @classmethod
     def zeros(cls, max_batch: int, n_kv_heads: int, max_seq: int, head_dim: int, device, layers: int | None = None):
@@ -636,7 +644,7 @@ class KV8(_KV8):
             _want(what, "v codes", v, _E4M3, want_v)
             _want(what, "k exponents", ks, torch.uint8, lead)
             _want(what, "v exponents", vs, torch.uint8, lead)
-        self._checked = layers, (lead[-3], lead[-2], S, D), _same_device(k, v, ks, vs), self.ptrs()
+        self._checked = layers, (lead[-3], lead[-2], S, D), _same_device(k, v, ks, vs)
         return self._checked[1]
 
 
@@ -652,7 +660,7 @@ class KV4(_KV4):
     byte e + 127.  A layer's tensors, or with a leading layer axis those of several, all uint8:
       k and v [B, Hkv, S/64, D/32, 64, 16], ks [B, Hkv, S/64, D/32, 16, 4] and vs [B, Hkv, S/64, D/32, 64].
     The tensors' types, shapes and devices are checked by the object's first use; they have to stay as they are."""
-    _checked = None                                   # (layers, dims, device, addresses) that the tensors were found with
+    _checked = None                                   # (layers, dims, device) that the tensors were found with
 
     @classmethod
     def zeros(cls, max_batch: int, n_kv_heads: int, max_seq: int, head_dim: int, device, layers: int | None = None):
@@ -698,8 +706,7 @@ class KV4(_KV4):
             _want(what, "v codes", v, torch.uint8, codes)
             _want(what, "k exponents", ks, torch.uint8, (*lead, 16, 4))
             _want(what, "v exponents", vs, torch.uint8, (*lead, 64))
-        self._checked = layers, (lead[-4], lead[-3], lead[-2] * 64, lead[-1] * 32), _same_device(k, v, ks, vs), \
-            self.ptrs()
+        self._checked = layers, (lead[-4], lead[-3], lead[-2] * 64, lead[-1] * 32), _same_device(k, v, ks, vs)
         return self._checked[1]
 
 
@@ -712,7 +719,7 @@ def _cache_of(name: str, cache, kind) -> tuple:
     """(dims, device, addresses) of a layer's cache of that kind; LskError otherwise."""
     _want_kind(name, cache, kind)
     cache.check(name)
-    return cache._checked[1:]
+    return *cache._checked[1:], cache.ptrs()
 
 
 def _codes_append(name: str, kind, k, v, cache, rows_i32, pos_i32) -> None:
@@ -971,7 +978,7 @@ def _codes_attn(name: str, kind, fmt: int, q, cache, plan: AttnPlan, mask, scale
     scale, out, workspace, ws = _plan_call(name, dev, q, plan, p, dims, fmt, cache.k.dtype, mask, scale, out, workspace)
     if p.n_items:
         st_t, st_h, _ = q.stride()
-        masked = (None, 0) if mask is None else (mask.data_ptr(), mask.shape[1])
+        masked = (0, 0) if mask is None else (mask.data_ptr(), mask.shape[1])
         _launch(dev, "lsk_" + name, q.data_ptr(), st_t, st_h, *ptrs, *masked, *p.args, out.data_ptr(), plan.n_heads,
                 dims[1], dims[3], dims[2], scale, _ptr(workspace), ws)
     return out

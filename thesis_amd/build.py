@@ -12,7 +12,8 @@ from pathlib import Path
 
 ROOT = Path(__file__).resolve().parents[1]
 SOURCES = ["lsk_elementwise.hip", "lsk_attention.hip", "lsk_attn_cache.hip", "lsk_kv8.hip", "lsk_kv4.hip", "lsk_tree.hip",
-           "lsk_norm_rope.hip", "lsk_gemm.hip", "lsk_gemm_deep.hip", "lsk_gemm_i8.hip", "lsk_runtime.hip"]
+           "lsk_norm_rope.hip", "lsk_gemm.hip", "lsk_gemm_deep.hip", "lsk_gemm_i8.hip", "lsk_runtime.hip",
+           "lsk_call.hip"]
 OUT = ROOT / "thesis_amd" / "_lib" / "liblsk.so"
 
 FLAGS = [
