@@ -266,7 +266,7 @@ __device__ __forceinline__ void softmax_tile(lsk_f32x4 (&s)[NA], uint32_t reads,
     mt = fmaxf(mt, s[i >> 2][i & 3]);
   }
   mt *= scale_log2;
-  const bool far = FAR && fabsf(mt) > 0x1p26f;
+  const bool far = FAR && fabsf(mt) > 0x1p26f && (FULL || mt != -INFINITY);
   float mm = m;
   if (__builtin_amdgcn_ballot_w64(mt > m + LAG || far) != 0ull) {
     mt = rows_max(mt);
@@ -320,7 +320,7 @@ __device__ __forceinline__ uint32_t largest8(lsk_bf16x8 x) {  // |bits|
   for (int i = 0; i < 4; ++i) m = max(m, max((uint32_t)w[i] & 0x7fffu, (uint32_t)w[i] >> 16 & 0x7fffu));
   return m;
 }
-// the smallest e >= 10 - 127 with m <= 448 * 2^e (biased; lo's is four less), 0 where m is not finite
+// the smallest e >= 10 - 127 with m <= 448 * 2^e (biased; lo's is four less); 2^0 where m is not finite
 __device__ __forceinline__ int power_of(uint32_t m) {
   return m >= 0x7f80u ? 127 : max((int)(m >> 7) - 8 + ((m & 0x7fu) > 0x60u ? 1 : 0), 10);
 }
@@ -529,7 +529,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
     for (int qt = 0; qt < QT; ++qt) {
       const int rl = rb + 16 * qt + l16;
       qpos[qt] = rl < cur.nrows ? cur.pos0 + (cur.row0 + rl) / G : -1;
-      qe[qt] = KOP ? s_qe[KOP ? rl : 0][lg] : 0;
+      qe[qt] = KOP ? s_qe[KOP ? min(rl, QROWS - 1) : 0][lg] : 0;
     }
     // slots that every row of the item reads
     const int full_lim = min(kv_hi - 1, TREE ? cur.pos0 - 1 : cur.pos0 + cur.row0 / G);
@@ -559,7 +559,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
       constexpr bool FULL = decltype(full_)::value;
       constexpr int NQ = decltype(nq_)::value;
       // V's scales of a 4-bit cache multiply the weights, once for every 32 dims; with more than one query tile V itself
-      // (a wave's instructions per step of 64 positions and 128 dims: 160 a tile against 192)
+      // (a wave's instructions per step of 64 positions and 128 dims: 160 a tile against 192; a row's bits are the same)
       constexpr bool VS = KV4 && FULL && NQ > 1;
       // In a step that some row does not read whole, a slot whose V holds an infinity or NaN must not reach the rows
       // that do not read it (0 x NaN): the values past the item and the non-finite ones are cleared here, and the rows
@@ -1361,8 +1361,10 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 //           positions, 4 / 2 / 1 row groups: 64 stripes, 64-node trees 30 / 22 / 21 us; 128 stripes, 32 nodes
 //           29 / 22 / 21, 64 nodes 32 / 34 / 37; 256 stripes, 16 nodes - / 29 / 26, 32 nodes 31 / 34 / 37, 64 nodes
 //           46 / 60 / 69).  A 4-bit cache of 128 dims: items of 64 rows where the launch has at most HALF_ITEMS of 128
-//           (below; 128 stripes, 64 nodes, 16 trees 40 / 36 us), and more than 64 rows are tiles up to n_slots / 2 only
-//           (128 stripes, 30 to 40 nodes 44 / 32 us, 32 stripes, 64 nodes 19 / 25).
+//           (below; 128 stripes, 64 nodes, 16 trees 40 / 36 us); and all blocks of more than 64 rows count as MANY_TILES
+//           tiles, since blocks on both sides of the rule are two launches (300 to 900 positions, tiles / both / items of
+//           64 rows: 64 stripes, 10 to 40 nodes 17 / 35 / -; 128 stripes, 10 to 40 nodes 22 / 35 / -, 20 to 64 34 / 40 /
+//           24; 256 stripes, 10 to 64 nodes 56 / 56 / -).
 //   wide    a block of more than 64 rows without a mask over a 4-bit cache (a piece of a prompt), where the cache's
 //           stripes times the block's tiles of 32 rows are more than WIDE_TILES: items of 128 rows for the tree kernels,
 //           whose waves share the conversions of K and V (8B heads after 1000 positions, wide / not, unsplit: 256 stripes
@@ -1384,6 +1386,7 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 #define WIDE_SPLIT 4096
 #define PAIR_TILES 512
 #define HALF_ITEMS 256
+#define MANY_TILES 4
 static int cache_plan(const char* what, const int32_t* blocks, int nb, int group, int split, int max_batch,
                       int n_kv_heads, int head_dim, int format, int tree, int row_groups, int n_slots, int32_t* meta,
                       long meta_cap, long* counts) {
@@ -1427,8 +1430,9 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
   }
   // log2 of a tree's row groups
   const auto tree_groups = [&](long rows) {
-    const long least = format == FMT_KV4 && head_dim == 128 && rows > 64 ? n_slots / 2 : n_slots;
-    const bool few = (long)max_batch * n_kv_heads * ((rows + 31) / 32) <= least;
+    // (a 4-bit cache of 128 dims: the same for all blocks of more than 64 rows)
+    const long n_tiles = format == FMT_KV4 && head_dim == 128 && rows > 64 ? MANY_TILES : (rows + 31) / 32;
+    const bool few = (long)max_batch * n_kv_heads * n_tiles <= n_slots;
     const int most_groups = row_groups ? row_groups : few ? 1 : 4;
     int lr = 0;
     while ((1 << lr) < most_groups && rows > (32L << lr)) ++lr;

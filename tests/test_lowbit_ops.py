@@ -789,6 +789,31 @@ def test_gemm_i8(cuda, dtype, epilogue, M, N, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("epilogue,M,N,K", [(1, 131, 106, 70), (0, 130, 2048, 8192), (0, 65, 10006, 70),
+                                            (1, 65, 10004, 4100), (1, 1602, 20011, 70), (0, 65, 20030, 70),
+                                            (0, 257, 20002, 1100), (2, 65, 10000, 2104), (2, 66, 96, 70),
+                                            (2, 65, 96, 600), (2, 65, 28000, 2100)])
+def test_gemm_i8_of_many_tokens(cuda, epilogue, M, N, K):
+    """A shape for each tiling of the many-token kernel; every row has the bits of the few-token kernel's."""
+    lsk = _lsk()
+    g = _gen(M + N + K)
+    x = torch.randn(M, K, generator=g).to(BF16).to(cuda)
+    w = lsk.PackedWeightI8(torch.randn(2 * N if epilogue == 2 else N, K, generator=g).to(cuda))
+    res = torch.randn(M, N, generator=g).to(BF16).to(cuda) if epilogue == 1 else None
+    a = lsk.quant_rows_i8(x)
+    got = lsk.gemm_i8(a, w, residual=res, epilogue=epilogue)
+    for lo in range(0, M, 64):
+        part = lsk.gemm_i8(lsk.quant_rows_i8(x[lo:lo + 64]), w, residual=None if res is None else res[lo:lo + 64],
+                           epilogue=epilogue)
+        assert torch.equal(part, got[lo:lo + 64])
+    pick = torch.tensor([0, M // 2, M - 1])
+    ca, sa = rows8(x[pick.to(cuda)].cpu())
+    cw, sw = (t.cpu() for t in (w.unpack().double(), w.scales))
+    assert_project(got[pick.to(cuda)], project(ca, sa, cw, sw, BF16, epilogue, None if res is None else
+                                               res[pick.to(cuda)].cpu()), BF16)
+
+
+@pytest.mark.gpu
 def test_gemm_i8_sums_do_not_overflow(cuda):
     """The longest rows, all of the largest magnitude: 127^2 * 131072 is below 2^31, and exact in fp32's rounding."""
     lsk = _lsk()
