@@ -364,7 +364,25 @@ __device__ __forceinline__ void scores4(const lsk_i32x4 (&k)[4], int ks, const i
 #define CACHE_WAVES 4
 #define PAIR_ROWS 48  // of an item of two row groups without a mask: with the merge's buffer half a CU's LDS
 template <int D, int QT, int FMT, bool TREE>
-__global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const CacheAttnArgs A) {
+struct AttnLds {
+  static constexpr bool KOP = FMT == FMT_KV4 && D == 128;       // K's codes are an operand
+  static constexpr bool QREG = QT == 1 && !KOP;      // one tile: Q fragments in registers (items of one row group)
+  static constexpr bool GROUPS = QT == 2 && (TREE || KOP);      // items of two row groups
+  static constexpr int MT = TREE || QT < ATTN_MERGE_TILES ? 1 : ATTN_MERGE_TILES;  // (two workgroups' fits a CU's)
+  static constexpr int MR = 16 * MT;                 // rows of a wave merged per pass
+  // rows of an item at most
+  static constexpr int QROWS = QREG ? 0 : GROUPS && TREE ? 32 * QT : GROUPS && D == 128 ? PAIR_ROWS : 16 * QT;
+  static constexpr int QLD = D + 8;                  // 16 rows' 16-byte reads hit distinct banks
+  alignas(16) float o[CACHE_WAVES][MR][D + 4];
+  alignas(16) uint16_t q[QREG ? 1 : QROWS][QLD];
+  uint16_t qe[KOP ? QROWS : 1][4];                   // (KOP: a row of q is its hi, then its lo)
+  float ml[KOP ? 1 : CACHE_WAVES][2][16 * QT];       // (KOP: behind a row of o)
+};
+
+// The items of slot `block`.
+template <int D, int QT, int FMT, bool TREE>
+__device__ __forceinline__ void cache_attn_items(const CacheAttnArgs& A, AttnLds<D, QT, FMT, TREE>& lds, int block) {
+  using L = AttnLds<D, QT, FMT, TREE>;
   constexpr bool KV8 = FMT == FMT_KV8, KV4 = FMT == FMT_KV4, CODES = KV8 || KV4;
   constexpr int STEP = CODES ? 64 : 32;              // positions per step of a wave
   constexpr int BLK = (KV4 ? 32 : 64) * D;           // bytes of a step's K, and of its V
@@ -376,26 +394,20 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
   constexpr int LT = KV4 ? CT / 2 : CT;              // 16-byte loads per lane of a step, for K and for V
   constexpr int NW = CACHE_WAVES;
   constexpr int GR = 16 * QT;                        // rows of a wave
-  constexpr bool KOP = KV4 && D == 128;              // K's codes are an operand
-  constexpr bool QREG = QT == 1 && !KOP;             // one tile: Q fragments in registers (items of one row group)
-  constexpr bool GROUPS = QT == 2 && (TREE || KOP);  // items of two row groups
-  constexpr int MT = TREE || QT < ATTN_MERGE_TILES ? 1 : ATTN_MERGE_TILES;  // (two workgroups' LDS fits a CU's)
-  constexpr int MR = 16 * MT;                        // rows of a wave merged per pass
-  // rows of an item at most
-  constexpr int QROWS = QREG ? 0 : GROUPS && TREE ? 2 * GR : GROUPS && D == 128 ? PAIR_ROWS : GR;
-  constexpr int QLD = D + 8;                         // 16 rows' 16-byte reads hit distinct banks
+  constexpr bool KOP = L::KOP, QREG = L::QREG, GROUPS = L::GROUPS;
+  constexpr int MT = L::MT, MR = L::MR, QROWS = L::QROWS;
   constexpr int QCH = D / 8;
   constexpr int QPT = QREG ? 1 : (QROWS * QCH + 64 * NW - 1) / (64 * NW);
-  __shared__ __attribute__((aligned(16))) float s_o[NW][MR][D + 4];
-  __shared__ __attribute__((aligned(16))) uint16_t s_q[QREG ? 1 : QROWS][QLD];
-  __shared__ uint16_t s_qe[KOP ? QROWS : 1][4];      // (KOP: a row is its hi, then its lo)
-  __shared__ float s_ml[KOP ? 1 : NW][2][GR];        // (KOP: behind a row of s_o)
+  auto& s_o = lds.o;
+  auto& s_q = lds.q;
+  auto& s_qe = lds.qe;
+  auto& s_ml = lds.ml;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, lg = lane >> 4;
   const int G = A.G, Hkv = A.Hkv, S = A.S, Hq = Hkv * G;
-  const int32_t* my_recs = A.recs + (long)blockIdx.x * A.n_rounds * 8;
+  const int32_t* my_recs = A.recs + (long)block * A.n_rounds * 8;
 
   // lr: log2 of the item's row groups; the waves of a row group share the item's steps
   struct Item {
@@ -774,6 +786,12 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const C
   }
 }
 
+template <int D, int QT, int FMT, bool TREE>
+__global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const CacheAttnArgs A) {
+  __shared__ AttnLds<D, QT, FMT, TREE> lds;
+  cache_attn_items<D, QT, FMT, TREE>(A, lds, blockIdx.x);
+}
+
 // The end of an item of cache_tree_kernel: a wave's rows, from rb on, or its part of them
 template <bool TREE, int QT, int CT>
 __device__ __forceinline__ void tree_store(const CacheAttnArgs& A, const lsk_f32x4 (&oacc)[QT][CT],
@@ -1033,17 +1051,15 @@ __device__ __forceinline__ void split_q(const uint16_t* q, int lg, i32x8& hi, i3
   exps = powers(lg == 0 ? e[0] : lg == 3 ? e[1] : other);
 }
 
+#define TREE4_BUF (128 / 16 * 2 * 1024)  // a chunk's V in LDS
 template <bool TREE, int QT>
-__global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree4_kernel(const CacheAttnArgs A,
-                                                                         const int32_t* __restrict__ items) {
+__device__ __forceinline__ void cache_tree4_item(const CacheAttnArgs& A, const int32_t* __restrict__ wk, char* s_v) {
   constexpr int D = 128, CT = D / 16, CHUNK = 64, NE = 16;
   constexpr uint32_t ALL = 0xffffu;
-  constexpr int HALF = CT * 1024, BUF = 2 * HALF;    // V fragments (half hv of a lane group's 16 positions, c)
-  __shared__ __attribute__((aligned(16))) char s_v[2 * BUF];
+  constexpr int HALF = CT * 1024, BUF = TREE4_BUF;   // V fragments (half hv of a lane group's 16 positions, c)
   const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = A.G, Hkv = A.Hkv;
-  const int32_t* wk = items + (long)blockIdx.x * 8;
   const int q_start = wk[0], row0 = wk[1], nrows = wk[2] & 1023, kvh = wk[2] >> 12;
   const int kv_lo = wk[3], kv_hi = wk[4], part = wk[5], pos0 = wk[6], crow = wk[7];
   const int rb = wave * 16 * QT;
@@ -1143,6 +1159,27 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree4_kernel(const C
   chunks(std::true_type{}, min(kv_hi, TREE ? pos0 : pos0 + row0 / G + 1) - CHUNK + 1);  // (every row reads them whole)
   chunks(std::false_type{}, kv_hi);
   tree_store<TREE>(A, oacc, m_run, l_run, q_start, row0, nrows, rb, kvh, part, pos0);
+}
+
+template <bool TREE, int QT>
+__global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree4_kernel(const CacheAttnArgs A,
+                                                                         const int32_t* __restrict__ items) {
+  __shared__ __attribute__((aligned(16))) char s_v[2 * TREE4_BUF];
+  cache_tree4_item<TREE, QT>(A, items + (long)blockIdx.x * 8, s_v);
+}
+
+// Both in one launch: the first n_shared workgroups take an item each, the others are the slots of cache_attn_kernel (one
+// launch after the other / this, 8B heads, 300 to 900 positions: 32 trees of 10 to 64 nodes 56 / 39 us, of 10 to 30 40 /
+// 25, 24 of 10 to 64 49 / 33; two and three prompts of up to 500 tokens, 7B heads, 38 / 26 and 34 / 25).
+template <bool TREE, int QT>
+__global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_both4_kernel(const CacheAttnArgs A,
+                                                                         const int32_t* __restrict__ items, int n_shared) {
+  __shared__ union {
+    AttnLds<128, 2, FMT_KV4, TREE> attn;
+    char v[2 * TREE4_BUF];
+  } lds;
+  if ((int)blockIdx.x < n_shared) cache_tree4_item<TREE, QT>(A, items + (long)blockIdx.x * 8, lds.v);
+  else cache_attn_items<128, 2, FMT_KV4, TREE>(A, lds.attn, blockIdx.x - n_shared);
 }
 
 // Merge the splits of a row in split order: M = max_s m_s, w_s = exp2(m_s - M), out = sum w_s O_s / sum w_s l_s (zeros
@@ -1362,9 +1399,8 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 //           29 / 22 / 21, 64 nodes 32 / 34 / 37; 256 stripes, 16 nodes - / 29 / 26, 32 nodes 31 / 34 / 37, 64 nodes
 //           46 / 60 / 69).  A 4-bit cache of 128 dims: items of 64 rows where the launch has at most HALF_ITEMS of 128
 //           (below; 128 stripes, 64 nodes, 16 trees 40 / 36 us); and all blocks of more than 64 rows count as MANY_TILES
-//           tiles, since blocks on both sides of the rule are two launches (300 to 900 positions, tiles / both / items of
-//           64 rows: 64 stripes, 10 to 40 nodes 17 / 35 / -; 128 stripes, 10 to 40 nodes 22 / 35 / -, 20 to 64 34 / 40 /
-//           24; 256 stripes, 10 to 64 nodes 56 / 56 / -).
+//           tiles (8B heads, 300 to 900 positions, tiles for all / these items: 64 stripes, 10 to 40 nodes 17 / 21 us, 96
+//           stripes, 10 to 64 nodes 30 / 23, 128 stripes, 20 to 64 nodes 34 / 24).
 //   wide    a block of more than 64 rows without a mask over a 4-bit cache (a piece of a prompt), where the cache's
 //           stripes times the block's tiles of 32 rows are more than WIDE_TILES: items of 128 rows for the tree kernels,
 //           whose waves share the conversions of K and V (8B heads after 1000 positions, wide / not, unsplit: 256 stripes
@@ -1386,7 +1422,7 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 #define WIDE_SPLIT 4096
 #define PAIR_TILES 512
 #define HALF_ITEMS 256
-#define MANY_TILES 4
+#define MANY_TILES 8
 static int cache_plan(const char* what, const int32_t* blocks, int nb, int group, int split, int max_batch,
                       int n_kv_heads, int head_dim, int format, int tree, int row_groups, int n_slots, int32_t* meta,
                       long meta_cap, long* counts) {
@@ -1587,7 +1623,8 @@ static int cache_attn(const char* what, int format, CacheAttnArgs a, const int32
     else if (tiles == 1) LSK_CACHE_ATTN(64, 1, F, TR);                     \
     else if (tiles == 2) LSK_CACHE_ATTN(64, 2, F, TR);                     \
   } while (0)
-  if (a.n_rounds == 0) ;
+  const bool both = format == FMT_KV4 && head_dim == 128 && a.n_rounds > 0 && n_shared > 0;
+  if (a.n_rounds == 0 || both) ;
   else if (format == FMT_BF16) LSK_CACHE_ATTN_D(FMT_BF16, true);
   else if (format == FMT_KV8 && a.mask != nullptr) LSK_CACHE_ATTN_D(FMT_KV8, true);
   else if (format == FMT_KV4 && a.mask != nullptr) LSK_CACHE_ATTN_D(FMT_KV4, true);
@@ -1597,7 +1634,7 @@ static int cache_attn(const char* what, int format, CacheAttnArgs a, const int32
   else LSK_CACHE_ATTN_D(FMT_KV4, false);
 #undef LSK_CACHE_ATTN_D
 #undef LSK_CACHE_ATTN
-  if (a.n_rounds > 0 && (rc = lsk_check_launch(what))) return rc;
+  if (a.n_rounds > 0 && !both && (rc = lsk_check_launch(what))) return rc;
   if (n_shared > 0) {
     const int32_t* items = a.recs + 8L * n_slots * a.n_rounds;
 #define LSK_CACHE_TREE(F, TR)                                                                        \
@@ -1605,7 +1642,11 @@ static int cache_attn(const char* what, int format, CacheAttnArgs a, const int32
     if (head_dim == 128) cache_tree_kernel<128, F, TR><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items); \
     else cache_tree_kernel<64, F, TR><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);                 \
   } while (0)
-#define LSK_CACHE_TREE4(TR, QT) cache_tree4_kernel<TR, QT><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items)
+#define LSK_CACHE_TREE4(TR, QT)                                                                                     \
+  do {                                                                                                             \
+    if (both) cache_both4_kernel<TR, QT><<<n_shared + n_slots, 64 * TREE_WAVES, 0, s>>>(a, items, n_shared);        \
+    else cache_tree4_kernel<TR, QT><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);                                 \
+  } while (0)
     if (format == FMT_BF16) LSK_CACHE_TREE(FMT_BF16, true);
     else if (format == FMT_KV8) LSK_CACHE_TREE(FMT_KV8, true);
     else if (head_dim == 128 && row_groups == 4 && a.mask != nullptr) LSK_CACHE_TREE4(true, 2);
