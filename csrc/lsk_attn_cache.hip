@@ -1397,18 +1397,21 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 //           times the block's tiles of 32 rows are at most n_slots, each tile is an item instead (8B heads, 960
 //           positions, 4 / 2 / 1 row groups: 64 stripes, 64-node trees 30 / 22 / 21 us; 128 stripes, 32 nodes
 //           29 / 22 / 21, 64 nodes 32 / 34 / 37; 256 stripes, 16 nodes - / 29 / 26, 32 nodes 31 / 34 / 37, 64 nodes
-//           46 / 60 / 69).  A 4-bit cache of 128 dims: items of 64 rows where the launch has at most HALF_ITEMS of 128
-//           (below; 128 stripes, 64 nodes, 16 trees 40 / 36 us); and all blocks of more than 64 rows count as MANY_TILES
-//           tiles (8B heads, 300 to 900 positions, tiles for all / these items: 64 stripes, 10 to 40 nodes 17 / 21 us, 96
-//           stripes, 10 to 64 nodes 30 / 23, 128 stripes, 20 to 64 nodes 34 / 24).
-//   wide    a block of more than 64 rows without a mask over a 4-bit cache (a piece of a prompt), where the cache's
-//           stripes times the block's tiles of 32 rows are more than WIDE_TILES: items of 128 rows for the tree kernels,
+//           46 / 60 / 69).  A 4-bit cache of 128 dims: items of 4 row groups from 33 rows on, of 64 rows where that fits
+//           them better (below; 512 stripes, 7B heads, trees of 33 to 64 nodes, 2 groups / these 32 / 27 us, 768 stripes
+//           of 20 to 40 41 / 37; behind with few items of long contexts, 512 stripes of 20 to 40 nodes 29 / 30), and all
+//           blocks of more than 64 rows count as MANY_TILES tiles (8B heads, 300 to 900 positions, tiles for all / these
+//           items: 64 stripes, 10 to 40 nodes 17 / 21 us, 96 stripes, 10 to 64 nodes 30 / 23, 128 stripes, 20 to 64
+//           nodes 34 / 24).
+//   wide    a block of more than 64 rows (128 dims: 48) without a mask over a 4-bit cache (a piece of a prompt), where
+//           the cache's stripes times the block's tiles of 32 rows are more than WIDE_TILES: items of 128 rows for the tree kernels,
 //           whose waves share the conversions of K and V (8B heads after 1000 positions, wide / not, unsplit: 256 stripes
 //           of 64 tokens 52 / 83 us, 64 stripes of 256 54 / 88; 1024 tiles, 64 stripes of 128, 36 / 45; behind at 512: 8
 //           of 512 tokens 29 / 26; 17 tokens in 256 stripes 39 / 38; 1B heads: 64 stripes of 128 tokens 37 / 32, of 256
-//           44 / 60).  Over 128 dims items are of 64 rows, one query tile a wave, where the launch has at most
-//           HALF_ITEMS of 128, one for each CU: it is bound by the longest item, and two workgroups' products and softmax
-//           overlap (251 items, one of 1001 tokens: 53 -> 44 us; 376, one of 1500: 69 -> 80; a row's bits are the same).
+//           44 / 60; 8B heads, 64 requests of 16 tokens 34 / 45).  Over 128 dims items are of 64 rows, one query tile a wave,
+//           where the launch has at most HALF_ITEMS of 128, one for each CU, since it is bound by the longest item, and two
+//           workgroups' products and softmax overlap (251 items, one of 1001 tokens: 53 -> 44 us; 376, one of 1500: 69 ->
+//           80), and where items of 128 would be less than two thirds full; a row's bits are the same.
 //           The cache full of such blocks has 192 items of 128 rows and more, so its splits are of WIDE_SPLIT positions
 //           at least (8 stripes, a prompt of 4001 tokens: 640 positions 218 us, 1280 174, 2560 155, whole 142; the other
 //           way round for one short piece in a large cache: 256 tokens after 5000 whole 107, 2560 63).
@@ -1449,7 +1452,7 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
     n_tokens += T;
   }
   const auto wide = [&](long rows) {
-    return format == FMT_KV4 && !tree && rows > 64 &&
+    return format == FMT_KV4 && !tree && rows > (head_dim == 128 ? PAIR_ROWS : 64) &&
            (long)max_batch * n_kv_heads * ((rows + 31) / 32) > WIDE_TILES(head_dim);
   };
   const auto pair = [&](long rows) {
@@ -1472,14 +1475,18 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
     const int most_groups = row_groups ? row_groups : few ? 1 : 4;
     int lr = 0;
     while ((1 << lr) < most_groups && rows > (32L << lr)) ++lr;
+    if (format == FMT_KV4 && head_dim == 128 && most_groups == 4 && lr == 1) lr = 2;
     return lr;
   };
-  long n_shared = 0;                                 // items of 128 rows
+  long n_shared = 0, n_half = 0;                     // items of 128 rows, of 64
   for (int b = 0; b < nb; ++b) {
     const long rows = (long)blocks[(long)b * 4 + 2] * group;
-    if (tree ? tree_groups(rows) == 2 : wide(rows)) n_shared += (rows + 127) / 128 * n_kv_heads;
+    if (tree ? tree_groups(rows) < 2 : !wide(rows)) continue;
+    n_shared += (rows + 127) / 128 * n_kv_heads;
+    n_half += (rows + 63) / 64 * n_kv_heads;
   }
-  const int shared_rows = format == FMT_KV4 && head_dim == 128 && n_shared <= HALF_ITEMS ? 64 : 128;
+  const bool half = n_shared <= HALF_ITEMS || 2 * n_half < 3 * n_shared;
+  const int shared_rows = format == FMT_KV4 && head_dim == 128 && half ? 64 : 128;
   const int tiles = most <= 16 ? 1 : most <= 32 || tree || head_dim == 128 ? 2 : 3;
   struct It { int32_t rec[8]; int cost; };
   thread_local std::vector<It> items, shared;

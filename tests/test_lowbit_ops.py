@@ -428,7 +428,7 @@ def test_kv4_plans_cover_every_row_and_position_once(G, split, tree, D):
     p = plan.tree if tree else plan.causal
     items, seen = _items(p, p), []
     for (q0, p0, t, _) in tab:
-        wide = not tree and t * G > 64 and B * Hkv * -(-t * G // 32) > (768 if D == 128 else 1280)
+        wide = not tree and t * G > (48 if D == 128 else 64) and B * Hkv * -(-t * G // 32) > (768 if D == 128 else 1280)
         two = D == 128 and not wide and -(-t * G // 48) < -(-t * G // 32) and B * Hkv * -(-t * G // 32) > 512
         covered = np.zeros((Hkv, t * G, S), dtype=np.int8)
         for (_, r0, nr, g, h, lo, hi, part) in (i for i in items if i[0] == q0 and t):
