@@ -473,7 +473,7 @@ def test_kv4_attention_strides_streams_batches_and_graphs(cuda):
     x = torch.randn(n, 2 * Hkv, D, generator=g).to(BF16).to(cuda)
     rows, pos = (_i32(np.concatenate(y), cuda) for y in zip(*[([r] * t, np.arange(p, p + t)) for (r, p, t) in blocks]))
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with torch.inference_mode(), torch.cuda.graph(graph):  # (as the engine captures: the generator state is shared)
         lsk.kv4_append(x[:, :Hkv], x[:, Hkv:], cache, rows, pos)
         lsk.kv4_attn(q, cache, plan, out=out, workspace=ws)
     for i in range(4):
@@ -657,7 +657,7 @@ def test_qk_norm_rope_of_prompts_and_in_graphs(cuda):
     q, kc, vc = fresh()
     graph = torch.cuda.CUDAGraph()
     lsk.qk_norm_rope_append(x, q, kc, vc, *tabs, r_t, p_t, Hq, Hkv, D)
-    with torch.cuda.graph(graph):
+    with torch.inference_mode(), torch.cuda.graph(graph):  # (as the engine captures: the generator state is shared)
         lsk.qk_norm_rope_append(x, q, kc, vc, *tabs, r_t, p_t, Hq, Hkv, D)
     for i in range(3):
         x.normal_(generator=torch.Generator(device=cuda).manual_seed(i))
@@ -839,7 +839,7 @@ def test_gemm_i8_in_graphs_and_on_streams(cuda):
     a = lsk.quant_rows_i8(x)
     out = lsk.gemm_i8(a, w, epilogue=lsk.EPI_SILU_MUL)
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with torch.inference_mode(), torch.cuda.graph(graph):  # (as the engine captures: the generator state is shared)
         lsk.gemm_i8(lsk.quant_rows_i8(x, out=a), w, out=out, epilogue=lsk.EPI_SILU_MUL)
     side = torch.cuda.Stream()
     for i in range(3):
