@@ -1,7 +1,8 @@
 // 8-bit integer projections: activations quantised row by row, weights output channel by output channel, multiplied by
 // the integer matrix instructions.
 //
-//   a row of x [M, K]: amax = max |x|, r = fl(127 / amax), s = fl(amax / 127), code = rne(x r), -127 .. 127;
+//   a row of x [M, K]: amax = max |x|, r = fl(127 fl(1 / amax)), s = fl(amax / 127), code = rne(x r), -127 .. 127
+//   (r as an array program computes 127 / amax: a reciprocal, then a product);
 //   C[m][n] = epilogue(s_m sw_n sum_k code_m[k] codew_n[k])
 //
 // x r is rounded once, to an integer (fma with 1.5 * 2^23), so codes do not depend on how the product would round in
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(QUANT_THREADS) void quant_rows_kernel(const T* __re
   for (int w = 0; w < QUANT_THREADS / 64; ++w) top = max(top, s_m[w]);
   const float amax = __uint_as_float(top);
   const bool finite = top < 0x7f800000u, some = finite && amax >= 0x1p-100f;
-  const float r = some ? 127.f / amax : 0.f;
+  const float r = some ? 127.f * (1.f / amax) : 0.f;
   if (threadIdx.x == 0) scales[m] = !finite ? __builtin_nanf("") : some ? amax / 127.f : 0.f;
   uint8_t* to = codes + (long)(m >> 4) * nks * 1024 + (m & 15) * 16;
   auto put = [&](const Raw16<T>& q, int c) {

@@ -397,8 +397,8 @@ int lsk_qk_norm_rope(int dtype, const void* qkv, long ld, const void* w_q, const
                      void* vcache, int max_batch, int max_seq, void* stream);
 
 /* ---- 8-bit integer projections (the reference multiplies in the model's dtype) ----
- * A row x of K values (a token's activations, an output channel's weights): amax = max |x|, codes rne(x fl(127 / amax)),
- * scale fl(amax / 127); a row that holds a NaN or an infinity has the scale NaN, one with amax < 2^-100 the scale 0.
+ * A row x of K values (a token's activations, an output channel's weights): amax = max |x|, codes
+ * rne(x fl(127 fl(1 / amax))), scale fl(amax / 127); a row that holds a NaN or an infinity has the scale NaN, one with amax < 2^-100 the scale 0.
  * Packed codes of R rows: (R+15)/16 * (K+63)/64 fragments of 1 KiB at a multiple of 16 bytes; lane 16 lg + l16 of
  * fragment (g, j) = row 16 g + l16, k = 64 j + 16 lg .. + 15; fragments ordered [g][j].  K <= 131072.
  *

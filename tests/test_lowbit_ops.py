@@ -675,11 +675,11 @@ def test_qk_norm_rope_of_prompts_and_in_graphs(cuda):
 # ----------------------------------------------------------------------------- 8-bit integer projections
 
 def rows8(x):
-    """(codes, scales) of the definition, 64 bits with its two fp32 roundings."""
+    """(codes, scales) of the definition, 64 bits with its three fp32 roundings."""
     amax = x.float().abs().amax(1)
     ok = torch.isfinite(amax) & (amax >= 2.0 ** -100)
     safe = torch.where(ok, amax, torch.ones_like(amax))
-    r, s = torch.full_like(safe, 127.0) / safe, safe / 127.0          # fp32 (a number over a tensor is rounded twice)
+    r, s = (torch.ones_like(safe) / safe) * 127.0, safe / 127.0       # fp32
     codes = torch.where(ok[:, None], torch.round(x.double().nan_to_num(0, 0, 0) * r.double()[:, None]), 0.0)
     s = torch.where(ok, s, torch.where(torch.isfinite(amax), 0.0, math.nan))
     return codes, s
