@@ -8,9 +8,10 @@
 //
 //   out = sum_p w_p v_p / sum_p w_p,   w_p = exp2(s_p - max s),   s_p = scale log2(e) (q . k_p)
 //
-// Work items, their records and the splits of long contexts are lsk_cache_attn_plan's (below).  Two kernels walk them:
-// cache_attn_kernel, whose waves share the positions of up to two row groups of 32 rows, and cache_tree_kernel for
-// trees of more rows, whose waves share K and V.
+// Work items, their records and the splits of long contexts are lsk_cache_attn_plan's (below).  cache_attn_kernel walks
+// them, its waves sharing the positions of up to two row groups of 32 rows; cache_tree_kernel those of more rows (trees,
+// and pieces of prompts over a 4-bit cache), its waves sharing K and V; over a 4-bit cache of 128 dims the latter is
+// cache_tree4_kernel, and one launch takes both kinds of item (cache_both4_kernel).
 //
 // The cache formats are read as 1 KiB fragments in lane order, 64 D (4-bit: 32 D) bytes per block of STEP positions:
 //   bf16   STEP = 32: K fragment (a, f), lane 16 lg + l16: position 8 (l16 / 4) + 4 a + l16 % 4,
@@ -18,13 +19,14 @@
 //   8-bit  STEP = 64: e4m3 codes; K fragment (a, j): position 16 (l16 / 4) + 4 a + l16 % 4, d = 64 j + 16 lg .. + 15
 //          (two MFMA operands of 8 d each); V^T: row d, positions 16 lg .. + 15 (two operands of 8 positions each).
 //          A position's K and V are its codes times 2^(ks - 127) and 2^(vs - 127).
-//   4-bit  STEP = 64: e2m1 codes, a scale per 32 dims; the same positions, lane group lg of K with d = D / 4 lg .. + D / 4 -
-//          1 (D / 32 operands of 8 d each); V^T: rows d = 32 c + l16 and 32 c + 16 + l16, positions 16 lg .. + 15 of each.
+//   4-bit  STEP = 64: e2m1 codes, a scale per 32 dims; the same positions, lane group lg of K with the D / 4 dims from
+//          d = D / 4 lg (D / 32 operands of 8 d each); V^T: rows d = 32 c + l16 and 32 c + 16 + l16, positions
+//          16 lg .. + 15 of each.
 // Per step of a wave (v_mfma_f32_16x16x32_bf16): S^T[pos][q] = K Q^T, whose rows are mapped to positions so that lane
 // group lg ends up with the consecutive positions its V^T load needs; online softmax with fp32 statistics; O^T[d][q] +=
 // V^T P^T.  e4m3 values times a power of two are bf16 values, so the conversions in registers are exact and K's scale
 // costs nothing (the conversion takes one); V's scale, which differs per position, multiplies the weights (4-bit: once
-// for every 32 dims).  The weights
+// for every 32 dims, or V itself).  Over a 4-bit cache of 128 dims K is an operand as it is (scores4).  The weights
 // are rounded to bf16 for the second product, as the ragged attention's are (by at most 2^-8 each, independent of one
 // another: with the bf16 output's rounding the error against 64 bits is 0.0021 to 0.0023 of the outputs' size, where
 // fp32 weights leave 0.0017); the sum of the weights is taken before that rounding.
@@ -229,11 +231,12 @@ __device__ __forceinline__ void add_odd(const CacheAttnArgs& A, const Stripe& st
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         ORDER();
-        // V[kp][16 c + 4 lg + i]: a dim's slots of a block are 64 bytes in bf16 and in 8 bits; in 4 bits NaN is a scale's
+        // V[kp][16 c + 4 lg + i]: a dim's slots of a block are 64 bytes in bf16 and 8 bits; in 4 bits NaN is a scale's
         const int so = kp / STEP * 64 * D + (16 * c + i) * 64 + kp % STEP * (FMT == FMT_KV8 ? 1 : 2);
         float x;
         if constexpr (FMT == FMT_KV4) {
-          const uint32_t b = __builtin_amdgcn_raw_buffer_load_b8(st.vs, 0, (kp / 64 * (D / 32) + c / 2) * 64 + kp % 64, 0);
+          const int at = (kp / 64 * (D / 32) + c / 2) * 64 + kp % 64;
+          const uint32_t b = __builtin_amdgcn_raw_buffer_load_b8(st.vs, 0, at, 0);
           x = b == 255u ? __builtin_nanf("") : 0.f;
         } else if constexpr (FMT == FMT_KV8) {
           const uint32_t b = __builtin_amdgcn_raw_buffer_load_b8(st.v, 256 * lg, so, 0);
@@ -499,7 +502,8 @@ __device__ __forceinline__ void cache_attn_items(const CacheAttnArgs& A, AttnLds
     }
     if constexpr (KV4) {                             // (a byte of the dword for each tile)
       if (a == 2 * HV - 1)
-        ksr[0] = __builtin_amdgcn_raw_buffer_load_b32(s.ks, 64 * (D == 128 ? lg : lg >> 1) + 4 * l16, sb * (D / 32), AUX);
+        ksr[0] = __builtin_amdgcn_raw_buffer_load_b32(s.ks, 64 * (D == 128 ? lg : lg >> 1) + 4 * l16, sb * (D / 32),
+                                                      AUX);
     }
   };
   auto load_v = [&](const Stripe& s, int sb, int c) { vr[c] = ld(s.v, v_vo, sb / STEP * BLK + c * 1024); };
@@ -900,7 +904,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree_kernel(const Ca
             const int g = 4 * u + w, a = g / KF;
             *(lsk_bf16x8*)(to + (a >> 1) * HALF + ((a & 1) * KF + g % KF) * 1024) =
                 codes4_to_bf16(x, exp_byte((uint32_t)st_s[i][0], a));
-          } else {                                   // rows 32 (u - LT) + 16 (w / 2) + l16, positions 16 lg + 8 (w % 2) ..
+          } else {                                   // rows 32 (u - LT) + 16 (w / 2) + l16, positions from 16 lg + 8 (w % 2)
             *(lsk_bf16x8*)(to + (w & 1) * HALF + (CT + 2 * (u - LT) + (w >> 1)) * 1024) =
                 codes4_to_bf16(x, st_s[i], w & 1);
           }
@@ -1078,7 +1082,7 @@ __device__ __forceinline__ void cache_tree4_item(const CacheAttnArgs& A, const i
     v = ld(sr.v, 16 * lane, sb / 2 * D + wave * 1024);
     vs = ld(sr.vs, 16 * lg, sb * (D / 32) + 64 * wave);
   };
-  auto write_v = [&](int buf) {                      // rows 32 wave + 16 (w / 2) + l16, positions 16 lg + 8 (w % 2) ..
+  auto write_v = [&](int buf) {                      // rows 32 wave + 16 (w / 2) + l16, positions from 16 lg + 8 (w % 2)
     char* to = s_v + buf * BUF + 16 * lane + 2 * wave * 1024;
 #pragma unroll
     for (int w = 0; w < 4; ++w)
@@ -1403,22 +1407,23 @@ __global__ __launch_bounds__(64 * F32_ROWS) void tree_attn_f32_kernel(
 //           blocks of more than 64 rows count as MANY_TILES tiles (8B heads, 300 to 900 positions, tiles for all / these
 //           items: 64 stripes, 10 to 40 nodes 17 / 21 us, 96 stripes, 10 to 64 nodes 30 / 23, 128 stripes, 20 to 64
 //           nodes 34 / 24).
-//   wide    a block of more than 64 rows (128 dims: 48) without a mask over a 4-bit cache (a piece of a prompt), where
-//           the cache's stripes times the block's tiles of 32 rows are more than WIDE_TILES: items of 128 rows for the tree kernels,
-//           whose waves share the conversions of K and V (8B heads after 1000 positions, wide / not, unsplit: 256 stripes
-//           of 64 tokens 52 / 83 us, 64 stripes of 256 54 / 88; 1024 tiles, 64 stripes of 128, 36 / 45; behind at 512: 8
-//           of 512 tokens 29 / 26; 17 tokens in 256 stripes 39 / 38; 1B heads: 64 stripes of 128 tokens 37 / 32, of 256
-//           44 / 60; 8B heads, 64 requests of 16 tokens 34 / 45).  Over 128 dims items are of 64 rows, one query tile a wave,
-//           where the launch has at most HALF_ITEMS of 128, one for each CU, since it is bound by the longest item, and two
-//           workgroups' products and softmax overlap (251 items, one of 1001 tokens: 53 -> 44 us; 376, one of 1500: 69 ->
-//           80), and where items of 128 would be less than two thirds full; a row's bits are the same.
-//           The cache full of such blocks has 192 items of 128 rows and more, so its splits are of WIDE_SPLIT positions
-//           at least (8 stripes, a prompt of 4001 tokens: 640 positions 218 us, 1280 174, 2560 155, whole 142; the other
-//           way round for one short piece in a large cache: 256 tokens after 5000 whole 107, 2560 63).
-//   pairs   a block that is not wide, over a 4-bit cache of 128 dims, whose rows make fewer items of PAIR_ROWS than of 32,
-//           where the stripes times the tiles of 32 rows are more than PAIR_TILES: items of two row groups of two waves (8B
-//           heads after 1000 positions, pairs / not: 64 requests of 9 tokens 32 / 48 us, of 12 33 / 46, 128 of 9 62 / 93;
-//           32 of 9, 512 tiles, 25 / 24; 64 of 16, 48 + 16 rows or 32 + 32, 61 / 48).
+//   wide    a block of more than 64 rows (128 dims: 48) without a mask over a 4-bit cache (a piece of a prompt),
+//           where the cache's stripes times the block's tiles of 32 rows are more than WIDE_TILES: items of 128 rows
+//           for the tree kernels, whose waves share the conversions of K and V (8B heads after 1000 positions, wide
+//           / not, unsplit: 256 stripes of 64 tokens 52 / 83 us, 64 stripes of 256 54 / 88; 1024 tiles, 64 stripes
+//           of 128, 36 / 45; behind at 512: 8 of 512 tokens 29 / 26; 17 tokens in 256 stripes 39 / 38; 1B heads: 64
+//           stripes of 128 tokens 37 / 32, of 256 44 / 60; 8B heads, 64 requests of 16 tokens 34 / 45).  Over 128
+//           dims items are of 64 rows, one query tile a wave, where the launch has at most HALF_ITEMS of 128, one
+//           for each CU, since it is bound by the longest item, and two workgroups' products and softmax overlap
+//           (251 items, one of 1001 tokens: 53 -> 44 us; 376, one of 1500: 69 -> 80), and where items of 128 would
+//           be less than two thirds full; a row's bits are the same. The cache full of such blocks has 192 items of
+//           128 rows and more, so its splits are of WIDE_SPLIT positions at least (8 stripes, a prompt of 4001
+//           tokens: 640 positions 218 us, 1280 174, 2560 155, whole 142; the other way round for one short piece in
+//           a large cache: 256 tokens after 5000 whole 107, 2560 63).
+//   pairs   a block that is not wide, over a 4-bit cache of 128 dims, whose rows make fewer items of PAIR_ROWS than
+//           of 32, where the stripes times the tiles of 32 rows are more than PAIR_TILES: items of two row groups of
+//           two waves (8B heads after 1000 positions, pairs / not: 64 requests of 9 tokens 32 / 48 us, of 12 33 /
+//           46, 128 of 9 62 / 93; 32 of 9, 512 tiles, 25 / 24; 64 of 16, 48 + 16 rows or 32 + 32, 61 / 48).
 // The number of row groups follows from the block's rows and the cache alone, so it never makes a row's result depend
 // on the batch.  Items go longest first to the least-loaded of n_slots persistent workgroups, as in lsk_attn_schedule.
 #define WIDE_TILES(D) ((D) == 64 ? 1280 : 768)

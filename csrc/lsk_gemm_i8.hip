@@ -99,7 +99,7 @@ __device__ __forceinline__ void store_out(float* c, const float* r, float* o, in
 #define QUANT_THREADS 256
 // A workgroup a row: the largest magnitude, then the codes.  NC: 16-value pieces of a thread, held in registers between
 // the two (0: longer rows, read again).  The 16 rows of a fragment go to one XCD, whose L2 puts their 16-byte stores
-// together.
+// together.  Bound by HBM: 2001 bf16 rows of 14336 22 us (86 MB read and written, 4.0 TB/s); one row of 2048 2.4.
 template <typename T, int NC>
 __global__ __launch_bounds__(QUANT_THREADS) void quant_rows_kernel(const T* __restrict__ x, long ldx,
                                                                    uint8_t* __restrict__ codes,
@@ -180,7 +180,8 @@ __global__ __launch_bounds__(256) void pack_i8_kernel(const int8_t* __restrict__
 
 // Few tokens: a workgroup of four waves owns 16 NS weight rows (silu-mul: of gate and of up) x 16 MS tokens; the waves
 // take the k-steps round robin, U at a time with the next U in flight, both operands straight from memory as fragments,
-// and add their sums up in LDS (integers: in any order).
+// and add their sums up in LDS (integers: in any order).  Bound by the weights' bytes: 32 tokens of the 8B shape's gate and
+// up projection 22 us (117 MB, 5.3 TB/s); one token of the 1B shape's o projection (4 MB) 4.3.
 template <int NS, int MS, int EPI, typename T>
 __global__ __launch_bounds__(256) void gemm_i8_kernel(const uint8_t* __restrict__ A, const float* __restrict__ sa,
                                                       const uint8_t* __restrict__ W, const float* __restrict__ sw,
@@ -268,7 +269,8 @@ __global__ __launch_bounds__(256) void gemm_i8_kernel(const uint8_t* __restrict_
 
 // Many tokens: a workgroup of four waves owns 256 weight rows (silu-mul: 128 of gate and of up), 64 a wave, read straight
 // into registers three k-steps ahead (no other wave needs them), x MG 16-token groups, staged through LDS half a chunk of
-// four k-steps at a time and shared by the waves.  KP > 1: that many such sets of four waves share the k-steps.
+// four k-steps at a time and shared by the waves.  KP > 1: that many such sets of four waves share the k-steps.  Bound by
+// the matrix instructions at the clock that they leave: 2001 tokens of the 8B shape's w2 110 us, 2.1 POP/s.
 template <int NG, int MG, int KP, int EPI, typename T>
 __global__ __launch_bounds__(256 * KP, NG * MG == 32 || KP > 1 ? 1 : 2) void gemm_i8_deep_kernel(
     const uint8_t* __restrict__ A, const float* __restrict__ sa, const uint8_t* __restrict__ W,

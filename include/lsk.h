@@ -398,7 +398,8 @@ int lsk_qk_norm_rope(int dtype, const void* qkv, long ld, const void* w_q, const
 
 /* ---- 8-bit integer projections (the reference multiplies in the model's dtype) ----
  * A row x of K values (a token's activations, an output channel's weights): amax = max |x|, codes
- * rne(x fl(127 fl(1 / amax))), scale fl(amax / 127); a row that holds a NaN or an infinity has the scale NaN, one with amax < 2^-100 the scale 0.
+ * rne(x fl(127 fl(1 / amax))), scale fl(amax / 127); a row that holds a NaN or an infinity has the scale NaN, one with
+ * amax < 2^-100 the scale 0.
  * Packed codes of R rows: (R+15)/16 * (K+63)/64 fragments of 1 KiB at a multiple of 16 bytes; lane 16 lg + l16 of
  * fragment (g, j) = row 16 g + l16, k = 64 j + 16 lg .. + 15; fragments ordered [g][j].  K <= 131072.
  *
@@ -433,8 +434,8 @@ int lsk_gemm_i8(int dtype, const void* A, const float* a_scales, const void* W, 
  *
  * lsk_kv_compact: slot pos0[b] + j of cache row rows[b] takes what slot pos0[b] + path[b][j] holds, j = 1 ..
  * accepted[b] (negative: none), in every layer and KV head (caches [n_layers, max_batch, ...], contiguous; k_exp, v_exp
- * for LSK_DTYPE_KV8 and LSK_DTYPE_KV4, else NULL); then lsk_kv_rollback's pointer update holds as for a chain.  path as lsk_tree_accept
- * writes it (increasing); the rows of a call have to differ.  Blocks outside the cache are skipped.  V's neighbouring
+ * for LSK_DTYPE_KV8 and LSK_DTYPE_KV4, else NULL); then lsk_kv_rollback's pointer update holds as for a chain.  path as
+ * lsk_tree_accept writes it (increasing); the rows of a call have to differ.  Blocks outside the cache are skipped.  V's neighbouring
  * slots of a moved one (16 bytes) are written back as they were. */
 int lsk_tree_masks(const int32_t* parents, const int32_t* starts, const int32_t* lens, int nb, int n_tokens,
                    int max_nodes, uint32_t* mask, int mask_words, int32_t* depth, void* stream);
