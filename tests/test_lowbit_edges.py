@@ -1,0 +1,55 @@
+"""The low-precision operators at the edges of what a caller may hand them: rows closer together than their length,
+buffers that do not fit, plans of another kind.  Refusals run on the CPU: the wrappers' launches are caught there."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from test_cache_ops import BF16, F32, _lsk
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The wrappers on CPU tensors: the launches [(entry point, its arguments)] that they would make."""
+    lsk, made = _lsk(), []
+    monkeypatch.setattr(lsk, "_dev", lambda *ts: None)
+    monkeypatch.setattr(lsk, "_one_device", lambda *ts: 0)
+    monkeypatch.setattr(lsk, "_launch", lambda dev, what, *args: made.append((what, args)))
+    return made
+
+
+def _refused(launches, f):
+    lsk = _lsk()
+    launches.clear()
+    with pytest.raises(lsk.LskError):
+        f()
+    assert not [what for what, _ in launches if what != "lsk_pack_i8"]
+
+
+def _overlapping(m, n, pitch, dtype=BF16):
+    """[m, n] with rows `pitch` < n elements apart."""
+    return torch.zeros((m - 1) * pitch + n, dtype=dtype).as_strided((m, n), (pitch, 1))
+
+
+# ----------------------------------------------------------------------------- rows closer together than their length
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gemm_i8_takes_the_pitch_of_out_and_residual_as_it_is(launches, dtype):
+    lsk = _lsk()
+    M, N, K = 5, 32, 64
+    w = lsk.PackedWeightI8(torch.zeros(N, K, dtype=torch.int8), torch.ones(N))
+    a = lsk.quant_rows_i8(torch.zeros(M, K, dtype=dtype))
+    bias = torch.zeros(N, dtype=dtype)
+    for r in (bias.expand(M, N), _overlapping(M, N, 8, dtype), _overlapping(M, N, N - 1, dtype)):
+        _refused(launches, lambda: lsk.gemm_i8(a, w, residual=r, epilogue=lsk.EPI_RESIDUAL))
+        _refused(launches, lambda: lsk.gemm_i8(a, w, out=r))
+    launches.clear()
+    out, res = torch.zeros(M, N + 3, dtype=dtype)[:, :N], torch.zeros(2 * M, N, dtype=dtype)[::2]
+    lsk.gemm_i8(a, w, out=out, residual=res, epilogue=lsk.EPI_RESIDUAL)
+    one = lsk.quant_rows_i8(torch.zeros(1, K, dtype=dtype))           # (the pitch of a single row means nothing)
+    lsk.gemm_i8(one, w, out=bias.as_strided((1, N), (3, 1)), residual=bias.expand(1, N), epilogue=lsk.EPI_RESIDUAL)
+    (_, args), (_, single) = (x for x in launches if x[0] == "lsk_gemm_i8")
+    assert args[6] == N + 3 and args[8] == 2 * N                      # ldc, ldr
+    assert single[6] >= N and single[8] >= N

@@ -583,6 +583,14 @@ def _want(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tupl
                        f"{t.dtype}{'' if t.is_contiguous() else ', not contiguous'}")
 
 
+def _row_pitch(what: str, name: str, t: torch.Tensor, width: int) -> int:
+    """Elements between the rows of a 2-D tensor whose stride(0) is below its `width` columns: the width for a single row,
+    whose stride means nothing; LskError where rows share memory (an expanded row, say)."""
+    if t.shape[0] > 1:
+        raise LskError(f"{what}: the rows of {name} are {t.stride(0)} elements apart and {width} long")
+    return width
+
+
 _E4M3 = torch.float8_e4m3fn
 
 
@@ -1259,10 +1267,12 @@ def gemm_i8(a: RowsI8, w: PackedWeightI8, out: torch.Tensor | None = None, resid
             if t.shape != (M, N) or t.dtype is not dtype or (one != 1 and t.numel()):
                 raise LskError(f"gemm_i8: out and residual must be {[M, N]} {dtype} with contiguous rows, got "
                                f"{list(t.shape)} {t.dtype}")
+            if ld < N:
+                ld = _row_pitch("gemm_i8", "out" if t is out else "residual", t, N)
             if t is out:
-                ldc = max(ld, N)
+                ldc = ld
             else:
-                ldr = max(ld, N)
+                ldr = ld
     if M:
         codes = a.data.data_ptr()
         _launch(dev, "lsk_gemm_i8", dtype_code(dtype), codes, codes + a.offset, w.data.data_ptr(), w.scales.data_ptr(),
