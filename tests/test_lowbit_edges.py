@@ -53,3 +53,31 @@ def test_gemm_i8_takes_the_pitch_of_out_and_residual_as_it_is(launches, dtype):
     (_, args), (_, single) = (x for x in launches if x[0] == "lsk_gemm_i8")
     assert args[6] == N + 3 and args[8] == 2 * N                      # ldc, ldr
     assert single[6] >= N and single[8] >= N
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_quant_rows_i8_takes_the_pitch_of_the_rows_as_it_is(launches, dtype):
+    lsk = _lsk()
+    K = 64
+    row = torch.zeros(K, dtype=dtype)
+    for x in (row.expand(5, K), _overlapping(5, K, 8, dtype), _overlapping(5, K, K - 1, dtype)):
+        _refused(launches, lambda: lsk.quant_rows_i8(x))
+        _refused(launches, lambda: lsk.PackedWeightI8(x))
+    launches.clear()
+    lsk.quant_rows_i8(torch.zeros(5, K + 7, dtype=dtype)[:, 3:K + 3])
+    lsk.PackedWeightI8(torch.zeros(10, K, dtype=dtype)[::2])
+    lsk.quant_rows_i8(row.as_strided((1, K), (1, 1)))
+    assert [args[2] for _, args in launches] == [K + 7, 2 * K, K]
+
+
+def test_packed_weights_take_the_pitch_of_the_codes_as_it_is(launches):
+    lsk = _lsk()
+    N, K = 6, 64
+    for w in (torch.zeros(K, dtype=torch.int8).expand(N, K), _overlapping(N, K, 16, torch.int8)):
+        launches.clear()
+        with pytest.raises(lsk.LskError):
+            lsk.PackedWeightI8(w, torch.ones(N))
+        assert not launches
+    lsk.PackedWeightI8(torch.zeros(N, K + 5, dtype=torch.int8)[:, :K], torch.ones(N))
+    lsk.PackedWeightI8(torch.zeros(K, dtype=torch.int8).expand(1, K), torch.ones(1))
+    assert [args[1] for _, args in launches] == [K + 5, K]

@@ -1193,7 +1193,9 @@ def quant_rows_i8(x: torch.Tensor, out: RowsI8 | None = None) -> RowsI8:
     if len(shape) != 2 or (x.stride(1) != 1 and x.numel()):
         raise LskError(f"quant_rows_i8: a 2-D tensor with contiguous rows is needed, got {list(shape)}")
     M, K = shape
-    code = dtype_code(dtype)
+    code, ld = dtype_code(dtype), x.stride(0)
+    if ld < K:
+        ld = _row_pitch("quant_rows_i8", "x", x, K)
     if out is None:
         out = RowsI8(x.new_empty(_i8_bytes(M, K) + 4 * M, dtype=torch.int8), (M, K), dtype)
         dev = x.get_device()
@@ -1205,7 +1207,7 @@ def quant_rows_i8(x: torch.Tensor, out: RowsI8 | None = None) -> RowsI8:
         dev = _one_device(x, out.data)
     if M:
         codes = out.data.data_ptr()
-        _launch(dev, "lsk_quant_rows_i8", code, x.data_ptr(), max(x.stride(0), K), codes, codes + out.offset, M, K)
+        _launch(dev, "lsk_quant_rows_i8", code, x.data_ptr(), ld, codes, codes + out.offset, M, K)
     return out
 
 
@@ -1219,13 +1221,14 @@ class PackedWeightI8:
             raise LskError(f"PackedWeightI8: a 2-D tensor with contiguous rows is needed, got {list(w.shape)}")
         N, K = self.shape = tuple(w.shape)
         self.device = w.device
+        ld = w.stride(0) if w.stride(0) >= K else _row_pitch("PackedWeightI8", "the weight", w, K)
         if w.dtype == torch.int8:
             if scales is None:
                 raise LskError("PackedWeightI8: codes without scales")
             _want("PackedWeightI8", "scales", scales, torch.float32, (N,))
             dev = _one_device(w, scales)
             self.data, self.scales = w.new_empty(_i8_bytes(N, K)), scales.clone()
-            _launch(dev, "lsk_pack_i8", w.data_ptr(), max(w.stride(0), K), self.data.data_ptr(), N, K)
+            _launch(dev, "lsk_pack_i8", w.data_ptr(), ld, self.data.data_ptr(), N, K)
         else:
             if scales is not None:
                 raise LskError("PackedWeightI8: scales belong to int8 codes")
