@@ -81,3 +81,30 @@ def test_packed_weights_take_the_pitch_of_the_codes_as_it_is(launches):
     lsk.PackedWeightI8(torch.zeros(N, K + 5, dtype=torch.int8)[:, :K], torch.ones(N))
     lsk.PackedWeightI8(torch.zeros(K, dtype=torch.int8).expand(1, K), torch.ones(1))
     assert [args[1] for _, args in launches] == [K + 5, K]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_qk_norm_rope_takes_the_pitch_of_the_rows_as_it_is(launches, dtype):
+    lsk = _lsk()
+    n, Hq, Hkv, D, S = 5, 4, 2, 32, 64
+    W = (Hq + 2 * Hkv) * D
+    w, tab = torch.ones(D, dtype=dtype), torch.zeros(S, D)
+    kc = torch.zeros(1, Hkv, S // 32, D // 16, 64, 8, dtype=dtype) if dtype == BF16 else torch.zeros(1, Hkv, S, D)
+    vc = torch.zeros(1, Hkv, S // 32, D, 32, dtype=dtype)
+
+    def both(qkv):
+        m = len(qkv)
+        i = torch.zeros(m, dtype=torch.int32)
+        return (lambda: lsk.qk_norm_rope(qkv, w, w, 1e-5, tab, tab, i, Hq, Hkv, D),
+                lambda: lsk.qk_norm_rope_append(qkv, torch.zeros(m, Hq, D, dtype=dtype), kc, vc, w, w, 1e-5, tab, tab, i, i,
+                                                Hq, Hkv, D))
+
+    for qkv in (torch.zeros(W, dtype=dtype).expand(n, W), _overlapping(n, W, D, dtype), _overlapping(n, W, W - 1, dtype)):
+        for f in both(qkv):
+            _refused(launches, f)
+    launches.clear()
+    for qkv in (torch.zeros(n, W + 9, dtype=dtype)[:, :W], torch.zeros(3 * n, W, dtype=dtype)[::3],
+                torch.zeros(W, dtype=dtype).expand(1, W)):
+        for f in both(qkv):
+            f()
+    assert [args[2] for _, args in launches] == [W + 9] * 2 + [3 * W] * 2 + [W] * 2

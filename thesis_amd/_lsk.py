@@ -1123,7 +1123,8 @@ def _norm_rope(name: str, qkv, w_q, w_k, eps, cos_tab, sin_tab, pos_i32, n_heads
         _want(name, "pos", pos_i32, torch.int32, (n,))
         _want(name, "q_out", q_out, dtype, (n, n_heads, head_dim))
     if n:
-        _launch(dev, "lsk_qk_norm_rope", code, qkv.data_ptr(), max(strides[0], width), w_q.data_ptr(), w_k.data_ptr(),
+        ld = strides[0] if strides[0] >= width else _row_pitch(name, "qkv", qkv, width)
+        _launch(dev, "lsk_qk_norm_rope", code, qkv.data_ptr(), ld, w_q.data_ptr(), w_k.data_ptr(),
                 float(eps), cos_tab.data_ptr(), sin_tab.data_ptr(), table[0], _ptr(rows_i32), pos_i32.data_ptr(), n,
                 n_heads, n_kv_heads, head_dim, q_out.data_ptr(), _ptr(k_out), _ptr(kcache), _ptr(vcache), max_batch,
                 max_seq)
