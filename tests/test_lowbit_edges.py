@@ -108,3 +108,32 @@ def test_qk_norm_rope_takes_the_pitch_of_the_rows_as_it_is(launches, dtype):
         for f in both(qkv):
             f()
     assert [args[2] for _, args in launches] == [W + 9] * 2 + [3 * W] * 2 + [W] * 2
+
+
+# ----------------------------------------------------------------------------- buffers of quantised rows
+
+def test_rows_i8_refuse_buffers_that_do_not_hold_them():
+    """The kernel writes codes and scales behind them: (M + 15) / 16 * (K + 63) / 64 KiB and 4 M bytes."""
+    lsk = _lsk()
+    M, K = 17, 100
+    need = 2 * 2 * 1024 + 4 * M
+    new = lambda n, dtype=torch.int8: torch.zeros(n, dtype=dtype)     # noqa: E731
+    for n in (need, need + 5):
+        rows = lsk.RowsI8(new(n), (M, K), BF16)
+        assert rows.codes.numel() == need - 4 * M and rows.scales.shape == (M,)
+    lsk.RowsI8(new(0), (0, K), F32)
+    for data, shape, dtype in ((new(need - 1), (M, K), BF16), (new(16), (1, 2097152), BF16), (new(0), (1, 1), F32),
+                               (new(need, torch.float32), (M, K), BF16), (new(2 * need)[::2], (M, K), BF16),
+                               (new(1).expand(need), (M, K), BF16), (new(need).view(1, need), (M, K), BF16),
+                               (new(need), (M, K), torch.float16), (new(need), (M,), BF16), (new(need), (-1, K), BF16),
+                               (new(need), (M, 0), BF16), (new(need + 1)[1:], (M, K), BF16)):
+        with pytest.raises(lsk.LskError):
+            lsk.RowsI8(data, shape, dtype)
+
+
+def test_quantised_rows_given_again_have_to_be_of_the_same_shape(launches):
+    lsk = _lsk()
+    a = lsk.quant_rows_i8(torch.zeros(3, 64, dtype=BF16))
+    assert lsk.quant_rows_i8(torch.ones(3, 64, dtype=BF16), out=a) is a
+    for x in (torch.zeros(4, 64, dtype=BF16), torch.zeros(3, 65, dtype=BF16), torch.zeros(3, 64)):
+        _refused(launches, lambda: lsk.quant_rows_i8(x, out=a))

@@ -1172,11 +1172,24 @@ def _i8_bytes(rows: int, k: int) -> int:
 
 class RowsI8:
     """Activations [M, K] as 8-bit integers with a scale per row (quant_rows_i8), in the matrix instructions' order: data
-    holds the codes and, behind them, the fp32 scales."""
+    holds the codes and, behind them, the fp32 scales: a contiguous int8 vector at a multiple of 16 bytes, of
+    (M + 15) // 16 * ((K + 63) // 64) * 1024 + 4 M bytes or more.  dtype: the activations', and the products'."""
     __slots__ = ("data", "offset", "shape", "dtype")
 
     def __init__(self, data: torch.Tensor, shape: tuple, dtype: torch.dtype):
+        if len(shape) != 2 or shape[0] < 0 or shape[1] < (shape[0] > 0):
+            raise LskError(f"RowsI8: a shape (rows, columns) is needed, got {tuple(shape)}")
+        dtype_code(dtype)
+        self._set(data, tuple(shape), dtype)
+        need = self.offset + 4 * shape[0]
+        if data.dtype is not torch.int8 or data.dim() != 1 or not data.is_contiguous() or data.numel() < need or \
+                data.data_ptr() % 16:
+            raise LskError(f"RowsI8: {list(shape)} need a contiguous int8 vector of {need} bytes at a multiple of 16, got "
+                           f"{list(data.shape)} {data.dtype}")
+
+    def _set(self, data: torch.Tensor, shape: tuple, dtype: torch.dtype) -> "RowsI8":
         self.data, self.offset, self.shape, self.dtype = data, _i8_bytes(*shape), shape, dtype
+        return self
 
     @property
     def codes(self) -> torch.Tensor:
@@ -1184,7 +1197,7 @@ class RowsI8:
 
     @property
     def scales(self) -> torch.Tensor:
-        return self.data[self.offset:].view(torch.float32)
+        return self.data[self.offset:self.offset + 4 * self.shape[0]].view(torch.float32)
 
 
 def quant_rows_i8(x: torch.Tensor, out: RowsI8 | None = None) -> RowsI8:
@@ -1198,7 +1211,7 @@ def quant_rows_i8(x: torch.Tensor, out: RowsI8 | None = None) -> RowsI8:
     if ld < K:
         ld = _row_pitch("quant_rows_i8", "x", x, K)
     if out is None:
-        out = RowsI8(x.new_empty(_i8_bytes(M, K) + 4 * M, dtype=torch.int8), (M, K), dtype)
+        out = RowsI8.__new__(RowsI8)._set(x.new_empty(_i8_bytes(M, K) + 4 * M, dtype=torch.int8), (M, K), dtype)
         dev = x.get_device()
         if dev < 0:
             _dev(x)
