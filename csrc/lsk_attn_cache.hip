@@ -1564,7 +1564,8 @@ static int cache_plan(const char* what, const int32_t* blocks, int nb, int group
   }
   const long len = (long)groups.size() + 8L * n_slots * rounds + 8L * (long)shared.size();
   counts[0] = n_tokens; counts[1] = (long)groups.size() / 8; counts[2] = np; counts[3] = rounds; counts[4] = tiles;
-  counts[5] = part_rows; counts[6] = len; counts[7] = used; counts[8] = (long)shared.size();
+  counts[5] = part_rows; counts[6] = len; counts[8] = (long)shared.size();
+  counts[7] = !tree && used > 1 ? used | LSK_PLAN_CAUSAL : used;
   if (meta == nullptr) return 0;
   LSK_REQUIRE(len <= meta_cap, LSK_EWORKSPACE, "%s: %ld metadata words > %ld", what, len, meta_cap);
   std::copy(groups.begin(), groups.end(), meta);
@@ -1606,8 +1607,13 @@ static int cache_attn(const char* what, int format, CacheAttnArgs a, const int32
               head_dim);
   LSK_REQUIRE(tiles == 1 || tiles == 2 || (tiles == 3 && head_dim == 64 && a.mask == nullptr), LSK_EARG,
               "%s: a plan of %d tiles", what, tiles);
-  LSK_REQUIRE((row_groups == 1 && n_shared == 0) || a.mask != nullptr ||
-                  (format == FMT_KV4 && (row_groups != 2 || head_dim == 128)), LSK_EARG,
+  // A plan of several row groups is a tree's unless it says otherwise: without a mask its items of two hold PAIR_ROWS.
+  const int n_row_groups = row_groups & ~LSK_PLAN_CAUSAL;
+  const bool causal = row_groups != n_row_groups;
+  LSK_REQUIRE((n_row_groups == 1 && !causal) || n_row_groups == 2 || n_row_groups == 4, LSK_EARG,
+              "%s: a plan of %d row groups", what, row_groups);
+  LSK_REQUIRE((n_row_groups == 1 && n_shared == 0) || a.mask != nullptr ||
+                  (causal && format == FMT_KV4 && (n_row_groups != 2 || head_dim == 128)), LSK_EARG,
               "%s: a tree's plan (%d row groups) without a mask", what, row_groups);
   LSK_REQUIRE(n_slots > 0 && n_groups >= 0 && n_parts >= 0 && (n_groups > 0) == (n_parts > 0), LSK_EARG,
               "%s: a plan of %d slots, %d groups and %d partial slots", what, n_slots, n_groups, n_parts);
@@ -1662,8 +1668,8 @@ static int cache_attn(const char* what, int format, CacheAttnArgs a, const int32
   } while (0)
     if (format == FMT_BF16) LSK_CACHE_TREE(FMT_BF16, true);
     else if (format == FMT_KV8) LSK_CACHE_TREE(FMT_KV8, true);
-    else if (head_dim == 128 && row_groups == 4 && a.mask != nullptr) LSK_CACHE_TREE4(true, 2);
-    else if (head_dim == 128 && row_groups == 4) LSK_CACHE_TREE4(false, 2);
+    else if (head_dim == 128 && n_row_groups == 4 && a.mask != nullptr) LSK_CACHE_TREE4(true, 2);
+    else if (head_dim == 128 && n_row_groups == 4) LSK_CACHE_TREE4(false, 2);
     else if (head_dim == 128 && a.mask != nullptr) LSK_CACHE_TREE4(true, 1);
     else if (head_dim == 128) LSK_CACHE_TREE4(false, 1);
     else if (a.mask != nullptr) cache_tree_kernel<64, FMT_KV4, true><<<n_shared, 64 * TREE_WAVES, 0, s>>>(a, items);

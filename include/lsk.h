@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define LSK_ABI_VERSION 15
+#define LSK_ABI_VERSION 16
 
 #define LSK_EPI_NONE 0     /* C = rnd(A W^T)                                   */
 #define LSK_EPI_RESIDUAL 1 /* C = rnd(R + rnd(A W^T))                          */
@@ -335,7 +335,10 @@ int lsk_kv8_read(int dtype, const void* k8, const void* v8, const void* k_exp, c
  * n_slots: persistent workgroups, two per CU; recs: their items, and behind them the n_shared items of four row groups
  * (a workgroup each; over a 4-bit cache of at most 64 rows where row_groups is 2).  meta = [groups int32 n_groups*8][recs
  * n_slots*n_rounds*8, then n_shared*8]; counts[9] = {tokens, n_groups, n_parts, n_rounds, tiles, part_rows, words of
- * meta, row_groups used, n_shared}.  meta == NULL: counts only; meta_cap too small: LSK_EWORKSPACE with counts written. */
+ * meta, row_groups used, n_shared}, the row groups of a plan without a mask, where they are more than one, with
+ * LSK_PLAN_CAUSAL: a launch takes them as they are, and refuses a tree's without its mask.  meta == NULL: counts only;
+ * meta_cap too small: LSK_EWORKSPACE with counts written. */
+#define LSK_PLAN_CAUSAL 8
 int lsk_cache_attn_plan(const int32_t* blocks, int nb, int group, int split, int max_batch, int n_kv_heads,
                         int head_dim, int format, int tree, int row_groups, int n_slots, int32_t* meta, long meta_cap,
                         long* counts);

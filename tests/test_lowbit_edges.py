@@ -137,3 +137,45 @@ def test_quantised_rows_given_again_have_to_be_of_the_same_shape(launches):
     assert lsk.quant_rows_i8(torch.ones(3, 64, dtype=BF16), out=a) is a
     for x in (torch.zeros(4, 64, dtype=BF16), torch.zeros(3, 65, dtype=BF16), torch.zeros(3, 64)):
         _refused(launches, lambda: lsk.quant_rows_i8(x, out=a))
+
+
+# ----------------------------------------------------------------------------- plans of another kind
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_trees_plan_over_a_4_bit_cache_needs_its_mask(D):
+    """The kernels without a mask hold fewer rows of an item of two row groups than a tree's plan gives them.  The check of
+    the workspace comes after that of the plan's kind: -4 says that the kind was taken."""
+    lsk = _lsk()
+    lib, P = lsk.load(), 16
+
+    def attn(cnt, mask, fmt=2, rg=None):
+        _, ng, parts, rounds, tiles, part_rows, _, used, shared = (int(x) for x in cnt)
+        args = (P, 512, 64, P, P, P, P, P if mask else None, 4 if mask else 0, P, ng, parts, P, rounds, 512, shared, tiles,
+                used if rg is None else rg, part_rows, P, 32, 8, D, 8192, 0.125, None, 0, None)
+        return (lib.lsk_kv4_attn if fmt == 2 else lib.lsk_kv8_attn)(*args)
+
+    def plan(t, tree, rows=8, groups=0, fmt=2, pos0=5000):
+        blk, cnt = np.array([0, pos0, t, 0], dtype=np.int32), np.zeros(9, dtype=np.int64)
+        assert lib.lsk_cache_attn_plan(blk.ctypes.data, 1, 4, 64, rows, 8, D, fmt, int(tree), groups, 512, None, 0,
+                                       cnt.ctypes.data) == 0 and cnt[2] > 0
+        return cnt
+
+    for t in (9, 12, 16, 40, 100):
+        for groups in (0, 1, 2, 4):
+            for fmt in (1, 2):
+                cnt = plan(t, True, 8, groups, fmt)
+                assert cnt[7] in (1, 2, 4) and attn(cnt, True, fmt) == -4
+                assert attn(cnt, False, fmt) == (-4 if cnt[7] == 1 else -1)
+        for rows in (8, 40, 100, 1000):               # no groups, pairs, wide blocks
+            cnt = plan(t, False, rows)
+            assert attn(cnt, False) == -4
+            assert cnt[7] == 1 and cnt[8] == 0 or cnt[7] in (8 + 2, 8 + 4)
+            if cnt[7] > 1:                            # (a tree's of as many row groups; no 8-bit plan has them)
+                assert attn(cnt, False, rg=int(cnt[7]) & 7) == -1 and attn(cnt, False, 1) == -1
+    cnt = plan(40, False, 1000)
+    assert cnt[8] > 0
+    for rg in (0, 1, 2, 3, 4, 5, 6, 8, 9, 11, 16, -2):
+        assert attn(cnt, False, rg=rg) == -1
+    one = lsk.AttnPlan([(0, 3, 40, 0)], 32, lsk.KV4(*(t.expand(1000, 8, *t.shape[2:]) for t in lsk.KV4.zeros(
+        1, 1, 64, D, "cpu"))), tree=False).causal
+    assert one.row_groups in (2, 4) and one.args[8] == 8 + one.row_groups

@@ -26,8 +26,9 @@ DTYPE_KV4 = 4             # a 4-bit KV cache
 EPI_NONE, EPI_RESIDUAL, EPI_SILU_MUL = 0, 1, 2
 EPI_PARTIAL, EPI_ARGMAX, EPI_QKV_ROPE = 3, 4, 5   # launch kinds known to lsk_gemm_wide_config
 ATTN_SPLIT = 8192         # LSK_ATTN_SPLIT
+PLAN_CAUSAL = 8           # LSK_PLAN_CAUSAL
 ATTN_ROWS = 48            # query rows per attention work item (csrc/lsk_attention.hip ATTN_ROWS)
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 # name -> (restype, argtypes)
 _P, _I, _L, _F, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float, ctypes.c_size_t
@@ -832,7 +833,7 @@ class _Launch:
                  n_slots: int, n_shared: int, tiles: int, row_groups: int, part_rows: int, ws_bytes: int):
         self.groups, self.recs, self.n_groups, self.n_parts, self.n_rounds = groups, recs, n_groups, n_parts, n_rounds
         self.n_slots, self.n_shared, self.tiles, self.row_groups, self.part_rows, self.ws_bytes = \
-            n_slots, n_shared, tiles, row_groups, part_rows, ws_bytes
+            n_slots, n_shared, tiles, row_groups & ~PLAN_CAUSAL, part_rows, ws_bytes
         self.n_items = n_rounds + n_shared           # (0: nothing to launch)
         self.args = (_ptr(groups), n_groups, n_parts, _ptr(recs), n_rounds, n_slots, n_shared, tiles, row_groups,
                      part_rows)
