@@ -65,7 +65,8 @@ struct Raw16<float> {
   __device__ __forceinline__ float get(int i) const { return u[i >> 2][i & 3]; }
 };
 
-// 4 consecutive outputs of a row, of which the first `left` exist (at any address that aligns one of them)
+// 4 consecutive outputs of a row, of which the first `left` exist (at any address that aligns one of them).  R may be C, here
+// and below: the thread that writes an element has read it before, and no other does.
 template <int EPI>
 __device__ __forceinline__ void store_out(uint16_t* c, const uint16_t* r, float* o, int left) {
   typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));

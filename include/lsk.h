@@ -410,7 +410,7 @@ int lsk_qk_norm_rope(int dtype, const void* qkv, long ld, const void* w_q, const
  * written) and scales [M].  lsk_pack_i8 / lsk_unpack_i8: codes [N, K] row-major <-> packed (zeros past N and K).
  * lsk_gemm_i8: C[m][n] = epilogue(a_scales[m] w_scales[n] sum_k A[m][k] W[n][k]), the sum exact, the rest fp32 with one
  * rounding: LSK_EPI_NONE, LSK_EPI_RESIDUAL (+ R) or LSK_EPI_SILU_MUL (W of 2 ffn rows [gate; up], N == ffn a multiple of
- * 16: silu(g) u).  C and R [M, N] of `dtype`.  A result does not depend on what else is in the launch.
+ * 16: silu(g) u).  C and R [M, N] of `dtype`, R may be C.  A result does not depend on what else is in the launch.
  * Beside lsk_gemm (solutions/packed.py:175, 182-185). */
 int lsk_quant_rows_i8(int dtype, const void* x, long ldx, void* codes, float* scales, int M, int K, void* stream);
 int lsk_pack_i8(const void* codes, long ld, void* packed, int N, int K, void* stream);

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_cache_ops import BF16, F32, _lsk
+from test_cache_ops import BF16, F32, _gen, _lsk
 
 
 @pytest.fixture
@@ -179,3 +179,30 @@ def test_a_trees_plan_over_a_4_bit_cache_needs_its_mask(D):
     one = lsk.AttnPlan([(0, 3, 40, 0)], 32, lsk.KV4(*(t.expand(1000, 8, *t.shape[2:]) for t in lsk.KV4.zeros(
         1, 1, 64, D, "cpu"))), tree=False).causal
     assert one.row_groups in (2, 4) and one.args[8] == 8 + one.row_groups
+
+
+# ----------------------------------------------------------------------------- a residual that takes the result
+
+def test_gemm_i8_takes_the_residuals_pitch_where_it_is_the_output(launches):
+    lsk = _lsk()
+    M, N, K = 5, 32, 64
+    w = lsk.PackedWeightI8(torch.zeros(N, K, dtype=torch.int8), torch.ones(N))
+    h = torch.zeros(M, N + 4, dtype=BF16)[:, :N]
+    lsk.gemm_i8(lsk.quant_rows_i8(torch.zeros(M, K, dtype=BF16)), w, out=h, residual=h, epilogue=lsk.EPI_RESIDUAL)
+    what, args = launches[-1]
+    assert what == "lsk_gemm_i8" and args[5] == args[7] == h.data_ptr() and args[6] == args[8] == N + 4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,N,K", [(1, 33, 100), (5, 32, 64), (64, 130, 300), (130, 272, 640), (513, 520, 192)])
+def test_gemm_i8_adds_to_its_output_in_place(cuda, dtype, M, N, K):
+    lsk = _lsk()
+    g = _gen(M + K)
+    a = lsk.quant_rows_i8(torch.randn(M, K, generator=g).to(dtype).to(cuda))
+    w = lsk.PackedWeightI8(torch.randn(N, K, generator=g).to(cuda))
+    buf = torch.randn(M, N + 5, generator=g).to(dtype).to(cuda)
+    for h in (buf[:, 2:N + 2], buf[:, :N].contiguous()):
+        want = lsk.gemm_i8(a, w, residual=h.clone(), epilogue=lsk.EPI_RESIDUAL)
+        assert lsk.gemm_i8(a, w, out=h, residual=h, epilogue=lsk.EPI_RESIDUAL) is h
+        assert torch.equal(h, want)

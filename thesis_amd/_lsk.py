@@ -1264,7 +1264,7 @@ class PackedWeightI8:
 def gemm_i8(a: RowsI8, w: PackedWeightI8, out: torch.Tensor | None = None, residual: torch.Tensor | None = None,
             epilogue: int = EPI_NONE) -> torch.Tensor:
     """gemm over 8-bit integers (lsk_gemm_i8): out[m, n] = epilogue(scale_m scale_n sum_k a w) of a's dtype, fp32 until
-    its one rounding.  EPI_RESIDUAL adds residual [M, N]; for EPI_SILU_MUL w holds [gate; up]."""
+    its one rounding.  EPI_RESIDUAL adds residual [M, N], which may be out; for EPI_SILU_MUL w holds [gate; up]."""
     if a.shape[1] != w.shape[1]:
         raise LskError(f"gemm_i8: {a.shape} against a weight of {w.shape}")
     M, K = a.shape
@@ -1278,23 +1278,18 @@ def gemm_i8(a: RowsI8, w: PackedWeightI8, out: torch.Tensor | None = None, resid
     dtype, dev = a.dtype, _one_device(a.data, w.data, w.scales, out, residual)
     if out is None:
         out = torch.empty((M, N), dtype=dtype, device=a.data.device)
-    ldr = 0
-    for t in (out, residual):
+    pitch = [0, 0]
+    for i, t in enumerate((out, residual)):
         if t is not None:
             ld, one = t.stride() if t.dim() == 2 else (0, 0)
             if t.shape != (M, N) or t.dtype is not dtype or (one != 1 and t.numel()):
                 raise LskError(f"gemm_i8: out and residual must be {[M, N]} {dtype} with contiguous rows, got "
                                f"{list(t.shape)} {t.dtype}")
-            if ld < N:
-                ld = _row_pitch("gemm_i8", "out" if t is out else "residual", t, N)
-            if t is out:
-                ldc = ld
-            else:
-                ldr = ld
+            pitch[i] = ld if ld >= N else _row_pitch("gemm_i8", ("out", "residual")[i], t, N)
     if M:
         codes = a.data.data_ptr()
         _launch(dev, "lsk_gemm_i8", dtype_code(dtype), codes, codes + a.offset, w.data.data_ptr(), w.scales.data_ptr(),
-                out.data_ptr(), ldc, _ptr(residual), ldr, M, N, K, epilogue, N if epilogue == EPI_SILU_MUL else 0)
+                out.data_ptr(), pitch[0], _ptr(residual), pitch[1], M, N, K, epilogue, N if epilogue == EPI_SILU_MUL else 0)
     return out
 
 
