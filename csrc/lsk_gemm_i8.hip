@@ -23,6 +23,14 @@
 
 namespace {
 
+// sum * s * w for a token's scale s and a channel's w.  From 2^90 on, where sum * s alone could pass fp32's range, s goes in
+// without 2^32, which comes back at the end (bits are the same: powers of two).
+struct TokenScale {
+  float s, up;
+  __device__ __forceinline__ TokenScale(float x) : s(x > 0x1p90f ? x * 0x1p-32f : x), up(x > 0x1p90f ? 0x1p32f : 1.f) {}
+  __device__ __forceinline__ float times(int sum, float w) const { return (float)sum * s * w * up; }
+};
+
 __device__ __forceinline__ uint32_t code_bits(float x, float r) {
   return __float_as_uint(__builtin_fmaf(x, r, 0x1.8p23f)) & 255u;
 }
@@ -256,10 +264,10 @@ __global__ __launch_bounds__(256) void gemm_i8_kernel(const uint8_t* __restrict_
     const int nl = o % (16 * NS), ml = o / (16 * NS);
     const int n = 16 * g0 + nl, m = 16 * t0 + ml;
     if (n >= N || m >= M) continue;
-    const float s = sa[m];
-    float v = (float)sum(nl >> 4, ml >> 4, nl & 15, ml & 15) * s * sw[n];
+    const TokenScale s(sa[m]);
+    float v = s.times(sum(nl >> 4, ml >> 4, nl & 15, ml & 15), sw[n]);
     if constexpr (SILU) {
-      const float u = (float)sum((nl >> 4) + NS, ml >> 4, nl & 15, ml & 15) * s * sw[ffn + n];
+      const float u = s.times(sum((nl >> 4) + NS, ml >> 4, nl & 15, ml & 15), sw[ffn + n]);
       v = silu_f(v) * u;
     } else if constexpr (EPI == LSK_EPI_RESIDUAL) {
       v += Elem<T>::ld(R + (long)m * ldr + n);
@@ -426,15 +434,15 @@ __global__ __launch_bounds__(256 * KP, NG * MG == 32 || KP > 1 ? 1 : 2) void gem
   for (int t = 0; t < MG; ++t) {
     const int m = (g0 + t) * 16 + l16;
     if (t >= gn || m >= M) continue;
-    const float s = sa[m];
+    const TokenScale s(sa[m]);
 #pragma unroll
     for (int g = 0; g < WN; ++g) {
       const int n = (r0 + g) * 16 + 4 * lg;
       float o[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        o[i] = (float)acc[g][t][i] * s * ws[g][i];
-        if constexpr (SILU) o[i] = silu_f(o[i]) * ((float)acc[g + WN][t][i] * s * ws[g + WN][i]);
+        o[i] = s.times(acc[g][t][i], ws[g][i]);
+        if constexpr (SILU) o[i] = silu_f(o[i]) * s.times(acc[g + WN][t][i], ws[g + WN][i]);
       }
       store_out<EPI>(C + (long)m * ldc + n, EPI == LSK_EPI_RESIDUAL ? R + (long)m * ldr + n : nullptr, o, N - n);
     }

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from test_cache_ops import BF16, F32, _gen, _lsk
+from test_lowbit_ops import assert_project, project, rows8
 
 
 @pytest.fixture
@@ -206,3 +207,30 @@ def test_gemm_i8_adds_to_its_output_in_place(cuda, dtype, M, N, K):
         want = lsk.gemm_i8(a, w, residual=h.clone(), epilogue=lsk.EPI_RESIDUAL)
         assert lsk.gemm_i8(a, w, out=h, residual=h, epilogue=lsk.EPI_RESIDUAL) is h
         assert torch.equal(h, want)
+
+
+# ----------------------------------------------------------------------------- scales at the ends of fp32's range
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("epilogue", [0, 1, 2])
+@pytest.mark.parametrize("M", [4, 130])
+def test_gemm_i8_of_the_largest_activations_stays_finite(cuda, dtype, epilogue, M):
+    """Rows up to the type's largest value against weights that bring the products back: sum * scale alone passes 2^128."""
+    lsk = _lsk()
+    g = _gen(M)
+    N, K = 48, 256
+    x = torch.randn(M, K, generator=g)
+    x *= torch.exp2(torch.linspace(-60, 120, M))[:, None]             # (the last rows' scales pass 2^90)
+    x[-1] = torch.finfo(dtype).max * torch.sign(x[-1])
+    x = x.to(dtype)
+    w = torch.randn(2 * N if epilogue == 2 else N, K, generator=g) * 2.0 ** -75
+    w[0] = w[0].abs() * torch.sign(x[-1].float())                     # 256 products of one sign
+    res = torch.randn(M, N, generator=g).to(dtype) if epilogue == 1 else None
+    (ca, sa), (cw, sw) = rows8(x), rows8(w)
+    assert ((ca @ cw.T).float().abs().amax(1) * sa).isinf().any()
+    want = project(ca, sa, cw, sw, dtype, epilogue, res)
+    assert torch.isfinite(want[0].to(dtype)).all()
+    got = lsk.gemm_i8(lsk.quant_rows_i8(x.to(cuda)), lsk.PackedWeightI8(w.to(cuda)),
+                      residual=None if res is None else res.to(cuda), epilogue=epilogue)
+    assert_project(got, want, dtype)
