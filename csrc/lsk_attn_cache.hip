@@ -376,15 +376,18 @@ struct AttnLds {
   // rows of an item at most
   static constexpr int QROWS = QREG ? 0 : GROUPS && TREE ? 32 * QT : GROUPS && D == 128 ? PAIR_ROWS : 16 * QT;
   static constexpr int QLD = D + 8;                  // 16 rows' 16-byte reads hit distinct banks
-  alignas(16) float o[CACHE_WAVES][MR][D + 4];
-  alignas(16) uint16_t q[QREG ? 1 : QROWS][QLD];
-  uint16_t qe[KOP ? QROWS : 1][4];                   // (KOP: a row of q is its hi, then its lo)
-  float ml[KOP ? 1 : CACHE_WAVES][2][16 * QT];       // (KOP: behind a row of o)
+  typedef float Partial[CACHE_WAVES][MR][D + 4];
+  static __device__ __forceinline__ Partial& partial() {
+    __shared__ __attribute__((aligned(16))) Partial o;
+    return o;
+  }
 };
 
-// The items of slot `block`.
+// The items of slot `block`.  The arrays in LDS are objects of their own: as members of one, or by reference, the 8-bit
+// trees' instance over 128 dims waits for spilt registers before its first loads (16 MHA trees of 20 to 40 nodes 33.7 us
+// against 32.2).
 template <int D, int QT, int FMT, bool TREE>
-__device__ __forceinline__ void cache_attn_items(const CacheAttnArgs& A, AttnLds<D, QT, FMT, TREE>& lds, int block) {
+__device__ __forceinline__ void cache_attn_items(const CacheAttnArgs& A, int block) {
   using L = AttnLds<D, QT, FMT, TREE>;
   constexpr bool KV8 = FMT == FMT_KV8, KV4 = FMT == FMT_KV4, CODES = KV8 || KV4;
   constexpr int STEP = CODES ? 64 : 32;              // positions per step of a wave
@@ -401,10 +404,10 @@ __device__ __forceinline__ void cache_attn_items(const CacheAttnArgs& A, AttnLds
   constexpr int MT = L::MT, MR = L::MR, QROWS = L::QROWS;
   constexpr int QCH = D / 8;
   constexpr int QPT = QREG ? 1 : (QROWS * QCH + 64 * NW - 1) / (64 * NW);
-  auto& s_o = lds.o;
-  auto& s_q = lds.q;
-  auto& s_qe = lds.qe;
-  auto& s_ml = lds.ml;
+  auto& s_o = L::partial();
+  __shared__ __attribute__((aligned(16))) uint16_t s_q[QREG ? 1 : QROWS][L::QLD];
+  __shared__ uint16_t s_qe[KOP ? QROWS : 1][4];      // (KOP: a row of s_q is its hi, then its lo)
+  __shared__ float s_ml[KOP ? 1 : NW][2][GR];        // (KOP: behind a row of s_o)
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -792,8 +795,7 @@ __device__ __forceinline__ void cache_attn_items(const CacheAttnArgs& A, AttnLds
 
 template <int D, int QT, int FMT, bool TREE>
 __global__ __launch_bounds__(64 * CACHE_WAVES, 2) void cache_attn_kernel(const CacheAttnArgs A) {
-  __shared__ AttnLds<D, QT, FMT, TREE> lds;
-  cache_attn_items<D, QT, FMT, TREE>(A, lds, blockIdx.x);
+  cache_attn_items<D, QT, FMT, TREE>(A, blockIdx.x);
 }
 
 // The end of an item of cache_tree_kernel: a wave's rows, from rb on, or its part of them
@@ -1178,12 +1180,10 @@ __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_tree4_kernel(const C
 template <bool TREE, int QT>
 __global__ __launch_bounds__(64 * TREE_WAVES, 2) void cache_both4_kernel(const CacheAttnArgs A,
                                                                          const int32_t* __restrict__ items, int n_shared) {
-  __shared__ union {
-    AttnLds<128, 2, FMT_KV4, TREE> attn;
-    char v[2 * TREE4_BUF];
-  } lds;
-  if ((int)blockIdx.x < n_shared) cache_tree4_item<TREE, QT>(A, items + (long)blockIdx.x * 8, lds.v);
-  else cache_attn_items<128, 2, FMT_KV4, TREE>(A, lds.attn, blockIdx.x - n_shared);
+  using L = AttnLds<128, 2, FMT_KV4, TREE>;
+  static_assert(sizeof(typename L::Partial) >= 2 * TREE4_BUF, "V's buffers where the other items merge");
+  if ((int)blockIdx.x < n_shared) cache_tree4_item<TREE, QT>(A, items + (long)blockIdx.x * 8, (char*)L::partial());
+  else cache_attn_items<128, 2, FMT_KV4, TREE>(A, blockIdx.x - n_shared);
 }
 
 // Merge the splits of a row in split order: M = max_s m_s, w_s = exp2(m_s - M), out = sum w_s O_s / sum w_s l_s (zeros
