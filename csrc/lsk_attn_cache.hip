@@ -311,7 +311,7 @@ __device__ __forceinline__ void softmax_tile(lsk_f32x4 (&s)[NA], uint32_t reads,
 // Over a 4-bit cache of 128 dims a lane's 32 codes of K and their scale are an operand of the scaled matrix instruction
 // (v_mfma_scale_f32_16x16x128_f8f6f4: 16 positions x 128 dims) as they are.  Its partner Q is given as two e4m3 numbers
 // per value, q = 2^e (hi + lo / 16) with a power of two for every 32 dims of a row: hi holds the upper four of a bf16
-// value's eight bits, lo the rest, exactly for values down to 2^-15 of the 32 dims' largest; below, off by at most 2^-21
+// value's eight bits, lo the rest, exactly for values down to 2^-13 of the 32 dims' largest; below, off by at most 2^-21
 // of that.  An infinity becomes NaN: the row's result is NaN either way.  Lane group lg's operand of Q is dims 16 lg ..
 // + 15 and 64 + 16 lg .. + 15 (of K's codes, dims 32 lg .. + 31), its scale that of dims 32 lg .. + 31.
 typedef int i32x8 __attribute__((ext_vector_type(8)));

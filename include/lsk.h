@@ -315,14 +315,15 @@ int lsk_kv8_read(int dtype, const void* k8, const void* v8, const void* k_exp, c
  * mask (uint32 [n_tokens][mask_words]), of the block's own slots only those whose bit is set: bit j % 32 of word j / 32
  * for node j; bits of later nodes and bits past the words count as 0.  A row that reads nothing gives zeros, one whose
  * scores are all -infinity NaN.  Values in slots that a row does not read never reach it, whatever they are.
- * bf16 and 8-bit: scores, statistics and sums are fp32; the weights are rounded to bf16 for their product with V, as
- * lsk_ragged_attn's are.
+ * bf16 and coded caches: scores, statistics and sums are fp32; the weights are rounded to bf16 for their product with V,
+ * as lsk_ragged_attn's are.
  * Weights are relative to a running maximum that may lag by 2^8 and are summed in fp32 before the division: 2^8 |V|
- * times the positions read has to stay below 2^128.
+ * times the positions read has to stay below 2^128 (over bf16 and 8-bit caches this holds for scores, scale log2(e)
+ * q . k, below 2^26; from there on the maximum's own rounding adds to the 2^8).
  * groups .. part_rows: lsk_cache_attn_plan's (fp32 trees: works, n_works, rows_cap of an unsplit lsk_attn_plan).
  * workspace >= lsk_cache_attn_workspace_bytes(n_parts, n_kv_heads, part_rows, head_dim), 16-byte aligned, and a call's
  * own (one that two captured graphs share is written by both).  head_dim 64 or 128 (fp32 also 16 and 32); scale not
- * negative; bf16 and 8-bit: max_seq a multiple of 64, max_seq * head_dim below 2^30.  A row's result depends on
+ * negative; bf16 and coded caches: max_seq a multiple of 64, max_seq * head_dim below 2^30.  A row's result depends on
  * its own block (with a mask: also on the plan's row_groups) and the split only, not on the rest of the launch; an fp32
  * chain (every ancestor's bit set) gives lsk_ragged_attn's bits.
  * Beside lsk_ragged_attn (solutions/packed.py:142-166).
@@ -372,7 +373,8 @@ int lsk_tree_attn(int dtype, const void* q, long q_stride_t, long q_stride_h, co
  * by side in one call do not disturb each other; calls that overlap (on two streams) have to write different 16-position
  * groups of a row.
  * lsk_kv4_attn: lsk_kv8_attn over a layer's 4-bit cache, with a plan of format 2.  A NaN in 32 dims of V reaches those
- * dims of the rows that read it, one of K the rows.  lsk_kv_compact takes LSK_DTYPE_KV4.
+ * dims of the rows that read it, one of K the rows.  At head_dim 128 a query's values are exact down to 2^-13 of the
+ * largest of their 32 dims, smaller ones off by at most 2^-21 of that.  lsk_kv_compact takes LSK_DTYPE_KV4.
  * Beside lsk_kv_append and lsk_ragged_attn (solutions/packed.py:142-166, 180-181). */
 int lsk_kv4_append(int dtype, const void* k, const void* v, long stride_t, long stride_h, void* k4, void* v4,
                    void* k_exp, void* v_exp, const int32_t* rows, const int32_t* pos, int n_tokens, int n_kv_heads,
@@ -392,7 +394,9 @@ int lsk_kv4_attn(const void* q, long q_stride_t, long q_stride_h, const void* k4
  * tables [tab_len, head_dim]; fp32 until the one rounding of the result.  q_out [n_tokens, n_heads, head_dim].  Either
  * k_out [n_tokens, n_kv_heads, head_dim] (rows and the caches NULL; values are not read), or K and the values go to
  * (rows[t], pos[t]) of the caches in lsk_rope_append's layouts.  A token outside the tables or the cache writes nothing.
- * head_dim 32, 64, 128 or 256; max_seq a multiple of 32.  All tensors may start at any address that aligns their elements.
+ * head_dim 32, 64, 128 or 256; max_seq a multiple of 32; at most 2^20 tokens and 1024 query heads, a multiple of the KV
+ * heads; ld not below a row's length.  The squares are summed in fp32, as lsk_rmsnorm's: a head whose sum passes its
+ * range becomes zeros.  All tensors may start at any address that aligns their elements.
  * Beside lsk_rope_append (solutions/packed.py:176-181). */
 int lsk_qk_norm_rope(int dtype, const void* qkv, long ld, const void* w_q, const void* w_k, float eps,
                      const float* cos_tab, const float* sin_tab, int tab_len, const int32_t* rows, const int32_t* pos,
@@ -405,12 +409,14 @@ int lsk_qk_norm_rope(int dtype, const void* qkv, long ld, const void* w_q, const
  * amax < 2^-100 the scale 0.
  * Packed codes of R rows: (R+15)/16 * (K+63)/64 fragments of 1 KiB at a multiple of 16 bytes; lane 16 lg + l16 of
  * fragment (g, j) = row 16 g + l16, k = 64 j + 16 lg .. + 15; fragments ordered [g][j].  K <= 131072.
+ * Pitches (ldx, ld, ldc, ldr) are not below a row's length where there is more than one row: rows do not share memory.
  *
  * lsk_quant_rows_i8: x [M, K] (bf16 or fp32, ldx) -> packed codes (zeros past K; rows past M in the last group are not
  * written) and scales [M].  lsk_pack_i8 / lsk_unpack_i8: codes [N, K] row-major <-> packed (zeros past N and K).
  * lsk_gemm_i8: C[m][n] = epilogue(a_scales[m] w_scales[n] sum_k A[m][k] W[n][k]), the sum exact, the rest fp32 with one
- * rounding: LSK_EPI_NONE, LSK_EPI_RESIDUAL (+ R) or LSK_EPI_SILU_MUL (W of 2 ffn rows [gate; up], N == ffn a multiple of
- * 16: silu(g) u).  C and R [M, N] of `dtype`, R may be C.  A result does not depend on what else is in the launch.
+ * rounding to `dtype`, M <= 2^20: LSK_EPI_NONE, LSK_EPI_RESIDUAL (+ R) or LSK_EPI_SILU_MUL (W of 2 ffn rows [gate; up],
+ * N == ffn a multiple of 16: silu(g) u).  C and R [M, N] of `dtype`, R may be C.  A result does not depend on what else is
+ * in the launch.
  * Beside lsk_gemm (solutions/packed.py:175, 182-185). */
 int lsk_quant_rows_i8(int dtype, const void* x, long ldx, void* codes, float* scales, int M, int K, void* stream);
 int lsk_pack_i8(const void* codes, long ld, void* packed, int N, int K, void* stream);
